@@ -357,6 +357,102 @@ int polar_b200_fdense_grad(uint64_t rows, uint64_t kh, uint64_t n, const float* 
                            uint64_t workspace_bytes, void* stream);
 uint64_t polar_b200_fdense_grad_workspace_bytes(uint64_t rows, uint64_t kh, uint64_t n);
 
+/* ---- rows: layer norm, log probabilities, AdamW ---------------------------------------------
+ * What stands around the matrix products of a step that trains or answers with a network of
+ * classes or tokens.  No counterpart in the reference, whose fsoftmax takes the whole tensor and
+ * whose flogloss one element at a time, and whose update is fadd(W, 1, dW, -lr). */
+
+/* flayernorm: for each row of in[rows, cols]
+ *   mean = sum(x) / cols,  rstd = 1 / sqrt(sum((x - mean)^2) / cols + eps),
+ *   out = (x - mean) * rstd * gamma + beta.
+ * gamma and beta [cols] may be NULL (ones, zeros), mean and rstd [rows] too (not wanted); out may be in.
+ * Sums are held in fp32 over two levels and more, and the deviations are summed around the mean.
+ * As a builtin: T in[..., cols], T gamma, T beta, f32 eps, T out, T mean, T rstd (three results). */
+int polar_b200_flayernorm(const float* in, const float* gamma, const float* beta, float eps, uint64_t rows,
+                          uint64_t cols, float* out, float* mean, float* rstd, void* stream);
+
+/* flayernorm_grad: with h = (in - mean) * rstd and q = gradient * gamma, per row
+ *   dIn = rstd * (q - sum(q) / cols - h * sum(q * h) / cols)
+ * and over the rows  dGamma = sum(gradient * h),  dBeta = sum(gradient).  mean and rstd are flayernorm's.
+ * gamma may be NULL (ones); dGamma or dBeta or both may be NULL (not wanted); dIn may be gradient or in.
+ * The sums over rows are taken in a fixed order: the same bits run to run.  No rows: dGamma and dBeta are zeros.
+ * As a builtin: T gradient[..., cols], T in, T gamma, T mean, T rstd, T dIn, T dGamma, T dBeta (three
+ * results).  Scratch as for fmatmul (polar_b200_flayernorm_grad_workspace_bytes; 16-byte aligned). */
+int polar_b200_flayernorm_grad(const float* gradient, const float* in, const float* gamma, const float* mean,
+                               const float* rstd, uint64_t rows, uint64_t cols, float* dIn, float* dGamma,
+                               float* dBeta, void* workspace, uint64_t workspace_bytes, void* stream);
+uint64_t polar_b200_flayernorm_grad_workspace_bytes(uint64_t rows, uint64_t cols);
+
+/* How ids of classes or tokens are held: as whole numbers in fp32 (all a graph of the framework has; exact to
+ * 2^24), in 32 or in 64 bits. */
+#define POLAR_B200_IDS_F32 0
+#define POLAR_B200_IDS_I32 1
+#define POLAR_B200_IDS_I64 2
+
+/* flogprob: for each row x of logits[rows, classes] (rows `pitch` floats apart, pitch >= classes)
+ *   logSumExp = log(sum(exp(x))),  logProb = x[id] - logSumExp,  entropy = -sum(p * log p), p = exp(x - logSumExp),
+ * and the `top` (0..32, at most `classes`) largest logits, ties to the lowest index: topIds and topLogProb
+ * [rows, top].  One pass over the logits with a running maximum.  Every result but logProb may be NULL;
+ * ids may be NULL when logProb is.  topIds are held as the ids are; with fp32 ids classes is at most 2^24.
+ *  - an id below zero marks a row without one (padding): logProb 0;
+ *  - an id that is no class of the row, or no whole number: logProb NaN (nothing is read there);
+ *  - a logit of -inf has no probability; a row of nothing else gives logSumExp and all logProbs -inf, entropy 0;
+ *  - a row with a NaN or +inf gives NaN (a NaN counts as the largest logit).
+ * As a builtin: "flogprob" T logits[rows, classes], T ids[rows], T logProb, T entropy, T logSumExp (three results),
+ * "flogprob_top" the same and T topIds[rows, top], T topLogProb[rows, top] (five results); ids in fp32. */
+int polar_b200_flogprob(const float* logits, uint64_t rows, uint64_t classes, uint64_t pitch, const void* ids,
+                        int id_type, float* logProb, float* entropy, float* logSumExp, uint64_t top, void* topIds,
+                        float* topLogProb, void* stream);
+
+/* flogprob_grad: dLogits[rows, classes] (rows dPitch floats apart) of  sum(gLogProb * logProb + gEntropy * entropy):
+ *   dLogits = p * (-gLogProb - gEntropy * (log p + entropy)) + (gLogProb at the id).
+ * logSumExp and entropy are flogprob's; gEntropy may be NULL (zeros), and entropy then too.  dLogits may be logits
+ * (with dPitch == pitch).  A row's gLogProb counts as zero where its id is below zero; an id that is no class of
+ * the row makes the row NaN (unless gLogProb is zero there).  A row that nothing reaches - both gradients zero, or all its logits -inf - gets zeros,
+ * whatever its logits hold.
+ * As a builtin: T logits, T ids, T logSumExp, T gLogProb, T dLogits, or with the entropy T logits, T ids,
+ * T logSumExp, T entropy, T gLogProb, T gEntropy, T dLogits; ids in fp32. */
+int polar_b200_flogprob_grad(const float* logits, uint64_t rows, uint64_t classes, uint64_t pitch, const void* ids,
+                             int id_type, const float* logSumExp, const float* entropy, const float* gLogProb,
+                             const float* gEntropy, float* dLogits, uint64_t dPitch, void* stream);
+
+/* fadamw: one AdamW step over any number of tensors, in place:
+ *   m <- beta1 * m + (1 - beta1) * g,   v <- beta2 * v + ((1 - beta2) * g) * g,
+ *   w <- w * (1 - lr * weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps).
+ * In the moments each product and each sum is rounded to fp32 (no fused multiply-add); 1 - beta is fp32's.
+ * Moments are held
+ *  - in 32 bits: first and second point at `count` floats each (first_scales and second_scales NULL), or
+ *  - in 8 bits: `count` e4m3 codes each, and a scale for each block of 128 of them (ceil(count / 128) floats).
+ *    `first` stands for code * scale, `second` holds sqrt(v).  A block with largest magnitude a below 2^-100
+ *    becomes zeros; else scale = a * (1/448 in fp32), code = e4m3(x * (1 / scale)), rounded to nearest even, and
+ *    a second moment above zero gets the least code at least (a zero there would leave eps alone as the
+ *    divisor).  Zero bytes are the state before the first step.  A gradient that is not finite makes its block's
+ *    moments NaN, where in 32 bits it makes NaN of its own element only.
+ * No tensor may be named twice or overlap another (POLAR_B200_ERR_INVALID for weights and moments).  One launch for every few
+ * hundred tensors of a kind.  `step` counts from 1.  With `schedule` (device memory, two floats: the number of the
+ * step and lr) both are read on the device when the kernel runs, so that a captured or prepared step can be replayed.
+ * As builtins, one tensor each: "fadamw" T gradient, T schedule[2], f32 beta1, f32 beta2, f32 eps, f32 weight_decay, T weights,
+ * T first, T second (three results); "fadamw8" T gradient, T schedule[2], f32 beta1, f32 beta2, f32 eps, f32 weight_decay,
+ * T weights, T first, T first_scales, T second, T second_scales (five results), with the codes of n weights in a tensor of
+ * ceil(n / 4) elements or more.  In a program, fadamw builtins in a row share a launch. */
+typedef struct polar_b200_adamw_tensor {
+  float* weights;
+  const float* gradient;
+  void* first;
+  void* second;
+  float* first_scales;
+  float* second_scales;
+  uint64_t count;
+  float weight_decay;
+} polar_b200_adamw_tensor;
+typedef struct polar_b200_adamw_options {
+  float lr, beta1, beta2, eps;
+  uint64_t step;
+  const float* schedule;
+} polar_b200_adamw_options;
+int polar_b200_fadamw(const polar_b200_adamw_tensor* tensors, uint64_t count, const polar_b200_adamw_options* options,
+                      void* stream);
+
 /* Sum of n floats into *sum (a device double, ADDED to: clear it first), with
  * warp-shuffle + one atomic per block.  Used to report the scalar mean of an
  * elementwise flogloss output; the reference has no reduction builtin. */
@@ -392,7 +488,8 @@ typedef struct polar_b200_arg {
  * Transpose all "ftranspose" - PolarGraphOps.td:461-523 - so each gets a name of its own
  * here), and
  * the extended "fsigmoid_grad", "fsigmoid_logloss_grad", "fmatmul_x_y_sigmoid",
- * "fmatmul_x_y_sigmoid_grad", "fmatmul_t_f_rows", "fdense_grad", "fsum".
+ * "fmatmul_x_y_sigmoid_grad", "fmatmul_t_f_rows", "fdense_grad", "fsum", "flayernorm", "flayernorm_grad",
+ * "flogprob", "flogprob_top", "flogprob_grad", "fadamw", "fadamw8".
  *
  * Launches the builtin called `nativeKernelName` ("fadd", "fmatmul_t_f", ...)
  * on arguments in LaunchCommand order; this is what Device::launch forwards to
@@ -454,7 +551,8 @@ int polar_b200_allreduce_fadd(void* const* buffers, uint32_t rank, uint32_t worl
 
 /* How many of the builtin's trailing tensor arguments it WRITES: 1 for every native name (the
  * reference's convention: the last tensor is the result, e.g. AddOperationInternal.cpp:61-66)
- * except "fdense_grad", which has two.  A runtime takes write locks accordingly. */
+ * except "fdense_grad", which has two, and the builtins on rows and weights, which have what is said
+ * there.  A runtime takes write locks accordingly. */
 int polar_b200_result_count(const char* nativeKernelName);
 
 /* The same exchange for a PART of the payload, floats [first, first + count) (first a multiple

@@ -33,6 +33,15 @@ class Op(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char_p), ("args", ctypes.POINTER(Arg)), ("argc", _u64)]
 
 
+class AdamwTensor(ctypes.Structure):
+    _fields_ = [("weights", _p), ("gradient", _p), ("first", _p), ("second", _p), ("first_scales", _p),
+                ("second_scales", _p), ("count", _u64), ("weight_decay", _f)]
+
+
+class AdamwOptions(ctypes.Structure):
+    _fields_ = [("lr", _f), ("beta1", _f), ("beta2", _f), ("eps", _f), ("step", _u64), ("schedule", _p)]
+
+
 SIGNATURES = {
     "polar_b200_last_error": (ctypes.c_char_p, []),
     "polar_b200_version": (_i, []),
@@ -74,6 +83,12 @@ SIGNATURES = {
     "polar_b200_check_device_status": (_i, []),
     "polar_b200_set_wait_limit_ns": (None, [_u64]),
     "polar_b200_wait_limit_ns": (_u64, []),
+    "polar_b200_flayernorm": (_i, [_p, _p, _p, _f, _u64, _u64, _p, _p, _p, _p]),
+    "polar_b200_flayernorm_grad": (_i, [_p, _p, _p, _p, _p, _u64, _u64, _p, _p, _p, _p, _u64, _p]),
+    "polar_b200_flayernorm_grad_workspace_bytes": (_u64, [_u64, _u64]),
+    "polar_b200_flogprob": (_i, [_p, _u64, _u64, _u64, _p, _i, _p, _p, _p, _u64, _p, _p, _p]),
+    "polar_b200_flogprob_grad": (_i, [_p, _u64, _u64, _u64, _p, _i, _p, _p, _p, _p, _p, _u64, _p]),
+    "polar_b200_fadamw": (_i, [ctypes.POINTER(AdamwTensor), _u64, ctypes.POINTER(AdamwOptions), _p]),
     "polar_b200_fsum": (_i, [_p, _p, _u64, _p]),
     "polar_b200_fsum_f32": (_i, [_p, _p, _u64, _p, _u64, _p]),
     "polar_b200_fsum_f32_workspace_bytes": (_u64, [_u64]),

@@ -34,6 +34,7 @@ int launch_dense_grad(const float* H, const float* dz, const float* W, float* di
 uint64_t ragged_rows_workspace_bytes(uint64_t rem, uint64_t n, uint64_t k);
 int launch_ragged_rows(const float* left_tail, uint64_t left_pitch, const float* right, float* out_tail,
                        float* ws, uint64_t rem, uint64_t n, uint64_t k, cudaStream_t st);
+bool adamw_arguments(const char* name, const polar_b200_arg* a, uint64_t argc, polar_b200_adamw_tensor* t, polar_b200_adamw_options* o);
 
 namespace {
 
@@ -359,7 +360,21 @@ uint64_t polar_b200_fmatmul_workspace_bytes(int tl, int tr, uint64_t m, uint64_t
   return workspace_need(tl, tr, m, n, k, 0);
 }
 
-int polar_b200_result_count(const char* name) { return name && !std::strcmp(name, "fdense_grad") ? 2 : 1; }
+int polar_b200_result_count(const char* name) {
+  static const struct { const char* name; int results; } several[] = {
+      {"fdense_grad", 2}, {"flayernorm", 3}, {"flayernorm_grad", 3}, {"flogprob", 3}, {"flogprob_top", 5}, {"fadamw", 3}, {"fadamw8", 5}};
+  for (const auto& s : several)
+    if (name && !std::strcmp(name, s.name)) return s.results;
+  return 1;
+}
+
+// (T gradient[..., cols], T in, T gamma, T mean, T rstd, T dIn, T dGamma, T dBeta) and its like: rows and columns of the first
+// tensor, by the last extent.
+static void rows_of(const polar_b200_tensor& t, uint64_t* rows, uint64_t* cols) {
+  *rows = t.dims ? 1 : 0;
+  *cols = t.dims ? t.shape[t.dims - 1] : 0;
+  for (uint64_t d = 0; d + 1 < t.dims; ++d) *rows *= t.shape[d];
+}
 
 uint64_t polar_b200_launch_workspace_bytes(const char* name, const polar_b200_arg* a, uint64_t argc) {
   if (name && a && !std::strcmp(name, "fmatmul_t_f_rows") && argc == 5 && a[0].is_tensor && a[1].is_tensor &&
@@ -368,6 +383,11 @@ uint64_t polar_b200_launch_workspace_bytes(const char* name, const polar_b200_ar
   if (name && a && !std::strcmp(name, "fdense_grad") && argc == 5 && a[0].is_tensor && a[1].is_tensor &&
       a[0].tensor.dims == 2 && a[1].tensor.dims == 2 && a[0].tensor.shape && a[1].tensor.shape)
     return polar_b200_fdense_grad_workspace_bytes(a[0].tensor.shape[0], a[1].tensor.shape[0], a[0].tensor.shape[1]);
+  if (name && a && !std::strcmp(name, "flayernorm_grad") && argc == 8 && a[0].is_tensor && a[0].tensor.dims && a[0].tensor.shape) {
+    uint64_t rows, cols;
+    rows_of(a[0].tensor, &rows, &cols);
+    return polar_b200_flayernorm_grad_workspace_bytes(rows, cols);
+  }
   if (name && a && !std::strcmp(name, "fsum") && argc == 2 && a[0].is_tensor && (!a[0].tensor.dims || a[0].tensor.shape)) {
     uint64_t n = 1;
     for (uint64_t d = 0; d < a[0].tensor.dims; ++d) n *= a[0].tensor.shape[d];
@@ -832,6 +852,62 @@ int polar_b200_launch_by_name(const char* name, const polar_b200_arg* a, uint64_
       return fail(bad_args, "fdense_grad: shapes do not agree");
     return polar_b200_fdense_grad(rows, kh, n, a[0].tensor.data, a[1].tensor.data, a[2].tensor.data, a[3].tensor.data,
                                   a[4].tensor.data, workspace, workspace_bytes, stream);
+  }
+  if (!std::strcmp(name, "flayernorm")) {
+    // (T in[..., cols], T gamma, T beta, f32 eps, T out, T mean, T rstd): three results
+    if (!pattern("TTTfTTT") || a[0].tensor.dims < 1) return fail(bad_args, "flayernorm expects (T in, T gamma, T beta, f32 eps, T out, T mean, T rstd)");
+    uint64_t rows, cols;
+    rows_of(a[0].tensor, &rows, &cols);
+    if (numel(a[1].tensor) != cols || numel(a[2].tensor) != cols || !same(0, 4) || numel(a[5].tensor) != rows || numel(a[6].tensor) != rows)
+      return fail(bad_args, "flayernorm: shapes do not agree");
+    return polar_b200_flayernorm(a[0].tensor.data, a[1].tensor.data, a[2].tensor.data, a[3].scalar, rows, cols, a[4].tensor.data,
+                                 a[5].tensor.data, a[6].tensor.data, stream);
+  }
+  if (!std::strcmp(name, "flayernorm_grad")) {
+    // (T gradient[..., cols], T in, T gamma, T mean, T rstd, T dIn, T dGamma, T dBeta): three results
+    if (!pattern("TTTTTTTT") || a[0].tensor.dims < 1)
+      return fail(bad_args, "flayernorm_grad expects (T gradient, T in, T gamma, T mean, T rstd, T dIn, T dGamma, T dBeta)");
+    uint64_t rows, cols;
+    rows_of(a[0].tensor, &rows, &cols);
+    if (!same(0, 1) || numel(a[2].tensor) != cols || numel(a[3].tensor) != rows || numel(a[4].tensor) != rows || !same(0, 5) ||
+        numel(a[6].tensor) != cols || numel(a[7].tensor) != cols)
+      return fail(bad_args, "flayernorm_grad: shapes do not agree");
+    return polar_b200_flayernorm_grad(a[0].tensor.data, a[1].tensor.data, a[2].tensor.data, a[3].tensor.data, a[4].tensor.data, rows, cols,
+                                      a[5].tensor.data, a[6].tensor.data, a[7].tensor.data, workspace, workspace_bytes, stream);
+  }
+  if (!std::strcmp(name, "flogprob") || !std::strcmp(name, "flogprob_top")) {
+    // (T logits[rows, classes], T ids[rows], T logProb, T entropy, T logSumExp [, T topIds[rows, top], T topLogProb])
+    const bool alternatives = name[8] != 0;
+    if (!pattern(alternatives ? "TTTTTTT" : "TTTTT") || a[0].tensor.dims != 2 || (alternatives && (a[5].tensor.dims != 2 || a[6].tensor.dims != 2)))
+      return fail(bad_args, "flogprob expects (T logits[rows,classes], T ids, T logProb, T entropy, T logSumExp [, T topIds[rows,top], T topLogProb])");
+    const uint64_t rows = a[0].tensor.shape[0], classes = a[0].tensor.shape[1], top = alternatives ? a[5].tensor.shape[1] : 0;
+    for (int i = 1; i < 5; ++i)
+      if (numel(a[i].tensor) != rows) return fail(bad_args, "flogprob: shapes do not agree");
+    if (alternatives && (a[5].tensor.shape[0] != rows || a[6].tensor.shape[0] != rows || a[6].tensor.shape[1] != top))
+      return fail(bad_args, "flogprob: shapes do not agree");
+    return polar_b200_flogprob(a[0].tensor.data, rows, classes, classes, a[1].tensor.data, POLAR_B200_IDS_F32, a[2].tensor.data,
+                               a[3].tensor.data, a[4].tensor.data, top, alternatives ? a[5].tensor.data : nullptr,
+                               alternatives ? a[6].tensor.data : nullptr, stream);
+  }
+  if (!std::strcmp(name, "flogprob_grad")) {
+    // (T logits, T ids, T logSumExp, T gLogProb, T dLogits), or with entropy behind logSumExp and gEntropy behind gLogProb
+    const bool both = argc == 7;
+    if (!pattern(both ? "TTTTTTT" : "TTTTT") || a[0].tensor.dims != 2 || !same(0, argc - 1))
+      return fail(bad_args, "flogprob_grad expects (T logits[rows,classes], T ids, T logSumExp, [T entropy,] T gLogProb, [T gEntropy,] T dLogits)");
+    const uint64_t rows = a[0].tensor.shape[0], classes = a[0].tensor.shape[1];
+    for (uint64_t i = 1; i + 1 < argc; ++i)
+      if (numel(a[i].tensor) != rows) return fail(bad_args, "flogprob_grad: shapes do not agree");
+    return polar_b200_flogprob_grad(a[0].tensor.data, rows, classes, classes, a[1].tensor.data, POLAR_B200_IDS_F32, a[2].tensor.data,
+                                    both ? a[3].tensor.data : nullptr, a[both ? 4 : 3].tensor.data, both ? a[5].tensor.data : nullptr,
+                                    a[argc - 1].tensor.data, classes, stream);
+  }
+  if (!std::strcmp(name, "fadamw") || !std::strcmp(name, "fadamw8")) {
+    polar_b200_adamw_tensor t;
+    polar_b200_adamw_options o;
+    if (!adamw_arguments(name, a, argc, &t, &o))
+      return fail(bad_args, "fadamw expects (T gradient, T schedule[2], f32 beta1, f32 beta2, f32 eps, f32 weight_decay, T weights, T first, T second), "
+                            "fadamw8 with T first_scales and T second_scales behind their moments");
+    return polar_b200_fadamw(&t, 1, &o, stream);
   }
   if (!std::strcmp(name, "fsum")) {
     if (!pattern("TT") || numel(a[1].tensor) < 1) return fail(bad_args, "fsum expects (T in, T out[1])");

@@ -44,6 +44,35 @@ public:
     device_ = t.get_device();
     return &t;
   }
+  // None: no tensor, which is no reason to decline.
+  const at::Tensor* tensor_or_none(int i) { return ok_ && args_[i] == Py_None ? nullptr : tensor(i); }
+  // A matrix whose rows may lie further apart than they are long.
+  const at::Tensor* matrix(int i, uint64_t* pitch) {
+    const at::Tensor* t = any(args_[i]);
+    if (!t) return nullptr;
+    ok_ = t->scalar_type() == at::kFloat && t->dim() == 2 && (t->size(1) <= 1 || t->stride(1) == 1) &&
+          (t->size(0) <= 1 || t->stride(0) >= t->size(1));
+    if (!ok_) return nullptr;
+    *pitch = (uint64_t)(t->size(0) <= 1 ? t->size(1) : t->stride(0));
+    return t;
+  }
+  // Ids: whole numbers in fp32, 32 or 64 bits.
+  const at::Tensor* ids(int i, int* type) {
+    const at::Tensor* t = ok_ && args_[i] == Py_None ? nullptr : any(args_[i]);
+    if (!t) return nullptr;
+    const auto s = t->scalar_type();
+    ok_ = t->is_contiguous() && (s == at::kFloat || s == at::kInt || s == at::kLong);
+    *type = s == at::kFloat ? POLAR_B200_IDS_F32 : s == at::kInt ? POLAR_B200_IDS_I32 : POLAR_B200_IDS_I64;
+    return ok_ ? t : nullptr;
+  }
+  // An element of a list: contiguous, of `size` bytes each.
+  const at::Tensor* element(PyObject* o, size_t size) {
+    const at::Tensor* t = any(o);
+    if (!t) return nullptr;
+    ok_ = t->is_contiguous() && (size == 4 ? t->scalar_type() == at::kFloat
+                                           : t->scalar_type() == at::kFloat8_e4m3fn || t->scalar_type() == at::kByte);
+    return ok_ ? t : nullptr;
+  }
   float scalar(int i) {
     if (!ok_) return 0.f;
     const double v = PyFloat_AsDouble(args_[i]);
@@ -68,6 +97,17 @@ public:
   void* stream() const { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device_).stream(); }
 
 private:
+  // A tensor on the call's device.
+  const at::Tensor* any(PyObject* o) {
+    if (!ok_) return nullptr;
+    ok_ = THPVariable_Check(o);
+    if (!ok_) return nullptr;
+    const at::Tensor& t = THPVariable_Unpack(o);
+    ok_ = t.defined() && t.is_cuda() && (device_ < 0 || t.get_device() == device_);
+    if (!ok_) return nullptr;
+    device_ = t.get_device();
+    return &t;
+  }
   PyObject* const* args_;
   bool ok_;
   int device_ = -1;
@@ -84,6 +124,8 @@ auto unlocked(F f) {
 
 float* data(const at::Tensor* t) { return static_cast<float*>(t->data_ptr()); }
 uint64_t numel(const at::Tensor* t) { return (uint64_t)t->numel(); }
+float* data_or_null(const at::Tensor* t) { return t ? data(t) : nullptr; }
+bool has(const at::Tensor* t, uint64_t n) { return !t || numel(t) == n; }
 PyObject* answer(bool launched) { return PyBool_FromLong(launched); }
 template <class F, class... A>
 PyObject* launched(F f, A... args) {
@@ -195,6 +237,120 @@ BUILTIN(fmatmul) {
                   nullptr, 0, c.stream());
 }
 
+// flayernorm(x, gamma or None, beta or None, eps, out, mean or None, rstd or None)
+BUILTIN(flayernorm) {
+  Call c(args, n, 7);
+  const at::Tensor *x = c.tensor(0), *gamma = c.tensor_or_none(1), *beta = c.tensor_or_none(2);
+  const float eps = c.scalar(3);
+  const at::Tensor *out = c.tensor(4), *mean = c.tensor_or_none(5), *rstd = c.tensor_or_none(6);
+  if (c.ok()) c.require(x->dim() >= 1 && x->size(-1) > 0);
+  if (!c.ok()) return answer(false);
+  const uint64_t cols = (uint64_t)x->size(-1), rows = numel(x) / cols;
+  if (numel(out) != numel(x) || !has(gamma, cols) || !has(beta, cols) || !has(mean, rows) || !has(rstd, rows)) return answer(false);
+  return launched(polar_b200_flayernorm, data(x), data_or_null(gamma), data_or_null(beta), eps, rows, cols, data(out), data_or_null(mean),
+                  data_or_null(rstd), c.stream());
+}
+// flayernorm_grad(gradient, x, gamma or None, mean, rstd, dx, dgamma or None, dbeta or None)
+BUILTIN(flayernorm_grad) {
+  Call c(args, n, 8);
+  const at::Tensor *g = c.tensor(0), *x = c.tensor(1), *gamma = c.tensor_or_none(2), *mean = c.tensor(3), *rstd = c.tensor(4);
+  const at::Tensor *dx = c.tensor(5), *dgamma = c.tensor_or_none(6), *dbeta = c.tensor_or_none(7);
+  if (c.ok()) c.require(x->dim() >= 1 && x->size(-1) > 0);
+  if (!c.ok()) return answer(false);
+  const uint64_t cols = (uint64_t)x->size(-1), rows = numel(x) / cols;
+  if (numel(g) != numel(x) || numel(dx) != numel(x) || !has(gamma, cols) || !has(mean, rows) || !has(rstd, rows) || !has(dgamma, cols) ||
+      !has(dbeta, cols))
+    return answer(false);
+  return launched(polar_b200_flayernorm_grad, data(g), data(x), data_or_null(gamma), data(mean), data(rstd), rows, cols, data(dx),
+                  data_or_null(dgamma), data_or_null(dbeta), nullptr, 0, c.stream());
+}
+// flogprob(logits, ids or None, logprob or None, entropy or None, logsumexp or None, top_ids or None, top_logprob or None)
+BUILTIN(flogprob) {
+  Call c(args, n, 7);
+  uint64_t pitch = 0;
+  int type = POLAR_B200_IDS_I64, top_type = -1;
+  const at::Tensor *x = c.matrix(0, &pitch), *ids = c.ids(1, &type), *lp = c.tensor_or_none(2), *entropy = c.tensor_or_none(3),
+                   *lse = c.tensor_or_none(4), *top_ids = c.ids(5, &top_type), *top_lp = c.tensor_or_none(6);
+  if (!c.ok()) return answer(false);
+  const uint64_t rows = (uint64_t)x->size(0), classes = (uint64_t)x->size(1);
+  if (!has(ids, rows) || !has(lp, rows) || !has(entropy, rows) || !has(lse, rows) || (lp && !ids) || (top_ids && ids && top_type != type))
+    return answer(false);
+  if (top_ids && !ids) type = top_type;
+  uint64_t top = 0;
+  for (const at::Tensor* t : {top_ids, top_lp}) {
+    if (!t) continue;
+    if (t->dim() != 2 || (uint64_t)t->size(0) != rows || (top && (uint64_t)t->size(1) != top)) return answer(false);
+    top = (uint64_t)t->size(1);
+  }
+  return launched(polar_b200_flogprob, data(x), rows, classes, pitch, ids ? ids->data_ptr() : nullptr, type, data_or_null(lp),
+                  data_or_null(entropy), data_or_null(lse), top, top_ids ? top_ids->data_ptr() : nullptr, data_or_null(top_lp), c.stream());
+}
+// flogprob_grad(logits, ids, logsumexp, entropy or None, g_logprob, g_entropy or None, dlogits)
+BUILTIN(flogprob_grad) {
+  Call c(args, n, 7);
+  uint64_t pitch = 0, dpitch = 0;
+  int type = POLAR_B200_IDS_I64;
+  const at::Tensor *x = c.matrix(0, &pitch), *ids = c.ids(1, &type), *lse = c.tensor(2), *entropy = c.tensor_or_none(3), *g = c.tensor(4),
+                   *ge = c.tensor_or_none(5), *dx = c.matrix(6, &dpitch);
+  if (!c.ok() || !ids) return answer(false);
+  const uint64_t rows = (uint64_t)x->size(0), classes = (uint64_t)x->size(1);
+  if ((uint64_t)dx->size(0) != rows || (uint64_t)dx->size(1) != classes || !has(ids, rows) || !has(lse, rows) || !has(entropy, rows) ||
+      !has(g, rows) || !has(ge, rows))
+    return answer(false);
+  return launched(polar_b200_flogprob_grad, data(x), rows, classes, pitch, ids->data_ptr(), type, data(lse), data_or_null(entropy), data(g),
+                  data_or_null(ge), data(dx), dpitch, c.stream());
+}
+
+// A list or tuple, as long as it lives here.
+struct Sequence {
+  explicit Sequence(PyObject* o) : list(o == Py_None ? nullptr : PySequence_Fast(o, "")) {
+    if (!list) PyErr_Clear();
+  }
+  ~Sequence() { Py_XDECREF(list); }
+  Py_ssize_t size() const { return list ? PySequence_Fast_GET_SIZE(list) : -1; }
+  PyObject* operator[](Py_ssize_t i) const { return PySequence_Fast_GET_ITEM(list, i); }
+  PyObject* list;
+};
+// fadamw(weights, gradients, first, second, first_scales or None, second_scales or None, step, lr, beta1, beta2, eps,
+// weight decays, schedule or None): lists of tensors, and one decay for each
+BUILTIN(fadamw) {
+  Call c(args, n, 13);
+  if (!c.ok()) return answer(false);
+  const Sequence w(args[0]), g(args[1]), m(args[2]), v(args[3]), ms(args[4]), vs(args[5]), decays(args[11]);
+  const Py_ssize_t count = w.size();
+  const bool eight = ms.list != nullptr;
+  if (count < 0 || g.size() != count || m.size() != count || v.size() != count || decays.size() != count || (vs.list != nullptr) != eight ||
+      (eight && (ms.size() != count || vs.size() != count)))
+    return answer(false);
+  polar_b200_adamw_options o;
+  o.step = c.whole(6);
+  o.lr = c.scalar(7), o.beta1 = c.scalar(8), o.beta2 = c.scalar(9), o.eps = c.scalar(10);
+  std::vector<polar_b200_adamw_tensor> tensors((size_t)count);
+  for (Py_ssize_t i = 0; i < count && c.ok(); ++i) {
+    polar_b200_adamw_tensor& t = tensors[(size_t)i];
+    const at::Tensor *wt = c.element(w[i], 4), *gt = c.element(g[i], 4), *mt = c.element(m[i], eight ? 1 : 4), *vt = c.element(v[i], eight ? 1 : 4);
+    const at::Tensor *mst = eight ? c.element(ms[i], 4) : nullptr, *vst = eight ? c.element(vs[i], 4) : nullptr;
+    if (!c.ok()) break;
+    t.count = numel(wt);
+    const uint64_t blocks = (t.count + 127) / 128;
+    c.require(numel(gt) == t.count && numel(mt) == t.count && numel(vt) == t.count && has(mst, blocks) && has(vst, blocks));
+    t.weights = data(wt), t.gradient = data(gt), t.first = mt->data_ptr(), t.second = vt->data_ptr();
+    t.first_scales = data_or_null(mst), t.second_scales = data_or_null(vst);
+    const double decay = PyFloat_AsDouble(decays[i]);
+    if (decay == -1.0 && PyErr_Occurred()) {
+      PyErr_Clear();
+      c.require(false);
+    }
+    t.weight_decay = (float)decay;
+  }
+  const at::Tensor* schedule = c.tensor_or_none(12);
+  if (c.ok()) c.require(has(schedule, 2));
+  if (!c.ok()) return answer(false);
+  o.schedule = data_or_null(schedule);
+  if (count == 0) return answer(true);
+  return launched(polar_b200_fadamw, tensors.data(), (uint64_t)count, &o, c.stream());
+}
+
 // A program's operations as Python has them: a list of (native name, address of the argument structs, their count).
 bool operations(PyObject* list, std::vector<polar_b200_op>* ops) {
   if (!PyList_Check(list)) {
@@ -258,6 +414,11 @@ PyMethodDef methods[] = {
     ENTRY("fconv2d", declining<fconv2d>),
     ENTRY("ftranspose", declining<ftranspose>),
     ENTRY("fmatmul", declining<fmatmul>),
+    ENTRY("flayernorm", declining<flayernorm>),
+    ENTRY("flayernorm_grad", declining<flayernorm_grad>),
+    ENTRY("flogprob", declining<flogprob>),
+    ENTRY("flogprob_grad", declining<flogprob_grad>),
+    ENTRY("fadamw", declining<fadamw>),
     ENTRY("workspace_bytes", raising<workspace_bytes>),
     ENTRY("create_program", raising<create_program>),
     ENTRY("run_program", raising<run_program>),

@@ -1,0 +1,32 @@
+// Sums and maxima over the threads that share a row.
+#pragma once
+#include "common.cuh"
+
+namespace polar_b200 {
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
+}
+
+// The sums of `N` values over the CTA, in every thread; added in the same order in each of them.  `slots`: N values for
+// each warp, not in use by anything since the last barrier.
+template <int THREADS, int N>
+__device__ __forceinline__ void block_sums(float (&v)[N], float* slots) {
+  constexpr int kWarps = THREADS / 32;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
+  if (kWarps == 1) return;
+  if ((threadIdx.x & 31) == 0)
+#pragma unroll
+    for (int i = 0; i < N; ++i) slots[(threadIdx.x >> 5) * N + i] = v[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t lane = threadIdx.x & 31;
+    v[i] = warp_sum(lane < kWarps ? slots[lane * N + i] : 0.f);
+  }
+}
+
+}  // namespace polar_b200

@@ -10,10 +10,12 @@ and launches without the interpreter; what that declines - tensors it would reje
 call - runs the checked path below it, which raises.  An input may be longer than the result and a result
 tensor larger than what is written; what would be read or written outside a tensor is a ValueError.
 """
+import ctypes
+
 import numpy as np
 import torch
 
-from .capi import binding, lib
+from .capi import AdamwOptions, AdamwTensor, binding, lib
 
 
 def _ptr(t):
@@ -35,6 +37,45 @@ def _long_enough(n, *ts):
     for t in ts:
         if t.numel() < n:
             raise ValueError(f"a tensor of {t.numel()} elements where the builtin takes {n}")
+
+
+def _chk_rows(*ts):
+    """The tensors of a builtin on rows that are not None: as _chk, and all on one device."""
+    _chk(*ts)
+    _same_device(*ts)
+
+
+def _same_device(*ts):
+    if any(t.device != ts[0].device for t in ts):
+        raise ValueError("the tensors of one call lie on one device")
+
+
+def _exactly(what, n, *ts):
+    for t in ts:
+        if t is not None and t.numel() != n:
+            raise ValueError(f"{what}: a tensor of {t.numel()} elements where {n} are taken")
+
+
+_ID_TYPES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
+
+
+def _matrix(t):
+    """Its rows, their length and how far they lie apart."""
+    if not (t.is_cuda and t.dtype == torch.float32 and t.dim() == 2 and (t.shape[1] <= 1 or t.stride(1) == 1)
+            and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])):
+        raise ValueError("logits are float32 CUDA matrices of contiguous rows")
+    rows, cols = t.shape
+    return rows, cols, (cols if rows <= 1 else t.stride(0))
+
+
+def _ids(t):
+    if not (t.is_cuda and t.is_contiguous() and t.dtype in _ID_TYPES):
+        raise ValueError("ids are contiguous CUDA tensors of float32, int32 or int64")
+    return _ID_TYPES[t.dtype]
+
+
+def _present(*ts):
+    return [t for t in ts if t is not None]
 
 
 class DeviceBuiltins:
@@ -181,6 +222,109 @@ class DeviceBuiltins:
         self.lib.call("polar_b200_fmatmul_tc", int(tl), int(tr), m, n, k, _ptr(left), _ptr(right),
                       _ptr(out), tile_n, slab_k, passes, write_hi, splits, _stream(out))
         return out
+
+    def flayernorm(self, x, gamma, beta, eps, out, mean=None, rstd=None):
+        """out = (x - mean) * rstd * gamma + beta over the last dimension of x; gamma, beta, mean, rstd may be None."""
+        if not self._native.flayernorm(x, gamma, beta, eps, out, mean, rstd):
+            _chk_rows(*_present(x, gamma, beta, out, mean, rstd))
+            cols = x.shape[-1] if x.dim() else 0
+            rows = x.numel() // cols if cols else 0
+            _exactly("flayernorm", x.numel(), out)
+            _exactly("flayernorm", cols, gamma, beta)
+            _exactly("flayernorm", rows, mean, rstd)
+            self.lib.call("polar_b200_flayernorm", _ptr(x), _ptr(gamma), _ptr(beta), float(eps), rows, cols, _ptr(out), _ptr(mean),
+                          _ptr(rstd), _stream(out))
+        return out
+
+    def flayernorm_grad(self, gradient, x, gamma, mean, rstd, dx, dgamma=None, dbeta=None):
+        """The gradients at flayernorm's x, gamma and beta (the last two may be None, as gamma may); mean, rstd are flayernorm's."""
+        if not self._native.flayernorm_grad(gradient, x, gamma, mean, rstd, dx, dgamma, dbeta):
+            _chk_rows(*_present(gradient, x, gamma, mean, rstd, dx, dgamma, dbeta))
+            cols = x.shape[-1] if x.dim() else 0
+            rows = x.numel() // cols if cols else 0
+            _exactly("flayernorm_grad", x.numel(), gradient, dx)
+            _exactly("flayernorm_grad", cols, gamma, dgamma, dbeta)
+            _exactly("flayernorm_grad", rows, mean, rstd)
+            self.lib.call("polar_b200_flayernorm_grad", _ptr(gradient), _ptr(x), _ptr(gamma), _ptr(mean), _ptr(rstd), rows, cols,
+                          _ptr(dx), _ptr(dgamma), _ptr(dbeta), None, 0, _stream(dx))
+        return dx
+
+    def flogprob(self, logits, ids, logprob, entropy=None, logsumexp=None, top_ids=None, top_logprob=None):
+        """Per row of logits: the log probability of its id (0 where the id is below zero), the entropy, log(sum(exp)), and the
+        likeliest alternatives [rows, top] (up to 32; ids of the type of `ids`).  What is None is left out."""
+        if not self._native.flogprob(logits, ids, logprob, entropy, logsumexp, top_ids, top_logprob):
+            rows, classes, pitch = _matrix(logits)
+            some = _present(logprob, entropy, logsumexp, top_logprob)
+            if some:
+                _chk(*some)
+            kinds = {_ids(t) for t in _present(ids, top_ids)}
+            _same_device(logits, *some, *_present(ids, top_ids))
+            if len(kinds) > 1:
+                raise ValueError("flogprob: top_ids are of the type of ids")
+            _exactly("flogprob", rows, ids, logprob, entropy, logsumexp)
+            tops = {tuple(t.shape) for t in _present(top_ids, top_logprob)}
+            if len(tops) > 1 or any(len(s) != 2 or s[0] != rows for s in tops):
+                raise ValueError("flogprob: alternatives are [rows, top]")
+            if logprob is not None and ids is None:
+                raise ValueError("flogprob: a log probability needs ids")
+            self.lib.call("polar_b200_flogprob", _ptr(logits), rows, classes, pitch, _ptr(ids), kinds.pop() if kinds else 2,
+                          _ptr(logprob), _ptr(entropy), _ptr(logsumexp), tops.pop()[1] if tops else 0, _ptr(top_ids), _ptr(top_logprob),
+                          _stream(logits))
+        return logprob
+
+    def flogprob_grad(self, logits, ids, logsumexp, entropy, g_logprob, g_entropy, dlogits):
+        """The gradient at the logits of sum(g_logprob * logprob + g_entropy * entropy); entropy and g_entropy may be None."""
+        if not self._native.flogprob_grad(logits, ids, logsumexp, entropy, g_logprob, g_entropy, dlogits):
+            rows, classes, pitch = _matrix(logits)
+            drows, dclasses, dpitch = _matrix(dlogits)
+            given = _present(logsumexp, entropy, g_logprob, g_entropy)
+            _chk(*given)
+            kind = _ids(ids)
+            _same_device(logits, dlogits, ids, *given)
+            if (drows, dclasses) != (rows, classes):
+                raise ValueError("flogprob_grad: dlogits has the shape of logits")
+            _exactly("flogprob_grad", rows, ids, *given)
+            if g_entropy is not None and entropy is None:
+                raise ValueError("flogprob_grad: the entropy's gradient needs the entropy")
+            self.lib.call("polar_b200_flogprob_grad", _ptr(logits), rows, classes, pitch, _ptr(ids), kind, _ptr(logsumexp), _ptr(entropy),
+                          _ptr(g_logprob), _ptr(g_entropy), _ptr(dlogits), dpitch, _stream(dlogits))
+        return dlogits
+
+    def fadamw(self, weights, gradients, first, second, first_scales=None, second_scales=None, *, step=0, lr=0.0, beta1=0.9,
+               beta2=0.999, eps=1e-8, weight_decay=0.01, schedule=None):
+        """One AdamW step over lists of tensors, in place.  `first` and `second` are the moments: float32 of the weights' sizes or,
+        with scales, float8_e4m3fn (or uint8) codes of the weights' sizes, whose scales are float32 of ceil(n / 128).
+        weight_decay: one for all, or a list.  The number of the step (from 1) and lr come from the call or, for steps that are
+        captured, from `schedule`, a device tensor of the two."""
+        decays = [weight_decay] * len(weights) if isinstance(weight_decay, (int, float)) else weight_decay
+        if not self._native.fadamw(weights, gradients, first, second, first_scales, second_scales, step, lr, beta1, beta2, eps, decays,
+                                   schedule):
+            lists = _present(weights, gradients, first, second, first_scales, second_scales)
+            if (first_scales is None) != (second_scales is None) or any(len(x) != len(weights) for x in [*lists, decays]):
+                raise ValueError("fadamw: lists of one length, and scales for both moments or neither")
+            eight = first_scales is not None
+            tensors = (AdamwTensor * len(weights))()
+            for t, decay, w, g, m, v, *scales in zip(tensors, decays, *lists):
+                _chk(w, g, *scales, *(() if eight else (m, v)))
+                if eight and not all(x.is_cuda and x.is_contiguous() and x.dtype in (torch.float8_e4m3fn, torch.uint8) for x in (m, v)):
+                    raise ValueError("fadamw: moments in 8 bits are contiguous float8_e4m3fn or uint8 CUDA tensors")
+                _same_device(weights[0], w, g, m, v, *scales)
+                _exactly("fadamw", w.numel(), g, m, v)
+                _exactly("fadamw", -(-w.numel() // 128), *scales)
+                t.weights, t.gradient, t.first, t.second = (x.data_ptr() for x in (w, g, m, v))
+                if eight:
+                    t.first_scales, t.second_scales = (x.data_ptr() for x in scales)
+                t.count, t.weight_decay = w.numel(), float(decay)
+            if schedule is not None:
+                _chk(schedule)
+                _exactly("fadamw", 2, schedule)
+                _same_device(schedule, *weights[:1])
+            if int(step) < 0:
+                raise ValueError("fadamw: steps count from 1")
+            if weights:
+                options = AdamwOptions(float(lr), float(beta1), float(beta2), float(eps), int(step), _ptr(schedule))
+                self.lib.call("polar_b200_fadamw", tensors, len(weights), ctypes.byref(options), _stream(weights[0]))
+        return weights
 
     def device_status(self):
         return int(self.lib.cdll.polar_b200_device_status())
