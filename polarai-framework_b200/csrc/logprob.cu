@@ -39,71 +39,517 @@ __device__ __forceinline__ uint32_t ordered(float v) {
 }
 __device__ __forceinline__ uint64_t rank_of(float v, uint32_t index) { return (uint64_t)ordered(v) << 32 | (uint32_t)~index; }
 
-struct LogProbOut {
+// What the id, the sums and the alternatives of a row become.
+struct Results {
+  const void* ids;
+  int id_type;
   float *logprob, *entropy, *logsumexp;
   void* top_ids;
   float* top_logprob;
   uint32_t top;
 };
 
-__global__ void __launch_bounds__(kThreads) logprob_kernel(const float* logits, uint64_t classes, uint64_t pitch, const void* ids,
-                                                           int id_type, LogProbOut o) {
-  pdl_enter();
-  __shared__ float slots[2 * kThreads / 32], shared_max;
-  __shared__ unsigned long long best[kThreads / 32];
-  const uint64_t row = blockIdx.x;
-  const float* x = logits + row * pitch;
-  float m = -INFINITY;
-  for (uint64_t c = threadIdx.x; c < classes; c += kThreads) m = fmaxf(m, x[c]);
+// ---- the running sums ---------------------------------------------------------------------------------
+// A thread's (or a row's) maximum so far, clamped to finite values, with S and T relative to it.  A row of nothing but -inf keeps S = 0.
+struct Running {
+  float m = -3.402823466e38f, s = 0.f, t = 0.f;
+};
+// d = x - m never enters below this: the exponential is zero there, and zero times d is zero and no NaN.  NaN stays NaN.
+__device__ __forceinline__ float at_least(float d) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(d) : "f"(-1000.f));
+  return d;
+}
+__device__ __forceinline__ float exp_fast(float d) {       // 2^(d log2 e): off by |d| 2^-24 from the product and 2 ulp
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d * 1.4426950408889634f));
+  return e;
+}
+__device__ __forceinline__ void raise_to(Running& r, float m) {
+  const float d = at_least(r.m - m), f = exp_fast(d);
+  r.t = f * (r.t + d * r.s);
+  r.s *= f;
+  r.m = m;
+}
+__device__ __forceinline__ void add(Running& r, float x) {
+  const float d = at_least(x - r.m), e = exp_fast(d);
+  r.s += e;
+  r.t += e * d;
+}
+__device__ __forceinline__ void add4(Running& r, float4 v) {
+  const float d0 = at_least(v.x - r.m), d1 = at_least(v.y - r.m), d2 = at_least(v.z - r.m), d3 = at_least(v.w - r.m);
+  const float e0 = exp_fast(d0), e1 = exp_fast(d1), e2 = exp_fast(d2), e3 = exp_fast(d3);
+  r.s += (e0 + e1) + (e2 + e3);
+  r.t += (e0 * d0 + e1 * d1) + (e2 * d2 + e3 * d3);
+}
+__device__ __forceinline__ float max4(float4 v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
+__device__ __forceinline__ Running warp_join(Running r) {
+  float m = r.m;
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kThreads / 32; ++w) m = fmaxf(m, slots[w]);
-    shared_max = m;
+  raise_to(r, m);
+  r.s = warp_sum(r.s);
+  r.t = warp_sum(r.t);
+  return r;
+}
+
+// ---- a row as vectors -----------------------------------------------------------------------------------
+// Rows begin where they begin (an odd number of classes, a pitch): vector i holds the elements 4 i - shift ... + 3, so that all but the
+// first and the last one are whole and on a 16-byte boundary.
+struct Row {
+  const float* aligned;
+  uint32_t shift, classes, vectors, whole_from, whole_to;
+  __device__ __forceinline__ Row(const float* x, uint32_t n) {
+    shift = (uint32_t)(reinterpret_cast<uintptr_t>(x) & 15) >> 2;
+    aligned = x - shift;
+    classes = n;
+    vectors = (uint32_t)(((uint64_t)n + shift + 3) >> 2);
+    whole_from = shift ? 1 : 0;
+    whole_to = (uint32_t)(((uint64_t)n + shift) >> 2);
   }
-  __syncthreads();
-  m = shared_max == -INFINITY ? 0.f : shared_max;          // (a row of NaNs alone as well: its sum is NaN)
-  float s[2] = {0.f, 0.f};
-  for (uint64_t c = threadIdx.x; c < classes; c += kThreads) {
-    const float d = x[c] - m, e = expf(d);
-    s[0] += e;
-    if (!(e == 0.f)) s[1] += e * d;
+  __device__ __forceinline__ float4 whole(uint32_t i) const { return reinterpret_cast<const float4*>(aligned)[i]; }
+  __device__ __forceinline__ bool is_whole(uint32_t i) const { return i >= whole_from && i < whole_to; }
+  // whether component c of vector i is an element
+  __device__ __forceinline__ bool has(uint32_t i, uint32_t c) const {
+    const uint64_t e = 4ull * i + c;
+    return e >= shift && e < (uint64_t)classes + shift;
   }
-  block_sums<kThreads>(s, slots);
-  const bool dead = s[0] == 0.f;                           // nothing in the row has any probability
-  const float log_sum = logf(s[0]);
-  if (threadIdx.x == 0) {
-    if (o.logprob) {
-      const int64_t id = read_id(ids, id_type, row, classes);
-      o.logprob[row] = id == kPadding ? 0.f : id == kWrong ? NAN : dead ? -INFINITY : x[id] - m - log_sum;
+  __device__ __forceinline__ uint32_t element(uint32_t i, uint32_t c) const { return 4 * i + c - shift; }
+  // a vector at the edge, -inf where there is no element
+  __device__ __forceinline__ float4 edge(uint32_t i) const {
+    const float* p = aligned + 4ull * i;
+    return make_float4(has(i, 0) ? p[0] : -INFINITY, has(i, 1) ? p[1] : -INFINITY, has(i, 2) ? p[2] : -INFINITY, has(i, 3) ? p[3] : -INFINITY);
+  }
+  __device__ __forceinline__ float4 vector(uint32_t i) const { return is_whole(i) ? whole(i) : edge(i); }
+};
+
+// ---- the alternatives -----------------------------------------------------------------------------------
+// One pass finds them too.  If `top` threads or more have met a maximum of at least some bound, the `top` largest elements are all of at
+// least that bound.  So after the first few vectors, and again whenever the part of the row that has been seen has grown fourfold, the
+// threads' maxima give a bound (a search by counting them), and from then on an element that reaches it is kept: about 4 `top` for each
+// fourfold, whatever the row's length.  At the end the bound is taken once more, what it leaves (little more than `top`) is placed by
+// counting what is above it.  -inf is never kept: where fewer than `top` elements are above it, the first of it follow.  A row where more is kept
+// than there is room for (equal logits by the hundred), or with a NaN, which no maximum shows, is looked through a second time by
+// warps that sort as they go.
+constexpr float kLowest = -3.402823466e38f;
+constexpr int kInFlight = 4;                               // vectors of a thread in flight
+constexpr uint32_t kFewTop = 8;
+__device__ __forceinline__ float float_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+
+// The largest bound, nearly, that `top` of the LANES N keys of neighbouring lanes of a warp reach (all lanes take part; each group finds its
+// own).  Keys of kLowest count for vectors not met; with fewer keys than `top` that is the bound, and everything reaches it.
+template <int LANES, int N>
+__device__ __forceinline__ float bound_of(const uint32_t (&key)[N], uint32_t top) {
+  uint32_t most = 0, least = ~0u;
+#pragma unroll
+  for (int i = 0; i < N; ++i) most = max(most, key[i]), least = min(least, key[i]);
+  if (top <= kFewTop && top <= LANES) {                    // few: the largest key of the lanes, the next, ...
+    uint32_t mine = most, largest = 0;
+    for (uint32_t k = 0; k < top; ++k) {
+      largest = mine;
+      if (LANES == 32) {
+        largest = __reduce_max_sync(0xffffffffu, largest);
+      } else {
+#pragma unroll
+        for (int off = LANES / 2; off > 0; off >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, off));
+      }
+      if (mine == largest) mine = 0;                       // (more than one lane at a time where maxima are equal: 0 in the end, at most)
     }
-    if (o.entropy) o.entropy[row] = dead ? 0.f : log_sum - s[1] / s[0];
-    if (o.logsumexp) o.logsumexp[row] = dead ? -INFINITY : m + log_sum;
+    return float_of(max(largest, ordered(kLowest)));
   }
-  unsigned long long last = ~0ull;
-  for (uint32_t k = 0; k < o.top; ++k) {                   // the largest below the one before
-    unsigned long long mine = 0;
-    for (uint64_t c = threadIdx.x; c < classes; c += kThreads) {
-      const unsigned long long r = rank_of(x[c], (uint32_t)c);
-      if (r < last && r > mine) mine = r;
+  if (LANES == 32) {
+    most = __reduce_max_sync(0xffffffffu, most);
+    least = __reduce_min_sync(0xffffffffu, least);
+  } else {
+#pragma unroll
+    for (int off = LANES / 2; off > 0; off >>= 1) {
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
+      least = min(least, __shfl_xor_sync(0xffffffffu, least, off));
+    }
+  }
+  const uint32_t group = LANES == 32 ? 0xffffffffu : ((1u << (LANES & 31)) - 1) << (threadIdx.x & 31 & ~(LANES - 1));
+  // `top` or more reach lo, fewer reach hi; between them a step for each halving: maxima lie within a few powers of two
+  uint32_t lo = LANES * N >= kMaxTop || LANES * N >= top ? least : ordered(kLowest), hi = max(most + 1, lo);
+  while (LANES == 32 ? hi - lo > 1 : __any_sync(0xffffffffu, hi - lo > 1)) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    uint32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) n += __popc(__ballot_sync(0xffffffffu, key[i] >= mid) & group);
+    if (n >= top) lo = mid;
+    else hi = mid;
+    if (n >= top && n <= top + top / 4 + 1) hi = lo;
+  }
+  return float_of(lo);
+}
+
+// What a team (a CTA, a warp or a part of one) keeps.
+struct Kept {
+  unsigned long long* rank;
+  uint32_t* count;                                         // goes on beyond the room
+  uint32_t room;
+};
+
+// The running sums over the vectors first, first + stride, ... of a row, kInFlight of them on their way; `base` is the first of the warp's
+// `first`s, `chunks` the same for a warp (or, where bounds are a matter for the CTA, for all of it).  find_bound(maxima) takes the whole team.
+template <bool TOP, class FindBound>
+__device__ __forceinline__ Running scan(const Row& row, uint32_t base, uint32_t first, uint32_t stride, uint32_t chunks, float (&maxima)[kInFlight],
+                                        const Kept& kept, FindBound find_bound) {
+  Running r;
+  float bound = INFINITY;
+  const uint32_t chunk = kInFlight * stride;
+  uint32_t next_bound = 0;
+  const bool edges = row.whole_from != 0 || row.whole_to != row.vectors;
+#pragma unroll
+  for (int u = 0; u < kInFlight; ++u) maxima[u] = kLowest;
+  for (uint32_t n = 0; n < chunks; ++n) {
+    const uint32_t i = first + n * chunk;
+    float4 v[kInFlight];
+    const bool inner = n > 0 && (n + 1) * chunk <= row.whole_to;   // all vectors of the chunk are whole
+    if (inner) {
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u) v[u] = row.whole(i + u * stride);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u) {
+        v[u] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (row.is_whole(i + u * stride)) v[u] = row.whole(i + u * stride);
+      }
+      if (edges) {
+#pragma unroll
+        for (int u = 0; u < kInFlight; ++u)
+          if (i + u * stride < row.vectors && !row.is_whole(i + u * stride)) v[u] = row.edge(i + u * stride);
+      }
+    }
+    float m[kInFlight], most;
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      m[u] = max4(v[u]);
+      if (TOP) maxima[u] = fmaxf(maxima[u], m[u]);
+    }
+    most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+    if (most > r.m) raise_to(r, most);
+    if (TOP) {
+      if (n == next_bound) {
+        bound = find_bound(maxima, r.m);
+        next_bound = 4 * n + 3;
+      }
+      if (most >= bound && *(volatile uint32_t*)kept.count <= kept.room) {
+        uint32_t which = 0;                                // of the 16 elements, those that reach the bound
+#pragma unroll
+        for (int u = 0; u < kInFlight; ++u)
+          which |= (v[u].x >= bound ? 1u << 4 * u : 0) | (v[u].y >= bound ? 2u << 4 * u : 0) | (v[u].z >= bound ? 4u << 4 * u : 0) |
+                   (v[u].w >= bound ? 8u << 4 * u : 0);
+        while (which) {
+          const uint32_t e = __ffs(which) - 1, u = e >> 2;
+          which &= which - 1;
+          const float4 x = u & 2 ? (u & 1 ? v[3] : v[2]) : (u & 1 ? v[1] : v[0]);
+          const float value = e & 2 ? (e & 1 ? x.w : x.z) : (e & 1 ? x.y : x.x);
+          const uint32_t at = atomicAdd(kept.count, 1u);
+          if (at < kept.room) kept.rank[at] = rank_of(value, row.element(i + u * stride, e & 3));
+        }
+      }
     }
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      const unsigned long long other = __shfl_xor_sync(0xffffffffu, mine, off);
-      mine = other > mine ? other : mine;
+    for (int u = 0; u < kInFlight; ++u)
+      if (inner || base + n * chunk + u * stride < row.vectors) add4(r, v[u]);
+  }
+  return r;
+}
+
+// A warp's sorted list of ranks, the largest in lane 0; takes the elements of one vector per lane.
+__device__ __forceinline__ void take(unsigned long long& list, const Row& row, uint32_t i, uint32_t top, uint32_t lane) {
+  const float4 v = i < row.vectors ? row.vector(i) : make_float4(0.f, 0.f, 0.f, 0.f);
+  const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (uint32_t c = 0; c < 4; ++c) {
+    const unsigned long long rank = i < row.vectors && row.has(i, c) ? rank_of(x[c], row.element(i, c)) : 0;
+    uint32_t left = __ballot_sync(0xffffffffu, rank > __shfl_sync(0xffffffffu, list, top - 1));
+    while (left) {
+      const unsigned long long r = __shfl_sync(0xffffffffu, rank, __ffs(left) - 1), above = __shfl_up_sync(0xffffffffu, list, 1);
+      const uint32_t at = __popc(__ballot_sync(0xffffffffu, list > r));
+      if (lane == at) list = r;
+      else if (lane > at) list = above;
+      left &= left - 1;
+      left &= __ballot_sync(0xffffffffu, rank > __shfl_sync(0xffffffffu, list, top - 1));
     }
-    if ((threadIdx.x & 31) == 0) best[threadIdx.x >> 5] = mine;
-    __syncthreads();
-    last = 0;
-    for (int w = 0; w < kThreads / 32; ++w) last = best[w] > last ? best[w] : last;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      const uint32_t at = ~(uint32_t)last;
-      if (o.top_ids) write_id(o.top_ids, id_type, row * o.top + k, at);
-      if (o.top_logprob) o.top_logprob[row * o.top + k] = dead ? -INFINITY : x[at] - m - log_sum;
+  }
+}
+// The first `wanted` elements of -inf among the vectors that a team has, in their order, one after the other into `to`; by one warp.
+__device__ __forceinline__ void take_shut_out(unsigned long long* to, uint32_t wanted, const Row& row, uint32_t begin, uint32_t width, uint32_t stride,
+                                              uint32_t lane) {
+  uint32_t found = 0;
+  for (uint32_t j = lane;; j += 32) {
+    const uint32_t i = j / width * stride + begin + j % width;
+    if (!__any_sync(0xffffffffu, i < row.vectors) || found >= wanted) return;
+    const float4 v = i < row.vectors ? row.vector(i) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float x[4] = {v.x, v.y, v.z, v.w};
+    uint32_t mine = 0;
+#pragma unroll
+    for (uint32_t c = 0; c < 4; ++c) mine += x[c] == -INFINITY && i < row.vectors && row.has(i, c);
+    uint32_t at = mine;                                    // lanes lie in the order of their elements
+#pragma unroll
+    for (int off = 1; off < 32; off *= 2) {
+      const uint32_t o = __shfl_up_sync(0xffffffffu, at, off);
+      if ((int)lane >= off) at += o;
     }
+    const uint32_t all = __shfl_sync(0xffffffffu, at, 31);
+    at += found - mine;
+#pragma unroll
+    for (uint32_t c = 0; c < 4; ++c)
+      if (x[c] == -INFINITY && i < row.vectors && row.has(i, c)) {
+        if (at < wanted) to[at] = rank_of(x[c], row.element(i, c));
+        ++at;
+      }
+    found += all;
+  }
+}
+__device__ __forceinline__ void write_row(const Results& o, uint64_t row, int64_t id, float given, const Running& r) {
+  const float log_sum = logf(r.s);
+  const bool dead = r.s == 0.f;
+  if (o.logprob) o.logprob[row] = id == kPadding ? 0.f : id == kWrong ? NAN : dead ? -INFINITY : given - r.m - log_sum;
+  if (o.entropy) o.entropy[row] = dead ? 0.f : log_sum - r.t / r.s;
+  if (o.logsumexp) o.logsumexp[row] = dead ? -INFINITY : r.m + log_sum;
+}
+__device__ __forceinline__ void write_top(const Results& o, uint64_t row, uint32_t at, uint32_t id, float x, const Running& r, float log_sum) {
+  if (o.top_ids) write_id(o.top_ids, o.id_type, row * o.top + at, id);
+  if (o.top_logprob) o.top_logprob[row * o.top + at] = r.s == 0.f ? -INFINITY : x - r.m - log_sum;
+}
+__device__ __forceinline__ void write_top(const Results& o, uint64_t row, uint32_t at, unsigned long long rank, const Running& r) {
+  write_top(o, row, at, ~(uint32_t)rank, float_of((uint32_t)(rank >> 32)), r, logf(r.s));
+}
+
+// Many classes: a CTA per row, or a cluster of CTAs where there are few rows.
+template <int THREADS, bool TOP>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_wide_kernel(const float* logits, uint32_t classes, uint64_t pitch, Results o) {
+  constexpr uint32_t kWarps = THREADS / 32, kRoom = TOP ? 512 : 1, kTop = TOP ? kMaxTop : 1;
+  __shared__ float part[3][kWarps], joined[3];
+  __shared__ unsigned long long kept_ranks[kRoom], left[kRoom], sorted[kTop], theirs[8 * kTop];
+  __shared__ uint32_t n_kept, n_left, keys[2][TOP ? THREADS : 1];
+  pdl_enter();
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, ctas = gridDim.y, rank = blockIdx.y;
+  const uint64_t r = blockIdx.x;
+  const Row row(logits + r * pitch, classes);
+  const uint32_t first = rank * THREADS + tid, stride = ctas * THREADS;
+  int64_t id = kPadding;
+  float given = 0.f;
+  if (rank == 0 && tid == 0 && o.logprob) {
+    id = read_id(o.ids, o.id_type, r, classes);
+    if (id >= 0) given = logits[r * pitch + id];
+  }
+  if (TOP) {
+    if (tid == 0) n_kept = n_left = 0;
+    if (tid < kMaxTop) sorted[tid] = 0;
+  }
+  int turn = 0;
+  // (two arrays in turn: a barrier is between a round's reads and the writes of the next but one)
+  auto find_bound = [&](const float (&)[kInFlight], float mine) {
+    uint32_t k[4];                                         // of 128 groups of threads: enough for 32 alternatives
+    keys[turn][tid] = ordered(mine);
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      k[i] = keys[turn][32 * i + lane];
+#pragma unroll
+      for (uint32_t j = 128; j < THREADS; j += 128) k[i] = max(k[i], keys[turn][j + 32 * i + lane]);
+    }
+    turn ^= 1;
+    return bound_of<32>(k, o.top);
+  };
+  float maxima[kInFlight];
+  const uint32_t chunks = (row.vectors + kInFlight * stride - 1) / (kInFlight * stride);
+  const Running own = scan<TOP>(row, first - lane, first, stride, chunks, maxima, Kept{kept_ranks, &n_kept, kRoom}, find_bound);
+  Running all = warp_join(own);
+  if (lane == 0) part[0][warp] = all.m, part[1][warp] = all.s, part[2][warp] = all.t;
+  __syncthreads();
+  all = Running();
+  if (lane < kWarps) all.m = part[0][lane], all.s = part[1][lane], all.t = part[2][lane];
+  all = warp_join(all);
+  if (TOP) {
+    const uint32_t n = n_kept;                             // the same for all threads, as what hangs on it
+    if (n <= kRoom && all.s == all.s) {
+      const float bound = n > 64 ? find_bound(maxima, own.m) : kLowest;
+      for (uint32_t i = tid; i < n; i += THREADS)
+        if (kept_ranks[i] >= (uint64_t)ordered(bound) << 32) left[atomicAdd(&n_left, 1u)] = kept_ranks[i];
+    } else {
+      unsigned long long list = 0;
+      for (uint32_t j = warp * 32 + lane;; j += THREADS) {
+        const uint32_t i = j / THREADS * stride + rank * THREADS + j % THREADS;
+        if (!__any_sync(0xffffffffu, i < row.vectors)) break;
+        take(list, row, i, o.top, lane);
+      }
+      if (lane < o.top && list) left[atomicAdd(&n_left, 1u)] = list;
+    }
+    __syncthreads();
+    const uint32_t total = n_left;
+    for (uint32_t i = tid; i < total; i += THREADS) {      // no two ranks are alike: a place for each
+      uint32_t above = 0;
+      const unsigned long long mine = left[i];
+      for (uint32_t j = 0; j < total; ++j) above += left[j] > mine;
+      if (above < o.top) sorted[above] = mine;
+    }
+    if (total < o.top && warp == 0) take_shut_out(sorted + total, o.top - total, row, rank * THREADS, THREADS, stride, lane);
+    __syncthreads();
+  }
+  if (ctas == 1) {
+    if (tid == 0) write_row(o, r, id, given, all);
+    if (TOP && tid < o.top) write_top(o, r, tid, sorted[tid], all);
+    return;
+  }
+  if (tid == 0) joined[0] = all.m, joined[1] = all.s, joined[2] = all.t;
+  __syncthreads();
+  cluster_arrive();
+  cluster_wait();
+  if (rank == 0) {
+    all = Running();
+    if (lane < ctas) all.m = ld_cluster(&joined[0], lane), all.s = ld_cluster(&joined[1], lane), all.t = ld_cluster(&joined[2], lane);
+    all = warp_join(all);
+    if (tid == 0) write_row(o, r, id, given, all);
+    if (TOP) {
+      const uint32_t total = ctas * o.top;
+      for (uint32_t i = tid; i < total; i += THREADS)
+        theirs[i] = __double_as_longlong(ld_cluster(reinterpret_cast<const double*>(&sorted[i % o.top]), i / o.top));
+      __syncthreads();
+      for (uint32_t i = tid; i < total; i += THREADS) {
+        uint32_t above = 0;
+        const unsigned long long mine = theirs[i];
+#pragma unroll
+        for (uint32_t c = 0; c < 8; ++c) {                 // each list is sorted: how many of it are above, a halving at a time
+          uint32_t n = 0;
+#pragma unroll
+          for (uint32_t step = 32; step > 0; step /= 2)
+            if (c < ctas && n + step <= o.top && theirs[c * o.top + n + step - 1] > mine) n += step;
+          above += n;
+        }
+        if (above < o.top && mine) write_top(o, r, above, mine, all);
+      }
+    }
+  }
+  cluster_arrive();                                        // nobody leaves while its shared memory may still be read
+  cluster_wait();
+}
+
+// A warp per row or, for short rows, LANES lanes.
+template <int LANES, bool TOP>
+__global__ void __launch_bounds__(kThreads) logprob_warp_kernel(const float* logits, uint32_t rows, uint32_t classes, uint64_t pitch, Results o) {
+  constexpr uint32_t kRoom = TOP ? 128 : 1, kTeams = kThreads / LANES, kRows = 32 / LANES;
+  __shared__ unsigned long long kept_ranks[kTeams][kRoom];
+  __shared__ uint32_t n_kept[kTeams];
+  pdl_enter();
+  const uint32_t lane = threadIdx.x & 31, team = threadIdx.x / LANES, member = threadIdx.x % LANES;
+  const uint64_t r = (uint64_t)blockIdx.x * kTeams + team;
+  if (r - team % kRows >= rows) return;                    // (a whole warp)
+  const Row row(logits + (r < rows ? r : rows - 1) * pitch, classes);   // (lanes without a row of their own look at the last)
+  int64_t id = kPadding;
+  float given = 0.f;
+  if (member == 0 && o.logprob && r < rows) {
+    id = read_id(o.ids, o.id_type, r, classes);
+    if (id >= 0) given = logits[r * pitch + id];
+  }
+  unsigned long long* kept = kept_ranks[team];
+  if (TOP && member == 0) n_kept[team] = 0;
+  __syncwarp();
+  auto find_bound = [&](const float (&maxima)[kInFlight], float) {
+    uint32_t k[kInFlight];
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) k[u] = ordered(maxima[u]);
+    return bound_of<LANES>(k, o.top);
+  };
+  float maxima[kInFlight];
+  // (rows that begin elsewhere on a boundary may have a vector more or less: as many chunks as the longest)
+  const uint32_t chunks = ((classes + 6) / 4 + kInFlight * LANES - 1) / (kInFlight * LANES);
+  const Running own = scan<TOP>(row, 0, member, LANES, chunks, maxima, Kept{kept, &n_kept[team], kRoom}, find_bound);
+  Running all = own;
+  float m = own.m;
+#pragma unroll
+  for (int off = LANES / 2; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  raise_to(all, m);
+#pragma unroll
+  for (int off = LANES / 2; off > 0; off >>= 1) {
+    all.s += __shfl_xor_sync(0xffffffffu, all.s, off);
+    all.t += __shfl_xor_sync(0xffffffffu, all.t, off);
+  }
+  if (member == 0 && r < rows) write_row(o, r, id, given, all);
+  if (!TOP) return;
+  __syncwarp();
+  const uint32_t n = n_kept[team];
+  const bool sorts = n > kRoom || all.s != all.s;
+  uint32_t total = 0;
+  if (!sorts) {
+    for (uint32_t i = member; i < n; i += LANES) {
+      uint32_t above = 0;
+      const unsigned long long mine = kept[i];
+      for (uint32_t j = 0; j < n; ++j) above += kept[j] > mine;
+      if (above < o.top && r < rows) write_top(o, r, above, mine, all);
+    }
+    total = n;
+  }
+  // rows that the warp looks through again, one after the other
+  const uint32_t again = __ballot_sync(0xffffffffu, (sorts || total < o.top) && member == 0 && r < rows);
+  for (uint32_t left = again; left; left &= left - 1) {
+    const int who = __ffs(left) - 1;
+    const uint64_t q = r - team % kRows + who / LANES;
+    const Row its(logits + q * pitch, classes);
+    Running sums;
+    sums.m = __shfl_sync(0xffffffffu, all.m, who), sums.s = __shfl_sync(0xffffffffu, all.s, who), sums.t = 0.f;
+    const uint32_t have = __shfl_sync(0xffffffffu, total, who);
+    if (__shfl_sync(0xffffffffu, (int)sorts, who)) {
+      unsigned long long list = 0;
+      for (uint32_t i = lane; i - lane < its.vectors; i += 32) take(list, its, i, o.top, lane);
+      if (lane < o.top) write_top(o, q, lane, list, sums);
+    } else {
+      unsigned long long* to = kept_ranks[team - team % kRows + who / LANES];
+      __syncwarp();
+      take_shut_out(to, o.top - have, its, 0, 32, 32, lane);
+      __syncwarp();
+      if (lane + have < o.top) write_top(o, q, lane + have, to[lane], sums);
+    }
+  }
+}
+
+// Up to kThreadClasses classes: a thread per row, its logits in registers.  STAGED: the rows come through shared memory, since 32 threads
+// that each read a float of a long row touch as many cache lines at a time (65536 x 32: 12.7 us, 7.6 staged; 65536 x 10: 2.8, 5.2 staged).
+constexpr uint32_t kThreadClasses = 32, kThreadRows = 128;
+template <int MOST, bool STAGED>
+__global__ void __launch_bounds__(kThreadRows) logprob_thread_kernel(const float* logits, uint32_t rows, uint32_t classes, uint64_t pitch, Results o) {
+  __shared__ float tile[STAGED ? kThreadRows * (MOST | 1) : 1];
+  pdl_enter();
+  const uint64_t r0 = (uint64_t)blockIdx.x * kThreadRows, r = r0 + threadIdx.x;
+  const float* x = logits + r * pitch;
+  if (STAGED) {
+    const uint32_t here = rows - r0 < kThreadRows ? (uint32_t)(rows - r0) : kThreadRows, wide = classes | 1;   // (odd: no two threads in a bank)
+    for (uint32_t e = threadIdx.x; e < here * classes; e += kThreadRows) {
+      const uint32_t q = e / classes, c = e - q * classes;
+      tile[q * wide + c] = logits[(r0 + q) * pitch + c];
+    }
+    x = tile + threadIdx.x * wide;
+    __syncthreads();
+  }
+  if (r >= rows) return;
+  float v[MOST];
+#pragma unroll
+  for (int c = 0; c < MOST; ++c) v[c] = c < classes ? x[c] : -INFINITY;
+  int64_t id = kPadding;
+  float given = 0.f;
+  if (o.logprob) {
+    id = read_id(o.ids, o.id_type, r, classes);
+    if (id >= 0) given = x[id];
+  }
+  Running all;
+#pragma unroll
+  for (int c = 0; c < MOST; ++c) all.m = fmaxf(all.m, v[c]);
+#pragma unroll
+  for (int c = 0; c < MOST; ++c) add(all, v[c]);
+  write_row(o, r, id, given, all);
+  const float log_sum = logf(all.s);
+  unsigned long long last = ~0ull;
+  for (uint32_t k = 0; k < o.top; ++k) {                   // the largest below the one before
+    unsigned long long best = 0;
+#pragma unroll
+    for (int c = 0; c < MOST; ++c) {
+      const unsigned long long q = c < classes ? rank_of(v[c], c) : 0;
+      if (q < last && q > best) best = q;
+    }
+    write_top(o, r, k, ~(uint32_t)best, float_of((uint32_t)(best >> 32)), all, log_sum);
+    last = best;
   }
 }
 
@@ -166,8 +612,37 @@ int polar_b200_flogprob(const float* logits, uint64_t rows, uint64_t classes, ui
   const void* some = logprob ? logprob : entropy ? entropy : logsumexp ? logsumexp : top_logprob ? (const void*)top_logprob : top_ids;
   if (!some) return POLAR_B200_OK;                         // nothing is asked for
   LaunchDeviceScope on(stream, some);
-  return launch("flogprob", logprob_kernel, dim3((unsigned)rows), kThreads, 0, as_stream(stream), logits, classes, pitch, ids, id_type,
-                LogProbOut{logprob, entropy, logsumexp, top_ids, top_logprob, (uint32_t)top});
+  cudaStream_t st = as_stream(stream);
+  const Results o{ids, id_type, logprob, entropy, logsumexp, top_ids, top_logprob, (uint32_t)top};
+  const uint32_t n = (uint32_t)classes;
+  if (classes <= kThreadClasses) {
+    const dim3 grid((unsigned)((rows + kThreadRows - 1) / kThreadRows));
+    auto go = [&](auto kernel) { return launch("flogprob", kernel, grid, kThreadRows, 0, st, logits, (uint32_t)rows, n, pitch, o); };
+    return classes <= 8 ? go(logprob_thread_kernel<8, false>) : classes <= 16 ? go(logprob_thread_kernel<16, false>) : go(logprob_thread_kernel<32, true>);
+  }
+  // A warp per row as long as there are rows enough for every SM (20000 x 8192: 95 us against 104 with a CTA of 128 threads per row, with five
+  // alternatives 131 and 162; 300 x 8000 with five 18.6 and 8.4; up to 1024 classes always); eight lanes for the shortest (60000 x 100: 7.6 us
+  // against 20, with five alternatives 23 and 63).
+  const uint64_t sms = (uint64_t)sm_count();
+  if (classes <= 1024 || (classes <= 8192 && rows >= 16 * sms)) {
+    const uint32_t lanes = classes <= 128 ? 8 : 32;
+    const dim3 grid((unsigned)((rows * lanes + kThreads - 1) / kThreads));
+    auto go = [&](auto kernel) { return launch("flogprob", kernel, grid, kThreads, 0, st, logits, (uint32_t)rows, n, pitch, o); };
+    return lanes == 8 ? (top ? go(logprob_warp_kernel<8, true>) : go(logprob_warp_kernel<8, false>))
+                      : (top ? go(logprob_warp_kernel<32, true>) : go(logprob_warp_kernel<32, false>));
+  }
+  // Few rows: clusters of up to eight CTAs per row, the largest that the SMs hold at two per SM, of 512 threads (1 x 131072: 4.3 us, with
+  // twenty alternatives 9.1; of 128 threads 6.3 and 14.2).  Many rows: CTAs of 128 threads, since barriers then hold up fewer loads
+  // (2048 x 50001: 69 us, with five alternatives 81; of 512 threads 76 and 96); in between 256 (300 x 8000 with five 7.1 us, 128 threads 8.4).
+  unsigned ctas = 1;
+  while (ctas < 8 && rows * ctas * 2 <= 2 * sms && classes / (2 * ctas) >= 4096) ctas *= 2;
+  const dim3 grid((unsigned)rows, ctas);
+  auto go = [&](auto with, auto without, unsigned threads) {
+    return launch_clusters("flogprob", top ? with : without, grid, threads, 0, st, ctas, logits, n, pitch, o);
+  };
+  if (ctas > 1) return go(logprob_wide_kernel<512, true>, logprob_wide_kernel<512, false>, 512);
+  return rows >= 4 * sms ? go(logprob_wide_kernel<128, true>, logprob_wide_kernel<128, false>, 128)
+                         : go(logprob_wide_kernel<256, true>, logprob_wide_kernel<256, false>, 256);
 }
 
 int polar_b200_flogprob_grad(const float* logits, uint64_t rows, uint64_t classes, uint64_t pitch, const void* ids, int id_type,
