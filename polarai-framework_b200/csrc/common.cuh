@@ -185,6 +185,29 @@ int launch(const char* what, void (*kernel)(P...), dim3 grid, unsigned threads, 
   return launch_clusters(what, kernel, grid, threads, smem, stream, 1, args...);
 }
 
+// The same for a kernel of one large parameter, which is handed on where it lies: by value it would be copied three times on the way (32 KB:
+// some 4 us of host time).
+template <typename P>
+int launch_large(const char* what, void (*kernel)(const P), dim3 grid, unsigned threads, cudaStream_t stream, P& param) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid;
+  c.blockDim = dim3(threads);
+  c.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = at;
+  c.numAttrs = 1;
+  void* args[1] = {&param};
+  cudaError_t e = cudaLaunchKernelExC(&c, reinterpret_cast<const void*>(kernel), args);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(POLAR_B200_ERR_CUDA, what, e);
+  }
+  count_launch();
+  return POLAR_B200_OK;
+}
+
 // ---- clusters: the CTA's rank, the two halves of the cluster barrier, a read of another CTA's shared memory
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
