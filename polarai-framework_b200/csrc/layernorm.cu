@@ -11,7 +11,159 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Rows of any length, any alignment: three passes over a row that the caches hold.
+// A load (0 otherwise) and a store where k < live, under predicates: the compiler makes a branch of each, some four instructions more for every
+// float (65536 x 1511: 174 us, so 133).
+__device__ __forceinline__ float ld_if(const float* p, int k, uint32_t live) {
+  float v;
+  asm volatile("{.reg .pred q; setp.lt.s32 q, %2, %3; mov.f32 %0, 0f00000000; @q ld.global.f32 %0, [%1];}" : "=f"(v) : "l"(p), "r"(k), "r"(live) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_if(const float4* p, int k, uint32_t live) {
+  float4 v;
+  asm volatile("{.reg .pred q; setp.lt.s32 q, %5, %6; mov.f32 %0, 0f00000000; mov.f32 %1, 0f00000000; mov.f32 %2, 0f00000000; mov.f32 %3, 0f00000000;"
+               " @q ld.global.v4.f32 {%0, %1, %2, %3}, [%4];}"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p), "r"(k), "r"(live) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_if(float* p, float v, int k, uint32_t live) {
+  asm volatile("{.reg .pred q; setp.lt.s32 q, %2, %3; @q st.global.f32 [%0], %1;}" ::"l"(p), "f"(v), "r"(k), "r"(live) : "memory");
+}
+__device__ __forceinline__ void st_if(float4* p, float4 v, int k, uint32_t live) {
+  asm volatile("{.reg .pred q; setp.lt.s32 q, %5, %6; @q st.global.v4.f32 [%0], {%1, %2, %3, %4};}" ::"l"(p), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w),
+               "r"(k), "r"(live)
+               : "memory");
+}
+
+// A thread's share of a row: 4 V elements of it, TEAM threads to a row.  VECTOR: vectors of four, a team's side by side; else single floats.
+// Of the V fours, all threads have the first FULL (cols >= 4 TEAM FULL); `live`: how many of the vectors or floats this thread has in all.
+template <int TEAM, int V, bool VECTOR, int FULL>
+struct Share {
+  static constexpr int N = 4 * V;
+  static __device__ __forceinline__ uint32_t live(uint32_t member, uint32_t cols) {
+    const uint32_t first = VECTOR ? 4 * member : member, step = VECTOR ? 4 * TEAM : TEAM;
+    return first < cols ? (cols - first + step - 1) / step : 0;
+  }
+  static __device__ __forceinline__ bool has(uint32_t live, int k) { return k < 4 * FULL || (VECTOR ? k / 4 : k) < (int)live; }
+  static __device__ __forceinline__ void load(float (&v)[N], const float* row, uint32_t member, uint32_t live) {
+    if (VECTOR) {
+      const float4* p = reinterpret_cast<const float4*>(row) + member;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float4 x = i < FULL ? p[TEAM * i] : ld_if(p + TEAM * i, i, live);
+        v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
+      }
+    } else {
+      const float* p = row + member;
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[k] = k < 4 * FULL ? p[TEAM * k] : ld_if(p + TEAM * k, k, live);
+    }
+  }
+  static __device__ __forceinline__ void store(const float (&v)[N], float* row, uint32_t member, uint32_t live) {
+    if (VECTOR) {
+      float4* p = reinterpret_cast<float4*>(row) + member;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float4 x = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        if (i < FULL) p[TEAM * i] = x;
+        else st_if(p + TEAM * i, x, i, live);
+      }
+    } else {
+      float* p = row + member;
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (k < 4 * FULL) p[TEAM * k] = v[k];
+        else st_if(p + TEAM * k, v[k], k, live);
+    }
+  }
+};
+// Sums over the threads of a team: lanes side by side, or the CTA (`slots` as for block_sums).
+template <int TEAM, int N>
+__device__ __forceinline__ void team_sums(float (&v)[N], float* slots) {
+  if (TEAM > 32) {
+    block_sums<TEAM < 32 ? 32 : TEAM>(v, slots);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int off = TEAM / 2; off > 0; off >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], off);
+  }
+}
+
+// The sum over the CTAs of a cluster, added in the same order in each of them.
+template <int CTAS>
+__device__ __forceinline__ float cluster_sum(float v, float* mine) {
+  if (CTAS == 1) return v;
+  if (threadIdx.x == 0) *mine = v;
+  __syncthreads();
+  cluster_arrive();
+  cluster_wait();
+  float part[CTAS], s = 0.f;
+#pragma unroll
+  for (int r = 0; r < CTAS; ++r) part[r] = ld_cluster(mine, (uint32_t)r);
+#pragma unroll
+  for (int r = 0; r < CTAS; ++r) s += part[r];
+  return s;
+}
+
+// Forward, a row in a team's registers: read once, summed twice.  CTAS > 1: a cluster of so many CTAs, as one team.  A CTA's loads, sums and
+// stores take turns, so several CTAs have to share an SM: at least 1024 threads of them (512 with 24 elements or more per thread, but for the widest
+// rows: 16384 x 16384 with one CTA of 512 threads on an SM 452 us, with two, in 64 registers, 311).
+constexpr int resident(int lanes, int v) {
+  const int threads = lanes > 32 ? lanes : kThreads, least = v > 4 && lanes < 512 ? 512 : 1024;
+  return least / threads > 1 ? least / threads : 1;
+}
+template <int LANES, int V, bool VECTOR, int FULL, int CTAS>
+__global__ void __launch_bounds__(LANES > 32 ? LANES : kThreads, resident(LANES, V)) norm_rows_kernel(const float* in, const float* gamma, const float* beta, float eps,
+                                                                              uint32_t rows, uint32_t cols, float per_col, float* out,
+                                                                              float* mean_out, float* rstd_out) {
+  using S = Share<LANES * CTAS, V, VECTOR, FULL>;
+  constexpr int kBlock = LANES > 32 ? LANES : kThreads;
+  __shared__ float slots[2][kBlock / 32], part[2];
+  pdl_enter();
+  const uint32_t member = blockIdx.y * LANES + threadIdx.x % LANES;   // (blockIdx.y: the CTA's rank in its cluster)
+  const uint64_t r = (uint64_t)blockIdx.x * (kBlock / LANES) + threadIdx.x / LANES;
+  const uint32_t live = S::live(member, cols);
+  float x[S::N];
+  S::load(x, in + (r < rows ? r : rows - 1) * cols, member, live);   // (the lanes of a warp stay together, with a row or without)
+  float s[1] = {0.f};
+#pragma unroll
+  for (int k = 0; k < S::N; ++k) s[0] += x[k];
+  team_sums<LANES>(s, slots[0]);
+  const float mean = cluster_sum<CTAS>(s[0], &part[0]) * per_col;
+  s[0] = 0.f;
+#pragma unroll
+  for (int k = 0; k < S::N; ++k) {
+    x[k] -= mean;
+    if (S::has(live, k)) s[0] += x[k] * x[k];
+  }
+  team_sums<LANES>(s, slots[1]);
+  const float rstd = rsqrtf(cluster_sum<CTAS>(s[0], &part[1]) * per_col + eps);
+  if (CTAS > 1) cluster_arrive();                          // (nobody leaves while its part may still be read)
+  if (r >= rows) return;                                   // (of a cluster, all or none)
+  if (gamma) {
+    float g[S::N];
+    S::load(g, gamma, member, live);
+#pragma unroll
+    for (int k = 0; k < S::N; ++k) x[k] = x[k] * rstd * g[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < S::N; ++k) x[k] = x[k] * rstd;
+  }
+  if (beta) {
+    float b[S::N];
+    S::load(b, beta, member, live);
+#pragma unroll
+    for (int k = 0; k < S::N; ++k) x[k] = x[k] + b[k];
+  }
+  S::store(x, out + r * cols, member, live);
+  if (member == 0) {
+    if (mean_out) mean_out[r] = mean;
+    if (rstd_out) rstd_out[r] = rstd;
+  }
+  if (CTAS > 1) cluster_wait();
+}
+
+// Rows of any length: three passes over a row that the caches hold.
 __global__ void __launch_bounds__(kThreads) norm_kernel(const float* in, const float* gamma, const float* beta, float eps,
                                                         uint64_t cols, float* out, float* mean_out, float* rstd_out) {
   pdl_enter();
@@ -111,6 +263,52 @@ int polar_b200_flayernorm(const float* in, const float* gamma, const float* beta
   if (rows > kMaxRows || cols > kMaxCols) return fail(POLAR_B200_ERR_INVALID, "flayernorm: too many rows or columns");
   if (!in || !out) return fail(POLAR_B200_ERR_INVALID, "null device pointer");
   LaunchDeviceScope on(stream, out);
+  const bool vectors = (cols & 3) == 0 && aligned16(in) && aligned16(out) && aligned16(gamma) && aligned16(beta);
+  cudaStream_t st = as_stream(stream);
+  auto go = [&](auto with, auto without, unsigned lanes, unsigned ctas) {
+    const unsigned per_cta = lanes > 32 ? 1 : kThreads / lanes;
+    return launch_clusters("flayernorm", vectors ? with : without, dim3((unsigned)((rows + per_cta - 1) / per_cta), ctas),
+                           lanes > 32 ? lanes : kThreads, 0, st, ctas, in, gamma, beta, eps, (uint32_t)rows, (uint32_t)cols, (float)(1.0 / (double)cols), out, mean, rstd);
+  };
+#define ROWS(LANES, V, FULL, CTAS) go(norm_rows_kernel<LANES, V, true, FULL, CTAS>, norm_rows_kernel<LANES, V, false, FULL, CTAS>, LANES, CTAS)
+#define LANES_OF(V)                       \
+  switch (lanes) {                        \
+    case 8: return ROWS(8, V, V - 1, 1);         \
+    case 16: return ROWS(16, V, V - 1, 1);       \
+    case 32: return ROWS(32, V, V - 1, 1);       \
+    case 64: return ROWS(64, V, V - 1, 1);       \
+    case 128: return ROWS(128, V, V - 1, 1);     \
+    case 256: return ROWS(256, V, V - 1, 1);     \
+    case 512: return ROWS(512, V, V - 1, 1);     \
+    default: return ROWS(1024, V, V - 1, 1);     \
+  }
+  // How many elements a thread takes: 4 where there are few rows, for the shortest chain; 8 while the threads do not fill the SMs; then 16 and,
+  // of long rows, 32, whose loads are all in flight at once (65536 x 4096 in teams of 128 threads: 312 us, of 256 314, of 512 403).
+  const uint64_t sms = (uint64_t)sm_count();
+  // (The number of elements per thread that a form is made for is its V: FULL fours of every thread are there without asking, so each form serves
+  // cols > 4 LANES CTAS FULL only.)
+  const bool few = rows <= 2 * sms, little = rows * cols < (4ull << 20);
+  if (cols <= 8192) {
+    const unsigned each = few && cols <= 4096 ? 4 : little ? 8 : vectors && cols >= 4096 ? 32 : 16;
+    if (vectors && !little && cols > 512 && cols <= 1024) return cols <= 640 ? ROWS(32, 5, 4, 1) : cols <= 768 ? ROWS(32, 6, 5, 1) : ROWS(32, 8, 6, 1);
+    unsigned lanes = 8;
+    while (lanes * each < cols) lanes *= 2;
+    const unsigned v = (unsigned)((cols + lanes - 1) / lanes + 3) / 4;
+    if (v > 4) return lanes == 128 ? (v > 6 ? ROWS(128, 8, 6, 1) : ROWS(128, 6, 4, 1)) : (v > 6 ? ROWS(256, 8, 6, 1) : ROWS(256, 6, 4, 1));
+    if (v == 1) LANES_OF(1)
+    if (v == 2) LANES_OF(2)
+    if (v == 3) LANES_OF(3)
+    LANES_OF(4)
+  }
+  // Longer ones: a large CTA, clusters of CTAs where the row is beyond one or, as single floats, beyond its registers, and smaller shares in
+  // larger clusters where there are few rows (1 x 32768: 4.3 us, one CTA 6.7).
+  if (rows * 8 <= 2 * sms && cols <= 32768) return ROWS(512, 2, 0, 8);
+  if (!vectors && cols <= 65536) return cols <= 16384 ? ROWS(512, 4, 2, 2) : cols <= 32768 ? ROWS(512, 4, 2, 4) : ROWS(512, 4, 2, 8);
+  if (cols <= 16384) return ROWS(512, 8, 4, 1);
+  if (cols <= 32768) return ROWS(1024, 8, 4, 1);
+  if (cols <= 65536) return ROWS(1024, 8, 4, 2);
+#undef LANES_OF
+#undef ROWS
   return launch("flayernorm", norm_kernel, dim3((unsigned)rows), kThreads, 0, as_stream(stream), in, gamma, beta, eps, cols, out, mean,
                 rstd);
 }
