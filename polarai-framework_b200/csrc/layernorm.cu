@@ -4,6 +4,7 @@
 // written), and a dozen operations each.  Deviations are summed around the mean, never as the difference of
 // two large sums, and all sums are taken over two levels (threads, then the CTA), so that their rounding stays near that of a few dozen
 // additions whatever the row's length.
+#include <cstdlib>
 #include "rows.cuh"
 
 namespace polar_b200 {
@@ -188,6 +189,142 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const float* in, const f
   }
 }
 
+// ---- backward ---------------------------------------------------------------------------------------
+// One pass over the rows: a team walks over rows (its CTA or cluster, over every gridDim.x-th group of them), the weights' gradients of its
+// columns in registers.  The rows come through a ring in shared memory, STAGES - 1 of them on their way while one is computed, by asynchronous
+// copies that each thread makes and waits for by itself: what it copies is what it reads, so no barrier is needed but the one of the row's sums.
+// The sums over the team's rows go to `partials` [CTAs or clusters][2][cols], which a second kernel adds in order.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const float* from, bool on) {   // (zeros where not `on`)
+  const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to), bytes = on ? BYTES : 0;
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+template <int LANES>
+constexpr int kBlockOf = LANES > 32 ? LANES : kThreads;  // threads of a CTA
+template <int LANES, int V, bool VECTOR, int CTAS, int STAGES>
+__global__ void __launch_bounds__(kBlockOf<LANES>, 512 / kBlockOf<LANES>) norm_grad_rows_kernel(
+    const float* gradient, const float* in, const float* gamma, const float* mean, const float* rstd, uint32_t rows, uint32_t cols, float per_col,
+    float* din, float* partials) {
+  constexpr int kBlock = kBlockOf<LANES>, kGroups = kBlock / LANES, N = 4 * V, kTeam = LANES * CTAS;
+  using S = Share<kTeam, V, VECTOR, 0>;
+  extern __shared__ float4 ring4[];                        // [STAGES][gradient, in][N][kBlock], in vectors [..][V][kBlock]
+  __shared__ float slots[2][2 * kBlock / 32], part[2][2];
+  pdl_enter();
+  float* ring = reinterpret_cast<float*>(ring4);
+  const uint32_t tid = threadIdx.x, group = tid / LANES, member = blockIdx.y * LANES + tid % LANES, live = S::live(member, cols);
+  const uint32_t groups = (rows + kGroups - 1) / kGroups, trips = (groups - blockIdx.x + gridDim.x - 1) / gridDim.x;
+  auto row_of = [&](uint32_t trip) { return (uint64_t)(blockIdx.x + trip * gridDim.x) * kGroups + group; };
+  auto fetch = [&](uint32_t trip) {
+    if (trip < trips) {
+      const uint64_t r = row_of(trip);
+      const bool there = r < rows;
+      const uint64_t at = (there ? r : 0) * cols + (VECTOR ? 4 * member : member);
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        const float* src = (which ? in : gradient) + at;
+        if (VECTOR) {
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            copy_async<16>(ring4 + ((trip % STAGES * 2 + which) * V + i) * kBlock + tid, there && i < (int)live ? src + 4 * kTeam * i : gradient,
+                           there && i < (int)live);
+        } else {
+#pragma unroll
+          for (int k = 0; k < N; ++k)
+            copy_async<4>(ring + ((trip % STAGES * 2 + which) * N + k) * kBlock + tid, there && k < (int)live ? src + kTeam * k : gradient,
+                          there && k < (int)live);
+        }
+      }
+    }
+    copies_end();                                          // (an empty group as well: the count of groups is the count of trips)
+  };
+  auto stage = [&](float (&v)[N], uint32_t trip, int which) {
+    if (VECTOR) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        *reinterpret_cast<float4*>(v + 4 * i) = ring4[((trip % STAGES * 2 + which) * V + i) * kBlock + tid];
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[k] = ring[((trip % STAGES * 2 + which) * N + k) * kBlock + tid];
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) fetch(s);
+  float g[N], dgamma[N], dbeta[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) g[k] = 1.f, dgamma[k] = dbeta[k] = 0.f;
+  if (gamma) S::load(g, gamma, member, live);
+  uint64_t r = row_of(0);
+  float m = r < rows ? mean[r] : 0.f, s = r < rows ? rstd[r] : 0.f;
+  for (uint32_t trip = 0; trip < trips; ++trip) {
+    copies_wait<STAGES - 2>();
+    float dy[N], h[N];
+    stage(dy, trip, 0);
+    stage(h, trip, 1);
+    fetch(trip + STAGES - 1);                              // (into the stage of the trip before, which this thread has read)
+    const uint64_t next = row_of(trip + 1);
+    const bool more = trip + 1 < trips && next < rows;
+    const float next_m = more ? mean[next] : 0.f, next_s = more ? rstd[next] : 0.f;
+    float sums[2] = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      h[k] = (h[k] - m) * s;
+      dgamma[k] += dy[k] * h[k];
+      dbeta[k] += dy[k];
+      dy[k] *= g[k];
+      sums[0] += dy[k];
+      sums[1] += dy[k] * h[k];
+    }
+    team_sums<LANES>(sums, slots[trip & 1]);               // (a barrier lies between the reads of one trip and the writes of the next but one)
+    if (CTAS > 1) {
+      float* mine = part[trip & 1];
+      if (tid == 0) mine[0] = sums[0], mine[1] = sums[1];
+      cluster_arrive();
+      cluster_wait();
+      float p[2][CTAS];
+#pragma unroll
+      for (int c = 0; c < CTAS; ++c) p[0][c] = ld_cluster(mine, (uint32_t)c), p[1][c] = ld_cluster(mine + 1, (uint32_t)c);
+      sums[0] = sums[1] = 0.f;
+#pragma unroll
+      for (int c = 0; c < CTAS; ++c) sums[0] += p[0][c], sums[1] += p[1][c];
+    }
+    const float a = sums[0] * per_col, b = sums[1] * per_col;
+#pragma unroll
+    for (int k = 0; k < N; ++k) dy[k] = s * (dy[k] - a - h[k] * b);
+    if (r < rows) S::store(dy, din + r * cols, member, live);
+    r = next, m = next_m, s = next_s;
+  }
+  if (partials) {
+    float* to = partials + 2ull * blockIdx.x * cols;
+    if (kGroups == 1) {
+      S::store(dgamma, to, member, live);
+      S::store(dbeta, to + cols, member, live);
+    } else {                                               // the groups' sums meet in the ring: [groups][columns]
+      copies_wait<0>();
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < N; ++k) ring[group * (LANES * N) + (VECTOR ? 4 * (member + LANES * (k / 4)) + k % 4 : member + LANES * k)] = which ? dbeta[k] : dgamma[k];
+        __syncthreads();
+        for (uint32_t c = tid; c < cols; c += kBlock) {
+          float sum = 0.f;
+          for (int q = 0; q < kGroups; ++q) sum += ring[q * (LANES * N) + c];
+          to[(uint64_t)which * cols + c] = sum;
+        }
+      }
+    }
+  }
+  if (CTAS > 1) {                                          // nobody leaves while its part may still be read
+    cluster_arrive();
+    cluster_wait();
+  }
+}
+
 // Backward, rows of any length: the gradient at the input.
 __global__ void __launch_bounds__(kThreads) norm_grad_in_kernel(const float* gradient, const float* in, const float* gamma,
                                                                 const float* mean, const float* rstd, uint64_t cols, float* din) {
@@ -227,25 +364,67 @@ __global__ void __launch_bounds__(kThreads) norm_grad_columns_kernel(const float
   partials[(2ull * blockIdx.y + 1) * cols + c] = db;
 }
 
-// The partial sums of `parts` stretches of rows, in their order.
-__global__ void __launch_bounds__(kThreads) norm_grad_finish_kernel(const float* partials, uint32_t parts, uint64_t cols, float* dgamma,
-                                                                    float* dbeta) {
+// The partial sums of `parts` stretches of rows: a warp per stretch of 32 columns and every 32nd part, then the warps' sums by columns.
+constexpr int kFinishThreads = 1024;
+__global__ void __launch_bounds__(kFinishThreads) norm_grad_finish_kernel(const float* partials, uint32_t parts, uint64_t cols, float* dgamma,
+                                                                          float* dbeta) {
+  __shared__ float tile[32][33];
   pdl_enter();
-  const uint64_t c = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (c >= cols) return;
   float* out = blockIdx.y ? dbeta : dgamma;
   if (!out) return;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint64_t c = (uint64_t)blockIdx.x * 32 + lane;
   float s = 0.f;
-  for (uint32_t p = 0; p < parts; ++p) s += partials[(2ull * p + blockIdx.y) * cols + c];
-  out[c] = s;
+  if (c < cols)
+    for (uint32_t p = warp; p < parts; p += 32) s += partials[(2ull * p + blockIdx.y) * cols + c];
+  tile[warp][lane] = s;
+  __syncthreads();
+  s = warp_sum(tile[lane][warp]);
+  if (lane == 0 && (uint64_t)blockIdx.x * 32 + warp < cols) out[(uint64_t)blockIdx.x * 32 + warp] = s;
 }
 
 constexpr uint64_t kMaxCols = 1ull << 31, kMaxRows = 0x7fffffffull;
 
-// Stretches of rows whose sums over the rows are kept apart.
+// Stretches of rows whose sums are kept apart, for rows beyond the one-pass kernel.
 uint64_t stretches(uint64_t rows) {
   const uint64_t n = (rows + 63) / 64;
   return n < 256 ? n : 256;
+}
+
+// How the one-pass kernel runs a shape: lanes and CTAs of a team (lanes 0: not at all), fours per thread, and CTAs or clusters in all.
+constexpr int kStages = 3;
+constexpr uint64_t kOnePassCols = 65536;
+struct GradPlan {
+  unsigned lanes, v, ctas, grid;
+};
+GradPlan grad_plan(uint64_t rows, uint64_t cols) {
+  if (cols > kOnePassCols) return GradPlan{0, 0, 0, 0};
+  GradPlan p{8, 4, 1, 0};
+  if (cols <= 32) p.v = 1;
+  else if (cols <= 64) p.v = 2;
+  while ((uint64_t)p.lanes * p.v * 4 < cols && p.lanes < 512) p.lanes *= 2;
+  while ((uint64_t)p.lanes * p.v * 4 * p.ctas < cols) p.ctas *= 2;
+  // 512 threads on an SM, with three stages of up to 64 KB; each CTA some rows, so that the partial sums are few beside them
+  const uint64_t sms = (uint64_t)sm_count(), block = p.lanes > 32 ? p.lanes : kThreads, groups = (rows * p.lanes + block - 1) / block;
+  uint64_t most = sms * (512 / block) / p.ctas;
+  if (p.ctas >= 4) most = most * 7 / 8;                    // (larger clusters leave SMs of a GPC unused)
+  static const int MR = getenv("MR") ? atoi(getenv("MR")) : 8;
+  const uint64_t wanted = (groups + MR - 1) / MR;
+  p.grid = (unsigned)(wanted < most ? wanted : most);
+  return p;
+}
+
+template <int LANES, int V, bool VECTOR, int CTAS>
+int launch_grad_rows(const GradPlan& p, cudaStream_t st, const float* gradient, const float* in, const float* gamma, const float* mean,
+                     const float* rstd, uint64_t rows, uint64_t cols, float* din, float* partials) {
+  constexpr auto kernel = norm_grad_rows_kernel<LANES, V, VECTOR, CTAS, kStages>;
+  constexpr size_t bytes = (size_t)kStages * 2 * 4 * V * kBlockOf<LANES> * sizeof(float);
+  if (bytes > 48 * 1024 - 1024) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != cudaSuccess) return fail(POLAR_B200_ERR_CUDA, "cudaFuncSetAttribute(flayernorm_grad)", e);
+  }
+  return launch_clusters("flayernorm_grad", kernel, dim3(p.grid, CTAS), kBlockOf<LANES>, bytes, st, CTAS, gradient, in, gamma, mean, rstd, (uint32_t)rows,
+                         (uint32_t)cols, (float)(1.0 / (double)cols), din, partials);
 }
 
 }  // namespace
@@ -315,7 +494,8 @@ int polar_b200_flayernorm(const float* in, const float* gamma, const float* beta
 
 uint64_t polar_b200_flayernorm_grad_workspace_bytes(uint64_t rows, uint64_t cols) {
   if (rows == 0 || cols == 0 || rows > kMaxRows || cols > kMaxCols) return 0;
-  return stretches(rows) * 2 * cols * sizeof(float);
+  const GradPlan p = grad_plan(rows, cols);
+  return (p.lanes ? p.grid : stretches(rows)) * 2 * cols * sizeof(float);
 }
 
 int polar_b200_flayernorm_grad(const float* gradient, const float* in, const float* gamma, const float* mean, const float* rstd,
@@ -333,30 +513,51 @@ int polar_b200_flayernorm_grad(const float* gradient, const float* in, const flo
   LaunchDeviceScope on(stream, din);
   cudaStream_t st = as_stream(stream);
   int rc = POLAR_B200_OK;
+  const GradPlan plan = grad_plan(rows, cols);
+  const uint64_t need = polar_b200_flayernorm_grad_workspace_bytes(rows, cols);
+  void* own = nullptr;
+  float* partials = nullptr;
   if (dgamma || dbeta) {
-    const uint64_t need = polar_b200_flayernorm_grad_workspace_bytes(rows, cols);
     if (workspace && (workspace_bytes < need || !aligned16(workspace)))
       return fail(POLAR_B200_ERR_WORKSPACE, "workspace too small or not 16-byte aligned");
-    void* own = nullptr;
     if (!workspace) {
       cudaError_t e = scratch_alloc(&own, need, st);
       if (e != cudaSuccess) return fail(POLAR_B200_ERR_CUDA, "scratch (sums over rows)", e);
     }
-    float* partials = static_cast<float*>(workspace ? workspace : own);
-    const uint64_t parts = stretches(rows), stretch = (rows + parts - 1) / parts;
-    const unsigned wide = (unsigned)((cols + kThreads - 1) / kThreads);
-    rc = launch("flayernorm_grad_columns", norm_grad_columns_kernel, dim3(wide, (unsigned)parts), kThreads, 0, st, gradient, in, mean, rstd,
-                rows, cols, stretch, partials);
-    if (rc == POLAR_B200_OK)
-      rc = launch("flayernorm_grad_sum", norm_grad_finish_kernel, dim3(wide, 2), kThreads, 0, st, partials, (uint32_t)parts, cols, dgamma,
-                  dbeta);
-    if (own) {
-      cudaError_t e = scratch_free(own, st);
-      if (rc == POLAR_B200_OK && e != cudaSuccess) rc = fail(POLAR_B200_ERR_CUDA, "returning scratch", e);
-    }
-    if (rc) return rc;
+    partials = static_cast<float*>(workspace ? workspace : own);
   }
-  return launch("flayernorm_grad", norm_grad_in_kernel, dim3((unsigned)rows), kThreads, 0, st, gradient, in, gamma, mean, rstd, cols, din);
+  uint32_t parts = plan.grid;
+  if (plan.lanes) {
+    const bool vectors = (cols & 3) == 0 && aligned16(gradient) && aligned16(in) && aligned16(gamma) && aligned16(din);
+    auto go = [&](auto with, auto without) {
+      return (vectors ? with : without)(plan, st, gradient, in, gamma, mean, rstd, rows, cols, din, partials);
+    };
+#define ROWS(LANES, V, CTAS) go(launch_grad_rows<LANES, V, true, CTAS>, launch_grad_rows<LANES, V, false, CTAS>)
+    switch (plan.lanes) {
+      case 8: rc = plan.v == 1 ? ROWS(8, 1, 1) : plan.v == 2 ? ROWS(8, 2, 1) : ROWS(8, 4, 1); break;
+      case 16: rc = ROWS(16, 4, 1); break;
+      case 32: rc = ROWS(32, 4, 1); break;
+      case 64: rc = ROWS(64, 4, 1); break;
+      case 128: rc = ROWS(128, 4, 1); break;
+      case 256: rc = ROWS(256, 4, 1); break;
+      default: rc = plan.ctas == 1 ? ROWS(512, 4, 1) : plan.ctas == 2 ? ROWS(512, 4, 2) : plan.ctas == 4 ? ROWS(512, 4, 4) : ROWS(512, 4, 8);
+    }
+#undef ROWS
+  } else if (partials) {
+    parts = (uint32_t)stretches(rows);
+    rc = launch("flayernorm_grad_columns", norm_grad_columns_kernel, dim3((unsigned)((cols + kThreads - 1) / kThreads), parts), kThreads, 0, st,
+                gradient, in, mean, rstd, rows, cols, (rows + parts - 1) / parts, partials);
+  }
+  if (rc == POLAR_B200_OK && partials)
+    rc = launch("flayernorm_grad_sum", norm_grad_finish_kernel, dim3((unsigned)((cols + 31) / 32), 2), kFinishThreads, 0, st, partials, parts, cols,
+                dgamma, dbeta);
+  if (rc == POLAR_B200_OK && !plan.lanes)                  // (last: din may be gradient or in)
+    rc = launch("flayernorm_grad", norm_grad_in_kernel, dim3((unsigned)rows), kThreads, 0, st, gradient, in, gamma, mean, rstd, cols, din);
+  if (own) {
+    cudaError_t e = scratch_free(own, st);
+    if (rc == POLAR_B200_OK && e != cudaSuccess) rc = fail(POLAR_B200_ERR_CUDA, "returning scratch", e);
+  }
+  return rc;
 }
 
 }  // extern "C"
