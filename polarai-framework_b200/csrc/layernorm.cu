@@ -4,7 +4,6 @@
 // written), and a dozen operations each.  Deviations are summed around the mean, never as the difference of
 // two large sums, and all sums are taken over two levels (threads, then the CTA), so that their rounding stays near that of a few dozen
 // additions whatever the row's length.
-#include <cstdlib>
 #include "rows.cuh"
 
 namespace polar_b200 {
@@ -195,8 +194,8 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const float* in, const f
 // copies that each thread makes and waits for by itself: what it copies is what it reads, so no barrier is needed but the one of the row's sums.
 // The sums over the team's rows go to `partials` [CTAs or clusters][2][cols], which a second kernel adds in order.
 template <int BYTES>
-__device__ __forceinline__ void copy_async(void* to, const float* from, bool on) {   // (zeros where not `on`)
-  const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to), bytes = on ? BYTES : 0;
+__device__ __forceinline__ void copy_async(void* to, const float* from, uint32_t bytes) {   // (zeros behind `bytes`)
+  const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to);
   if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
   else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
 }
@@ -205,81 +204,142 @@ template <int LEFT>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
 template <int LANES>
-constexpr int kBlockOf = LANES > 32 ? LANES : kThreads;  // threads of a CTA
+constexpr int kBlockOf = LANES > kThreads ? LANES : kThreads;   // threads of a CTA
+// A barrier of a team and the sums over it, in every thread, where several teams share a CTA (`group`: the team's number; `slots`: 2 for each warp).
+template <int LANES>
+__device__ __forceinline__ void team_barrier(uint32_t group) {
+  if (LANES <= 32) __syncwarp();
+  else if (LANES >= kThreads) __syncthreads();
+  else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(LANES) : "memory");
+}
+template <int LANES>
+__device__ __forceinline__ void grad_sums(float (&v)[2], float* slots, uint32_t group) {
+  constexpr int kWarps = LANES / 32;
+#pragma unroll
+  for (int off = (LANES < 32 ? LANES : 32) / 2; off > 0; off >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], off), v[1] += __shfl_xor_sync(0xffffffffu, v[1], off);
+  if (LANES <= 32) return;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) slots[2 * warp] = v[0], slots[2 * warp + 1] = v[1];
+  team_barrier<LANES>(group);
+  const float* mine = slots + 2 * group * kWarps;
+  v[0] = lane < kWarps ? mine[2 * lane] : 0.f, v[1] = lane < kWarps ? mine[2 * lane + 1] : 0.f;
+#pragma unroll
+  for (int off = kWarps / 2; off > 0; off >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], off), v[1] += __shfl_xor_sync(0xffffffffu, v[1], off);
+  v[0] = __shfl_sync(0xffffffffu, v[0], 0), v[1] = __shfl_sync(0xffffffffu, v[1], 0);
+}
 template <int LANES, int V, bool VECTOR, int CTAS, int STAGES>
 __global__ void __launch_bounds__(kBlockOf<LANES>, 512 / kBlockOf<LANES>) norm_grad_rows_kernel(
     const float* gradient, const float* in, const float* gamma, const float* mean, const float* rstd, uint32_t rows, uint32_t cols, float per_col,
     float* din, float* partials) {
-  constexpr int kBlock = kBlockOf<LANES>, kGroups = kBlock / LANES, N = 4 * V, kTeam = LANES * CTAS;
-  using S = Share<kTeam, V, VECTOR, 0>;
-  extern __shared__ float4 ring4[];                        // [STAGES][gradient, in][N][kBlock], in vectors [..][V][kBlock]
+  constexpr int kBlock = kBlockOf<LANES>, kGroups = kBlock / LANES, N = 4 * V;
+  // (the plan doubles LANES only for rows beyond half of it, so half of the fours are full, except for a cluster's last CTA and the shortest rows)
+  constexpr int FULL = CTAS == 1 ? V / 2 : 0;
+  using S = Share<LANES, V, VECTOR, FULL>;
+  // VECTOR: [STAGES][gradient, in][V][kBlock] vectors, of which a thread copies and reads its own.  Else rows are copied as they lie, vectors from
+  // the boundary before their beginning on, and read as single floats by other threads than copied them: [STAGES][gradient, in][kGroups][kImage].
+  constexpr int kImage = LANES * N + 4;
+  extern __shared__ float4 ring4[];
   __shared__ float slots[2][2 * kBlock / 32], part[2][2];
   pdl_enter();
   float* ring = reinterpret_cast<float*>(ring4);
-  const uint32_t tid = threadIdx.x, group = tid / LANES, member = blockIdx.y * LANES + tid % LANES, live = S::live(member, cols);
+  const uint32_t tid = threadIdx.x, group = tid / LANES, member = tid % LANES;
+  // the CTA's part of the columns, and how many this thread has of it
+  const uint32_t from = blockIdx.y * (LANES * N), here = from < cols ? min(cols - from, (uint32_t)(LANES * N)) : 0, live = S::live(member, here);
   const uint32_t groups = (rows + kGroups - 1) / kGroups, trips = (groups - blockIdx.x + gridDim.x - 1) / gridDim.x;
-  auto row_of = [&](uint32_t trip) { return (uint64_t)(blockIdx.x + trip * gridDim.x) * kGroups + group; };
-  auto fetch = [&](uint32_t trip) {
-    if (trip < trips) {
-      const uint64_t r = row_of(trip);
-      const bool there = r < rows;
-      const uint64_t at = (there ? r : 0) * cols + (VECTOR ? 4 * member : member);
+  uint64_t r = (uint64_t)blockIdx.x * kGroups + group;
+  const uint64_t step = (uint64_t)gridDim.x * kGroups;
+  // where the fetches are: the row, its places, the stage
+  uint64_t fetched = r;
+  const float *src_g = gradient + r * cols + from, *src_x = in + r * cols + from;
+  uint32_t to_stage = 0;
+  auto past = [](const float* p) { return (uint32_t)(reinterpret_cast<uintptr_t>(p) >> 2) & 3; };
+  auto image = [&](uint32_t stage, int which) { return ring + ((stage * 2 + which) * kGroups + group) * kImage; };
+  auto fetch = [&] {
+    if (fetched < rows) {
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
-        const float* src = (which ? in : gradient) + at;
+        const float* src = which ? src_x : src_g;
         if (VECTOR) {
+          src += 4 * member;
 #pragma unroll
           for (int i = 0; i < V; ++i)
-            copy_async<16>(ring4 + ((trip % STAGES * 2 + which) * V + i) * kBlock + tid, there && i < (int)live ? src + 4 * kTeam * i : gradient,
-                           there && i < (int)live);
+            copy_async<16>(ring4 + ((to_stage * 2 + which) * V + i) * kBlock + tid, S::has(live, 4 * i) ? src + 4 * LANES * i : gradient,
+                           S::has(live, 4 * i) ? 16 : 0);
         } else {
+          const uint32_t shift = past(src);
+          float* to = image(to_stage, which);
 #pragma unroll
-          for (int k = 0; k < N; ++k)
-            copy_async<4>(ring + ((trip % STAGES * 2 + which) * N + k) * kBlock + tid, there && k < (int)live ? src + kTeam * k : gradient,
-                          there && k < (int)live);
+          for (int j = 0; j <= V; ++j) {                   // (a row that begins past a boundary has a vector more)
+            const uint32_t i = member + LANES * j;
+            const int left = 4 * (int)(shift + here) - 16 * (int)i;
+            if (left <= 0 || (j == V && member)) continue;
+            if (j == 0 && i == 0 && shift) {
+              for (uint32_t k = shift; k < 4 && k < shift + here; ++k) copy_async<4>(to + k, src + (k - shift), 4);
+            } else {
+              copy_async<16>(to + 4 * i, src + (int64_t)(4 * i) - shift, left < 16 ? left : 16);
+            }
+          }
         }
       }
     }
     copies_end();                                          // (an empty group as well: the count of groups is the count of trips)
+    fetched += step, src_g += step * cols, src_x += step * cols;
+    to_stage = to_stage + 1 == STAGES ? 0 : to_stage + 1;
   };
-  auto stage = [&](float (&v)[N], uint32_t trip, int which) {
-    if (VECTOR) {
+  auto read_stage = [&](float (&v)[N], uint32_t stage, int which) {
+    if (r >= rows) {                                       // no row: of a warp's last groups
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        *reinterpret_cast<float4*>(v + 4 * i) = ring4[((trip % STAGES * 2 + which) * V + i) * kBlock + tid];
+      for (int k = 0; k < N; ++k) v[k] = 0.f;
+    } else if (VECTOR) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) *reinterpret_cast<float4*>(v + 4 * i) = ring4[((stage * 2 + which) * V + i) * kBlock + tid];
     } else {
+      const float* p = image(stage, which) + past((which ? in : gradient) + r * cols + from) + member;
 #pragma unroll
-      for (int k = 0; k < N; ++k) v[k] = ring[((trip % STAGES * 2 + which) * N + k) * kBlock + tid];
+      for (int k = 0; k < N; ++k) v[k] = S::has(live, k) ? p[LANES * k] : 0.f;
     }
   };
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) fetch(s);
-  float g[N], dgamma[N], dbeta[N];
+  for (int s = 0; s < STAGES - 1; ++s) fetch();
+  float g[N];
 #pragma unroll
-  for (int k = 0; k < N; ++k) g[k] = 1.f, dgamma[k] = dbeta[k] = 0.f;
-  if (gamma) S::load(g, gamma, member, live);
-  uint64_t r = row_of(0);
+  for (int k = 0; k < N; ++k) g[k] = 1.f;
+  if (gamma) S::load(g, gamma + from, member, live);
+  Pair gamma2[N / 2], dgamma[N / 2], dbeta[N / 2];
+#pragma unroll
+  for (int k = 0; k < N / 2; ++k) gamma2[k] = pair(g[2 * k], g[2 * k + 1]), dgamma[k] = dbeta[k] = 0;
   float m = r < rows ? mean[r] : 0.f, s = r < rows ? rstd[r] : 0.f;
+  uint32_t stage = 0;
+  const Pair one = pair(1.f, 1.f);
   for (uint32_t trip = 0; trip < trips; ++trip) {
     copies_wait<STAGES - 2>();
-    float dy[N], h[N];
-    stage(dy, trip, 0);
-    stage(h, trip, 1);
-    fetch(trip + STAGES - 1);                              // (into the stage of the trip before, which this thread has read)
-    const uint64_t next = row_of(trip + 1);
-    const bool more = trip + 1 < trips && next < rows;
-    const float next_m = more ? mean[next] : 0.f, next_s = more ? rstd[next] : 0.f;
-    float sums[2] = {0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      h[k] = (h[k] - m) * s;
-      dgamma[k] += dy[k] * h[k];
-      dbeta[k] += dy[k];
-      dy[k] *= g[k];
-      sums[0] += dy[k];
-      sums[1] += dy[k] * h[k];
+    if (!VECTOR) {                                         // what other threads have copied, and their reads of the trip before
+      team_barrier<LANES>(group);
     }
-    team_sums<LANES>(sums, slots[trip & 1]);               // (a barrier lies between the reads of one trip and the writes of the next but one)
+    float v[N];
+    Pair dy[N / 2], h[N / 2];
+    read_stage(v, stage, 0);
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) dy[k] = pair(v[2 * k], v[2 * k + 1]);
+    read_stage(v, stage, 1);
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) h[k] = pair(v[2 * k], v[2 * k + 1]);
+    fetch();                                               // (into the stage of the trip before, which has been read)
+    const uint64_t next = r + step;
+    const float next_m = next < rows ? mean[next] : 0.f, next_s = next < rows ? rstd[next] : 0.f;
+    const Pair minus_m = pair(-m, -m), s2 = pair(s, s);
+    Pair sum_q = 0, sum_qh = 0;
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) {                      // (sums of pairs as 1 * a + b)
+      h[k] = mul2(fma2(one, h[k], minus_m), s2);
+      dgamma[k] = fma2(dy[k], h[k], dgamma[k]);
+      dbeta[k] = fma2(one, dy[k], dbeta[k]);
+      dy[k] = mul2(dy[k], gamma2[k]);
+      sum_q = fma2(one, dy[k], sum_q);
+      sum_qh = fma2(dy[k], h[k], sum_qh);
+    }
+    float sums[2] = {halves(sum_q).x + halves(sum_q).y, halves(sum_qh).x + halves(sum_qh).y};
+    grad_sums<LANES>(sums, slots[trip & 1], group);        // (a barrier lies between the reads of one trip and the writes of the next but one)
     if (CTAS > 1) {
       float* mine = part[trip & 1];
       if (tid == 0) mine[0] = sums[0], mine[1] = sums[1];
@@ -293,23 +353,35 @@ __global__ void __launch_bounds__(kBlockOf<LANES>, 512 / kBlockOf<LANES>) norm_g
       for (int c = 0; c < CTAS; ++c) sums[0] += p[0][c], sums[1] += p[1][c];
     }
     const float a = sums[0] * per_col, b = sums[1] * per_col;
+    const Pair minus_a = pair(-a, -a), minus_b = pair(-b, -b);
 #pragma unroll
-    for (int k = 0; k < N; ++k) dy[k] = s * (dy[k] - a - h[k] * b);
-    if (r < rows) S::store(dy, din + r * cols, member, live);
+    for (int k = 0; k < N / 2; ++k) {
+      const float2 d = halves(mul2(fma2(h[k], minus_b, fma2(one, dy[k], minus_a)), s2));
+      v[2 * k] = d.x, v[2 * k + 1] = d.y;
+    }
+    if (r < rows) S::store(v, din + r * cols + from, member, live);
     r = next, m = next_m, s = next_s;
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
   }
   if (partials) {
-    float* to = partials + 2ull * blockIdx.x * cols;
+    float* to = partials + 2ull * blockIdx.x * cols + from;
+    auto unpack = [&](const Pair (&p)[N / 2]) {
+#pragma unroll
+      for (int k = 0; k < N / 2; ++k) g[2 * k] = halves(p[k]).x, g[2 * k + 1] = halves(p[k]).y;
+    };
     if (kGroups == 1) {
-      S::store(dgamma, to, member, live);
-      S::store(dbeta, to + cols, member, live);
+      unpack(dgamma);
+      S::store(g, to, member, live);
+      unpack(dbeta);
+      S::store(g, to + cols, member, live);
     } else {                                               // the groups' sums meet in the ring: [groups][columns]
       copies_wait<0>();
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
+        unpack(which ? dbeta : dgamma);
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < N; ++k) ring[group * (LANES * N) + (VECTOR ? 4 * (member + LANES * (k / 4)) + k % 4 : member + LANES * k)] = which ? dbeta[k] : dgamma[k];
+        for (int k = 0; k < N; ++k) ring[group * (LANES * N) + (VECTOR ? 4 * (member + LANES * (k / 4)) + k % 4 : member + LANES * k)] = g[k];
         __syncthreads();
         for (uint32_t c = tid; c < cols; c += kBlock) {
           float sum = 0.f;
@@ -375,8 +447,12 @@ __global__ void __launch_bounds__(kFinishThreads) norm_grad_finish_kernel(const 
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint64_t c = (uint64_t)blockIdx.x * 32 + lane;
   float s = 0.f;
-  if (c < cols)
-    for (uint32_t p = warp; p < parts; p += 32) s += partials[(2ull * p + blockIdx.y) * cols + c];
+  if (c < cols) {
+    const float* q = partials + (2ull * warp + blockIdx.y) * cols + c;
+    const uint64_t step = 64 * cols;                       // two rows of sums for each of the CTA's warps
+#pragma unroll 8
+    for (uint32_t p = warp; p < parts; p += 32, q += step) s += *q;   // (eight loads on their way)
+  }
   tile[warp][lane] = s;
   __syncthreads();
   s = warp_sum(tile[lane][warp]);
@@ -403,13 +479,15 @@ GradPlan grad_plan(uint64_t rows, uint64_t cols) {
   if (cols <= 32) p.v = 1;
   else if (cols <= 64) p.v = 2;
   while ((uint64_t)p.lanes * p.v * 4 < cols && p.lanes < 512) p.lanes *= 2;
-  while ((uint64_t)p.lanes * p.v * 4 * p.ctas < cols) p.ctas *= 2;
+  if (cols > 8192) {
+    p.lanes = cols <= 32768 ? 256 : 512;
+    while ((uint64_t)p.lanes * p.v * 4 * p.ctas < cols) p.ctas *= 2;
+  }
   // 512 threads on an SM, with three stages of up to 64 KB; each CTA some rows, so that the partial sums are few beside them
-  const uint64_t sms = (uint64_t)sm_count(), block = p.lanes > 32 ? p.lanes : kThreads, groups = (rows * p.lanes + block - 1) / block;
+  const uint64_t sms = (uint64_t)sm_count(), block = p.lanes > kThreads ? p.lanes : kThreads, groups = (rows * p.lanes + block - 1) / block;
   uint64_t most = sms * (512 / block) / p.ctas;
   if (p.ctas >= 4) most = most * 7 / 8;                    // (larger clusters leave SMs of a GPC unused)
-  static const int MR = getenv("MR") ? atoi(getenv("MR")) : 8;
-  const uint64_t wanted = (groups + MR - 1) / MR;
+  const uint64_t wanted = (groups + 1) / 2;
   p.grid = (unsigned)(wanted < most ? wanted : most);
   return p;
 }
@@ -418,7 +496,7 @@ template <int LANES, int V, bool VECTOR, int CTAS>
 int launch_grad_rows(const GradPlan& p, cudaStream_t st, const float* gradient, const float* in, const float* gamma, const float* mean,
                      const float* rstd, uint64_t rows, uint64_t cols, float* din, float* partials) {
   constexpr auto kernel = norm_grad_rows_kernel<LANES, V, VECTOR, CTAS, kStages>;
-  constexpr size_t bytes = (size_t)kStages * 2 * 4 * V * kBlockOf<LANES> * sizeof(float);
+  constexpr size_t bytes = (size_t)kStages * 2 * (4 * V * LANES + (VECTOR ? 0 : 4)) * (kBlockOf<LANES> / LANES) * sizeof(float);
   if (bytes > 48 * 1024 - 1024) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (e != cudaSuccess) return fail(POLAR_B200_ERR_CUDA, "cudaFuncSetAttribute(flayernorm_grad)", e);
@@ -539,7 +617,7 @@ int polar_b200_flayernorm_grad(const float* gradient, const float* in, const flo
       case 32: rc = ROWS(32, 4, 1); break;
       case 64: rc = ROWS(64, 4, 1); break;
       case 128: rc = ROWS(128, 4, 1); break;
-      case 256: rc = ROWS(256, 4, 1); break;
+      case 256: rc = plan.ctas == 1 ? ROWS(256, 4, 1) : plan.ctas == 4 ? ROWS(256, 4, 4) : ROWS(256, 4, 8); break;
       default: rc = plan.ctas == 1 ? ROWS(512, 4, 1) : plan.ctas == 2 ? ROWS(512, 4, 2) : plan.ctas == 4 ? ROWS(512, 4, 4) : ROWS(512, 4, 8);
     }
 #undef ROWS
