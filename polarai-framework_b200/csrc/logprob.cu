@@ -186,6 +186,7 @@ struct Kept {
   unsigned long long* rank;
   uint32_t* count;                                         // goes on beyond the room
   uint32_t room;
+  bool all = false;                                        // everything, each element in its place, and no bound
 };
 
 // The running sums over the vectors first, first + stride, ... of a row, kInFlight of them on their way; `base` is the first of the warp's
@@ -228,11 +229,19 @@ __device__ __forceinline__ Running scan(const Row& row, uint32_t base, uint32_t 
     most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
     if (most > r.m) raise_to(r, most);
     if (TOP) {
-      if (n == next_bound) {
+      if (kept.all) {
+#pragma unroll
+        for (int u = 0; u < kInFlight; ++u) {
+          const float x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+          for (uint32_t c = 0; c < 4; ++c)
+            if (row.has(i + u * stride, c)) kept.rank[row.element(i + u * stride, c)] = rank_of(x[c], row.element(i + u * stride, c));
+        }
+      } else if (n == next_bound) {
         bound = find_bound(maxima, r.m);
         next_bound = 4 * n + 3;
       }
-      if (most >= bound && *(volatile uint32_t*)kept.count <= kept.room) {
+      if (!kept.all && most >= bound && *(volatile uint32_t*)kept.count <= kept.room) {
         uint32_t which = 0;                                // of the 16 elements, those that reach the bound
 #pragma unroll
         for (int u = 0; u < kInFlight; ++u)
@@ -427,20 +436,26 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_wide_kernel(c
   cluster_wait();
 }
 
-// A warp per row or, for short rows, LANES lanes.
+// A warp per row or, for short rows, LANES lanes; `per_warp` of the warp's teams have rows (one where there are few: then what the whole warp
+// does for a row has only that one to do).
 template <int LANES, bool TOP>
-__global__ void __launch_bounds__(kThreads) logprob_warp_kernel(const float* logits, uint32_t rows, uint32_t classes, uint64_t pitch, Results o) {
-  constexpr uint32_t kRoom = TOP ? 128 : 1, kTeams = kThreads / LANES, kRows = 32 / LANES;
+__global__ void __launch_bounds__(kThreads) logprob_warp_kernel(const float* logits, uint32_t rows, uint32_t classes, uint64_t pitch, uint32_t per_warp,
+                                                                Results o) {
+  // (room for all of a short row: where there are many alternatives, all are placed, without looking for a bound)
+  constexpr uint32_t kRoom = !TOP ? 1 : LANES == 32 ? 256 : 128, kTeams = kThreads / LANES;
+  const bool all_kept = TOP && LANES < 32 && (o.top > kFewTop || (classes <= 32 && per_warp == 1));
   __shared__ unsigned long long kept_ranks[kTeams][kRoom];
   __shared__ uint32_t n_kept[kTeams];
   pdl_enter();
   const uint32_t lane = threadIdx.x & 31, team = threadIdx.x / LANES, member = threadIdx.x % LANES;
-  const uint64_t r = (uint64_t)blockIdx.x * kTeams + team;
-  if (r - team % kRows >= rows) return;                    // (a whole warp)
-  const Row row(logits + (r < rows ? r : rows - 1) * pitch, classes);   // (lanes without a row of their own look at the last)
+  const uint64_t first = ((uint64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32) * per_warp;   // the warp's first row
+  if (first >= rows) return;
+  const uint64_t r = first + lane / LANES;
+  const bool live = lane / LANES < per_warp && r < rows;
+  const Row row(logits + (live ? r : first) * pitch, classes);   // (lanes without a row of their own look at the warp's first)
   int64_t id = kPadding;
   float given = 0.f;
-  if (member == 0 && o.logprob && r < rows) {
+  if (member == 0 && o.logprob && live) {
     id = read_id(o.ids, o.id_type, r, classes);
     if (id >= 0) given = logits[r * pitch + id];
   }
@@ -456,7 +471,7 @@ __global__ void __launch_bounds__(kThreads) logprob_warp_kernel(const float* log
   float maxima[kInFlight];
   // (rows that begin elsewhere on a boundary may have a vector more or less: as many chunks as the longest)
   const uint32_t chunks = ((classes + 6) / 4 + kInFlight * LANES - 1) / (kInFlight * LANES);
-  const Running own = scan<TOP>(row, 0, member, LANES, chunks, maxima, Kept{kept, &n_kept[team], kRoom}, find_bound);
+  const Running own = scan<TOP>(row, 0, member, LANES, chunks, maxima, Kept{kept, &n_kept[team], kRoom, all_kept}, find_bound);
   Running all = own;
   float m = own.m;
 #pragma unroll
@@ -467,63 +482,80 @@ __global__ void __launch_bounds__(kThreads) logprob_warp_kernel(const float* log
     all.s += __shfl_xor_sync(0xffffffffu, all.s, off);
     all.t += __shfl_xor_sync(0xffffffffu, all.t, off);
   }
-  if (member == 0 && r < rows) write_row(o, r, id, given, all);
+  if (member == 0 && live) write_row(o, r, id, given, all);
   if (!TOP) return;
   __syncwarp();
-  const uint32_t n = n_kept[team];
-  const bool sorts = n > kRoom || all.s != all.s;
-  uint32_t total = 0;
-  if (!sorts) {
+  const uint32_t n = !live ? o.top : all_kept ? classes : n_kept[team];
+  const bool sorts = live && !all_kept && (n > kRoom || all.s != all.s);
+  const bool simple = !sorts && n >= o.top && n <= (LANES == 32 ? 64 : per_warp > 1 ? 32 : 8) && !all_kept;
+  if (simple && live) {                                    // few: each team places its own, by counting what is above
     for (uint32_t i = member; i < n; i += LANES) {
       uint32_t above = 0;
       const unsigned long long mine = kept[i];
       for (uint32_t j = 0; j < n; ++j) above += kept[j] > mine;
-      if (above < o.top && r < rows) write_top(o, r, above, mine, all);
+      if (above < o.top) write_top(o, r, above, mine, all);
     }
-    total = n;
   }
-  // rows that the warp looks through again, one after the other
-  const uint32_t again = __ballot_sync(0xffffffffu, (sorts || total < o.top) && member == 0 && r < rows);
-  for (uint32_t left = again; left; left &= left - 1) {
-    const int who = __ffs(left) - 1;
-    const uint64_t q = r - team % kRows + who / LANES;
-    const Row its(logits + q * pitch, classes);
+  uint32_t others = __ballot_sync(0xffffffffu, live && !simple && member == 0);
+  if (others == 0) return;
+  // the other rows one after the other, by the whole warp
+  const float last_bound = all_kept ? 0.f : find_bound(maxima, own.m);
+  for (; others; others &= others - 1) {
+    const int who = __ffs(others) - 1;
+    const uint64_t q = first + who / LANES;
     Running sums;
-    sums.m = __shfl_sync(0xffffffffu, all.m, who), sums.s = __shfl_sync(0xffffffffu, all.s, who), sums.t = 0.f;
-    const uint32_t have = __shfl_sync(0xffffffffu, total, who);
+    sums.m = __shfl_sync(0xffffffffu, all.m, who), sums.s = __shfl_sync(0xffffffffu, all.s, who);
     if (__shfl_sync(0xffffffffu, (int)sorts, who)) {
+      const Row its(logits + q * pitch, classes);
       unsigned long long list = 0;
       for (uint32_t i = lane; i - lane < its.vectors; i += 32) take(list, its, i, o.top, lane);
       if (lane < o.top) write_top(o, q, lane, list, sums);
-    } else {
-      unsigned long long* to = kept_ranks[team - team % kRows + who / LANES];
-      __syncwarp();
-      take_shut_out(to, o.top - have, its, 0, 32, 32, lane);
-      __syncwarp();
-      if (lane + have < o.top) write_top(o, q, lane + have, to[lane], sums);
+      continue;
     }
+    unsigned long long* its_kept = kept_ranks[(threadIdx.x - lane + who) / LANES];
+    const uint32_t its_n = __shfl_sync(0xffffffffu, n, who);
+    const uint64_t least = (uint64_t)ordered(__shfl_sync(0xffffffffu, last_bound, who)) << 32;
+    uint32_t total = all_kept ? its_n : 0;                 // what reaches the bound of the whole row moves to the front
+    for (uint32_t i = 0; i < its_n && !all_kept; i += 32) {
+      const unsigned long long rank = i + lane < its_n ? its_kept[i + lane] : 0;
+      const uint32_t up = __ballot_sync(0xffffffffu, rank >= least && rank);
+      __syncwarp();
+      if (up >> lane & 1) its_kept[total + __popc(up & ((1u << lane) - 1))] = rank;   // (never behind what has been read)
+      total += __popc(up);
+      __syncwarp();
+    }
+    for (uint32_t i = lane; i < total; i += 64) {          // two of them against all, for each lane
+      uint32_t above_a = 0, above_b = 0;
+      const unsigned long long a = its_kept[i], b = i + 32 < total ? its_kept[i + 32] : 0;
+#pragma unroll 4
+      for (uint32_t j = 0; j < total; ++j) {
+        const unsigned long long other = its_kept[j];
+        above_a += other > a;
+        above_b += other > b;
+      }
+      if (above_a < o.top) write_top(o, q, above_a, a, sums);
+      if (above_b < o.top && b) write_top(o, q, above_b, b, sums);
+    }
+    if (total < o.top) {
+      const Row its(logits + q * pitch, classes);
+      __syncwarp();
+      take_shut_out(its_kept, o.top - total, its, 0, 32, 32, lane);
+      __syncwarp();
+      if (lane + total < o.top) write_top(o, q, lane + total, its_kept[lane], sums);
+    }
+    __syncwarp();
   }
 }
 
-// Up to kThreadClasses classes: a thread per row, its logits in registers.  STAGED: the rows come through shared memory, since 32 threads
-// that each read a float of a long row touch as many cache lines at a time (65536 x 32: 12.7 us, 7.6 staged; 65536 x 10: 2.8, 5.2 staged).
-constexpr uint32_t kThreadClasses = 32, kThreadRows = 128;
-template <int MOST, bool STAGED>
+// Up to kThreadClasses classes: a thread per row, its logits in registers (65536 x 10: 2.8 us; x 32, where 32 threads that each read a float of
+// their row touch as many cache lines at a time, 12.7, with eight lanes per row 7.5).
+constexpr uint32_t kThreadClasses = 16, kThreadRows = 128;
+template <int MOST>
 __global__ void __launch_bounds__(kThreadRows) logprob_thread_kernel(const float* logits, uint32_t rows, uint32_t classes, uint64_t pitch, Results o) {
-  __shared__ float tile[STAGED ? kThreadRows * (MOST | 1) : 1];
   pdl_enter();
-  const uint64_t r0 = (uint64_t)blockIdx.x * kThreadRows, r = r0 + threadIdx.x;
-  const float* x = logits + r * pitch;
-  if (STAGED) {
-    const uint32_t here = rows - r0 < kThreadRows ? (uint32_t)(rows - r0) : kThreadRows, wide = classes | 1;   // (odd: no two threads in a bank)
-    for (uint32_t e = threadIdx.x; e < here * classes; e += kThreadRows) {
-      const uint32_t q = e / classes, c = e - q * classes;
-      tile[q * wide + c] = logits[(r0 + q) * pitch + c];
-    }
-    x = tile + threadIdx.x * wide;
-    __syncthreads();
-  }
+  const uint64_t r = (uint64_t)blockIdx.x * kThreadRows + threadIdx.x;
   if (r >= rows) return;
+  const float* x = logits + r * pitch;
   float v[MOST];
 #pragma unroll
   for (int c = 0; c < MOST; ++c) v[c] = c < classes ? x[c] : -INFINITY;
@@ -704,16 +736,18 @@ int polar_b200_flogprob(const float* logits, uint64_t rows, uint64_t classes, ui
   if (classes <= kThreadClasses) {
     const dim3 grid((unsigned)((rows + kThreadRows - 1) / kThreadRows));
     auto go = [&](auto kernel) { return launch("flogprob", kernel, grid, kThreadRows, 0, st, logits, (uint32_t)rows, n, pitch, o); };
-    return classes <= 8 ? go(logprob_thread_kernel<8, false>) : classes <= 16 ? go(logprob_thread_kernel<16, false>) : go(logprob_thread_kernel<32, true>);
+    return classes <= 8 ? go(logprob_thread_kernel<8>) : go(logprob_thread_kernel<16>);
   }
   // A warp per row as long as there are rows enough for every SM (20000 x 8192: 95 us against 104 with a CTA of 128 threads per row, with five
   // alternatives 131 and 162; 300 x 8000 with five 18.6 and 8.4; up to 1024 classes always); eight lanes for the shortest (60000 x 100: 7.6 us
-  // against 20, with five alternatives 23 and 63).
+  // against 20, with five alternatives 23 and 63), four rows to a warp once every SM has its warps.
   const uint64_t sms = (uint64_t)sm_count();
   if (classes <= 1024 || (classes <= 8192 && rows >= 16 * sms)) {
     const uint32_t lanes = classes <= 128 ? 8 : 32;
-    const dim3 grid((unsigned)((rows * lanes + kThreads - 1) / kThreads));
-    auto go = [&](auto kernel) { return launch("flogprob", kernel, grid, kThreads, 0, st, logits, (uint32_t)rows, n, pitch, o); };
+    const uint32_t per_warp = lanes == 8 && rows > 48 * sms ? 4 : 1;
+    const uint64_t warps = (rows + per_warp - 1) / per_warp;
+    const dim3 grid((unsigned)((warps + kThreads / 32 - 1) / (kThreads / 32)));
+    auto go = [&](auto kernel) { return launch("flogprob", kernel, grid, kThreads, 0, st, logits, (uint32_t)rows, n, pitch, per_warp, o); };
     return lanes == 8 ? (top ? go(logprob_warp_kernel<8, true>) : go(logprob_warp_kernel<8, false>))
                       : (top ? go(logprob_warp_kernel<32, true>) : go(logprob_warp_kernel<32, false>));
   }
