@@ -3,6 +3,8 @@ TEST INFRASTRUCTURE ONLY: used by the tests, the smoke check and the bench's
 CPU-baseline legs to execute the identical builtin sequence on host cores."""
 import numpy as np
 
+from . import rows_oracle
+
 
 class OracleExecutor:
     def __init__(self, program, impl, allreduce=None):
@@ -60,6 +62,24 @@ class OracleExecutor:
                 one = o.ffill(1.0, t[h].size)
                 r = o.fmul(r.ravel(), o.fmul(o.fadd(one, 1.0, t[h].ravel(), -1.0), t[h].ravel()))
                 t[din] = np.asarray(r, np.float32).reshape(self.program.tensors[din])
+                continue
+            if kernel in ("flayernorm", "flayernorm_grad", "flogprob", "flogprob_grad", "fadamw"):
+                # several results, the last arguments; what the oracle gives besides (alternatives) is not asked for
+                a = [t[x] if isinstance(x, str) else x for x in args]
+                if kernel == "flayernorm":
+                    given, r = 4, rows_oracle.flayernorm(a[0], a[1], a[2], a[3])
+                elif kernel == "flayernorm_grad":
+                    given, r = 5, rows_oracle.flayernorm_grad(*a[:5])
+                elif kernel == "flogprob":
+                    given, r = 2, rows_oracle.flogprob(a[0], a[1].ravel())[:3]
+                elif kernel == "flogprob_grad":
+                    both = len(a) == 7
+                    given, r = len(a) - 1, [rows_oracle.flogprob_grad(a[0], a[1].ravel(), a[2].ravel(), a[3].ravel() if both else None,
+                                                               a[4 if both else 3].ravel(), a[5].ravel() if both else None)]
+                else:
+                    given, r = 6, rows_oracle.fadamw(a[6], a[0], a[7], a[8], float(a[1][0]), float(a[1][1]), *a[2:6])
+                for name, value in zip(args[given:], r):
+                    t[name] = np.asarray(value, np.float32).reshape(self.program.tensors[name])
                 continue
             out = args[-1]
             shape = self.program.tensors[out]

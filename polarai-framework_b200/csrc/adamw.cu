@@ -340,6 +340,23 @@ bool disjoint(const polar_b200_adamw_tensor* tensors, uint64_t count) {
 
 }  // namespace
 
+// Whether the steps may run in any order or at once: no written array overlaps another, a gradient or the schedule.
+bool adamw_independent(const polar_b200_adamw_tensor* tensors, uint64_t count, const float* schedule) {
+  if (!disjoint(tensors, count)) return false;
+  auto written = [&](const void* p, uint64_t bytes) {
+    const uintptr_t from = reinterpret_cast<uintptr_t>(p), to = from + bytes;
+    for (uint64_t i = 0; i < count; ++i)
+      for (int kind = 0; kind < 5; ++kind) {
+        const Span s = span_of(tensors[i], kind);
+        if (s.first != s.second && from < s.second && s.first < to) return true;
+      }
+    return false;
+  };
+  for (uint64_t i = 0; i < count; ++i)
+    if (written(tensors[i].gradient, 4 * tensors[i].count)) return false;
+  return !written(schedule, 8);
+}
+
 // The argument list of the builtin "fadamw" or "fadamw8" as the entry point takes it; false where it is none.
 bool adamw_arguments(const char* name, const polar_b200_arg* a, uint64_t argc, polar_b200_adamw_tensor* t, polar_b200_adamw_options* o) {
   const bool eight = !std::strcmp(name, "fadamw8");

@@ -10,6 +10,7 @@
 //    result is still written, with the bits its own launch gives; what goes away is reading a
 //    tensor back that the same pass has just computed or read (the four-builtin chain of
 //    (a + b) * c / d -> sigmoid moves 32 instead of 44 bytes per element).
+//  - Weight updates (fadamw, fadamw8) in a row are one launch for all their tensors.
 //  - From its third run on, a program of many short launches is replayed as a CUDA graph: one host call instead of 2 us
 //    of host time per launch.  Programs of up to three steps, and programs with tensors of two million elements or
 //    more, whose kernels outlast their launches, stay with launches: programmatic dependent launch overlaps them more
@@ -32,6 +33,9 @@ namespace polar_b200 {
 // dispatch.cu: while a thread captures a program, its forks take this stream set instead of the device's
 // shared one, which other threads may be using at the same time.
 bool use_capture_side_stream(bool on);
+// adamw.cu: the arguments of the builtins "fadamw" and "fadamw8"; whether steps share no memory that one of them writes.
+bool adamw_arguments(const char* name, const polar_b200_arg* a, uint64_t argc, polar_b200_adamw_tensor* t, polar_b200_adamw_options* o);
+bool adamw_independent(const polar_b200_adamw_tensor* tensors, uint64_t count, const float* schedule);
 
 namespace {
 
@@ -147,7 +151,9 @@ struct Op {                    // one builtin, its argument list owned by the pr
   std::vector<polar_b200_arg> args;
   std::vector<std::vector<uint64_t>> shapes;
 };
-struct Step {                  // one builtin, a chain, or two chains
+struct Step {                  // one builtin, a chain, two chains, or weight updates
+  std::vector<polar_b200_adamw_tensor> updates;
+  polar_b200_adamw_options options = {};
   int op = -1;
   ChainParams chain = {}, second = {};   // (one elementwise builtin is a chain of one, for pairing)
   size_t smem = 0;
@@ -345,7 +351,26 @@ void plan(Program* p) {
     }
     p->steps.push_back(s);
   };
+  // A weight update joins those right before it that have the same betas and schedule, where none touches what another writes.
+  auto update = [&](const Op& op) {
+    Step s;
+    s.updates.resize(1);
+    if (!adamw_arguments(op.name.c_str(), op.args.data(), op.args.size(), s.updates.data(), &s.options)) return false;
+    flush();
+    if (!p->steps.empty() && !p->steps.back().updates.empty()) {
+      Step& last = p->steps.back();
+      const polar_b200_adamw_options &a = last.options, &b = s.options;
+      if (a.beta1 == b.beta1 && a.beta2 == b.beta2 && a.eps == b.eps && a.schedule == b.schedule) {
+        last.updates.push_back(s.updates[0]);
+        if (adamw_independent(last.updates.data(), last.updates.size(), a.schedule)) return true;
+        last.updates.pop_back();
+      }
+    }
+    p->steps.push_back(std::move(s));
+    return true;
+  };
   for (size_t i = 0; i < p->ops.size(); ++i) {
+    if (update(p->ops[i])) continue;
     Elementwise e;
     const bool ok = elementwise(p->ops[i], &e);
     if (!ok || !chain.add(e)) {
@@ -365,7 +390,9 @@ void plan(Program* p) {
 int run_steps(Program* p, cudaStream_t stream) {
   for (const Step& s : p->steps) {
     int rc;
-    if (s.op >= 0) {
+    if (!s.updates.empty()) {
+      rc = polar_b200_fadamw(s.updates.data(), s.updates.size(), &s.options, stream);
+    } else if (s.op >= 0) {
       const Op& op = p->ops[s.op];
       rc = polar_b200_launch_by_name(op.name.c_str(), op.args.data(), op.args.size(), p->workspace, p->workspace_bytes, stream);
     } else {

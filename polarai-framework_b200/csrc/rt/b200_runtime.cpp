@@ -448,17 +448,17 @@ auto B200Device::launch(BackendAllocator& allocator, LaunchCommand& cmd, Event* 
     if (be->getDevice() != this && be->native())
       note("cudaStreamWaitEvent", cudaStreamWaitEvent(s, be->native(), 0));
   }
-  constexpr uint64_t kMaxArgs = 8;
+  constexpr uint64_t kMaxArgs = 16;
   polar_b200_arg args[kMaxArgs];
   const char* name = cmd.nativeKernelName ? cmd.nativeKernelName : "";
   if (cmd.argsCount > kMaxArgs || (cmd.argsCount && !cmd.args)) {
     status = POLAR_B200_ERR_UNSUPPORTED;
     mLastError = "launch: bad argument list";
   }
-  // the builtin writes its LAST tensor argument (its last two, for the one builtin with two results)
-  MemoryRecord results[2] = {{0, 0}, {0, 0}};
+  // the builtin writes its LAST tensor argument (its last few, for the builtins with several results)
+  MemoryRecord tensors[kMaxArgs];
   int n_seen = 0;
-  const int n_results = polar_b200_result_count(name) > 1 ? 2 : 1;
+  const int n_results = polar_b200_result_count(name);
   for (uint64_t i = 0; status == POLAR_B200_OK && i < cmd.argsCount; ++i) {
     const ArgDesc& a = cmd.args[i];
     if (a.type == ArgDesc::TENSOR) {
@@ -482,9 +482,7 @@ auto B200Device::launch(BackendAllocator& allocator, LaunchCommand& cmd, Event* 
         status = POLAR_B200_ERR_INVALID;
         mLastError = "launch: tensor is not allocated on this device";
       }
-      results[0] = results[1];
-      results[1] = rec;
-      ++n_seen;
+      tensors[n_seen++] = rec;
     } else {
       args[i].is_tensor = 0;
       args[i].tensor = polar_b200_tensor{nullptr, 0, nullptr};
@@ -525,7 +523,7 @@ auto B200Device::launch(BackendAllocator& allocator, LaunchCommand& cmd, Event* 
                  cmd.kernelName ? cmd.kernelName : "", mLastError.c_str());
     mLastStatus = status;
   } else {
-    for (int r = 0; r < n_results && r < n_seen; ++r) mAllocator->markWritten(results[1 - r]);
+    for (int r = 0; r < n_results && r < n_seen; ++r) mAllocator->markWritten(tensors[n_seen - 1 - r]);
     if (verbose()) std::fprintf(stderr, "[polar_rt_cuda] %s: launched %s\n", mName.c_str(), name);
   }
   cudaEvent_t evt = CudaApi::takeEvent(mOrdinal);

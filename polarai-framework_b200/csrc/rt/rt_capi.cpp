@@ -173,7 +173,7 @@ int polar_b200_rt_launch(polar_b200_rt* rt, int device, struct LaunchCommand* cm
   B200Device* d = dev(rt, device);
   if (!d || !cmd) return fail(rt, POLAR_B200_ERR_INVALID, "no such device or null command");
   // Locks as the operations' gen() methods take them: the result (last tensor argument; the
-  // last two for the one builtin with two results) READ_WRITE, every other tensor READ.
+  // last few for the builtins with several results) READ_WRITE, every other tensor READ.
   std::vector<uint64_t> tensors;
   for (uint64_t i = 0; i < cmd->argsCount; ++i)
     if (cmd->args[i].type == ArgDesc::TENSOR) tensors.push_back(i);

@@ -412,6 +412,36 @@ class HostBuiltins:
         a = self._up(a)
         return self._down(self.d.fslice(a, index, torch.empty(tuple(a.shape[1:]), device=self.dev)))
 
+    def flayernorm(self, x, gamma, beta, eps):
+        x, gamma, beta = self._up(x), self._up(gamma), self._up(beta)
+        mean, rstd = (torch.empty(x.shape[:-1], device=self.dev) for _ in range(2))
+        out = self.d.flayernorm(x, gamma, beta, eps, torch.empty_like(x), mean, rstd)
+        return tuple(self._down(t) for t in (out, mean, rstd))
+
+    def flayernorm_grad(self, gradient, x, gamma, mean, rstd):
+        g, x, gamma, mean, rstd = (self._up(t) for t in (gradient, x, gamma, mean, rstd))
+        dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(gamma)
+        dx = self.d.flayernorm_grad(g, x, gamma, mean, rstd, torch.empty_like(x), dgamma, dbeta)
+        return tuple(self._down(t) for t in (dx, dgamma, dbeta))
+
+    def flogprob(self, logits, ids, top=0):
+        x, ids = self._up(logits), torch.from_numpy(np.ascontiguousarray(ids, np.int64)).to(self.dev)
+        lp, entropy, lse = (torch.empty(len(ids), device=self.dev) for _ in range(3))
+        top_ids = torch.empty((len(ids), top), dtype=torch.int64, device=self.dev)
+        top_lp = torch.empty((len(ids), top), device=self.dev)
+        self.d.flogprob(x, ids, lp, entropy, lse, top_ids if top else None, top_lp if top else None)
+        return tuple(self._down(t) for t in (lp, entropy, lse, top_ids, top_lp))
+
+    def flogprob_grad(self, logits, ids, logsumexp, entropy, g_logprob, g_entropy):
+        x, ids = self._up(logits), torch.from_numpy(np.ascontiguousarray(ids, np.int64)).to(self.dev)
+        lse, h, g, gh = (None if t is None else self._up(t) for t in (logsumexp, entropy, g_logprob, g_entropy))
+        return self._down(self.d.flogprob_grad(x, ids, lse, h, g, gh, torch.empty_like(x)))
+
+    def fadamw(self, w, g, m, v, step, lr, beta1, beta2, eps, decay):
+        w, g, m, v = (self._up(t).clone() for t in (w, g, m, v))
+        self.d.fadamw([w], [g], [m], [v], step=step, lr=lr, beta1=beta1, beta2=beta2, eps=eps, weight_decay=decay)
+        return tuple(self._down(t) for t in (w, m, v))
+
     def fmatmul(self, tl, tr, left, right, which="auto", **kw):
         l, r = self._up(left), self._up(right)
         m, n, k = matmul_dims(tl, tr, l.shape, r.shape)

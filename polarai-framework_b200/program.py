@@ -53,6 +53,14 @@ class Program:
         return names
 
 
+_RESULTS = {"fdense_grad": 2, "flayernorm": 3, "flayernorm_grad": 3, "flogprob": 3, "flogprob_top": 5, "fadamw": 3, "fadamw8": 5}
+
+
+def results_of(kernel, args):
+    """The tensors that an op writes: its last arguments."""
+    return list(args[-_RESULTS.get(kernel, 1):])
+
+
 def exchange_pieces(args):
     """(weight, gradient, first row, rows) of every piece an ALLREDUCE_FADD_PART op exchanges;
     rows < 0 = the whole tensor.  args = [scale_w, scale_g, channel, overlapped, W, g, row0, rows, ...]."""
@@ -148,6 +156,69 @@ def mlp_program(batch, n_in=784, n_hidden=4096, n_out=10, lr=0.1):
     return p
 
 
+def adamw_moments(p, weight, state_bits=32):
+    """Declares the moments of a program's weight tensor and returns their names, in the order that fadamw (32 bits) or fadamw8 takes them;
+    all of them begin as zeros."""
+    n = 1
+    for s in p.tensors[weight]:
+        n *= s
+    if state_bits == 32:
+        return [p.tensor(f"{k}_{weight}", *p.tensors[weight]) for k in "mv"]
+    if state_bits != 8:
+        raise ValueError("moments are held in 32 or in 8 bits")
+    return [p.tensor(f"{k}_{weight}", s) for k, s in (("m", -(-n // 4)), ("ms", -(-n // 128)), ("v", -(-n // 4)), ("vs", -(-n // 128)))]
+
+
+def norm_classifier_program(batch, n_in=784, n_hidden=4096, n_classes=10, samples=None, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01,
+                            state_bits=32):
+    """A training step of a 2-layer classifier with a layer norm before the hidden activation, on `batch` rows (the rows that one rank holds of
+    `samples` in all): the loss is the mean of -log probability of the rows' labels, the update AdamW.
+
+    Inputs: X, labels (class numbers; below zero: a row that does not count), the weights W1, W2, gamma, beta, the moments m_*, v_*
+    (with 8 bits also ms_*, vs_*: zeros at the beginning) and schedule = [number of steps done, learning rate].  Decay is for the matrices."""
+    p = Program("norm_classifier_step")
+    p.tensor("X", batch, n_in), p.tensor("labels", batch), p.tensor("schedule", 2)
+    weights = {"W1": (n_in, n_hidden), "W2": (n_hidden, n_classes), "gamma": (n_hidden,), "beta": (n_hidden,)}
+    for w, s in weights.items():
+        p.tensor(w, *s), p.tensor("d" + w, *s)
+    moments = {w: adamw_moments(p, w, state_bits) for w in weights}
+    p.inputs = ["X", "labels", "schedule", *weights, *[m for ms in moments.values() for m in ms]]
+    p.tensor("ones_h", batch, n_hidden), p.tensor("g", batch), p.tensor("tick", 2)
+    p.constants = {"ones_h": 1.0, "g": -1.0 / (samples or batch)}
+    p.inputs.append("tick")                                  # [1, 0]: what a step adds to the schedule
+    for t in ("Z1", "N", "H", "dH", "omh", "sh", "dN", "dZ1"):
+        p.tensor(t, batch, n_hidden)
+    for t in ("mean", "rstd", "logp", "entropy", "lse"):
+        p.tensor(t, batch)
+    for t in ("Z2", "dZ2"):
+        p.tensor(t, batch, n_classes)
+    # forward
+    p.op("fmatmul_f_f", "X", "W1", "Z1")
+    p.op("flayernorm", "Z1", "gamma", "beta", 1e-5, "N", "mean", "rstd")
+    p.op("fsigmoid", "N", "H")
+    p.op("fmatmul_f_f", "H", "W2", "Z2")
+    p.op("flogprob", "Z2", "labels", "logp", "entropy", "lse")
+    # backward
+    p.op("flogprob_grad", "Z2", "labels", "lse", "g", "dZ2")
+    p.op("fmatmul_t_f", "H", "dZ2", "dW2")
+    p.op("ALLREDUCE", "dW2")
+    p.op("fmatmul_f_t", "dZ2", "W2", "dH")
+    p.op("fadd", "ones_h", 1.0, "H", -1.0, "omh")
+    p.op("fmul", "omh", "H", "sh")
+    p.op("fmul", "dH", "sh", "dN")
+    p.op("flayernorm_grad", "dN", "Z1", "gamma", "mean", "rstd", "dZ1", "dgamma", "dbeta")
+    p.op("ALLREDUCE", "dgamma")
+    p.op("ALLREDUCE", "dbeta")
+    p.op("fmatmul_t_f", "X", "dZ1", "dW1")
+    p.op("ALLREDUCE", "dW1")
+    # update
+    p.op("fadd", "schedule", 1.0, "tick", 1.0, "schedule")
+    for w in weights:
+        p.op("fadamw" if state_bits == 32 else "fadamw8", "d" + w, "schedule", beta1, beta2, eps, weight_decay if w[0] == "W" else 0.0, w, *moments[w])
+    p.outputs = ["logp", "entropy", *weights, *["d" + w for w in weights]]
+    return p
+
+
 def fuse_program(program):
     """Rewrites a program with the extended builtins, keeping every result bit-identical:
 
@@ -214,12 +285,14 @@ def fuse_program(program):
                     if kj == "ALLREDUCE":
                         continue
                     if z in aj[:-1] or aj[-1] == z:
+                        # the product moves to the other op: nothing between them may write its operands
+                        if any(w in a[:2] for o in ops[i + 1:j] if o[0] != "ALLREDUCE" for w in results_of(*o)):
+                            break
                         if kj == "fsigmoid" and aj[0] == z and dead_after(z, {i, j}):
                             ops[j] = (k + "_sigmoid", [a[0], a[1], aj[1]])
                             del ops[i]
                             changed = True
-                        elif (kj == "fsigmoid_grad" and aj[0] == z and aj[1] != z and dead_after(z, {i, j})
-                              and not any(o[1][-1] in (a[0], a[1]) for o in ops[i + 1:j] if o[0] != "ALLREDUCE")):
+                        elif kj == "fsigmoid_grad" and aj[0] == z and aj[1] != z and dead_after(z, {i, j}):
                             ops[j] = (k + "_sigmoid_grad", [a[0], a[1], aj[1], aj[2]])
                             del ops[i]
                             changed = True
@@ -444,6 +517,11 @@ class DeviceExecutor:
     def set_inputs(self, **arrays):
         for name, a in arrays.items():
             self.t[name].copy_(a if isinstance(a, torch.Tensor) else torch.from_numpy(a))
+
+    def set_zeros(self, *names):
+        """Inputs that begin as zeros, such as an optimizer's moments."""
+        for name in names:
+            self.t[name].zero_()
 
     def run(self):
         if self._only is not None:
