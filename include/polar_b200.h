@@ -428,9 +428,10 @@ int polar_b200_flogprob_grad(const float* logits, uint64_t rows, uint64_t classe
  *    a second moment above zero gets the least code at least (a zero there would leave eps alone as the
  *    divisor).  Zero bytes are the state before the first step.  A gradient that is not finite makes its block's
  *    moments NaN, where in 32 bits it makes NaN of its own element only.
- * No tensor may be named twice or overlap another (POLAR_B200_ERR_INVALID for weights and moments).  One launch for every few
- * hundred tensors of a kind.  `step` counts from 1.  With `schedule` (device memory, two floats: the number of the
- * step and lr) both are read on the device when the kernel runs, so that a captured or prepared step can be replayed.
+ * What is written - weights, moments, scales - may overlap nothing else that the call names (POLAR_B200_ERR_INVALID), but a
+ * tensor's weights may be its own gradient, and a gradient may serve several weights.  One launch for every few hundred tensors
+ * of a kind.  `step` counts from 1.  With `schedule` (device memory, two floats: the number of the step and lr) both are read on
+ * the device when the kernel runs, so that a captured or prepared step can be replayed.
  * As builtins, one tensor each: "fadamw" T gradient, T schedule[2], f32 beta1, f32 beta2, f32 eps, f32 weight_decay, T weights,
  * T first, T second (three results); "fadamw8" T gradient, T schedule[2], f32 beta1, f32 beta2, f32 eps, f32 weight_decay,
  * T weights, T first, T first_scales, T second, T second_scales (five results), with the codes of n weights in a tensor of

@@ -8,6 +8,7 @@
 #include <cmath>
 #include <cstring>
 #include <exception>
+#include <iterator>
 #include <utility>
 #include <vector>
 
@@ -294,19 +295,22 @@ int launch_table(const polar_b200_adamw_tensor* tensors, uint64_t count, bool ei
   else return launch_large("fadamw", adamw_kernel<N, 1>, dim3((unsigned)chunks), kThreads, stream, table);
 }
 
-// Whether no two of the arrays that a step writes share memory: two threads would race on it.  Usually each kind of array lies in
-// ascending order in memory of its own, which one walk sees; else the spans are sorted.
+// Whether no two of the arrays that a step writes share memory, nor one of them with a gradient: two threads would race on it.  (A tensor's
+// weights may be its own gradient: the thread that writes an element has read it.)  Usually each kind of array lies in ascending order in
+// memory of its own, which one walk sees; else the spans are sorted.
 using Span = std::pair<uintptr_t, uintptr_t>;
+constexpr int kWritten = 5;                                // kinds of arrays; the gradients come behind
 Span span_of(const polar_b200_adamw_tensor& t, int kind) {
-  const uint64_t bytes = kind == 0 ? 4 * t.count : kind <= 2 ? (t.first_scales ? t.count : 4 * t.count)
+  if (kind == kWritten && t.gradient == t.weights) return Span(0, 0);
+  const uint64_t bytes = kind == 0 || kind == kWritten ? 4 * t.count : kind <= 2 ? (t.first_scales ? t.count : 4 * t.count)
                          : t.first_scales ? (t.count + kBlock - 1) / kBlock * 4 : 0;
-  const void* p = kind == 0 ? t.weights : kind == 1 ? t.first : kind == 2 ? t.second : kind == 3 ? t.first_scales : t.second_scales;
+  const void* p = kind == 0 ? t.weights : kind == 1 ? t.first : kind == 2 ? t.second : kind == 3 ? t.first_scales : kind == 4 ? t.second_scales : t.gradient;
   return Span(reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes);
 }
 bool disjoint(const polar_b200_adamw_tensor* tensors, uint64_t count) {
   bool ascending = true;
-  Span range[5];
-  for (int kind = 0; kind < 5; ++kind) {
+  Span range[kWritten + 1];
+  for (int kind = 0; kind <= kWritten; ++kind) {
     Span& r = range[kind] = Span(0, 0);
     for (uint64_t i = 0; i < count; ++i) {
       const Span s = span_of(tensors[i], kind);
@@ -315,26 +319,31 @@ bool disjoint(const polar_b200_adamw_tensor* tensors, uint64_t count) {
         r = s;
         continue;
       }
-      ascending = ascending && s.first >= r.second;
-      r.second = std::max(r.second, s.second);
+      ascending = ascending && (s.first >= r.second || kind == kWritten);   // (gradients may lie as they like)
+      r = Span(std::min(r.first, s.first), std::max(r.second, s.second));
     }
   }
   if (ascending) {
     bool apart = true;
-    for (int a = 0; a < 5; ++a)
+    for (int a = 0; a <= kWritten; ++a)
       for (int b = 0; b < a; ++b) apart = apart && (range[a].first >= range[b].second || range[b].first >= range[a].second);
     if (apart) return true;
   }
   std::vector<Span> all;
-  all.reserve(5 * count);
+  all.reserve(kWritten * count);
   for (uint64_t i = 0; i < count; ++i)
-    for (int kind = 0; kind < 5; ++kind) {
+    for (int kind = 0; kind < kWritten; ++kind) {
       const Span s = span_of(tensors[i], kind);
       if (s.first != s.second) all.push_back(s);
     }
   std::sort(all.begin(), all.end());
   for (size_t i = 1; i < all.size(); ++i)
     if (all[i].first < all[i - 1].second) return false;
+  for (uint64_t i = 0; i < count; ++i) {
+    const Span s = span_of(tensors[i], kWritten);
+    const auto next = std::lower_bound(all.begin(), all.end(), Span(s.second, 0));   // the first one that begins behind the gradient
+    if (s.first != s.second && next != all.begin() && std::prev(next)->second > s.first) return false;
+  }
   return true;
 }
 
@@ -343,18 +352,14 @@ bool disjoint(const polar_b200_adamw_tensor* tensors, uint64_t count) {
 // Whether the steps may run in any order or at once: no written array overlaps another, a gradient or the schedule.
 bool adamw_independent(const polar_b200_adamw_tensor* tensors, uint64_t count, const float* schedule) {
   if (!disjoint(tensors, count)) return false;
-  auto written = [&](const void* p, uint64_t bytes) {
-    const uintptr_t from = reinterpret_cast<uintptr_t>(p), to = from + bytes;
-    for (uint64_t i = 0; i < count; ++i)
-      for (int kind = 0; kind < 5; ++kind) {
-        const Span s = span_of(tensors[i], kind);
-        if (s.first != s.second && from < s.second && s.first < to) return true;
-      }
-    return false;
-  };
+  if (!schedule) return true;
+  const uintptr_t from = reinterpret_cast<uintptr_t>(schedule);
   for (uint64_t i = 0; i < count; ++i)
-    if (written(tensors[i].gradient, 4 * tensors[i].count)) return false;
-  return !written(schedule, 8);
+    for (int kind = 0; kind < kWritten; ++kind) {
+      const Span s = span_of(tensors[i], kind);
+      if (s.first != s.second && from < s.second && s.first < from + 8) return false;
+    }
+  return true;
 }
 
 // The argument list of the builtin "fadamw" or "fadamw8" as the entry point takes it; false where it is none.
@@ -401,7 +406,7 @@ extern "C" int polar_b200_fadamw(const polar_b200_adamw_tensor* tensors, uint64_
     if (t.count > 1ull << 37) return fail(POLAR_B200_ERR_INVALID, "fadamw: tensor too large");
   }
   try {
-    if (!disjoint(tensors, count)) return fail(POLAR_B200_ERR_INVALID, "fadamw: a tensor is named twice, or two overlap");
+    if (!adamw_independent(tensors, count, o->schedule)) return fail(POLAR_B200_ERR_INVALID, "fadamw: what is written overlaps something else");
   } catch (const std::exception&) {                        // (no exception may leave a C entry)
     return fail(POLAR_B200_ERR_INVALID, "out of host memory");
   }

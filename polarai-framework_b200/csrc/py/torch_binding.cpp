@@ -276,12 +276,10 @@ BUILTIN(flogprob) {
   if (!has(ids, rows) || !has(lp, rows) || !has(entropy, rows) || !has(lse, rows) || (lp && !ids) || (top_ids && ids && top_type != type))
     return answer(false);
   if (top_ids && !ids) type = top_type;
-  uint64_t top = 0;
-  for (const at::Tensor* t : {top_ids, top_lp}) {
-    if (!t) continue;
-    if (t->dim() != 2 || (uint64_t)t->size(0) != rows || (top && (uint64_t)t->size(1) != top)) return answer(false);
-    top = (uint64_t)t->size(1);
-  }
+  for (const at::Tensor* t : {top_ids, top_lp})
+    if (t && (t->dim() != 2 || (uint64_t)t->size(0) != rows)) return answer(false);
+  if (top_ids && top_lp && top_ids->size(1) != top_lp->size(1)) return answer(false);
+  const uint64_t top = top_ids ? (uint64_t)top_ids->size(1) : top_lp ? (uint64_t)top_lp->size(1) : 0;
   return launched(polar_b200_flogprob, data(x), rows, classes, pitch, ids ? ids->data_ptr() : nullptr, type, data_or_null(lp),
                   data_or_null(entropy), data_or_null(lse), top, top_ids ? top_ids->data_ptr() : nullptr, data_or_null(top_lp), c.stream());
 }

@@ -11,6 +11,7 @@ call - runs the checked path below it, which raises.  An input may be longer tha
 tensor larger than what is written; what would be read or written outside a tensor is a ValueError.
 """
 import ctypes
+import numbers
 
 import numpy as np
 import torch
@@ -296,7 +297,7 @@ class DeviceBuiltins:
         with scales, float8_e4m3fn (or uint8) codes of the weights' sizes, whose scales are float32 of ceil(n / 128).
         weight_decay: one for all, or a list.  The number of the step (from 1) and lr come from the call or, for steps that are
         captured, from `schedule`, a device tensor of the two."""
-        decays = [weight_decay] * len(weights) if isinstance(weight_decay, (int, float)) else weight_decay
+        decays = [weight_decay] * len(weights) if isinstance(weight_decay, numbers.Real) else weight_decay
         if not self._native.fadamw(weights, gradients, first, second, first_scales, second_scales, step, lr, beta1, beta2, eps, decays,
                                    schedule):
             lists = _present(weights, gradients, first, second, first_scales, second_scales)

@@ -84,6 +84,12 @@ def test_adamw_statuses(c):
     assert call([{}, {}]) == 1 and call([{}, {**far, "weights": P + 60}]) == 1 and call([{}, {**far, "first": P}]) == 1
     assert call([{"second": P << 9}]) == 1 and call([{}, {**far, "second": (P << 9) - 4}]) == 1
     assert call([{"weights": P << 9}]) == 1
+    # a gradient inside another tensor's weights or its own moments, the schedule inside what is written
+    for gradient, more in ((P, far), (P + 63, far), (P - 63, far), ((P << 11) + 60, far), (P << 12, far)):
+        assert call([{}, {**more, "gradient": gradient}]) == 1 and b"overlaps" in c.polar_b200_last_error()
+    assert call([{"gradient": P << 10}]) == 1 and b"overlaps" in c.polar_b200_last_error()
+    for schedule in (P, P + 60, P - 4, (P << 9) + 32):
+        assert call([{}], schedule=schedule) == 1 and b"overlaps" in c.polar_b200_last_error()
 
 
 def test_by_name_patterns(c):
