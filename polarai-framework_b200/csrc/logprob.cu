@@ -126,13 +126,14 @@ struct Row {
 // One pass finds them too.  If `top` threads or more have met a maximum of at least some bound, the `top` largest elements are all of at
 // least that bound.  So after the first few vectors, and again whenever the part of the row that has been seen has grown fourfold, the
 // threads' maxima give a bound (a search by counting them), and from then on an element that reaches it is kept: about 4 `top` for each
-// fourfold, whatever the row's length.  At the end the bound is taken once more, what it leaves (little more than `top`) is placed by
-// counting what is above it.  -inf is never kept: where fewer than `top` elements are above it, the first of it follow.  A row where more is kept
+// fourfold, whatever the row's length.  Where a chunk holds all of a row, the bound is one of its elements.  At the end what is kept is thinned
+// out by a bound of its own, and what that leaves (little more than `top`) is placed by counting what is above it.  -inf is never kept: where fewer than `top` elements are above it, the first of it follow.  A row where more is kept
 // than there is room for (equal logits by the hundred), or with a NaN, which no maximum shows, is looked through a second time by
 // warps that sort as they go.
 constexpr float kLowest = -3.402823466e38f;
 constexpr int kInFlight = 4;                               // vectors of a thread in flight
 constexpr uint32_t kFewTop = 8;
+constexpr uint32_t kPlaced = 48;                           // as many a part of a warp places right away, by counting
 __device__ __forceinline__ float float_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
 // The largest bound, nearly, that `top` of the LANES N keys of neighbouring lanes of a warp reach (all lanes take part; each group finds its
@@ -166,16 +167,21 @@ __device__ __forceinline__ float bound_of(const uint32_t (&key)[N], uint32_t top
       least = min(least, __shfl_xor_sync(0xffffffffu, least, off));
     }
   }
-  const uint32_t group = LANES == 32 ? 0xffffffffu : ((1u << (LANES & 31)) - 1) << (threadIdx.x & 31 & ~(LANES - 1));
-  // `top` or more reach lo, fewer reach hi; between them a step for each halving: maxima lie within a few powers of two
-  uint32_t lo = LANES * N >= kMaxTop || LANES * N >= top ? least : ordered(kLowest), hi = max(most + 1, lo);
-  while (LANES == 32 ? hi - lo > 1 : __any_sync(0xffffffffu, hi - lo > 1)) {
-    const uint32_t mid = lo + (hi - lo) / 2;
+  // `top` or more reach lo, fewer reach hi + 1
+  uint32_t lo = LANES * N >= kMaxTop || LANES * N >= top ? least : ordered(kLowest), hi = max(most, lo);
+  while (LANES == 32 ? lo < hi : __any_sync(0xffffffffu, lo < hi)) {
+    const uint32_t mid = hi - (hi - lo) / 2;
     uint32_t n = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) n += __popc(__ballot_sync(0xffffffffu, key[i] >= mid) & group);
+    for (int i = 0; i < N; ++i) n += key[i] >= mid;
+    if (LANES == 32) {
+      n = __reduce_add_sync(0xffffffffu, n);
+    } else {
+#pragma unroll
+      for (int off = LANES / 2; off > 0; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
+    }
     if (n >= top) lo = mid;
-    else hi = mid;
+    else hi = mid - 1;
     if (n >= top && n <= top + top / 4 + 1) hi = lo;
   }
   return float_of(lo);
@@ -186,11 +192,11 @@ struct Kept {
   unsigned long long* rank;
   uint32_t* count;                                         // goes on beyond the room
   uint32_t room;
-  bool all = false;                                        // everything, each element in its place, and no bound
 };
 
 // The running sums over the vectors first, first + stride, ... of a row, kInFlight of them on their way; `base` is the first of the warp's
-// `first`s, `chunks` the same for a warp (or, where bounds are a matter for the CTA, for all of it).  find_bound(maxima) takes the whole team.
+// `first`s, `chunks` the same for a warp (or, where bounds are a matter for the CTA, for all of it).  find_bound(maxima, maximum,
+// chunk, whether it is all) takes the whole team.
 template <bool TOP, class FindBound>
 __device__ __forceinline__ Running scan(const Row& row, uint32_t base, uint32_t first, uint32_t stride, uint32_t chunks, float (&maxima)[kInFlight],
                                         const Kept& kept, FindBound find_bound) {
@@ -229,31 +235,24 @@ __device__ __forceinline__ Running scan(const Row& row, uint32_t base, uint32_t 
     most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
     if (most > r.m) raise_to(r, most);
     if (TOP) {
-      if (kept.all) {
-#pragma unroll
-        for (int u = 0; u < kInFlight; ++u) {
-          const float x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-#pragma unroll
-          for (uint32_t c = 0; c < 4; ++c)
-            if (row.has(i + u * stride, c)) kept.rank[row.element(i + u * stride, c)] = rank_of(x[c], row.element(i + u * stride, c));
-        }
-      } else if (n == next_bound) {
-        bound = find_bound(maxima, r.m);
+      if (n == next_bound) {
+        bound = find_bound(maxima, r.m, v, chunks == 1);
         next_bound = 4 * n + 3;
       }
-      if (!kept.all && most >= bound && *(volatile uint32_t*)kept.count <= kept.room) {
+      if (most >= bound && *(volatile uint32_t*)kept.count <= kept.room) {
         uint32_t which = 0;                                // of the 16 elements, those that reach the bound
 #pragma unroll
         for (int u = 0; u < kInFlight; ++u)
           which |= (v[u].x >= bound ? 1u << 4 * u : 0) | (v[u].y >= bound ? 2u << 4 * u : 0) | (v[u].z >= bound ? 4u << 4 * u : 0) |
                    (v[u].w >= bound ? 8u << 4 * u : 0);
+        uint32_t at = atomicAdd(kept.count, (uint32_t)__popc(which));
         while (which) {
           const uint32_t e = __ffs(which) - 1, u = e >> 2;
           which &= which - 1;
           const float4 x = u & 2 ? (u & 1 ? v[3] : v[2]) : (u & 1 ? v[1] : v[0]);
           const float value = e & 2 ? (e & 1 ? x.w : x.z) : (e & 1 ? x.y : x.x);
-          const uint32_t at = atomicAdd(kept.count, 1u);
           if (at < kept.room) kept.rank[at] = rank_of(value, row.element(i + u * stride, e & 3));
+          ++at;
         }
       }
     }
@@ -262,6 +261,45 @@ __device__ __forceinline__ Running scan(const Row& row, uint32_t base, uint32_t 
       if (inner || base + n * chunk + u * stride < row.vectors) add4(r, v[u]);
   }
   return r;
+}
+
+// Of `n` ranks in shared memory, up to ROOM, those stay that may be among the `top` largest, in front: a warp looks for a bound that `top` of them
+// reach and few more, by counting them, as above.  Returns how many stay.
+template <uint32_t ROOM>
+__device__ __forceinline__ uint32_t thin_out(unsigned long long* ranks, uint32_t n, uint32_t top, uint32_t lane) {
+  const uint32_t enough = top + top / 4 + 1;
+  if (n <= enough || n <= 32) return n;                    // (not worth it)
+  constexpr uint32_t kEach = ROOM / 32;
+  unsigned long long rank[kEach];
+  uint32_t key[kEach], most = 0, least = ~0u;
+#pragma unroll
+  for (uint32_t i = 0; i < kEach; ++i) {
+    rank[i] = 32 * i + lane < n ? ranks[32 * i + lane] : 0;
+    key[i] = (uint32_t)(rank[i] >> 32);
+    most = max(most, key[i]);
+    if (key[i]) least = min(least, key[i]);
+  }
+  uint32_t lo = __reduce_min_sync(0xffffffffu, least), hi = __reduce_max_sync(0xffffffffu, most);   // all reach lo; of hi + 1 none
+  while (lo < hi) {
+    const uint32_t mid = hi - (hi - lo) / 2;
+    uint32_t reach = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) reach += key[i] >= mid;
+    reach = __reduce_add_sync(0xffffffffu, reach);
+    if (reach >= top) lo = mid;
+    else hi = mid - 1;
+    if (reach >= top && reach <= enough) hi = lo;
+  }
+  uint32_t total = 0;
+  __syncwarp();
+#pragma unroll
+  for (uint32_t i = 0; i < kEach; ++i) {
+    const uint32_t up = __ballot_sync(0xffffffffu, key[i] >= lo && key[i] != 0);
+    if (up >> lane & 1) ranks[total + __popc(up & ((1u << lane) - 1))] = rank[i];
+    total += __popc(up);
+  }
+  __syncwarp();
+  return total;
 }
 
 // A warp's sorted list of ranks, the largest in lane 0; takes the elements of one vector per lane.
@@ -322,8 +360,8 @@ __device__ __forceinline__ void write_top(const Results& o, uint64_t row, uint32
   if (o.top_ids) write_id(o.top_ids, o.id_type, row * o.top + at, id);
   if (o.top_logprob) o.top_logprob[row * o.top + at] = r.s == 0.f ? -INFINITY : x - r.m - log_sum;
 }
-__device__ __forceinline__ void write_top(const Results& o, uint64_t row, uint32_t at, unsigned long long rank, const Running& r) {
-  write_top(o, row, at, ~(uint32_t)rank, float_of((uint32_t)(rank >> 32)), r, logf(r.s));
+__device__ __forceinline__ void write_top(const Results& o, uint64_t row, uint32_t at, unsigned long long rank, const Running& r, float log_sum) {
+  write_top(o, row, at, ~(uint32_t)rank, float_of((uint32_t)(rank >> 32)), r, log_sum);
 }
 
 // Many classes: a CTA per row, or a cluster of CTAs where there are few rows.
@@ -350,7 +388,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_wide_kernel(c
   }
   int turn = 0;
   // (two arrays in turn: a barrier is between a round's reads and the writes of the next but one)
-  auto find_bound = [&](const float (&)[kInFlight], float mine) {
+  auto find_bound = [&](const float (&)[kInFlight], float mine, const float4 (&)[kInFlight], bool) {
     uint32_t k[4];                                         // of 128 groups of threads: enough for 32 alternatives
     keys[turn][tid] = ordered(mine);
     __syncthreads();
@@ -375,7 +413,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_wide_kernel(c
   if (TOP) {
     const uint32_t n = n_kept;                             // the same for all threads, as what hangs on it
     if (n <= kRoom && all.s == all.s) {
-      const float bound = n > 64 ? find_bound(maxima, own.m) : kLowest;
+      const float4 none[kInFlight] = {};
+      const float bound = n > 64 ? find_bound(maxima, own.m, none, false) : kLowest;
       for (uint32_t i = tid; i < n; i += THREADS)
         if (kept_ranks[i] >= (uint64_t)ordered(bound) << 32) left[atomicAdd(&n_left, 1u)] = kept_ranks[i];
     } else {
@@ -400,7 +439,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_wide_kernel(c
   }
   if (ctas == 1) {
     if (tid == 0) write_row(o, r, id, given, all);
-    if (TOP && tid < o.top) write_top(o, r, tid, sorted[tid], all);
+    if (TOP && tid < o.top) write_top(o, r, tid, sorted[tid], all, logf(all.s));
     return;
   }
   if (tid == 0) joined[0] = all.m, joined[1] = all.s, joined[2] = all.t;
@@ -428,7 +467,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_wide_kernel(c
             if (c < ctas && n + step <= o.top && theirs[c * o.top + n + step - 1] > mine) n += step;
           above += n;
         }
-        if (above < o.top && mine) write_top(o, r, above, mine, all);
+        if (above < o.top && mine) write_top(o, r, above, mine, all, logf(all.s));
       }
     }
   }
@@ -436,22 +475,18 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_wide_kernel(c
   cluster_wait();
 }
 
-// A warp per row or, for short rows, LANES lanes; `per_warp` of the warp's teams have rows (one where there are few: then what the whole warp
-// does for a row has only that one to do).
+// A warp per row or, for short rows, LANES lanes.
 template <int LANES, bool TOP>
-__global__ void __launch_bounds__(kThreads) logprob_warp_kernel(const float* logits, uint32_t rows, uint32_t classes, uint64_t pitch, uint32_t per_warp,
-                                                                Results o) {
-  // (room for all of a short row: where there are many alternatives, all are placed, without looking for a bound)
-  constexpr uint32_t kRoom = !TOP ? 1 : LANES == 32 ? 256 : 128, kTeams = kThreads / LANES;
-  const bool all_kept = TOP && LANES < 32 && (o.top > kFewTop || (classes <= 32 && per_warp == 1));
+__global__ void __launch_bounds__(kThreads) logprob_warp_kernel(const float* logits, uint32_t rows, uint32_t classes, uint64_t pitch, Results o) {
+  constexpr uint32_t kRoom = !TOP ? 1 : LANES == 32 ? 512 : 128, kTeams = kThreads / LANES, kRows = 32 / LANES;
   __shared__ unsigned long long kept_ranks[kTeams][kRoom];
   __shared__ uint32_t n_kept[kTeams];
   pdl_enter();
   const uint32_t lane = threadIdx.x & 31, team = threadIdx.x / LANES, member = threadIdx.x % LANES;
-  const uint64_t first = ((uint64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32) * per_warp;   // the warp's first row
+  const uint64_t first = ((uint64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32) * kRows;   // the warp's first row
   if (first >= rows) return;
   const uint64_t r = first + lane / LANES;
-  const bool live = lane / LANES < per_warp && r < rows;
+  const bool live = r < rows;
   const Row row(logits + (live ? r : first) * pitch, classes);   // (lanes without a row of their own look at the warp's first)
   int64_t id = kPadding;
   float given = 0.f;
@@ -462,16 +497,26 @@ __global__ void __launch_bounds__(kThreads) logprob_warp_kernel(const float* log
   unsigned long long* kept = kept_ranks[team];
   if (TOP && member == 0) n_kept[team] = 0;
   __syncwarp();
-  auto find_bound = [&](const float (&maxima)[kInFlight], float) {
+  auto find_bound = [&](const float (&maxima)[kInFlight], float, const float4 (&v)[kInFlight], bool all_of_it) {
+    if (o.top > kFewTop && classes <= kPlaced) return kLowest;
+    if (o.top > kFewTop && all_of_it) {                    // the row is here: a bound of its elements, which few more than `top` reach
+      uint32_t k[4 * kInFlight];
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u) {
+        k[4 * u] = ordered(fmaxf(v[u].x, kLowest)), k[4 * u + 1] = ordered(fmaxf(v[u].y, kLowest));
+        k[4 * u + 2] = ordered(fmaxf(v[u].z, kLowest)), k[4 * u + 3] = ordered(fmaxf(v[u].w, kLowest));
+      }
+      return bound_of<LANES>(k, o.top);
+    }
     uint32_t k[kInFlight];
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) k[u] = ordered(maxima[u]);
     return bound_of<LANES>(k, o.top);
   };
   float maxima[kInFlight];
-  // (rows that begin elsewhere on a boundary may have a vector more or less: as many chunks as the longest)
+  // (rows that begin elsewhere on a boundary may have a vector more or less: as many chunks as the longest; eight lanes have one)
   const uint32_t chunks = ((classes + 6) / 4 + kInFlight * LANES - 1) / (kInFlight * LANES);
-  const Running own = scan<TOP>(row, 0, member, LANES, chunks, maxima, Kept{kept, &n_kept[team], kRoom, all_kept}, find_bound);
+  const Running own = scan<TOP>(row, 0, member, LANES, chunks, maxima, Kept{kept, &n_kept[team], kRoom}, find_bound);
   Running all = own;
   float m = own.m;
 #pragma unroll
@@ -485,45 +530,37 @@ __global__ void __launch_bounds__(kThreads) logprob_warp_kernel(const float* log
   if (member == 0 && live) write_row(o, r, id, given, all);
   if (!TOP) return;
   __syncwarp();
-  const uint32_t n = !live ? o.top : all_kept ? classes : n_kept[team];
-  const bool sorts = live && !all_kept && (n > kRoom || all.s != all.s);
-  const bool simple = !sorts && n >= o.top && n <= (LANES == 32 ? 64 : per_warp > 1 ? 32 : 8) && !all_kept;
+  const uint32_t n = live ? n_kept[team] : o.top;
+  const bool sorts = live && (n > kRoom || all.s != all.s);
+  const bool simple = !sorts && n >= o.top && n <= (LANES == 32 ? 64 : kPlaced);
+  const float log_sum = logf(all.s);
   if (simple && live) {                                    // few: each team places its own, by counting what is above
     for (uint32_t i = member; i < n; i += LANES) {
       uint32_t above = 0;
       const unsigned long long mine = kept[i];
       for (uint32_t j = 0; j < n; ++j) above += kept[j] > mine;
-      if (above < o.top) write_top(o, r, above, mine, all);
+      if (above < o.top) write_top(o, r, above, mine, all, log_sum);
     }
   }
   uint32_t others = __ballot_sync(0xffffffffu, live && !simple && member == 0);
   if (others == 0) return;
   // the other rows one after the other, by the whole warp
-  const float last_bound = all_kept ? 0.f : find_bound(maxima, own.m);
   for (; others; others &= others - 1) {
     const int who = __ffs(others) - 1;
     const uint64_t q = first + who / LANES;
     Running sums;
     sums.m = __shfl_sync(0xffffffffu, all.m, who), sums.s = __shfl_sync(0xffffffffu, all.s, who);
+    const float its_log_sum = __shfl_sync(0xffffffffu, log_sum, who);
     if (__shfl_sync(0xffffffffu, (int)sorts, who)) {
       const Row its(logits + q * pitch, classes);
       unsigned long long list = 0;
       for (uint32_t i = lane; i - lane < its.vectors; i += 32) take(list, its, i, o.top, lane);
-      if (lane < o.top) write_top(o, q, lane, list, sums);
+      if (lane < o.top) write_top(o, q, lane, list, sums, its_log_sum);
       continue;
     }
     unsigned long long* its_kept = kept_ranks[(threadIdx.x - lane + who) / LANES];
     const uint32_t its_n = __shfl_sync(0xffffffffu, n, who);
-    const uint64_t least = (uint64_t)ordered(__shfl_sync(0xffffffffu, last_bound, who)) << 32;
-    uint32_t total = all_kept ? its_n : 0;                 // what reaches the bound of the whole row moves to the front
-    for (uint32_t i = 0; i < its_n && !all_kept; i += 32) {
-      const unsigned long long rank = i + lane < its_n ? its_kept[i + lane] : 0;
-      const uint32_t up = __ballot_sync(0xffffffffu, rank >= least && rank);
-      __syncwarp();
-      if (up >> lane & 1) its_kept[total + __popc(up & ((1u << lane) - 1))] = rank;   // (never behind what has been read)
-      total += __popc(up);
-      __syncwarp();
-    }
+    const uint32_t total = LANES < 32 || its_n <= 128 ? thin_out<128>(its_kept, its_n, o.top, lane) : thin_out<512>(its_kept, its_n, o.top, lane);
     for (uint32_t i = lane; i < total; i += 64) {          // two of them against all, for each lane
       uint32_t above_a = 0, above_b = 0;
       const unsigned long long a = its_kept[i], b = i + 32 < total ? its_kept[i + 32] : 0;
@@ -533,15 +570,15 @@ __global__ void __launch_bounds__(kThreads) logprob_warp_kernel(const float* log
         above_a += other > a;
         above_b += other > b;
       }
-      if (above_a < o.top) write_top(o, q, above_a, a, sums);
-      if (above_b < o.top && b) write_top(o, q, above_b, b, sums);
+      if (above_a < o.top) write_top(o, q, above_a, a, sums, its_log_sum);
+      if (above_b < o.top && b) write_top(o, q, above_b, b, sums, its_log_sum);
     }
     if (total < o.top) {
       const Row its(logits + q * pitch, classes);
       __syncwarp();
       take_shut_out(its_kept, o.top - total, its, 0, 32, 32, lane);
       __syncwarp();
-      if (lane + total < o.top) write_top(o, q, lane + total, its_kept[lane], sums);
+      if (lane + total < o.top) write_top(o, q, lane + total, its_kept[lane], sums, its_log_sum);
     }
     __syncwarp();
   }
@@ -739,30 +776,32 @@ int polar_b200_flogprob(const float* logits, uint64_t rows, uint64_t classes, ui
     return classes <= 8 ? go(logprob_thread_kernel<8>) : go(logprob_thread_kernel<16>);
   }
   // A warp per row as long as there are rows enough for every SM (20000 x 8192: 95 us against 104 with a CTA of 128 threads per row, with five
-  // alternatives 131 and 162; 300 x 8000 with five 18.6 and 8.4; up to 1024 classes always); eight lanes for the shortest (60000 x 100: 7.6 us
-  // against 20, with five alternatives 23 and 63), four rows to a warp once every SM has its warps.
+  // alternatives 131 and 162; 300 x 8000 with five 18.6 and 8.4; up to 1024 classes always).  Where there are more rows than six to an SM, as many
+  // lanes to a short row as hold it in one chunk: 60000 x 100 7.6 us with 8 lanes, with a warp 20; x 200 14.2 with 16, with a warp 23, with twenty
+  // alternatives 62 and 91; but 300 x 100 with twenty 7.4 us with 8 lanes, 5.0 with a warp.
   const uint64_t sms = (uint64_t)sm_count();
   if (classes <= 1024 || (classes <= 8192 && rows >= 16 * sms)) {
-    const uint32_t lanes = classes <= 128 ? 8 : 32;
-    const uint32_t per_warp = lanes == 8 && rows > 48 * sms ? 4 : 1;
-    const uint64_t warps = (rows + per_warp - 1) / per_warp;
+    const uint32_t lanes = rows <= 6 * sms ? 32 : classes <= 4 * kInFlight * 8 - 3 ? 8 : classes <= 4 * kInFlight * 16 - 3 ? 16 : 32;
+    const uint64_t warps = (rows * lanes + 31) / 32;
     const dim3 grid((unsigned)((warps + kThreads / 32 - 1) / (kThreads / 32)));
-    auto go = [&](auto kernel) { return launch("flogprob", kernel, grid, kThreads, 0, st, logits, (uint32_t)rows, n, pitch, per_warp, o); };
-    return lanes == 8 ? (top ? go(logprob_warp_kernel<8, true>) : go(logprob_warp_kernel<8, false>))
-                      : (top ? go(logprob_warp_kernel<32, true>) : go(logprob_warp_kernel<32, false>));
+    auto go = [&](auto kernel) { return launch("flogprob", kernel, grid, kThreads, 0, st, logits, (uint32_t)rows, n, pitch, o); };
+    return lanes == 8    ? (top ? go(logprob_warp_kernel<8, true>) : go(logprob_warp_kernel<8, false>))
+           : lanes == 16 ? (top ? go(logprob_warp_kernel<16, true>) : go(logprob_warp_kernel<16, false>))
+                         : (top ? go(logprob_warp_kernel<32, true>) : go(logprob_warp_kernel<32, false>));
   }
-  // Few rows: clusters of up to eight CTAs per row, the largest that the SMs hold at two per SM, of 512 threads (1 x 131072: 4.3 us, with
-  // twenty alternatives 9.1; of 128 threads 6.3 and 14.2).  Many rows: CTAs of 128 threads, since barriers then hold up fewer loads
-  // (2048 x 50001: 69 us, with five alternatives 81; of 512 threads 76 and 96); in between 256 (300 x 8000 with five 7.1 us, 128 threads 8.4).
+  // Few rows: CTAs of 512 threads, in clusters of up to eight per row while the SMs hold them at two per SM and each has some 7000 classes
+  // (1 x 131072: 4.3 us, with twenty alternatives 8.7; of 128 threads 6.3 and 14.2; 20 x 9000 with five 5.0 us in one CTA, 6.8 in two).  Many rows:
+  // CTAs of 128 threads, since barriers then hold up fewer loads (2048 x 50001: 69 us, with five alternatives 79; of 512 threads 76 and 96).  In
+  // between, threads for all of an SM: 200 x 60000 12.2 us with 512, 17.9 with 256; 592 x 29572 14.8 with 256, 18.5 with 128.
   unsigned ctas = 1;
-  while (ctas < 8 && rows * ctas * 2 <= 2 * sms && classes / (2 * ctas) >= 4096) ctas *= 2;
+  while (ctas < 8 && rows * ctas * 2 <= 2 * sms && classes / (2 * ctas) >= 7000) ctas *= 2;
   const dim3 grid((unsigned)rows, ctas);
   auto go = [&](auto with, auto without, unsigned threads) {
     return launch_clusters("flogprob", top ? with : without, grid, threads, 0, st, ctas, logits, n, pitch, o);
   };
-  if (ctas > 1) return go(logprob_wide_kernel<512, true>, logprob_wide_kernel<512, false>, 512);
-  return rows >= 4 * sms ? go(logprob_wide_kernel<128, true>, logprob_wide_kernel<128, false>, 128)
-                         : go(logprob_wide_kernel<256, true>, logprob_wide_kernel<256, false>, 256);
+  if (rows <= 2 * sms) return go(logprob_wide_kernel<512, true>, logprob_wide_kernel<512, false>, 512);
+  return rows <= 4 * sms ? go(logprob_wide_kernel<256, true>, logprob_wide_kernel<256, false>, 256)
+                         : go(logprob_wide_kernel<128, true>, logprob_wide_kernel<128, false>, 128);
 }
 
 int polar_b200_flogprob_grad(const float* logits, uint64_t rows, uint64_t classes, uint64_t pitch, const void* ids, int id_type,

@@ -133,20 +133,17 @@ def test_rows_apart_and_on_odd_boundaries(env, rows, classes, pitch, offset, top
         check(torch, x, ids, run(torch, d, x, ids, top, kind), top)
 
 
-@pytest.mark.parametrize("classes", [7, 32, 40, 500, 3000, 30000, 140001])
-def test_ties_masks_and_values_at_the_edges(env, classes):
-    torch, d = env
-    top = min(classes, 20)
-    x, ids = logits(torch, 14, classes)
-    low = torch.finfo(torch.float32).min
+def edge_rows(x, ids, classes):
+    """Into the first 13 rows; the third one is shut out altogether."""
+    low = float(np.finfo(np.float32).min)
     x[0] = 1.25                                              # all alike
     x[1, ::2] = -np.inf                                      # half of them shut out
     x[2] = -np.inf                                           # all of them
     x[3] = low                                               # all at the type's lowest value
     x[4, classes // 2:] = low
-    x[5] = torch.round(x[5])                                 # many ties
-    x[6] = torch.arange(classes, device="cuda") * 1e-3       # rising, and falling
-    x[7] = -torch.arange(classes, device="cuda") * 1e-3
+    x[5] = x[5].round()                                 # many ties
+    x[6] = x.new_tensor(range(classes)) * 1e-3       # rising, and falling
+    x[7] = -x.new_tensor(range(classes)) * 1e-3
     x[8] = 0.0
     x[8, ::3] = -0.0                                         # a zero is a zero
     x[9] = 3e38                                              # the largest
@@ -158,6 +155,14 @@ def test_ties_masks_and_values_at_the_edges(env, classes):
     # (differences of the lowest value and others are beyond fp32, and their exponential is zero all the same)
     ids[1], ids[4], ids[10] = 1, 0, 0
     ids[12] = 0
+
+
+@pytest.mark.parametrize("classes", [7, 32, 40, 500, 3000, 30000, 140001])
+def test_ties_masks_and_values_at_the_edges(env, classes):
+    torch, d = env
+    top = min(classes, 20)
+    x, ids = logits(torch, 14, classes)
+    edge_rows(x, ids, classes)
     o = run(torch, d, x, ids, top)
     keep = [i for i in range(14) if i != 2]
     check(torch, x[keep], ids[keep], {k: v[keep] for k, v in o.items()}, top)
@@ -180,6 +185,22 @@ def test_ties_masks_and_values_at_the_edges(env, classes):
     lp = torch.empty(12, device="cuda")
     d.flogprob(logits(torch, 12, classes, seed=1)[0], f, lp)
     assert torch.isnan(lp[[0, 2, 3, 4]]).all() and lp[1] == 0 and torch.isfinite(lp[5:]).all()
+
+
+@pytest.mark.parametrize("rows", [600, 1003])
+@pytest.mark.parametrize("classes", [17, 33, 48, 49, 100, 125, 126, 200, 253, 254, 256, 509, 510, 1024])
+def test_edges_among_many_rows(env, rows, classes):
+    torch, d = env
+    for top, at in ((5, 0), (12, 301), (min(classes, 32), rows - 14)):   # the edges in front, in the middle, at the end
+        x, ids = logits(torch, rows, classes, offset=at % 4)
+        edge_rows(x[at:], ids[at:], classes)
+        nan = rows // 3
+        x[nan, classes - 1] = np.nan
+        o = run(torch, d, x, ids, top)
+        keep = torch.tensor([i for i in range(rows) if i not in (at + 2, nan)], device="cuda")
+        check(torch, x[keep], ids[keep], {k: v[keep] for k, v in o.items()}, top)
+        assert o["logprob"][at + 2] == -np.inf and o["top_ids"][at + 2].tolist() == list(range(top))
+        assert torch.isnan(o["logprob"][nan]) and torch.equal(o["top_ids"][nan:nan + 1], best(torch, x[nan:nan + 1], top))
 
 
 def expect_grad(torch, x, ids, lse, ent, g, ge):
