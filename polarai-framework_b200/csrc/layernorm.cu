@@ -4,6 +4,9 @@
 // written), and a dozen operations each.  Deviations are summed around the mean, never as the difference of
 // two large sums, and all sums are taken over two levels (threads, then the CTA), so that their rounding stays near that of a few dozen
 // additions whatever the row's length.
+#include <algorithm>
+#include <atomic>
+
 #include "rows.cuh"
 
 namespace polar_b200 {
@@ -481,19 +484,44 @@ GradPlan grad_plan(uint64_t rows, uint64_t cols) {
   while ((uint64_t)p.lanes * p.v * 4 < cols && p.lanes < 512) p.lanes *= 2;
   if (cols > 8192) {
     p.lanes = cols <= 32768 ? 256 : 512;
-    while ((uint64_t)p.lanes * p.v * 4 * p.ctas < cols) p.ctas *= 2;
+    p.ctas = (unsigned)((cols + p.lanes * p.v * 4 - 1) / (p.lanes * p.v * 4));
   }
-  // 512 threads on an SM, with three stages of up to 64 KB; each CTA some rows, so that the partial sums are few beside them
+  // 512 threads on an SM, with three stages of up to 64 KB; where there are many rows, some for each CTA, so that the partial sums are few beside
+  // them (3 x 7560: 7.2 us with a CTA per row, 8.5 with one for two)
   const uint64_t sms = (uint64_t)sm_count(), block = p.lanes > kThreads ? p.lanes : kThreads, groups = (rows * p.lanes + block - 1) / block;
-  uint64_t most = sms * (512 / block) / p.ctas;
-  if (p.ctas >= 4) most = most * 7 / 8;                    // (larger clusters leave SMs of a GPC unused)
-  const uint64_t wanted = (groups + 1) / 2;
+  const uint64_t most = sms * (512 / block) / p.ctas, wanted = groups <= sms ? groups : (groups + 1) / 2;
   p.grid = (unsigned)(wanted < most ? wanted : most);
   return p;
 }
 
+// How many of a kernel's clusters a device holds at a time: fewer than SMs by CTAs, as a cluster lies within a GPC.  A property of the device and the
+// kernel, asked for once.
+template <auto KERNEL>
+unsigned resident_clusters(unsigned threads, size_t bytes, unsigned ctas, unsigned most) {
+  constexpr int kDevices = 64;
+  static std::atomic<unsigned> known[kDevices];
+  int device = 0, n = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kDevices) return most * 3 / 4;
+  if (const unsigned before = known[device].load(std::memory_order_relaxed)) return before;
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3(most, ctas);
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = bytes;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 1, at[0].val.clusterDim.y = ctas, at[0].val.clusterDim.z = 1;
+  c.attrs = at;
+  c.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, KERNEL, &c) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    return most * 3 / 4;
+  }
+  known[device].store((unsigned)n, std::memory_order_relaxed);
+  return (unsigned)n;
+}
+
 template <int LANES, int V, bool VECTOR, int CTAS>
-int launch_grad_rows(const GradPlan& p, cudaStream_t st, const float* gradient, const float* in, const float* gamma, const float* mean,
+int launch_grad_rows(GradPlan& p, cudaStream_t st, const float* gradient, const float* in, const float* gamma, const float* mean,
                      const float* rstd, uint64_t rows, uint64_t cols, float* din, float* partials) {
   constexpr auto kernel = norm_grad_rows_kernel<LANES, V, VECTOR, CTAS, kStages>;
   constexpr size_t bytes = (size_t)kStages * 2 * (4 * V * LANES + (VECTOR ? 0 : 4)) * (kBlockOf<LANES> / LANES) * sizeof(float);
@@ -501,6 +529,7 @@ int launch_grad_rows(const GradPlan& p, cudaStream_t st, const float* gradient, 
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (e != cudaSuccess) return fail(POLAR_B200_ERR_CUDA, "cudaFuncSetAttribute(flayernorm_grad)", e);
   }
+  if (CTAS > 1) p.grid = std::max(1u, std::min(p.grid, resident_clusters<kernel>(kBlockOf<LANES>, bytes, CTAS, p.grid)));
   return launch_clusters("flayernorm_grad", kernel, dim3(p.grid, CTAS), kBlockOf<LANES>, bytes, st, CTAS, gradient, in, gamma, mean, rstd, (uint32_t)rows,
                          (uint32_t)cols, (float)(1.0 / (double)cols), din, partials);
 }
@@ -559,7 +588,7 @@ int polar_b200_flayernorm(const float* in, const float* gamma, const float* beta
   }
   // Longer ones: a large CTA, clusters of CTAs where the row is beyond one or, as single floats, beyond its registers, and smaller shares in
   // larger clusters where there are few rows (1 x 32768: 4.3 us, one CTA 6.7).
-  if (rows * 8 <= 2 * sms && cols <= 32768) return ROWS(512, 2, 0, 8);
+  if (rows * 8 <= 2 * sms && cols > 16384 && cols <= 32768) return ROWS(512, 2, 0, 8);
   if (!vectors && cols <= 65536) return cols <= 16384 ? ROWS(512, 4, 2, 2) : cols <= 32768 ? ROWS(512, 4, 2, 4) : ROWS(512, 4, 2, 8);
   if (cols <= 16384) return ROWS(512, 8, 4, 1);
   if (cols <= 32768) return ROWS(1024, 8, 4, 1);
@@ -591,7 +620,7 @@ int polar_b200_flayernorm_grad(const float* gradient, const float* in, const flo
   LaunchDeviceScope on(stream, din);
   cudaStream_t st = as_stream(stream);
   int rc = POLAR_B200_OK;
-  const GradPlan plan = grad_plan(rows, cols);
+  GradPlan plan = grad_plan(rows, cols);
   const uint64_t need = polar_b200_flayernorm_grad_workspace_bytes(rows, cols);
   void* own = nullptr;
   float* partials = nullptr;
@@ -604,7 +633,7 @@ int polar_b200_flayernorm_grad(const float* gradient, const float* in, const flo
     }
     partials = static_cast<float*>(workspace ? workspace : own);
   }
-  uint32_t parts = plan.grid;
+  uint32_t parts = 0;
   if (plan.lanes) {
     const bool vectors = (cols & 3) == 0 && aligned16(gradient) && aligned16(in) && aligned16(gamma) && aligned16(din);
     auto go = [&](auto with, auto without) {
@@ -617,9 +646,27 @@ int polar_b200_flayernorm_grad(const float* gradient, const float* in, const flo
       case 32: rc = ROWS(32, 4, 1); break;
       case 64: rc = ROWS(64, 4, 1); break;
       case 128: rc = ROWS(128, 4, 1); break;
-      case 256: rc = plan.ctas == 1 ? ROWS(256, 4, 1) : plan.ctas == 4 ? ROWS(256, 4, 4) : ROWS(256, 4, 8); break;
-      default: rc = plan.ctas == 1 ? ROWS(512, 4, 1) : plan.ctas == 2 ? ROWS(512, 4, 2) : plan.ctas == 4 ? ROWS(512, 4, 4) : ROWS(512, 4, 8);
+      case 256:
+        switch (plan.ctas) {
+          case 1: rc = ROWS(256, 4, 1); break;
+          case 3: rc = ROWS(256, 4, 3); break;
+          case 4: rc = ROWS(256, 4, 4); break;
+          case 5: rc = ROWS(256, 4, 5); break;
+          case 6: rc = ROWS(256, 4, 6); break;
+          case 7: rc = ROWS(256, 4, 7); break;
+          default: rc = ROWS(256, 4, 8);
+        }
+        break;
+      default:
+        switch (plan.ctas) {
+          case 1: rc = ROWS(512, 4, 1); break;
+          case 5: rc = ROWS(512, 4, 5); break;
+          case 6: rc = ROWS(512, 4, 6); break;
+          case 7: rc = ROWS(512, 4, 7); break;
+          default: rc = ROWS(512, 4, 8);
+        }
     }
+    parts = plan.grid;                                     // (with clusters what is resident, which is less than planned)
 #undef ROWS
   } else if (partials) {
     parts = (uint32_t)stretches(rows);
