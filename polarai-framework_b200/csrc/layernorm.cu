@@ -166,6 +166,97 @@ __global__ void __launch_bounds__(LANES > 32 ? LANES : kThreads, resident(LANES,
   if (CTAS > 1) cluster_wait();
 }
 
+// ---- rows through shared memory -----------------------------------------------------------------------
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const float* from, uint32_t bytes) {   // (zeros behind `bytes`)
+  const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to);
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+// Rows that do not begin on 16-byte boundaries are copied as they lie, vectors from the boundary before their beginning on: how far a row begins
+// past a boundary, and the copies that one of LANES threads makes of up to 4 V LANES floats.
+__device__ __forceinline__ uint32_t past(const float* p) { return (uint32_t)(reinterpret_cast<uintptr_t>(p) >> 2) & 3; }
+template <int LANES, int V>
+__device__ __forceinline__ void copy_image(float* to, const float* src, uint32_t count, uint32_t member) {
+  const uint32_t shift = past(src);
+#pragma unroll
+  for (int j = 0; j <= V; ++j) {                           // (a row that begins past a boundary has a vector more)
+    const uint32_t i = member + LANES * j;
+    const int left = 4 * (int)(shift + count) - 16 * (int)i;
+    if (left <= 0 || (j == V && member)) continue;
+    if (j == 0 && i == 0 && shift) {
+      for (uint32_t k = shift; k < 4 && k < shift + count; ++k) copy_async<4>(to + k, src + (k - shift), 4);
+    } else {
+      copy_async<16>(to + 4 * i, src + (int64_t)(4 * i) - shift, left < 16 ? left : 16);
+    }
+  }
+}
+
+// Forward, long rows that are not on 16-byte boundaries: an SM's CTAs stay and go through the rows with gamma and beta in their registers; two
+// rows are on their way while one is computed (8000 x 9001: 113 us, a cluster of two CTAs per row 265; 16384 x 16383: 343 and
+// 662; 8007 x 7830: 91, a CTA per row 110; 60000 x 2101: 170 and 214).
+constexpr int kRing = 3;
+template <int LANES, int V>
+__global__ void __launch_bounds__(LANES, 512 / LANES) norm_ring_kernel(const float* in, const float* gamma, const float* beta, float eps, uint32_t rows,
+                                                                       uint32_t cols, float per_col, float* out, float* mean_out, float* rstd_out) {
+  constexpr int N = 4 * V, kImage = LANES * N + 4;
+  using S = Share<LANES, V, false, V - 2>;                 // (cols > 4 LANES (V - 2))
+  extern __shared__ float4 images[];
+  __shared__ float slots[2][LANES / 32];
+  pdl_enter();
+  float* ring = reinterpret_cast<float*>(images);
+  const uint32_t member = threadIdx.x, live = S::live(member, cols);
+  uint64_t r = blockIdx.x, fetched = r;
+  uint32_t to_stage = 0, stage = 0;
+  auto fetch = [&] {
+    if (fetched < rows) copy_image<LANES, V>(ring + to_stage * kImage, in + fetched * cols, cols, member);
+    copies_end();                                          // (an empty group as well: a group for each row)
+    fetched += gridDim.x;
+    to_stage = to_stage + 1 == kRing ? 0 : to_stage + 1;
+  };
+#pragma unroll
+  for (int s = 0; s < kRing - 1; ++s) fetch();
+  float g[N], b[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) g[k] = 1.f, b[k] = 0.f;
+  if (gamma) S::load(g, gamma, member, live);
+  if (beta) S::load(b, beta, member, live);
+  for (; r < rows; r += gridDim.x) {
+    copies_wait<kRing - 2>();
+    __syncthreads();                                       // what other threads have copied is here, and all have read the row before
+    float x[N];
+    const float* p = ring + stage * kImage + past(in + r * cols) + member;
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[k] = S::has(live, k) ? p[LANES * k] : 0.f;
+    fetch();
+    float s[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < N; ++k) s[0] += x[k];
+    block_sums<LANES>(s, slots[0]);
+    const float mean = s[0] * per_col;
+    s[0] = 0.f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      x[k] -= mean;
+      if (S::has(live, k)) s[0] += x[k] * x[k];
+    }
+    block_sums<LANES>(s, slots[1]);
+    const float rstd = rsqrtf(s[0] * per_col + eps);
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[k] = x[k] * rstd * g[k] + b[k];
+    S::store(x, out + r * cols, member, live);
+    if (member == 0) {
+      if (mean_out) mean_out[r] = mean;
+      if (rstd_out) rstd_out[r] = rstd;
+    }
+    stage = stage + 1 == kRing ? 0 : stage + 1;
+  }
+}
+
 // Rows of any length: three passes over a row that the caches hold.
 __global__ void __launch_bounds__(kThreads) norm_kernel(const float* in, const float* gamma, const float* beta, float eps,
                                                         uint64_t cols, float* out, float* mean_out, float* rstd_out) {
@@ -196,16 +287,6 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const float* in, const f
 // columns in registers.  The rows come through a ring in shared memory, STAGES - 1 of them on their way while one is computed, by asynchronous
 // copies that each thread makes and waits for by itself: what it copies is what it reads, so no barrier is needed but the one of the row's sums.
 // The sums over the team's rows go to `partials` [CTAs or clusters][2][cols], which a second kernel adds in order.
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* to, const float* from, uint32_t bytes) {   // (zeros behind `bytes`)
-  const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to);
-  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int LEFT>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
-
 template <int LANES>
 constexpr int kBlockOf = LANES > kThreads ? LANES : kThreads;   // threads of a CTA
 // A barrier of a team and the sums over it, in every thread, where several teams share a CTA (`group`: the team's number; `slots`: 2 for each warp).
@@ -255,7 +336,6 @@ __global__ void __launch_bounds__(kBlockOf<LANES>, 512 / kBlockOf<LANES>) norm_g
   uint64_t fetched = r;
   const float *src_g = gradient + r * cols + from, *src_x = in + r * cols + from;
   uint32_t to_stage = 0;
-  auto past = [](const float* p) { return (uint32_t)(reinterpret_cast<uintptr_t>(p) >> 2) & 3; };
   auto image = [&](uint32_t stage, int which) { return ring + ((stage * 2 + which) * kGroups + group) * kImage; };
   auto fetch = [&] {
     if (fetched < rows) {
@@ -269,19 +349,7 @@ __global__ void __launch_bounds__(kBlockOf<LANES>, 512 / kBlockOf<LANES>) norm_g
             copy_async<16>(ring4 + ((to_stage * 2 + which) * V + i) * kBlock + tid, S::has(live, 4 * i) ? src + 4 * LANES * i : gradient,
                            S::has(live, 4 * i) ? 16 : 0);
         } else {
-          const uint32_t shift = past(src);
-          float* to = image(to_stage, which);
-#pragma unroll
-          for (int j = 0; j <= V; ++j) {                   // (a row that begins past a boundary has a vector more)
-            const uint32_t i = member + LANES * j;
-            const int left = 4 * (int)(shift + here) - 16 * (int)i;
-            if (left <= 0 || (j == V && member)) continue;
-            if (j == 0 && i == 0 && shift) {
-              for (uint32_t k = shift; k < 4 && k < shift + here; ++k) copy_async<4>(to + k, src + (k - shift), 4);
-            } else {
-              copy_async<16>(to + 4 * i, src + (int64_t)(4 * i) - shift, left < 16 ? left : 16);
-            }
-          }
+          copy_image<LANES, V>(image(to_stage, which), src, here, member);
         }
       }
     }
@@ -573,6 +641,21 @@ int polar_b200_flayernorm(const float* in, const float* gamma, const float* beta
   const uint64_t sms = (uint64_t)sm_count();
   // (The number of elements per thread that a form is made for is its V: FULL fours of every thread are there without asking, so each form serves
   // cols > 4 LANES CTAS FULL only.)
+  auto ring = [&](auto kernel, unsigned threads, unsigned v) {
+    const size_t bytes = kRing * (threads * v * 4 + 4) * sizeof(float);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != cudaSuccess) return fail(POLAR_B200_ERR_CUDA, "cudaFuncSetAttribute(flayernorm)", e);
+    const uint64_t most = sms * (512 / threads);
+    return launch("flayernorm", kernel, dim3((unsigned)(rows < most ? rows : most)), threads, bytes, st, in, gamma, beta, eps, (uint32_t)rows,
+                  (uint32_t)cols, (float)(1.0 / (double)cols), out, mean, rstd);
+  };
+  // (once every SM has its CTAs, and four rows for each of the smaller ones: 600 x 7830 9.6 us and 10.2, 300 x 7830 7.1 and 7.4, 3000 x 2501 13.4 and
+  // 15.0; up to 2048 columns loads into registers do as well)
+  if (!vectors && cols > 2048 && cols <= 16384 && rows >= (cols <= 4096 ? 16 : 4) * sms) {
+    if (cols <= 4096) return cols <= 128 * 24 ? ring(norm_ring_kernel<128, 6>, 128, 6) : ring(norm_ring_kernel<128, 8>, 128, 8);
+    if (cols <= 8192) return cols <= 256 * 24 ? ring(norm_ring_kernel<256, 6>, 256, 6) : ring(norm_ring_kernel<256, 8>, 256, 8);
+    return cols <= 512 * 24 ? ring(norm_ring_kernel<512, 6>, 512, 6) : ring(norm_ring_kernel<512, 8>, 512, 8);
+  }
   const bool few = rows <= 2 * sms, little = rows * cols < (4ull << 20);
   if (cols <= 8192) {
     const unsigned each = few && cols <= 4096 ? 4 : little ? 8 : vectors && cols >= 4096 ? 32 : 16;
