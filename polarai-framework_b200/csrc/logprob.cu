@@ -137,12 +137,15 @@ constexpr uint32_t kPlaced = 48;                           // as many a part of 
 __device__ __forceinline__ float float_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
 // The largest bound, nearly, that `top` of the LANES N keys of neighbouring lanes of a warp reach (all lanes take part; each group finds its
-// own).  Keys of kLowest count for vectors not met; with fewer keys than `top` that is the bound, and everything reaches it.
-template <int LANES, int N>
+// own).  Keys of kLowest count for vectors not met; with fewer keys than `top` that is the bound, and everything reaches it.  Found by halving, the first
+// BY_VALUE steps by value, where numbers of a short row are told apart sooner (60000 x 400 with 20 alternatives: 92 us, without 107, since the steps
+// by order go through all the powers of two down to zero); by order it takes 32 steps at most, whatever the numbers are.
+template <int BY_VALUE, int LANES, int N>
 __device__ __forceinline__ float bound_of(const uint32_t (&key)[N], uint32_t top) {
-  uint32_t most = 0, least = ~0u;
+  const uint32_t lowest = ordered(kLowest);
+  uint32_t most = 0;
 #pragma unroll
-  for (int i = 0; i < N; ++i) most = max(most, key[i]), least = min(least, key[i]);
+  for (int i = 0; i < N; ++i) most = max(most, key[i]);
   if (top <= kFewTop && top <= LANES) {                    // few: the largest key of the lanes, the next, ...
     uint32_t mine = most, largest = 0;
     for (uint32_t k = 0; k < top; ++k) {
@@ -157,20 +160,27 @@ __device__ __forceinline__ float bound_of(const uint32_t (&key)[N], uint32_t top
     }
     return float_of(max(largest, ordered(kLowest)));
   }
+  // the numbers met, the largest and the least of them
+  uint32_t least = ~0u, met = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) least = min(least, key[i] > lowest ? key[i] : ~0u), met += key[i] > lowest;
   if (LANES == 32) {
     most = __reduce_max_sync(0xffffffffu, most);
     least = __reduce_min_sync(0xffffffffu, least);
+    met = __reduce_add_sync(0xffffffffu, met);
   } else {
 #pragma unroll
     for (int off = LANES / 2; off > 0; off >>= 1) {
       most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
       least = min(least, __shfl_xor_sync(0xffffffffu, least, off));
+      met += __shfl_xor_sync(0xffffffffu, met, off);
     }
   }
   // `top` or more reach lo, fewer reach hi + 1
-  uint32_t lo = LANES * N >= kMaxTop || LANES * N >= top ? least : ordered(kLowest), hi = max(most, lo);
-  while (LANES == 32 ? lo < hi : __any_sync(0xffffffffu, lo < hi)) {
-    const uint32_t mid = hi - (hi - lo) / 2;
+  uint32_t lo = met < top ? lowest : least, hi = met < top ? lowest : most;
+  for (int step = 0; LANES == 32 ? lo < hi : __any_sync(0xffffffffu, lo < hi); ++step) {
+    uint32_t mid = hi - (hi - lo) / 2;
+    if (step < BY_VALUE) mid = min(max(ordered(0.5f * float_of(lo) + 0.5f * float_of(hi)), lo + 1), hi);
     uint32_t n = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) n += key[i] >= mid;
@@ -399,7 +409,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_wide_kernel(c
       for (uint32_t j = 128; j < THREADS; j += 128) k[i] = max(k[i], keys[turn][j + 32 * i + lane]);
     }
     turn ^= 1;
-    return bound_of<32>(k, o.top);
+    return bound_of<0, 32>(k, o.top);
   };
   float maxima[kInFlight];
   const uint32_t chunks = (row.vectors + kInFlight * stride - 1) / (kInFlight * stride);
@@ -499,19 +509,21 @@ __global__ void __launch_bounds__(kThreads) logprob_warp_kernel(const float* log
   __syncwarp();
   auto find_bound = [&](const float (&maxima)[kInFlight], float, const float4 (&v)[kInFlight], bool all_of_it) {
     if (o.top > kFewTop && classes <= kPlaced) return kLowest;
-    if (o.top > kFewTop && all_of_it) {                    // the row is here: a bound of its elements, which few more than `top` reach
+    // Where the row is here and has few vectors beside `top`, a bound of its elements, which few more than `top` reach (60000 x 200 with 32: 73 us, of
+    // the vectors' maxima 85; x 400 with 20 92 and 76)
+    if (o.top > kFewTop && all_of_it && classes < 8 * o.top) {
       uint32_t k[4 * kInFlight];
 #pragma unroll
       for (int u = 0; u < kInFlight; ++u) {
         k[4 * u] = ordered(fmaxf(v[u].x, kLowest)), k[4 * u + 1] = ordered(fmaxf(v[u].y, kLowest));
         k[4 * u + 2] = ordered(fmaxf(v[u].z, kLowest)), k[4 * u + 3] = ordered(fmaxf(v[u].w, kLowest));
       }
-      return bound_of<LANES>(k, o.top);
+      return bound_of<6, LANES>(k, o.top);
     }
     uint32_t k[kInFlight];
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) k[u] = ordered(maxima[u]);
-    return bound_of<LANES>(k, o.top);
+    return bound_of<6, LANES>(k, o.top);
   };
   float maxima[kInFlight];
   // (rows that begin elsewhere on a boundary may have a vector more or less: as many chunks as the longest; eight lanes have one)
@@ -778,7 +790,7 @@ int polar_b200_flogprob(const float* logits, uint64_t rows, uint64_t classes, ui
   // A warp per row as long as there are rows enough for every SM (20000 x 8192: 95 us against 104 with a CTA of 128 threads per row, with five
   // alternatives 131 and 162; 300 x 8000 with five 18.6 and 8.4; up to 1024 classes always).  Where there are more rows than six to an SM, as many
   // lanes to a short row as hold it in one chunk: 60000 x 100 7.6 us with 8 lanes, with a warp 20; x 200 14.2 with 16, with a warp 23, with twenty
-  // alternatives 62 and 91; but 300 x 100 with twenty 7.4 us with 8 lanes, 5.0 with a warp.
+  // alternatives 56 and, a warp then, 91; but 300 x 100 with twenty 7.4 us with 8 lanes, 5.0 with a warp.
   const uint64_t sms = (uint64_t)sm_count();
   if (classes <= 1024 || (classes <= 8192 && rows >= 16 * sms)) {
     const uint32_t lanes = rows <= 6 * sms ? 32 : classes <= 4 * kInFlight * 8 - 3 ? 8 : classes <= 4 * kInFlight * 16 - 3 ? 16 : 32;

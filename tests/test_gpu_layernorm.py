@@ -236,3 +236,27 @@ def test_two_streams_and_a_captured_call(env):
                 graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for o in outs for a, b in zip(o, want))
+
+
+@pytest.mark.parametrize("rows,cols", [(700, 9001), (300, 20000), (2400, 2050)])
+def test_long_rows_captured_and_on_two_streams(env, rows, cols):
+    torch, d = env
+    x, g, gamma, beta = inputs(torch, rows, cols)
+
+    def call(o):
+        d.flayernorm(x, gamma, beta, EPS, *o[:3])
+        d.flayernorm_grad(g, x, gamma, o[1], o[2], *o[3:])
+
+    new = lambda: [torch.zeros_like(t) for t in (x, x[:, 0].contiguous(), x[:, 0].contiguous(), x, gamma, beta)]  # noqa: E731
+    captured, got = new(), [new(), new()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):                            # (before any other call of this shape)
+        call(captured)
+    torch.cuda.synchronize()
+    for o in got:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(3):
+                call(o)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for o in got for a, b in zip(o, captured))
