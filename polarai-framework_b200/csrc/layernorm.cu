@@ -284,8 +284,8 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const float* in, const f
 
 // ---- backward ---------------------------------------------------------------------------------------
 // One pass over the rows: a team walks over rows (its CTA or cluster, over every gridDim.x-th group of them), the weights' gradients of its
-// columns in registers.  The rows come through a ring in shared memory, STAGES - 1 of them on their way while one is computed, by asynchronous
-// copies that each thread makes and waits for by itself: what it copies is what it reads, so no barrier is needed but the one of the row's sums.
+// columns in registers (65536 x 4096: 520 us, 6.2 TB/s; 2001 x 1511, a few rows to a team: 13.3).  The rows come through a ring in shared memory,
+// STAGES - 1 of them on their way while one is computed, by asynchronous copies that each thread makes and waits for by itself: what it copies is what it reads, so no barrier is needed but the one of the row's sums.
 // The sums over the team's rows go to `partials` [CTAs or clusters][2][cols], which a second kernel adds in order.
 template <int LANES>
 constexpr int kBlockOf = LANES > kThreads ? LANES : kThreads;   // threads of a CTA
@@ -445,20 +445,22 @@ __global__ void __launch_bounds__(kBlockOf<LANES>, 512 / kBlockOf<LANES>) norm_g
       S::store(g, to, member, live);
       unpack(dbeta);
       S::store(g, to + cols, member, live);
-    } else {                                               // the groups' sums meet in the ring: [groups][columns]
+    } else {                                               // the groups' sums meet in the ring: [dGamma, dBeta][groups][columns]
+      constexpr int kWidth = LANES * N;
       copies_wait<0>();
+      __syncthreads();
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
         unpack(which ? dbeta : dgamma);
-        __syncthreads();
 #pragma unroll
-        for (int k = 0; k < N; ++k) ring[group * (LANES * N) + (VECTOR ? 4 * (member + LANES * (k / 4)) + k % 4 : member + LANES * k)] = g[k];
-        __syncthreads();
-        for (uint32_t c = tid; c < cols; c += kBlock) {
-          float sum = 0.f;
-          for (int q = 0; q < kGroups; ++q) sum += ring[q * (LANES * N) + c];
-          to[(uint64_t)which * cols + c] = sum;
-        }
+        for (int k = 0; k < N; ++k)
+          ring[(which * kGroups + group) * kWidth + (VECTOR ? 4 * (member + LANES * (k / 4)) + k % 4 : member + LANES * k)] = g[k];
+      }
+      __syncthreads();
+      for (uint32_t c = tid; c < cols; c += kBlock) {
+        float sum[2] = {0.f, 0.f};
+        for (int q = 0; q < kGroups; ++q) sum[0] += ring[q * kWidth + c], sum[1] += ring[(kGroups + q) * kWidth + c];
+        to[c] = sum[0], to[(uint64_t)cols + c] = sum[1];
       }
     }
   }
@@ -507,27 +509,34 @@ __global__ void __launch_bounds__(kThreads) norm_grad_columns_kernel(const float
   partials[(2ull * blockIdx.y + 1) * cols + c] = db;
 }
 
-// The partial sums of `parts` stretches of rows: a warp per stretch of 32 columns and every 32nd part, then the warps' sums by columns.
+// The partial sums of `parts` stretches of rows: COLS columns to a CTA, every (1024 / COLS)th part to a thread, then the threads' sums by columns.
 constexpr int kFinishThreads = 1024;
+template <int COLS>
 __global__ void __launch_bounds__(kFinishThreads) norm_grad_finish_kernel(const float* partials, uint32_t parts, uint64_t cols, float* dgamma,
                                                                           float* dbeta) {
-  __shared__ float tile[32][33];
+  constexpr int kRows = kFinishThreads / COLS;
+  __shared__ float tile[kRows][COLS + 1];
   pdl_enter();
   float* out = blockIdx.y ? dbeta : dgamma;
   if (!out) return;
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint64_t c = (uint64_t)blockIdx.x * 32 + lane;
+  const uint32_t row = threadIdx.x / COLS, col = threadIdx.x % COLS;
+  const uint64_t c = (uint64_t)blockIdx.x * COLS + col;
   float s = 0.f;
   if (c < cols) {
-    const float* q = partials + (2ull * warp + blockIdx.y) * cols + c;
-    const uint64_t step = 64 * cols;                       // two rows of sums for each of the CTA's warps
+    const float* q = partials + (2ull * row + blockIdx.y) * cols + c;
+    const uint64_t step = 2ull * kRows * cols;             // two rows of sums for each part
 #pragma unroll 8
-    for (uint32_t p = warp; p < parts; p += 32, q += step) s += *q;   // (eight loads on their way)
+    for (uint32_t p = row; p < parts; p += kRows, q += step) s += *q;   // (eight loads on their way)
   }
-  tile[warp][lane] = s;
+  tile[row][col] = s;
   __syncthreads();
-  s = warp_sum(tile[lane][warp]);
-  if (lane == 0 && (uint64_t)blockIdx.x * 32 + warp < cols) out[(uint64_t)blockIdx.x * 32 + warp] = s;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp >= COLS) return;
+  s = 0.f;
+#pragma unroll
+  for (int r = 0; r < kRows; r += 32) s += tile[r + lane][warp];
+  s = warp_sum(s);
+  if (lane == 0 && (uint64_t)blockIdx.x * COLS + warp < cols) out[(uint64_t)blockIdx.x * COLS + warp] = s;
 }
 
 constexpr uint64_t kMaxCols = 1ull << 31, kMaxRows = 0x7fffffffull;
@@ -756,9 +765,14 @@ int polar_b200_flayernorm_grad(const float* gradient, const float* in, const flo
     rc = launch("flayernorm_grad_columns", norm_grad_columns_kernel, dim3((unsigned)((cols + kThreads - 1) / kThreads), parts), kThreads, 0, st,
                 gradient, in, mean, rstd, rows, cols, (rows + parts - 1) / parts, partials);
   }
-  if (rc == POLAR_B200_OK && partials)
-    rc = launch("flayernorm_grad_sum", norm_grad_finish_kernel, dim3((unsigned)((cols + 31) / 32), 2), kFinishThreads, 0, st, partials, parts, cols,
-                dgamma, dbeta);
+  if (rc == POLAR_B200_OK && partials) {
+    // Few columns: 16 to a CTA, and so half the loads one after the other (4000 x 300 in all 7.6 us, with 32 8.5; 8000 x 1000 21.2 and 20.1, where more
+    // CTAs are more rows of 64 bytes at a time)
+    auto go = [&](auto kernel, unsigned each) {
+      return launch("flayernorm_grad_sum", kernel, dim3((unsigned)((cols + each - 1) / each), 2), kFinishThreads, 0, st, partials, parts, cols, dgamma, dbeta);
+    };
+    rc = cols <= 5 * (uint64_t)sm_count() ? go(norm_grad_finish_kernel<16>, 16) : go(norm_grad_finish_kernel<32>, 32);
+  }
   if (rc == POLAR_B200_OK && !plan.lanes)                  // (last: din may be gradient or in)
     rc = launch("flayernorm_grad", norm_grad_in_kernel, dim3((unsigned)rows), kThreads, 0, st, gradient, in, gamma, mean, rstd, cols, din);
   if (own) {
