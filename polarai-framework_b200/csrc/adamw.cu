@@ -3,7 +3,7 @@
 // HBM-bound: with moments in 32 bits a weight reads 16 bytes (weight, gradient, two moments) and writes 12; with moments in
 // 8 bits it reads 10 and writes 6, and a block of 128 weights reads and writes two scales.  All tensors of a kind share a launch: a CTA finds
 // its chunk's tensor in a table among the kernel's parameters.  One chunk per CTA: loops over several measured 10 to 20 % slower.
-// Measured, 235 M weights in 163 tensors: 943 us in 32 bits (7.0 TB/s), 617 us in 8 (6.1 TB/s; issue slots 69 % busy).
+// Measured, 235 M weights in 163 tensors: 943 us in 32 bits (7.0 TB/s), 606 us in 8 (6.2 TB/s; issue slots 69 % busy); 113 small ones 3.5 us.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -58,13 +58,19 @@ __device__ __forceinline__ Rates rates_of(const Common& c, float decay) {
   const float step = c.schedule[0], lr = c.schedule[1];
   return Rates{1.f - lr * decay, lr / -expm1f(step * c.log_beta1), 1.f / sqrtf(-expm1f(step * c.log_beta2))};
 }
-// The tensor that a chunk belongs to.
+// The tensor that a chunk belongs to: in each round the begins of seven at a time, which are read together (235 M weights in 163 tensors, moments in 8 bits: 606 us, one
+// after the other 620).  The places behind the last tensor hold the largest number.
 template <int N>
 __device__ __forceinline__ uint32_t tensor_of(const Table<N>& t, uint32_t chunk) {
   uint32_t at = 0;
 #pragma unroll
-  for (uint32_t step = N > 256 ? 256 : N > 128 ? 128 : N / 2; step > 0; step /= 2)
-    if (at + step < t.count && t.first[at + step] <= chunk) at += step;
+  for (uint32_t step = N > 64 ? 64 : 8; step > 0; step /= 8) {
+    uint32_t more = 0;
+#pragma unroll
+    for (uint32_t k = 1; k < 8; ++k)
+      if (k * step < N) more += at + k * step < N && t.first[at + k * step] <= chunk;
+    at += more * step;
+  }
   return at;
 }
 
@@ -78,7 +84,7 @@ __device__ __forceinline__ float new_weight(const Common& c, const Rates& r, flo
   return w * r.keep - r.rate * __fdividef(m, root * r.inv_root2 + c.eps);
 }
 
-// Moments in 32 bits: a chunk of kThreads x UNROLL vectors of four weights per CTA.
+// Moments in 32 bits: a chunk of kThreads vectors of four weights per CTA.
 constexpr int kThreads = 256;
 __device__ __forceinline__ void step4(const Common& c, const Rates& r, float4& w, const float4& g, float4& m, float4& v) {
   float* wp = &w.x;
@@ -91,43 +97,48 @@ __device__ __forceinline__ void step4(const Common& c, const Rates& r, float4& w
     wp[k] = new_weight(c, r, wp[k], mp[k], __fsqrt_rn(vp[k]));
   }
 }
-template <int N, int UNROLL>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<N> table) {
+template <int N>
+__global__ void __launch_bounds__(kThreads, 6) adamw_kernel(const __grid_constant__ Table<N> table) {
   pdl_enter();
   const Common& c = table.c;
   const uint32_t at = tensor_of(table, blockIdx.x);
   const Tensor& t = table.tensor[at];
   float *first = static_cast<float*>(t.first), *second = static_cast<float*>(t.second);
-  const uint64_t begin = (uint64_t)(blockIdx.x - table.first[at]) * (kThreads * UNROLL * 4);
+  const uint64_t begin = (uint64_t)(blockIdx.x - table.first[at]) * (kThreads * 4);
   const bool vectors = ((reinterpret_cast<uintptr_t>(t.weights) | reinterpret_cast<uintptr_t>(t.gradient) | reinterpret_cast<uintptr_t>(first) |
                          reinterpret_cast<uintptr_t>(second)) & 15) == 0;
-  if (vectors && begin + kThreads * UNROLL * 4 <= t.count) {
-    const uint64_t i = begin / 4 + threadIdx.x;
-    float4 w[UNROLL], g[UNROLL], m[UNROLL], v[UNROLL];
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      w[u] = ld_stream(reinterpret_cast<const float4*>(t.weights) + i + u * kThreads);
-      g[u] = ld_stream(reinterpret_cast<const float4*>(t.gradient) + i + u * kThreads);
-      m[u] = ld_stream(reinterpret_cast<const float4*>(first) + i + u * kThreads);
-      v[u] = ld_stream(reinterpret_cast<const float4*>(second) + i + u * kThreads);
-    }
-    const Rates r = rates_of(c, t.decay);
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      step4(c, r, w[u], g[u], m[u], v[u]);
-      st_stream(reinterpret_cast<float4*>(t.weights) + i + u * kThreads, w[u]);
-      st_stream(reinterpret_cast<float4*>(first) + i + u * kThreads, m[u]);
-      st_stream(reinterpret_cast<float4*>(second) + i + u * kThreads, v[u]);
-    }
+  const uint64_t i = begin + (vectors ? 4 * threadIdx.x : threadIdx.x);
+  if (vectors && i + 4 <= t.count) {
+    float4 w = ld_stream(reinterpret_cast<const float4*>(t.weights + i));
+    const float4 g = ld_stream(reinterpret_cast<const float4*>(t.gradient + i));
+    float4 m = ld_stream(reinterpret_cast<const float4*>(first + i)), v = ld_stream(reinterpret_cast<const float4*>(second + i));
+    step4(c, rates_of(c, t.decay), w, g, m, v);
+    st_stream(reinterpret_cast<float4*>(t.weights + i), w);
+    st_stream(reinterpret_cast<float4*>(first + i), m);
+    st_stream(reinterpret_cast<float4*>(second + i), v);
     return;
   }
-  const Rates r = rates_of(c, t.decay);                    // the last chunk of a tensor, or one on odd boundaries
-  const uint64_t end = begin + kThreads * UNROLL * 4 < t.count ? begin + kThreads * UNROLL * 4 : t.count;
-  for (uint64_t i = begin + threadIdx.x; i < end; i += kThreads) {
-    const float g = t.gradient[i], m = new_first(c, first[i], g), v = new_second(c, second[i], g);
-    first[i] = m;
-    second[i] = v;
-    t.weights[i] = new_weight(c, r, t.weights[i], m, __fsqrt_rn(v));
+  // the last few of a tensor, or tensors on odd boundaries: four floats of each, eight loads on their way (sixteen take registers that more threads
+  // would use: 943 us, 957)
+  const Rates r = rates_of(c, t.decay);
+  const uint32_t step = vectors ? 1 : kThreads;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    float w[2], g[2], m[2], v[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint64_t e = i + (2 * half + k) * step;
+      const bool live = e < t.count;
+      w[k] = live ? t.weights[e] : 0.f, g[k] = live ? t.gradient[e] : 0.f, m[k] = live ? first[e] : 0.f, v[k] = live ? second[e] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint64_t e = i + (2 * half + k) * step;
+      if (e >= t.count) return;
+      first[e] = m[k] = new_first(c, m[k], g[k]);
+      second[e] = v[k] = new_second(c, v[k], g[k]);
+      t.weights[e] = new_weight(c, r, w[k], m[k], __fsqrt_rn(v[k]));
+    }
   }
 }
 
@@ -242,24 +253,32 @@ __global__ void __launch_bounds__(kThreads, 5) adamw8_kernel(const __grid_consta
   const Rates r = rates_of(c, t.decay);                    // the last blocks of a tensor, or blocks on odd boundaries
   for (uint64_t b = block; b < block + UNROLL && b * kBlock < t.count; ++b) {
     const uint64_t i = b * kBlock + 4 * lane;
-    float w[4], g[4];
+    const bool whole = vectors && i + 4 <= t.count;
+    float4 w, g;
     Codes q = {0, 0, t.first_scales[b], t.second_scales[b]};
+    if (whole) {
+      w = *reinterpret_cast<const float4*>(t.weights + i), g = *reinterpret_cast<const float4*>(t.gradient + i);
+      q.first = *reinterpret_cast<const uint32_t*>(first + i), q.second = *reinterpret_cast<const uint32_t*>(second + i);
+    } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const bool live = i + k < t.count;
-      w[k] = live ? t.weights[i + k] : 0.f;
-      g[k] = live ? t.gradient[i + k] : 0.f;
-      q.first |= (live ? (uint32_t)first[i + k] : 0u) << 8 * k;
-      q.second |= (live ? (uint32_t)second[i + k] : 0u) << 8 * k;
+      for (int k = 0; k < 4; ++k) {
+        const bool live = i + k < t.count;
+        (&w.x)[k] = live ? t.weights[i + k] : 0.f;
+        (&g.x)[k] = live ? t.gradient[i + k] : 0.f;
+        q.first |= (live ? (uint32_t)first[i + k] : 0u) << 8 * k;
+        q.second |= (live ? (uint32_t)second[i + k] : 0u) << 8 * k;
+      }
     }
-    float4 w4 = make_float4(w[0], w[1], w[2], w[3]);
-    const float4 g4 = make_float4(g[0], g[1], g[2], g[3]);
-    step4(c, r, w4, g4, q);
-    w[0] = w4.x, w[1] = w4.y, w[2] = w4.z, w[3] = w4.w;
+    __syncwarp();
+    step4(c, r, w, g, q);
+    if (whole) {
+      *reinterpret_cast<float4*>(t.weights + i) = w;
+      *reinterpret_cast<uint32_t*>(first + i) = q.first, *reinterpret_cast<uint32_t*>(second + i) = q.second;
+    }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if (i + k >= t.count) continue;
-      t.weights[i + k] = w[k];
+      if (whole || i + k >= t.count) continue;
+      t.weights[i + k] = (&w.x)[k];
       first[i + k] = (uint8_t)(q.first >> 8 * k);
       second[i + k] = (uint8_t)(q.second >> 8 * k);
     }
@@ -289,10 +308,11 @@ int launch_table(const polar_b200_adamw_tensor* tensors, uint64_t count, bool ei
   }
   *taken = i;
   if (table.count == 0) return POLAR_B200_OK;
+  std::fill(table.first + table.count, table.first + N, 0xffffffffu);
   // moments in 8 bits: two blocks per warp in flight (one is a fifth slower, four the same within 3 %); in 32 bits one vector per thread and
   // more threads (943 us, two 949)
   if constexpr (UNROLL == 2) return launch_large("fadamw8", adamw8_kernel<N, 2>, dim3((unsigned)chunks), kThreads, stream, table);
-  else return launch_large("fadamw", adamw_kernel<N, 1>, dim3((unsigned)chunks), kThreads, stream, table);
+  else return launch_large("fadamw", adamw_kernel<N>, dim3((unsigned)chunks), kThreads, stream, table);
 }
 
 // Whether no two of the arrays that a step writes share memory, nor one of them with a gradient: two threads would race on it.  (A tensor's
