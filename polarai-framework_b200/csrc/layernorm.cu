@@ -284,11 +284,13 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const float* in, const f
 
 // ---- backward ---------------------------------------------------------------------------------------
 // One pass over the rows: a team walks over rows (its CTA or cluster, over every gridDim.x-th group of them), the weights' gradients of its
-// columns in registers (65536 x 4096: 520 us, 6.2 TB/s; 2001 x 1511, a few rows to a team: 13.3).  The rows come through a ring in shared memory,
+// columns in registers (65536 x 4096: 520 us, 6.2 TB/s; 2001 x 1511, a few rows to a team: 12.5).  The rows come through a ring in shared memory,
 // STAGES - 1 of them on their way while one is computed, by asynchronous copies that each thread makes and waits for by itself: what it copies is what it reads, so no barrier is needed but the one of the row's sums.
 // The sums over the team's rows go to `partials` [CTAs or clusters][2][cols], which a second kernel adds in order.
+// Threads of a CTA: several teams where they are small, as many as an SM's registers take.
+constexpr int block_of(int lanes) { return lanes == 96 || lanes == 160 ? 480 : lanes == 224 ? 448 : lanes > kThreads ? lanes : kThreads; }
 template <int LANES>
-constexpr int kBlockOf = LANES > kThreads ? LANES : kThreads;   // threads of a CTA
+constexpr int kBlockOf = block_of(LANES);
 // A barrier of a team and the sums over it, in every thread, where several teams share a CTA (`group`: the team's number; `slots`: 2 for each warp).
 template <int LANES>
 __device__ __forceinline__ void team_barrier(uint32_t group) {
@@ -308,7 +310,7 @@ __device__ __forceinline__ void grad_sums(float (&v)[2], float* slots, uint32_t 
   const float* mine = slots + 2 * group * kWarps;
   v[0] = lane < kWarps ? mine[2 * lane] : 0.f, v[1] = lane < kWarps ? mine[2 * lane + 1] : 0.f;
 #pragma unroll
-  for (int off = kWarps / 2; off > 0; off >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], off), v[1] += __shfl_xor_sync(0xffffffffu, v[1], off);
+  for (int off = kWarps > 8 ? 8 : kWarps > 4 ? 4 : kWarps > 2 ? 2 : 1; off > 0; off >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], off), v[1] += __shfl_xor_sync(0xffffffffu, v[1], off);
   v[0] = __shfl_sync(0xffffffffu, v[0], 0), v[1] = __shfl_sync(0xffffffffu, v[1], 0);
 }
 template <int LANES, int V, bool VECTOR, int CTAS, int STAGES>
@@ -316,7 +318,7 @@ __global__ void __launch_bounds__(kBlockOf<LANES>, 512 / kBlockOf<LANES>) norm_g
     const float* gradient, const float* in, const float* gamma, const float* mean, const float* rstd, uint32_t rows, uint32_t cols, float per_col,
     float* din, float* partials) {
   constexpr int kBlock = kBlockOf<LANES>, kGroups = kBlock / LANES, N = 4 * V;
-  // (the plan doubles LANES only for rows beyond half of it, so half of the fours are full, except for a cluster's last CTA and the shortest rows)
+  // (a team has columns for more than half of its places, so half of the fours are full, except for a cluster's last CTA and the shortest rows)
   constexpr int FULL = CTAS == 1 ? V / 2 : 0;
   using S = Share<LANES, V, VECTOR, FULL>;
   // VECTOR: [STAGES][gradient, in][V][kBlock] vectors, of which a thread copies and reads its own.  Else rows are copied as they lie, vectors from
@@ -553,19 +555,29 @@ constexpr uint64_t kOnePassCols = 65536;
 struct GradPlan {
   unsigned lanes, v, ctas, grid;
 };
-GradPlan grad_plan(uint64_t rows, uint64_t cols) {
+GradPlan grad_plan(uint64_t rows, uint64_t cols, bool vectors) {
   if (cols > kOnePassCols) return GradPlan{0, 0, 0, 0};
   GradPlan p{8, 4, 1, 0};
   if (cols <= 32) p.v = 1;
   else if (cols <= 64) p.v = 2;
   while ((uint64_t)p.lanes * p.v * 4 < cols && p.lanes < 512) p.lanes *= 2;
+  // Rows that are read as single floats pay for every place of a team that has no column, so theirs are teams of any number of warps (65536 x 1511:
+  // 193 us in five teams of 96 lanes, 222 in four of 128; 30000 x 2101 138 and 193; 10000 x 5001 133 and 155; where rows are vectors smaller CTAs are
+  // better: 65536 x 1280 153 and, in teams of 96, 163).  Few rows take more, smaller CTAs (40 x 1511: 5.2, 6.4).
+  const uint64_t sms = (uint64_t)sm_count();
+  if (!vectors && rows > 2 * sms)
+    for (const unsigned lanes : {96u, 160u, 224u, 320u, 384u, 448u})
+      if (p.lanes > lanes && p.lanes < 2 * lanes && cols <= lanes * 16) {
+        p.lanes = lanes;
+        break;
+      }
   if (cols > 8192) {
     p.lanes = cols <= 32768 ? 256 : 512;
     p.ctas = (unsigned)((cols + p.lanes * p.v * 4 - 1) / (p.lanes * p.v * 4));
   }
   // 512 threads on an SM, with three stages of up to 64 KB; where there are many rows, some for each CTA, so that the partial sums are few beside
   // them (3 x 7560: 7.2 us with a CTA per row, 8.5 with one for two)
-  const uint64_t sms = (uint64_t)sm_count(), block = p.lanes > kThreads ? p.lanes : kThreads, groups = (rows * p.lanes + block - 1) / block;
+  const uint64_t block = block_of((int)p.lanes), teams = block / p.lanes, groups = (rows + teams - 1) / teams;
   const uint64_t most = sms * (512 / block) / p.ctas, wanted = groups <= sms ? groups : (groups + 1) / 2;
   p.grid = (unsigned)(wanted < most ? wanted : most);
   return p;
@@ -693,8 +705,8 @@ int polar_b200_flayernorm(const float* in, const float* gamma, const float* beta
 
 uint64_t polar_b200_flayernorm_grad_workspace_bytes(uint64_t rows, uint64_t cols) {
   if (rows == 0 || cols == 0 || rows > kMaxRows || cols > kMaxCols) return 0;
-  const GradPlan p = grad_plan(rows, cols);
-  return (p.lanes ? p.grid : stretches(rows)) * 2 * cols * sizeof(float);
+  const unsigned grid = std::max(grad_plan(rows, cols, true).grid, grad_plan(rows, cols, false).grid);   // (where the tensors lie is not known yet)
+  return (grid ? grid : stretches(rows)) * 2 * cols * sizeof(float);
 }
 
 int polar_b200_flayernorm_grad(const float* gradient, const float* in, const float* gamma, const float* mean, const float* rstd,
@@ -712,7 +724,8 @@ int polar_b200_flayernorm_grad(const float* gradient, const float* in, const flo
   LaunchDeviceScope on(stream, din);
   cudaStream_t st = as_stream(stream);
   int rc = POLAR_B200_OK;
-  GradPlan plan = grad_plan(rows, cols);
+  const bool vectors = (cols & 3) == 0 && aligned16(gradient) && aligned16(in) && aligned16(gamma) && aligned16(din);
+  GradPlan plan = grad_plan(rows, cols, vectors);
   const uint64_t need = polar_b200_flayernorm_grad_workspace_bytes(rows, cols);
   void* own = nullptr;
   float* partials = nullptr;
@@ -727,17 +740,23 @@ int polar_b200_flayernorm_grad(const float* gradient, const float* in, const flo
   }
   uint32_t parts = 0;
   if (plan.lanes) {
-    const bool vectors = (cols & 3) == 0 && aligned16(gradient) && aligned16(in) && aligned16(gamma) && aligned16(din);
     auto go = [&](auto with, auto without) {
       return (vectors ? with : without)(plan, st, gradient, in, gamma, mean, rstd, rows, cols, din, partials);
     };
 #define ROWS(LANES, V, CTAS) go(launch_grad_rows<LANES, V, true, CTAS>, launch_grad_rows<LANES, V, false, CTAS>)
+#define FLOATS(LANES) launch_grad_rows<LANES, 4, false, 1>(plan, st, gradient, in, gamma, mean, rstd, rows, cols, din, partials)
     switch (plan.lanes) {
       case 8: rc = plan.v == 1 ? ROWS(8, 1, 1) : plan.v == 2 ? ROWS(8, 2, 1) : ROWS(8, 4, 1); break;
       case 16: rc = ROWS(16, 4, 1); break;
       case 32: rc = ROWS(32, 4, 1); break;
       case 64: rc = ROWS(64, 4, 1); break;
       case 128: rc = ROWS(128, 4, 1); break;
+      case 96: rc = FLOATS(96); break;
+      case 160: rc = FLOATS(160); break;
+      case 224: rc = FLOATS(224); break;
+      case 320: rc = FLOATS(320); break;
+      case 384: rc = FLOATS(384); break;
+      case 448: rc = FLOATS(448); break;
       case 256:
         switch (plan.ctas) {
           case 1: rc = ROWS(256, 4, 1); break;
@@ -759,6 +778,7 @@ int polar_b200_flayernorm_grad(const float* gradient, const float* in, const flo
         }
     }
     parts = plan.grid;                                     // (with clusters what is resident, which is less than planned)
+#undef FLOATS
 #undef ROWS
   } else if (partials) {
     parts = (uint32_t)stretches(rows);
