@@ -199,12 +199,14 @@ __device__ __forceinline__ void copy_image(float* to, const float* src, uint32_t
 // Forward, long rows that are not on 16-byte boundaries: an SM's CTAs stay and go through the rows with gamma and beta in their registers; two
 // rows are on their way while one is computed (8000 x 9001: 113 us, a cluster of two CTAs per row 265; 16384 x 16383: 343 and
 // 662; 8007 x 7830: 91, a CTA per row 110; 60000 x 2101: 170 and 214).
-constexpr int kRing = 3;
-template <int LANES, int V>
-__global__ void __launch_bounds__(LANES, 512 / LANES) norm_ring_kernel(const float* in, const float* gamma, const float* beta, float eps, uint32_t rows,
-                                                                       uint32_t cols, float per_col, float* out, float* mean_out, float* rstd_out) {
-  constexpr int N = 4 * V, kImage = LANES * N + 4;
-  using S = Share<LANES, V, false, V - 2>;                 // (cols > 4 LANES (V - 2))
+// HELD: gamma and beta are in registers; of rows beyond 16384 columns they are read for each row, and one row is on its way (5294 x 17287: 183 us, a
+// cluster of four CTAs per row 396; 300 x 17287 16.6 and 22.9).
+template <int LANES, int V, int FULL, bool HELD>
+__global__ void __launch_bounds__(LANES, LANES < 512 ? 512 / LANES : 1)
+    norm_ring_kernel(const float* in, const float* gamma, const float* beta, float eps, uint32_t rows, uint32_t cols, float per_col, float* out,
+                     float* mean_out, float* rstd_out) {
+  constexpr int N = 4 * V, kImage = LANES * N + 4, kRing = HELD ? 3 : 2;
+  using S = Share<LANES, V, false, FULL>;                  // (cols > 4 LANES FULL)
   extern __shared__ float4 images[];
   __shared__ float slots[2][LANES / 32];
   pdl_enter();
@@ -220,11 +222,13 @@ __global__ void __launch_bounds__(LANES, 512 / LANES) norm_ring_kernel(const flo
   };
 #pragma unroll
   for (int s = 0; s < kRing - 1; ++s) fetch();
-  float g[N], b[N];
+  float g[HELD ? N : 1], b[HELD ? N : 1];
+  if constexpr (HELD) {
 #pragma unroll
-  for (int k = 0; k < N; ++k) g[k] = 1.f, b[k] = 0.f;
-  if (gamma) S::load(g, gamma, member, live);
-  if (beta) S::load(b, beta, member, live);
+    for (int k = 0; k < N; ++k) g[k] = 1.f, b[k] = 0.f;
+    if (gamma) S::load(g, gamma, member, live);
+    if (beta) S::load(b, beta, member, live);
+  }
   for (; r < rows; r += gridDim.x) {
     copies_wait<kRing - 2>();
     __syncthreads();                                       // what other threads have copied is here, and all have read the row before
@@ -247,7 +251,20 @@ __global__ void __launch_bounds__(LANES, 512 / LANES) norm_ring_kernel(const flo
     block_sums<LANES>(s, slots[1]);
     const float rstd = rsqrtf(s[0] * per_col + eps);
 #pragma unroll
-    for (int k = 0; k < N; ++k) x[k] = x[k] * rstd * g[k] + b[k];
+    for (int k = 0; k < N; ++k) x[k] *= rstd;
+    if constexpr (HELD) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) x[k] = x[k] * g[k] + b[k];
+    } else {
+      if (gamma) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) x[k] *= k < 4 * FULL ? gamma[member + LANES * k] : ld_if(gamma + member + LANES * k, k, live);
+      }
+      if (beta) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) x[k] += k < 4 * FULL ? beta[member + LANES * k] : ld_if(beta + member + LANES * k, k, live);
+      }
+    }
     S::store(x, out + r * cols, member, live);
     if (member == 0) {
       if (mean_out) mean_out[r] = mean;
@@ -663,20 +680,24 @@ int polar_b200_flayernorm(const float* in, const float* gamma, const float* beta
   // (The number of elements per thread that a form is made for is its V: FULL fours of every thread are there without asking, so each form serves
   // cols > 4 LANES CTAS FULL only.)
   auto ring = [&](auto kernel, unsigned threads, unsigned v) {
-    const size_t bytes = kRing * (threads * v * 4 + 4) * sizeof(float);
+    const size_t bytes = (threads > 512 ? 2 : 3) * (size_t)(threads * v * 4 + 4) * sizeof(float);
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (e != cudaSuccess) return fail(POLAR_B200_ERR_CUDA, "cudaFuncSetAttribute(flayernorm)", e);
-    const uint64_t most = sms * (512 / threads);
+    const uint64_t most = sms * (threads < 512 ? 512 / threads : 1);
     return launch("flayernorm", kernel, dim3((unsigned)(rows < most ? rows : most)), threads, bytes, st, in, gamma, beta, eps, (uint32_t)rows,
                   (uint32_t)cols, (float)(1.0 / (double)cols), out, mean, rstd);
   };
   // (once every SM has its CTAs, and four rows for each of the smaller ones: 600 x 7830 9.6 us and 10.2, 300 x 7830 7.1 and 7.4, 3000 x 2501 13.4 and
   // 15.0; up to 2048 columns loads into registers do as well)
   if (!vectors && cols > 2048 && cols <= 16384 && rows >= (cols <= 4096 ? 16 : 4) * sms) {
-    if (cols <= 4096) return cols <= 128 * 24 ? ring(norm_ring_kernel<128, 6>, 128, 6) : ring(norm_ring_kernel<128, 8>, 128, 8);
-    if (cols <= 8192) return cols <= 256 * 24 ? ring(norm_ring_kernel<256, 6>, 256, 6) : ring(norm_ring_kernel<256, 8>, 256, 8);
-    return cols <= 512 * 24 ? ring(norm_ring_kernel<512, 6>, 512, 6) : ring(norm_ring_kernel<512, 8>, 512, 8);
+    if (cols <= 4096) return cols <= 128 * 24 ? ring(norm_ring_kernel<128, 6, 4, true>, 128, 6) : ring(norm_ring_kernel<128, 8, 6, true>, 128, 8);
+    if (cols <= 8192) return cols <= 256 * 24 ? ring(norm_ring_kernel<256, 6, 4, true>, 256, 6) : ring(norm_ring_kernel<256, 8, 6, true>, 256, 8);
+    return cols <= 512 * 24 ? ring(norm_ring_kernel<512, 6, 4, true>, 512, 6) : ring(norm_ring_kernel<512, 8, 6, true>, 512, 8);
   }
+  if (!vectors && cols > 16384 && cols <= 1024 * 28 && rows >= 2 * sms)   // (two rows fill the shared memory)
+    return cols <= 1024 * 20   ? ring(norm_ring_kernel<1024, 5, 4, false>, 1024, 5)
+           : cols <= 1024 * 24 ? ring(norm_ring_kernel<1024, 6, 5, false>, 1024, 6)
+                               : ring(norm_ring_kernel<1024, 7, 6, false>, 1024, 7);
   const bool few = rows <= 2 * sms, little = rows * cols < (4ull << 20);
   if (cols <= 8192) {
     const unsigned each = few && cols <= 4096 ? 4 : little ? 8 : vectors && cols >= 4096 ? 32 : 16;

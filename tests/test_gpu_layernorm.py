@@ -60,7 +60,8 @@ SIZES = [(1, 1), (3, 1), (5, 2), (4, 3), (33, 7), (70, 13), (9, 32), (5, 33), (1
          (17, 8192), (2, 9001), (3, 16384), (2, 16388), (2, 20001), (1, 32768), (2, 32772), (1, 70001),
          (2400, 2050), (2500, 3099), (2370, 4095), (600, 4101), (700, 6145), (900, 8191), (620, 8193), (610, 12289), (600, 16383),
          (200, 9001), (150, 24001), (90, 28010), (3, 45000), (2, 53001), (40, 60001),
-         (2001, 1511), (400, 1033), (310, 2101), (320, 2701), (310, 3583), (300, 4301), (350, 6001), (310, 7001)]
+         (2001, 1511), (400, 1033), (310, 2101), (320, 2701), (310, 3583), (300, 4301), (350, 6001), (310, 7001),
+         (300, 16385), (310, 20481), (300, 24577), (297, 28671)]
 
 
 @pytest.mark.parametrize("rows,cols", SIZES)
