@@ -663,6 +663,8 @@ int polar_b200_flayernorm(const float* in, const float* gamma, const float* beta
                            lanes > 32 ? lanes : kThreads, 0, st, ctas, in, gamma, beta, eps, (uint32_t)rows, (uint32_t)cols, (float)(1.0 / (double)cols), out, mean, rstd);
   };
 #define ROWS(LANES, V, FULL, CTAS) go(norm_rows_kernel<LANES, V, true, FULL, CTAS>, norm_rows_kernel<LANES, V, false, FULL, CTAS>, LANES, CTAS)
+#define VECTORS(LANES, V, FULL, CTAS) go(norm_rows_kernel<LANES, V, true, FULL, CTAS>, norm_rows_kernel<LANES, V, true, FULL, CTAS>, LANES, CTAS)
+#define FLOATS(LANES, V, FULL, CTAS) go(norm_rows_kernel<LANES, V, false, FULL, CTAS>, norm_rows_kernel<LANES, V, false, FULL, CTAS>, LANES, CTAS)
 #define LANES_OF(V)                       \
   switch (lanes) {                        \
     case 8: return ROWS(8, V, V - 1, 1);         \
@@ -671,8 +673,7 @@ int polar_b200_flayernorm(const float* in, const float* gamma, const float* beta
     case 64: return ROWS(64, V, V - 1, 1);       \
     case 128: return ROWS(128, V, V - 1, 1);     \
     case 256: return ROWS(256, V, V - 1, 1);     \
-    case 512: return ROWS(512, V, V - 1, 1);     \
-    default: return ROWS(1024, V, V - 1, 1);     \
+    default: return ROWS(512, V, V - 1, 1);      \
   }
   // How many elements a thread takes: 4 where there are few rows, for the shortest chain; 8 while the threads do not fill the SMs; then 16 and,
   // of long rows, 32, whose loads are all in flight at once (65536 x 4096 in teams of 128 threads: 312 us, of 256 314, of 512 403).
@@ -701,11 +702,12 @@ int polar_b200_flayernorm(const float* in, const float* gamma, const float* beta
   const bool few = rows <= 2 * sms, little = rows * cols < (4ull << 20);
   if (cols <= 8192) {
     const unsigned each = few && cols <= 4096 ? 4 : little ? 8 : vectors && cols >= 4096 ? 32 : 16;
-    if (vectors && !little && cols > 512 && cols <= 1024) return cols <= 640 ? ROWS(32, 5, 4, 1) : cols <= 768 ? ROWS(32, 6, 5, 1) : ROWS(32, 8, 6, 1);
+    if (vectors && !little && cols > 512 && cols <= 1024) return cols <= 640 ? VECTORS(32, 5, 4, 1) : cols <= 768 ? VECTORS(32, 6, 5, 1) : VECTORS(32, 8, 6, 1);
     unsigned lanes = 8;
     while (lanes * each < cols) lanes *= 2;
     const unsigned v = (unsigned)((cols + lanes - 1) / lanes + 3) / 4;
-    if (v > 4) return lanes == 128 ? (v > 6 ? ROWS(128, 8, 6, 1) : ROWS(128, 6, 4, 1)) : (v > 6 ? ROWS(256, 8, 6, 1) : ROWS(256, 6, 4, 1));
+    if (v > 4) return lanes == 128 ? VECTORS(128, 8, 6, 1) : v > 6 ? VECTORS(256, 8, 6, 1) : VECTORS(256, 6, 4, 1);
+    if (lanes == 1024) return v == 1 ? ROWS(1024, 1, 0, 1) : ROWS(1024, 2, 1, 1);
     if (v == 1) LANES_OF(1)
     if (v == 2) LANES_OF(2)
     if (v == 3) LANES_OF(3)
@@ -714,11 +716,13 @@ int polar_b200_flayernorm(const float* in, const float* gamma, const float* beta
   // Longer ones: a large CTA, clusters of CTAs where the row is beyond one or, as single floats, beyond its registers, and smaller shares in
   // larger clusters where there are few rows (1 x 32768: 4.3 us, one CTA 6.7).
   if (rows * 8 <= 2 * sms && cols > 16384 && cols <= 32768) return ROWS(512, 2, 0, 8);
-  if (!vectors && cols <= 65536) return cols <= 16384 ? ROWS(512, 4, 2, 2) : cols <= 32768 ? ROWS(512, 4, 2, 4) : ROWS(512, 4, 2, 8);
-  if (cols <= 16384) return ROWS(512, 8, 4, 1);
-  if (cols <= 32768) return ROWS(1024, 8, 4, 1);
-  if (cols <= 65536) return ROWS(1024, 8, 4, 2);
+  if (!vectors && cols <= 65536) return cols <= 16384 ? FLOATS(512, 4, 2, 2) : cols <= 32768 ? FLOATS(512, 4, 2, 4) : FLOATS(512, 4, 2, 8);
+  if (cols <= 16384) return VECTORS(512, 8, 4, 1);
+  if (cols <= 32768) return VECTORS(1024, 8, 4, 1);
+  if (cols <= 65536) return VECTORS(1024, 8, 4, 2);
 #undef LANES_OF
+#undef FLOATS
+#undef VECTORS
 #undef ROWS
   return launch("flayernorm", norm_kernel, dim3((unsigned)rows), kThreads, 0, as_stream(stream), in, gamma, beta, eps, cols, out, mean,
                 rstd);
