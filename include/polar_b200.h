@@ -367,6 +367,7 @@ uint64_t polar_b200_fdense_grad_workspace_bytes(uint64_t rows, uint64_t kh, uint
  *   out = (x - mean) * rstd * gamma + beta.
  * gamma and beta [cols] may be NULL (ones, zeros), mean and rstd [rows] too (not wanted); out may be in.
  * Sums are held in fp32 over two levels and more, and the deviations are summed around the mean.
+ * Up to 2^31 - 1 rows and 2^31 columns (as everywhere in this section).
  * As a builtin: T in[..., cols], T gamma, T beta, f32 eps, T out, T mean, T rstd (three results). */
 int polar_b200_flayernorm(const float* in, const float* gamma, const float* beta, float eps, uint64_t rows,
                           uint64_t cols, float* out, float* mean, float* rstd, void* stream);
