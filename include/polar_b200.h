@@ -366,7 +366,8 @@ uint64_t polar_b200_fdense_grad_workspace_bytes(uint64_t rows, uint64_t kh, uint
  *   mean = sum(x) / cols,  rstd = 1 / sqrt(sum((x - mean)^2) / cols + eps),
  *   out = (x - mean) * rstd * gamma + beta.
  * gamma and beta [cols] may be NULL (ones, zeros), mean and rstd [rows] too (not wanted); out may be in.
- * Sums are held in fp32 over two levels and more, and the deviations are summed around the mean.
+ * Sums are held in fp32 over two levels and more.  The deviations are taken around a mean that they correct once more, so
+ * that of a constant row nothing but beta is left, and a row far from zero loses no digits to its mean.
  * Up to 2^31 - 1 rows and 2^31 columns (as everywhere in this section).
  * As a builtin: T in[..., cols], T gamma, T beta, f32 eps, T out, T mean, T rstd (three results). */
 int polar_b200_flayernorm(const float* in, const float* gamma, const float* beta, float eps, uint64_t rows,

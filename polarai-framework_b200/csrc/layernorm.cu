@@ -41,7 +41,7 @@ __device__ __forceinline__ void st_if(float4* p, float4 v, int k, uint32_t live)
 // Of the V fours, all threads have the first FULL (cols >= 4 TEAM FULL); `live`: how many of the vectors or floats this thread has in all.
 template <int TEAM, int V, bool VECTOR, int FULL>
 struct Share {
-  static constexpr int N = 4 * V;
+  static constexpr int N = 4 * V, kFull = FULL;
   static __device__ __forceinline__ uint32_t live(uint32_t member, uint32_t cols) {
     const uint32_t first = VECTOR ? 4 * member : member, step = VECTOR ? 4 * TEAM : TEAM;
     return first < cols ? (cols - first + step - 1) / step : 0;
@@ -79,33 +79,126 @@ struct Share {
     }
   }
 };
-// Sums over the threads of a team: lanes side by side, or the CTA (`slots` as for block_sums).
-template <int TEAM, int N>
-__device__ __forceinline__ void team_sums(float (&v)[N], float* slots) {
+// The sum over the threads of a team: lanes side by side, or the CTA (`slots` as for block_sums).
+template <int TEAM>
+__device__ __forceinline__ void team_sum(float (&v)[1], float* slots) {
   if (TEAM > 32) {
     block_sums<TEAM < 32 ? 32 : TEAM>(v, slots);
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-      for (int off = TEAM / 2; off > 0; off >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], off);
+    for (int off = TEAM / 2; off > 0; off >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], off);
   }
 }
+// Two sums over the team: each half of the lanes takes one of them, which takes 6 exchanges in a warp where 10 would do both in every lane.
+template <int LANES>
+__device__ __forceinline__ float sum_by_halves(float a, float b) {   // the sum of a in the lower half of the lanes, of b in the upper
+  constexpr int kHalf = LANES / 2;
+  const bool upper = threadIdx.x & kHalf;
+  float v = (upper ? b : a) + __shfl_xor_sync(0xffffffffu, upper ? a : b, kHalf);
+#pragma unroll
+  for (int off = kHalf / 2; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
+}
+template <int TEAM>
+__device__ __forceinline__ void team_sums(float (&v)[2], float* slots) {
+  constexpr int kLanes = TEAM < 32 ? TEAM : 32, kWarps = TEAM < 32 ? 1 : TEAM / 32;
+  const bool upper = threadIdx.x & (kLanes / 2);
+  float s = sum_by_halves<kLanes>(v[0], v[1]);
+  if (TEAM > 32) {
+    const uint32_t at = threadIdx.x & 15;
+    if (at == 0) slots[(upper ? kWarps : 0) + (threadIdx.x >> 5)] = s;
+    __syncthreads();
+    const float* mine = slots + (upper ? kWarps : 0);
+    s = mine[at % kWarps];
+    if (kWarps > 16) s += mine[at + 16];
+#pragma unroll
+    for (int off = (kWarps < 16 ? kWarps : 16) / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+  }
+  const float other = __shfl_xor_sync(0xffffffffu, s, kLanes / 2);
+  v[0] = upper ? other : s, v[1] = upper ? s : other;
+}
 
-// The sum over the CTAs of a cluster, added in the same order in each of them.
-template <int CTAS>
-__device__ __forceinline__ float cluster_sum(float v, float* mine) {
-  if (CTAS == 1) return v;
-  if (threadIdx.x == 0) *mine = v;
+// The sums of one or two values over the CTAs of a cluster, added in the same order in each of them; `mine`: for them, not in use by anything else.
+template <int CTAS, int N>
+__device__ __forceinline__ void cluster_sums(float (&v)[N], double* mine) {
+  if (CTAS == 1) return;
+  float* own = reinterpret_cast<float*>(mine);
+  if (threadIdx.x == 0)
+#pragma unroll
+    for (int i = 0; i < N; ++i) own[i] = v[i];
   __syncthreads();
   cluster_arrive();
   cluster_wait();
-  float part[CTAS], s = 0.f;
+  float part[N][CTAS];
 #pragma unroll
-  for (int r = 0; r < CTAS; ++r) part[r] = ld_cluster(mine, (uint32_t)r);
+  for (int r = 0; r < CTAS; ++r) {
+    if (N == 1) {
+      part[0][r] = ld_cluster(own, (uint32_t)r);
+    } else {                                               // (both by one load: they are what a row waits for)
+      const long long both = __double_as_longlong(ld_cluster(mine, (uint32_t)r));
+      part[0][r] = __int_as_float((int)both), part[N - 1][r] = __int_as_float((int)(both >> 32));
+    }
+  }
 #pragma unroll
-  for (int r = 0; r < CTAS; ++r) s += part[r];
-  return s;
+  for (int i = 0; i < N; ++i) {
+    v[i] = 0.f;
+#pragma unroll
+    for (int r = 0; r < CTAS; ++r) v[i] += part[i][r];
+  }
+}
+
+// What the deviations d = x - m from a first mean m leave to do: the mean is m + c and the variance mean(d^2) - c^2 with c = mean(d), which takes the
+// first mean's rounding out of both.  (Of a row of 1000.3, whose sum is rounded, (x - m) / sqrt(eps) is 0.02; x - m is the same whole number of
+// steps in all of its columns, so c has to be exactly that: the product with 1 / cols is followed by what its rounding left.)
+struct Correction {
+  float c, var;
+  __device__ __forceinline__ Correction(float squares, float deviations, uint32_t cols, float per_col) {
+    c = __fmul_rn(deviations, per_col);
+    c = __fmaf_rn(__fmaf_rn(-c, (float)cols, deviations), per_col, c);
+    var = squares * per_col - c * c;
+    if (var < 0.f) var = 0.f;                              // (NaN stays)
+  }
+};
+
+template <int N>
+__device__ __forceinline__ void unpack(float (&v)[N], const Pair (&x)[N / 2]) {
+#pragma unroll
+  for (int k = 0; k < N / 2; ++k) v[2 * k] = halves(x[k]).x, v[2 * k + 1] = halves(x[k]).y;
+}
+// A team's row, as its threads have read it (zeros where a thread has no column), as pairs, and its mean but for rounding.
+template <int LANES, int CTAS, class S>
+__device__ __forceinline__ float first_mean(const float (&v)[S::N], Pair (&x)[S::N / 2], float per_col, float* slots, double* part) {
+  Pair sum = 0;
+#pragma unroll
+  for (int k = 0; k < S::N / 2; ++k) x[k] = pair(v[2 * k], v[2 * k + 1]), sum = add2(sum, x[k]);
+  float s[1] = {halves(sum).x + halves(sum).y};
+  team_sum<LANES>(s, slots);
+  cluster_sums<CTAS>(s, part);
+  return __fmul_rn(s[0], per_col);                         // (rounded by itself, as the mean that the deviations are around)
+}
+// The row's deviations from it, and what their sums leave to correct.
+template <int LANES, int CTAS, class S>
+__device__ __forceinline__ Correction deviations(Pair (&x)[S::N / 2], float first, uint32_t live, uint32_t cols, float per_col, float* slots, double* part) {
+  const Pair minus = pair(-first, -first);
+  Pair squares = 0, sum = 0;
+#pragma unroll
+  for (int k = 0; k < S::N / 2; ++k) {
+    x[k] = add2(x[k], minus);
+    const float2 d = halves(x[k]);                         // (no column, no deviation)
+    if (2 * k >= 4 * S::kFull) x[k] = pair(S::has(live, 2 * k) ? d.x : 0.f, S::has(live, 2 * k + 1) ? d.y : 0.f);
+    squares = fma2(x[k], x[k], squares);
+    sum = add2(sum, x[k]);
+  }
+  float s[2] = {halves(squares).x + halves(squares).y, halves(sum).x + halves(sum).y};
+  team_sums<LANES>(s, slots);
+  cluster_sums<CTAS>(s, part);
+  return Correction(s[0], s[1], cols, per_col);
+}
+template <int N>
+__device__ __forceinline__ void normalized(Pair (&x)[N / 2], float c, float rstd) {
+  const Pair minus = pair(-c, -c), r = pair(rstd, rstd);
+#pragma unroll
+  for (int k = 0; k < N / 2; ++k) x[k] = mul2(add2(x[k], minus), r);
 }
 
 // Forward, a row in a team's registers: read once, summed twice.  CTAS > 1: a cluster of so many CTAs, as one team.  A CTA's loads, sums and
@@ -121,44 +214,33 @@ __global__ void __launch_bounds__(LANES > 32 ? LANES : kThreads, resident(LANES,
                                                                               float* mean_out, float* rstd_out) {
   using S = Share<LANES * CTAS, V, VECTOR, FULL>;
   constexpr int kBlock = LANES > 32 ? LANES : kThreads;
-  __shared__ float slots[2][kBlock / 32], part[2];
+  __shared__ float slots[3 * kBlock / 32];
+  __shared__ double part[2];
   pdl_enter();
   const uint32_t member = blockIdx.y * LANES + threadIdx.x % LANES;   // (blockIdx.y: the CTA's rank in its cluster)
   const uint64_t r = (uint64_t)blockIdx.x * (kBlock / LANES) + threadIdx.x / LANES;
   const uint32_t live = S::live(member, cols);
-  float x[S::N];
-  S::load(x, in + (r < rows ? r : rows - 1) * cols, member, live);   // (the lanes of a warp stay together, with a row or without)
-  float s[1] = {0.f};
-#pragma unroll
-  for (int k = 0; k < S::N; ++k) s[0] += x[k];
-  team_sums<LANES>(s, slots[0]);
-  const float mean = cluster_sum<CTAS>(s[0], &part[0]) * per_col;
-  s[0] = 0.f;
-#pragma unroll
-  for (int k = 0; k < S::N; ++k) {
-    x[k] -= mean;
-    if (S::has(live, k)) s[0] += x[k] * x[k];
-  }
-  team_sums<LANES>(s, slots[1]);
-  const float rstd = rsqrtf(cluster_sum<CTAS>(s[0], &part[1]) * per_col + eps);
+  float v[S::N];
+  S::load(v, in + (r < rows ? r : rows - 1) * cols, member, live);   // (the lanes of a warp stay together, with a row or without)
+  Pair x[S::N / 2];
+  const float first = first_mean<LANES, CTAS, S>(v, x, per_col, slots, part);
+  const Correction by = deviations<LANES, CTAS, S>(x, first, live, cols, per_col, slots + kBlock / 32, part + 1);
+  const float mean = first + by.c, rstd = rsqrtf(by.var + eps);
   if (CTAS > 1) cluster_arrive();                          // (nobody leaves while its part may still be read)
   if (r >= rows) return;                                   // (of a cluster, all or none)
+  normalized<S::N>(x, by.c, rstd);
   if (gamma) {
-    float g[S::N];
-    S::load(g, gamma, member, live);
+    S::load(v, gamma, member, live);
 #pragma unroll
-    for (int k = 0; k < S::N; ++k) x[k] = x[k] * rstd * g[k];
-  } else {
-#pragma unroll
-    for (int k = 0; k < S::N; ++k) x[k] = x[k] * rstd;
+    for (int k = 0; k < S::N / 2; ++k) x[k] = mul2(x[k], pair(v[2 * k], v[2 * k + 1]));
   }
   if (beta) {
-    float b[S::N];
-    S::load(b, beta, member, live);
+    S::load(v, beta, member, live);
 #pragma unroll
-    for (int k = 0; k < S::N; ++k) x[k] = x[k] + b[k];
+    for (int k = 0; k < S::N / 2; ++k) x[k] = add2(x[k], pair(v[2 * k], v[2 * k + 1]));
   }
-  S::store(x, out + r * cols, member, live);
+  unpack<S::N>(v, x);
+  S::store(v, out + r * cols, member, live);
   if (member == 0) {
     if (mean_out) mean_out[r] = mean;
     if (rstd_out) rstd_out[r] = rstd;
@@ -208,7 +290,7 @@ __global__ void __launch_bounds__(LANES, LANES < 512 ? 512 / LANES : 1)
   constexpr int N = 4 * V, kImage = LANES * N + 4, kRing = HELD ? 3 : 2;
   using S = Share<LANES, V, false, FULL>;                  // (cols > 4 LANES FULL)
   extern __shared__ float4 images[];
-  __shared__ float slots[2][LANES / 32];
+  __shared__ float slots[3 * LANES / 32];
   pdl_enter();
   float* ring = reinterpret_cast<float*>(images);
   const uint32_t member = threadIdx.x, live = S::live(member, cols);
@@ -222,50 +304,49 @@ __global__ void __launch_bounds__(LANES, LANES < 512 ? 512 / LANES : 1)
   };
 #pragma unroll
   for (int s = 0; s < kRing - 1; ++s) fetch();
-  float g[HELD ? N : 1], b[HELD ? N : 1];
+  Pair g[HELD ? N / 2 : 1], b[HELD ? N / 2 : 1];
   if constexpr (HELD) {
+    float w[N];
 #pragma unroll
-    for (int k = 0; k < N; ++k) g[k] = 1.f, b[k] = 0.f;
-    if (gamma) S::load(g, gamma, member, live);
-    if (beta) S::load(b, beta, member, live);
+    for (int k = 0; k < N; ++k) w[k] = 1.f;
+    if (gamma) S::load(w, gamma, member, live);
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) g[k] = pair(w[2 * k], w[2 * k + 1]);
+#pragma unroll
+    for (int k = 0; k < N; ++k) w[k] = 0.f;
+    if (beta) S::load(w, beta, member, live);
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) b[k] = pair(w[2 * k], w[2 * k + 1]);
   }
   for (; r < rows; r += gridDim.x) {
     copies_wait<kRing - 2>();
     __syncthreads();                                       // what other threads have copied is here, and all have read the row before
-    float x[N];
+    float v[N];
     const float* p = ring + stage * kImage + past(in + r * cols) + member;
 #pragma unroll
-    for (int k = 0; k < N; ++k) x[k] = S::has(live, k) ? p[LANES * k] : 0.f;
+    for (int k = 0; k < N; ++k) v[k] = S::has(live, k) ? p[LANES * k] : 0.f;
     fetch();
-    float s[1] = {0.f};
-#pragma unroll
-    for (int k = 0; k < N; ++k) s[0] += x[k];
-    block_sums<LANES>(s, slots[0]);
-    const float mean = s[0] * per_col;
-    s[0] = 0.f;
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      x[k] -= mean;
-      if (S::has(live, k)) s[0] += x[k] * x[k];
-    }
-    block_sums<LANES>(s, slots[1]);
-    const float rstd = rsqrtf(s[0] * per_col + eps);
-#pragma unroll
-    for (int k = 0; k < N; ++k) x[k] *= rstd;
+    Pair x[N / 2];
+    const float first = first_mean<LANES, 1, S>(v, x, per_col, slots, nullptr);
+    const Correction by = deviations<LANES, 1, S>(x, first, live, cols, per_col, slots + LANES / 32, nullptr);
+    const float mean = first + by.c, rstd = rsqrtf(by.var + eps);
+    normalized<N>(x, by.c, rstd);
     if constexpr (HELD) {
 #pragma unroll
-      for (int k = 0; k < N; ++k) x[k] = x[k] * g[k] + b[k];
+      for (int k = 0; k < N / 2; ++k) x[k] = fma2(x[k], g[k], b[k]);
+      unpack<N>(v, x);
     } else {
+      unpack<N>(v, x);
       if (gamma) {
 #pragma unroll
-        for (int k = 0; k < N; ++k) x[k] *= k < 4 * FULL ? gamma[member + LANES * k] : ld_if(gamma + member + LANES * k, k, live);
+        for (int k = 0; k < N; ++k) v[k] *= k < 4 * FULL ? gamma[member + LANES * k] : ld_if(gamma + member + LANES * k, k, live);
       }
       if (beta) {
 #pragma unroll
-        for (int k = 0; k < N; ++k) x[k] += k < 4 * FULL ? beta[member + LANES * k] : ld_if(beta + member + LANES * k, k, live);
+        for (int k = 0; k < N; ++k) v[k] += k < 4 * FULL ? beta[member + LANES * k] : ld_if(beta + member + LANES * k, k, live);
       }
     }
-    S::store(x, out + r * cols, member, live);
+    S::store(v, out + r * cols, member, live);
     if (member == 0) {
       if (mean_out) mean_out[r] = mean;
       if (rstd_out) rstd_out[r] = rstd;
@@ -278,21 +359,22 @@ __global__ void __launch_bounds__(LANES, LANES < 512 ? 512 / LANES : 1)
 __global__ void __launch_bounds__(kThreads) norm_kernel(const float* in, const float* gamma, const float* beta, float eps,
                                                         uint64_t cols, float* out, float* mean_out, float* rstd_out) {
   pdl_enter();
-  __shared__ float slots[2][kThreads / 32];
+  __shared__ float slots[3 * kThreads / 32];
   const float* x = in + blockIdx.x * cols;
   float s[1] = {0.f};
   for (uint64_t c = threadIdx.x; c < cols; c += kThreads) s[0] += x[c];
-  block_sums<kThreads>(s, slots[0]);
-  const float mean = s[0] / (float)cols;
-  s[0] = 0.f;
+  block_sums<kThreads>(s, slots);
+  const float first = s[0] / (float)cols;
+  float t[2] = {0.f, 0.f};
   for (uint64_t c = threadIdx.x; c < cols; c += kThreads) {
-    const float d = x[c] - mean;
-    s[0] += d * d;
+    const float d = x[c] - first;
+    t[0] += d * d, t[1] += d;
   }
-  block_sums<kThreads>(s, slots[1]);
-  const float rstd = 1.0f / sqrtf(s[0] / (float)cols + eps);
+  block_sums<kThreads>(t, slots + kThreads / 32);
+  const Correction by(t[0], t[1], (uint32_t)cols, 1.f / (float)cols);
+  const float mean = first + by.c, rstd = rsqrtf(by.var + eps);
   for (uint64_t c = threadIdx.x; c < cols; c += kThreads)
-    out[blockIdx.x * cols + c] = (x[c] - mean) * rstd * (gamma ? gamma[c] : 1.f) + (beta ? beta[c] : 0.f);
+    out[blockIdx.x * cols + c] = ((x[c] - first) - by.c) * rstd * (gamma ? gamma[c] : 1.f) + (beta ? beta[c] : 0.f);
   if (threadIdx.x == 0) {
     if (mean_out) mean_out[blockIdx.x] = mean;
     if (rstd_out) rstd_out[blockIdx.x] = rstd;

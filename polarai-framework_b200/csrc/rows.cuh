@@ -24,8 +24,9 @@ __device__ __forceinline__ void block_sums(float (&v)[N], float* slots) {
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const uint32_t lane = threadIdx.x & 31;
-    v[i] = warp_sum(lane < kWarps ? slots[lane * N + i] : 0.f);
+    v[i] = slots[threadIdx.x % kWarps * N + i];            // (a power of two)
+#pragma unroll
+    for (int off = kWarps / 2; off > 0; off >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], off);
   }
 }
 
@@ -40,6 +41,11 @@ __device__ __forceinline__ float2 halves(Pair p) {
   float2 v;
   asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(p));
   return v;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 __device__ __forceinline__ Pair mul2(Pair a, Pair b) {
   Pair r;
