@@ -283,6 +283,8 @@ def fuse_program(program):
                 for j in range(i + 1, len(ops)):
                     kj, aj = ops[j]
                     if kj == "ALLREDUCE":
+                        if aj[0] in a:                       # an exchange of the product, or of what it has read before
+                            break
                         continue
                     if z in aj[:-1] or aj[-1] == z:
                         # the product moves to the other op: nothing between them may write its operands
