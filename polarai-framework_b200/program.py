@@ -54,6 +54,7 @@ class Program:
 
 
 _RESULTS = {"fdense_grad": 2, "flayernorm": 3, "flayernorm_grad": 3, "flogprob": 3, "flogprob_top": 5, "fadamw": 3, "fadamw8": 5}
+_IN_PLACE = ("fadamw", "fadamw8")                            # these read what they write
 
 
 def results_of(kernel, args):
@@ -241,7 +242,7 @@ def fuse_program(program):
         for i, (k, a) in enumerate(ops):
             if i in skip or k == "ALLREDUCE":
                 continue
-            ins = a[:-1]
+            ins = a if k in _IN_PLACE else a[:-1]
             n += sum(1 for x in ins if x == name)
         return n
 

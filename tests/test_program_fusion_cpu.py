@@ -53,3 +53,17 @@ def test_an_exchange_of_something_else_is_no_obstacle(oracle):
     assert [k for k, _ in fuse_program(p).ops] == ["ALLREDUCE", "fmatmul_f_f_sigmoid"]
     plain, fused = both(oracle, p, values("X", "W", "G"))
     assert all(np.array_equal(plain[n], fused[n]) for n in "HG")
+
+
+def test_an_update_reads_its_moments_in_place(oracle):
+    # the last argument of fadamw is a result that the step reads first: the product that made it stays
+    p = square("moments", "XWZHGUm", "XWGUm", "HU")
+    p.tensor("schedule", 2)
+    p.inputs.append("schedule")
+    p.op("fmatmul_f_f", "X", "W", "Z")
+    p.op("fsigmoid", "Z", "H")
+    p.op("fadamw", "G", "schedule", 0.9, 0.999, 1e-8, 0.0, "U", "m", "Z")
+    given = {n: np.abs(v) for n, v in values("X", "W", "G", "U", "m").items()}
+    plain, fused = both(oracle, p, {**given, "schedule": np.array([1, 1e-2], np.float32)})
+    assert all(np.array_equal(plain[n], fused[n]) for n in "HU")
+    assert [k for k, _ in fuse_program(p).ops] == [k for k, _ in p.ops]
