@@ -63,15 +63,31 @@ class OracleExecutor:
                 r = o.fmul(r.ravel(), o.fmul(o.fadd(one, 1.0, t[h].ravel(), -1.0), t[h].ravel()))
                 t[din] = np.asarray(r, np.float32).reshape(self.program.tensors[din])
                 continue
-            if kernel in ("flayernorm", "flayernorm_grad", "flogprob", "flogprob_grad", "fadamw"):
-                # several results, the last arguments; what the oracle gives besides (alternatives) is not asked for
+            if kernel == "fadamw8":
+                # codes lie in the bytes of float tensors
+                w, names = t[args[6]], args[6:]
+                n = w.size
+                first, second = (t[names[i]].ravel().view(np.uint8)[:n] for i in (1, 3))
+                r = rows_oracle.fadamw8(w, t[args[0]].reshape(w.shape), first, t[names[2]], second, t[names[4]], float(t[args[1]].ravel()[0]),
+                                        float(t[args[1]].ravel()[1]), *args[2:6])
+                for i, value in enumerate(r):
+                    if i in (1, 3):
+                        held = np.ascontiguousarray(t[names[i]]).copy()
+                        held.reshape(-1).view(np.uint8)[:n] = value
+                        t[names[i]] = held
+                    else:
+                        t[names[i]] = np.asarray(value, np.float32).reshape(self.program.tensors[names[i]])
+                continue
+            if kernel in ("flayernorm", "flayernorm_grad", "flogprob", "flogprob_top", "flogprob_grad", "fadamw"):
+                # several results, the last arguments
                 a = [t[x] if isinstance(x, str) else x for x in args]
                 if kernel == "flayernorm":
                     given, r = 4, rows_oracle.flayernorm(a[0], a[1], a[2], a[3])
                 elif kernel == "flayernorm_grad":
                     given, r = 5, rows_oracle.flayernorm_grad(*a[:5])
-                elif kernel == "flogprob":
-                    given, r = 2, rows_oracle.flogprob(a[0], a[1].ravel())[:3]
+                elif kernel in ("flogprob", "flogprob_top"):
+                    top = a[5].shape[1] if kernel == "flogprob_top" else 0
+                    given, r = 2, rows_oracle.flogprob(a[0], a[1].ravel(), top)[:len(a) - 2]
                 elif kernel == "flogprob_grad":
                     both = len(a) == 7
                     given, r = len(a) - 1, [rows_oracle.flogprob_grad(a[0], a[1].ravel(), a[2].ravel(), a[3].ravel() if both else None,

@@ -59,3 +59,52 @@ def fadamw(w, g, m, v, step, lr, beta1, beta2, eps, decay):
     c1, c2, lr = 1 - float(b1) ** step, 1 - float(b2) ** step, float(f(lr))
     update = lr / c1 * m.astype(np.float64) / (np.sqrt(v.astype(np.float64) / c2) + float(f(eps)))
     return _f32(w.astype(np.float64) * (1 - lr * float(f(decay))) - update), m, v
+
+
+def to_e4m3(y):
+    """float32 to e4m3 codes: to nearest even, saturating at 448; NaN is 0x7f."""
+    y = np.asarray(y, np.float32)
+    a = np.minimum(np.where(np.isnan(y), 0, np.abs(y)).astype(np.float64), 448.0)
+    exponent = np.maximum(np.frexp(a)[1] - 1, -6)            # of the step 2^(exponent - 3); -6 for what is subnormal
+    a = np.minimum(np.rint(a / 2.0 ** (exponent - 3)) * 2.0 ** (exponent - 3), 448.0)
+    exponent = np.maximum(np.frexp(a)[1] - 1, -6)
+    code = np.where(a < 2.0 ** -6, a * 2.0 ** 9, (exponent + 7) * 8 + (a / 2.0 ** exponent - 1) * 8)
+    code = np.where(np.isnan(y), 0x7f, code).astype(np.uint8)
+    return code | np.where(np.signbit(y) & ~np.isnan(y), 0x80, 0).astype(np.uint8)
+
+
+def from_e4m3(code):
+    code = np.asarray(code, np.uint8)
+    exponent, digits = (code >> 3 & 15).astype(int), (code & 7).astype(np.float64)
+    a = np.where(exponent == 0, digits * 2.0 ** -9, (1 + digits / 8) * 2.0 ** (exponent - 7))
+    a = np.where((code & 0x7f) == 0x7f, np.nan, a)
+    return np.where(code & 0x80, -a, a).astype(np.float32)
+
+
+def fadamw8(w, g, first, first_scales, second, second_scales, step, lr, beta1, beta2, eps, decay):
+    """(weights, first, first scales, second, second scales) with moments as e4m3 codes in blocks of 128, one scale each."""
+    f, n = np.float32, np.size(w)
+    w, g = np.asarray(w, f), np.asarray(g, f)
+
+    def blocks(x):
+        x = np.ravel(x)
+        return np.concatenate([x, np.zeros(-len(x) % 128, x.dtype)]).reshape(-1, 128)
+
+    def held(x, never_zero):
+        largest = np.abs(x).max(1)
+        scale = np.where(largest < f(2.0 ** -100), f(0), largest * f(1 / 448)).astype(f)
+        by = np.where(scale == 0, f(0), f(1) / np.where(scale == 0, f(1), scale)).astype(f)
+        code = to_e4m3(x * by[:, None])
+        if never_zero:
+            code[(code == 0) & (x > 0) & (scale > 0)[:, None]] = 1
+        return code.ravel()[:n], scale
+
+    b1, b2 = f(beta1), f(beta2)
+    m = from_e4m3(blocks(first)) * np.asarray(first_scales, f).ravel()[:, None]
+    u = from_e4m3(blocks(second)) * np.asarray(second_scales, f).ravel()[:, None]
+    m = m * b1 + blocks(g) * (f(1) - b1)
+    u = np.sqrt(u * u * b2 + blocks(g) * (f(1) - b2) * blocks(g))
+    m64, u64 = (x.ravel()[:n].reshape(w.shape).astype(np.float64) for x in (m, u))
+    c1, c2, lr = 1 - float(b1) ** step, 1 - float(b2) ** step, float(f(lr))
+    new = _f32(w.astype(np.float64) * (1 - lr * float(f(decay))) - lr / c1 * m64 / (u64 / np.sqrt(c2) + float(f(eps))))
+    return (new, *held(m, False), *held(u, True))
