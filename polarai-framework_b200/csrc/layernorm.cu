@@ -767,15 +767,17 @@ int polar_b200_flayernorm(const float* in, const float* gamma, const float* beta
 #define ROWS(LANES, V, FULL, CTAS) go(norm_rows_kernel<LANES, V, true, FULL, CTAS>, norm_rows_kernel<LANES, V, false, FULL, CTAS>, LANES, CTAS)
 #define VECTORS(LANES, V, FULL, CTAS) go(norm_rows_kernel<LANES, V, true, FULL, CTAS>, norm_rows_kernel<LANES, V, true, FULL, CTAS>, LANES, CTAS)
 #define FLOATS(LANES, V, FULL, CTAS) go(norm_rows_kernel<LANES, V, false, FULL, CTAS>, norm_rows_kernel<LANES, V, false, FULL, CTAS>, LANES, CTAS)
-#define LANES_OF(V)                       \
-  switch (lanes) {                        \
-    case 8: return ROWS(8, V, V - 1, 1);         \
-    case 16: return ROWS(16, V, V - 1, 1);       \
-    case 32: return ROWS(32, V, V - 1, 1);       \
-    case 64: return ROWS(64, V, V - 1, 1);       \
-    case 128: return ROWS(128, V, V - 1, 1);     \
-    case 256: return ROWS(256, V, V - 1, 1);     \
-    default: return ROWS(512, V, V - 1, 1);      \
+// (12 and 16 elements to a thread: rows that are vectors are a warp's from 516 to 1024 columns and take 24 or 32 from 4096, so 64 and 512 lanes are
+// for single floats; of these, rows of up to 6144 columns that are many enough for 512 lanes are enough for the ring)
+#define LANES_OF(V, WITH_64, WITH_512)          \
+  switch (lanes) {                              \
+    case 8: return ROWS(8, V, V - 1, 1);        \
+    case 16: return ROWS(16, V, V - 1, 1);      \
+    case 32: return ROWS(32, V, V - 1, 1);      \
+    case 64: return WITH_64(64, V, V - 1, 1);   \
+    case 128: return ROWS(128, V, V - 1, 1);    \
+    case 256: return ROWS(256, V, V - 1, 1);    \
+    default: return WITH_512;                   \
   }
   // How many elements a thread takes: 4 where there are few rows, for the shortest chain; 8 while the threads do not fill the SMs; then 16 and,
   // of long rows, 32, whose loads are all in flight at once (65536 x 4096 in teams of 128 threads: 312 us, of 256 314, of 512 403).
@@ -801,6 +803,9 @@ int polar_b200_flayernorm(const float* in, const float* gamma, const float* beta
     return cols <= 1024 * 20   ? ring(norm_ring_kernel<1024, 5, 4, false>, 1024, 5)
            : cols <= 1024 * 24 ? ring(norm_ring_kernel<1024, 6, 5, false>, 1024, 6)
                                : ring(norm_ring_kernel<1024, 7, 6, false>, 1024, 7);
+  auto any_length = [&] {
+    return launch("flayernorm", norm_kernel, dim3((unsigned)rows), kThreads, 0, st, in, gamma, beta, eps, cols, out, mean, rstd);
+  };
   const bool few = rows <= 2 * sms, little = rows * cols < (4ull << 20);
   if (cols <= 8192) {
     const unsigned each = few && cols <= 4096 ? 4 : little ? 8 : vectors && cols >= 4096 ? 32 : 16;
@@ -810,10 +815,10 @@ int polar_b200_flayernorm(const float* in, const float* gamma, const float* beta
     const unsigned v = (unsigned)((cols + lanes - 1) / lanes + 3) / 4;
     if (v > 4) return lanes == 128 ? VECTORS(128, 8, 6, 1) : v > 6 ? VECTORS(256, 8, 6, 1) : VECTORS(256, 6, 4, 1);
     if (lanes == 1024) return v == 1 ? ROWS(1024, 1, 0, 1) : ROWS(1024, 2, 1, 1);
-    if (v == 1) LANES_OF(1)
-    if (v == 2) LANES_OF(2)
-    if (v == 3) LANES_OF(3)
-    LANES_OF(4)
+    if (v == 1) LANES_OF(1, ROWS, ROWS(512, 1, 0, 1))
+    if (v == 2) LANES_OF(2, ROWS, ROWS(512, 2, 1, 1))
+    if (v == 3) LANES_OF(3, FLOATS, any_length())
+    LANES_OF(4, FLOATS, FLOATS(512, 4, 3, 1))
   }
   // Longer ones: a large CTA, clusters of CTAs where the row is beyond one or, as single floats, beyond its registers, and smaller shares in
   // larger clusters where there are few rows (1 x 32768: 4.3 us, one CTA 6.7).
@@ -826,8 +831,7 @@ int polar_b200_flayernorm(const float* in, const float* gamma, const float* beta
 #undef FLOATS
 #undef VECTORS
 #undef ROWS
-  return launch("flayernorm", norm_kernel, dim3((unsigned)rows), kThreads, 0, as_stream(stream), in, gamma, beta, eps, cols, out, mean,
-                rstd);
+  return any_length();
 }
 
 uint64_t polar_b200_flayernorm_grad_workspace_bytes(uint64_t rows, uint64_t cols) {
