@@ -80,43 +80,65 @@ struct Share {
     }
   }
 };
-// The sum over the threads of a team: lanes side by side, or the CTA (`slots` as for block_sums).
+// The sum over the threads of a team, in every thread and added in the same order in each: lanes side by side, or the CTA, of whose warps' sums each
+// thread reads up to eight as vectors (6000 x 500: 7.0 us, by a second round of exchanges 7.4); more are exchanged (400 x 8192: 6.6 us, as vectors
+// 8.0).  `slots`: a float for each warp, aligned to 16 bytes and not in use by anything since the last barrier.
 template <int TEAM>
-__device__ __forceinline__ void team_sum(float (&v)[1], float* slots) {
-  if (TEAM > 32) {
-    block_sums<TEAM < 32 ? 32 : TEAM>(v, slots);
-  } else {
+__device__ __forceinline__ float team_sum(float v, float* slots) {
+  constexpr int kLanes = TEAM < 32 ? TEAM : 32, kWarps = TEAM / 32;
 #pragma unroll
-    for (int off = TEAM / 2; off > 0; off >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], off);
+  for (int off = kLanes / 2; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  if (kWarps < 2) return v;
+  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
+  __syncthreads();
+  if (kWarps == 2) return slots[0] + slots[1];
+  if (kWarps > 8) {
+    v = slots[threadIdx.x % (kWarps > 8 ? kWarps : 32)];
+#pragma unroll
+    for (int off = kWarps / 2; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    return v;
   }
-}
-// Two sums over the team: each half of the lanes takes one of them, which takes 6 exchanges in a warp where 10 would do both in every lane.
-template <int LANES>
-__device__ __forceinline__ float sum_by_halves(float a, float b) {   // the sum of a in the lower half of the lanes, of b in the upper
-  constexpr int kHalf = LANES / 2;
-  const bool upper = threadIdx.x & kHalf;
-  float v = (upper ? b : a) + __shfl_xor_sync(0xffffffffu, upper ? a : b, kHalf);
+  Pair s[2] = {0, 0};
 #pragma unroll
-  for (int off = kHalf / 2; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-  return v;
+  for (int w = 0; w < kWarps; w += 4) {
+    const float4 f = *reinterpret_cast<const float4*>(slots + w);
+    s[0] = add2(s[0], pair(f.x, f.y)), s[1] = add2(s[1], pair(f.z, f.w));
+  }
+  s[0] = add2(s[0], s[1]);
+  return halves(s[0]).x + halves(s[0]).y;
 }
+// Two sums over the team: each half of the lanes takes one of them, which takes 6 exchanges in a warp where 10 would do both in every lane.  `slots`: two
+// floats for each warp.
 template <int TEAM>
 __device__ __forceinline__ void team_sums(float (&v)[2], float* slots) {
-  constexpr int kLanes = TEAM < 32 ? TEAM : 32, kWarps = TEAM < 32 ? 1 : TEAM / 32;
-  const bool upper = threadIdx.x & (kLanes / 2);
-  float s = sum_by_halves<kLanes>(v[0], v[1]);
-  if (TEAM > 32) {
-    const uint32_t at = threadIdx.x & 15;
-    if (at == 0) slots[(upper ? kWarps : 0) + (threadIdx.x >> 5)] = s;
-    __syncthreads();
-    const float* mine = slots + (upper ? kWarps : 0);
-    s = mine[at % kWarps];
-    if (kWarps > 16) s += mine[at + 16];
+  constexpr int kLanes = TEAM < 32 ? TEAM : 32, kHalf = kLanes / 2, kWarps = TEAM / 32;
+  const bool upper = threadIdx.x & kHalf;
+  float s = (upper ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, upper ? v[0] : v[1], kHalf);
 #pragma unroll
-    for (int off = (kWarps < 16 ? kWarps : 16) / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+  for (int off = kHalf / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+  if (kWarps > 8) {
+    if ((threadIdx.x & 15) == 0) slots[(upper ? kWarps : 0) + (threadIdx.x >> 5)] = s;
+    __syncthreads();
+    const float* mine = slots + (upper ? kWarps : 0) + (threadIdx.x & 15);
+    s = kWarps > 16 ? mine[0] + mine[16] : mine[0];
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
   }
-  const float other = __shfl_xor_sync(0xffffffffu, s, kLanes / 2);
-  v[0] = upper ? other : s, v[1] = upper ? s : other;
+  if (kWarps < 2 || kWarps > 8) {
+    const float other = __shfl_xor_sync(0xffffffffu, s, kHalf);
+    v[0] = upper ? other : s, v[1] = upper ? s : other;
+    return;
+  }
+  if ((threadIdx.x & 15) == 0) slots[threadIdx.x >> 4] = s;   // (a warp's lanes 0 and 16 have one each)
+  __syncthreads();
+  Pair t[2] = {0, 0};
+#pragma unroll
+  for (int w = 0; w < 2 * kWarps; w += 4) {
+    const float4 f = *reinterpret_cast<const float4*>(slots + w);
+    t[0] = add2(t[0], pair(f.x, f.y)), t[1] = add2(t[1], pair(f.z, f.w));
+  }
+  t[0] = add2(t[0], t[1]);
+  v[0] = halves(t[0]).x, v[1] = halves(t[0]).y;
 }
 
 // The sums of one or two values over the CTAs of a cluster, added in the same order in each of them; `mine`: for them, not in use by anything else.
@@ -172,8 +194,7 @@ __device__ __forceinline__ float first_mean(const float (&v)[S::N], Pair (&x)[S:
   Pair sum = 0;
 #pragma unroll
   for (int k = 0; k < S::N / 2; ++k) x[k] = pair(v[2 * k], v[2 * k + 1]), sum = add2(sum, x[k]);
-  float s[1] = {halves(sum).x + halves(sum).y};
-  team_sum<LANES>(s, slots);
+  float s[1] = {team_sum<LANES>(halves(sum).x + halves(sum).y, slots)};
   cluster_sums<CTAS>(s, part);
   return __fmul_rn(s[0], per_col);                         // (rounded by itself, as the mean that the deviations are around)
 }
@@ -203,10 +224,11 @@ __device__ __forceinline__ void normalized(Pair (&x)[N / 2], float c, float rstd
 }
 
 // Forward, a row in a team's registers: read once, summed twice.  CTAS > 1: a cluster of so many CTAs, as one team.  A CTA's loads, sums and
-// stores take turns, so several CTAs have to share an SM: at least 1024 threads of them (512 with 24 elements or more per thread, but for the widest
-// rows: 16384 x 16384 with one CTA of 512 threads on an SM 452 us, with two, in 64 registers, 311).
+// stores take turns, so several CTAs have to share an SM: 2048 threads of them with up to 8 elements per thread (300 x 7830: 7.2 us, in two more registers than
+// that allows 8.8), else at least 1024 (512 with 32 elements, but for the widest rows: 16384 x 16384 with one CTA of 512 threads on an SM 452 us, with two, in
+// 64 registers, 311).
 constexpr int resident(int lanes, int v) {
-  const int threads = lanes > 32 ? lanes : kThreads, least = v > 4 && lanes < 512 ? 512 : 1024;
+  const int threads = lanes > 32 ? lanes : kThreads, least = v <= 2 ? 2048 : v > 6 && lanes < 512 ? 512 : 1024;
   return least / threads > 1 ? least / threads : 1;
 }
 template <int LANES, int V, bool VECTOR, int FULL, int CTAS>
@@ -215,7 +237,7 @@ __global__ void __launch_bounds__(LANES > 32 ? LANES : kThreads, resident(LANES,
                                                                               float* mean_out, float* rstd_out) {
   using S = Share<LANES * CTAS, V, VECTOR, FULL>;
   constexpr int kBlock = LANES > 32 ? LANES : kThreads;
-  __shared__ float slots[3 * kBlock / 32];
+  __shared__ __align__(16) float slots[kBlock / 8];        // (a warp's: one of the first sum, two of the others, one that aligns these)
   __shared__ double part[2];
   pdl_enter();
   const uint32_t member = blockIdx.y * LANES + threadIdx.x % LANES;   // (blockIdx.y: the CTA's rank in its cluster)
@@ -225,7 +247,7 @@ __global__ void __launch_bounds__(LANES > 32 ? LANES : kThreads, resident(LANES,
   S::load(v, in + (r < rows ? r : rows - 1) * cols, member, live);   // (the lanes of a warp stay together, with a row or without)
   Pair x[S::N / 2];
   const float first = first_mean<LANES, CTAS, S>(v, x, per_col, slots, part);
-  const Correction by = deviations<LANES, CTAS, S>(x, first, live, cols, per_col, slots + kBlock / 32, part + 1);
+  const Correction by = deviations<LANES, CTAS, S>(x, first, live, cols, per_col, slots + kBlock / 16, part + 1);
   const float mean = first + by.c, rstd = rsqrtf(by.var + eps);
   if (CTAS > 1) cluster_arrive();                          // (nobody leaves while its part may still be read)
   if (r >= rows) return;                                   // (of a cluster, all or none)
@@ -291,7 +313,7 @@ __global__ void __launch_bounds__(LANES, LANES < 512 ? 512 / LANES : 1)
   constexpr int N = 4 * V, kImage = LANES * N + 4, kRing = HELD ? 3 : 2;
   using S = Share<LANES, V, false, FULL>;                  // (cols > 4 LANES FULL)
   extern __shared__ float4 images[];
-  __shared__ float slots[3 * LANES / 32];
+  __shared__ __align__(16) float slots[LANES / 8];
   pdl_enter();
   float* ring = reinterpret_cast<float*>(images);
   const uint32_t member = threadIdx.x, live = S::live(member, cols);
@@ -329,7 +351,7 @@ __global__ void __launch_bounds__(LANES, LANES < 512 ? 512 / LANES : 1)
     fetch();
     Pair x[N / 2];
     const float first = first_mean<LANES, 1, S>(v, x, per_col, slots, nullptr);
-    const Correction by = deviations<LANES, 1, S>(x, first, live, cols, per_col, slots + LANES / 32, nullptr);
+    const Correction by = deviations<LANES, 1, S>(x, first, live, cols, per_col, slots + LANES / 16, nullptr);
     const float mean = first + by.c, rstd = rsqrtf(by.var + eps);
     normalized<N>(x, by.c, rstd);
     if constexpr (HELD) {
