@@ -843,8 +843,9 @@ int polar_b200_flayernorm(const float* in, const float* gamma, const float* beta
     LANES_OF(4, FLOATS, FLOATS(512, 4, 3, 1))
   }
   // Longer ones: a large CTA, clusters of CTAs where the row is beyond one or, as single floats, beyond its registers, and smaller shares in
-  // larger clusters where there are few rows (1 x 32768: 4.3 us, one CTA 6.7).
-  if (rows * 8 <= 2 * sms && cols > 16384 && cols <= 32768) return ROWS(512, 2, 0, 8);
+  // larger clusters for up to nine rows, half of the SMs (1 x 32768: 4.0 us, one CTA 6.4; 10 x 32768 5.9 and 6.5; 10 x 20000 5.4 and 5.1; 18 x 32768 8.3
+  // and 6.6).
+  if (rows * 16 <= sms && cols > 16384 && cols <= 32768) return ROWS(512, 2, 0, 8);
   if (!vectors && cols <= 65536) return cols <= 16384 ? FLOATS(512, 4, 2, 2) : cols <= 32768 ? FLOATS(512, 4, 2, 4) : FLOATS(512, 4, 2, 8);
   if (cols <= 16384) return VECTORS(512, 8, 4, 1);
   if (cols <= 32768) return VECTORS(1024, 8, 4, 1);
