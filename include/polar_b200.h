@@ -394,8 +394,9 @@ uint64_t polar_b200_flayernorm_grad_workspace_bytes(uint64_t rows, uint64_t cols
 /* flogprob: for each row x of logits[rows, classes] (rows `pitch` floats apart, pitch >= classes)
  *   logSumExp = log(sum(exp(x))),  logProb = x[id] - logSumExp,  entropy = -sum(p * log p), p = exp(x - logSumExp),
  * and the `top` (0..32, at most `classes`) largest logits, ties to the lowest index: topIds and topLogProb
- * [rows, top].  One pass over the logits with a running maximum.  Every result but logProb may be NULL;
- * ids may be NULL when logProb is.  topIds are held as the ids are; with fp32 ids classes is at most 2^24.
+ * [rows, top].  One pass over the logits with a running maximum; the largest logit's own 1 is left out of the sum of
+ * exponentials, so that the small logarithms of a row that is nearly certain keep their digits.  What is NULL is not
+ * wanted; ids may be NULL when logProb is.  topIds are held as the ids are; with fp32 ids classes is at most 2^24.
  *  - an id below zero marks a row without one (padding): logProb 0;
  *  - an id that is no class of the row, or no whole number: logProb NaN (nothing is read there);
  *  - a logit of -inf has no probability; a row of nothing else gives logSumExp and all logProbs -inf, entropy 0;

@@ -3,6 +3,8 @@
 // With m the row's maximum, d = x - m, S = sum(exp d) and T = sum(exp(d) * d):
 //   logSumExp = m + log S,   logProb = d[id] - log S,   entropy = log S - T / S,
 // where no term cancels another: d <= 0, so T <= 0 and log S >= 0.  A -inf logit has exp d = 0 and no part in T.
+// Of a row that is nearly certain S is 1 and a little, and log S that little: the one largest element is left out of the sum, so that nothing is
+// rounded beside its 1, and log S = log1p(the rest).
 #include "rows.cuh"
 
 namespace polar_b200 {
@@ -50,9 +52,13 @@ struct Results {
 };
 
 // ---- the running sums ---------------------------------------------------------------------------------
-// A thread's (or a row's) maximum so far, clamped to finite values, with S and T relative to it.  A row of nothing but -inf keeps S = 0.
+// A thread's (or a row's) largest element so far (-inf: none), S without the 1 of that element, and T; both relative to m, the largest clamped to finite
+// values, so that no difference from it is a NaN where an element is -inf.
+constexpr float kLowest = -3.402823466e38f;
 struct Running {
-  float m = -3.402823466e38f, s = 0.f, t = 0.f;
+  float top = -INFINITY, m = kLowest, s = 0.f, t = 0.f;
+  __device__ __forceinline__ bool any() const { return top > -INFINITY; }
+  __device__ __forceinline__ float log_sum() const { return log1pf(s); }
 };
 // d = x - m never enters below this: the exponential is zero there, and zero times d is zero and no NaN.  NaN stays NaN.
 __device__ __forceinline__ float at_least(float d) {
@@ -64,32 +70,93 @@ __device__ __forceinline__ float exp_fast(float d) {       // 2^(d log2 e): off 
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d * 1.4426950408889634f));
   return e;
 }
-__device__ __forceinline__ void raise_to(Running& r, float m) {
-  const float d = at_least(r.m - m), f = exp_fast(d);
-  r.t = f * (r.t + d * r.s);
-  r.s *= f;
-  r.m = m;
-}
 __device__ __forceinline__ void add(Running& r, float x) {
   const float d = at_least(x - r.m), e = exp_fast(d);
   r.s += e;
   r.t += e * d;
 }
-__device__ __forceinline__ void add4(Running& r, float4 v) {
-  const float d0 = at_least(v.x - r.m), d1 = at_least(v.y - r.m), d2 = at_least(v.z - r.m), d3 = at_least(v.w - r.m);
-  const float e0 = exp_fast(d0), e1 = exp_fast(d1), e2 = exp_fast(d2), e3 = exp_fast(d3);
-  r.s += (e0 + e1) + (e2 + e3);
-  r.t += (e0 * d0 + e1 * d1) + (e2 * d2 + e3 * d3);
+// To a larger top; `before`: whether the largest so far, which is of the sum now, was this thread's.
+__device__ __forceinline__ void raise_to(Running& r, float top, bool before) {
+  const float m = fmaxf(top, kLowest), d = at_least(r.m - m), f = exp_fast(d), sum = r.s + (before ? 1.f : 0.f);
+  r.t = f * (r.t + d * sum);
+  r.s = f * sum;
+  r.m = m;
+  r.top = top;
 }
+// The same sums two elements at a time.
+struct RunningPair {
+  float top = -INFINITY, m = kLowest;
+  Pair s = 0, t = 0;
+  __device__ __forceinline__ Running joined() const {
+    Running r;
+    r.top = top, r.m = m, r.s = halves(s).x + halves(s).y, r.t = halves(t).x + halves(t).y;
+    return r;
+  }
+};
+__device__ __forceinline__ void raise_to(RunningPair& r, float top, bool before) {
+  Running one = r.joined();
+  raise_to(one, top, before);
+  r.top = one.top, r.m = one.m, r.s = pair(one.s, 0.f), r.t = pair(one.t, 0.f);
+}
+__device__ __forceinline__ void add(RunningPair& r, float a, float b) {
+  const float2 x = halves(add2(pair(a, b), pair(-r.m, -r.m)));
+  const Pair d = pair(at_least(x.x), at_least(x.y));
+  const float2 w = halves(mul2(d, pair(1.4426950408889634f, 1.4426950408889634f)));
+  float2 e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(w.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(w.y));
+  const Pair p = pair(e.x, e.y);
+  r.s = add2(r.s, p);
+  r.t = fma2(p, d, r.t);
+}
+__device__ __forceinline__ void add(RunningPair& r, float4 v) { add(r, v.x, v.y), add(r, v.z, v.w); }
 __device__ __forceinline__ float max4(float4 v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
-__device__ __forceinline__ Running warp_join(Running r) {
-  float m = r.m;
+// The largest of the lanes' values (NaN only where all are).
+template <int LANES>
+__device__ __forceinline__ float lanes_max(float v) {
+  if (LANES == 32) {
+    float m;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+    return m;
+  }
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-  raise_to(r, m);
-  r.s = warp_sum(r.s);
-  r.t = warp_sum(r.t);
-  return r;
+  for (int off = LANES / 2; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+  return v;
+}
+// The larger and the smaller of two; NaN for both where one is.
+__device__ __forceinline__ void order(float& high, float& low) {
+  const float a = high, b = low;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(high) : "f"(a), "f"(b));
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(low) : "f"(a), "f"(b));
+}
+// Whether the lane is the first of `LANES` neighbouring ones for which something holds.
+template <int LANES>
+__device__ __forceinline__ bool first_of(bool holds) {
+  const uint32_t lane = threadIdx.x & 31, group = LANES == 32 ? 0xffffffffu : ((1u << LANES % 32) - 1) << (lane & ~(LANES - 1));
+  return lane + 1 == (uint32_t)__ffs(__ballot_sync(0xffffffffu, holds) & group);
+}
+// The lanes' sums, which are around the same maximum.  A row with +inf is NaN.
+template <int LANES>
+__device__ __forceinline__ void sum_over(Running& r) {
+#pragma unroll
+  for (int off = LANES / 2; off > 0; off >>= 1) {
+    r.s += __shfl_xor_sync(0xffffffffu, r.s, off);
+    r.t += __shfl_xor_sync(0xffffffffu, r.t, off);
+  }
+  if (r.top == INFINITY) r.s = NAN;
+}
+// The sums of `LANES` neighbouring lanes, in each of them: of the lanes that have met the largest element, the first keeps its 1 out.
+template <int LANES>
+__device__ __forceinline__ Running join(const Running& r) {
+  Running all;
+  all.top = lanes_max<LANES>(r.top);
+  all.m = fmaxf(all.top, kLowest);
+  const bool keeps_out = first_of<LANES>(r.any() && r.top == all.top);
+  const float d = at_least(r.m - all.m), f = exp_fast(d), sum = r.s + (r.any() && !keeps_out ? 1.f : 0.f);
+  all.s = f * sum;
+  all.t = f * (r.t + d * sum);
+  sum_over<LANES>(all);
+  return all;
 }
 
 // ---- a row as vectors -----------------------------------------------------------------------------------
@@ -130,7 +197,6 @@ struct Row {
 // out by a bound of its own, and what that leaves (little more than `top`) is placed by counting what is above it.  -inf is never kept: where fewer than `top` elements are above it, the first of it follow.  A row where more is kept
 // than there is room for (equal logits by the hundred), or with a NaN, which no maximum shows, is looked through a second time by
 // warps that sort as they go.
-constexpr float kLowest = -3.402823466e38f;
 constexpr int kInFlight = 4;                               // vectors of a thread in flight
 constexpr uint32_t kFewTop = 8;
 constexpr uint32_t kPlaced = 48;                           // as many a part of a warp places right away, by counting
@@ -204,73 +270,148 @@ struct Kept {
   uint32_t room;
 };
 
-// The running sums over the vectors first, first + stride, ... of a row, kInFlight of them on their way; `base` is the first of the warp's
-// `first`s, `chunks` the same for a warp (or, where bounds are a matter for the CTA, for all of it).  find_bound(maxima, maximum,
-// chunk, whether it is all) takes the whole team.
-template <bool TOP, class FindBound>
-__device__ __forceinline__ Running scan(const Row& row, uint32_t base, uint32_t first, uint32_t stride, uint32_t chunks, float (&maxima)[kInFlight],
-                                        const Kept& kept, FindBound find_bound) {
-  Running r;
-  float bound = INFINITY;
-  const uint32_t chunk = kInFlight * stride;
-  uint32_t next_bound = 0;
-  const bool edges = row.whole_from != 0 || row.whole_to != row.vectors;
-#pragma unroll
-  for (int u = 0; u < kInFlight; ++u) maxima[u] = kLowest;
-  for (uint32_t n = 0; n < chunks; ++n) {
-    const uint32_t i = first + n * chunk;
-    float4 v[kInFlight];
-    const bool inner = n > 0 && (n + 1) * chunk <= row.whole_to;   // all vectors of the chunk are whole
+// A chunk: kInFlight vectors of a thread, `stride` apart, all of them on their way at once.
+struct Chunk {
+  float4 v[kInFlight];
+  float high[kInFlight], rest[kInFlight][3];               // of each vector the largest element and the others (order_all)
+
+  // `inner`: all of them are whole.  -inf where there is no element.
+  __device__ __forceinline__ void load(const Row& row, uint32_t i, uint32_t stride, bool inner, bool edges) {
     if (inner) {
 #pragma unroll
       for (int u = 0; u < kInFlight; ++u) v[u] = row.whole(i + u * stride);
-    } else {
-#pragma unroll
-      for (int u = 0; u < kInFlight; ++u) {
-        v[u] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        if (row.is_whole(i + u * stride)) v[u] = row.whole(i + u * stride);
-      }
-      if (edges) {
-#pragma unroll
-        for (int u = 0; u < kInFlight; ++u)
-          if (i + u * stride < row.vectors && !row.is_whole(i + u * stride)) v[u] = row.edge(i + u * stride);
-      }
+      return;
     }
-    float m[kInFlight], most;
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      v[u] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      if (row.is_whole(i + u * stride)) v[u] = row.whole(i + u * stride);
+    }
+    if (edges) {
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u)
+        if (i + u * stride < row.vectors && !row.is_whole(i + u * stride)) v[u] = row.edge(i + u * stride);
+    }
+  }
+  // The largest element (a NaN is none), and of each vector the largest met so far.
+  template <bool TOP>
+  __device__ __forceinline__ float largest(float (&maxima)[kInFlight]) const {
+    float m[kInFlight];
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
       m[u] = max4(v[u]);
       if (TOP) maxima[u] = fmaxf(maxima[u], m[u]);
     }
-    most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-    if (most > r.m) raise_to(r, most);
-    if (TOP) {
-      if (n == next_bound) {
-        bound = find_bound(maxima, r.m, v, chunks == 1);
-        next_bound = 4 * n + 3;
-      }
-      if (most >= bound && *(volatile uint32_t*)kept.count <= kept.room) {
-        uint32_t which = 0;                                // of the 16 elements, those that reach the bound
+    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+  }
+  // The elements with the largest of all in high[0], the other vectors' in high[1] and so on; all are NaN that one of these is ordered with.
+  __device__ __forceinline__ void order_all() {
 #pragma unroll
-        for (int u = 0; u < kInFlight; ++u)
-          which |= (v[u].x >= bound ? 1u << 4 * u : 0) | (v[u].y >= bound ? 2u << 4 * u : 0) | (v[u].z >= bound ? 4u << 4 * u : 0) |
-                   (v[u].w >= bound ? 8u << 4 * u : 0);
-        uint32_t at = atomicAdd(kept.count, (uint32_t)__popc(which));
-        while (which) {
-          const uint32_t e = __ffs(which) - 1, u = e >> 2;
-          which &= which - 1;
-          const float4 x = u & 2 ? (u & 1 ? v[3] : v[2]) : (u & 1 ? v[1] : v[0]);
-          const float value = e & 2 ? (e & 1 ? x.w : x.z) : (e & 1 ? x.y : x.x);
-          if (at < kept.room) kept.rank[at] = rank_of(value, row.element(i + u * stride, e & 3));
-          ++at;
-        }
-      }
+    for (int u = 0; u < kInFlight; ++u) {
+      float a = v[u].x, b = v[u].y, c = v[u].z, d = v[u].w;
+      order(a, b), order(c, d), order(a, c);
+      high[u] = a, rest[u][0] = b, rest[u][1] = c, rest[u][2] = d;
     }
+    order(high[0], high[1]), order(high[2], high[3]), order(high[0], high[2]);
+  }
+  // The elements that reach the bound.
+  __device__ __forceinline__ void keep(const Kept& kept, float most, float bound, const Row& row, uint32_t i, uint32_t stride) const {
+    if (!(most >= bound && *(volatile uint32_t*)kept.count <= kept.room)) return;
+    uint32_t which = 0;                                    // of the 16 elements
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u)
-      if (inner || base + n * chunk + u * stride < row.vectors) add4(r, v[u]);
+      which |= (v[u].x >= bound ? 1u << 4 * u : 0) | (v[u].y >= bound ? 2u << 4 * u : 0) | (v[u].z >= bound ? 4u << 4 * u : 0) |
+               (v[u].w >= bound ? 8u << 4 * u : 0);
+    uint32_t at = atomicAdd(kept.count, (uint32_t)__popc(which));
+    while (which) {
+      const uint32_t e = __ffs(which) - 1, u = e >> 2;
+      which &= which - 1;
+      const float4 x = u & 2 ? (u & 1 ? v[3] : v[2]) : (u & 1 ? v[1] : v[0]);
+      const float value = e & 2 ? (e & 1 ? x.w : x.z) : (e & 1 ? x.y : x.x);
+      if (at < kept.room) kept.rank[at] = rank_of(value, row.element(i + u * stride, e & 3));
+      ++at;
+    }
   }
-  return r;
+  // The elements enter the sums.  `left`: the number of vectors from the first of the warp's to the row's end, where not `all` are there.
+  __device__ __forceinline__ void add_to(RunningPair& r, bool all, uint32_t left, uint32_t stride) const {
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u)
+      if (all || u * stride < left) add(r, v[u]);
+  }
+  // The same with `instead` in the place of the largest one (order_all).
+  __device__ __forceinline__ void add_to(RunningPair& r, float instead, bool all, uint32_t left, uint32_t stride) const {
+    add(r, instead, high[1]);
+    add(r, high[2], high[3]);
+#pragma unroll
+    for (int u = 0; u < kInFlight; u += 2)                 // (two vectors at a time)
+      if (all || u * stride < left) {
+        add(r, rest[u][0], rest[u][1]);
+        add(r, rest[u][2], rest[u + 1][0]);
+        add(r, rest[u + 1][1], rest[u + 1][2]);
+      }
+  }
+};
+
+// The sums of a warp over the vectors first, first + stride, ... of a row, joined; `base` is the first of the warp's
+// `first`s, `chunks` the same for a warp (or, where bounds are a matter for the CTA, for all of it).  All lanes go by the largest element that one of
+// them has met: a chunk that has a larger one is rare, and only such a chunk is ordered, so that its largest can stay out of the sum (all chunks
+// ordered, by each lane's own largest: 200 x 60000 10.9 us, so 9.8).  find_bound(maxima, chunk) takes the whole team.
+template <bool TOP, class FindBound>
+__device__ __forceinline__ Running scan(const Row& row, uint32_t base, uint32_t first, uint32_t stride, uint32_t chunks, float (&maxima)[kInFlight],
+                                        const Kept& kept, FindBound find_bound) {
+  RunningPair r;
+  float bound = INFINITY;
+  const uint32_t chunk = kInFlight * stride, lane = threadIdx.x & 31;
+  uint32_t next_bound = 0, holder = 32;                    // the lane that has met the largest element
+  const bool edges = row.whole_from != 0 || row.whole_to != row.vectors;
+#pragma unroll
+  for (int u = 0; u < kInFlight; ++u) maxima[u] = kLowest;
+  for (uint32_t n = 0; n < chunks; ++n) {
+    const uint32_t i = first + n * chunk, left = row.vectors > base + n * chunk ? row.vectors - (base + n * chunk) : 0;
+    const bool inner = n > 0 && (n + 1) * chunk <= row.whole_to;   // all vectors of the chunk are whole
+    Chunk c;
+    c.load(row, i, stride, inner, edges);
+    const float most = c.template largest<TOP>(maxima);
+    if (TOP) {
+      if (n == next_bound) {
+        bound = find_bound(maxima, c.v);
+        next_bound = 4 * n + 3;
+      }
+      c.keep(kept, most, bound, row, i, stride);
+    }
+    if (__any_sync(0xffffffffu, most > r.top)) {
+      const float top = lanes_max<32>(most);
+      raise_to(r, top, lane == holder);
+      holder = __ffs(__ballot_sync(0xffffffffu, most == top)) - 1;
+      c.order_all();
+      c.add_to(r, lane == holder ? -INFINITY : c.high[0], inner, left, stride);
+    } else {
+      c.add_to(r, inner, left, stride);
+    }
+  }
+  Running all = r.joined();
+  sum_over<32>(all);
+  return all;
+}
+// The same of rows that are one chunk of `LANES` lanes.
+template <int LANES, bool TOP, class FindBound>
+__device__ __forceinline__ Running scan_once(const Row& row, uint32_t member, const Kept& kept, FindBound find_bound) {
+  Chunk c;
+  float maxima[kInFlight];
+#pragma unroll
+  for (int u = 0; u < kInFlight; ++u) maxima[u] = kLowest;
+  c.load(row, member, LANES, false, row.whole_from != 0 || row.whole_to != row.vectors);
+  const float most = c.template largest<TOP>(maxima);
+  if (TOP) c.keep(kept, most, find_bound(maxima, c.v), row, member, LANES);
+  RunningPair r;
+  r.top = lanes_max<LANES>(most);
+  if (r.top != r.top) r.top = -INFINITY;                   // (nothing but NaN)
+  r.m = fmaxf(r.top, kLowest);
+  c.order_all();
+  c.add_to(r, first_of<LANES>(r.top > -INFINITY && most == r.top) ? -INFINITY : c.high[0], false, row.vectors, LANES);
+  Running all = r.joined();
+  sum_over<LANES>(all);
+  return all;
 }
 
 // Of `n` ranks in shared memory, up to ROOM, those stay that may be among the `top` largest, in front: a warp looks for a bound that `top` of them
@@ -360,15 +501,15 @@ __device__ __forceinline__ void take_shut_out(unsigned long long* to, uint32_t w
   }
 }
 __device__ __forceinline__ void write_row(const Results& o, uint64_t row, int64_t id, float given, const Running& r) {
-  const float log_sum = logf(r.s);
-  const bool dead = r.s == 0.f;
+  const float log_sum = r.log_sum();
+  const bool dead = !r.any() && r.s == 0.f;                // (NaN is none)
   if (o.logprob) o.logprob[row] = id == kPadding ? 0.f : id == kWrong ? NAN : dead ? -INFINITY : given - r.m - log_sum;
-  if (o.entropy) o.entropy[row] = dead ? 0.f : log_sum - r.t / r.s;
+  if (o.entropy) o.entropy[row] = dead ? 0.f : log_sum - r.t / (1.f + r.s);
   if (o.logsumexp) o.logsumexp[row] = dead ? -INFINITY : r.m + log_sum;
 }
 __device__ __forceinline__ void write_top(const Results& o, uint64_t row, uint32_t at, uint32_t id, float x, const Running& r, float log_sum) {
   if (o.top_ids) write_id(o.top_ids, o.id_type, row * o.top + at, id);
-  if (o.top_logprob) o.top_logprob[row * o.top + at] = r.s == 0.f ? -INFINITY : x - r.m - log_sum;
+  if (o.top_logprob) o.top_logprob[row * o.top + at] = !r.any() && r.s == 0.f ? -INFINITY : x - r.m - log_sum;
 }
 __device__ __forceinline__ void write_top(const Results& o, uint64_t row, uint32_t at, unsigned long long rank, const Running& r, float log_sum) {
   write_top(o, row, at, ~(uint32_t)rank, float_of((uint32_t)(rank >> 32)), r, log_sum);
@@ -398,9 +539,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_wide_kernel(c
   }
   int turn = 0;
   // (two arrays in turn: a barrier is between a round's reads and the writes of the next but one)
-  auto find_bound = [&](const float (&)[kInFlight], float mine, const float4 (&)[kInFlight], bool) {
+  auto find_bound = [&](const float (&maxima)[kInFlight], const float4 (&)[kInFlight]) {
     uint32_t k[4];                                         // of 128 groups of threads: enough for 32 alternatives
-    keys[turn][tid] = ordered(mine);
+    keys[turn][tid] = ordered(fmaxf(fmaxf(maxima[0], maxima[1]), fmaxf(maxima[2], maxima[3])));
     __syncthreads();
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) {
@@ -413,18 +554,17 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_wide_kernel(c
   };
   float maxima[kInFlight];
   const uint32_t chunks = (row.vectors + kInFlight * stride - 1) / (kInFlight * stride);
-  const Running own = scan<TOP>(row, first - lane, first, stride, chunks, maxima, Kept{kept_ranks, &n_kept, kRoom}, find_bound);
-  Running all = warp_join(own);
-  if (lane == 0) part[0][warp] = all.m, part[1][warp] = all.s, part[2][warp] = all.t;
+  Running all = scan<TOP>(row, first - lane, first, stride, chunks, maxima, Kept{kept_ranks, &n_kept, kRoom}, find_bound);
+  if (lane == 0) part[0][warp] = all.top, part[1][warp] = all.s, part[2][warp] = all.t;
   __syncthreads();
   all = Running();
-  if (lane < kWarps) all.m = part[0][lane], all.s = part[1][lane], all.t = part[2][lane];
-  all = warp_join(all);
+  if (lane < kWarps) all.top = part[0][lane], all.m = fmaxf(all.top, kLowest), all.s = part[1][lane], all.t = part[2][lane];
+  all = join<32>(all);
   if (TOP) {
     const uint32_t n = n_kept;                             // the same for all threads, as what hangs on it
     if (n <= kRoom && all.s == all.s) {
       const float4 none[kInFlight] = {};
-      const float bound = n > 64 ? find_bound(maxima, own.m, none, false) : kLowest;
+      const float bound = n > 64 ? find_bound(maxima, none) : kLowest;
       for (uint32_t i = tid; i < n; i += THREADS)
         if (kept_ranks[i] >= (uint64_t)ordered(bound) << 32) left[atomicAdd(&n_left, 1u)] = kept_ranks[i];
     } else {
@@ -449,17 +589,20 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_wide_kernel(c
   }
   if (ctas == 1) {
     if (tid == 0) write_row(o, r, id, given, all);
-    if (TOP && tid < o.top) write_top(o, r, tid, sorted[tid], all, logf(all.s));
+    if (TOP && tid < o.top) write_top(o, r, tid, sorted[tid], all, all.log_sum());
     return;
   }
-  if (tid == 0) joined[0] = all.m, joined[1] = all.s, joined[2] = all.t;
+  if (tid == 0) joined[0] = all.top, joined[1] = all.s, joined[2] = all.t;
   __syncthreads();
   cluster_arrive();
   cluster_wait();
   if (rank == 0) {
     all = Running();
-    if (lane < ctas) all.m = ld_cluster(&joined[0], lane), all.s = ld_cluster(&joined[1], lane), all.t = ld_cluster(&joined[2], lane);
-    all = warp_join(all);
+    if (lane < ctas) {
+      all.top = ld_cluster(&joined[0], lane), all.s = ld_cluster(&joined[1], lane), all.t = ld_cluster(&joined[2], lane);
+      all.m = fmaxf(all.top, kLowest);
+    }
+    all = join<32>(all);
     if (tid == 0) write_row(o, r, id, given, all);
     if (TOP) {
       const uint32_t total = ctas * o.top;
@@ -477,7 +620,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_wide_kernel(c
             if (c < ctas && n + step <= o.top && theirs[c * o.top + n + step - 1] > mine) n += step;
           above += n;
         }
-        if (above < o.top && mine) write_top(o, r, above, mine, all, logf(all.s));
+        if (above < o.top && mine) write_top(o, r, above, mine, all, all.log_sum());
       }
     }
   }
@@ -485,9 +628,13 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_wide_kernel(c
   cluster_wait();
 }
 
-// A warp per row or, for short rows, LANES lanes.
-template <int LANES, bool TOP>
-__global__ void __launch_bounds__(kThreads) logprob_warp_kernel(const float* logits, uint32_t rows, uint32_t classes, uint64_t pitch, Results o) {
+// The vectors of a row, at most: rows that begin elsewhere on a boundary may have one more or less.
+__host__ __device__ constexpr uint32_t chunk_vectors(uint32_t classes) { return (classes + 6) / 4; }
+
+// A warp per row or, for short rows, LANES lanes.  ONCE: a row is one chunk, whose largest element is known before the sums (60000 x 400 with five
+// alternatives 51 us, by the loop 58).  As many CTAs on an SM as do without spills.
+template <int LANES, bool TOP, bool ONCE>
+__global__ void __launch_bounds__(kThreads, TOP ? 4 : ONCE ? 6 : 5) logprob_warp_kernel(const float* logits, uint32_t rows, uint32_t classes, uint64_t pitch, Results o) {
   constexpr uint32_t kRoom = !TOP ? 1 : LANES == 32 ? 512 : 128, kTeams = kThreads / LANES, kRows = 32 / LANES;
   __shared__ unsigned long long kept_ranks[kTeams][kRoom];
   __shared__ uint32_t n_kept[kTeams];
@@ -507,11 +654,11 @@ __global__ void __launch_bounds__(kThreads) logprob_warp_kernel(const float* log
   unsigned long long* kept = kept_ranks[team];
   if (TOP && member == 0) n_kept[team] = 0;
   __syncwarp();
-  auto find_bound = [&](const float (&maxima)[kInFlight], float, const float4 (&v)[kInFlight], bool all_of_it) {
+  auto find_bound = [&](const float (&maxima)[kInFlight], const float4 (&v)[kInFlight]) {
     if (o.top > kFewTop && classes <= kPlaced) return kLowest;
     // Where the row is here and has few vectors beside `top`, a bound of its elements, which few more than `top` reach (60000 x 200 with 32: 73 us, of
     // the vectors' maxima 85; x 400 with 20 92 and 76)
-    if (o.top > kFewTop && all_of_it && classes < 8 * o.top) {
+    if (o.top > kFewTop && ONCE && classes < 8 * o.top) {
       uint32_t k[4 * kInFlight];
 #pragma unroll
       for (int u = 0; u < kInFlight; ++u) {
@@ -525,19 +672,14 @@ __global__ void __launch_bounds__(kThreads) logprob_warp_kernel(const float* log
     for (int u = 0; u < kInFlight; ++u) k[u] = ordered(maxima[u]);
     return bound_of<6, LANES>(k, o.top);
   };
-  float maxima[kInFlight];
-  // (rows that begin elsewhere on a boundary may have a vector more or less: as many chunks as the longest; eight lanes have one)
-  const uint32_t chunks = ((classes + 6) / 4 + kInFlight * LANES - 1) / (kInFlight * LANES);
-  const Running own = scan<TOP>(row, 0, member, LANES, chunks, maxima, Kept{kept, &n_kept[team], kRoom}, find_bound);
-  Running all = own;
-  float m = own.m;
-#pragma unroll
-  for (int off = LANES / 2; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-  raise_to(all, m);
-#pragma unroll
-  for (int off = LANES / 2; off > 0; off >>= 1) {
-    all.s += __shfl_xor_sync(0xffffffffu, all.s, off);
-    all.t += __shfl_xor_sync(0xffffffffu, all.t, off);
+  const Kept to{kept, &n_kept[team], kRoom};
+  Running all;
+  if constexpr (ONCE) {
+    all = scan_once<LANES, TOP>(row, member, to, find_bound);
+  } else {
+    float maxima[kInFlight];
+    const uint32_t chunks = (chunk_vectors(classes) + kInFlight * LANES - 1) / (kInFlight * LANES);
+    all = scan<TOP>(row, 0, member, LANES, chunks, maxima, to, find_bound);
   }
   if (member == 0 && live) write_row(o, r, id, given, all);
   if (!TOP) return;
@@ -545,7 +687,7 @@ __global__ void __launch_bounds__(kThreads) logprob_warp_kernel(const float* log
   const uint32_t n = live ? n_kept[team] : o.top;
   const bool sorts = live && (n > kRoom || all.s != all.s);
   const bool simple = !sorts && n >= o.top && n <= (LANES == 32 ? 64 : kPlaced);
-  const float log_sum = logf(all.s);
+  const float log_sum = all.log_sum();
   if (simple && live) {                                    // few: each team places its own, by counting what is above
     for (uint32_t i = member; i < n; i += LANES) {
       uint32_t above = 0;
@@ -561,7 +703,7 @@ __global__ void __launch_bounds__(kThreads) logprob_warp_kernel(const float* log
     const int who = __ffs(others) - 1;
     const uint64_t q = first + who / LANES;
     Running sums;
-    sums.m = __shfl_sync(0xffffffffu, all.m, who), sums.s = __shfl_sync(0xffffffffu, all.s, who);
+    sums.top = __shfl_sync(0xffffffffu, all.top, who), sums.m = __shfl_sync(0xffffffffu, all.m, who), sums.s = __shfl_sync(0xffffffffu, all.s, who);
     const float its_log_sum = __shfl_sync(0xffffffffu, log_sum, who);
     if (__shfl_sync(0xffffffffu, (int)sorts, who)) {
       const Row its(logits + q * pitch, classes);
@@ -616,11 +758,18 @@ __global__ void __launch_bounds__(kThreadRows) logprob_thread_kernel(const float
   }
   Running all;
 #pragma unroll
-  for (int c = 0; c < MOST; ++c) all.m = fmaxf(all.m, v[c]);
+  for (int c = 0; c < MOST; ++c) all.top = fmaxf(all.top, v[c]);
+  all.m = fmaxf(all.top, kLowest);
+  bool out = !all.any();                                   // whether the one that stays out of the sum has been
 #pragma unroll
-  for (int c = 0; c < MOST; ++c) add(all, v[c]);
+  for (int c = 0; c < MOST; ++c) {
+    const bool this_one = !out && v[c] == all.top;
+    add(all, this_one ? -INFINITY : v[c]);
+    out = out || this_one;
+  }
+  if (all.top == INFINITY) all.s = NAN;
   write_row(o, r, id, given, all);
-  const float log_sum = logf(all.s);
+  const float log_sum = all.log_sum();
   unsigned long long last = ~0ull;
   for (uint32_t k = 0; k < o.top; ++k) {                   // the largest below the one before
     unsigned long long best = 0;
@@ -797,9 +946,10 @@ int polar_b200_flogprob(const float* logits, uint64_t rows, uint64_t classes, ui
     const uint64_t warps = (rows * lanes + 31) / 32;
     const dim3 grid((unsigned)((warps + kThreads / 32 - 1) / (kThreads / 32)));
     auto go = [&](auto kernel) { return launch("flogprob", kernel, grid, kThreads, 0, st, logits, (uint32_t)rows, n, pitch, o); };
-    return lanes == 8    ? (top ? go(logprob_warp_kernel<8, true>) : go(logprob_warp_kernel<8, false>))
-           : lanes == 16 ? (top ? go(logprob_warp_kernel<16, true>) : go(logprob_warp_kernel<16, false>))
-                         : (top ? go(logprob_warp_kernel<32, true>) : go(logprob_warp_kernel<32, false>));
+    if (lanes == 8) return top ? go(logprob_warp_kernel<8, true, true>) : go(logprob_warp_kernel<8, false, true>);
+    if (lanes == 16) return top ? go(logprob_warp_kernel<16, true, true>) : go(logprob_warp_kernel<16, false, true>);
+    if (chunk_vectors(n) <= kInFlight * 32) return top ? go(logprob_warp_kernel<32, true, true>) : go(logprob_warp_kernel<32, false, true>);
+    return top ? go(logprob_warp_kernel<32, true, false>) : go(logprob_warp_kernel<32, false, false>);
   }
   // Few rows: CTAs of 512 threads, in clusters of up to eight per row while the SMs hold them at two per SM and each has some 7000 classes
   // (1 x 131072: 4.3 us, with twenty alternatives 8.7; of 128 threads 6.3 and 14.2; 20 x 9000 with five 5.0 us in one CTA, 6.8 in two).  Many rows:
