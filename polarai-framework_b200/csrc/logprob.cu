@@ -70,11 +70,6 @@ __device__ __forceinline__ float exp_fast(float d) {       // 2^(d log2 e): off 
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d * 1.4426950408889634f));
   return e;
 }
-__device__ __forceinline__ void add(Running& r, float x) {
-  const float d = at_least(x - r.m), e = exp_fast(d);
-  r.s += e;
-  r.t += e * d;
-}
 // To a larger top; `before`: whether the largest so far, which is of the sum now, was this thread's.
 __device__ __forceinline__ void raise_to(Running& r, float top, bool before) {
   const float m = fmaxf(top, kLowest), d = at_least(r.m - m), f = exp_fast(d), sum = r.s + (before ? 1.f : 0.f);
@@ -756,17 +751,14 @@ __global__ void __launch_bounds__(kThreadRows) logprob_thread_kernel(const float
     id = read_id(o.ids, o.id_type, r, classes);
     if (id >= 0) given = x[id];
   }
-  Running all;
+  RunningPair sums;                                        // of each element and the largest before it the smaller one: all but the largest
+  float low[MOST];
 #pragma unroll
-  for (int c = 0; c < MOST; ++c) all.top = fmaxf(all.top, v[c]);
-  all.m = fmaxf(all.top, kLowest);
-  bool out = !all.any();                                   // whether the one that stays out of the sum has been
+  for (int c = 0; c < MOST; ++c) low[c] = v[c], order(sums.top, low[c]);
+  sums.m = fmaxf(sums.top, kLowest);
 #pragma unroll
-  for (int c = 0; c < MOST; ++c) {
-    const bool this_one = !out && v[c] == all.top;
-    add(all, this_one ? -INFINITY : v[c]);
-    out = out || this_one;
-  }
+  for (int c = 0; c < MOST; c += 2) add(sums, low[c], low[c + 1]);
+  Running all = sums.joined();
   if (all.top == INFINITY) all.s = NAN;
   write_row(o, r, id, given, all);
   const float log_sum = all.log_sum();
