@@ -3,7 +3,8 @@
 // HBM-bound: with moments in 32 bits a weight reads 16 bytes (weight, gradient, two moments) and writes 12; with moments in
 // 8 bits it reads 10 and writes 6, and a block of 128 weights reads and writes two scales.  All tensors of a kind share a launch: a CTA finds
 // its chunk's tensor in a table among the kernel's parameters.  One chunk per CTA: loops over several measured 10 to 20 % slower.
-// Measured, 235 M weights in 163 tensors: 943 us in 32 bits (7.0 TB/s), 606 us in 8 (6.2 TB/s; issue slots 69 % busy); 113 small ones 3.5 us.
+// Measured, 235 M weights in 163 tensors: 941 us in 32 bits (7.0 TB/s), 668 us in 8 (5.7 TB/s; 606 in short runs, at higher clocks; issue slots 70 %
+// busy); 113 small ones 3.5 us.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -58,8 +59,8 @@ __device__ __forceinline__ Rates rates_of(const Common& c, float decay) {
   const float step = c.schedule[0], lr = c.schedule[1];
   return Rates{1.f - lr * decay, lr / -expm1f(step * c.log_beta1), 1.f / sqrtf(-expm1f(step * c.log_beta2))};
 }
-// The tensor that a chunk belongs to: in each round the begins of seven at a time, which are read together (235 M weights in 163 tensors, moments in 8 bits: 606 us, one
-// after the other 620).  The places behind the last tensor hold the largest number.
+// The tensor that a chunk belongs to: in each round the begins of seven at a time, which are read together (235 M weights in 163 tensors, moments in 8 bits: 669 us, by
+// halving 675).  The places behind the last tensor hold the largest number.
 template <int N>
 __device__ __forceinline__ uint32_t tensor_of(const Table<N>& t, uint32_t chunk) {
   uint32_t at = 0;
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(kThreads, 6) adamw_kernel(const __grid_constan
     return;
   }
   // the last few of a tensor, or tensors on odd boundaries: four floats of each, eight loads on their way (sixteen take registers that more threads
-  // would use: 943 us, 957)
+  // would use: 941 us, 957)
   const Rates r = rates_of(c, t.decay);
   const uint32_t step = vectors ? 1 : kThreads;
 #pragma unroll
@@ -310,7 +311,7 @@ int launch_table(const polar_b200_adamw_tensor* tensors, uint64_t count, bool ei
   if (table.count == 0) return POLAR_B200_OK;
   std::fill(table.first + table.count, table.first + N, 0xffffffffu);
   // moments in 8 bits: two blocks per warp in flight (one is a fifth slower, four the same within 3 %); in 32 bits one vector per thread and
-  // more threads (943 us, two 949)
+  // more threads (941 us, two 949)
   if constexpr (UNROLL == 2) return launch_large("fadamw8", adamw8_kernel<N, 2>, dim3((unsigned)chunks), kThreads, stream, table);
   else return launch_large("fadamw", adamw_kernel<N>, dim3((unsigned)chunks), kThreads, stream, table);
 }

@@ -16,7 +16,7 @@ namespace {
 constexpr int kThreads = 256;
 
 // A load (0 otherwise) and a store where k < live, under predicates: the compiler makes a branch of each, some four instructions more for every
-// float (65536 x 1511: 174 us, so 133).
+// float (65536 x 1511: 125 us, by branches a third more).
 __device__ __forceinline__ float ld_if(const float* p, int k, uint32_t live) {
   float v;
   asm volatile("{.reg .pred q; setp.lt.s32 q, %2, %3; mov.f32 %0, 0f00000000; @q ld.global.f32 %0, [%1];}" : "=f"(v) : "l"(p), "r"(k), "r"(live) : "memory");
@@ -302,10 +302,10 @@ __device__ __forceinline__ void copy_image(float* to, const float* src, uint32_t
 }
 
 // Forward, long rows that are not on 16-byte boundaries: an SM's CTAs stay and go through the rows with gamma and beta in their registers; two
-// rows are on their way while one is computed (8000 x 9001: 113 us, a cluster of two CTAs per row 265; 16384 x 16383: 343 and
-// 662; 8007 x 7830: 91, a CTA per row 110; 60000 x 2101: 170 and 214).
-// HELD: gamma and beta are in registers; of rows beyond 16384 columns they are read for each row, and one row is on its way (5294 x 17287: 183 us, a
-// cluster of four CTAs per row 396; 300 x 17287 16.6 and 22.9).
+// rows are on their way while one is computed (8000 x 9001: 123 us, a cluster of two CTAs per row 271; 16384 x 16383: 362 and
+// 681; 8007 x 7830: 90, a CTA per row 101; 60000 x 2101: 173 and 217).
+// HELD: gamma and beta are in registers; of rows beyond 16384 columns they are read for each row, and one row is on its way (5294 x 17287: 188 us, a
+// cluster of four CTAs per row 412; 300 x 17287 16.6 and 23.1).
 template <int LANES, int V, int FULL, bool HELD>
 __global__ void __launch_bounds__(LANES, LANES < 512 ? 512 / LANES : 1)
     norm_ring_kernel(const float* in, const float* gamma, const float* beta, float eps, uint32_t rows, uint32_t cols, float per_col, float* out,
@@ -802,7 +802,8 @@ int polar_b200_flayernorm(const float* in, const float* gamma, const float* beta
     default: return WITH_512;                   \
   }
   // How many elements a thread takes: 4 where there are few rows, for the shortest chain; 8 while the threads do not fill the SMs; then 16 and,
-  // of long rows, 32, whose loads are all in flight at once (65536 x 4096 in teams of 128 threads: 312 us, of 256 314, of 512 403).
+  // of long rows, 32, whose loads are all in flight at once (20000 x 5000 120 us, with 16 140; 20000 x 8192 189 and
+  // 218; at 4096 columns either: 65536 rows 310 and 305, 2048 rows 9.2 and 9.7).
   const uint64_t sms = (uint64_t)sm_count();
   // (The number of elements per thread that a form is made for is its V: FULL fours of every thread are there without asking, so each form serves
   // cols > 4 LANES CTAS FULL only.)
@@ -814,8 +815,8 @@ int polar_b200_flayernorm(const float* in, const float* gamma, const float* beta
     return launch("flayernorm", kernel, dim3((unsigned)(rows < most ? rows : most)), threads, bytes, st, in, gamma, beta, eps, (uint32_t)rows,
                   (uint32_t)cols, (float)(1.0 / (double)cols), out, mean, rstd);
   };
-  // (once every SM has its CTAs, and four rows for each of the smaller ones: 600 x 7830 9.6 us and 10.2, 300 x 7830 7.1 and 7.4, 3000 x 2501 13.4 and
-  // 15.0; up to 2048 columns loads into registers do as well)
+  // (once every SM has its CTAs, and four rows for each of the smaller ones: 600 x 7830 9.4 us, a CTA per row 9.8; 3000 x 2501 11.5 and 12.2; up to
+  // 2048 columns loads into registers do as well)
   if (!vectors && cols > 2048 && cols <= 16384 && rows >= (cols <= 4096 ? 16 : 4) * sms) {
     if (cols <= 4096) return cols <= 128 * 24 ? ring(norm_ring_kernel<128, 6, 4, true>, 128, 6) : ring(norm_ring_kernel<128, 8, 6, true>, 128, 8);
     if (cols <= 8192) return cols <= 256 * 24 ? ring(norm_ring_kernel<256, 6, 4, true>, 256, 6) : ring(norm_ring_kernel<256, 8, 6, true>, 256, 8);

@@ -199,7 +199,7 @@ __device__ __forceinline__ float float_of(uint32_t key) { return __uint_as_float
 
 // The largest bound, nearly, that `top` of the LANES N keys of neighbouring lanes of a warp reach (all lanes take part; each group finds its
 // own).  Keys of kLowest count for vectors not met; with fewer keys than `top` that is the bound, and everything reaches it.  Found by halving, the first
-// BY_VALUE steps by value, where numbers of a short row are told apart sooner (60000 x 400 with 20 alternatives: 92 us, without 107, since the steps
+// BY_VALUE steps by value, where numbers of a short row are told apart sooner (60000 x 400 with 20 alternatives: 73 us, without 77, since the steps
 // by order go through all the powers of two down to zero); by order it takes 32 steps at most, whatever the numbers are.
 template <int BY_VALUE, int LANES, int N>
 __device__ __forceinline__ float bound_of(const uint32_t (&key)[N], uint32_t top) {
@@ -651,8 +651,8 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : ONCE ? 6 : 5) logprob_warp
   __syncwarp();
   auto find_bound = [&](const float (&maxima)[kInFlight], const float4 (&v)[kInFlight]) {
     if (o.top > kFewTop && classes <= kPlaced) return kLowest;
-    // Where the row is here and has few vectors beside `top`, a bound of its elements, which few more than `top` reach (60000 x 200 with 32: 73 us, of
-    // the vectors' maxima 85; x 400 with 20 92 and 76)
+    // Where the row is here and has few vectors beside `top`, a bound of its elements, which few more than `top` reach (60000 x 200 with 32: 71 us, of
+    // the vectors' maxima 81; x 400 with 20, from where on it is these, 73 either way)
     if (o.top > kFewTop && ONCE && classes < 8 * o.top) {
       uint32_t k[4 * kInFlight];
 #pragma unroll
@@ -928,10 +928,10 @@ int polar_b200_flogprob(const float* logits, uint64_t rows, uint64_t classes, ui
     auto go = [&](auto kernel) { return launch("flogprob", kernel, grid, kThreadRows, 0, st, logits, (uint32_t)rows, n, pitch, o); };
     return classes <= 8 ? go(logprob_thread_kernel<8>) : go(logprob_thread_kernel<16>);
   }
-  // A warp per row as long as there are rows enough for every SM (20000 x 8192: 95 us against 104 with a CTA of 128 threads per row, with five
-  // alternatives 131 and 162; 300 x 8000 with five 18.6 and 8.4; up to 1024 classes always).  Where there are more rows than six to an SM, as many
-  // lanes to a short row as hold it in one chunk: 60000 x 100 7.6 us with 8 lanes, with a warp 20; x 200 14.2 with 16, with a warp 23, with twenty
-  // alternatives 56 and, a warp then, 91; but 300 x 100 with twenty 7.4 us with 8 lanes, 5.0 with a warp.
+  // A warp per row as long as there are rows enough for every SM (20000 x 8192: 100 us against 111 with a CTA of 128 threads per row, with five
+  // alternatives 132 and 155; 300 x 8000 with five 16.6 and 7.1; up to 1024 classes always).  Where there are more rows than six to an SM, as many
+  // lanes to a short row as hold it in one chunk: 60000 x 100 7.3 us with 8 lanes, with a warp 21; x 200 13.0 with 16, with a warp 21, with twenty
+  // alternatives 54 and, a warp then, 73; but 300 x 100 with twenty 7.1 us with 8 lanes, 4.5 with a warp.
   const uint64_t sms = (uint64_t)sm_count();
   if (classes <= 1024 || (classes <= 8192 && rows >= 16 * sms)) {
     const uint32_t lanes = rows <= 6 * sms ? 32 : classes <= 4 * kInFlight * 8 - 3 ? 8 : classes <= 4 * kInFlight * 16 - 3 ? 16 : 32;
@@ -944,9 +944,9 @@ int polar_b200_flogprob(const float* logits, uint64_t rows, uint64_t classes, ui
     return top ? go(logprob_warp_kernel<32, true, false>) : go(logprob_warp_kernel<32, false, false>);
   }
   // Few rows: CTAs of 512 threads, in clusters of up to eight per row while the SMs hold them at two per SM and each has some 7000 classes
-  // (1 x 131072: 4.3 us, with twenty alternatives 8.7; of 128 threads 6.3 and 14.2; 20 x 9000 with five 5.0 us in one CTA, 6.8 in two).  Many rows:
-  // CTAs of 128 threads, since barriers then hold up fewer loads (2048 x 50001: 69 us, with five alternatives 79; of 512 threads 76 and 96).  In
-  // between, threads for all of an SM: 200 x 60000 12.2 us with 512, 17.9 with 256; 592 x 29572 14.8 with 256, 18.5 with 128.
+  // (1 x 131072: 4.7 us, with twenty alternatives 9.2; of 128 threads 6.5 and 14.0; 20 x 9000 with five 4.7 us in one CTA, 7.5 in two).  Many rows:
+  // CTAs of 128 threads, since barriers then hold up fewer loads (2048 x 50001: 69 us, with five alternatives 79; of 512 threads 76 and 97).  In
+  // between, threads for all of an SM: 200 x 60000 9.9 us with 512, 14.8 with 256; 592 x 29572 11.3 with 256, 13.8 with 128.
   unsigned ctas = 1;
   while (ctas < 8 && rows * ctas * 2 <= 2 * sms && classes / (2 * ctas) >= 7000) ctas *= 2;
   const dim3 grid((unsigned)rows, ctas);
@@ -987,7 +987,8 @@ int polar_b200_flogprob_grad(const float* logits, uint64_t rows, uint64_t classe
                   dpitch, (uint32_t)parts);
   };
   // A team per row, four vectors of a thread in flight: 65536 x 100 10.7 us with eight lanes, 18.9 with a warp; 20000 x 1000 29.9 with a warp, 41
-  // with a CTA; 20000 x 4000 103 and 99; 8192 x 32000 321 us with CTAs (6.5 TB/s; two vectors 333).
+  // with a CTA; 20000 x 4000 103 and 99; 8192 x 32000 329 us with CTAs (6.4 TB/s), as with two vectors; 999 x 10007 10.9, with two 12.4;
+  // 20000 x 4000 with two 103.
   if (classes <= 400) return alike ? go(logprob_grad_kernel<8, 4, true>, 8, 4) : go(logprob_grad_kernel<8, 4, false>, 8, 4);
   if (classes <= 3000) return alike ? go(logprob_grad_kernel<32, 4, true>, 32, 4) : go(logprob_grad_kernel<32, 4, false>, 32, 4);
   return alike ? go(logprob_grad_kernel<kThreads, 4, true>, kThreads, 4) : go(logprob_grad_kernel<kThreads, 4, false>, kThreads, 4);
