@@ -178,7 +178,7 @@ struct Correction {
   __device__ __forceinline__ Correction(float squares, float deviations, uint32_t cols, float per_col) {
     c = __fmul_rn(deviations, per_col);
     c = __fmaf_rn(__fmaf_rn(-c, (float)cols, deviations), per_col, c);
-    var = squares * per_col - c * c;
+    var = squares * per_col - fminf(c * c, 3.402823466e38f);   // (an infinite sum of squares stays that)
     if (var < 0.f) var = 0.f;                              // (NaN stays)
   }
 };

@@ -82,3 +82,14 @@ def test_values_that_are_none_and_no_eps(env):  # noqa: F811
         d.flayernorm(x, None, None, 1e-30, out, mean, rstd)
         assert torch.isnan(out[:3]).all() and torch.isnan(rstd[:3]).all()
         assert not out[[3, 5]].any() and torch.isfinite(rstd[3:]).all() and (rstd[3:] > 0).all()
+
+
+def test_deviations_whose_squares_are_beyond_fp32(env):  # noqa: F811
+    # of a constant row the first mean may be a step off, whose square is infinite here: still nothing is left of it
+    torch, d = env
+    for cols in (7, 41, 1000, 9001, 20001, 45001, 70001):
+        x = torch.tensor([1e30, -1.1e30, 7.7e29], device="cuda")[:, None].repeat(1, cols)
+        beta = torch.randn(cols, device="cuda")
+        out, mean, rstd = torch.empty_like(x), torch.empty(3, device="cuda"), torch.empty(3, device="cuda")
+        d.flayernorm(x, None, beta, EPS, out, mean, rstd)
+        assert torch.equal(out, beta.expand(3, cols)) and torch.equal(mean, x[:, 0].contiguous()) and (rstd >= 0).all()
