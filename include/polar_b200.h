@@ -457,6 +457,69 @@ typedef struct polar_b200_adamw_options {
 int polar_b200_fadamw(const polar_b200_adamw_tensor* tensors, uint64_t count, const polar_b200_adamw_options* options,
                       void* stream);
 
+/* ---- losses over packed sequences, and orthogonalised momentum ------------------------------------
+ * What a step that trains a token policy ends with: the losses that are computed from flogprob's log probabilities and
+ * entropies and hand flogprob_grad its gradients, and the weight update of matrices beside fadamw.  No counterpart in
+ * the reference.
+ * Sequences lie behind one another: sequence s has the tokens [offsets[s], offsets[s + 1]), offsets[sequences + 1]; ids and offsets
+ * are held as id_type says (offsets in fp32: up to 2^24 tokens).  An id below zero marks a token that does not count (a
+ * prompt's, or padding): whatever the other arrays hold there, it adds nothing and its gradient is zero.  Gradients
+ * before the first sequence and behind the last one are left as they are.  Offsets that do not ascend, or lead outside the tokens, give
+ * results without meaning, but nothing is read or written outside the arrays. */
+
+/* fpolicy_loss: for each token that counts, with d = logProb - oldLogProb, r = exp(d), a its advantage, q = refLogProb - logProb,
+ *   surrogate = min(r * a, clip(r, 1 - clip_low, 1 + clip_high) * a),  kl = exp(q) - 1 - q,
+ * and with its weight w, 1 / (tokens that count) or, by_sequence, 1 / (sequences with such a token * such tokens of its own),
+ *   loss[0] = sum(w * (-surrogate + kl_weight * kl - entropy_weight * entropy)),
+ *   loss[1..4] = sum(w * surrogate), sum(w * kl), sum(w * entropy), sum(w) over the tokens whose ratio is clipped (r * a above the other),
+ *   gLogProb = w * (-(r * a where it is not clipped) + kl_weight * (1 - exp(q))),  gEntropy = -entropy_weight * w.
+ * The advantage is one for each token or for each sequence.  refLogProb or entropy may be NULL (without that term), gLogProb and
+ * gEntropy too (not wanted).  `count` above zero takes the place of the number of tokens (by_sequence: sequences) that count, where the
+ * batch is a part of a larger one.  On which side of the border a token lies is decided by d in 64 bits.  Nothing counts: all zeros.
+ * A gradient may be one of the arrays of a value per token that are read; else what is written may overlap nothing that the call names.
+ * As a builtin: T logProb, T oldLogProb, T refLogProb, T entropy, T advantage[tokens or sequences], T ids, T offsets, f32 clip_low,
+ * f32 clip_high, f32 kl_weight, f32 entropy_weight, f32 by_sequence (0 or 1), T loss[5], T gLogProb, T gEntropy (three results); ids
+ * and offsets in fp32; an advantage of as many values as there are tokens is one for each token.  Scratch as for fmatmul. */
+typedef struct polar_b200_policy_batch {
+  const float* logProb;
+  const float* oldLogProb;
+  const float* refLogProb;
+  const float* entropy;
+  const float* advantage;
+  const void* ids;
+  const void* offsets;
+  int id_type;
+  int advantage_per_token;
+  uint64_t tokens;
+  uint64_t sequences;
+} polar_b200_policy_batch;
+typedef struct polar_b200_policy_options {
+  float clip_low, clip_high, kl_weight, entropy_weight, count;
+  int by_sequence;
+} polar_b200_policy_options;
+int polar_b200_fpolicy_loss(const polar_b200_policy_batch* batch, const polar_b200_policy_options* options, float* loss,
+                            float* gLogProb, float* gEntropy, void* workspace, uint64_t workspace_bytes, void* stream);
+uint64_t polar_b200_fpolicy_loss_workspace_bytes(uint64_t tokens, uint64_t sequences);
+
+/* fpreference_loss: of pairs of sequences, 2i the chosen and 2i + 1 the rejected one.  With D(s) the sum over the tokens of s that
+ * count of logProb - refLogProb (refLogProb NULL: of logProb) or, average, their mean (0 where there are none), and
+ *   reward(s) = beta * D(s),  gap = reward(2i) - reward(2i + 1),  z = gap - margin:
+ *   loss[0] = mean((1 - smoothing) * -log(sigmoid(z)) + smoothing * -log(sigmoid(-z))),
+ *   loss[1] = the share of pairs with a gap above zero,  loss[2] = mean(gap),  rewards[2 * pairs] (NULL: not wanted),
+ *   gLogProb (NULL: not wanted) the derivative of loss[0] at each token.
+ * Sums over sequences are held in 64 bits.  `count` above zero takes the place of the number of pairs.  What is written may overlap
+ * nothing that the call names, but gLogProb may be logProb or refLogProb.
+ * As a builtin: T logProb, T refLogProb, T ids, T offsets[2 * pairs + 1], f32 beta, f32 smoothing, f32 margin, f32 average (0 or 1),
+ * T loss[3], T rewards[2 * pairs], T gLogProb (three results); ids and offsets in fp32.  Scratch as for fmatmul. */
+typedef struct polar_b200_preference_options {
+  float beta, smoothing, margin, count;
+  int average;
+} polar_b200_preference_options;
+int polar_b200_fpreference_loss(const float* logProb, const float* refLogProb, const void* ids, const void* offsets, int id_type,
+                                uint64_t tokens, uint64_t pairs, const polar_b200_preference_options* options, float* loss,
+                                float* rewards, float* gLogProb, void* workspace, uint64_t workspace_bytes, void* stream);
+uint64_t polar_b200_fpreference_loss_workspace_bytes(uint64_t tokens, uint64_t pairs);
+
 /* Sum of n floats into *sum (a device double, ADDED to: clear it first), with
  * warp-shuffle + one atomic per block.  Used to report the scalar mean of an
  * elementwise flogloss output; the reference has no reduction builtin. */
@@ -493,7 +556,7 @@ typedef struct polar_b200_arg {
  * here), and
  * the extended "fsigmoid_grad", "fsigmoid_logloss_grad", "fmatmul_x_y_sigmoid",
  * "fmatmul_x_y_sigmoid_grad", "fmatmul_t_f_rows", "fdense_grad", "fsum", "flayernorm", "flayernorm_grad",
- * "flogprob", "flogprob_top", "flogprob_grad", "fadamw", "fadamw8".
+ * "flogprob", "flogprob_top", "flogprob_grad", "fadamw", "fadamw8", "fpolicy_loss", "fpreference_loss".
  *
  * Launches the builtin called `nativeKernelName` ("fadd", "fmatmul_t_f", ...)
  * on arguments in LaunchCommand order; this is what Device::launch forwards to

@@ -78,6 +78,12 @@ class OracleExecutor:
                     else:
                         t[names[i]] = np.asarray(value, np.float32).reshape(self.program.tensors[names[i]])
                 continue
+            if kernel in ("fpolicy_loss", "fpreference_loss"):
+                a = [t[x].ravel() if isinstance(x, str) else x for x in args]
+                r = (rows_oracle.fpolicy_loss(*a[:12], a[13], a[14]) if kernel == "fpolicy_loss" else rows_oracle.fpreference_loss(*a[:8], a[10]))
+                for name, value in zip(args[-3:], r):
+                    t[name] = np.asarray(value, np.float32).reshape(self.program.tensors[name])
+                continue
             if kernel in ("flayernorm", "flayernorm_grad", "flogprob", "flogprob_top", "flogprob_grad", "fadamw"):
                 # several results, the last arguments
                 a = [t[x] if isinstance(x, str) else x for x in args]

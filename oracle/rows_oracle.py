@@ -108,3 +108,91 @@ def fadamw8(w, g, first, first_scales, second, second_scales, step, lr, beta1, b
     c1, c2, lr = 1 - float(b1) ** step, 1 - float(b2) ** step, float(f(lr))
     new = _f32(w.astype(np.float64) * (1 - lr * float(f(decay))) - lr / c1 * m64 / (u64 / np.sqrt(c2) + float(f(eps))))
     return (new, *held(m, False), *held(u, True))
+
+
+def _tokens(ids, offsets):
+    """The sequence of each token of [offsets[0], offsets[-1]), and which of them count."""
+    offsets = np.asarray(offsets).astype(np.int64)
+    of = np.repeat(np.arange(len(offsets) - 1), np.diff(offsets))
+    counts = ~(np.asarray(ids)[offsets[0]:offsets[-1]] < 0) if len(of) else np.zeros(0, bool)
+    return of, counts, slice(int(offsets[0]), int(offsets[0]) + len(of))
+
+
+def policy_loss64(logprob, old, reference, entropy, advantage, ids, offsets, clip_low, clip_high, kl_weight, entropy_weight, by_sequence=False,
+                  per_token=False, count=0.0):
+    """(loss[5], g_logprob, g_entropy, size) in 64 bits; NaN outside the sequences.  size: per token, what the terms of its gradient come to by
+    magnitude, and the same for the five sums, for bounds of rounding errors."""
+    f = lambda v: float(np.float32(v))  # noqa: E731
+    low, high, beta, alpha = f(clip_low), f(clip_high), f(kl_weight), f(entropy_weight)
+    of, counts, span = _tokens(ids, offsets)
+    n, sequences = len(ids), len(offsets) - 1
+    per = np.bincount(of[counts], minlength=sequences)
+    units = f(count) if count > 0 else max((per > 0).sum() if by_sequence else counts.sum(), 1)
+    w = counts / units / (np.maximum(per, 1)[of] if by_sequence else 1)
+    pick = lambda t: np.where(counts, np.asarray(t, np.float64)[span], 0.0)  # noqa: E731
+    lp, a = pick(logprob), np.asarray(advantage, np.float64)
+    a = np.where(counts, a[span] if per_token else a[of], 0.0)
+    d = lp - pick(old)
+    with np.errstate(over="ignore", invalid="ignore"):
+        free = np.exp(d) * a
+        over, under = d > np.log1p(high), (d < np.log1p(-low) if low < 1 else np.zeros(len(d), bool))
+        cut = (over & (a > 0)) | (under & (a < 0))
+        surrogate = np.where(cut, np.where(over, 1 + high, 1 - low) * a, free)
+        slope = np.where(cut, 0.0, -free)
+        q = pick(reference) - lp if reference is not None else np.zeros(len(lp))
+        kl = np.where(np.abs(q) < 1e-3, q * q * (0.5 + q / 6 + q * q / 24), np.expm1(q) - q)
+        beta = beta if reference is not None else 0.0
+        h = pick(entropy) if entropy is not None else np.zeros(len(lp))
+        alpha = alpha if entropy is not None else 0.0
+        g = np.where(counts, (slope - beta * np.expm1(q)) * w, 0.0)
+        parts = [np.where(counts, t * w, 0.0) for t in (surrogate, kl, h, cut * 1.0)]
+        sums = [t.sum() for t in parts]
+        # (an exponential has its argument's rounding times the argument)
+        sizes = [np.abs(t * by).sum() for t, by in zip(parts, (1 + np.abs(d) * ~cut, 1 + np.abs(q), 1.0, 1.0))]
+        loss = np.array([beta * sums[1] - sums[0] - alpha * sums[2], *sums])
+        size = np.array([beta * sizes[1] + sizes[0] + alpha * sizes[2], *sizes])
+        token = w * (np.abs(slope) * (1 + np.abs(d)) + np.abs(beta * np.expm1(q)) + np.abs(beta * q * np.exp(q)))
+    spread = lambda v: np.concatenate([np.full(span.start, np.nan), v, np.full(n - span.stop, np.nan)])  # noqa: E731
+    return loss, spread(g), spread(-alpha * w), (size, spread(np.where(counts, token, 0.0)))
+
+
+def _over(old, new):
+    """Gradients outside the sequences stay as they were."""
+    return np.where(np.isnan(new) & ~np.isnan(old), old, new) if old is not None else new
+
+
+def preference_loss64(logprob, reference, ids, offsets, beta, smoothing, margin, average=False, count=0.0):
+    """(loss[3], rewards, g_logprob, size) in 64 bits; NaN outside the sequences.  size: the sum of each sequence by magnitude."""
+    f = lambda v: float(np.float32(v))  # noqa: E731
+    beta, e, margin = f(beta), f(smoothing), f(margin)
+    of, counts, span = _tokens(ids, offsets)
+    n, sequences = len(ids), len(offsets) - 1
+    ratio = np.asarray(logprob, np.float64)[span] - (np.asarray(reference, np.float64)[span] if reference is not None else 0.0)
+    ratio = np.where(counts, ratio, 0.0)
+    per = np.maximum(np.bincount(of[counts], minlength=sequences), 1) if average else np.ones(sequences)
+    total = np.bincount(of, weights=ratio, minlength=sequences) / per
+    rewards = beta * total
+    gap = rewards[0::2] - rewards[1::2]
+    z = gap - margin
+    units = f(count) if count > 0 else max(len(gap), 1)
+    loss = (1 - e) * np.logaddexp(0, -z) + e * np.logaddexp(0, z)
+    with np.errstate(over="ignore"):
+        slope = (e / (1 + np.exp(-z)) - (1 - e) / (1 + np.exp(z))) * beta / units
+    g = np.where(counts, (np.stack([slope, -slope], 1).ravel() / per)[of], 0.0)
+    out = np.array([loss.sum(), (gap > 0).sum(), gap.sum()]) / units
+    return out, rewards, np.concatenate([np.full(span.start, np.nan), g, np.full(n - span.stop, np.nan)]), z
+
+
+def fpolicy_loss(logprob, old, reference, entropy, advantage, ids, offsets, clip_low, clip_high, kl_weight, entropy_weight, by_sequence, g_logprob,
+                 g_entropy):
+    """(loss[5], g_logprob, g_entropy) as the builtin of a program gives them."""
+    tokens = len(ids)
+    loss, g, ge, _ = policy_loss64(logprob, old, reference, entropy, advantage, ids, offsets, clip_low, clip_high, kl_weight, entropy_weight, bool(by_sequence),
+                                   np.size(advantage) == tokens)
+    return _f32(loss), _f32(_over(g_logprob, g)), _f32(_over(g_entropy, ge))
+
+
+def fpreference_loss(logprob, reference, ids, offsets, beta, smoothing, margin, average, g_logprob):
+    """(loss[3], rewards, g_logprob)."""
+    loss, rewards, g, _ = preference_loss64(logprob, reference, ids, offsets, beta, smoothing, margin, bool(average))
+    return _f32(loss), _f32(rewards), _f32(_over(g_logprob, g))

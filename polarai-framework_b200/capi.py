@@ -42,6 +42,19 @@ class AdamwOptions(ctypes.Structure):
     _fields_ = [("lr", _f), ("beta1", _f), ("beta2", _f), ("eps", _f), ("step", _u64), ("schedule", _p)]
 
 
+class PolicyBatch(ctypes.Structure):
+    _fields_ = [("logprob", _p), ("old_logprob", _p), ("ref_logprob", _p), ("entropy", _p), ("advantage", _p), ("ids", _p),
+                ("offsets", _p), ("id_type", _i), ("advantage_per_token", _i), ("tokens", _u64), ("sequences", _u64)]
+
+
+class PolicyOptions(ctypes.Structure):
+    _fields_ = [("clip_low", _f), ("clip_high", _f), ("kl_weight", _f), ("entropy_weight", _f), ("count", _f), ("by_sequence", _i)]
+
+
+class PreferenceOptions(ctypes.Structure):
+    _fields_ = [("beta", _f), ("smoothing", _f), ("margin", _f), ("count", _f), ("average", _i)]
+
+
 SIGNATURES = {
     "polar_b200_last_error": (ctypes.c_char_p, []),
     "polar_b200_version": (_i, []),
@@ -89,6 +102,10 @@ SIGNATURES = {
     "polar_b200_flogprob": (_i, [_p, _u64, _u64, _u64, _p, _i, _p, _p, _p, _u64, _p, _p, _p]),
     "polar_b200_flogprob_grad": (_i, [_p, _u64, _u64, _u64, _p, _i, _p, _p, _p, _p, _p, _u64, _p]),
     "polar_b200_fadamw": (_i, [ctypes.POINTER(AdamwTensor), _u64, ctypes.POINTER(AdamwOptions), _p]),
+    "polar_b200_fpolicy_loss": (_i, [ctypes.POINTER(PolicyBatch), ctypes.POINTER(PolicyOptions), _p, _p, _p, _p, _u64, _p]),
+    "polar_b200_fpolicy_loss_workspace_bytes": (_u64, [_u64, _u64]),
+    "polar_b200_fpreference_loss": (_i, [_p, _p, _p, _p, _i, _u64, _u64, ctypes.POINTER(PreferenceOptions), _p, _p, _p, _p, _u64, _p]),
+    "polar_b200_fpreference_loss_workspace_bytes": (_u64, [_u64, _u64]),
     "polar_b200_fsum": (_i, [_p, _p, _u64, _p]),
     "polar_b200_fsum_f32": (_i, [_p, _p, _u64, _p, _u64, _p]),
     "polar_b200_fsum_f32_workspace_bytes": (_u64, [_u64]),

@@ -349,6 +349,50 @@ BUILTIN(fadamw) {
   return launched(polar_b200_fadamw, tensors.data(), (uint64_t)count, &o, c.stream());
 }
 
+// The ids and offsets of packed sequences, of one type.
+bool packed(Call& c, int i, int* type, const at::Tensor** ids, const at::Tensor** offsets) {
+  int other = -1;
+  *ids = c.ids(i, type), *offsets = c.ids(i + 1, &other);
+  return c.ok() && *ids && *offsets && other == *type && numel(*offsets) >= 1;
+}
+// fpolicy_loss(logprob, old_logprob, reference or None, entropy or None, advantage, ids, offsets, advantage_per_token, clip_low, clip_high,
+// kl_weight, entropy_weight, count, by_sequence, loss, g_logprob or None, g_entropy or None)
+BUILTIN(fpolicy_loss) {
+  Call c(args, n, 17);
+  int type = POLAR_B200_IDS_I64;
+  const at::Tensor *lp = c.tensor(0), *old = c.tensor(1), *ref = c.tensor_or_none(2), *entropy = c.tensor_or_none(3), *advantage = c.tensor(4);
+  const at::Tensor *ids, *offsets;
+  if (!packed(c, 5, &type, &ids, &offsets)) return answer(false);
+  polar_b200_policy_options o;
+  const bool per_token = c.whole(7) != 0;
+  o.clip_low = c.scalar(8), o.clip_high = c.scalar(9), o.kl_weight = c.scalar(10), o.entropy_weight = c.scalar(11), o.count = c.scalar(12);
+  o.by_sequence = c.whole(13) != 0;
+  const at::Tensor *loss = c.tensor(14), *g = c.tensor_or_none(15), *ge = c.tensor_or_none(16);
+  if (!c.ok()) return answer(false);
+  const uint64_t tokens = numel(ids), sequences = numel(offsets) - 1;
+  for (const at::Tensor* t : {lp, old, ref, entropy, g, ge})
+    if (!has(t, tokens)) return answer(false);
+  if (numel(advantage) != (per_token ? tokens : sequences) || numel(loss) != 5 || (ge && !entropy)) return answer(false);
+  const polar_b200_policy_batch b = {data(lp), data(old), data_or_null(ref), data_or_null(entropy), data(advantage), ids->data_ptr(),
+                                     offsets->data_ptr(), type, per_token, tokens, sequences};
+  return launched(polar_b200_fpolicy_loss, &b, &o, data(loss), data_or_null(g), data_or_null(ge), nullptr, 0, c.stream());
+}
+// fpreference_loss(logprob, reference or None, ids, offsets, beta, smoothing, margin, count, average, loss, rewards or None, g_logprob or None)
+BUILTIN(fpreference_loss) {
+  Call c(args, n, 12);
+  int type = POLAR_B200_IDS_I64;
+  const at::Tensor *lp = c.tensor(0), *ref = c.tensor_or_none(1), *ids, *offsets;
+  if (!packed(c, 2, &type, &ids, &offsets)) return answer(false);
+  polar_b200_preference_options o;
+  o.beta = c.scalar(4), o.smoothing = c.scalar(5), o.margin = c.scalar(6), o.count = c.scalar(7), o.average = c.whole(8) != 0;
+  const at::Tensor *loss = c.tensor(9), *rewards = c.tensor_or_none(10), *g = c.tensor_or_none(11);
+  if (!c.ok()) return answer(false);
+  const uint64_t tokens = numel(ids), sequences = numel(offsets) - 1;
+  if (sequences % 2 || !has(lp, tokens) || !has(ref, tokens) || !has(g, tokens) || !has(rewards, sequences) || numel(loss) != 3) return answer(false);
+  return launched(polar_b200_fpreference_loss, data(lp), data_or_null(ref), ids->data_ptr(), offsets->data_ptr(), type, tokens, sequences / 2, &o,
+                  data(loss), data_or_null(rewards), data_or_null(g), nullptr, 0, c.stream());
+}
+
 // A program's operations as Python has them: a list of (native name, address of the argument structs, their count).
 bool operations(PyObject* list, std::vector<polar_b200_op>* ops) {
   if (!PyList_Check(list)) {
@@ -417,6 +461,8 @@ PyMethodDef methods[] = {
     ENTRY("flogprob", declining<flogprob>),
     ENTRY("flogprob_grad", declining<flogprob_grad>),
     ENTRY("fadamw", declining<fadamw>),
+    ENTRY("fpolicy_loss", declining<fpolicy_loss>),
+    ENTRY("fpreference_loss", declining<fpreference_loss>),
     ENTRY("workspace_bytes", raising<workspace_bytes>),
     ENTRY("create_program", raising<create_program>),
     ENTRY("run_program", raising<run_program>),

@@ -1,0 +1,890 @@
+// Losses over the log probabilities of packed sequences, and their gradients: the clipped policy loss and the loss of pairs.
+//
+// Sequence s has the tokens [offsets[s], offsets[s + 1]); an id below zero marks a token that does not count.  Both are HBM-bound: a token
+// reads its log probabilities, its id and what else is given once and writes a gradient, 20 to 36 bytes in all.  What stands against one pass
+// is that a gradient hangs on how many tokens count, or on its sequence's sum: the first pass over the ids leaves a bit for each token, so
+// that the second one reads an eighth of a byte in their place.
+//   few tokens (kFew): everything by one CTA in one launch;
+//   else a pass over the ids (policy) or over all (pairs), one over the sequences, one over the tokens.
+// Every sum is taken in a fixed order, over a CTA's tokens in fp32 and beyond that, as of the sums over a sequence, in 64 bits.
+#include <cmath>
+#include <limits>
+#include <type_traits>
+
+#include "rows.cuh"
+
+namespace polar_b200 {
+namespace {
+
+constexpr uint32_t kTile = 4096;                           // tokens of a CTA in the passes that count and sum
+constexpr uint32_t kWords = kTile / 32;
+constexpr int kThreads = 256;
+constexpr uint32_t kPass = 2048;                           // tokens of a CTA in the pass that writes gradients
+constexpr uint32_t kFew = 8192, kFewSequences = 2048;      // what one CTA does alone
+constexpr int kFewThreads = 1024, kFewEach = kFew / kFewThreads;
+
+// ---- sequences
+
+template <class Id>
+struct Packed {
+  const Id *ids, *offsets;
+  uint64_t tokens;
+  uint32_t sequences;
+  // An offset as it is used: none leads outside the tokens, whatever the memory holds.
+  __device__ __forceinline__ uint64_t offset(uint32_t s) const {
+    const Id v = offsets[s];
+    if (!(v > Id(0))) return 0;
+    if constexpr (std::is_floating_point<Id>::value) return v >= (float)tokens ? tokens : (uint64_t)v;   // (exact: tokens up to 2^24)
+    else return min((uint64_t)v, tokens);
+  }
+  __device__ __forceinline__ bool counts(uint64_t t) const { return !(ids[t] < Id(0)); }
+};
+
+// The last sequence that begins at or before token t, found by a whole warp: 32 of what is left are looked at together.
+template <class Id>
+__device__ __forceinline__ uint32_t sequence_of(const Packed<Id>& p, uint64_t t) {
+  uint32_t lo = 0, end = p.sequences;
+  while (end - lo > 1) {
+    const uint32_t step = (end - lo + 32) / 33, at = lo + ((threadIdx.x & 31) + 1) * step;
+    const uint32_t before = __popc(__ballot_sync(0xffffffffu, at < end && p.offset(at) <= t));
+    lo += before * step;
+    end = min(end, lo + step);
+  }
+  return lo;
+}
+
+// The sequences of the warp's 128 tokens from `base` on, four neighbours to each lane.
+template <class Id>
+__device__ __forceinline__ void sequences_of(const Packed<Id>& p, uint64_t base, uint32_t (&of)[4]) {
+  const uint32_t lane = threadIdx.x & 31, first = sequence_of(p, base);
+  const uint64_t none = ~0ull, next = first + 1 + lane < p.sequences ? p.offset(first + 1 + lane) : none;
+  const uint32_t begins = __popc(__ballot_sync(0xffffffffu, next < base + 128));
+  const uint64_t mine = base + 4 * lane;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) of[k] = first;
+  if (begins < 32) {                                       // the 32 next beginnings reach over the 128 tokens
+    for (uint32_t i = 0; i < begins; ++i) {
+      const uint64_t b = __shfl_sync(0xffffffffu, next, i);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) of[k] += b <= mine + k;
+    }
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {                            // sequences of a few tokens, or many empty ones: each lane for itself
+    uint32_t lo = first, end = p.sequences;
+    while (end - lo > 1) {
+      const uint32_t middle = lo + (end - lo) / 2;
+      if (p.offset(middle) <= mine + k) lo = middle;
+      else end = middle;
+    }
+    of[k] = lo;
+  }
+}
+
+// What the passes leave for one another.
+struct Shared {
+  uint32_t ticket;                                         // CTAs that have finished
+  uint32_t live;                                           // sequences with a token that counts
+  float share;                                             // 1 / the tokens that count
+};
+struct Workspace {
+  Shared* shared;
+  uint32_t* counts;                                        // of each tile
+  uint32_t* bits;                                          // which tokens count
+  float* share;                                            // of each sequence: 1 / its tokens that count (0: there is none); or its gradient
+  float4* partial;                                         // of each CTA of the pass over the tokens
+  double *whole, *head, *tail;                             // sums: of sequences inside a tile; of a tile's part of one that began before, or goes on
+};
+uint64_t up(uint64_t n) { return (n + 255) & ~255ull; }
+uint64_t tiles_of(uint64_t tokens) { return tokens ? (tokens + kTile - 1) / kTile : 1; }   // (the first one clears the ticket)
+Workspace lay_out(void* base, uint64_t tokens, uint64_t sequences, bool pairs, uint64_t* bytes) {
+  uint64_t at = 0;
+  auto take = [&](uint64_t n) {
+    char* p = static_cast<char*>(base) + at;
+    at += up(n);
+    return p;
+  };
+  const uint64_t tiles = tiles_of(tokens);
+  Workspace w = {};
+  w.shared = reinterpret_cast<Shared*>(take(sizeof(Shared)));
+  w.counts = reinterpret_cast<uint32_t*>(take(tiles * 4));
+  w.bits = reinterpret_cast<uint32_t*>(take(tiles * kWords * 4));
+  w.share = reinterpret_cast<float*>(take(sequences * 4));
+  if (pairs) {
+    w.partial = reinterpret_cast<float4*>(take((sequences / 2 + kThreads / 32 - 1) / (kThreads / 32) * sizeof(float4)));
+    w.whole = reinterpret_cast<double*>(take(sequences * 8));
+    w.head = reinterpret_cast<double*>(take(tiles * 8));
+    w.tail = reinterpret_cast<double*>(take(tiles * 8));
+  } else {
+    w.partial = reinterpret_cast<float4*>(take((tokens + kPass - 1) / kPass * sizeof(float4)));
+  }
+  *bytes = at;
+  return w;
+}
+
+using polar_b200::warp_sum;
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
+}
+// The sums of four values over the CTA, in its first warp.
+template <int THREADS, class T>
+__device__ __forceinline__ void sums4(T (&v)[4], T* slots) {
+  constexpr int kWarps = THREADS / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] = warp_sum(v[i]);
+    if (lane == 0) slots[warp * 4 + i] = v[i];
+  }
+  __syncthreads();
+  if (warp == 0)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = warp_sum(lane < kWarps ? slots[lane * 4 + i] : T(0));
+}
+
+// Leaves a CTA's sums and tells whether it was the last one to; then the sums of all CTAs are in `total` of its first thread, added in an
+// order that does not hang on which CTA was last.
+template <int THREADS>
+__device__ bool last_sums(float4 mine, float4* partial, uint32_t ctas, uint32_t* ticket, double (&total)[4], double* slots) {
+  __shared__ bool last;
+  if (threadIdx.x == 0) {
+    partial[blockIdx.x] = mine;
+    __threadfence();
+    last = atomicAdd(ticket, 1u) == ctas - 1;
+  }
+  __syncthreads();
+  if (!last) return false;
+  __threadfence();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) total[i] = 0;
+#pragma unroll 8
+  for (uint32_t c = threadIdx.x; c < ctas; c += THREADS) {
+    const float4 p = __ldcg(partial + c);
+    total[0] += p.x, total[1] += p.y, total[2] += p.z, total[3] += p.w;
+  }
+  sums4<THREADS>(total, slots);
+  return true;
+}
+
+// A bit for each token of a tile that counts, and how many there are; nothing outside the sequences counts.
+template <class Id>
+__global__ void __launch_bounds__(kThreads) mark_kernel(Packed<Id> p, Workspace w) {
+  __shared__ uint32_t sums[kThreads / 32];
+  pdl_enter();
+  if (blockIdx.x == 0 && threadIdx.x == 0) w.shared->ticket = w.shared->live = 0;
+  const uint64_t begin = p.offset(0), end = p.offset(p.sequences);
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint64_t base = (uint64_t)blockIdx.x * kTile + warp * (kTile / 8);
+  uint32_t mine = 0;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const uint64_t t = base + 32 * j + lane;
+    const uint32_t b = __ballot_sync(0xffffffffu, t < p.tokens && p.counts(t) && t >= begin && t < end);
+    if (lane == j) mine = b;
+  }
+  if (lane < 16) w.bits[base / 32 + lane] = mine;
+  const uint32_t n = __reduce_add_sync(0xffffffffu, __popc(mine));
+  if (lane == 0) sums[warp] = n;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint32_t total = 0;
+    for (uint32_t s : sums) total += s;
+    w.counts[blockIdx.x] = total;
+  }
+}
+
+// How many tokens of [from, to) count, by a whole warp; from < to.
+__device__ __forceinline__ uint64_t counted(const Workspace& w, uint64_t from, uint64_t to) {
+  const uint32_t lane = threadIdx.x & 31;
+  auto words = [&](uint64_t a, uint64_t b) {               // bits [a, b) of one tile
+    uint32_t n = 0;
+    for (uint64_t i = a / 32 + lane; i * 32 < b; i += 32) {
+      uint32_t bits = w.bits[i];
+      if (i * 32 < a) bits &= ~0u << (a & 31);
+      if (i * 32 + 32 > b) bits &= ~0u >> (32 - (b & 31));
+      n += __popc(bits);
+    }
+    return n;
+  };
+  const uint64_t first = from / kTile, last = (to - 1) / kTile;
+  uint32_t n;
+  uint64_t total = 0;
+  if (first == last) {
+    n = words(from, to);
+  } else {
+    n = words(from, (first + 1) * kTile) + words(last * kTile, to);
+#pragma unroll 4
+    for (uint64_t i = first + 1 + lane; i < last; i += 32) total += w.counts[i];
+  }
+  total += n;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+  return total;
+}
+
+// What a token's term is multiplied by: the tokens that count altogether by one CTA, or of each sequence by a warp.
+constexpr int kTotalThreads = 1024;
+__global__ void __launch_bounds__(kTotalThreads) total_kernel(Workspace w, uint32_t tiles, float count) {
+  __shared__ unsigned long long sums[kTotalThreads / 32];
+  pdl_enter();
+  unsigned long long n = 0;
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < tiles; i += kTotalThreads) n += w.counts[i];
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = n;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    n = 0;
+    for (unsigned long long s : sums) n += s;
+    w.shared->share = count > 0.f ? 1.f / count : n ? 1.f / (float)n : 0.f;
+  }
+}
+template <class Id>
+__global__ void __launch_bounds__(kThreads) shares_kernel(Packed<Id> p, Workspace w) {
+  __shared__ uint32_t live;
+  if (threadIdx.x == 0) live = 0;
+  __syncthreads();
+  pdl_enter();
+  uint32_t mine = 0;
+  for (uint32_t s = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); s < p.sequences; s += gridDim.x * (kThreads / 32)) {
+    const uint64_t from = p.offset(s), to = p.offset(s + 1);
+    const uint64_t n = from < to ? counted(w, from, to) : 0;
+    if ((threadIdx.x & 31) == 0) w.share[s] = n ? 1.f / (float)n : 0.f;
+    mine += n != 0;
+  }
+  if ((threadIdx.x & 31) == 0 && mine) atomicAdd(&live, mine);
+  __syncthreads();
+  if (threadIdx.x == 0 && live) atomicAdd(&w.shared->live, live);
+}
+
+// ---- the policy loss
+
+struct Policy {
+  const float *logprob, *old, *reference, *entropy, *advantage;
+  float *loss, *g_logprob, *g_entropy;
+  float high, low;                                         // what the ratio is clipped to
+  double log_high, log_low;
+  float kl, bonus, count;
+  int by_sequence, per_token;
+};
+
+// exp(q) - 1 - q and, in `grown`, exp(q) - 1.  Near zero by the series from its second term on (the ninth is below 2^-24 of the first
+// up to 1/2): as a difference all digits of it would go.
+__device__ __forceinline__ float excess(float q, float* grown) {
+  if (fabsf(q) < 0.5f) {
+    float s = 1.f / 40320;
+    s = fmaf(s, q, 1.f / 5040), s = fmaf(s, q, 1.f / 720), s = fmaf(s, q, 1.f / 120), s = fmaf(s, q, 1.f / 24);
+    s = fmaf(s, q, 1.f / 6), s = fmaf(s, q, 0.5f);
+    const float k = s * q * q;
+    *grown = q + k;
+    return k;
+  }
+  *grown = expm1f(q);
+  return *grown - q;
+}
+
+struct Term {
+  float surrogate, kl, clipped, slope;
+};
+// A token that counts.  On which side of the clipping border it lies is decided by the difference of the logarithms in 64 bits, where it is
+// exact: in fp32 rounding would decide for tokens on the border.
+__device__ __forceinline__ Term term(const Policy& o, float logprob, float old, float reference, float advantage) {
+  const double d = (double)logprob - (double)old;
+  const bool over = d > o.log_high, under = d < o.log_low;
+  const bool cut = (advantage > 0.f && over) || (advantage < 0.f && under);
+  const float free = expf((float)d) * advantage;
+  Term t;
+  t.surrogate = cut ? (over ? o.high : o.low) * advantage : free;
+  t.clipped = cut ? 1.f : 0.f;
+  t.slope = cut ? 0.f : -free;
+  t.kl = 0.f;
+  if (o.reference) {
+    float grown;
+    t.kl = excess(reference - logprob, &grown);
+    t.slope -= o.kl * grown;
+  }
+  return t;
+}
+__device__ __forceinline__ void write_loss(const Policy& o, const double* total) {
+  const double loss = (double)o.kl * total[1] - total[0] - (double)o.bonus * total[2];
+  o.loss[0] = (float)loss;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o.loss[i + 1] = (float)total[i];
+}
+
+__device__ __forceinline__ float4 load4(const float* p, uint64_t t, uint64_t end, bool vectors) {
+  if (!p) return make_float4(0.f, 0.f, 0.f, 0.f);
+  if (vectors && t + 4 <= end) return ld_stream(reinterpret_cast<const float4*>(p + t));
+  float4 v;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) (&v.x)[k] = t + k < end ? p[t + k] : 0.f;
+  return v;
+}
+// Of four neighbours those of [begin, end).
+__device__ __forceinline__ void store4(float* p, float4 v, uint64_t t, uint64_t begin, uint64_t end, bool vectors) {
+  if (vectors && t >= begin && t + 4 <= end) {
+    st_stream(reinterpret_cast<float4*>(p + t), v);
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (t + k >= begin && t + k < end) p[t + k] = (&v.x)[k];
+}
+
+// LOOK: a token's sequence is needed.
+template <class Id, bool LOOK>
+__global__ void __launch_bounds__(kThreads) policy_kernel(Packed<Id> p, Workspace w, Policy o, bool vectors) {
+  __shared__ float slots[kThreads / 8];
+  __shared__ double wide[kThreads / 8];
+  pdl_enter();
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint64_t begin = p.offset(0), end = p.offset(p.sequences);
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  const float even = o.by_sequence ? (o.count > 0.f ? 1.f / o.count : 1.f / (float)w.shared->live) : w.shared->share;
+  float4 lp[2], old[2], ref[2], ent[2], adv[2];
+  uint32_t bits[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint64_t t = (uint64_t)blockIdx.x * kPass + h * (kPass / 2) + threadIdx.x * 4;
+    lp[h] = load4(o.logprob, t, p.tokens, vectors), old[h] = load4(o.old, t, p.tokens, vectors);
+    ref[h] = load4(o.reference, t, p.tokens, vectors), ent[h] = load4(o.entropy, t, p.tokens, vectors);
+    adv[h] = o.per_token ? load4(o.advantage, t, p.tokens, vectors) : make_float4(0.f, 0.f, 0.f, 0.f);
+    bits[h] = t < p.tokens ? w.bits[t / 32] >> (t & 31) & 15 : 0;
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint64_t base = (uint64_t)blockIdx.x * kPass + h * (kPass / 2) + warp * 128, t = base + 4 * lane;
+    uint32_t of[4] = {0, 0, 0, 0};
+    if (LOOK && base < end) sequences_of(p, base, of);
+    float4 g, ge;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool counts = bits[h] >> k & 1;
+      const float a = o.per_token ? (&adv[h].x)[k] : counts ? o.advantage[of[k]] : 0.f;
+      const float weight = counts ? (o.by_sequence ? even * w.share[of[k]] : even) : 0.f;
+      const Term e = term(o, (&lp[h].x)[k], (&old[h].x)[k], (&ref[h].x)[k], a);
+      if (counts) sum[0] += e.surrogate * weight, sum[1] += e.kl * weight, sum[2] += (&ent[h].x)[k] * weight, sum[3] += e.clipped * weight;
+      (&g.x)[k] = counts ? e.slope * weight : 0.f;
+      (&ge.x)[k] = -o.bonus * weight;
+    }
+    if (o.g_logprob) store4(o.g_logprob, g, t, begin, end, vectors);
+    if (o.g_entropy) store4(o.g_entropy, ge, t, begin, end, vectors);
+  }
+  sums4<kThreads>(sum, slots);
+  double total[4];
+  if (last_sums<kThreads>(make_float4(sum[0], sum[1], sum[2], sum[3]), w.partial, gridDim.x, &w.shared->ticket, total, wide) && threadIdx.x == 0)
+    write_loss(o, total);
+}
+
+// ---- one CTA for few tokens: which of them count, and how many before each word of 32
+
+struct FewTokens {
+  uint32_t bits[kFew / 32], before[kFew / 32 + 1];
+  uint32_t offsets[kFewSequences + 1];
+  uint32_t warps[kFewThreads / 32];
+  __device__ __forceinline__ uint32_t until(uint32_t t) const {   // how many of the tokens before t count
+    return before[t / 32] + (t & 31 ? __popc(bits[t / 32] & ~(~0u << (t & 31))) : 0);
+  }
+  __device__ __forceinline__ uint32_t sequence(uint32_t t, uint32_t sequences) const {
+    uint32_t lo = 0, end = sequences;
+    while (end - lo > 1) {
+      const uint32_t middle = lo + (end - lo) / 2;
+      if (offsets[middle] <= t) lo = middle;
+      else end = middle;
+    }
+    return lo;
+  }
+  __device__ __forceinline__ bool counts(uint32_t t) const { return bits[t / 32] >> (t & 31) & 1; }
+};
+// Thread i's tokens are i, i + kFewThreads, ...
+template <class Id>
+__device__ __forceinline__ void few_tokens(const Packed<Id>& p, FewTokens& f) {
+  const uint32_t lane = threadIdx.x & 31;
+  const uint32_t begin = (uint32_t)p.offset(0), end = (uint32_t)p.offset(p.sequences);
+  for (uint32_t s = threadIdx.x; s <= p.sequences; s += kFewThreads) f.offsets[s] = (uint32_t)p.offset(s);
+#pragma unroll
+  for (int j = 0; j < kFewEach; ++j) {
+    const uint32_t t = j * kFewThreads + threadIdx.x;
+    const uint32_t b = __ballot_sync(0xffffffffu, t < p.tokens && t >= begin && t < end && p.counts(t));
+    if (lane == 0) f.bits[t / 32] = b;
+  }
+  __syncthreads();
+  if (threadIdx.x < kFew / 32) {                           // the words' counts, summed up over the warps of the first 256 threads
+    const uint32_t n = __popc(f.bits[threadIdx.x]);
+    uint32_t upto = n;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, upto, off);
+      if (lane >= off) upto += v;
+    }
+    f.before[threadIdx.x] = upto - n;
+    if (lane == 31) f.warps[threadIdx.x >> 5] = upto;
+  }
+  __syncthreads();
+  if (threadIdx.x < kFew / 32) {
+    uint32_t more = 0;
+    for (uint32_t i = 0; i < threadIdx.x >> 5; ++i) more += f.warps[i];
+    f.before[threadIdx.x] += more;
+    if (threadIdx.x == kFew / 32 - 1) f.before[kFew / 32] = f.before[threadIdx.x] + __popc(f.bits[threadIdx.x]);
+  }
+  __syncthreads();
+}
+
+template <class Id>
+__global__ void __launch_bounds__(kFewThreads) policy_few_kernel(Packed<Id> p, Policy o) {
+  __shared__ FewTokens f;
+  __shared__ float share[kFewSequences];
+  __shared__ double slots[kFewThreads / 8];
+  __shared__ uint32_t live;
+  if (threadIdx.x == 0) live = 0;
+  pdl_enter();
+  few_tokens(p, f);
+  const bool look = o.by_sequence || !o.per_token;
+  float even;
+  if (o.by_sequence) {
+    uint32_t mine = 0;
+    for (uint32_t s = threadIdx.x; s < p.sequences; s += kFewThreads) {
+      const uint32_t from = f.offsets[s], to = f.offsets[s + 1], n = from < to ? f.until(to) - f.until(from) : 0;
+      share[s] = n ? 1.f / (float)n : 0.f;
+      mine += n != 0;
+    }
+    if (mine) atomicAdd(&live, mine);
+    __syncthreads();
+    even = o.count > 0.f ? 1.f / o.count : 1.f / (float)live;
+  } else {
+    const uint32_t n = f.before[kFew / 32];
+    even = o.count > 0.f ? 1.f / o.count : n ? 1.f / (float)n : 0.f;
+  }
+  const uint32_t begin = f.offsets[0], end = f.offsets[p.sequences];
+  double total[4] = {0, 0, 0, 0};
+#pragma unroll 2
+  for (int j = 0; j < kFewEach; ++j) {
+    const uint32_t t = j * kFewThreads + threadIdx.x;
+    if (t < begin || t >= end) continue;
+    const bool counts = f.counts(t);
+    float g = 0.f, weight = 0.f;
+    if (counts) {
+      const uint32_t s = look ? f.sequence(t, p.sequences) : 0;
+      weight = o.by_sequence ? even * share[s] : even;
+      const Term e = term(o, o.logprob[t], o.old[t], o.reference ? o.reference[t] : 0.f, o.advantage[o.per_token ? t : s]);
+      total[0] += e.surrogate * weight, total[1] += e.kl * weight, total[3] += e.clipped * weight;
+      if (o.entropy) total[2] += o.entropy[t] * weight;
+      g = e.slope * weight;
+    }
+    if (o.g_logprob) o.g_logprob[t] = g;
+    if (o.g_entropy) o.g_entropy[t] = -o.bonus * weight;
+  }
+  sums4<kFewThreads>(total, slots);
+  if (threadIdx.x == 0) write_loss(o, total);
+}
+
+// ---- the loss of pairs
+
+struct Pairs {
+  const float *logprob, *reference;
+  float *loss, *rewards, *g_logprob;
+  float beta, smoothing, margin, count;
+  int average;
+};
+
+// A pair's loss by z, its rewards' difference without the margin, and the loss's derivative.  log(1 + e^-|z|) and e^-|z| / (1 + e^-|z|):
+// nothing overflows.
+__device__ __forceinline__ float pair_loss(float z, float smoothing, float* slope) {
+  const float e = expf(-fabsf(z)), more = log1pf(e);
+  const float against = e / (1.f + e), with = 1.f / (1.f + e);   // sigmoid(-|z|), sigmoid(|z|)
+  *slope = z >= 0.f ? smoothing * with - (1.f - smoothing) * against : smoothing * against - (1.f - smoothing) * with;
+  // smoothing * z is what the wrong side's logarithm has more
+  return more + fmaxf(-z, 0.f) + smoothing * z;
+}
+struct Pair2 {
+  float loss, right, gap;
+};
+// Rewards, the loss, and in `chosen` and `rejected` the gradients at each token that counts.  Sums in 64 bits; n: tokens that count.
+__device__ __forceinline__ Pair2 pair_terms(const Pairs& o, uint32_t pair, double chosen, double rejected, uint64_t n_chosen, uint64_t n_rejected,
+                                            float inv_count, float* g_chosen, float* g_rejected) {
+  const double beta = o.beta;
+  if (o.average) chosen /= (double)(n_chosen ? n_chosen : 1), rejected /= (double)(n_rejected ? n_rejected : 1);
+  const double gap = beta * (chosen - rejected);
+  if (o.rewards) o.rewards[2 * pair] = (float)(beta * chosen), o.rewards[2 * pair + 1] = (float)(beta * rejected);
+  float slope;
+  Pair2 r;
+  r.loss = pair_loss((float)(gap - (double)o.margin), o.smoothing, &slope);
+  r.right = gap > 0 ? 1.f : 0.f;
+  r.gap = (float)gap;
+  slope *= o.beta * inv_count;
+  *g_chosen = o.average ? (n_chosen ? slope / (float)n_chosen : 0.f) : slope;
+  *g_rejected = o.average ? (n_rejected ? -slope / (float)n_rejected : 0.f) : -slope;
+  return r;
+}
+
+// The sums of a tile's sequences, or of its parts of them, and which of its tokens count.
+template <class Id>
+__global__ void __launch_bounds__(kThreads) sums_kernel(Packed<Id> p, Workspace w, Pairs o) {
+  __shared__ double values[kTile];
+  __shared__ double slots[kThreads / 32];
+  __shared__ uint32_t sums[kThreads / 32], span[2];
+  pdl_enter();
+  if (blockIdx.x == 0 && threadIdx.x == 0) w.shared->ticket = 0;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint64_t begin = p.offset(0), end = p.offset(p.sequences);
+  const uint64_t tile = (uint64_t)blockIdx.x * kTile, tile_end = min(tile + kTile, p.tokens);
+  const uint64_t from = max(tile, begin), to = min(tile_end, end);
+  if (warp < 2 && from < to) {
+    const uint32_t s = sequence_of(p, warp == 0 ? from : to - 1);
+    if (lane == 0) span[warp] = s;
+  }
+  float lp[16], ref[16];
+  uint32_t mine = 0, bits = 0;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const uint64_t t = tile + warp * (kTile / 8) + 32 * j + lane;
+    const bool inside = t >= from && t < to;
+    lp[j] = inside ? ld_stream(o.logprob + t) : 0.f;
+    ref[j] = inside && o.reference ? ld_stream(o.reference + t) : 0.f;
+    const uint32_t b = __ballot_sync(0xffffffffu, inside && p.counts(t));
+    if (lane == j) mine = b;
+    bits |= (b >> lane & 1) << j;
+  }
+  if (lane < 16) w.bits[tile / 32 + warp * 16 + lane] = mine;
+  const uint32_t n = __reduce_add_sync(0xffffffffu, __popc(mine));
+  if (lane == 0) sums[warp] = n;
+  double sum = 0;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const double d = bits >> j & 1 ? (double)lp[j] - (double)ref[j] : 0.0;
+    values[warp * (kTile / 8) + 32 * j + lane] = d;
+    sum += d;
+  }
+  sum = warp_sum(sum);
+  if (lane == 0) slots[warp] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint32_t total = 0;
+    for (uint32_t s : sums) total += s;
+    w.counts[blockIdx.x] = total;
+  }
+  if (from >= to) return;
+  const uint32_t first = span[0], last = span[1];
+  auto keep = [&](uint32_t s, uint64_t a, uint64_t b, double v) {
+    if (a < tile) w.head[blockIdx.x] = v;
+    else if (b > tile + kTile) w.tail[blockIdx.x] = v;
+    else w.whole[s] = v;
+  };
+  if (first == last) {
+    if (threadIdx.x == 0) {
+      double v = 0;
+      for (double s : slots) v += s;
+      keep(first, p.offset(first), p.offset(first + 1), v);
+    }
+    return;
+  }
+  // each lane looks at one sequence, the warp sums those that are not empty
+  for (uint32_t chunk = first; chunk <= last; chunk += kThreads) {
+    const uint32_t s = chunk + lane * (kThreads / 32) + warp;
+    const uint64_t a = s <= last ? p.offset(s) : 0, b = s <= last ? p.offset(s + 1) : 0;
+    for (uint32_t todo = __ballot_sync(0xffffffffu, max(a, from) < min(b, to)); todo; todo &= todo - 1) {
+      const int who = __ffs(todo) - 1;
+      const uint64_t sa = __shfl_sync(0xffffffffu, a, who), sb = __shfl_sync(0xffffffffu, b, who);
+      double v = 0;
+      for (uint32_t i = (uint32_t)(max(sa, from) - tile) + lane; i < (uint32_t)(min(sb, to) - tile); i += 32) v += values[i];
+      v = warp_sum(v);
+      if (lane == who) keep(s, sa, sb, v);
+    }
+  }
+}
+
+// A sequence's sum from what its tiles have left, by a whole warp.
+__device__ __forceinline__ double sum_of(const Workspace& w, uint32_t s, uint64_t from, uint64_t to) {
+  const uint64_t first = from / kTile, last = (to - 1) / kTile;
+  if (first == last) {
+    // (one that ends where the tile does may have begun before it: then first < last)
+    return w.whole[s];
+  }
+  double v = 0;
+#pragma unroll 4
+  for (uint64_t i = first + 1 + (threadIdx.x & 31); i <= last; i += 32) v += w.head[i];
+  return warp_sum(v) + w.tail[first];
+}
+
+// A warp per pair; the last CTA writes the loss.
+template <class Id>
+__global__ void __launch_bounds__(kThreads) pairs_kernel(Packed<Id> p, Workspace w, Pairs o, float inv_count) {
+  __shared__ float slots[kThreads / 8];
+  __shared__ double wide[kThreads / 8];
+  pdl_enter();
+  const uint32_t pair = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  if (2 * pair < p.sequences) {
+    double d[2];
+    uint64_t n[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint64_t from = p.offset(2 * pair + k), to = p.offset(2 * pair + k + 1);
+      d[k] = from < to ? sum_of(w, 2 * pair + k, from, to) : 0;
+      n[k] = o.average && from < to ? counted(w, from, to) : 0;
+    }
+    if (lane == 0) {
+      const Pair2 r = pair_terms(o, pair, d[0], d[1], n[0], n[1], inv_count, w.share + 2 * pair, w.share + 2 * pair + 1);
+      sum[0] = r.loss * inv_count, sum[1] = r.right * inv_count, sum[2] = r.gap * inv_count;
+    }
+  }
+  sums4<kThreads>(sum, slots);
+  double total[4];
+  if (last_sums<kThreads>(make_float4(sum[0], sum[1], sum[2], 0.f), w.partial, gridDim.x, &w.shared->ticket, total, wide) && threadIdx.x == 0)
+    o.loss[0] = (float)total[0], o.loss[1] = (float)total[1], o.loss[2] = (float)total[2];
+}
+
+template <class Id>
+__global__ void __launch_bounds__(kThreads) pairs_grad_kernel(Packed<Id> p, Workspace w, float* g_logprob, bool vectors) {
+  pdl_enter();
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint64_t begin = p.offset(0), end = p.offset(p.sequences);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint64_t base = (uint64_t)blockIdx.x * kPass + h * (kPass / 2) + warp * 128, t = base + 4 * lane;
+    if (base >= end) return;
+    uint32_t of[4];
+    const uint32_t bits = t < p.tokens ? w.bits[t / 32] >> (t & 31) & 15 : 0;
+    sequences_of(p, base, of);
+    float4 g;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) (&g.x)[k] = bits >> k & 1 ? w.share[of[k]] : 0.f;
+    store4(g_logprob, g, t, begin, end, vectors);
+  }
+}
+
+template <class Id>
+__global__ void __launch_bounds__(kFewThreads) pairs_few_kernel(Packed<Id> p, Pairs o, float inv_count) {
+  extern __shared__ double values[];
+  __shared__ FewTokens f;
+  __shared__ float share[kFewSequences];
+  __shared__ double slots[kFewThreads / 8];
+  pdl_enter();
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float lp[kFewEach], ref[kFewEach];
+#pragma unroll
+  for (int j = 0; j < kFewEach; ++j) {
+    const uint32_t t = j * kFewThreads + threadIdx.x;
+    lp[j] = t < p.tokens ? o.logprob[t] : 0.f;
+    ref[j] = t < p.tokens && o.reference ? o.reference[t] : 0.f;
+  }
+  few_tokens(p, f);
+#pragma unroll
+  for (int j = 0; j < kFewEach; ++j) {
+    const uint32_t t = j * kFewThreads + threadIdx.x;
+    if (t < p.tokens) values[t] = f.counts(t) ? (double)lp[j] - (double)ref[j] : 0.0;
+  }
+  __syncthreads();
+  double total[4] = {0, 0, 0, 0};
+  for (uint32_t pair = warp; 2 * pair < p.sequences; pair += kFewThreads / 32) {
+    double d[2];
+    uint32_t n[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t from = f.offsets[2 * pair + k], to = f.offsets[2 * pair + k + 1];
+      double v = 0;
+      for (uint32_t t = from + lane; t < to; t += 32) v += values[t];
+      d[k] = warp_sum(v);
+      n[k] = from < to ? f.until(to) - f.until(from) : 0;
+    }
+    if (lane == 0) {
+      const Pair2 r = pair_terms(o, pair, d[0], d[1], n[0], n[1], inv_count, share + 2 * pair, share + 2 * pair + 1);
+      total[0] += (double)(r.loss * inv_count), total[1] += (double)(r.right * inv_count), total[2] += (double)(r.gap * inv_count);
+    }
+  }
+  sums4<kFewThreads>(total, slots);                        // (with a barrier, behind which the shares are read)
+  if (threadIdx.x == 0) o.loss[0] = (float)total[0], o.loss[1] = (float)total[1], o.loss[2] = (float)total[2];
+  if (!o.g_logprob) return;
+  const uint32_t begin = f.offsets[0], end = f.offsets[p.sequences];
+  for (uint32_t t = begin + threadIdx.x; t < end; t += kFewThreads)
+    o.g_logprob[t] = f.counts(t) ? share[f.sequence(t, p.sequences)] : 0.f;
+}
+
+// ---- host side
+
+template <class F>
+int with_ids(int id_type, F f) {
+  switch (id_type) {
+    case POLAR_B200_IDS_F32: return f(float());
+    case POLAR_B200_IDS_I32: return f(int32_t());
+    default: return f(int64_t());
+  }
+}
+bool few(uint64_t tokens, uint64_t sequences) { return tokens <= kFew && sequences <= kFewSequences; }
+int check_sequences(const void* ids, const void* offsets, int id_type, uint64_t tokens, uint64_t sequences) {
+  if (id_type < POLAR_B200_IDS_F32 || id_type > POLAR_B200_IDS_I64) return fail(POLAR_B200_ERR_INVALID, "unknown type of ids");
+  if (tokens > 1ull << 36 || sequences > 0x7fffffffull) return fail(POLAR_B200_ERR_INVALID, "too many tokens or sequences");
+  if (id_type == POLAR_B200_IDS_F32 && tokens > 1ull << 24)
+    return fail(POLAR_B200_ERR_INVALID, "offsets in fp32 are exact up to 2^24 tokens");
+  if (id_type == POLAR_B200_IDS_I32 && tokens > 0x7fffffffull) return fail(POLAR_B200_ERR_INVALID, "offsets in 32 bits reach up to 2^31 - 1 tokens");
+  if (sequences && !offsets) return fail(POLAR_B200_ERR_INVALID, "null device pointer");
+  if (sequences && tokens && !ids) return fail(POLAR_B200_ERR_INVALID, "null device pointer");
+  return POLAR_B200_OK;
+}
+// Whether a written array of a value per token overlaps one that is read or written, unless it is read by the same thread (`same`: an array
+// of a value per token, at the same place).
+bool overlaps(const void* w, uint64_t w_bytes, const void* o, uint64_t o_bytes, bool same) {
+  if (!w || !o || !w_bytes || !o_bytes || (same && w == o)) return false;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(w), b = reinterpret_cast<uintptr_t>(o);
+  return a < b + o_bytes && b < a + w_bytes;
+}
+uint64_t id_bytes(int id_type) { return id_type == POLAR_B200_IDS_I64 ? 8 : 4; }
+
+// The caller's workspace, or one from the pool for as long as `f` takes.
+template <class F>
+int with_workspace(void* workspace, uint64_t workspace_bytes, uint64_t need, cudaStream_t st, F f) {
+  if (workspace) {
+    if (workspace_bytes < need || !aligned16(workspace)) return fail(POLAR_B200_ERR_WORKSPACE, "workspace too small or not 16-byte aligned");
+    return f(workspace);
+  }
+  void* own = nullptr;
+  cudaError_t e = scratch_alloc(&own, need, st);
+  if (e != cudaSuccess) return fail(POLAR_B200_ERR_CUDA, "scratch (workspace)", e);
+  const int rc = f(own);
+  e = scratch_free(own, st);
+  if (rc == POLAR_B200_OK && e != cudaSuccess) return fail(POLAR_B200_ERR_CUDA, "returning scratch", e);
+  return rc;
+}
+
+template <class Id>
+int run_policy(const Packed<Id>& p, const Policy& o, void* workspace, uint64_t workspace_bytes, cudaStream_t st) {
+  if (few(p.tokens, p.sequences)) return launch("fpolicy_loss", policy_few_kernel<Id>, dim3(1), kFewThreads, 0, st, p, o);
+  uint64_t need;
+  lay_out(nullptr, p.tokens, p.sequences, false, &need);
+  return with_workspace(workspace, workspace_bytes, need, st, [&](void* base) {
+    const Workspace w = lay_out(base, p.tokens, p.sequences, false, &need);
+    const uint32_t tiles = (uint32_t)tiles_of(p.tokens);
+    int rc = launch("fpolicy_loss: ids", mark_kernel<Id>, dim3(tiles), kThreads, 0, st, p, w);
+    if (rc) return rc;
+    if (o.by_sequence) {
+      const uint64_t ctas = ((uint64_t)p.sequences + kThreads / 32 - 1) / (kThreads / 32), most = 8ull * sm_count();
+      rc = launch("fpolicy_loss: shares", shares_kernel<Id>, dim3((unsigned)(ctas < most ? ctas : most)), kThreads, 0, st, p, w);
+    } else {
+      rc = launch("fpolicy_loss: total", total_kernel, dim3(1), kTotalThreads, 0, st, w, tiles, o.count);
+    }
+    if (rc) return rc;
+    const bool vectors = aligned16(o.logprob) && aligned16(o.old) && aligned16(o.reference) && aligned16(o.entropy) && aligned16(o.g_logprob) &&
+                         aligned16(o.g_entropy) && (!o.per_token || aligned16(o.advantage));
+    auto kernel = o.by_sequence || !o.per_token ? policy_kernel<Id, true> : policy_kernel<Id, false>;
+    return launch("fpolicy_loss", kernel, dim3((unsigned)((p.tokens + kPass - 1) / kPass)), kThreads, 0, st, p, w, o, vectors);
+  });
+}
+
+template <class Id>
+int run_pairs(const Packed<Id>& p, const Pairs& o, void* workspace, uint64_t workspace_bytes, cudaStream_t st) {
+  const float inv_count = o.count > 0.f ? 1.f / o.count : 2.f / (float)p.sequences;
+  if (few(p.tokens, p.sequences)) {
+    constexpr size_t kBytes = kFew * sizeof(double);
+    const cudaError_t e = cudaFuncSetAttribute(pairs_few_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBytes);
+    if (e != cudaSuccess) return fail(POLAR_B200_ERR_CUDA, "fpreference_loss", e);
+    return launch("fpreference_loss", pairs_few_kernel<Id>, dim3(1), kFewThreads, p.tokens * sizeof(double), st, p, o, inv_count);
+  }
+  uint64_t need;
+  lay_out(nullptr, p.tokens, p.sequences, true, &need);
+  return with_workspace(workspace, workspace_bytes, need, st, [&](void* base) {
+    const Workspace w = lay_out(base, p.tokens, p.sequences, true, &need);
+    const uint32_t tiles = (uint32_t)tiles_of(p.tokens);
+    int rc = launch("fpreference_loss: sums", sums_kernel<Id>, dim3(tiles), kThreads, 0, st, p, w, o);
+    if (rc) return rc;
+    rc = launch("fpreference_loss", pairs_kernel<Id>, dim3((p.sequences / 2 + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, st, p, w, o, inv_count);
+    if (rc || !o.g_logprob || !p.tokens) return rc;
+    return launch("fpreference_loss: gradient", pairs_grad_kernel<Id>, dim3((unsigned)((p.tokens + kPass - 1) / kPass)), kThreads, 0, st, p, w,
+                  o.g_logprob, aligned16(o.g_logprob));
+  });
+}
+
+}  // namespace
+}  // namespace polar_b200
+
+using namespace polar_b200;
+
+extern "C" {
+
+uint64_t polar_b200_fpolicy_loss_workspace_bytes(uint64_t tokens, uint64_t sequences) {
+  if (tokens > 1ull << 36 || sequences > 0x7fffffffull || few(tokens, sequences)) return 0;
+  uint64_t bytes;
+  lay_out(nullptr, tokens, sequences, false, &bytes);
+  return bytes;
+}
+uint64_t polar_b200_fpreference_loss_workspace_bytes(uint64_t tokens, uint64_t pairs) {
+  if (tokens > 1ull << 36 || pairs > 0x3fffffffull || few(tokens, 2 * pairs)) return 0;
+  uint64_t bytes;
+  lay_out(nullptr, tokens, 2 * pairs, true, &bytes);
+  return bytes;
+}
+
+int polar_b200_fpolicy_loss(const polar_b200_policy_batch* b, const polar_b200_policy_options* o, float* loss, float* gLogProb, float* gEntropy,
+                            void* workspace, uint64_t workspace_bytes, void* stream) {
+  clear_error();
+  if (!b || !o || !loss) return fail(POLAR_B200_ERR_INVALID, "fpolicy_loss: no batch, options or loss");
+  int rc = check_sequences(b->ids, b->offsets, b->id_type, b->tokens, b->sequences);
+  if (rc) return rc;
+  if (!(o->clip_low >= 0.f && o->clip_low <= 1.f && o->clip_high >= 0.f)) return fail(POLAR_B200_ERR_INVALID, "fpolicy_loss: 0 <= clip_low <= 1 and clip_high >= 0 are needed");
+  if (!(std::isfinite(o->kl_weight) && std::isfinite(o->entropy_weight) && std::isfinite(o->count) && o->count >= 0.f))
+    return fail(POLAR_B200_ERR_INVALID, "fpolicy_loss: finite weights and a count of zero or more are needed");
+  if (gEntropy && !b->entropy) return fail(POLAR_B200_ERR_INVALID, "fpolicy_loss: the entropy's gradient needs the entropy");
+  const uint64_t n = b->sequences ? b->tokens : 0;
+  if (n && (!b->logProb || !b->oldLogProb || !b->advantage)) return fail(POLAR_B200_ERR_INVALID, "null device pointer");
+  const uint64_t advantages = b->advantage_per_token ? b->tokens : b->sequences;
+  const struct { const void* p; uint64_t bytes; bool by_token; } read[] = {
+      {b->logProb, 4 * b->tokens, true}, {b->oldLogProb, 4 * b->tokens, true}, {b->refLogProb, 4 * b->tokens, true}, {b->entropy, 4 * b->tokens, true},
+      {b->advantage, 4 * advantages, b->advantage_per_token != 0}, {b->ids, id_bytes(b->id_type) * b->tokens, false},
+      {b->offsets, id_bytes(b->id_type) * (b->sequences + 1), false}};
+  for (const auto& r : read)
+    if (overlaps(gLogProb, 4 * b->tokens, r.p, r.bytes, r.by_token) || overlaps(gEntropy, 4 * b->tokens, r.p, r.bytes, r.by_token) ||
+        overlaps(loss, 20, r.p, r.bytes, false))
+      return fail(POLAR_B200_ERR_INVALID, "fpolicy_loss: what is written overlaps something else");
+  if (overlaps(gLogProb, 4 * b->tokens, gEntropy, 4 * b->tokens, false) || overlaps(loss, 20, gLogProb, 4 * b->tokens, false) ||
+      overlaps(loss, 20, gEntropy, 4 * b->tokens, false))
+    return fail(POLAR_B200_ERR_INVALID, "fpolicy_loss: what is written overlaps something else");
+  if (n == 0) return polar_b200_ffill(0.f, loss, 5, stream);
+  LaunchDeviceScope on(stream, loss);
+  Policy k = {};
+  k.logprob = b->logProb, k.old = b->oldLogProb, k.reference = b->refLogProb, k.entropy = b->entropy, k.advantage = b->advantage;
+  k.loss = loss, k.g_logprob = gLogProb, k.g_entropy = gEntropy;
+  k.high = 1.f + o->clip_high, k.low = 1.f - o->clip_low;
+  k.log_high = std::log1p((double)o->clip_high), k.log_low = o->clip_low == 1.f ? -std::numeric_limits<double>::infinity() : std::log1p(-(double)o->clip_low);
+  k.kl = b->refLogProb ? o->kl_weight : 0.f, k.bonus = b->entropy ? o->entropy_weight : 0.f, k.count = o->count;
+  k.by_sequence = o->by_sequence, k.per_token = b->advantage_per_token;
+  return with_ids(b->id_type, [&](auto id) {
+    using Id = decltype(id);
+    const Packed<Id> p = {static_cast<const Id*>(b->ids), static_cast<const Id*>(b->offsets), b->tokens, (uint32_t)b->sequences};
+    return run_policy(p, k, workspace, workspace_bytes, as_stream(stream));
+  });
+}
+
+int polar_b200_fpreference_loss(const float* logProb, const float* refLogProb, const void* ids, const void* offsets, int id_type, uint64_t tokens,
+                                uint64_t pairs, const polar_b200_preference_options* o, float* loss, float* rewards, float* gLogProb,
+                                void* workspace, uint64_t workspace_bytes, void* stream) {
+  clear_error();
+  if (!o || !loss) return fail(POLAR_B200_ERR_INVALID, "fpreference_loss: no options or loss");
+  if (pairs > 0x3fffffffull) return fail(POLAR_B200_ERR_INVALID, "too many tokens or sequences");
+  int rc = check_sequences(ids, offsets, id_type, tokens, 2 * pairs);
+  if (rc) return rc;
+  if (!(std::isfinite(o->beta) && std::isfinite(o->margin) && o->smoothing >= 0.f && o->smoothing <= 1.f && std::isfinite(o->count) && o->count >= 0.f))
+    return fail(POLAR_B200_ERR_INVALID, "fpreference_loss: finite beta and margin, 0 <= smoothing <= 1 and a count of zero or more are needed");
+  if (pairs && tokens && !logProb) return fail(POLAR_B200_ERR_INVALID, "null device pointer");
+  const uint64_t reward_bytes = 8 * pairs;
+  const struct { const void* p; uint64_t bytes; } read[] = {{logProb, 4 * tokens}, {refLogProb, 4 * tokens}, {ids, id_bytes(id_type) * tokens},
+                                                            {offsets, id_bytes(id_type) * (2 * pairs + 1)}};
+  for (const auto& r : read)
+    if (overlaps(gLogProb, 4 * tokens, r.p, r.bytes, &r < read + 2) || overlaps(rewards, reward_bytes, r.p, r.bytes, false) ||
+        overlaps(loss, 12, r.p, r.bytes, false))
+      return fail(POLAR_B200_ERR_INVALID, "fpreference_loss: what is written overlaps something else");
+  if (overlaps(rewards, reward_bytes, gLogProb, 4 * tokens, false) || overlaps(loss, 12, gLogProb, 4 * tokens, false) || overlaps(loss, 12, rewards, reward_bytes, false))
+    return fail(POLAR_B200_ERR_INVALID, "fpreference_loss: what is written overlaps something else");
+  if (pairs == 0) return polar_b200_ffill(0.f, loss, 3, stream);
+  LaunchDeviceScope on(stream, loss);
+  const Pairs k = {logProb, refLogProb, loss, rewards, gLogProb, o->beta, o->smoothing, o->margin, o->count, o->average};
+  return with_ids(id_type, [&](auto id) {
+    using Id = decltype(id);
+    const Packed<Id> p = {static_cast<const Id*>(ids), static_cast<const Id*>(offsets), tokens, (uint32_t)(2 * pairs)};
+    return run_pairs(p, k, workspace, workspace_bytes, as_stream(stream));
+  });
+}
+
+}  // extern "C"

@@ -16,7 +16,7 @@ import numbers
 import numpy as np
 import torch
 
-from .capi import AdamwOptions, AdamwTensor, binding, lib
+from .capi import AdamwOptions, AdamwTensor, PolicyBatch, PolicyOptions, PreferenceOptions, binding, lib
 
 
 def _ptr(t):
@@ -77,6 +77,17 @@ def _ids(t):
 
 def _present(*ts):
     return [t for t in ts if t is not None]
+
+
+def _packed(what, ids, offsets, *ts):
+    """The tokens and the sequences of a batch, and how its ids and offsets are held."""
+    _chk(*ts)
+    if _ids(ids) != _ids(offsets):
+        raise ValueError(f"{what}: ids and offsets are of one type")
+    _same_device(ids, offsets, *ts)
+    if offsets.numel() < 1:
+        raise ValueError(f"{what}: offsets are one more than the sequences")
+    return ids.numel(), offsets.numel() - 1, _ids(ids)
 
 
 class DeviceBuiltins:
@@ -326,6 +337,47 @@ class DeviceBuiltins:
                 options = AdamwOptions(float(lr), float(beta1), float(beta2), float(eps), int(step), _ptr(schedule))
                 self.lib.call("polar_b200_fadamw", tensors, len(weights), ctypes.byref(options), _stream(weights[0]))
         return weights
+
+    def fpolicy_loss(self, logprob, old_logprob, advantage, ids, offsets, loss, g_logprob=None, g_entropy=None, *, reference=None, entropy=None,
+                     clip_low=0.2, clip_high=0.2, kl_weight=0.0, entropy_weight=0.0, by_sequence=False, advantage_per_token=False, count=0.0):
+        """The clipped policy loss of packed sequences into loss[5] - the loss and, as means over the tokens that count, surrogate, KL term,
+        entropy, share of clipped tokens - and its gradients at the log probabilities and the entropies.  Sequence s has the tokens
+        [offsets[s], offsets[s + 1]), a token with an id below zero does not count; `reference`: log probabilities for the KL term.
+        The mean goes over the tokens or, by_sequence, over the sequences' means; `count` above zero is divided by in place of their number.
+        The advantage is one for each sequence or, advantage_per_token, for each token."""
+        if not self._native.fpolicy_loss(logprob, old_logprob, reference, entropy, advantage, ids, offsets, advantage_per_token, clip_low, clip_high,
+                                         kl_weight, entropy_weight, count, by_sequence, loss, g_logprob, g_entropy):
+            arrays = _present(logprob, old_logprob, reference, entropy, g_logprob, g_entropy)
+            tokens, sequences, kind = _packed("fpolicy_loss", ids, offsets, loss, advantage, *arrays)
+            _exactly("fpolicy_loss", tokens, *arrays)
+            _exactly("fpolicy_loss", tokens if advantage_per_token else sequences, advantage)
+            _exactly("fpolicy_loss", 5, loss)
+            if g_entropy is not None and entropy is None:
+                raise ValueError("fpolicy_loss: the entropy's gradient needs the entropy")
+            batch = PolicyBatch(_ptr(logprob), _ptr(old_logprob), _ptr(reference), _ptr(entropy), _ptr(advantage), _ptr(ids), _ptr(offsets), kind,
+                                int(bool(advantage_per_token)), tokens, sequences)
+            options = PolicyOptions(float(clip_low), float(clip_high), float(kl_weight), float(entropy_weight), float(count), int(bool(by_sequence)))
+            self.lib.call("polar_b200_fpolicy_loss", ctypes.byref(batch), ctypes.byref(options), _ptr(loss), _ptr(g_logprob), _ptr(g_entropy),
+                          None, 0, _stream(loss))
+        return loss
+
+    def fpreference_loss(self, logprob, ids, offsets, loss, rewards=None, g_logprob=None, *, reference=None, beta=0.1, smoothing=0.0, margin=0.0,
+                         average=False, count=0.0):
+        """The loss of pairs of packed sequences, 2i the chosen and 2i + 1 the rejected one, into loss[3] - the loss, the share of pairs in the
+        right order, their mean difference - with the sequences' rewards, beta times the sum (average: the mean) of logprob - reference over
+        the tokens that count, and the loss's gradient at the log probabilities.  `count` above zero is divided by in place of the pairs' number."""
+        if not self._native.fpreference_loss(logprob, reference, ids, offsets, beta, smoothing, margin, count, average, loss, rewards, g_logprob):
+            arrays = _present(logprob, reference, g_logprob)
+            tokens, sequences, kind = _packed("fpreference_loss", ids, offsets, loss, *_present(rewards), *arrays)
+            if sequences % 2:
+                raise ValueError("fpreference_loss: pairs of sequences")
+            _exactly("fpreference_loss", tokens, *arrays)
+            _exactly("fpreference_loss", sequences, rewards)
+            _exactly("fpreference_loss", 3, loss)
+            options = PreferenceOptions(float(beta), float(smoothing), float(margin), float(count), int(bool(average)))
+            self.lib.call("polar_b200_fpreference_loss", _ptr(logprob), _ptr(reference), _ptr(ids), _ptr(offsets), kind, tokens, sequences // 2,
+                          ctypes.byref(options), _ptr(loss), _ptr(rewards), _ptr(g_logprob), None, 0, _stream(loss))
+        return loss
 
     def device_status(self):
         return int(self.lib.cdll.polar_b200_device_status())

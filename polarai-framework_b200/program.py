@@ -53,7 +53,8 @@ class Program:
         return names
 
 
-_RESULTS = {"fdense_grad": 2, "flayernorm": 3, "flayernorm_grad": 3, "flogprob": 3, "flogprob_top": 5, "fadamw": 3, "fadamw8": 5}
+_RESULTS = {"fdense_grad": 2, "flayernorm": 3, "flayernorm_grad": 3, "flogprob": 3, "flogprob_top": 5, "fadamw": 3, "fadamw8": 5,
+            "fpolicy_loss": 3, "fpreference_loss": 3}
 _IN_PLACE = ("fadamw", "fadamw8")                            # these read what they write
 
 
