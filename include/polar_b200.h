@@ -520,6 +520,37 @@ int polar_b200_fpreference_loss(const float* logProb, const float* refLogProb, c
                                 float* rewards, float* gLogProb, void* workspace, uint64_t workspace_bytes, void* stream);
 uint64_t polar_b200_fpreference_loss_workspace_bytes(uint64_t tokens, uint64_t pairs);
 
+/* fmuon: one step of orthogonalised momentum over any number of matrices, in place.  For each of them, with g its gradient:
+ *   m <- momentum * m + g,   u = g + momentum * m (nesterov) or m,   X = u / |u| (the root of the sum of its squares; zeros stay zeros),
+ *   `steps` times  X <- a X + b G X + c G^2 X,  G = X X^T where rows <= cols, else X G with G = X^T X,
+ *   w <- w * (1 - lr * weight_decay) - lr * scale * X.
+ * With a, b, c = 3.4445, -4.7750, 2.0315 five rounds bring the singular values of X, whatever they were, to between 0.7 and 1.2.
+ * A tensor is `matrices` matrices of [rows, cols] behind one another, each by itself.  The polynomial may let no singular value pass 1.4, beginning
+ * at up to 1 (POLAR_B200_ERR_INVALID else).  Products keep 22 bits of their operands and sum in fp32; the results agree with
+ * exact products to some 1e-5 of the update.  A matrix with a gradient that is not finite ends as NaNs, and it alone.
+ * What is written may overlap nothing else that the call names.  With `schedule` (device memory, two floats as fadamw's: the number of the step, which is not
+ * used, and lr) lr is read on the device.  The shorter side is at most 32768, the longer one 2^20.
+ * Scratch as for fmatmul, 256-byte aligned: some 20 bytes per element, for at most 3 GiB of it or one matrix at a time.
+ * As a builtin: T gradient[..., rows, cols], T schedule[2], f32 momentum, f32 nesterov (0 or 1), f32 steps, f32 weight_decay, f32 scale, T weights,
+ * T momentum (two results), with the polynomial above.  In a program, fmuon builtins in a row share their launches. */
+typedef struct polar_b200_muon_tensor {
+  float* weights;
+  const float* gradient;
+  float* momentum;
+  uint64_t matrices, rows, cols;
+  float weight_decay, scale;
+} polar_b200_muon_tensor;
+typedef struct polar_b200_muon_options {
+  float lr, momentum;
+  int nesterov;
+  uint32_t steps;
+  float a, b, c;
+  const float* schedule;
+} polar_b200_muon_options;
+int polar_b200_fmuon(const polar_b200_muon_tensor* tensors, uint64_t count, const polar_b200_muon_options* options,
+                     void* workspace, uint64_t workspace_bytes, void* stream);
+uint64_t polar_b200_fmuon_workspace_bytes(const polar_b200_muon_tensor* tensors, uint64_t count);
+
 /* Sum of n floats into *sum (a device double, ADDED to: clear it first), with
  * warp-shuffle + one atomic per block.  Used to report the scalar mean of an
  * elementwise flogloss output; the reference has no reduction builtin. */
@@ -556,7 +587,7 @@ typedef struct polar_b200_arg {
  * here), and
  * the extended "fsigmoid_grad", "fsigmoid_logloss_grad", "fmatmul_x_y_sigmoid",
  * "fmatmul_x_y_sigmoid_grad", "fmatmul_t_f_rows", "fdense_grad", "fsum", "flayernorm", "flayernorm_grad",
- * "flogprob", "flogprob_top", "flogprob_grad", "fadamw", "fadamw8", "fpolicy_loss", "fpreference_loss".
+ * "flogprob", "flogprob_top", "flogprob_grad", "fadamw", "fadamw8", "fpolicy_loss", "fpreference_loss", "fmuon".
  *
  * Launches the builtin called `nativeKernelName` ("fadd", "fmatmul_t_f", ...)
  * on arguments in LaunchCommand order; this is what Device::launch forwards to

@@ -55,6 +55,15 @@ class PreferenceOptions(ctypes.Structure):
     _fields_ = [("beta", _f), ("smoothing", _f), ("margin", _f), ("count", _f), ("average", _i)]
 
 
+class MuonTensor(ctypes.Structure):
+    _fields_ = [("weights", _p), ("gradient", _p), ("momentum", _p), ("matrices", _u64), ("rows", _u64), ("cols", _u64), ("weight_decay", _f),
+                ("scale", _f)]
+
+
+class MuonOptions(ctypes.Structure):
+    _fields_ = [("lr", _f), ("momentum", _f), ("nesterov", _i), ("steps", ctypes.c_uint32), ("a", _f), ("b", _f), ("c", _f), ("schedule", _p)]
+
+
 SIGNATURES = {
     "polar_b200_last_error": (ctypes.c_char_p, []),
     "polar_b200_version": (_i, []),
@@ -106,6 +115,8 @@ SIGNATURES = {
     "polar_b200_fpolicy_loss_workspace_bytes": (_u64, [_u64, _u64]),
     "polar_b200_fpreference_loss": (_i, [_p, _p, _p, _p, _i, _u64, _u64, ctypes.POINTER(PreferenceOptions), _p, _p, _p, _p, _u64, _p]),
     "polar_b200_fpreference_loss_workspace_bytes": (_u64, [_u64, _u64]),
+    "polar_b200_fmuon": (_i, [ctypes.POINTER(MuonTensor), _u64, ctypes.POINTER(MuonOptions), _p, _u64, _p]),
+    "polar_b200_fmuon_workspace_bytes": (_u64, [ctypes.POINTER(MuonTensor), _u64]),
     "polar_b200_fsum": (_i, [_p, _p, _u64, _p]),
     "polar_b200_fsum_f32": (_i, [_p, _p, _u64, _p, _u64, _p]),
     "polar_b200_fsum_f32_workspace_bytes": (_u64, [_u64]),

@@ -1,0 +1,831 @@
+// One step of orthogonalised momentum over many matrices: the momentum's matrix U is brought close to the nearest one with orthonormal rows
+// (or columns) by rounds of  X <- a X + b G X + c G^2 X,  G = X X^T (of the shorter side),  X = U / |U| at the beginning, and taken off the weights.
+//
+// Every round is three matrix products, G, P = a + b G + c G G and P X, on the tensor cores.  They hold their operands as PAIRS of
+// fp16 numbers, hi + lo with 22 bits between them, and multiply hi hi + lo hi + hi lo with sums in fp32: three products at the fp16 rate,
+// twice as fast as three of TF32 and as exact, which is possible because the range of all values is known.  No singular value of X passes
+// kBound on the way, so that no entry of X, G or P leaves fp16 when they are held times the powers of two kX, kG and kP; what lo cannot
+// hold below 2^-24 is small against the largest entries.  The pairs are written by the product before, so that a product needs no pass over its
+// operands: TMA brings both planes of a tile in one box, and nothing but tcgen05.mma touches shared memory.
+// G and P are symmetric: tiles below the diagonal are not computed, the epilogue of the others writes both halves.
+//
+// All matrices of a step take part in each launch: those of one shape lie behind one another and share a tensor map, and a launch's tiles
+// are those of all shapes.
+#include <cuda.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cmath>
+#include <exception>
+#include <mutex>
+#include <utility>
+#include <vector>
+
+#include "rows.cuh"
+#include "tc_ptx.cuh"
+
+namespace polar_b200 {
+namespace {
+using namespace tc;
+
+constexpr float kX = 32768.f, kG = 32768.f, kP = 16384.f;  // what X, G and P are held times
+constexpr float kBound = 1.4f, kBoundP = 3.98f;            // largest singular value of X, of P: 1.4^2 * 2^15 and 3.98 * 2^14 are below 65504
+
+// ---- the passes before the products
+
+struct Target {                                            // a matrix's weights, for the last product
+  float* weights;
+  float decay, scale;
+};
+struct Matrix {
+  float* weights;
+  const float* gradient;
+  float* momentum;
+  __half* x;                                               // hi plane; lo `plane` behind it
+  uint64_t plane, count;
+  uint32_t cols, pitch, chunk;                             // chunk: elements per CTA
+  uint32_t first;                                          // its first chunk
+  float decay, scale;
+};
+template <int N>
+struct Table {
+  uint32_t count;
+  uint32_t chunks_before, matrices_before;                 // of tables launched before
+  float momentum;
+  int nesterov;
+  double* partial;                                         // of each chunk: the sum of its squares
+  Target* targets;
+  Matrix m[N];
+};
+constexpr int kFewMatrices = 16, kManyMatrices = 400;
+static_assert(sizeof(Table<kManyMatrices>) <= 32764, "kernel parameters");
+constexpr int kThreads = 256;
+constexpr uint32_t kChunk = 4096, kMostChunks = 512;       // elements of a CTA, or more where a matrix has more than 512 times as many
+
+template <int N>
+__device__ __forceinline__ uint32_t matrix_of(const Table<N>& t, uint32_t chunk) {
+  uint32_t lo = 0, end = t.count;
+  while (end - lo > 1) {
+    const uint32_t middle = (lo + end) / 2;
+    if (t.m[middle].first <= chunk) lo = middle;
+    else end = middle;
+  }
+  return lo;
+}
+__device__ __forceinline__ double block_sum(double v, double* slots) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0;
+#pragma unroll
+  for (int i = 0; i < kThreads / 32; ++i) v += slots[i];
+  return v;
+}
+
+// m <- momentum * m + g, and the sum of the squares of u = g + momentum * m (nesterov) or m: in 64 bits, where no square of an fp32 number
+// overflows or vanishes.
+template <int N>
+__global__ void __launch_bounds__(kThreads) momentum_kernel(const __grid_constant__ Table<N> t) {
+  __shared__ double slots[kThreads / 32];
+  pdl_enter();
+  const uint32_t at = matrix_of(t, blockIdx.x);
+  const Matrix& m = t.m[at];
+  const uint32_t chunk = blockIdx.x - m.first;
+  if (chunk == 0 && threadIdx.x == 0) t.targets[t.matrices_before + at] = Target{m.weights, m.decay, m.scale};
+  const uint64_t from = (uint64_t)chunk * m.chunk, to = min(from + m.chunk, m.count);
+  const bool vectors = ((reinterpret_cast<uintptr_t>(m.gradient) | reinterpret_cast<uintptr_t>(m.momentum)) & 15) == 0;
+  double sum = 0;
+  auto one = [&](float g, float& v) {
+    v = fmaf(t.momentum, v, g);
+    const float u = t.nesterov ? fmaf(t.momentum, v, g) : v;
+    sum += (double)u * (double)u;
+  };
+  if (vectors) {
+#pragma unroll 4
+    for (uint64_t i = from + 4 * threadIdx.x; i < to; i += 4 * kThreads) {
+      if (i + 4 <= to) {
+        const float4 g = *reinterpret_cast<const float4*>(m.gradient + i);
+        float4 v = *reinterpret_cast<const float4*>(m.momentum + i);
+        one(g.x, v.x), one(g.y, v.y), one(g.z, v.z), one(g.w, v.w);
+        *reinterpret_cast<float4*>(m.momentum + i) = v;
+      } else {
+        for (uint64_t e = i; e < to; ++e) one(m.gradient[e], m.momentum[e]);
+      }
+    }
+  } else {
+#pragma unroll 4
+    for (uint64_t i = from + threadIdx.x; i < to; i += kThreads) one(m.gradient[i], m.momentum[i]);
+  }
+  sum = block_sum(sum, slots);
+  if (threadIdx.x == 0) t.partial[t.chunks_before + blockIdx.x] = sum;
+}
+
+// A value times a power of two as a pair of fp16 numbers.
+__device__ __forceinline__ void split(float v, __half* hi, __half* lo) {
+  *hi = __float2half_rn(v);
+  *lo = __float2half_rn(v - __half2float(*hi));
+}
+
+// X = u / |u| as pairs, zeros for a matrix of zeros.
+template <int N>
+__global__ void __launch_bounds__(kThreads) begin_kernel(const __grid_constant__ Table<N> t) {
+  __shared__ double slots[kThreads / 32];
+  pdl_enter();
+  const uint32_t at = matrix_of(t, blockIdx.x);
+  const Matrix& m = t.m[at];
+  const uint32_t chunk = blockIdx.x - m.first, chunks = (uint32_t)((m.count + m.chunk - 1) / m.chunk);
+  double sum = 0;
+  for (uint32_t i = threadIdx.x; i < chunks; i += kThreads) sum += t.partial[t.chunks_before + m.first + i];
+  sum = block_sum(sum, slots);
+  const double by = sum == 0 ? 0 : (double)kX / sqrt(sum);
+  const uint64_t from = (uint64_t)chunk * m.chunk, to = min(from + m.chunk, m.count);
+  const bool vectors = ((reinterpret_cast<uintptr_t>(m.gradient) | reinterpret_cast<uintptr_t>(m.momentum)) & 15) == 0 && (m.cols & 3) == 0;
+  auto value = [&](float g, float v) { return (float)((double)(t.nesterov ? fmaf(t.momentum, v, g) : v) * by); };
+  if (vectors) {
+#pragma unroll 2
+    for (uint64_t i = from + 4 * threadIdx.x; i < to; i += 4 * kThreads) {
+      const float4 g = *reinterpret_cast<const float4*>(m.gradient + i), v = *reinterpret_cast<const float4*>(m.momentum + i);
+      const uint64_t row = i / m.cols;
+      __half* x = m.x + row * m.pitch + (i - row * m.cols);
+      union { __half h[4]; uint2 bits; } hi, lo;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) split(value((&g.x)[k], (&v.x)[k]), &hi.h[k], &lo.h[k]);
+      *reinterpret_cast<uint2*>(x) = hi.bits;
+      *reinterpret_cast<uint2*>(x + m.plane) = lo.bits;
+    }
+    return;
+  }
+#pragma unroll 4
+  for (uint64_t i = from + threadIdx.x; i < to; i += kThreads) {
+    const uint64_t row = i / m.cols;
+    __half* x = m.x + row * m.pitch + (i - row * m.cols);
+    split(value(m.gradient[i], m.momentum[i]), x, x + m.plane);
+  }
+}
+
+// ---- the products
+
+constexpr int BM = 128, BK = 32;
+constexpr int kEpilogueWarps = 8, kProductThreads = 32 * (2 + kEpilogueWarps);
+template <int BN>
+struct Cfg {
+  static constexpr uint32_t kAPlane = BM * BK * 2, kBPlane = BN * BK * 2;
+  static constexpr uint32_t kStageBytes = 2 * (kAPlane + kBPlane);
+  static constexpr int kStages = (int)((200u * 1024u) / kStageBytes);
+  static constexpr uint32_t kTileBytes = kStages * kStageBytes;
+  static constexpr uint32_t kSmemBytes = kTileBytes + 1024 + 256;
+};
+
+enum Kind : int { kGram, kPolynomial, kRound, kUpdate };
+
+struct Shape {                                             // the matrices of one shape, in one product
+  CUtensorMap a, b;
+  uint32_t m, n, k;
+  uint32_t tiles_m, tiles_n, tiles;                        // tiles: of one matrix
+  uint32_t first_tile;                                     // of the launch
+  int a_mn, b_mn;                                          // operands whose rows are not contiguous along k
+  __half* out;                                             // matrix z: planes 2 z (hi) and 2 z + 1 (lo)
+  const __half* add;                                       // of the same layout
+  uint64_t plane;
+  uint32_t pitch;
+  uint32_t first_target;
+};
+constexpr int kShapes = 16;
+struct Product {
+  uint32_t shapes, tiles;
+  int kind;
+  float by, add_by, diagonal;                              // result = by * sum + add_by * add + diagonal (on the diagonal)
+  float lr;
+  const float* schedule;
+  const Target* targets;
+  int* status;
+  unsigned long long wait_ns;
+  Shape s[kShapes];
+};
+struct Place {
+  uint32_t shape, z;
+  int m0, n0;
+};
+// The launch's tile t.  A symmetric product has the tiles that reach above the diagonal, row by row; else 16 tile rows walk the columns
+// together and share their operands in L2.
+template <int BN>
+__device__ __forceinline__ Place place_of(const Product& p, uint32_t t) {
+  Place at;
+  at.shape = 0;
+  while (at.shape + 1 < p.shapes && p.s[at.shape + 1].first_tile <= t) ++at.shape;
+  const Shape& s = p.s[at.shape];
+  t -= s.first_tile;
+  at.z = t / s.tiles;
+  t -= at.z * s.tiles;
+  if (p.kind <= kPolynomial) {
+    uint32_t i = 0, skip = 0;
+    while (t >= s.tiles_n - skip) {
+      t -= s.tiles_n - skip;
+      ++i;
+      skip = i * BM / BN;
+    }
+    at.m0 = (int)(i * BM);
+    at.n0 = (int)((skip + t) * BN);
+  } else {
+    const uint32_t per = 16 * s.tiles_n, g = t / per, rows = min(s.tiles_m - g * 16, 16u), r = t - g * per;
+    at.m0 = (int)((g * 16 + r % rows) * BM);
+    at.n0 = (int)(r / rows * BN);
+  }
+  return at;
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map), "r"(bar),
+      "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_f16(uint32_t d_tmem, Operand a, uint32_t a_units, Operand b, uint32_t b_units, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %2};\n\t"
+      "mov.b64 db, {%3, %4};\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(d_tmem),
+      "r"(a.lo + a_units), "r"(a.hi), "r"(b.lo + b_units), "r"(b.hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// fp32 sums of fp16 operands (format 0 of both).
+__device__ __forceinline__ uint32_t f16_idesc(int n, int a_mn, int b_mn) {
+  return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+}
+__device__ __forceinline__ void st_v8(void* dst, const uint32_t* r) { st_global_v8(static_cast<float*>(dst), r); }
+
+// One CTA per SM walks 128 x BN tiles; two accumulators in tensor memory, so that a tile's epilogue runs beside the next one's products.
+//   warp 0     TMA: both planes of a slab of 32 k of each operand, one instruction each.  An operand that is contiguous along k is K-major
+//              (rows of 64 bytes in the 64-byte swizzle), else MN-major (chunks of 64 columns, 128-byte swizzle, a row per k).
+//   warp 1     tcgen05.mma: per 16 k  hi hi, lo hi, hi lo.
+//   warps 2-9  epilogue: two warps to each 32 rows of the accumulator, half of the columns each.
+// Every wait is bounded; when one gives up, all roles leave, and the status word holds its code (7xx).
+template <int BN>
+__global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __grid_constant__ Product p) {
+  using C = Cfg<BN>;
+  constexpr int S = C::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+  const uint32_t bar_base = smem_base + C::kTileBytes;
+  auto full = [&](int s) { return bar_base + 8u * s; };
+  auto empty = [&](int s) { return bar_base + 8u * (S + s); };
+  auto acc_full = [&](int a) { return bar_base + 8u * (2 * S + a); };
+  auto acc_empty = [&](int a) { return bar_base + 8u * (2 * S + 2 + a); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + C::kTileBytes + 8 * (2 * S + 4));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = uniform_warp();
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
+    for (int a = 0; a < 2; ++a) mbar_init(acc_full(a), 1), mbar_init(acc_empty(a), kEpilogueWarps);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), 2 * BN);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  pdl_enter();
+
+  if (warp == 0) {
+    const bool leader = elect_one();
+    int s = 0;
+    uint32_t ph = 1;
+    bool ok = true;
+    for (uint32_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x) {
+      const Place at = place_of<BN>(p, t);
+      const Shape& q = p.s[at.shape];
+      const int plane = (int)(2 * at.z), slabs = (int)((q.k + BK - 1) / BK);
+      for (int kb = 0; kb < slabs; ++kb) {
+        if (!mbar_wait(empty(s), ph, abort_flag, p.status, 701, p.wait_ns)) { ok = false; break; }
+        if (leader) {
+          const uint32_t stage = smem_base + s * C::kStageBytes;
+          mbar_expect_tx(full(s), C::kStageBytes);
+          if (q.a_mn) tma_load_4d(stage, &q.a, full(s), 0, kb * BK, at.m0 / 64, plane);
+          else tma_load_3d(stage, &q.a, full(s), kb * BK, at.m0, plane);
+          if (q.b_mn) tma_load_4d(stage + 2 * C::kAPlane, &q.b, full(s), 0, kb * BK, at.n0 / 64, plane);
+          else tma_load_3d(stage + 2 * C::kAPlane, &q.b, full(s), kb * BK, at.n0, plane);
+        }
+        if (++s == S) s = 0, ph ^= 1;
+      }
+    }
+  } else if (warp == 1) {
+    const bool leader = elect_one();
+    int s = 0;
+    uint32_t ph = 0, tile = 0;
+    bool ok = true;
+    for (uint32_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x, ++tile) {
+      const Shape& q = p.s[place_of<BN>(p, t).shape];
+      const int slabs = (int)((q.k + BK - 1) / BK);
+      const uint32_t idesc = f16_idesc(BN, q.a_mn, q.b_mn);
+      // K-major: 64-byte swizzle (layout 4), groups of 8 rows 512 bytes apart, 16 k 32 bytes on.  MN-major: 128-byte swizzle (layout 2), chunks
+      // of 64 columns BK rows apart, groups of 8 k 1024 bytes, 16 k 2048 bytes on.
+      const Operand a_op = q.a_mn ? make_desc(0, BK * 128, 1024, 2) : make_desc(0, 16, 512, 4);
+      const Operand b_op = q.b_mn ? make_desc(0, BK * 128, 1024, 2) : make_desc(0, 16, 512, 4);
+      const uint32_t a_step = (q.a_mn ? 2048u : 32u) >> 4, b_step = (q.b_mn ? 2048u : 32u) >> 4;
+      const uint32_t as = tile & 1u, acc = tmem_base + as * BN;
+      ok = mbar_wait(acc_empty(as), ((tile >> 1) & 1u) ^ 1u, abort_flag, p.status, 702, p.wait_ns);
+      if (!ok) break;
+      tc_fence_after();
+      for (int kb = 0; kb < slabs; ++kb) {
+        ok = mbar_wait(full(s), ph, abort_flag, p.status, 703, p.wait_ns);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t a_hi = ((smem_base & 0x3FFFFu) + s * C::kStageBytes) >> 4, a_lo = a_hi + (C::kAPlane >> 4);
+        const uint32_t b_hi = a_lo + (C::kAPlane >> 4), b_lo = b_hi + (C::kBPlane >> 4);
+        if (leader) {
+#pragma unroll
+          for (int kk = 0; kk < BK / 16; ++kk) {
+            tc_mma_f16(acc, a_op, a_hi + kk * a_step, b_op, b_hi + kk * b_step, idesc, kb || kk ? 1u : 0u);
+            tc_mma_f16(acc, a_op, a_lo + kk * a_step, b_op, b_hi + kk * b_step, idesc, 1u);
+            tc_mma_f16(acc, a_op, a_hi + kk * a_step, b_op, b_lo + kk * b_step, idesc, 1u);
+          }
+          tc_commit(empty(s));
+        }
+        if (++s == S) s = 0, ph ^= 1;
+      }
+      if (ok && leader) tc_commit(acc_full(as));
+    }
+  } else {
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const float lr = p.kind == kUpdate ? (p.schedule ? p.schedule[1] : p.lr) : 0.f;
+    uint32_t tile = 0;
+    for (uint32_t t = blockIdx.x; t < p.tiles; t += gridDim.x, ++tile) {
+      const Place at = place_of<BN>(p, t);
+      const Shape& q = p.s[at.shape];
+      const uint32_t as = tile & 1u;
+      if (!mbar_wait(acc_full(as), (tile >> 1) & 1u, abort_flag, p.status, 704, p.wait_ns)) break;
+      tc_fence_after();
+      const uint32_t r0 = (uint32_t)at.m0 + quarter * 32, row = r0 + lane;
+      __half* const hi_plane = q.out + 2 * at.z * q.plane;
+      Target target = {};
+      if (p.kind == kUpdate) target = p.targets[q.first_target + at.z];
+      const float keep = 1.f - lr * target.decay, rate = p.by * lr * target.scale;
+      const bool vectors = (q.n & 3) == 0 && (reinterpret_cast<uintptr_t>(target.weights) & 15) == 0;
+#pragma unroll 1
+      for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
+        const uint32_t c0 = (uint32_t)at.n0 + c;
+        if (c0 >= q.n || r0 >= q.m) break;
+        if (p.kind <= kPolynomial && c0 < r0) continue;      // below the diagonal: written by the block above it
+        uint32_t r[32];
+        __syncwarp();
+        tmem_ld_32x32(tmem_base + as * BN + c + ((uint32_t)(quarter * 32) << 16), r);
+        tmem_ld_wait();
+        if (p.kind == kUpdate) {
+          float* w = target.weights + (uint64_t)row * q.n + c0;
+          if (row >= q.m) {
+          } else if (vectors && c0 + 32 <= q.n) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              float4 v = *reinterpret_cast<const float4*>(w + j);
+              v.x = v.x * keep - rate * __uint_as_float(r[j]), v.y = v.y * keep - rate * __uint_as_float(r[j + 1]);
+              v.z = v.z * keep - rate * __uint_as_float(r[j + 2]), v.w = v.w * keep - rate * __uint_as_float(r[j + 3]);
+              *reinterpret_cast<float4*>(w + j) = v;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c0 + j < q.n) w[j] = w[j] * keep - rate * __uint_as_float(r[j]);
+          }
+          continue;
+        }
+        const uint64_t place = (uint64_t)row * q.pitch + c0;
+        uint32_t hi[16], lo[16];                           // two columns in each
+        if (p.kind == kPolynomial) {
+          const __half* add = q.add + 2 * at.z * q.plane + place;
+          if (row < q.m) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint4 h = *reinterpret_cast<const uint4*>(add + 8 * j), l = *reinterpret_cast<const uint4*>(add + q.plane + 8 * j);
+              hi[4 * j] = h.x, hi[4 * j + 1] = h.y, hi[4 * j + 2] = h.z, hi[4 * j + 3] = h.w;
+              lo[4 * j] = l.x, lo[4 * j + 1] = l.y, lo[4 * j + 2] = l.z, lo[4 * j + 3] = l.w;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float2 h = __half22float2(*reinterpret_cast<__half2*>(&hi[j])), l = __half22float2(*reinterpret_cast<__half2*>(&lo[j]));
+            float a = fmaf(p.by, __uint_as_float(r[2 * j]), p.add_by * (h.x + l.x));
+            float b = fmaf(p.by, __uint_as_float(r[2 * j + 1]), p.add_by * (h.y + l.y));
+            if (c0 + 2 * j == row) a += p.diagonal;
+            if (c0 + 2 * j + 1 == row) b += p.diagonal;
+            r[2 * j] = __float_as_uint(a), r[2 * j + 1] = __float_as_uint(b);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(p.by * __uint_as_float(r[j]));
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float a = __uint_as_float(r[2 * j]), b = __uint_as_float(r[2 * j + 1]);
+          const __half2 h = __floats2half2_rn(a, b);
+          const float2 f = __half22float2(h);
+          const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+          hi[j] = *reinterpret_cast<const uint32_t*>(&h), lo[j] = *reinterpret_cast<const uint32_t*>(&l);
+        }
+        if (row < q.m) {                                   // (columns behind the last one lie in the row's padding)
+          __half* o = hi_plane + place;
+          st_v8(o, hi), st_v8(o + 16, hi + 8);
+          st_v8(o + q.plane, lo), st_v8(o + q.plane + 16, lo + 8);
+        }
+        if (p.kind <= kPolynomial && c0 > r0) {            // its mirror image: a column of the block is a row there, 32 lanes side by side
+          unsigned short* o = reinterpret_cast<unsigned short*>(hi_plane) + (uint64_t)c0 * q.pitch + row;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if (c0 + j < q.n) {
+              o[(uint64_t)j * q.pitch] = (unsigned short)(hi[j / 2] >> (j & 1) * 16);
+              o[(uint64_t)j * q.pitch + q.plane] = (unsigned short)(lo[j / 2] >> (j & 1) * 16);
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty(as));
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    // let copies and products in flight finish before the tensor memory goes away
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000ll) { }
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 2 * BN);
+  }
+}
+
+// ---- host side
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static EncodeTiled fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiled>(p);
+  });
+  return fn;
+}
+
+// `planes` matrices of fp16 [rows][cols], rows `pitch` (a multiple of 64) apart.  MN-major boxes are chunks of 64 columns: the last one may
+// reach into a row's padding, whose values end in rows or columns of a product that nobody reads.
+int make_map(CUtensorMap* map, const __half* base, uint64_t rows, uint64_t cols, uint64_t pitch, uint64_t planes, bool mn, uint32_t tile) {
+  EncodeTiled encode = encode_tiled();
+  if (!encode) return fail(POLAR_B200_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  const cuuint32_t unit[4] = {1, 1, 1, 1};
+  CUresult r;
+  if (mn) {
+    const cuuint64_t dims[4] = {64, rows, pitch / 64, planes}, strides[3] = {pitch * 2, 128, rows * pitch * 2};
+    const cuuint32_t box[4] = {64, BK, tile / 64, 2};
+    r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<__half*>(base), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  } else {
+    const cuuint64_t dims[3] = {cols, rows, planes}, strides[2] = {pitch * 2, rows * pitch * 2};
+    const cuuint32_t box[3] = {BK, tile, 2};
+    r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(base), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  }
+  return r == CUDA_SUCCESS ? POLAR_B200_OK : fail(POLAR_B200_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+}
+
+struct One {                                               // a matrix of the call
+  float* weights;
+  const float* gradient;
+  float* momentum;
+  uint64_t rows, cols;
+  float decay, scale;
+};
+struct Kin {                                               // the matrices of one shape
+  uint64_t rows, cols, count, first;                       // first: among the sorted matrices
+  uint64_t pitch, side, side_pitch;                        // side: the shorter one
+  __half *x[2], *g, *p;
+};
+uint64_t up64(uint64_t n) { return (n + 63) / 64 * 64; }
+uint64_t up256(uint64_t n) { return (n + 255) & ~255ull; }
+uint64_t chunk_of(uint64_t count) {
+  const uint64_t each = (count + kMostChunks - 1) / kMostChunks;
+  return each <= kChunk ? kChunk : (each + kChunk - 1) / kChunk * kChunk;
+}
+uint64_t bytes_of(uint64_t rows, uint64_t cols) {          // of one matrix: X twice, G and P, two planes each
+  const uint64_t side = std::min(rows, cols);
+  return 2 * 2 * 2 * (rows * up64(cols) + side * up64(side)) + 4 * 256;
+}
+// What one group of matrices may take; a step of more is done in several.
+constexpr uint64_t kGroupBytes = 3ull << 30;
+
+// Lays out a group that is sorted by shape, in what lies behind `base`; its bytes.
+uint64_t lay_out(char* base, const std::vector<One>& all, size_t from, size_t to, std::vector<Kin>* kin, double** partial, Target** targets) {
+  uint64_t at = 0, chunks = 0;
+  auto take = [&](uint64_t n) {
+    char* p = base + at;
+    at += up256(n);
+    return p;
+  };
+  for (size_t i = from; i < to; ++i) {
+    const One& o = all[i];
+    chunks += (o.rows * o.cols + chunk_of(o.rows * o.cols) - 1) / chunk_of(o.rows * o.cols);
+    if (kin->empty() || kin->back().rows != o.rows || kin->back().cols != o.cols) {
+      const uint64_t side = std::min(o.rows, o.cols);
+      kin->push_back(Kin{o.rows, o.cols, 0, i - from, up64(o.cols), side, up64(side), {nullptr, nullptr}, nullptr, nullptr});
+    }
+    ++kin->back().count;
+  }
+  *partial = reinterpret_cast<double*>(take(chunks * sizeof(double)));
+  *targets = reinterpret_cast<Target*>(take((to - from) * sizeof(Target)));
+  for (Kin& k : *kin) {
+    for (int b = 0; b < 2; ++b) k.x[b] = reinterpret_cast<__half*>(take(k.count * 4 * k.rows * k.pitch));
+    k.g = reinterpret_cast<__half*>(take(k.count * 4 * k.side * k.side_pitch));
+    k.p = reinterpret_cast<__half*>(take(k.count * 4 * k.side * k.side_pitch));
+  }
+  return at;
+}
+
+template <int N>
+int launch_tables(const std::vector<One>& all, size_t from, size_t to, const std::vector<Kin>& kin, const polar_b200_muon_options& o, double* partial,
+                  Target* targets, cudaStream_t st, bool begin) {
+  static thread_local Table<N> t;
+  size_t k = 0, i = from;
+  uint32_t chunks_before = 0;
+  while (i < to) {
+    t.count = 0;
+    t.chunks_before = chunks_before, t.matrices_before = (uint32_t)(i - from);
+    t.momentum = o.momentum, t.nesterov = o.nesterov, t.partial = partial, t.targets = targets;
+    uint32_t chunks = 0;
+    for (; i < to && t.count < N; ++i) {
+      while (k + 1 < kin.size() && i - from >= kin[k + 1].first) ++k;
+      const One& q = all[i];
+      const uint64_t count = q.rows * q.cols, plane = q.rows * kin[k].pitch;
+      t.m[t.count++] = Matrix{q.weights, q.gradient, q.momentum, kin[k].x[0] + 2 * (i - from - kin[k].first) * plane, plane, count, (uint32_t)q.cols,
+                              (uint32_t)kin[k].pitch, (uint32_t)chunk_of(count), chunks, q.decay, q.scale};
+      chunks += (uint32_t)((count + chunk_of(count) - 1) / chunk_of(count));
+    }
+    const int rc = begin ? launch_large("fmuon: X", begin_kernel<N>, dim3(chunks), kThreads, st, t)
+                         : launch_large("fmuon: momentum", momentum_kernel<N>, dim3(chunks), kThreads, st, t);
+    if (rc) return rc;
+    chunks_before += chunks;
+  }
+  return POLAR_B200_OK;
+}
+
+template <int BN>
+int launch_product(const std::vector<Kin>& kin, int kind, int from_x, const polar_b200_muon_options& o, const Target* targets, int* status, cudaStream_t st) {
+  static thread_local Product p;
+  p.kind = kind;
+  p.lr = o.lr, p.schedule = o.schedule, p.targets = targets, p.status = status, p.wait_ns = wait_limit_ns(2000000000ull);
+  p.add_by = p.diagonal = 0.f;
+  switch (kind) {
+    case kGram: p.by = kG / (kX * kX); break;
+    case kPolynomial: p.by = o.c * (kP / (kG * kG)), p.add_by = o.b * (kP / kG), p.diagonal = o.a * kP; break;
+    case kRound: p.by = 1.f / kP; break;
+    default: p.by = 1.f / (kP * kX);
+  }
+  for (size_t k = 0; k < kin.size();) {
+    p.shapes = p.tiles = 0;
+    for (; k < kin.size() && p.shapes < kShapes; ++k) {
+      const Kin& q = kin[k];
+      const bool wide = q.rows <= q.cols, square = kind <= kPolynomial;
+      Shape& s = p.s[p.shapes];
+      int rc = POLAR_B200_OK;
+      auto x = [&](CUtensorMap* map, bool mn, uint32_t tile) { return make_map(map, q.x[from_x], q.rows, q.cols, q.pitch, 2 * q.count, mn, tile); };
+      auto symmetric = [&](CUtensorMap* map, const __half* t, uint32_t tile) {
+        return make_map(map, t, q.side, q.side, q.side_pitch, 2 * q.count, false, tile);
+      };
+      s.a_mn = s.b_mn = 0;
+      s.add = nullptr;
+      if (kind == kGram) {                                 // X X^T, or X^T X
+        s.m = s.n = (uint32_t)q.side, s.k = (uint32_t)std::max(q.rows, q.cols);
+        s.a_mn = s.b_mn = !wide;
+        rc = x(&s.a, !wide, BM);
+        if (!rc) rc = x(&s.b, !wide, BN);
+        s.out = q.g;
+      } else if (kind == kPolynomial) {
+        s.m = s.n = s.k = (uint32_t)q.side;
+        rc = symmetric(&s.a, q.g, BM);
+        if (!rc) rc = symmetric(&s.b, q.g, BN);
+        s.out = q.p, s.add = q.g;
+      } else {                                             // P X, or X P
+        s.m = (uint32_t)q.rows, s.n = (uint32_t)q.cols, s.k = (uint32_t)q.side;
+        s.b_mn = wide;
+        rc = wide ? symmetric(&s.a, q.p, BM) : x(&s.a, false, BM);
+        if (!rc) rc = wide ? x(&s.b, true, BN) : symmetric(&s.b, q.p, BN);
+        s.out = q.x[from_x ^ 1];
+      }
+      if (rc) return rc;
+      s.pitch = (uint32_t)(square ? q.side_pitch : q.pitch);
+      s.plane = square ? q.side * q.side_pitch : q.rows * q.pitch;
+      s.first_target = (uint32_t)q.first;
+      s.tiles_m = (s.m + BM - 1) / BM, s.tiles_n = (s.n + BN - 1) / BN;
+      s.tiles = 0;
+      for (uint32_t i = 0; i < s.tiles_m; ++i) s.tiles += s.tiles_n - (square ? i * BM / BN : 0);
+      s.first_tile = p.tiles;
+      p.tiles += s.tiles * (uint32_t)q.count;
+      ++p.shapes;
+    }
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(std::min(p.tiles, (uint32_t)sm_count()));
+    c.blockDim = dim3(kProductThreads);
+    c.dynamicSmemBytes = Cfg<BN>::kSmemBytes;
+    c.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = at;
+    c.numAttrs = 1;
+    cudaError_t e = cudaFuncSetAttribute(product_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<BN>::kSmemBytes);
+    void* args[1] = {&p};
+    if (e == cudaSuccess) e = cudaLaunchKernelExC(&c, reinterpret_cast<const void*>(product_kernel<BN>), args);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return fail(POLAR_B200_ERR_CUDA, "fmuon: product", e);
+    }
+    count_launch();
+  }
+  return POLAR_B200_OK;
+}
+
+// The matrices of the call, longest sums first, and the groups they are done in.
+void matrices_of(const polar_b200_muon_tensor* tensors, uint64_t count, std::vector<One>* all, std::vector<size_t>* ends) {
+  for (uint64_t i = 0; i < count; ++i) {
+    const polar_b200_muon_tensor& t = tensors[i];
+    for (uint64_t z = 0; z < t.matrices && t.rows && t.cols; ++z) {
+      const uint64_t at = z * t.rows * t.cols;
+      all->push_back(One{t.weights + at, t.gradient + at, t.momentum + at, t.rows, t.cols, t.weight_decay, t.scale});
+    }
+  }
+  std::stable_sort(all->begin(), all->end(), [](const One& a, const One& b) {
+    const uint64_t la = std::max(a.rows, a.cols), lb = std::max(b.rows, b.cols);
+    return la != lb ? la > lb : a.rows != b.rows ? a.rows > b.rows : a.cols > b.cols;
+  });
+  uint64_t bytes = 0;
+  for (size_t i = 0; i < all->size(); ++i) {
+    const uint64_t more = bytes_of((*all)[i].rows, (*all)[i].cols);
+    if (bytes && bytes + more > kGroupBytes) ends->push_back(i), bytes = 0;
+    bytes += more;
+  }
+  if (!all->empty()) ends->push_back(all->size());
+}
+
+int run_group(const std::vector<One>& all, size_t from, size_t to, const polar_b200_muon_options& o, char* base, cudaStream_t st) {
+  std::vector<Kin> kin;
+  double* partial;
+  Target* targets;
+  lay_out(base, all, from, to, &kin, &partial, &targets);
+  int rc;
+  int* status = device_status_word(&rc);
+  if (rc) return rc;
+  for (int begin = 0; begin < 2; ++begin) {
+    rc = to - from <= kFewMatrices ? launch_tables<kFewMatrices>(all, from, to, kin, o, partial, targets, st, begin)
+                                   : launch_tables<kManyMatrices>(all, from, to, kin, o, partial, targets, st, begin);
+    if (rc) return rc;
+  }
+  for (uint32_t i = 0; i < o.steps; ++i) {
+    for (int kind : {(int)kGram, (int)kPolynomial, i + 1 < o.steps ? (int)kRound : (int)kUpdate}) {
+      rc = launch_product<256>(kin, kind, (int)(i & 1), o, targets, status, st);
+      if (rc) return rc;
+    }
+  }
+  return POLAR_B200_OK;
+}
+
+// Whether no singular value passes kBound, nor one of P kBoundP, in any round: X begins with singular values up to 1.
+bool stays_bounded(float a, float b, float c, uint32_t steps) {
+  if (!(std::isfinite(a) && std::isfinite(b) && std::isfinite(c))) return false;
+  double most = 1.001;
+  for (uint32_t i = 0; i < steps && i < 32; ++i) {
+    double next = 0;
+    for (int j = 0; j <= 1024; ++j) {
+      const double s = most * j / 1024, p = a + s * s * (b + c * s * s);
+      if (!(std::fabs(p) <= kBoundP)) return false;
+      next = std::max(next, std::fabs(p) * s);
+    }
+    most = std::max(next * 1.0001, 1e-3);
+    if (!(most <= kBound)) return false;
+  }
+  return true;
+}
+
+bool disjoint(const polar_b200_muon_tensor* tensors, uint64_t count, const float* schedule) {
+  using Span = std::pair<uintptr_t, uintptr_t>;
+  std::vector<Span> written, read;
+  auto span = [](const void* p, uint64_t bytes) { return Span(reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes); };
+  for (uint64_t i = 0; i < count; ++i) {
+    const uint64_t bytes = 4 * tensors[i].matrices * tensors[i].rows * tensors[i].cols;
+    if (!bytes) continue;
+    written.push_back(span(tensors[i].weights, bytes));
+    written.push_back(span(tensors[i].momentum, bytes));
+    read.push_back(span(tensors[i].gradient, bytes));
+  }
+  if (schedule) read.push_back(span(schedule, 8));
+  std::sort(written.begin(), written.end());
+  for (size_t i = 1; i < written.size(); ++i)
+    if (written[i].first < written[i - 1].second) return false;
+  for (const Span& r : read) {
+    const auto next = std::lower_bound(written.begin(), written.end(), Span(r.second, 0));
+    if (next != written.begin() && std::prev(next)->second > r.first) return false;
+  }
+  return true;
+}
+
+bool valid(const polar_b200_muon_tensor& t) {
+  constexpr uint64_t kLong = 1ull << 20, kShort = 1ull << 15;
+  if (!t.matrices || !t.rows || !t.cols) return true;
+  return t.rows <= kLong && t.cols <= kLong && std::min(t.rows, t.cols) <= kShort && t.matrices <= 1ull << 20 && t.matrices * t.rows * t.cols <= 1ull << 36;
+}
+
+}  // namespace
+
+bool muon_independent(const polar_b200_muon_tensor* tensors, uint64_t count, const float* schedule) { return disjoint(tensors, count, schedule); }
+
+}  // namespace polar_b200
+
+using namespace polar_b200;
+
+extern "C" {
+
+uint64_t polar_b200_fmuon_workspace_bytes(const polar_b200_muon_tensor* tensors, uint64_t count) {
+  if (!tensors) return 0;
+  for (uint64_t i = 0; i < count; ++i)
+    if (!valid(tensors[i])) return 0;
+  try {
+    std::vector<One> all;
+    std::vector<size_t> ends;
+    matrices_of(tensors, count, &all, &ends);
+    uint64_t most = 0;
+    size_t from = 0;
+    for (size_t to : ends) {
+      std::vector<Kin> kin;
+      double* partial;
+      Target* targets;
+      most = std::max(most, lay_out(nullptr, all, from, to, &kin, &partial, &targets));
+      from = to;
+    }
+    return most;
+  } catch (const std::exception&) {
+    return 0;
+  }
+}
+
+int polar_b200_fmuon(const polar_b200_muon_tensor* tensors, uint64_t count, const polar_b200_muon_options* o, void* workspace, uint64_t workspace_bytes,
+                     void* stream) {
+  clear_error();
+  if (!o || (count && !tensors)) return fail(POLAR_B200_ERR_INVALID, "fmuon: no tensors or options");
+  if (!(o->momentum >= 0.f && o->momentum < 1.f)) return fail(POLAR_B200_ERR_INVALID, "fmuon: 0 <= momentum < 1 is needed");
+  if (o->steps < 1 || o->steps > 32 || !stays_bounded(o->a, o->b, o->c, o->steps))
+    return fail(POLAR_B200_ERR_INVALID, "fmuon: 1 to 32 rounds of a polynomial that lets no singular value pass 1.4");
+  const void* some = nullptr;
+  for (uint64_t i = 0; i < count; ++i) {
+    const polar_b200_muon_tensor& t = tensors[i];
+    if (!valid(t)) return fail(POLAR_B200_ERR_INVALID, "fmuon: matrix too large");
+    if (!(t.matrices && t.rows && t.cols)) continue;
+    if (!t.weights || !t.gradient || !t.momentum) return fail(POLAR_B200_ERR_INVALID, "null device pointer");
+    some = t.weights;
+  }
+  if (!some) return POLAR_B200_OK;
+  try {
+    if (!muon_independent(tensors, count, o->schedule)) return fail(POLAR_B200_ERR_INVALID, "fmuon: what is written overlaps something else");
+    const uint64_t need = polar_b200_fmuon_workspace_bytes(tensors, count);
+    if (workspace && (workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
+      return fail(POLAR_B200_ERR_WORKSPACE, "workspace too small or not 256-byte aligned");
+    std::vector<One> all;
+    std::vector<size_t> ends;
+    matrices_of(tensors, count, &all, &ends);
+    LaunchDeviceScope on(stream, some);
+    cudaStream_t st = as_stream(stream);
+    void* own = nullptr;
+    if (!workspace) {
+      cudaError_t e = scratch_alloc(&own, need, st);
+      if (e != cudaSuccess) return fail(POLAR_B200_ERR_CUDA, "scratch (workspace)", e);
+    }
+    int rc = POLAR_B200_OK;
+    size_t from = 0;
+    for (size_t to : ends) {
+      rc = run_group(all, from, to, *o, static_cast<char*>(workspace ? workspace : own), st);
+      if (rc) break;
+      from = to;
+    }
+    if (own) {
+      cudaError_t e = scratch_free(own, st);
+      if (rc == POLAR_B200_OK && e != cudaSuccess) rc = fail(POLAR_B200_ERR_CUDA, "returning scratch", e);
+    }
+    return rc;
+  } catch (const std::exception&) {                        // (no exception may leave a C entry)
+    return fail(POLAR_B200_ERR_INVALID, "out of host memory");
+  }
+}
+
+}  // extern "C"

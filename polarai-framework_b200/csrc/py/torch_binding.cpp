@@ -14,6 +14,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -349,6 +350,48 @@ BUILTIN(fadamw) {
   return launched(polar_b200_fadamw, tensors.data(), (uint64_t)count, &o, c.stream());
 }
 
+// fmuon(weights, gradients, momenta, lr, momentum, nesterov, steps, weight decays, scales, a, b, c, schedule or None): lists of tensors, one decay and
+// one scale for each.  Its workspace comes from torch's allocator, which keeps it: it is too large for the library's own pool to.
+BUILTIN(fmuon) {
+  Call c(args, n, 13);
+  if (!c.ok()) return answer(false);
+  const Sequence w(args[0]), g(args[1]), m(args[2]), decays(args[7]), scales(args[8]);
+  const Py_ssize_t count = w.size();
+  if (count < 0 || g.size() != count || m.size() != count || decays.size() != count || scales.size() != count) return answer(false);
+  polar_b200_muon_options o;
+  o.lr = c.scalar(3), o.momentum = c.scalar(4), o.nesterov = c.whole(5) != 0;
+  const uint64_t steps = c.whole(6);
+  o.steps = (uint32_t)std::min<uint64_t>(steps, 1000);
+  o.a = c.scalar(9), o.b = c.scalar(10), o.c = c.scalar(11);
+  std::vector<polar_b200_muon_tensor> tensors((size_t)count);
+  const at::Tensor* some = nullptr;
+  for (Py_ssize_t i = 0; i < count && c.ok(); ++i) {
+    polar_b200_muon_tensor& t = tensors[(size_t)i];
+    const at::Tensor *wt = c.element(w[i], 4), *gt = c.element(g[i], 4), *mt = c.element(m[i], 4);
+    if (!c.ok()) break;
+    c.require(wt->dim() >= 2 && numel(gt) == numel(wt) && numel(mt) == numel(wt));
+    if (!c.ok()) break;
+    t.weights = data(wt), t.gradient = data(gt), t.momentum = data(mt);
+    t.rows = (uint64_t)wt->size(-2), t.cols = (uint64_t)wt->size(-1);
+    t.matrices = t.rows && t.cols ? numel(wt) / (t.rows * t.cols) : 0;
+    const double decay = PyFloat_AsDouble(decays[i]), scale = PyFloat_AsDouble(scales[i]);
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      c.require(false);
+    }
+    t.weight_decay = (float)decay, t.scale = (float)scale;
+    some = wt;
+  }
+  const at::Tensor* schedule = c.tensor_or_none(12);
+  if (c.ok()) c.require(has(schedule, 2));
+  if (!c.ok()) return answer(false);
+  o.schedule = data_or_null(schedule);
+  if (count == 0) return answer(true);
+  const uint64_t need = polar_b200_fmuon_workspace_bytes(tensors.data(), (uint64_t)count);
+  at::Tensor workspace;
+  if (need) workspace = at::empty({(int64_t)need}, at::TensorOptions().dtype(at::kByte).device(some->device()));
+  return launched(polar_b200_fmuon, tensors.data(), (uint64_t)count, &o, need ? workspace.data_ptr() : nullptr, need, c.stream());
+}
 // The ids and offsets of packed sequences, of one type.
 bool packed(Call& c, int i, int* type, const at::Tensor** ids, const at::Tensor** offsets) {
   int other = -1;
@@ -461,6 +504,7 @@ PyMethodDef methods[] = {
     ENTRY("flogprob", declining<flogprob>),
     ENTRY("flogprob_grad", declining<flogprob_grad>),
     ENTRY("fadamw", declining<fadamw>),
+    ENTRY("fmuon", declining<fmuon>),
     ENTRY("fpolicy_loss", declining<fpolicy_loss>),
     ENTRY("fpreference_loss", declining<fpreference_loss>),
     ENTRY("workspace_bytes", raising<workspace_bytes>),

@@ -16,7 +16,7 @@ import numbers
 import numpy as np
 import torch
 
-from .capi import AdamwOptions, AdamwTensor, PolicyBatch, PolicyOptions, PreferenceOptions, binding, lib
+from .capi import AdamwOptions, AdamwTensor, MuonOptions, MuonTensor, PolicyBatch, PolicyOptions, PreferenceOptions, binding, lib
 
 
 def _ptr(t):
@@ -336,6 +336,39 @@ class DeviceBuiltins:
             if weights:
                 options = AdamwOptions(float(lr), float(beta1), float(beta2), float(eps), int(step), _ptr(schedule))
                 self.lib.call("polar_b200_fadamw", tensors, len(weights), ctypes.byref(options), _stream(weights[0]))
+        return weights
+
+    def fmuon(self, weights, gradients, momenta, *, lr=0.0, momentum=0.95, nesterov=True, steps=5, weight_decay=0.0, scale=None,
+              coefficients=(3.4445, -4.7750, 2.0315), schedule=None):
+        """One step of orthogonalised momentum over lists of matrices - tensors [rows, cols], or [..., rows, cols] of several, each by
+        itself - in place.  weight_decay and scale, by which the update is multiplied: one for all, or a list; no scale: sqrt(rows / cols) where
+        that is above 1.  lr comes from the call or, for steps that are captured, from `schedule`, fadamw's device tensor of the step's number and lr."""
+        decays = [weight_decay] * len(weights) if isinstance(weight_decay, numbers.Real) else weight_decay
+        scales = ([scale] * len(weights) if isinstance(scale, numbers.Real) else scale if scale is not None else
+                  [max(1.0, w.shape[-2] / max(w.shape[-1], 1)) ** 0.5 if len(w.shape) >= 2 else 1.0 for w in weights])
+        if not self._native.fmuon(weights, gradients, momenta, lr, momentum, bool(nesterov), steps, decays, scales, *coefficients, schedule):
+            if any(len(x) != len(weights) for x in (gradients, momenta, decays, scales)):
+                raise ValueError("fmuon: lists of one length")
+            tensors = (MuonTensor * len(weights))()
+            for t, w, g, m, decay, s in zip(tensors, weights, gradients, momenta, decays, scales):
+                _chk(w, g, m)
+                _same_device(weights[0], w, g, m)
+                _exactly("fmuon", w.numel(), g, m)
+                if len(w.shape) < 2:
+                    raise ValueError("fmuon: weights are matrices (vectors are for fadamw)")
+                t.weights, t.gradient, t.momentum = (x.data_ptr() for x in (w, g, m))
+                t.rows, t.cols = w.shape[-2:]
+                t.matrices = w.numel() // (t.rows * t.cols) if t.rows and t.cols else 0
+                t.weight_decay, t.scale = float(decay), float(s)
+            if schedule is not None:
+                _chk(schedule)
+                _exactly("fmuon", 2, schedule)
+                _same_device(schedule, *weights[:1])
+            if weights:
+                options = MuonOptions(float(lr), float(momentum), int(bool(nesterov)), max(int(steps), 0), *(float(c) for c in coefficients), _ptr(schedule))
+                need = self.lib.cdll.polar_b200_fmuon_workspace_bytes(tensors, len(weights))
+                workspace = torch.empty(need, dtype=torch.uint8, device=weights[0].device) if need else None
+                self.lib.call("polar_b200_fmuon", tensors, len(weights), ctypes.byref(options), _ptr(workspace), need, _stream(weights[0]))
         return weights
 
     def fpolicy_loss(self, logprob, old_logprob, advantage, ids, offsets, loss, g_logprob=None, g_entropy=None, *, reference=None, entropy=None,
