@@ -80,9 +80,13 @@ class OracleExecutor:
                 continue
             if kernel in ("fpolicy_loss", "fpreference_loss"):
                 a = [t[x].ravel() if isinstance(x, str) else x for x in args]
-                r = (rows_oracle.fpolicy_loss(*a[:12], a[13], a[14]) if kernel == "fpolicy_loss" else rows_oracle.fpreference_loss(*a[:8], a[10]))
+                r = (rows_oracle.fpolicy_loss(*a[:13], a[14], a[15]) if kernel == "fpolicy_loss" else rows_oracle.fpreference_loss(*a[:9], a[11]))
                 for name, value in zip(args[-3:], r):
                     t[name] = np.asarray(value, np.float32).reshape(self.program.tensors[name])
+                continue
+            if kernel == "fmuon":
+                lr = float(t[args[1]].ravel()[1])
+                t[args[7]], t[args[8]] = rows_oracle.fmuon(t[args[7]], t[args[0]], t[args[8]], lr, args[2], bool(args[3]), *args[4:7])
                 continue
             if kernel in ("flayernorm", "flayernorm_grad", "flogprob", "flogprob_top", "flogprob_grad", "fadamw"):
                 # several results, the last arguments

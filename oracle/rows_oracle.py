@@ -183,16 +183,41 @@ def preference_loss64(logprob, reference, ids, offsets, beta, smoothing, margin,
     return out, rewards, np.concatenate([np.full(span.start, np.nan), g, np.full(n - span.stop, np.nan)]), z
 
 
-def fpolicy_loss(logprob, old, reference, entropy, advantage, ids, offsets, clip_low, clip_high, kl_weight, entropy_weight, by_sequence, g_logprob,
-                 g_entropy):
+def fpolicy_loss(logprob, old, reference, entropy, advantage, ids, offsets, clip_low, clip_high, kl_weight, entropy_weight, count, by_sequence,
+                 g_logprob, g_entropy):
     """(loss[5], g_logprob, g_entropy) as the builtin of a program gives them."""
     tokens = len(ids)
     loss, g, ge, _ = policy_loss64(logprob, old, reference, entropy, advantage, ids, offsets, clip_low, clip_high, kl_weight, entropy_weight, bool(by_sequence),
-                                   np.size(advantage) == tokens)
+                                   np.size(advantage) == tokens, count)
     return _f32(loss), _f32(_over(g_logprob, g)), _f32(_over(g_entropy, ge))
 
 
-def fpreference_loss(logprob, reference, ids, offsets, beta, smoothing, margin, average, g_logprob):
+def fpreference_loss(logprob, reference, ids, offsets, beta, smoothing, margin, count, average, g_logprob):
     """(loss[3], rewards, g_logprob)."""
-    loss, rewards, g, _ = preference_loss64(logprob, reference, ids, offsets, beta, smoothing, margin, bool(average))
+    loss, rewards, g, _ = preference_loss64(logprob, reference, ids, offsets, beta, smoothing, margin, bool(average), count)
     return _f32(loss), _f32(rewards), _f32(_over(g_logprob, g))
+
+
+def muon64(w, g, m, lr, momentum, nesterov, steps, decay, scale, a=3.4445, b=-4.7750, c=2.0315):
+    """(weights, momentum, update) of one matrix in 64 bits; update: the orthogonalised matrix."""
+    f = lambda v: float(np.float32(v))  # noqa: E731
+    mu, lr = f(momentum), f(lr)
+    g, m = np.asarray(g, np.float64), np.asarray(m, np.float64)
+    m = mu * m + g
+    u = g + mu * m if nesterov else m
+    size = np.sqrt((u * u).sum())
+    x = u / size if size != 0 else u
+    x = x if x.shape[0] <= x.shape[1] else x.T
+    for _ in range(int(steps)):
+        gram = x @ x.T
+        x = f(a) * x + (f(b) * gram + f(c) * gram @ gram) @ x
+    x = x if x.shape == g.shape else x.T
+    return np.asarray(w, np.float64) * (1 - lr * f(decay)) - lr * f(scale) * x, m, x
+
+
+def fmuon(w, g, m, lr, momentum, nesterov, steps, decay, scale):
+    """(weights, momentum) of matrices [..., rows, cols]."""
+    shape = np.shape(w)
+    flat = [np.reshape(t, (-1, *shape[-2:])) for t in (w, g, m)]
+    r = [muon64(*t, lr, momentum, nesterov, steps, decay, scale)[:2] for t in zip(*flat)]
+    return _f32(np.stack([x[0] for x in r]).reshape(shape)), _f32(np.stack([x[1] for x in r]).reshape(shape))

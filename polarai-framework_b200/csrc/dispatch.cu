@@ -35,6 +35,7 @@ uint64_t ragged_rows_workspace_bytes(uint64_t rem, uint64_t n, uint64_t k);
 int launch_ragged_rows(const float* left_tail, uint64_t left_pitch, const float* right, float* out_tail,
                        float* ws, uint64_t rem, uint64_t n, uint64_t k, cudaStream_t st);
 bool adamw_arguments(const char* name, const polar_b200_arg* a, uint64_t argc, polar_b200_adamw_tensor* t, polar_b200_adamw_options* o);
+bool muon_arguments(const char* name, const polar_b200_arg* a, uint64_t argc, polar_b200_muon_tensor* t, polar_b200_muon_options* o);
 
 namespace {
 
@@ -363,7 +364,7 @@ uint64_t polar_b200_fmatmul_workspace_bytes(int tl, int tr, uint64_t m, uint64_t
 int polar_b200_result_count(const char* name) {
   static const struct { const char* name; int results; } several[] = {
       {"fdense_grad", 2}, {"flayernorm", 3}, {"flayernorm_grad", 3}, {"flogprob", 3}, {"flogprob_top", 5}, {"fadamw", 3}, {"fadamw8", 5},
-      {"fpolicy_loss", 3}, {"fpreference_loss", 3}};
+      {"fpolicy_loss", 3}, {"fpreference_loss", 3}, {"fmuon", 2}};
   for (const auto& s : several)
     if (name && !std::strcmp(name, s.name)) return s.results;
   return 1;
@@ -389,12 +390,17 @@ uint64_t polar_b200_launch_workspace_bytes(const char* name, const polar_b200_ar
     rows_of(a[0].tensor, &rows, &cols);
     return polar_b200_flayernorm_grad_workspace_bytes(rows, cols);
   }
-  if (name && a && !std::strcmp(name, "fpolicy_loss") && argc == 15 && a[5].is_tensor && a[6].is_tensor && a[5].tensor.dims == 1 &&
+  if (name && a && !std::strcmp(name, "fpolicy_loss") && argc == 16 && a[5].is_tensor && a[6].is_tensor && a[5].tensor.dims == 1 &&
       a[6].tensor.dims == 1 && a[5].tensor.shape && a[6].tensor.shape && a[6].tensor.shape[0])
     return polar_b200_fpolicy_loss_workspace_bytes(a[5].tensor.shape[0], a[6].tensor.shape[0] - 1);
-  if (name && a && !std::strcmp(name, "fpreference_loss") && argc == 11 && a[2].is_tensor && a[3].is_tensor && a[2].tensor.dims == 1 &&
+  if (name && a && !std::strcmp(name, "fpreference_loss") && argc == 12 && a[2].is_tensor && a[3].is_tensor && a[2].tensor.dims == 1 &&
       a[3].tensor.dims == 1 && a[2].tensor.shape && a[3].tensor.shape && a[3].tensor.shape[0])
     return polar_b200_fpreference_loss_workspace_bytes(a[2].tensor.shape[0], (a[3].tensor.shape[0] - 1) / 2);
+  if (name && a && !std::strcmp(name, "fmuon")) {
+    polar_b200_muon_tensor t;
+    polar_b200_muon_options o;
+    return muon_arguments(name, a, argc, &t, &o) ? polar_b200_fmuon_workspace_bytes(&t, 1) : 0;
+  }
   if (name && a && !std::strcmp(name, "fsum") && argc == 2 && a[0].is_tensor && (!a[0].tensor.dims || a[0].tensor.shape)) {
     uint64_t n = 1;
     for (uint64_t d = 0; d < a[0].tensor.dims; ++d) n *= a[0].tensor.shape[d];
@@ -919,31 +925,38 @@ int polar_b200_launch_by_name(const char* name, const polar_b200_arg* a, uint64_
   auto flag = [&](uint64_t i) { return a[i].scalar == 0.f || a[i].scalar == 1.f; };
   if (!std::strcmp(name, "fpolicy_loss")) {
     // (T logProb, T oldLogProb, T refLogProb, T entropy, T advantage, T ids, T offsets, f32 clip_low, f32 clip_high, f32 kl_weight,
-    //  f32 entropy_weight, f32 by_sequence, T loss[5], T gLogProb, T gEntropy): three results
-    if (!pattern("TTTTTTTfffffTTT") || a[5].tensor.dims != 1 || a[6].tensor.dims != 1 || a[6].tensor.shape[0] < 1 || !flag(11))
+    //  f32 entropy_weight, f32 count, f32 by_sequence, T loss[5], T gLogProb, T gEntropy): three results
+    if (!pattern("TTTTTTTffffffTTT") || a[5].tensor.dims != 1 || a[6].tensor.dims != 1 || a[6].tensor.shape[0] < 1 || !flag(12))
       return fail(bad_args, "fpolicy_loss expects (T logProb, T oldLogProb, T refLogProb, T entropy, T advantage, T ids[tokens], T offsets[sequences + 1], f32 clip_low, "
-                            "f32 clip_high, f32 kl_weight, f32 entropy_weight, f32 by_sequence, T loss[5], T gLogProb, T gEntropy)");
+                            "f32 clip_high, f32 kl_weight, f32 entropy_weight, f32 count, f32 by_sequence, T loss[5], T gLogProb, T gEntropy)");
     const uint64_t tokens = a[5].tensor.shape[0], sequences = a[6].tensor.shape[0] - 1, advantages = numel(a[4].tensor);
-    for (int i : {0, 1, 2, 3, 13, 14})
+    for (int i : {0, 1, 2, 3, 14, 15})
       if (numel(a[i].tensor) != tokens) return fail(bad_args, "fpolicy_loss: shapes do not agree");
-    if ((advantages != tokens && advantages != sequences) || numel(a[12].tensor) != 5) return fail(bad_args, "fpolicy_loss: shapes do not agree");
+    if ((advantages != tokens && advantages != sequences) || numel(a[13].tensor) != 5) return fail(bad_args, "fpolicy_loss: shapes do not agree");
     const polar_b200_policy_batch b = {a[0].tensor.data, a[1].tensor.data, a[2].tensor.data, a[3].tensor.data, a[4].tensor.data, a[5].tensor.data,
                                        a[6].tensor.data, POLAR_B200_IDS_F32, advantages == tokens, tokens, sequences};
-    const polar_b200_policy_options o = {a[7].scalar, a[8].scalar, a[9].scalar, a[10].scalar, 0.f, a[11].scalar != 0.f};
-    return polar_b200_fpolicy_loss(&b, &o, a[12].tensor.data, a[13].tensor.data, a[14].tensor.data, workspace, workspace_bytes, stream);
+    const polar_b200_policy_options o = {a[7].scalar, a[8].scalar, a[9].scalar, a[10].scalar, a[11].scalar, a[12].scalar != 0.f};
+    return polar_b200_fpolicy_loss(&b, &o, a[13].tensor.data, a[14].tensor.data, a[15].tensor.data, workspace, workspace_bytes, stream);
   }
   if (!std::strcmp(name, "fpreference_loss")) {
-    // (T logProb, T refLogProb, T ids, T offsets, f32 beta, f32 smoothing, f32 margin, f32 average, T loss[3], T rewards, T gLogProb): three results
-    if (!pattern("TTTTffffTTT") || a[2].tensor.dims != 1 || a[3].tensor.dims != 1 || a[3].tensor.shape[0] % 2 != 1 || !flag(7))
+    // (T logProb, T refLogProb, T ids, T offsets, f32 beta, f32 smoothing, f32 margin, f32 count, f32 average, T loss[3], T rewards, T gLogProb): three results
+    if (!pattern("TTTTfffffTTT") || a[2].tensor.dims != 1 || a[3].tensor.dims != 1 || a[3].tensor.shape[0] % 2 != 1 || !flag(8))
       return fail(bad_args, "fpreference_loss expects (T logProb, T refLogProb, T ids[tokens], T offsets[2 * pairs + 1], f32 beta, f32 smoothing, f32 margin, "
-                            "f32 average, T loss[3], T rewards[2 * pairs], T gLogProb)");
+                            "f32 count, f32 average, T loss[3], T rewards[2 * pairs], T gLogProb)");
     const uint64_t tokens = a[2].tensor.shape[0], sequences = a[3].tensor.shape[0] - 1;
-    if (numel(a[0].tensor) != tokens || numel(a[1].tensor) != tokens || numel(a[10].tensor) != tokens || numel(a[8].tensor) != 3 ||
-        numel(a[9].tensor) != sequences)
+    if (numel(a[0].tensor) != tokens || numel(a[1].tensor) != tokens || numel(a[11].tensor) != tokens || numel(a[9].tensor) != 3 ||
+        numel(a[10].tensor) != sequences)
       return fail(bad_args, "fpreference_loss: shapes do not agree");
-    const polar_b200_preference_options o = {a[4].scalar, a[5].scalar, a[6].scalar, 0.f, a[7].scalar != 0.f};
+    const polar_b200_preference_options o = {a[4].scalar, a[5].scalar, a[6].scalar, a[7].scalar, a[8].scalar != 0.f};
     return polar_b200_fpreference_loss(a[0].tensor.data, a[1].tensor.data, a[2].tensor.data, a[3].tensor.data, POLAR_B200_IDS_F32, tokens, sequences / 2, &o,
-                                       a[8].tensor.data, a[9].tensor.data, a[10].tensor.data, workspace, workspace_bytes, stream);
+                                       a[9].tensor.data, a[10].tensor.data, a[11].tensor.data, workspace, workspace_bytes, stream);
+  }
+  if (!std::strcmp(name, "fmuon")) {
+    polar_b200_muon_tensor t;
+    polar_b200_muon_options o;
+    if (!muon_arguments(name, a, argc, &t, &o))
+      return fail(bad_args, "fmuon expects (T gradient, T schedule[2], f32 momentum, f32 nesterov, f32 steps, f32 weight_decay, f32 scale, T weights[..., rows, cols], T momentum)");
+    return polar_b200_fmuon(&t, 1, &o, workspace, workspace_bytes, stream);
   }
   if (!std::strcmp(name, "fsum")) {
     if (!pattern("TT") || numel(a[1].tensor) < 1) return fail(bad_args, "fsum expects (T in, T out[1])");

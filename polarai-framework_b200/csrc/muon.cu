@@ -16,6 +16,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <exception>
 #include <mutex>
 #include <utility>
@@ -167,7 +168,11 @@ __global__ void __launch_bounds__(kThreads) begin_kernel(const __grid_constant__
 // ---- the products
 
 constexpr int BM = 128, BK = 32;
-constexpr int kEpilogueWarps = 8, kProductThreads = 32 * (2 + kEpilogueWarps);
+constexpr int kRun = 4;                                    // slabs that are summed in tensor memory
+constexpr int kEpilogueWarps = 8, kProductThreads = 32 * (4 + kEpilogueWarps);
+// Registers of a thread: 168 at launch (three warpgroups of 128 threads, 64512 in all), then what the sums need for the epilogue's two and
+// what is left for the other: 2 * 128 * 232 + 128 * 40 = 64512.
+constexpr int kFewRegisters = 40, kManyRegisters = 232;
 template <int BN>
 struct Cfg {
   static constexpr uint32_t kAPlane = BM * BK * 2, kBPlane = BN * BK * 2;
@@ -257,11 +262,15 @@ __device__ __forceinline__ uint32_t f16_idesc(int n, int a_mn, int b_mn) {
 }
 __device__ __forceinline__ void st_v8(void* dst, const uint32_t* r) { st_global_v8(static_cast<float*>(dst), r); }
 
-// One CTA per SM walks 128 x BN tiles; two accumulators in tensor memory, so that a tile's epilogue runs beside the next one's products.
+// One CTA per SM walks 128 x BN tiles.
 //   warp 0     TMA: both planes of a slab of 32 k of each operand, one instruction each.  An operand that is contiguous along k is K-major
 //              (rows of 64 bytes in the 64-byte swizzle), else MN-major (chunks of 64 columns, 128-byte swizzle, a row per k).
-//   warp 1     tcgen05.mma: per 16 k  hi hi, lo hi, hi lo.
-//   warps 2-9  epilogue: two warps to each 32 rows of the accumulator, half of the columns each.
+//   warp 1     tcgen05.mma: per 16 k  hi hi, lo hi, hi lo, into two accumulators in tensor memory by turns, each for kRun slabs.
+//   warps 4-11 add the finished accumulators to the tile's sums in registers, two warps to each 32 rows and half of the columns each, and
+//              write the tile, while the next one's products run.
+// The tensor core cuts every sum off at fp32's last bit, towards zero: over the 3 k / 16 additions of a long k that makes the sums too small by
+// more than all else does to them (784 x 4096: the update 6.4e-5 from the exact one).  The registers' sums are rounded to nearest, and with runs
+// of 128 k there are 24 additions to a cut sum (784 x 4096: 7.7e-6); reading the accumulators costs the tensor core nothing.
 // Every wait is bounded; when one gives up, all roles leave, and the status word holds its code (7xx).
 template <int BN>
 __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __grid_constant__ Product p) {
@@ -295,6 +304,132 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   pdl_enter();
 
+  if (warp >= 4) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const float lr = p.kind == kUpdate ? (p.schedule ? p.schedule[1] : p.lr) : 0.f;
+    uint32_t run = 0;
+    bool ok = true;
+    for (uint32_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x) {
+      const Place at = place_of<BN>(p, t);
+      const Shape& q = p.s[at.shape];
+      uint32_t sum[BN / 64][32];                           // this thread's row of its half of the tile, as bits of floats
+      const int runs = (int)((q.k + kRun * BK - 1) / (kRun * BK));
+      for (int i = 0; i < runs; ++i, ++run) {
+        const uint32_t as = run & 1u;
+        ok = mbar_wait(acc_full(as), (run >> 1) & 1u, abort_flag, p.status, 704, p.wait_ns);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t acc = tmem_base + as * BN + half * (BN / 2) + ((uint32_t)(quarter * 32) << 16);
+        if (i == 0) {
+#pragma unroll
+          for (int j = 0; j < BN / 64; ++j) tmem_ld_32x32(acc + 32 * j, sum[j]);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int j = 0; j < BN / 32; ++j) {
+            uint32_t v[16];
+            tmem_ld_32x16(acc + 16 * j, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              uint32_t& x = sum[j / 2][j % 2 * 16 + e];
+              x = __float_as_uint(__uint_as_float(x) + __uint_as_float(v[e]));
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty(as));
+      }
+      if (!ok) break;
+      const uint32_t r0 = (uint32_t)at.m0 + quarter * 32, row = r0 + lane;
+      __half* const hi_plane = q.out + 2 * at.z * q.plane;
+      Target target = {};
+      if (p.kind == kUpdate) target = p.targets[q.first_target + at.z];
+      const float keep = 1.f - lr * target.decay, rate = p.by * lr * target.scale;
+      const bool vectors = (q.n & 3) == 0 && (reinterpret_cast<uintptr_t>(target.weights) & 15) == 0;
+#pragma unroll
+      for (int block = 0; block < BN / 64; ++block) {
+        const uint32_t c0 = (uint32_t)at.n0 + half * (BN / 2) + 32 * block;
+        uint32_t(&r)[32] = sum[block];
+        if (c0 >= q.n || r0 >= q.m) break;
+        if (p.kind <= kPolynomial && c0 < r0) continue;      // below the diagonal: written by the block above it
+        if (p.kind == kUpdate) {
+          float* w = target.weights + (uint64_t)row * q.n + c0;
+          if (row >= q.m) {
+          } else if (vectors && c0 + 32 <= q.n) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              float4 v = *reinterpret_cast<const float4*>(w + j);
+              v.x = v.x * keep - rate * __uint_as_float(r[j]), v.y = v.y * keep - rate * __uint_as_float(r[j + 1]);
+              v.z = v.z * keep - rate * __uint_as_float(r[j + 2]), v.w = v.w * keep - rate * __uint_as_float(r[j + 3]);
+              *reinterpret_cast<float4*>(w + j) = v;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c0 + j < q.n) w[j] = w[j] * keep - rate * __uint_as_float(r[j]);
+          }
+          continue;
+        }
+        __half* const out = hi_plane + (uint64_t)row * q.pitch + c0;
+        unsigned short* const mirror = reinterpret_cast<unsigned short*>(hi_plane) + (uint64_t)c0 * q.pitch + row;
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          uint32_t* const v = r + 16 * part;
+          uint32_t hi[8], lo[8];                           // two columns in each
+          if (p.kind == kPolynomial) {
+            const __half* add = q.add + 2 * at.z * q.plane + (uint64_t)row * q.pitch + c0 + 16 * part;
+            if (row < q.m) {
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const uint4 h = *reinterpret_cast<const uint4*>(add + 8 * j), l = *reinterpret_cast<const uint4*>(add + q.plane + 8 * j);
+                hi[4 * j] = h.x, hi[4 * j + 1] = h.y, hi[4 * j + 2] = h.z, hi[4 * j + 3] = h.w;
+                lo[4 * j] = l.x, lo[4 * j + 1] = l.y, lo[4 * j + 2] = l.z, lo[4 * j + 3] = l.w;
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float2 h = __half22float2(*reinterpret_cast<__half2*>(&hi[j])), l = __half22float2(*reinterpret_cast<__half2*>(&lo[j]));
+              float a = fmaf(p.by, __uint_as_float(v[2 * j]), p.add_by * (h.x + l.x));
+              float b = fmaf(p.by, __uint_as_float(v[2 * j + 1]), p.add_by * (h.y + l.y));
+              const uint32_t col = c0 + 16 * part + 2 * j;
+              if (col == row) a += p.diagonal;
+              if (col + 1 == row) b += p.diagonal;
+              v[2 * j] = __float_as_uint(a), v[2 * j + 1] = __float_as_uint(b);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(p.by * __uint_as_float(v[j]));
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float a = __uint_as_float(v[2 * j]), b = __uint_as_float(v[2 * j + 1]);
+            const __half2 h = __floats2half2_rn(a, b);
+            const float2 f = __half22float2(h);
+            const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+            hi[j] = *reinterpret_cast<const uint32_t*>(&h), lo[j] = *reinterpret_cast<const uint32_t*>(&l);
+          }
+          if (row < q.m) {                                 // (columns behind the last one lie in the row's padding)
+            st_v8(out + 16 * part, hi);
+            st_v8(out + 16 * part + q.plane, lo);
+          }
+          if (p.kind <= kPolynomial && c0 > r0) {          // its mirror image: a column of the block is a row there, 32 lanes side by side
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              if (c0 + 16 * part + j < q.n) {
+                unsigned short* const o = mirror + (uint64_t)(16 * part + j) * q.pitch;
+                o[0] = (unsigned short)(hi[j / 2] >> (j & 1) * 16);
+                o[q.plane] = (unsigned short)(lo[j / 2] >> (j & 1) * 16);
+              }
+            }
+          }
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
   if (warp == 0) {
     const bool leader = elect_one();
     int s = 0;
@@ -320,136 +455,48 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
   } else if (warp == 1) {
     const bool leader = elect_one();
     int s = 0;
-    uint32_t ph = 0, tile = 0;
+    uint32_t ph = 0, run = 0;
     bool ok = true;
-    for (uint32_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x, ++tile) {
-      const Shape& q = p.s[place_of<BN>(p, t).shape];
+    for (uint32_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x) {
+      const Place at = place_of<BN>(p, t);
+      const Shape& q = p.s[at.shape];
       const int slabs = (int)((q.k + BK - 1) / BK);
-      const uint32_t idesc = f16_idesc(BN, q.a_mn, q.b_mn);
+      // where the left half of a symmetric product's tile lies below the diagonal, the right half alone: 128 rows or two chunks further
+      const uint32_t left_out = BN == 256 && p.kind <= kPolynomial && at.m0 == at.n0 + 128 ? 128 : 0;
+      const uint32_t idesc = f16_idesc(BN - left_out, q.a_mn, q.b_mn);
       // K-major: 64-byte swizzle (layout 4), groups of 8 rows 512 bytes apart, 16 k 32 bytes on.  MN-major: 128-byte swizzle (layout 2), chunks
       // of 64 columns BK rows apart, groups of 8 k 1024 bytes, 16 k 2048 bytes on.
       const Operand a_op = q.a_mn ? make_desc(0, BK * 128, 1024, 2) : make_desc(0, 16, 512, 4);
       const Operand b_op = q.b_mn ? make_desc(0, BK * 128, 1024, 2) : make_desc(0, 16, 512, 4);
       const uint32_t a_step = (q.a_mn ? 2048u : 32u) >> 4, b_step = (q.b_mn ? 2048u : 32u) >> 4;
-      const uint32_t as = tile & 1u, acc = tmem_base + as * BN;
-      ok = mbar_wait(acc_empty(as), ((tile >> 1) & 1u) ^ 1u, abort_flag, p.status, 702, p.wait_ns);
-      if (!ok) break;
-      tc_fence_after();
-      for (int kb = 0; kb < slabs; ++kb) {
-        ok = mbar_wait(full(s), ph, abort_flag, p.status, 703, p.wait_ns);
+      for (int kb = 0; kb < slabs; ++run) {
+        const uint32_t as = run & 1u, acc = tmem_base + as * BN + left_out;
+        ok = mbar_wait(acc_empty(as), ((run >> 1) & 1u) ^ 1u, abort_flag, p.status, 702, p.wait_ns);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t a_hi = ((smem_base & 0x3FFFFu) + s * C::kStageBytes) >> 4, a_lo = a_hi + (C::kAPlane >> 4);
-        const uint32_t b_hi = a_lo + (C::kAPlane >> 4), b_lo = b_hi + (C::kBPlane >> 4);
-        if (leader) {
+        const int end = min(kb + kRun, slabs);
+        for (uint32_t more = 0; kb < end; ++kb, more = 1) {
+          ok = mbar_wait(full(s), ph, abort_flag, p.status, 703, p.wait_ns);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a_hi = ((smem_base & 0x3FFFFu) + s * C::kStageBytes) >> 4, a_lo = a_hi + (C::kAPlane >> 4);
+          const uint32_t b_hi = a_lo + (C::kAPlane >> 4) + left_out * (BK * 2) / 16, b_lo = b_hi + (C::kBPlane >> 4);
+          if (leader) {
 #pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk) {
-            tc_mma_f16(acc, a_op, a_hi + kk * a_step, b_op, b_hi + kk * b_step, idesc, kb || kk ? 1u : 0u);
-            tc_mma_f16(acc, a_op, a_lo + kk * a_step, b_op, b_hi + kk * b_step, idesc, 1u);
-            tc_mma_f16(acc, a_op, a_hi + kk * a_step, b_op, b_lo + kk * b_step, idesc, 1u);
+            for (int kk = 0; kk < BK / 16; ++kk) {
+              tc_mma_f16(acc, a_op, a_hi + kk * a_step, b_op, b_hi + kk * b_step, idesc, kk ? 1u : more);
+              tc_mma_f16(acc, a_op, a_lo + kk * a_step, b_op, b_hi + kk * b_step, idesc, 1u);
+              tc_mma_f16(acc, a_op, a_hi + kk * a_step, b_op, b_lo + kk * b_step, idesc, 1u);
+            }
+            tc_commit(empty(s));
           }
-          tc_commit(empty(s));
+          if (++s == S) s = 0, ph ^= 1;
         }
-        if (++s == S) s = 0, ph ^= 1;
+        if (!ok) break;
+        if (leader) tc_commit(acc_full(as));
       }
-      if (ok && leader) tc_commit(acc_full(as));
     }
-  } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
-    const float lr = p.kind == kUpdate ? (p.schedule ? p.schedule[1] : p.lr) : 0.f;
-    uint32_t tile = 0;
-    for (uint32_t t = blockIdx.x; t < p.tiles; t += gridDim.x, ++tile) {
-      const Place at = place_of<BN>(p, t);
-      const Shape& q = p.s[at.shape];
-      const uint32_t as = tile & 1u;
-      if (!mbar_wait(acc_full(as), (tile >> 1) & 1u, abort_flag, p.status, 704, p.wait_ns)) break;
-      tc_fence_after();
-      const uint32_t r0 = (uint32_t)at.m0 + quarter * 32, row = r0 + lane;
-      __half* const hi_plane = q.out + 2 * at.z * q.plane;
-      Target target = {};
-      if (p.kind == kUpdate) target = p.targets[q.first_target + at.z];
-      const float keep = 1.f - lr * target.decay, rate = p.by * lr * target.scale;
-      const bool vectors = (q.n & 3) == 0 && (reinterpret_cast<uintptr_t>(target.weights) & 15) == 0;
-#pragma unroll 1
-      for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
-        const uint32_t c0 = (uint32_t)at.n0 + c;
-        if (c0 >= q.n || r0 >= q.m) break;
-        if (p.kind <= kPolynomial && c0 < r0) continue;      // below the diagonal: written by the block above it
-        uint32_t r[32];
-        __syncwarp();
-        tmem_ld_32x32(tmem_base + as * BN + c + ((uint32_t)(quarter * 32) << 16), r);
-        tmem_ld_wait();
-        if (p.kind == kUpdate) {
-          float* w = target.weights + (uint64_t)row * q.n + c0;
-          if (row >= q.m) {
-          } else if (vectors && c0 + 32 <= q.n) {
-#pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              float4 v = *reinterpret_cast<const float4*>(w + j);
-              v.x = v.x * keep - rate * __uint_as_float(r[j]), v.y = v.y * keep - rate * __uint_as_float(r[j + 1]);
-              v.z = v.z * keep - rate * __uint_as_float(r[j + 2]), v.w = v.w * keep - rate * __uint_as_float(r[j + 3]);
-              *reinterpret_cast<float4*>(w + j) = v;
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (c0 + j < q.n) w[j] = w[j] * keep - rate * __uint_as_float(r[j]);
-          }
-          continue;
-        }
-        const uint64_t place = (uint64_t)row * q.pitch + c0;
-        uint32_t hi[16], lo[16];                           // two columns in each
-        if (p.kind == kPolynomial) {
-          const __half* add = q.add + 2 * at.z * q.plane + place;
-          if (row < q.m) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint4 h = *reinterpret_cast<const uint4*>(add + 8 * j), l = *reinterpret_cast<const uint4*>(add + q.plane + 8 * j);
-              hi[4 * j] = h.x, hi[4 * j + 1] = h.y, hi[4 * j + 2] = h.z, hi[4 * j + 3] = h.w;
-              lo[4 * j] = l.x, lo[4 * j + 1] = l.y, lo[4 * j + 2] = l.z, lo[4 * j + 3] = l.w;
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float2 h = __half22float2(*reinterpret_cast<__half2*>(&hi[j])), l = __half22float2(*reinterpret_cast<__half2*>(&lo[j]));
-            float a = fmaf(p.by, __uint_as_float(r[2 * j]), p.add_by * (h.x + l.x));
-            float b = fmaf(p.by, __uint_as_float(r[2 * j + 1]), p.add_by * (h.y + l.y));
-            if (c0 + 2 * j == row) a += p.diagonal;
-            if (c0 + 2 * j + 1 == row) b += p.diagonal;
-            r[2 * j] = __float_as_uint(a), r[2 * j + 1] = __float_as_uint(b);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(p.by * __uint_as_float(r[j]));
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float a = __uint_as_float(r[2 * j]), b = __uint_as_float(r[2 * j + 1]);
-          const __half2 h = __floats2half2_rn(a, b);
-          const float2 f = __half22float2(h);
-          const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
-          hi[j] = *reinterpret_cast<const uint32_t*>(&h), lo[j] = *reinterpret_cast<const uint32_t*>(&l);
-        }
-        if (row < q.m) {                                   // (columns behind the last one lie in the row's padding)
-          __half* o = hi_plane + place;
-          st_v8(o, hi), st_v8(o + 16, hi + 8);
-          st_v8(o + q.plane, lo), st_v8(o + q.plane + 16, lo + 8);
-        }
-        if (p.kind <= kPolynomial && c0 > r0) {            // its mirror image: a column of the block is a row there, 32 lanes side by side
-          unsigned short* o = reinterpret_cast<unsigned short*>(hi_plane) + (uint64_t)c0 * q.pitch + row;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            if (c0 + j < q.n) {
-              o[(uint64_t)j * q.pitch] = (unsigned short)(hi[j / 2] >> (j & 1) * 16);
-              o[(uint64_t)j * q.pitch + q.plane] = (unsigned short)(lo[j / 2] >> (j & 1) * 16);
-            }
-          }
-        }
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty(as));
-    }
+  }
   }
 
   tc_fence_before();
@@ -749,7 +796,31 @@ bool valid(const polar_b200_muon_tensor& t) {
 
 }  // namespace
 
+// Whether the steps may run in any order or at once: no written array overlaps another, a gradient or the schedule.
 bool muon_independent(const polar_b200_muon_tensor* tensors, uint64_t count, const float* schedule) { return disjoint(tensors, count, schedule); }
+
+// The argument list of the builtin "fmuon" as the entry point takes it; false where it is none.
+bool muon_arguments(const char* name, const polar_b200_arg* a, uint64_t argc, polar_b200_muon_tensor* t, polar_b200_muon_options* o) {
+  static const char pattern[] = "TTfffffTT";
+  if (std::strcmp(name, "fmuon") || argc != sizeof(pattern) - 1) return false;
+  uint64_t n[9] = {};
+  for (uint64_t i = 0; i < argc; ++i) {
+    if ((pattern[i] == 'T') != (a[i].is_tensor != 0)) return false;
+    if (!a[i].is_tensor) continue;
+    if (a[i].tensor.dims && !a[i].tensor.shape) return false;
+    n[i] = 1;
+    for (uint64_t d = 0; d < a[i].tensor.dims; ++d) n[i] *= a[i].tensor.shape[d];
+  }
+  const polar_b200_tensor& w = a[7].tensor;
+  const float steps = a[4].scalar;
+  if (w.dims < 2 || n[0] != n[7] || n[8] != n[7] || n[1] != 2 || !a[1].tensor.data || (a[3].scalar != 0.f && a[3].scalar != 1.f) ||
+      !(steps >= 1.f && steps <= 32.f) || steps != (float)(uint32_t)steps)
+    return false;
+  const uint64_t rows = w.shape[w.dims - 2], cols = w.shape[w.dims - 1];
+  *t = polar_b200_muon_tensor{w.data, a[0].tensor.data, a[8].tensor.data, rows && cols ? n[7] / (rows * cols) : 0, rows, cols, a[5].scalar, a[6].scalar};
+  *o = polar_b200_muon_options{0.f, a[2].scalar, a[3].scalar != 0.f, (uint32_t)steps, 3.4445f, -4.7750f, 2.0315f, a[1].tensor.data};
+  return true;
+}
 
 }  // namespace polar_b200
 

@@ -10,7 +10,7 @@
 //    result is still written, with the bits its own launch gives; what goes away is reading a
 //    tensor back that the same pass has just computed or read (the four-builtin chain of
 //    (a + b) * c / d -> sigmoid moves 32 instead of 44 bytes per element).
-//  - Weight updates (fadamw, fadamw8) in a row are one launch for all their tensors.
+//  - Weight updates in a row share their launches: fadamw, fadamw8 one for all their tensors, fmuon those of one call for all their matrices.
 //  - From its third run on, a program of many short launches is replayed as a CUDA graph: one host call instead of 2 us
 //    of host time per launch.  Programs of up to three steps, and programs with tensors of two million elements or
 //    more, whose kernels outlast their launches, stay with launches: programmatic dependent launch overlaps them more
@@ -36,6 +36,9 @@ bool use_capture_side_stream(bool on);
 // adamw.cu: the arguments of the builtins "fadamw" and "fadamw8"; whether steps share no memory that one of them writes.
 bool adamw_arguments(const char* name, const polar_b200_arg* a, uint64_t argc, polar_b200_adamw_tensor* t, polar_b200_adamw_options* o);
 bool adamw_independent(const polar_b200_adamw_tensor* tensors, uint64_t count, const float* schedule);
+// muon.cu: the same for the builtin "fmuon".
+bool muon_arguments(const char* name, const polar_b200_arg* a, uint64_t argc, polar_b200_muon_tensor* t, polar_b200_muon_options* o);
+bool muon_independent(const polar_b200_muon_tensor* tensors, uint64_t count, const float* schedule);
 
 namespace {
 
@@ -154,6 +157,8 @@ struct Op {                    // one builtin, its argument list owned by the pr
 struct Step {                  // one builtin, a chain, two chains, or weight updates
   std::vector<polar_b200_adamw_tensor> updates;
   polar_b200_adamw_options options = {};
+  std::vector<polar_b200_muon_tensor> matrices;
+  polar_b200_muon_options muon = {};
   int op = -1;
   ChainParams chain = {}, second = {};   // (one elementwise builtin is a chain of one, for pairing)
   size_t smem = 0;
@@ -369,8 +374,25 @@ void plan(Program* p) {
     p->steps.push_back(std::move(s));
     return true;
   };
+  auto update_matrices = [&](const Op& op) {
+    Step s;
+    s.matrices.resize(1);
+    if (!muon_arguments(op.name.c_str(), op.args.data(), op.args.size(), s.matrices.data(), &s.muon)) return false;
+    flush();
+    if (!p->steps.empty() && !p->steps.back().matrices.empty()) {
+      Step& last = p->steps.back();
+      const polar_b200_muon_options &a = last.muon, &b = s.muon;
+      if (a.momentum == b.momentum && a.nesterov == b.nesterov && a.steps == b.steps && a.schedule == b.schedule) {
+        last.matrices.push_back(s.matrices[0]);
+        if (muon_independent(last.matrices.data(), last.matrices.size(), a.schedule)) return true;
+        last.matrices.pop_back();
+      }
+    }
+    p->steps.push_back(std::move(s));
+    return true;
+  };
   for (size_t i = 0; i < p->ops.size(); ++i) {
-    if (update(p->ops[i])) continue;
+    if (update(p->ops[i]) || update_matrices(p->ops[i])) continue;
     Elementwise e;
     const bool ok = elementwise(p->ops[i], &e);
     if (!ok || !chain.add(e)) {
@@ -392,6 +414,10 @@ int run_steps(Program* p, cudaStream_t stream) {
     int rc;
     if (!s.updates.empty()) {
       rc = polar_b200_fadamw(s.updates.data(), s.updates.size(), &s.options, stream);
+    } else if (!s.matrices.empty()) {
+      // (a workspace for one matrix may be too small for all of them)
+      const bool fits = p->workspace_bytes >= polar_b200_fmuon_workspace_bytes(s.matrices.data(), s.matrices.size());
+      rc = polar_b200_fmuon(s.matrices.data(), s.matrices.size(), &s.muon, fits ? p->workspace : nullptr, p->workspace_bytes, stream);
     } else if (s.op >= 0) {
       const Op& op = p->ops[s.op];
       rc = polar_b200_launch_by_name(op.name.c_str(), op.args.data(), op.args.size(), p->workspace, p->workspace_bytes, stream);

@@ -21,6 +21,7 @@
 #include <polar_b200.h>
 
 #include <algorithm>
+#include <cstring>
 #include <exception>
 #include <vector>
 
@@ -450,12 +451,16 @@ bool operations(PyObject* list, std::vector<polar_b200_op>* ops) {
   }
   return true;
 }
-// workspace_bytes(operations): what the most demanding one asks for.
+// workspace_bytes(operations): what the most demanding one asks for; fmuon builtins in a row, which share their launches, ask together.
 BUILTIN(workspace_bytes) {
   std::vector<polar_b200_op> ops;
   if (n != 1 || !operations(args[0], &ops)) return nullptr;
-  uint64_t need = 0;
-  for (const polar_b200_op& o : ops) need = std::max<uint64_t>(need, polar_b200_launch_workspace_bytes(o.name, o.args, o.argc));
+  uint64_t need = 0, row = 0;
+  for (const polar_b200_op& o : ops) {
+    const uint64_t one = polar_b200_launch_workspace_bytes(o.name, o.args, o.argc);
+    row = std::strcmp(o.name, "fmuon") ? 0 : row + one;
+    need = std::max<uint64_t>({need, one, row});
+  }
   return PyLong_FromUnsignedLongLong(need);
 }
 // create_program(operations, workspace address, its bytes): (status, handle).

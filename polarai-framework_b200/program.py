@@ -54,8 +54,8 @@ class Program:
 
 
 _RESULTS = {"fdense_grad": 2, "flayernorm": 3, "flayernorm_grad": 3, "flogprob": 3, "flogprob_top": 5, "fadamw": 3, "fadamw8": 5,
-            "fpolicy_loss": 3, "fpreference_loss": 3}
-_IN_PLACE = ("fadamw", "fadamw8")                            # these read what they write
+            "fpolicy_loss": 3, "fpreference_loss": 3, "fmuon": 2}
+_IN_PLACE = ("fadamw", "fadamw8", "fmuon")                            # these read what they write
 
 
 def results_of(kernel, args):
@@ -171,37 +171,29 @@ def adamw_moments(p, weight, state_bits=32):
     return [p.tensor(f"{k}_{weight}", s) for k, s in (("m", -(-n // 4)), ("ms", -(-n // 128)), ("v", -(-n // 4)), ("vs", -(-n // 128)))]
 
 
-def norm_classifier_program(batch, n_in=784, n_hidden=4096, n_classes=10, samples=None, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01,
-                            state_bits=32):
-    """A training step of a 2-layer classifier with a layer norm before the hidden activation, on `batch` rows (the rows that one rank holds of
-    `samples` in all): the loss is the mean of -log probability of the rows' labels, the update AdamW.
-
-    Inputs: X, labels (class numbers; below zero: a row that does not count), the weights W1, W2, gamma, beta, the moments m_*, v_*
-    (with 8 bits also ms_*, vs_*: zeros at the beginning) and schedule = [number of steps done, learning rate].  Decay is for the matrices."""
-    p = Program("norm_classifier_step")
-    p.tensor("X", batch, n_in), p.tensor("labels", batch), p.tensor("schedule", 2)
+def _norm_network_forward(p, batch, n_in, n_hidden, n_classes, labels):
+    """Declares a 2-layer network with a layer norm before the hidden activation and its gradients, and computes the rows' log probabilities."""
+    p.tensor("X", batch, n_in), p.tensor(labels, batch), p.tensor("schedule", 2)
     weights = {"W1": (n_in, n_hidden), "W2": (n_hidden, n_classes), "gamma": (n_hidden,), "beta": (n_hidden,)}
     for w, s in weights.items():
         p.tensor(w, *s), p.tensor("d" + w, *s)
-    moments = {w: adamw_moments(p, w, state_bits) for w in weights}
-    p.inputs = ["X", "labels", "schedule", *weights, *[m for ms in moments.values() for m in ms]]
     p.tensor("ones_h", batch, n_hidden), p.tensor("g", batch), p.tensor("tick", 2)
-    p.constants = {"ones_h": 1.0, "g": -1.0 / (samples or batch)}
-    p.inputs.append("tick")                                  # [1, 0]: what a step adds to the schedule
     for t in ("Z1", "N", "H", "dH", "omh", "sh", "dN", "dZ1"):
         p.tensor(t, batch, n_hidden)
     for t in ("mean", "rstd", "logp", "entropy", "lse"):
         p.tensor(t, batch)
     for t in ("Z2", "dZ2"):
         p.tensor(t, batch, n_classes)
-    # forward
     p.op("fmatmul_f_f", "X", "W1", "Z1")
     p.op("flayernorm", "Z1", "gamma", "beta", 1e-5, "N", "mean", "rstd")
     p.op("fsigmoid", "N", "H")
     p.op("fmatmul_f_f", "H", "W2", "Z2")
-    p.op("flogprob", "Z2", "labels", "logp", "entropy", "lse")
-    # backward
-    p.op("flogprob_grad", "Z2", "labels", "lse", "g", "dZ2")
+    p.op("flogprob", "Z2", labels, "logp", "entropy", "lse")
+    return weights
+
+
+def _norm_network_backward(p):
+    """From dZ2, the gradient at the logits, to those of the weights, summed over the ranks."""
     p.op("fmatmul_t_f", "H", "dZ2", "dW2")
     p.op("ALLREDUCE", "dW2")
     p.op("fmatmul_f_t", "dZ2", "W2", "dH")
@@ -213,11 +205,61 @@ def norm_classifier_program(batch, n_in=784, n_hidden=4096, n_classes=10, sample
     p.op("ALLREDUCE", "dbeta")
     p.op("fmatmul_t_f", "X", "dZ1", "dW1")
     p.op("ALLREDUCE", "dW1")
-    # update
+
+
+def norm_classifier_program(batch, n_in=784, n_hidden=4096, n_classes=10, samples=None, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01,
+                            state_bits=32):
+    """A training step of a 2-layer classifier with a layer norm before the hidden activation, on `batch` rows (the rows that one rank holds of
+    `samples` in all): the loss is the mean of -log probability of the rows' labels, the update AdamW.
+
+    Inputs: X, labels (class numbers; below zero: a row that does not count), the weights W1, W2, gamma, beta, the moments m_*, v_*
+    (with 8 bits also ms_*, vs_*: zeros at the beginning) and schedule = [number of steps done, learning rate].  Decay is for the matrices."""
+    p = Program("norm_classifier_step")
+    weights = _norm_network_forward(p, batch, n_in, n_hidden, n_classes, "labels")
+    moments = {w: adamw_moments(p, w, state_bits) for w in weights}
+    p.inputs = ["X", "labels", "schedule", *weights, *[m for ms in moments.values() for m in ms]]
+    p.constants = {"ones_h": 1.0, "g": -1.0 / (samples or batch)}
+    p.inputs.append("tick")                                  # [1, 0]: what a step adds to the schedule
+    p.op("flogprob_grad", "Z2", "labels", "lse", "g", "dZ2")
+    _norm_network_backward(p)
     p.op("fadd", "schedule", 1.0, "tick", 1.0, "schedule")
     for w in weights:
         p.op("fadamw" if state_bits == 32 else "fadamw8", "d" + w, "schedule", beta1, beta2, eps, weight_decay if w[0] == "W" else 0.0, w, *moments[w])
     p.outputs = ["logp", "entropy", *weights, *["d" + w for w in weights]]
+    return p
+
+
+def norm_policy_program(batch, sequences, n_in=784, n_hidden=4096, n_actions=10, clip_low=0.2, clip_high=0.2, kl_weight=0.0, entropy_weight=0.0,
+                        count=0.0, by_sequence=False, momentum=0.95, rounds=5, weight_decay=0.01, beta1=0.9, beta2=0.999, eps=1e-8):
+    """A policy gradient step of the network of norm_classifier_program on `batch` rows of `sequences` packed sequences: the clipped policy loss of the
+    actions that were sampled, with a KL term against a reference's log probabilities and an entropy bonus; the matrices are updated by
+    orthogonalised momentum, the vectors by AdamW.  `count`: what the loss's mean is taken over where the rows are one rank's share.
+
+    Inputs: X, actions (numbers of classes; below zero: a row that does not count), offsets[sequences + 1], old_logp and ref_logp of the
+    actions, advantage[sequences], the weights W1, W2, gamma, beta, the momenta M_W1, M_W2, the moments m_gamma, v_gamma, m_beta, v_beta
+    (zeros at the beginning), and schedule = [number of steps done, learning rate] and tick = [1, 0]."""
+    p = Program("norm_policy_step")
+    weights = _norm_network_forward(p, batch, n_in, n_hidden, n_actions, "actions")
+    p.tensor("offsets", sequences + 1), p.tensor("advantage", sequences), p.tensor("loss", 5)
+    for t in ("old_logp", "ref_logp", "g_entropy"):
+        p.tensor(t, batch)
+    momenta = [p.tensor("M_" + w, *weights[w]) for w in ("W1", "W2")]
+    moments = {w: adamw_moments(p, w) for w in ("gamma", "beta")}
+    p.inputs = ["X", "actions", "offsets", "old_logp", "ref_logp", "advantage", "schedule", "tick", *weights, *momenta,
+                *[m for ms in moments.values() for m in ms]]
+    # rows outside the sequences have no gradient: the loss leaves what stands there
+    p.constants = {"ones_h": 1.0, "g": 0.0, "g_entropy": 0.0}
+    p.op("fpolicy_loss", "logp", "old_logp", "ref_logp", "entropy", "advantage", "actions", "offsets", clip_low, clip_high, kl_weight, entropy_weight, count,
+         float(by_sequence), "loss", "g", "g_entropy")
+    p.op("flogprob_grad", "Z2", "actions", "lse", "entropy", "g", "g_entropy", "dZ2")
+    _norm_network_backward(p)
+    p.op("fadd", "schedule", 1.0, "tick", 1.0, "schedule")
+    for w, m in zip(("W1", "W2"), momenta):
+        rows, cols = weights[w]
+        p.op("fmuon", "d" + w, "schedule", momentum, 1.0, float(rounds), weight_decay, max(1.0, rows / cols) ** 0.5, w, m)
+    for w in ("gamma", "beta"):
+        p.op("fadamw", "d" + w, "schedule", beta1, beta2, eps, 0.0, w, *moments[w])
+    p.outputs = ["logp", "entropy", "loss", *weights, *["d" + w for w in weights]]
     return p
 
 

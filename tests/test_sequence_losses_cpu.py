@@ -100,20 +100,20 @@ def test_by_name_patterns(c):
         return c.polar_b200_launch_by_name(name.encode(), arr, len(given), None, 0, None), c.polar_b200_launch_workspace_bytes(name.encode(), arr, len(given))
 
     t, s, o = (50,), (4,), (5,)
-    good = [t, t, t, t, s, t, o, 0.2, 0.2, 0.1, 0.1, 0.0, (5,), t, t]
-    for i, bad in ((0, s), (3, s), (4, (3,)), (5, (5, 10)), (6, (0,)), (6, (2, 2)), (11, 0.5), (12, s), (13, s), (14, s), (7, t)):
+    good = [t, t, t, t, s, t, o, 0.2, 0.2, 0.1, 0.1, 0.0, 0.0, (5,), t, t]
+    for i, bad in ((0, s), (3, s), (4, (3,)), (5, (5, 10)), (6, (0,)), (6, (2, 2)), (12, 0.5), (13, s), (14, s), (15, s), (7, t)):
         args = list(good)
         args[i] = bad
         assert call("fpolicy_loss", *args)[0] == 3
     assert call("fpolicy_loss", *good[:-1])[0] == 3
-    good = [t, t, t, o, 0.1, 0.0, 0.0, 1.0, (3,), s, t]
-    for i, bad in ((0, s), (1, s), (3, s), (3, (1, 5)), (7, 2.0), (8, s), (9, o), (10, s), (4, t)):
+    good = [t, t, t, o, 0.1, 0.0, 0.0, 0.0, 1.0, (3,), s, t]
+    for i, bad in ((0, s), (1, s), (3, s), (3, (1, 5)), (8, 2.0), (9, s), (10, o), (11, s), (4, t)):
         args = list(good)
         args[i] = bad
         assert call("fpreference_loss", *args)[0] == 3
     big, offs = (100000,), (5,)
-    assert call("fpolicy_loss", big, big, big, big, (9,), big, offs, 0.2, 0.2, 0.1, 0.1, 0.0, (5,), big, big)[1] == c.polar_b200_fpolicy_loss_workspace_bytes(100000, 4)
-    assert call("fpreference_loss", big, big, big, offs, 0.1, 0.0, 0.0, 1.0, (3,), (9,), big)[1] == c.polar_b200_fpreference_loss_workspace_bytes(100000, 2)
+    assert call("fpolicy_loss", big, big, big, big, (9,), big, offs, 0.2, 0.2, 0.1, 0.1, 0.0, 0.0, (5,), big, big)[1] == c.polar_b200_fpolicy_loss_workspace_bytes(100000, 4)
+    assert call("fpreference_loss", big, big, big, offs, 0.1, 0.0, 0.0, 0.0, 1.0, (3,), (9,), big)[1] == c.polar_b200_fpreference_loss_workspace_bytes(100000, 2)
     assert c.polar_b200_result_count(b"fpolicy_loss") == 3 and c.polar_b200_result_count(b"fpreference_loss") == 3
 
 
