@@ -182,16 +182,18 @@ struct Cfg {
   static constexpr uint32_t kSmemBytes = kTileBytes + 1024 + 256;
 };
 
-enum Kind : int { kGram, kPolynomial, kRound, kUpdate };
+enum Kind : int { kSymmetric, kRound, kUpdate };
 
 struct Shape {                                             // the matrices of one shape, in one product
   CUtensorMap a, b;
+  int kind;
+  float by, add_by, diagonal;                              // result = by * sum + add_by * add + diagonal (on the diagonal)
   uint32_t m, n, k;
   uint32_t tiles_m, tiles_n, tiles;                        // tiles: of one matrix
   uint32_t first_tile;                                     // of the launch
   int a_mn, b_mn;                                          // operands whose rows are not contiguous along k
   __half* out;                                             // matrix z: planes 2 z (hi) and 2 z + 1 (lo)
-  const __half* add;                                       // of the same layout
+  const __half* add;                                       // of the same layout; or nullptr
   uint64_t plane;
   uint32_t pitch;
   uint32_t first_target;
@@ -199,8 +201,6 @@ struct Shape {                                             // the matrices of on
 constexpr int kShapes = 16;
 struct Product {
   uint32_t shapes, tiles;
-  int kind;
-  float by, add_by, diagonal;                              // result = by * sum + add_by * add + diagonal (on the diagonal)
   float lr;
   const float* schedule;
   const Target* targets;
@@ -223,7 +223,7 @@ __device__ __forceinline__ Place place_of(const Product& p, uint32_t t) {
   t -= s.first_tile;
   at.z = t / s.tiles;
   t -= at.z * s.tiles;
-  if (p.kind <= kPolynomial) {
+  if (s.kind == kSymmetric) {
     uint32_t i = 0, skip = 0;
     while (t >= s.tiles_n - skip) {
       t -= s.tiles_n - skip;
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
   if (warp >= 4) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
     const int quarter = warp & 3, half = (warp - 4) >> 2;
-    const float lr = p.kind == kUpdate ? (p.schedule ? p.schedule[1] : p.lr) : 0.f;
+    const float lr = p.schedule ? p.schedule[1] : p.lr;
     uint32_t run = 0;
     bool ok = true;
     for (uint32_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x) {
@@ -346,16 +346,16 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
       const uint32_t r0 = (uint32_t)at.m0 + quarter * 32, row = r0 + lane;
       __half* const hi_plane = q.out + 2 * at.z * q.plane;
       Target target = {};
-      if (p.kind == kUpdate) target = p.targets[q.first_target + at.z];
-      const float keep = 1.f - lr * target.decay, rate = p.by * lr * target.scale;
+      if (q.kind == kUpdate) target = p.targets[q.first_target + at.z];
+      const float keep = 1.f - lr * target.decay, rate = q.by * lr * target.scale;
       const bool vectors = (q.n & 3) == 0 && (reinterpret_cast<uintptr_t>(target.weights) & 15) == 0;
 #pragma unroll
       for (int block = 0; block < BN / 64; ++block) {
         const uint32_t c0 = (uint32_t)at.n0 + half * (BN / 2) + 32 * block;
         uint32_t(&r)[32] = sum[block];
         if (c0 >= q.n || r0 >= q.m) break;
-        if (p.kind <= kPolynomial && c0 < r0) continue;      // below the diagonal: written by the block above it
-        if (p.kind == kUpdate) {
+        if (q.kind == kSymmetric && c0 < r0) continue;      // below the diagonal: written by the block above it
+        if (q.kind == kUpdate) {
           float* w = target.weights + (uint64_t)row * q.n + c0;
           if (row >= q.m) {
           } else if (vectors && c0 + 32 <= q.n) {
@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
         for (int part = 0; part < 2; ++part) {
           uint32_t* const v = r + 16 * part;
           uint32_t hi[8], lo[8];                           // two columns in each
-          if (p.kind == kPolynomial) {
+          if (q.add) {
             const __half* add = q.add + 2 * at.z * q.plane + (uint64_t)row * q.pitch + c0 + 16 * part;
             if (row < q.m) {
 #pragma unroll
@@ -392,16 +392,16 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const float2 h = __half22float2(*reinterpret_cast<__half2*>(&hi[j])), l = __half22float2(*reinterpret_cast<__half2*>(&lo[j]));
-              float a = fmaf(p.by, __uint_as_float(v[2 * j]), p.add_by * (h.x + l.x));
-              float b = fmaf(p.by, __uint_as_float(v[2 * j + 1]), p.add_by * (h.y + l.y));
+              float a = fmaf(q.by, __uint_as_float(v[2 * j]), q.add_by * (h.x + l.x));
+              float b = fmaf(q.by, __uint_as_float(v[2 * j + 1]), q.add_by * (h.y + l.y));
               const uint32_t col = c0 + 16 * part + 2 * j;
-              if (col == row) a += p.diagonal;
-              if (col + 1 == row) b += p.diagonal;
+              if (col == row) a += q.diagonal;
+              if (col + 1 == row) b += q.diagonal;
               v[2 * j] = __float_as_uint(a), v[2 * j + 1] = __float_as_uint(b);
             }
           } else {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(p.by * __uint_as_float(v[j]));
+            for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(q.by * __uint_as_float(v[j]));
           }
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
             st_v8(out + 16 * part, hi);
             st_v8(out + 16 * part + q.plane, lo);
           }
-          if (p.kind <= kPolynomial && c0 > r0) {          // its mirror image: a column of the block is a row there, 32 lanes side by side
+          if (q.kind == kSymmetric && c0 > r0) {          // its mirror image: a column of the block is a row there, 32 lanes side by side
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               if (c0 + 16 * part + j < q.n) {
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
       const Shape& q = p.s[at.shape];
       const int slabs = (int)((q.k + BK - 1) / BK);
       // where the left half of a symmetric product's tile lies below the diagonal, the right half alone: 128 rows or two chunks further
-      const uint32_t left_out = BN == 256 && p.kind <= kPolynomial && at.m0 == at.n0 + 128 ? 128 : 0;
+      const uint32_t left_out = BN == 256 && q.kind == kSymmetric && at.m0 == at.n0 + 128 ? 128 : 0;
       const uint32_t idesc = f16_idesc(BN - left_out, q.a_mn, q.b_mn);
       // K-major: 64-byte swizzle (layout 4), groups of 8 rows 512 bytes apart, 16 k 32 bytes on.  MN-major: 128-byte swizzle (layout 2), chunks
       // of 64 columns BK rows apart, groups of 8 k 1024 bytes, 16 k 2048 bytes on.
@@ -560,7 +560,7 @@ struct One {                                               // a matrix of the ca
 struct Kin {                                               // the matrices of one shape
   uint64_t rows, cols, count, first;                       // first: among the sorted matrices
   uint64_t pitch, side, side_pitch;                        // side: the shorter one
-  __half *x[2], *g, *p;
+  __half *x[2], *s[3];                                     // X, and the symmetric matrices
 };
 uint64_t up64(uint64_t n) { return (n + 63) / 64 * 64; }
 uint64_t up256(uint64_t n) { return (n + 255) & ~255ull; }
@@ -568,9 +568,11 @@ uint64_t chunk_of(uint64_t count) {
   const uint64_t each = (count + kMostChunks - 1) / kMostChunks;
   return each <= kChunk ? kChunk : (each + kChunk - 1) / kChunk * kChunk;
 }
-uint64_t bytes_of(uint64_t rows, uint64_t cols) {          // of one matrix: X twice, G and P, two planes each
+// Two rounds at a time where the shorter side is so much shorter (see `operations_of`): then there are three symmetric matrices, else two.
+bool in_pairs(uint64_t rows, uint64_t cols) { return std::max(rows, cols) >= 2 * std::min(rows, cols); }
+uint64_t bytes_of(uint64_t rows, uint64_t cols) {          // of one matrix: X twice and the symmetric ones, two planes each
   const uint64_t side = std::min(rows, cols);
-  return 2 * 2 * 2 * (rows * up64(cols) + side * up64(side)) + 4 * 256;
+  return 2 * 2 * (2 * rows * up64(cols) + (in_pairs(rows, cols) ? 3 : 2) * side * up64(side)) + 5 * 256;
 }
 // What one group of matrices may take; a step of more is done in several.
 constexpr uint64_t kGroupBytes = 3ull << 30;
@@ -588,7 +590,7 @@ uint64_t lay_out(char* base, const std::vector<One>& all, size_t from, size_t to
     chunks += (o.rows * o.cols + chunk_of(o.rows * o.cols) - 1) / chunk_of(o.rows * o.cols);
     if (kin->empty() || kin->back().rows != o.rows || kin->back().cols != o.cols) {
       const uint64_t side = std::min(o.rows, o.cols);
-      kin->push_back(Kin{o.rows, o.cols, 0, i - from, up64(o.cols), side, up64(side), {nullptr, nullptr}, nullptr, nullptr});
+      kin->push_back(Kin{o.rows, o.cols, 0, i - from, up64(o.cols), side, up64(side), {nullptr, nullptr}, {nullptr, nullptr, nullptr}});
     }
     ++kin->back().count;
   }
@@ -596,8 +598,7 @@ uint64_t lay_out(char* base, const std::vector<One>& all, size_t from, size_t to
   *targets = reinterpret_cast<Target*>(take((to - from) * sizeof(Target)));
   for (Kin& k : *kin) {
     for (int b = 0; b < 2; ++b) k.x[b] = reinterpret_cast<__half*>(take(k.count * 4 * k.rows * k.pitch));
-    k.g = reinterpret_cast<__half*>(take(k.count * 4 * k.side * k.side_pitch));
-    k.p = reinterpret_cast<__half*>(take(k.count * 4 * k.side * k.side_pitch));
+    for (int b = 0; b < (in_pairs(k.rows, k.cols) ? 3 : 2); ++b) k.s[b] = reinterpret_cast<__half*>(take(k.count * 4 * k.side * k.side_pitch));
   }
   return at;
 }
@@ -629,50 +630,79 @@ int launch_tables(const std::vector<One>& all, size_t from, size_t to, const std
   return POLAR_B200_OK;
 }
 
-template <int BN>
-int launch_product(const std::vector<Kin>& kin, int kind, int from_x, const polar_b200_muon_options& o, const Target* targets, int* status, cudaStream_t st) {
-  static thread_local Product p;
-  p.kind = kind;
-  p.lr = o.lr, p.schedule = o.schedule, p.targets = targets, p.status = status, p.wait_ns = wait_limit_ns(2000000000ull);
-  p.add_by = p.diagonal = 0.f;
-  switch (kind) {
-    case kGram: p.by = kG / (kX * kX); break;
-    case kPolynomial: p.by = o.c * (kP / (kG * kG)), p.add_by = o.b * (kP / kG), p.diagonal = o.a * kP; break;
-    case kRound: p.by = 1.f / kP; break;
-    default: p.by = 1.f / (kP * kX);
+// One product of the matrices of a shape: of X (from x[from]) with itself, of symmetric matrices s[left] s[right] that commute, or of s[left] and X.
+struct Operation {
+  enum { kGram, kProduct, kMove } what;
+  int left, right, out, add;                               // add: -1 for none
+  float by, add_by, diagonal;
+  bool last;
+};
+// A round by itself: G, P = a + b G + c G G, X <- P X.  Two rounds P' P X with the second one's G' = (P X)(P X)^T = P G P:
+//   G, P, T = P G, G' = P T, P', Q = P' P, X <- Q X
+// are five products of the shorter side alone in place of two products with X (work of 3 short^2 long for one of 3 short^3): 1024 x 4096 takes three quarters
+// of the operations.  Not more rounds at a time: what rounding leaves in G for small singular values grows by a^2 in each further one.
+std::vector<Operation> operations_of(const Kin& k, const polar_b200_muon_options& o) {
+  std::vector<Operation> ops;
+  constexpr float kQ = 4096.f;                             // kBoundP^2 * 2^12 is below 65504
+  auto product = [&](int l, int r, int out, float by) { ops.push_back(Operation{Operation::kProduct, l, r, out, -1, by, 0.f, 0.f, false}); };
+  auto polynomial = [&](int g, int out) { ops.push_back(Operation{Operation::kProduct, g, g, out, g, o.c * (kP / (kG * kG)), o.b * (kP / kG), o.a * kP, false}); };
+  for (uint32_t i = 0; i < o.steps;) {
+    ops.push_back(Operation{Operation::kGram, 0, 0, 0, -1, kG / (kX * kX), 0.f, 0.f, false});
+    polynomial(0, 1);
+    const bool two = i + 1 < o.steps && in_pairs(k.rows, k.cols);
+    if (two) {
+      product(1, 0, 2, 1.f / kP);                          // T as G: its eigenvalues are products of two singular values of X, before and after
+      product(1, 2, 0, 1.f / kP);
+      polynomial(0, 2);
+      product(2, 1, 0, kQ / (kP * kP));
+    }
+    i += two ? 2 : 1;
+    const float held = two ? kQ : kP;
+    ops.push_back(Operation{Operation::kMove, two ? 0 : 1, 0, 0, -1, i < o.steps ? 1.f / held : 1.f / (held * kX), 0.f, 0.f, i == o.steps});
   }
-  for (size_t k = 0; k < kin.size();) {
+  return ops;
+}
+
+// The next operation of every shape, longest sums first.
+template <int BN>
+int launch_product(const std::vector<Kin>& kin, const std::vector<std::pair<size_t, Operation>>& ops, const std::vector<int>& from_x, const polar_b200_muon_options& o,
+                   const Target* targets, int* status, cudaStream_t st) {
+  static thread_local Product p;
+  p.lr = o.lr, p.schedule = o.schedule, p.targets = targets, p.status = status, p.wait_ns = wait_limit_ns(2000000000ull);
+  for (size_t k = 0; k < ops.size();) {
     p.shapes = p.tiles = 0;
-    for (; k < kin.size() && p.shapes < kShapes; ++k) {
-      const Kin& q = kin[k];
-      const bool wide = q.rows <= q.cols, square = kind <= kPolynomial;
+    for (; k < ops.size() && p.shapes < kShapes; ++k) {
+      const Kin& q = kin[ops[k].first];
+      const Operation& op = ops[k].second;
+      const int from = from_x[ops[k].first];
+      const bool wide = q.rows <= q.cols, square = op.what != Operation::kMove;
       Shape& s = p.s[p.shapes];
       int rc = POLAR_B200_OK;
-      auto x = [&](CUtensorMap* map, bool mn, uint32_t tile) { return make_map(map, q.x[from_x], q.rows, q.cols, q.pitch, 2 * q.count, mn, tile); };
-      auto symmetric = [&](CUtensorMap* map, const __half* t, uint32_t tile) {
-        return make_map(map, t, q.side, q.side, q.side_pitch, 2 * q.count, false, tile);
+      auto x = [&](CUtensorMap* map, bool mn, uint32_t tile) { return make_map(map, q.x[from], q.rows, q.cols, q.pitch, 2 * q.count, mn, tile); };
+      auto symmetric = [&](CUtensorMap* map, int t, uint32_t tile) {
+        return make_map(map, q.s[t], q.side, q.side, q.side_pitch, 2 * q.count, false, tile);
       };
+      s.kind = square ? kSymmetric : op.last ? kUpdate : kRound;
+      s.by = op.by, s.add_by = op.add_by, s.diagonal = op.diagonal;
+      s.add = op.add >= 0 ? q.s[op.add] : nullptr;
       s.a_mn = s.b_mn = 0;
-      s.add = nullptr;
-      if (kind == kGram) {                                 // X X^T, or X^T X
+      if (op.what == Operation::kGram) {                   // X X^T, or X^T X
         s.m = s.n = (uint32_t)q.side, s.k = (uint32_t)std::max(q.rows, q.cols);
         s.a_mn = s.b_mn = !wide;
         rc = x(&s.a, !wide, BM);
         if (!rc) rc = x(&s.b, !wide, BN);
-        s.out = q.g;
-      } else if (kind == kPolynomial) {
+      } else if (op.what == Operation::kProduct) {
         s.m = s.n = s.k = (uint32_t)q.side;
-        rc = symmetric(&s.a, q.g, BM);
-        if (!rc) rc = symmetric(&s.b, q.g, BN);
-        s.out = q.p, s.add = q.g;
+        rc = symmetric(&s.a, op.left, BM);
+        if (!rc) rc = symmetric(&s.b, op.right, BN);
       } else {                                             // P X, or X P
         s.m = (uint32_t)q.rows, s.n = (uint32_t)q.cols, s.k = (uint32_t)q.side;
         s.b_mn = wide;
-        rc = wide ? symmetric(&s.a, q.p, BM) : x(&s.a, false, BM);
-        if (!rc) rc = wide ? x(&s.b, true, BN) : symmetric(&s.b, q.p, BN);
-        s.out = q.x[from_x ^ 1];
+        rc = wide ? symmetric(&s.a, op.left, BM) : x(&s.a, false, BM);
+        if (!rc) rc = wide ? x(&s.b, true, BN) : symmetric(&s.b, op.left, BN);
       }
       if (rc) return rc;
+      s.out = square ? q.s[op.out] : q.x[from ^ 1];
       s.pitch = (uint32_t)(square ? q.side_pitch : q.pitch);
       s.plane = square ? q.side * q.side_pitch : q.rows * q.pitch;
       s.first_target = (uint32_t)q.first;
@@ -740,11 +770,24 @@ int run_group(const std::vector<One>& all, size_t from, size_t to, const polar_b
                                    : launch_tables<kManyMatrices>(all, from, to, kin, o, partial, targets, st, begin);
     if (rc) return rc;
   }
-  for (uint32_t i = 0; i < o.steps; ++i) {
-    for (int kind : {(int)kGram, (int)kPolynomial, i + 1 < o.steps ? (int)kRound : (int)kUpdate}) {
-      rc = launch_product<256>(kin, kind, (int)(i & 1), o, targets, status, st);
-      if (rc) return rc;
-    }
+  std::vector<std::vector<Operation>> ops;
+  std::vector<int> from_x(kin.size(), 0);
+  size_t most = 0;
+  for (const Kin& k : kin) {
+    ops.push_back(operations_of(k, o));
+    most = std::max(most, ops.back().size());
+  }
+  for (size_t i = 0; i < most; ++i) {
+    std::vector<std::pair<size_t, Operation>> now;
+    for (size_t k = 0; k < kin.size(); ++k)
+      if (i < ops[k].size()) now.emplace_back(k, ops[k][i]);
+    auto sum = [&](const std::pair<size_t, Operation>& a) {
+      return a.second.what == Operation::kGram ? std::max(kin[a.first].rows, kin[a.first].cols) : kin[a.first].side;
+    };
+    std::stable_sort(now.begin(), now.end(), [&](const auto& a, const auto& b) { return sum(a) > sum(b); });
+    rc = launch_product<256>(kin, now, from_x, o, targets, status, st);
+    if (rc) return rc;
+    for (const auto& a : now) from_x[a.first] ^= a.second.what == Operation::kMove;
   }
   return POLAR_B200_OK;
 }
