@@ -200,7 +200,7 @@ struct Shape {                                             // the matrices of on
 };
 constexpr int kShapes = 16;
 struct Product {
-  uint32_t shapes, tiles;
+  uint32_t shapes, tiles, splits;
   float lr;
   const float* schedule;
   const Target* targets;
@@ -261,8 +261,86 @@ __device__ __forceinline__ uint32_t f16_idesc(int n, int a_mn, int b_mn) {
   return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
 }
 __device__ __forceinline__ void st_v8(void* dst, const uint32_t* r) { st_global_v8(static_cast<float*>(dst), r); }
+__device__ __forceinline__ Target target_of(const Product& p, const Shape& q, const Place& at) {
+  return q.kind == kUpdate ? p.targets[q.first_target + at.z] : Target{};
+}
 
-// One CTA per SM walks 128 x BN tiles.
+// Writes 16 columns of the result from c0 on of row r0 + lane, whose sums are in `v`.
+__device__ __forceinline__ void finish(const Shape& q, const Place& at, const Target& target, float lr, uint32_t r0, uint32_t c0, int lane, uint32_t* v) {
+  const uint32_t row = r0 + lane, block = c0 & ~31u;
+  if (c0 >= q.n || r0 >= q.m) return;
+  if (q.kind == kSymmetric && block < r0) return;          // below the diagonal: written by the block above it
+  if (q.kind == kUpdate) {
+    const float keep = 1.f - lr * target.decay, rate = q.by * lr * target.scale;
+    float* const w = target.weights + (uint64_t)row * q.n + c0;
+    if (row >= q.m) return;
+    if ((q.n & 3) == 0 && (reinterpret_cast<uintptr_t>(target.weights) & 15) == 0 && c0 + 16 <= q.n) {
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) {
+        float4 x = *reinterpret_cast<const float4*>(w + j);
+        x.x = x.x * keep - rate * __uint_as_float(v[j]), x.y = x.y * keep - rate * __uint_as_float(v[j + 1]);
+        x.z = x.z * keep - rate * __uint_as_float(v[j + 2]), x.w = x.w * keep - rate * __uint_as_float(v[j + 3]);
+        *reinterpret_cast<float4*>(w + j) = x;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (c0 + j < q.n) w[j] = w[j] * keep - rate * __uint_as_float(v[j]);
+    }
+    return;
+  }
+  __half* const matrix = q.out + 2 * at.z * q.plane;
+  uint32_t hi[8], lo[8];                                   // two columns in each
+  if (q.add) {
+    const __half* add = q.add + 2 * at.z * q.plane + (uint64_t)row * q.pitch + c0;
+    if (row < q.m) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint4 h = *reinterpret_cast<const uint4*>(add + 8 * j), l = *reinterpret_cast<const uint4*>(add + q.plane + 8 * j);
+        hi[4 * j] = h.x, hi[4 * j + 1] = h.y, hi[4 * j + 2] = h.z, hi[4 * j + 3] = h.w;
+        lo[4 * j] = l.x, lo[4 * j + 1] = l.y, lo[4 * j + 2] = l.z, lo[4 * j + 3] = l.w;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 h = __half22float2(*reinterpret_cast<__half2*>(&hi[j])), l = __half22float2(*reinterpret_cast<__half2*>(&lo[j]));
+      float a = fmaf(q.by, __uint_as_float(v[2 * j]), q.add_by * (h.x + l.x));
+      float b = fmaf(q.by, __uint_as_float(v[2 * j + 1]), q.add_by * (h.y + l.y));
+      if (c0 + 2 * j == row) a += q.diagonal;
+      if (c0 + 2 * j + 1 == row) b += q.diagonal;
+      v[2 * j] = __float_as_uint(a), v[2 * j + 1] = __float_as_uint(b);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(q.by * __uint_as_float(v[j]));
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float a = __uint_as_float(v[2 * j]), b = __uint_as_float(v[2 * j + 1]);
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    hi[j] = *reinterpret_cast<const uint32_t*>(&h), lo[j] = *reinterpret_cast<const uint32_t*>(&l);
+  }
+  if (row < q.m) {                                         // (columns behind the last one lie in the row's padding)
+    __half* const out = matrix + (uint64_t)row * q.pitch + c0;
+    st_v8(out, hi);
+    st_v8(out + q.plane, lo);
+  }
+  if (q.kind == kSymmetric && block > r0) {                // its mirror image: a column of the block is a row there, 32 lanes side by side
+    unsigned short* const mirror = reinterpret_cast<unsigned short*>(matrix) + (uint64_t)c0 * q.pitch + row;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      if (c0 + j < q.n) {
+        mirror[(uint64_t)j * q.pitch] = (unsigned short)(hi[j / 2] >> (j & 1) * 16);
+        mirror[(uint64_t)j * q.pitch + q.plane] = (unsigned short)(lo[j / 2] >> (j & 1) * 16);
+      }
+    }
+  }
+}
+
+// One CTA per SM walks 128 x BN tiles; or, SPLIT, where there are too few tiles to go round, a cluster of up to eight CTAs has one tile, each CTA
+// a share of its slabs, and they add their sums through shared memory, each a part of the tile.
 //   warp 0     TMA: both planes of a slab of 32 k of each operand, one instruction each.  An operand that is contiguous along k is K-major
 //              (rows of 64 bytes in the 64-byte swizzle), else MN-major (chunks of 64 columns, 128-byte swizzle, a row per k).
 //   warp 1     tcgen05.mma: per 16 k  hi hi, lo hi, hi lo, into two accumulators in tensor memory by turns, each for kRun slabs.
@@ -272,7 +350,7 @@ __device__ __forceinline__ void st_v8(void* dst, const uint32_t* r) { st_global_
 // more than all else does to them (784 x 4096: the update 6.4e-5 from the exact one).  The registers' sums are rounded to nearest, and with runs
 // of 128 k there are 24 additions to a cut sum (784 x 4096: 7.7e-6); reading the accumulators costs the tensor core nothing.
 // Every wait is bounded; when one gives up, all roles leave, and the status word holds its code (7xx).
-template <int BN>
+template <int BN, bool SPLIT>
 __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __grid_constant__ Product p) {
   using C = Cfg<BN>;
   constexpr int S = C::kStages;
@@ -303,18 +381,32 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   pdl_enter();
+  const uint32_t splits = SPLIT ? p.splits : 1, rank = SPLIT ? cluster_rank() : 0;
+  const uint32_t first = SPLIT ? blockIdx.x / splits : blockIdx.x, step = SPLIT ? p.tiles : gridDim.x;
+  auto slabs_of = [&](const Shape& q, int* end) {            // this CTA's
+    const int slabs = (int)((q.k + BK - 1) / BK), each = (slabs + (int)splits - 1) / (int)splits;
+    *end = min(slabs, (int)(rank + 1) * each);
+    return min(slabs, (int)rank * each);
+  };
+  const float lr = p.schedule ? p.schedule[1] : p.lr;
 
   if (warp >= 4) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
+    if constexpr (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
     const int quarter = warp & 3, half = (warp - 4) >> 2;
-    const float lr = p.schedule ? p.schedule[1] : p.lr;
     uint32_t run = 0;
     bool ok = true;
-    for (uint32_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x) {
+    for (uint32_t t = first; ok && t < p.tiles; t += step) {
       const Place at = place_of<BN>(p, t);
       const Shape& q = p.s[at.shape];
       uint32_t sum[BN / 64][32];                           // this thread's row of its half of the tile, as bits of floats
-      const int runs = (int)((q.k + kRun * BK - 1) / (kRun * BK));
+      int end;
+      const int begin = slabs_of(q, &end), runs = (end - begin + kRun - 1) / kRun;
+      if (SPLIT && runs == 0) {
+#pragma unroll
+        for (int j = 0; j < BN / 64; ++j)
+#pragma unroll
+          for (int e = 0; e < 32; ++e) sum[j][e] = 0;
+      }
       for (int i = 0; i < runs; ++i, ++run) {
         const uint32_t as = run & 1u;
         ok = mbar_wait(acc_full(as), (run >> 1) & 1u, abort_flag, p.status, 704, p.wait_ns);
@@ -343,103 +435,34 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
         if (lane == 0) mbar_arrive(acc_empty(as));
       }
       if (!ok) break;
-      const uint32_t r0 = (uint32_t)at.m0 + quarter * 32, row = r0 + lane;
-      __half* const hi_plane = q.out + 2 * at.z * q.plane;
-      Target target = {};
-      if (q.kind == kUpdate) target = p.targets[q.first_target + at.z];
-      const float keep = 1.f - lr * target.decay, rate = q.by * lr * target.scale;
-      const bool vectors = (q.n & 3) == 0 && (reinterpret_cast<uintptr_t>(target.weights) & 15) == 0;
+      const Target target = target_of(p, q, at);
+      if constexpr (SPLIT) {
+        // (the slabs have been read: the last product has been waited for)
+        float* const shared = reinterpret_cast<float*>(smem_gen);
 #pragma unroll
-      for (int block = 0; block < BN / 64; ++block) {
-        const uint32_t c0 = (uint32_t)at.n0 + half * (BN / 2) + 32 * block;
-        uint32_t(&r)[32] = sum[block];
-        if (c0 >= q.n || r0 >= q.m) break;
-        if (q.kind == kSymmetric && c0 < r0) continue;      // below the diagonal: written by the block above it
-        if (q.kind == kUpdate) {
-          float* w = target.weights + (uint64_t)row * q.n + c0;
-          if (row >= q.m) {
-          } else if (vectors && c0 + 32 <= q.n) {
+        for (int j = 0; j < BN / 64; ++j)
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              float4 v = *reinterpret_cast<const float4*>(w + j);
-              v.x = v.x * keep - rate * __uint_as_float(r[j]), v.y = v.y * keep - rate * __uint_as_float(r[j + 1]);
-              v.z = v.z * keep - rate * __uint_as_float(r[j + 2]), v.w = v.w * keep - rate * __uint_as_float(r[j + 3]);
-              *reinterpret_cast<float4*>(w + j) = v;
-            }
-          } else {
+          for (int e = 0; e < 32; ++e) shared[(half * (BN / 2) + 32 * j + e) * BM + quarter * 32 + lane] = __uint_as_float(sum[j][e]);
+      } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (c0 + j < q.n) w[j] = w[j] * keep - rate * __uint_as_float(r[j]);
-          }
-          continue;
-        }
-        __half* const out = hi_plane + (uint64_t)row * q.pitch + c0;
-        unsigned short* const mirror = reinterpret_cast<unsigned short*>(hi_plane) + (uint64_t)c0 * q.pitch + row;
-#pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          uint32_t* const v = r + 16 * part;
-          uint32_t hi[8], lo[8];                           // two columns in each
-          if (q.add) {
-            const __half* add = q.add + 2 * at.z * q.plane + (uint64_t)row * q.pitch + c0 + 16 * part;
-            if (row < q.m) {
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const uint4 h = *reinterpret_cast<const uint4*>(add + 8 * j), l = *reinterpret_cast<const uint4*>(add + q.plane + 8 * j);
-                hi[4 * j] = h.x, hi[4 * j + 1] = h.y, hi[4 * j + 2] = h.z, hi[4 * j + 3] = h.w;
-                lo[4 * j] = l.x, lo[4 * j + 1] = l.y, lo[4 * j + 2] = l.z, lo[4 * j + 3] = l.w;
-              }
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float2 h = __half22float2(*reinterpret_cast<__half2*>(&hi[j])), l = __half22float2(*reinterpret_cast<__half2*>(&lo[j]));
-              float a = fmaf(q.by, __uint_as_float(v[2 * j]), q.add_by * (h.x + l.x));
-              float b = fmaf(q.by, __uint_as_float(v[2 * j + 1]), q.add_by * (h.y + l.y));
-              const uint32_t col = c0 + 16 * part + 2 * j;
-              if (col == row) a += q.diagonal;
-              if (col + 1 == row) b += q.diagonal;
-              v[2 * j] = __float_as_uint(a), v[2 * j + 1] = __float_as_uint(b);
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(q.by * __uint_as_float(v[j]));
-          }
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float a = __uint_as_float(v[2 * j]), b = __uint_as_float(v[2 * j + 1]);
-            const __half2 h = __floats2half2_rn(a, b);
-            const float2 f = __half22float2(h);
-            const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
-            hi[j] = *reinterpret_cast<const uint32_t*>(&h), lo[j] = *reinterpret_cast<const uint32_t*>(&l);
-          }
-          if (row < q.m) {                                 // (columns behind the last one lie in the row's padding)
-            st_v8(out + 16 * part, hi);
-            st_v8(out + 16 * part + q.plane, lo);
-          }
-          if (q.kind == kSymmetric && c0 > r0) {          // its mirror image: a column of the block is a row there, 32 lanes side by side
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              if (c0 + 16 * part + j < q.n) {
-                unsigned short* const o = mirror + (uint64_t)(16 * part + j) * q.pitch;
-                o[0] = (unsigned short)(hi[j / 2] >> (j & 1) * 16);
-                o[q.plane] = (unsigned short)(lo[j / 2] >> (j & 1) * 16);
-              }
-            }
-          }
-        }
+        for (int part = 0; part < BN / 32; ++part)
+          finish(q, at, target, lr, (uint32_t)at.m0 + quarter * 32, (uint32_t)at.n0 + half * (BN / 2) + 16 * part, lane,
+                 sum[part / 2] + part % 2 * 16);
       }
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
+    if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
   if (warp == 0) {
     const bool leader = elect_one();
     int s = 0;
     uint32_t ph = 1;
     bool ok = true;
-    for (uint32_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x) {
+    for (uint32_t t = first; ok && t < p.tiles; t += step) {
       const Place at = place_of<BN>(p, t);
       const Shape& q = p.s[at.shape];
-      const int plane = (int)(2 * at.z), slabs = (int)((q.k + BK - 1) / BK);
-      for (int kb = 0; kb < slabs; ++kb) {
+      const int plane = (int)(2 * at.z);
+      int end;
+      for (int kb = slabs_of(q, &end); kb < end; ++kb) {
         if (!mbar_wait(empty(s), ph, abort_flag, p.status, 701, p.wait_ns)) { ok = false; break; }
         if (leader) {
           const uint32_t stage = smem_base + s * C::kStageBytes;
@@ -457,10 +480,9 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
     int s = 0;
     uint32_t ph = 0, run = 0;
     bool ok = true;
-    for (uint32_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x) {
+    for (uint32_t t = first; ok && t < p.tiles; t += step) {
       const Place at = place_of<BN>(p, t);
       const Shape& q = p.s[at.shape];
-      const int slabs = (int)((q.k + BK - 1) / BK);
       // where the left half of a symmetric product's tile lies below the diagonal, the right half alone: 128 rows or two chunks further
       const uint32_t left_out = BN == 256 && q.kind == kSymmetric && at.m0 == at.n0 + 128 ? 128 : 0;
       const uint32_t idesc = f16_idesc(BN - left_out, q.a_mn, q.b_mn);
@@ -469,12 +491,13 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
       const Operand a_op = q.a_mn ? make_desc(0, BK * 128, 1024, 2) : make_desc(0, 16, 512, 4);
       const Operand b_op = q.b_mn ? make_desc(0, BK * 128, 1024, 2) : make_desc(0, 16, 512, 4);
       const uint32_t a_step = (q.a_mn ? 2048u : 32u) >> 4, b_step = (q.b_mn ? 2048u : 32u) >> 4;
-      for (int kb = 0; kb < slabs; ++run) {
+      int slabs;
+      for (int kb = slabs_of(q, &slabs); kb < slabs; ++run) {
         const uint32_t as = run & 1u, acc = tmem_base + as * BN + left_out;
         ok = mbar_wait(acc_empty(as), ((run >> 1) & 1u) ^ 1u, abort_flag, p.status, 702, p.wait_ns);
         if (!ok) break;
         tc_fence_after();
-        const int end = min(kb + kRun, slabs);
+        const int end = min(kb + kRun, slabs);             // of the run
         for (uint32_t more = 0; kb < end; ++kb, more = 1) {
           ok = mbar_wait(full(s), ph, abort_flag, p.status, 703, p.wait_ns);
           if (!ok) break;
@@ -501,6 +524,31 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
 
   tc_fence_before();
   __syncthreads();
+  if constexpr (SPLIT) {
+    cluster_arrive();
+    cluster_wait();
+    if (warp >= 4) {
+      const Place at = place_of<BN>(p, first);
+      const Shape& q = p.s[at.shape];
+      const Target target = target_of(p, q, at);
+      const float* const shared = reinterpret_cast<const float*>(smem_gen);
+      // pieces of 32 rows and 16 columns: those of a block of 32 x 32 need not be written by one warp, as each writes its own columns
+      for (uint32_t piece = rank * kEpilogueWarps + warp - 4; piece < 4 * BN / 16; piece += splits * kEpilogueWarps) {
+        const uint32_t quarter = piece & 3, c = piece / 4 * 16;
+        uint32_t v[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = 0;
+        for (uint32_t r = 0; r < splits; ++r)
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            v[j] = __float_as_uint(__uint_as_float(v[j]) + ld_cluster(shared + (c + j) * BM + quarter * 32 + lane, r));
+        finish(q, at, target, lr, (uint32_t)at.m0 + quarter * 32, (uint32_t)at.n0 + c, lane, v);
+      }
+    }
+    __syncthreads();
+    cluster_arrive();                                      // (no CTA leaves while another one reads its shared memory)
+    cluster_wait();
+  }
   if (*abort_flag) {
     // let copies and products in flight finish before the tensor memory goes away
     const long long t0 = clock64();
@@ -663,11 +711,47 @@ std::vector<Operation> operations_of(const Kin& k, const polar_b200_muon_options
   return ops;
 }
 
+// How a launch's products are computed: in tiles of 128 x bn, of which a cluster of `splits` CTAs has one (1: a CTA at a time).
+struct Way {
+  uint32_t bn, splits;
+};
+uint64_t tiles_of(uint64_t m, uint64_t n, bool symmetric, uint64_t bn) {
+  const uint64_t tiles_m = (m + BM - 1) / BM, tiles_n = (n + bn - 1) / bn;
+  if (!symmetric) return tiles_m * tiles_n;
+  uint64_t tiles = 0;
+  for (uint64_t i = 0; i < tiles_m; ++i) tiles += tiles_n - i * BM / bn;
+  return tiles;
+}
+struct Extent {
+  uint64_t m, n, k, count;
+  bool symmetric;
+};
+// The way whose busiest SM is done first.  A slab takes 0.42 us with tiles of 256 columns and 0.25 with tiles of 128, what stands around a tile 5 and 4 us (and with
+// a cluster, which adds its sums, 1.5 more).  Clusters of four or eight leave some SMs out.
+Way way_of(const std::vector<Extent>& e) {
+  Way best = {256, 1};
+  double least = 0;
+  for (const Way w : {Way{256, 1}, Way{128, 1}, Way{128, 2}, Way{128, 4}, Way{128, 8}}) {
+    const uint64_t sms = w.splits == 1 ? (uint64_t)sm_count() : w.splits == 2 ? 146 : w.splits == 4 ? 136 : 128;
+    const double slab = w.bn == 256 ? 0.42 : 0.25, around = w.bn == 256 ? 5.0 : w.splits == 1 ? 4.0 : 5.5;
+    double us = 0;
+    uint64_t before = 0, next = 0;                         // tiles passed, and the next one of the first SM
+    for (const Extent& x : e) {
+      const uint64_t units = tiles_of(x.m, x.n, x.symmetric, w.bn) * x.count * w.splits, slabs = (x.k + BK - 1) / BK;
+      const double each = (double)((slabs + w.splits - 1) / w.splits) * slab + around;
+      for (before += units; next < before; next += sms) us += each;
+    }
+    if (least == 0 || us < least) least = us, best = w;
+  }
+  return best;
+}
+
 // The next operation of every shape, longest sums first.
-template <int BN>
+template <int BN, bool SPLIT>
 int launch_product(const std::vector<Kin>& kin, const std::vector<std::pair<size_t, Operation>>& ops, const std::vector<int>& from_x, const polar_b200_muon_options& o,
-                   const Target* targets, int* status, cudaStream_t st) {
+                   const Target* targets, int* status, cudaStream_t st, uint32_t splits) {
   static thread_local Product p;
+  p.splits = splits;
   p.lr = o.lr, p.schedule = o.schedule, p.targets = targets, p.status = status, p.wait_ns = wait_limit_ns(2000000000ull);
   for (size_t k = 0; k < ops.size();) {
     p.shapes = p.tiles = 0;
@@ -707,25 +791,27 @@ int launch_product(const std::vector<Kin>& kin, const std::vector<std::pair<size
       s.plane = square ? q.side * q.side_pitch : q.rows * q.pitch;
       s.first_target = (uint32_t)q.first;
       s.tiles_m = (s.m + BM - 1) / BM, s.tiles_n = (s.n + BN - 1) / BN;
-      s.tiles = 0;
-      for (uint32_t i = 0; i < s.tiles_m; ++i) s.tiles += s.tiles_n - (square ? i * BM / BN : 0);
+      s.tiles = (uint32_t)tiles_of(s.m, s.n, square, BN);
       s.first_tile = p.tiles;
       p.tiles += s.tiles * (uint32_t)q.count;
       ++p.shapes;
     }
     cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(std::min(p.tiles, (uint32_t)sm_count()));
+    c.gridDim = dim3(SPLIT ? p.tiles * splits : std::min(p.tiles, (uint32_t)sm_count()));
     c.blockDim = dim3(kProductThreads);
     c.dynamicSmemBytes = Cfg<BN>::kSmemBytes;
     c.stream = st;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = splits;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     c.attrs = at;
-    c.numAttrs = 1;
-    cudaError_t e = cudaFuncSetAttribute(product_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<BN>::kSmemBytes);
+    c.numAttrs = SPLIT ? 2 : 1;
+    cudaError_t e = cudaFuncSetAttribute(product_kernel<BN, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<BN>::kSmemBytes);
     void* args[1] = {&p};
-    if (e == cudaSuccess) e = cudaLaunchKernelExC(&c, reinterpret_cast<const void*>(product_kernel<BN>), args);
+    if (e == cudaSuccess) e = cudaLaunchKernelExC(&c, reinterpret_cast<const void*>(product_kernel<BN, SPLIT>), args);
     if (e != cudaSuccess) {
       cudaGetLastError();
       return fail(POLAR_B200_ERR_CUDA, "fmuon: product", e);
@@ -785,7 +871,16 @@ int run_group(const std::vector<One>& all, size_t from, size_t to, const polar_b
       return a.second.what == Operation::kGram ? std::max(kin[a.first].rows, kin[a.first].cols) : kin[a.first].side;
     };
     std::stable_sort(now.begin(), now.end(), [&](const auto& a, const auto& b) { return sum(a) > sum(b); });
-    rc = launch_product<256>(kin, now, from_x, o, targets, status, st);
+    std::vector<Extent> extents;
+    for (const auto& a : now) {
+      const Kin& q = kin[a.first];
+      const bool square = a.second.what != Operation::kMove;
+      extents.push_back(Extent{square ? q.side : q.rows, square ? q.side : q.cols, sum(a), q.count, square});
+    }
+    const Way way = way_of(extents);
+    rc = way.splits > 1 ? launch_product<128, true>(kin, now, from_x, o, targets, status, st, way.splits)
+         : way.bn == 128 ? launch_product<128, false>(kin, now, from_x, o, targets, status, st, 1)
+                         : launch_product<256, false>(kin, now, from_x, o, targets, status, st, 1);
     if (rc) return rc;
     for (const auto& a : now) from_x[a.first] ^= a.second.what == Operation::kMove;
   }
