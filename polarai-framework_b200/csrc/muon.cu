@@ -561,6 +561,266 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
   }
 }
 
+// ---- small matrices: a whole step by one CTA for each
+
+// Its X lies in shared memory as pairs all the while, the shorter side's rows behind one another: 64 or 128 rows, in chunks of 64 columns and the 128-byte
+// swizzle, which is a K-major operand for X X^T and an MN-major one for P X.  Tall matrices are turned over on the way in and out.  The products are 0.2
+// to 0.8 us each; what stands between them - the sums out of tensor memory, the pairs into shared memory, a barrier - is as much.
+struct Small {
+  float* weights;
+  const float* gradient;
+  float* momentum;
+  uint32_t rows, cols;
+  float decay, scale;
+};
+template <int N>
+struct SmallTable {
+  float lr, momentum, a, b, c;
+  int nesterov;
+  uint32_t steps;
+  const float* schedule;
+  int* status;
+  unsigned long long wait_ns;
+  Small m[N];
+};
+constexpr int kFewSmall = 64, kManySmall = 800;
+static_assert(sizeof(SmallTable<kManySmall>) <= 32764, "kernel parameters");
+constexpr int kSmallThreads = 512, kSmallEach = 64;        // elements of a thread at most
+constexpr uint32_t kSmallX = 128 * 1024, kSmallP = 64 * 1024;
+// (an operand of 128 rows may reach 64 rows past the end of what lies there: those rows of the result are not read)
+constexpr uint32_t kSmallBytes = kSmallX + kSmallP + 16 * 1024 + 1024 + 256;
+__host__ __device__ constexpr bool is_small(uint64_t rows, uint64_t cols) {
+  const uint64_t side = rows < cols ? rows : cols, other = rows < cols ? cols : rows;
+  return (side <= 128 && other <= 256) || (side <= 64 && other <= 512);
+}
+
+template <int N>
+__global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_constant__ SmallTable<N> t) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ double slots[kSmallThreads / 32];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* const smem = smem_raw + (smem_base - smem_u32(smem_raw));
+  const uint32_t bar = smem_base + kSmallBytes - 1024 - 256;
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + kSmallBytes - 1024 - 256 + 8);
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = uniform_warp(), lane = threadIdx.x & 31;
+  const Small& m = t.m[blockIdx.x];
+  const bool tall = m.rows > m.cols;
+  const uint32_t side = tall ? m.cols : m.rows, length = tall ? m.rows : m.cols;
+  const uint32_t height = side <= 64 ? 64 : 128;           // rows that are held
+  const uint32_t chunk = height * 128;                     // bytes of a chunk of 64 columns
+  const uint32_t x_plane = (length + 63) / 64 * chunk, p_plane = (side + 63) / 64 * chunk;
+  if (threadIdx.x == 0) {
+    mbar_init(bar, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  // zeros behind the last row and column: they are part of sums
+  for (uint32_t i = threadIdx.x; i < (kSmallX + kSmallP) / 16; i += kSmallThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  pdl_enter();
+
+  // the momentum, u and its size
+  const uint32_t count = m.rows * m.cols;
+  float u[kSmallEach];
+  double sum = 0;
+#pragma unroll
+  for (int i = 0; i < kSmallEach; ++i) {
+    const uint32_t e = i * kSmallThreads + threadIdx.x;
+    u[i] = 0.f;
+    if (i * kSmallThreads < count && e < count) {
+      const float g = m.gradient[e], v = fmaf(t.momentum, m.momentum[e], g);
+      m.momentum[e] = v;
+      u[i] = t.nesterov ? fmaf(t.momentum, v, g) : v;
+      sum += (double)u[i] * (double)u[i];
+    }
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+  if (lane == 0) slots[warp] = sum;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  sum = 0;
+#pragma unroll
+  for (int i = 0; i < kSmallThreads / 32; ++i) sum += slots[i];
+  const double by = sum == 0 ? 0 : (double)kX / sqrt(sum);
+  // where 16 bytes of a row lie
+  auto place = [&](uint32_t row, uint32_t col) { return col / 64 * chunk + row * 128 + (((col & 63) / 8 ^ (row & 7)) << 4); };
+  {
+    uint32_t row = threadIdx.x / m.cols, col = threadIdx.x - row * m.cols;
+    const uint32_t down = kSmallThreads / m.cols, right = kSmallThreads - down * m.cols;
+#pragma unroll
+    for (int i = 0; i < kSmallEach; ++i) {
+      if (i * kSmallThreads >= count) break;
+      if (row < m.rows) {
+        const uint32_t r = tall ? col : row, c = tall ? row : col;
+        __half* const x = reinterpret_cast<__half*>(smem + place(r, c)) + (c & 7);
+        split((float)((double)u[i] * by), x, x + x_plane / 2);
+      }
+      row += down, col += right;
+      if (col >= m.cols) col -= m.cols, ++row;
+    }
+  }
+
+  const int quarter = warp & 3, group = warp >> 2;
+  const uint32_t row = quarter * 32 + lane;
+  const uint32_t lane_at = tmem + ((uint32_t)(quarter * 32) << 16);
+  const bool mine = quarter * 32 < side;                   // (the whole warp)
+  const uint32_t x_at = (smem_base & 0x3FFFFu) >> 4, p_at = x_at + (kSmallX >> 4);
+  const uint32_t side16 = (side + 15) / 16 * 16, length16 = (length + 15) / 16 * 16;
+  const Operand k_major = make_desc(0, 16, 1024, 2), mn_major = make_desc(0, chunk, 1024, 2);
+  uint32_t phase = 0;
+  // Products of the whole CTA's operands in shared memory: issued by one thread, waited for by all.
+  auto multiplied = [&](auto issue) {
+    fence_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag) return false;
+    if (warp == 0) {
+      tc_fence_after();
+      if (elect_one()) {
+        issue();
+        tc_commit(bar);
+      }
+      __syncwarp();
+    }
+    mbar_wait(bar, phase, abort_flag, t.status, 711, t.wait_ns);
+    phase ^= 1;
+    tc_fence_after();
+    return true;
+  };
+  auto three = [&](uint32_t acc, Operand a, uint32_t a_hi, uint32_t a_lo, Operand b, uint32_t b_hi, uint32_t b_lo, uint32_t idesc, uint32_t more) {
+    tc_mma_f16(acc, a, a_hi, b, b_hi, idesc, more);
+    tc_mma_f16(acc, a, a_lo, b, b_hi, idesc, 1u);
+    tc_mma_f16(acc, a, a_hi, b, b_lo, idesc, 1u);
+  };
+  auto k_offset = [&](uint32_t k16) { return (k16 / 4 * chunk + k16 % 4 * 32) >> 4; };
+  // 16 columns of this thread's row as pairs
+  auto keep = [&](uint32_t at, uint32_t plane, uint32_t col, const float* v) {
+    union { __half h[16]; uint4 bits[2]; } hi, lo;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) split(v[j], &hi.h[j], &lo.h[j]);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint8_t* const x = smem + at + place(row, col + 8 * j);
+      *reinterpret_cast<uint4*>(x) = hi.bits[j];
+      *reinterpret_cast<uint4*>(x + plane) = lo.bits[j];
+    }
+  };
+
+  for (uint32_t step = 0; step < t.steps; ++step) {
+    // G = X X^T; every 128 k in an accumulator of its own, as in the product kernel
+    if (!multiplied([&] {
+          for (uint32_t k = 0; k < length16 / 16; ++k) {
+            const uint32_t at = x_at + k_offset(k);
+            three(tmem + k / 8 * 128, k_major, at, at + (x_plane >> 4), k_major, at, at + (x_plane >> 4), f16_idesc((int)side16, 0, 0), k % 8 ? 1u : 0u);
+          }
+        }))
+      break;
+    float g[32];
+    if (mine && (uint32_t)group * 32 < side16) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) g[j] = 0.f;
+      for (uint32_t run = 0; run < (length16 + 127) / 128; ++run) {
+        uint32_t v[32];
+        tmem_ld_32x32(lane_at + run * 128 + group * 32, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) g[j] += __uint_as_float(v[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 32; ++j) g[j] = group * 32 + j < side ? g[j] * (kG / (kX * kX)) : 0.f;
+      if (row < side) keep(kSmallX, p_plane, group * 32, g), keep(kSmallX, p_plane, group * 32 + 16, g + 16);
+    }
+    // P = a + b G + c G G, in the place of G
+    if (!multiplied([&] {
+          for (uint32_t k = 0; k < side16 / 16; ++k) {
+            const uint32_t at = p_at + k_offset(k);
+            three(tmem, k_major, at, at + (p_plane >> 4), k_major, at, at + (p_plane >> 4), f16_idesc((int)side16, 0, 0), k ? 1u : 0u);
+          }
+        }))
+      break;
+    if (mine && (uint32_t)group * 32 < side16) {
+      uint32_t v[32];
+      tmem_ld_32x32(lane_at + group * 32, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const uint32_t col = group * 32 + j;
+        g[j] = fmaf(t.c * (kP / (kG * kG)), __uint_as_float(v[j]), t.b * (kP / kG) * g[j]) + (col == row ? t.a * kP : 0.f);
+        if (col >= side) g[j] = 0.f;
+      }
+      if (row < side) keep(kSmallX, p_plane, group * 32, g), keep(kSmallX, p_plane, group * 32 + 16, g + 16);
+    }
+    // P X
+    if (!multiplied([&] {
+          for (uint32_t from = 0; from < length16; from += 256) {
+            const uint32_t n = min(length16 - from, 256u), b_at = x_at + (from / 64 * chunk >> 4);
+            for (uint32_t k = 0; k < side16 / 16; ++k) {
+              const uint32_t a_at = p_at + k_offset(k), b = b_at + (k * 2048 >> 4);
+              three(tmem + from, k_major, a_at, a_at + (p_plane >> 4), mn_major, b, b + (x_plane >> 4), f16_idesc((int)n, 0, 1), k ? 1u : 0u);
+            }
+          }
+        }))
+      break;
+    if (!mine) continue;
+    const bool last = step + 1 == t.steps;
+    const float lr = t.schedule ? t.schedule[1] : t.lr, kept = 1.f - lr * m.decay, rate = lr * m.scale / (kP * kX);
+    for (uint32_t col = group * 16; col < length16; col += 64) {
+      uint32_t v[16];
+      __syncwarp();
+      tmem_ld_32x16(lane_at + col, v);
+      tmem_ld_wait();
+      if (row >= side) continue;
+      float x[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = __uint_as_float(v[j]) * (last ? rate : 1.f / kP);
+      if (!last) {
+        // (behind the last column X is zeros, and so are these)
+        keep(0, x_plane, col, x);
+      } else if (tall) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (col + j < length) {
+            float* const w = m.weights + (uint64_t)(col + j) * m.cols + row;
+            *w = *w * kept - x[j];
+          }
+      } else {
+        float* const w = m.weights + (uint64_t)row * m.cols + col;
+        if ((m.cols & 3) == 0 && (reinterpret_cast<uintptr_t>(m.weights) & 15) == 0 && col + 16 <= length) {
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) {
+            float4 o = *reinterpret_cast<const float4*>(w + j);
+            o.x = o.x * kept - x[j], o.y = o.y * kept - x[j + 1], o.z = o.z * kept - x[j + 2], o.w = o.w * kept - x[j + 3];
+            *reinterpret_cast<float4*>(w + j) = o;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (col + j < length) w[j] = w[j] * kept - x[j];
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000ll) { }
+    __syncthreads();
+  }
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
 // ---- host side
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -821,7 +1081,7 @@ int launch_product(const std::vector<Kin>& kin, const std::vector<std::pair<size
   return POLAR_B200_OK;
 }
 
-// The matrices of the call, longest sums first, and the groups they are done in.
+// The matrices of the call, longest sums first, and the groups they are done in; behind the last group's end the small ones.
 void matrices_of(const polar_b200_muon_tensor* tensors, uint64_t count, std::vector<One>* all, std::vector<size_t>* ends) {
   for (uint64_t i = 0; i < count; ++i) {
     const polar_b200_muon_tensor& t = tensors[i];
@@ -831,16 +1091,54 @@ void matrices_of(const polar_b200_muon_tensor* tensors, uint64_t count, std::vec
     }
   }
   std::stable_sort(all->begin(), all->end(), [](const One& a, const One& b) {
+    const bool sa = is_small(a.rows, a.cols), sb = is_small(b.rows, b.cols);
     const uint64_t la = std::max(a.rows, a.cols), lb = std::max(b.rows, b.cols);
-    return la != lb ? la > lb : a.rows != b.rows ? a.rows > b.rows : a.cols > b.cols;
+    return sa != sb ? sb : la != lb ? la > lb : a.rows != b.rows ? a.rows > b.rows : a.cols > b.cols;
   });
   uint64_t bytes = 0;
-  for (size_t i = 0; i < all->size(); ++i) {
+  size_t large = all->size();
+  while (large && is_small((*all)[large - 1].rows, (*all)[large - 1].cols)) --large;
+  for (size_t i = 0; i < large; ++i) {
     const uint64_t more = bytes_of((*all)[i].rows, (*all)[i].cols);
     if (bytes && bytes + more > kGroupBytes) ends->push_back(i), bytes = 0;
     bytes += more;
   }
-  if (!all->empty()) ends->push_back(all->size());
+  if (large) ends->push_back(large);
+}
+
+template <int N>
+int launch_small(const std::vector<One>& all, size_t from, size_t to, const polar_b200_muon_options& o, int* status, cudaStream_t st) {
+  static thread_local SmallTable<N> t;
+  t.lr = o.lr, t.momentum = o.momentum, t.a = o.a, t.b = o.b, t.c = o.c, t.nesterov = o.nesterov, t.steps = o.steps, t.schedule = o.schedule;
+  t.status = status, t.wait_ns = wait_limit_ns(2000000000ull);
+  cudaError_t e = cudaFuncSetAttribute(small_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmallBytes);
+  if (e != cudaSuccess) return fail(POLAR_B200_ERR_CUDA, "fmuon: small matrices", e);
+  while (from < to) {
+    const size_t n = std::min<size_t>(to - from, N);
+    for (size_t i = 0; i < n; ++i) {
+      const One& q = all[from + i];
+      t.m[i] = Small{q.weights, q.gradient, q.momentum, (uint32_t)q.rows, (uint32_t)q.cols, q.decay, q.scale};
+    }
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3((unsigned)n);
+    c.blockDim = dim3(kSmallThreads);
+    c.dynamicSmemBytes = kSmallBytes;
+    c.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = at;
+    c.numAttrs = 1;
+    void* args[1] = {&t};
+    e = cudaLaunchKernelExC(&c, reinterpret_cast<const void*>(small_kernel<N>), args);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return fail(POLAR_B200_ERR_CUDA, "fmuon: small matrices", e);
+    }
+    count_launch();
+    from += n;
+  }
+  return POLAR_B200_OK;
 }
 
 int run_group(const std::vector<One>& all, size_t from, size_t to, const polar_b200_muon_options& o, char* base, cudaStream_t st) {
@@ -1016,7 +1314,7 @@ int polar_b200_fmuon(const polar_b200_muon_tensor* tensors, uint64_t count, cons
     LaunchDeviceScope on(stream, some);
     cudaStream_t st = as_stream(stream);
     void* own = nullptr;
-    if (!workspace) {
+    if (!workspace && need) {
       cudaError_t e = scratch_alloc(&own, need, st);
       if (e != cudaSuccess) return fail(POLAR_B200_ERR_CUDA, "scratch (workspace)", e);
     }
@@ -1026,6 +1324,11 @@ int polar_b200_fmuon(const polar_b200_muon_tensor* tensors, uint64_t count, cons
       rc = run_group(all, from, to, *o, static_cast<char*>(workspace ? workspace : own), st);
       if (rc) break;
       from = to;
+    }
+    if (rc == POLAR_B200_OK && from < all.size()) {
+      int* status = device_status_word(&rc);
+      if (!rc) rc = all.size() - from <= kFewSmall ? launch_small<kFewSmall>(all, from, all.size(), *o, status, st)
+                                                   : launch_small<kManySmall>(all, from, all.size(), *o, status, st);
     }
     if (own) {
       cudaError_t e = scratch_free(own, st);

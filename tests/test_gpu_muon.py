@@ -81,7 +81,9 @@ def step(d, ts, lr=0.5, **k):
 
 SHAPES = [(1, 1), (1, 2), (2, 1), (1, 1000), (1000, 1), (3, 5), (5, 3), (16, 16), (31, 33), (33, 31), (63, 65), (64, 64), (64, 128), (128, 64), (127, 129), (128, 128),
           (129, 127), (128, 1000), (1000, 128), (130, 70), (70, 130), (255, 257), (256, 256), (257, 255), (300, 1000), (1000, 300), (384, 640), (640, 384), (513, 511), (10, 4096),
-          (4096, 10), (777, 1511), (1511, 777), (1024, 1024), (65, 5000), (5000, 65), (1280, 128), (2048, 512)]
+          (4096, 10), (777, 1511), (1511, 777), (1024, 1024), (65, 5000), (5000, 65), (1280, 128), (2048, 512),
+          # what one CTA does alone ends at 128 x 256 and 64 x 512
+          (128, 256), (256, 128), (128, 257), (257, 128), (129, 256), (64, 512), (512, 64), (64, 513), (65, 512), (65, 256), (512, 1), (1, 512), (17, 511), (100, 241)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
@@ -137,6 +139,9 @@ def test_several_shapes_stacks_and_lists_of_options(d):
 
 def test_more_shapes_than_a_launch_holds_and_more_matrices_than_a_table(d):
     ts = [make((20 + i, 300 + 3 * i), i) for i in range(19)]
+    for (nw, nm), t in zip(step(d, ts), ts):
+        check(nw, nm, *t)
+    ts = [make((130 + i, 300 + 3 * i), i) for i in range(19)]
     for (nw, nm), t in zip(step(d, ts), ts):
         check(nw, nm, *t)
     ts = [make((8 + i % 3, 12), i) for i in range(850)]
