@@ -283,9 +283,12 @@ __device__ __forceinline__ void finish(const Shape& q, const Place& at, const Ta
         *reinterpret_cast<float4*>(w + j) = x;
       }
     } else {
+      float x[16];                                         // (all loads before the first store, which might change what they read)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = c0 + j < q.n ? w[j] : 0.f;
 #pragma unroll
       for (int j = 0; j < 16; ++j)
-        if (c0 + j < q.n) w[j] = w[j] * keep - rate * __uint_as_float(v[j]);
+        if (c0 + j < q.n) w[j] = x[j] * keep - rate * __uint_as_float(v[j]);
     }
     return;
   }
@@ -628,14 +631,21 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
   float u[kSmallEach];
   double sum = 0;
 #pragma unroll
-  for (int i = 0; i < kSmallEach; ++i) {
-    const uint32_t e = i * kSmallThreads + threadIdx.x;
-    u[i] = 0.f;
-    if (i * kSmallThreads < count && e < count) {
-      const float g = m.gradient[e], v = fmaf(t.momentum, m.momentum[e], g);
-      m.momentum[e] = v;
-      u[i] = t.nesterov ? fmaf(t.momentum, v, g) : v;
-      sum += (double)u[i] * (double)u[i];
+  for (int from = 0; from < kSmallEach; from += 8) {        // eight elements' loads on their way
+    if (from * kSmallThreads >= count) break;
+    float g[8], v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t e = (from + i) * kSmallThreads + threadIdx.x;
+      g[i] = e < count ? m.gradient[e] : 0.f, v[i] = e < count ? m.momentum[e] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t e = (from + i) * kSmallThreads + threadIdx.x;
+      v[i] = fmaf(t.momentum, v[i], g[i]);
+      if (e < count) m.momentum[e] = v[i];
+      u[from + i] = t.nesterov ? fmaf(t.momentum, v[i], g[i]) : v[i];
+      sum += (double)u[from + i] * (double)u[from + i];
     }
   }
 #pragma unroll
@@ -675,7 +685,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
   const uint32_t side16 = (side + 15) / 16 * 16, length16 = (length + 15) / 16 * 16;
   const Operand k_major = make_desc(0, 16, 1024, 2), mn_major = make_desc(0, chunk, 1024, 2);
   uint32_t phase = 0;
-  // Products of the whole CTA's operands in shared memory: issued by one thread, waited for by all.
+  // Products of the whole CTA's operands in shared memory: issued by one lane of a warp that runs its loops as a whole, waited for by all.
+  const bool leader = elect_one();
   auto multiplied = [&](auto issue) {
     fence_async_smem();
     tc_fence_before();
@@ -683,10 +694,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
     if (*abort_flag) return false;
     if (warp == 0) {
       tc_fence_after();
-      if (elect_one()) {
-        issue();
-        tc_commit(bar);
-      }
+      issue();
+      if (leader) tc_commit(bar);
       __syncwarp();
     }
     mbar_wait(bar, phase, abort_flag, t.status, 711, t.wait_ns);
@@ -695,6 +704,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
     return true;
   };
   auto three = [&](uint32_t acc, Operand a, uint32_t a_hi, uint32_t a_lo, Operand b, uint32_t b_hi, uint32_t b_lo, uint32_t idesc, uint32_t more) {
+    if (!leader) return;
     tc_mma_f16(acc, a, a_hi, b, b_hi, idesc, more);
     tc_mma_f16(acc, a, a_lo, b, b_hi, idesc, 1u);
     tc_mma_f16(acc, a, a_hi, b, b_lo, idesc, 1u);
@@ -783,16 +793,10 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
       if (!last) {
         // (behind the last column X is zeros, and so are these)
         keep(0, x_plane, col, x);
-      } else if (tall) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (col + j < length) {
-            float* const w = m.weights + (uint64_t)(col + j) * m.cols + row;
-            *w = *w * kept - x[j];
-          }
       } else {
-        float* const w = m.weights + (uint64_t)row * m.cols + col;
-        if ((m.cols & 3) == 0 && (reinterpret_cast<uintptr_t>(m.weights) & 15) == 0 && col + 16 <= length) {
+        float* const w = m.weights + (tall ? col * m.cols + row : row * m.cols + col);
+        const uint32_t next = tall ? m.cols : 1;
+        if (!tall && (m.cols & 3) == 0 && (reinterpret_cast<uintptr_t>(m.weights) & 15) == 0 && col + 16 <= length) {
 #pragma unroll
           for (int j = 0; j < 16; j += 4) {
             float4 o = *reinterpret_cast<const float4*>(w + j);
@@ -800,9 +804,12 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
             *reinterpret_cast<float4*>(w + j) = o;
           }
         } else {
+          float o[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[j] = col + j < length ? w[j * next] : 0.f;
 #pragma unroll
           for (int j = 0; j < 16; ++j)
-            if (col + j < length) w[j] = w[j] * kept - x[j];
+            if (col + j < length) w[j * next] = o[j] * kept - x[j];
         }
       }
     }
@@ -909,6 +916,19 @@ uint64_t lay_out(char* base, const std::vector<One>& all, size_t from, size_t to
     for (int b = 0; b < (in_pairs(k.rows, k.cols) ? 3 : 2); ++b) k.s[b] = reinterpret_cast<__half*>(take(k.count * 4 * k.side * k.side_pitch));
   }
   return at;
+}
+
+uint64_t workspace_of(const std::vector<One>& all, const std::vector<size_t>& ends) {
+  uint64_t most = 0;
+  size_t from = 0;
+  for (size_t to : ends) {
+    std::vector<Kin> kin;
+    double* partial;
+    Target* targets;
+    most = std::max(most, lay_out(nullptr, all, from, to, &kin, &partial, &targets));
+    from = to;
+  }
+  return most;
 }
 
 template <int N>
@@ -1082,9 +1102,11 @@ int launch_product(const std::vector<Kin>& kin, const std::vector<std::pair<size
 }
 
 // The matrices of the call, longest sums first, and the groups they are done in; behind the last group's end the small ones.
-void matrices_of(const polar_b200_muon_tensor* tensors, uint64_t count, std::vector<One>* all, std::vector<size_t>* ends) {
+void matrices_of(const polar_b200_muon_tensor* tensors, uint64_t count, std::vector<One>* all, std::vector<size_t>* ends, bool large_only) {
+  all->reserve(count);
   for (uint64_t i = 0; i < count; ++i) {
     const polar_b200_muon_tensor& t = tensors[i];
+    if (large_only && is_small(t.rows, t.cols)) continue;
     for (uint64_t z = 0; z < t.matrices && t.rows && t.cols; ++z) {
       const uint64_t at = z * t.rows * t.cols;
       all->push_back(One{t.weights + at, t.gradient + at, t.momentum + at, t.rows, t.cols, t.weight_decay, t.scale});
@@ -1271,17 +1293,8 @@ uint64_t polar_b200_fmuon_workspace_bytes(const polar_b200_muon_tensor* tensors,
   try {
     std::vector<One> all;
     std::vector<size_t> ends;
-    matrices_of(tensors, count, &all, &ends);
-    uint64_t most = 0;
-    size_t from = 0;
-    for (size_t to : ends) {
-      std::vector<Kin> kin;
-      double* partial;
-      Target* targets;
-      most = std::max(most, lay_out(nullptr, all, from, to, &kin, &partial, &targets));
-      from = to;
-    }
-    return most;
+    matrices_of(tensors, count, &all, &ends, true);
+    return workspace_of(all, ends);
   } catch (const std::exception&) {
     return 0;
   }
@@ -1305,12 +1318,12 @@ int polar_b200_fmuon(const polar_b200_muon_tensor* tensors, uint64_t count, cons
   if (!some) return POLAR_B200_OK;
   try {
     if (!muon_independent(tensors, count, o->schedule)) return fail(POLAR_B200_ERR_INVALID, "fmuon: what is written overlaps something else");
-    const uint64_t need = polar_b200_fmuon_workspace_bytes(tensors, count);
-    if (workspace && (workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
-      return fail(POLAR_B200_ERR_WORKSPACE, "workspace too small or not 256-byte aligned");
     std::vector<One> all;
     std::vector<size_t> ends;
-    matrices_of(tensors, count, &all, &ends);
+    matrices_of(tensors, count, &all, &ends, false);
+    const uint64_t need = workspace_of(all, ends);
+    if (workspace && (workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
+      return fail(POLAR_B200_ERR_WORKSPACE, "workspace too small or not 256-byte aligned");
     LaunchDeviceScope on(stream, some);
     cudaStream_t st = as_stream(stream);
     void* own = nullptr;

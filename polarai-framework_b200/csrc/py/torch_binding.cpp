@@ -21,6 +21,7 @@
 #include <polar_b200.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <exception>
 #include <vector>
@@ -351,14 +352,35 @@ BUILTIN(fadamw) {
   return launched(polar_b200_fadamw, tensors.data(), (uint64_t)count, &o, c.stream());
 }
 
-// fmuon(weights, gradients, momenta, lr, momentum, nesterov, steps, weight decays, scales, a, b, c, schedule or None): lists of tensors, one decay and
-// one scale for each.  Its workspace comes from torch's allocator, which keeps it: it is too large for the library's own pool to.
+// A number for every element of a list, or a list of them.
+struct Numbers {
+  explicit Numbers(PyObject* o) : list(PyFloat_Check(o) || PyLong_Check(o) ? Py_None : o), one(list.list || o == Py_None ? 0.0 : PyFloat_AsDouble(o)) {
+    if (PyErr_Occurred()) PyErr_Clear(), bad = true;
+  }
+  bool fits(Py_ssize_t count) const { return !bad && (!list.list || list.size() == count); }
+  bool at(Py_ssize_t i, float* v) const {
+    const double d = list.list ? PyFloat_AsDouble(list[i]) : one;
+    if (d == -1.0 && PyErr_Occurred()) {
+      PyErr_Clear();
+      return false;
+    }
+    *v = (float)d;
+    return true;
+  }
+  Sequence list;
+  double one;
+  bool bad = false;
+};
+// fmuon(weights, gradients, momenta, lr, momentum, nesterov, steps, weight decay or decays, scale or scales or None, a, b, c, schedule or None): lists of
+// tensors; no scale: the root of rows / cols where that is above 1.  Its workspace comes from torch's allocator, which keeps it: it is too large for the library's own pool to.
 BUILTIN(fmuon) {
   Call c(args, n, 13);
   if (!c.ok()) return answer(false);
-  const Sequence w(args[0]), g(args[1]), m(args[2]), decays(args[7]), scales(args[8]);
+  const Sequence w(args[0]), g(args[1]), m(args[2]);
+  const Numbers decays(args[7]), scales(args[8]);
+  const bool by_shape = args[8] == Py_None;
   const Py_ssize_t count = w.size();
-  if (count < 0 || g.size() != count || m.size() != count || decays.size() != count || scales.size() != count) return answer(false);
+  if (count < 0 || g.size() != count || m.size() != count || args[7] == Py_None || !decays.fits(count) || !scales.fits(count)) return answer(false);
   polar_b200_muon_options o;
   o.lr = c.scalar(3), o.momentum = c.scalar(4), o.nesterov = c.whole(5) != 0;
   const uint64_t steps = c.whole(6);
@@ -375,12 +397,8 @@ BUILTIN(fmuon) {
     t.weights = data(wt), t.gradient = data(gt), t.momentum = data(mt);
     t.rows = (uint64_t)wt->size(-2), t.cols = (uint64_t)wt->size(-1);
     t.matrices = t.rows && t.cols ? numel(wt) / (t.rows * t.cols) : 0;
-    const double decay = PyFloat_AsDouble(decays[i]), scale = PyFloat_AsDouble(scales[i]);
-    if (PyErr_Occurred()) {
-      PyErr_Clear();
-      c.require(false);
-    }
-    t.weight_decay = (float)decay, t.scale = (float)scale;
+    c.require(decays.at(i, &t.weight_decay) && scales.at(i, &t.scale));
+    if (by_shape) t.scale = (float)std::sqrt(std::max(1.0, (double)t.rows / (double)std::max<uint64_t>(t.cols, 1)));
     some = wt;
   }
   const at::Tensor* schedule = c.tensor_or_none(12);

@@ -343,10 +343,10 @@ class DeviceBuiltins:
         """One step of orthogonalised momentum over lists of matrices - tensors [rows, cols], or [..., rows, cols] of several, each by
         itself - in place.  weight_decay and scale, by which the update is multiplied: one for all, or a list; no scale: sqrt(rows / cols) where
         that is above 1.  lr comes from the call or, for steps that are captured, from `schedule`, fadamw's device tensor of the step's number and lr."""
-        decays = [weight_decay] * len(weights) if isinstance(weight_decay, numbers.Real) else weight_decay
-        scales = ([scale] * len(weights) if isinstance(scale, numbers.Real) else scale if scale is not None else
-                  [max(1.0, w.shape[-2] / max(w.shape[-1], 1)) ** 0.5 if len(w.shape) >= 2 else 1.0 for w in weights])
-        if not self._native.fmuon(weights, gradients, momenta, lr, momentum, bool(nesterov), steps, decays, scales, *coefficients, schedule):
+        if not self._native.fmuon(weights, gradients, momenta, lr, momentum, bool(nesterov), steps, weight_decay, scale, *coefficients, schedule):
+            decays = [weight_decay] * len(weights) if isinstance(weight_decay, numbers.Real) else weight_decay
+            scales = ([scale] * len(weights) if isinstance(scale, numbers.Real) else scale if scale is not None else
+                      [max(1.0, w.shape[-2] / max(w.shape[-1], 1)) ** 0.5 if len(w.shape) >= 2 else 1.0 for w in weights])
             if any(len(x) != len(weights) for x in (gradients, momenta, decays, scales)):
                 raise ValueError("fmuon: lists of one length")
             tensors = (MuonTensor * len(weights))()

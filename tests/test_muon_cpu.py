@@ -91,7 +91,9 @@ def test_by_name_patterns(c):
         return c.polar_b200_launch_by_name(b"fmuon", arr, len(given), None, 0, None), c.polar_b200_launch_workspace_bytes(b"fmuon", arr, len(given))
 
     good = [(20, 30), (2,), 0.95, 1.0, 5.0, 0.0, 1.0, (20, 30), (20, 30)]
-    assert by_name(*good)[1] > 0
+    big = [(200, 300), (2,), 0.95, 1.0, 5.0, 0.0, 1.0, (200, 300), (200, 300)]
+    assert by_name(*big)[1] == c.polar_b200_fmuon_workspace_bytes(tensors({"rows": 200, "cols": 300}), 1) > 0
+    assert by_name(*good)[1] == 0                            # (one CTA's shared memory holds it)
     for i, bad in ((0, (20, 29)), (0, 1.0), (1, (3,)), (3, 0.5), (4, 0.0), (4, 2.5), (4, 33.0), (4, math.nan), (7, (600,)), (8, (20, 31)), (2, (20, 30))):
         args = list(good)
         args[i] = bad
