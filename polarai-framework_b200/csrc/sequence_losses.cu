@@ -25,6 +25,19 @@ constexpr int kFewThreads = 1024, kFewEach = kFew / kFewThreads;
 
 // ---- sequences
 
+// An id, loaded where the call stands: left to itself the compiler moves loads down to the votes that need them, one round trip after another.
+__device__ __forceinline__ float ld_id(const float* p) { return ld_stream(p); }
+__device__ __forceinline__ int32_t ld_id(const int32_t* p) {
+  int32_t v;
+  asm volatile("ld.global.cs.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ int64_t ld_id(const int64_t* p) {
+  int64_t v;
+  asm volatile("ld.global.cs.s64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
+  return v;
+}
+
 template <class Id>
 struct Packed {
   const Id *ids, *offsets;
@@ -37,7 +50,6 @@ struct Packed {
     if constexpr (std::is_floating_point<Id>::value) return v >= (float)tokens ? tokens : (uint64_t)v;   // (exact: tokens up to 2^24)
     else return min((uint64_t)v, tokens);
   }
-  __device__ __forceinline__ bool counts(uint64_t t) const { return !(ids[t] < Id(0)); }
 };
 
 // The last sequence that begins at or before token t, found by a whole warp: 32 of what is left are looked at together.
@@ -112,12 +124,12 @@ Workspace lay_out(void* base, uint64_t tokens, uint64_t sequences, bool pairs, u
   w.bits = reinterpret_cast<uint32_t*>(take(tiles * kWords * 4));
   w.share = reinterpret_cast<float*>(take(sequences * 4));
   if (pairs) {
-    w.partial = reinterpret_cast<float4*>(take((sequences / 2 + kThreads / 32 - 1) / (kThreads / 32) * sizeof(float4)));
+    w.partial = reinterpret_cast<float4*>(take((sequences + kThreads / 32 - 1) / (kThreads / 32) * sizeof(float4)));
     w.whole = reinterpret_cast<double*>(take(sequences * 8));
     w.head = reinterpret_cast<double*>(take(tiles * 8));
     w.tail = reinterpret_cast<double*>(take(tiles * 8));
   } else {
-    w.partial = reinterpret_cast<float4*>(take((tokens + kPass - 1) / kPass * sizeof(float4)));
+    w.partial = reinterpret_cast<float4*>(take((tokens + kThreads * 4 - 1) / (kThreads * 4) * sizeof(float4)));
   }
   *bytes = at;
   return w;
@@ -179,10 +191,13 @@ __global__ void __launch_bounds__(kThreads) mark_kernel(Packed<Id> p, Workspace 
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint64_t base = (uint64_t)blockIdx.x * kTile + warp * (kTile / 8);
   uint32_t mine = 0;
+  Id ids[16];                                              // (all loads on their way before the first vote, and none behind a branch)
+#pragma unroll
+  for (int j = 0; j < 16; ++j) ids[j] = ld_id(p.ids + min(base + 32 * j + lane, p.tokens - 1));
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     const uint64_t t = base + 32 * j + lane;
-    const uint32_t b = __ballot_sync(0xffffffffu, t < p.tokens && p.counts(t) && t >= begin && t < end);
+    const uint32_t b = __ballot_sync(0xffffffffu, !(ids[j] < Id(0)) && t >= begin && t < end);
     if (lane == j) mine = b;
   }
   if (lane < 16) w.bits[base / 32 + lane] = mine;
@@ -268,6 +283,7 @@ struct Policy {
   float *loss, *g_logprob, *g_entropy;
   float high, low;                                         // what the ratio is clipped to
   double log_high, log_low;
+  float near_high, near_low;                               // how far from these borders fp32 decides
   float kl, bonus, count;
   int by_sequence, per_token;
 };
@@ -291,12 +307,17 @@ struct Term {
   float surrogate, kl, clipped, slope;
 };
 // A token that counts.  On which side of the clipping border it lies is decided by the difference of the logarithms in 64 bits, where it is
-// exact: in fp32 rounding would decide for tokens on the border.
+// exact: in fp32 rounding would decide for tokens on the border.  Away from the border both agree, and fp32 is asked, which is
+// three conversions and a sum in 64 bits less.
 __device__ __forceinline__ Term term(const Policy& o, float logprob, float old, float reference, float advantage) {
-  const double d = (double)logprob - (double)old;
-  const bool over = d > o.log_high, under = d < o.log_low;
+  const float d = logprob - old, high = (float)o.log_high, low = (float)o.log_low;
+  bool over = d > high, under = d < low;
+  if (fabsf(d - high) <= o.near_high || fabsf(d - low) <= o.near_low) {
+    const double exact = (double)logprob - (double)old;
+    over = exact > o.log_high, under = exact < o.log_low;
+  }
   const bool cut = (advantage > 0.f && over) || (advantage < 0.f && under);
-  const float free = expf((float)d) * advantage;
+  const float free = expf(d) * advantage;
   Term t;
   t.surrogate = cut ? (over ? o.high : o.low) * advantage : free;
   t.clipped = cut ? 1.f : 0.f;
@@ -316,12 +337,13 @@ __device__ __forceinline__ void write_loss(const Policy& o, const double* total)
   for (int i = 0; i < 4; ++i) o.loss[i + 1] = (float)total[i];
 }
 
-__device__ __forceinline__ float4 load4(const float* p, uint64_t t, uint64_t end, bool vectors) {
+// Four neighbours; `whole`: for all threads of the CTA a vector inside the array.  (Else no load stands behind a branch of its own either.)
+__device__ __forceinline__ float4 load4(const float* p, uint64_t t, uint64_t end, bool whole) {
   if (!p) return make_float4(0.f, 0.f, 0.f, 0.f);
-  if (vectors && t + 4 <= end) return ld_stream(reinterpret_cast<const float4*>(p + t));
+  if (whole) return ld_stream(reinterpret_cast<const float4*>(p + t));
   float4 v;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) (&v.x)[k] = t + k < end ? p[t + k] : 0.f;
+  for (int k = 0; k < 4; ++k) (&v.x)[k] = ld_stream(p + min(t + k, end - 1));
   return v;
 }
 // Of four neighbours those of [begin, end).
@@ -335,8 +357,9 @@ __device__ __forceinline__ void store4(float* p, float4 v, uint64_t t, uint64_t 
     if (t + k >= begin && t + k < end) p[t + k] = (&v.x)[k];
 }
 
-// LOOK: a token's sequence is needed.
-template <class Id, bool LOOK>
+// LOOK: a token's sequence is needed.  PARTS: of kPart tokens that a CTA has, with all their loads on their way.
+constexpr uint32_t kPart = kThreads * 4;
+template <class Id, bool LOOK, int PARTS>
 __global__ void __launch_bounds__(kThreads) policy_kernel(Packed<Id> p, Workspace w, Policy o, bool vectors) {
   __shared__ float slots[kThreads / 8];
   __shared__ double wide[kThreads / 8];
@@ -345,19 +368,20 @@ __global__ void __launch_bounds__(kThreads) policy_kernel(Packed<Id> p, Workspac
   const uint64_t begin = p.offset(0), end = p.offset(p.sequences);
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
   const float even = o.by_sequence ? (o.count > 0.f ? 1.f / o.count : 1.f / (float)w.shared->live) : w.shared->share;
-  float4 lp[2], old[2], ref[2], ent[2], adv[2];
-  uint32_t bits[2];
+  float4 lp[PARTS], old[PARTS], ref[PARTS], ent[PARTS], adv[PARTS];
+  uint32_t bits[PARTS];
+  const bool whole = vectors && (uint64_t)(blockIdx.x + 1) * PARTS * kPart <= p.tokens;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint64_t t = (uint64_t)blockIdx.x * kPass + h * (kPass / 2) + threadIdx.x * 4;
-    lp[h] = load4(o.logprob, t, p.tokens, vectors), old[h] = load4(o.old, t, p.tokens, vectors);
-    ref[h] = load4(o.reference, t, p.tokens, vectors), ent[h] = load4(o.entropy, t, p.tokens, vectors);
-    adv[h] = o.per_token ? load4(o.advantage, t, p.tokens, vectors) : make_float4(0.f, 0.f, 0.f, 0.f);
-    bits[h] = t < p.tokens ? w.bits[t / 32] >> (t & 31) & 15 : 0;
+  for (int h = 0; h < PARTS; ++h) {
+    const uint64_t t = ((uint64_t)blockIdx.x * PARTS + h) * kPart + threadIdx.x * 4;
+    lp[h] = load4(o.logprob, t, p.tokens, whole), old[h] = load4(o.old, t, p.tokens, whole);
+    ref[h] = load4(o.reference, t, p.tokens, whole), ent[h] = load4(o.entropy, t, p.tokens, whole);
+    adv[h] = load4(o.per_token ? o.advantage : nullptr, t, p.tokens, whole);
+    bits[h] = w.bits[t / 32] >> (t & 31) & 15;             // (the last tile's words are all there)
   }
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint64_t base = (uint64_t)blockIdx.x * kPass + h * (kPass / 2) + warp * 128, t = base + 4 * lane;
+  for (int h = 0; h < PARTS; ++h) {
+    const uint64_t base = ((uint64_t)blockIdx.x * PARTS + h) * kPart + warp * 128, t = base + 4 * lane;
     uint32_t of[4] = {0, 0, 0, 0};
     if (LOOK && base < end) sequences_of(p, base, of);
     float4 g, ge;
@@ -406,10 +430,16 @@ __device__ __forceinline__ void few_tokens(const Packed<Id>& p, FewTokens& f) {
   const uint32_t lane = threadIdx.x & 31;
   const uint32_t begin = (uint32_t)p.offset(0), end = (uint32_t)p.offset(p.sequences);
   for (uint32_t s = threadIdx.x; s <= p.sequences; s += kFewThreads) f.offsets[s] = (uint32_t)p.offset(s);
+  Id ids[kFewEach];
+#pragma unroll
+  for (int j = 0; j < kFewEach; ++j) {
+    if (j * kFewThreads >= p.tokens) break;
+    ids[j] = ld_id(p.ids + min((uint64_t)(j * kFewThreads + threadIdx.x), p.tokens - 1));
+  }
 #pragma unroll
   for (int j = 0; j < kFewEach; ++j) {
     const uint32_t t = j * kFewThreads + threadIdx.x;
-    const uint32_t b = __ballot_sync(0xffffffffu, t < p.tokens && t >= begin && t < end && p.counts(t));
+    const uint32_t b = j * kFewThreads < p.tokens ? __ballot_sync(0xffffffffu, t >= begin && t < end && !(ids[j] < Id(0))) : 0;
     if (lane == 0) f.bits[t / 32] = b;
   }
   __syncthreads();
@@ -442,6 +472,10 @@ __global__ void __launch_bounds__(kFewThreads) policy_few_kernel(Packed<Id> p, P
   __shared__ uint32_t live;
   if (threadIdx.x == 0) live = 0;
   pdl_enter();
+  // the first tokens' values are on their way while the ids are counted
+  const uint32_t early = min(threadIdx.x, (uint32_t)p.tokens - 1);
+  const float first_lp = ld_stream(o.logprob + early), first_old = ld_stream(o.old + early);
+  const float first_ref = o.reference ? ld_stream(o.reference + early) : 0.f, first_entropy = o.entropy ? ld_stream(o.entropy + early) : 0.f;
   few_tokens(p, f);
   const bool look = o.by_sequence || !o.per_token;
   float even;
@@ -461,8 +495,7 @@ __global__ void __launch_bounds__(kFewThreads) policy_few_kernel(Packed<Id> p, P
   }
   const uint32_t begin = f.offsets[0], end = f.offsets[p.sequences];
   double total[4] = {0, 0, 0, 0};
-#pragma unroll 2
-  for (int j = 0; j < kFewEach; ++j) {
+  for (int j = 0; j < kFewEach && j * kFewThreads < (int)p.tokens; ++j) {
     const uint32_t t = j * kFewThreads + threadIdx.x;
     if (t < begin || t >= end) continue;
     const bool counts = f.counts(t);
@@ -470,9 +503,10 @@ __global__ void __launch_bounds__(kFewThreads) policy_few_kernel(Packed<Id> p, P
     if (counts) {
       const uint32_t s = look ? f.sequence(t, p.sequences) : 0;
       weight = o.by_sequence ? even * share[s] : even;
-      const Term e = term(o, o.logprob[t], o.old[t], o.reference ? o.reference[t] : 0.f, o.advantage[o.per_token ? t : s]);
+      const Term e = term(o, j ? o.logprob[t] : first_lp, j ? o.old[t] : first_old, j ? (o.reference ? o.reference[t] : 0.f) : first_ref,
+                          o.advantage[o.per_token ? t : s]);
       total[0] += e.surrogate * weight, total[1] += e.kl * weight, total[3] += e.clipped * weight;
-      if (o.entropy) total[2] += o.entropy[t] * weight;
+      if (o.entropy) total[2] += (j ? o.entropy[t] : first_entropy) * weight;
       g = e.slope * weight;
     }
     if (o.g_logprob) o.g_logprob[t] = g;
@@ -533,21 +567,34 @@ __global__ void __launch_bounds__(kThreads) sums_kernel(Packed<Id> p, Workspace 
   const uint64_t begin = p.offset(0), end = p.offset(p.sequences);
   const uint64_t tile = (uint64_t)blockIdx.x * kTile, tile_end = min(tile + kTile, p.tokens);
   const uint64_t from = max(tile, begin), to = min(tile_end, end);
+  float lp[16], ref[16];
+  Id ids[16];                                              // (all loads on their way before the first vote, and none behind a branch)
+  uint32_t mine = 0, bits = 0;
+  if (p.tokens) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const uint64_t t = min(tile + warp * (kTile / 8) + 32 * j + lane, p.tokens - 1);
+      ids[j] = ld_id(p.ids + t);
+      lp[j] = ld_stream(o.logprob + t);
+      ref[j] = 0.f;
+    }
+    if (o.reference)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) ref[j] = ld_stream(o.reference + min(tile + warp * (kTile / 8) + 32 * j + lane, p.tokens - 1));
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const uint64_t t = tile + warp * (kTile / 8) + 32 * j + lane;
+      const uint32_t b = __ballot_sync(0xffffffffu, !(ids[j] < Id(0)) && t >= from && t < to);
+      if (lane == j) mine = b;
+      bits |= (b >> lane & 1) << j;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) lp[j] = ref[j] = 0.f;
+  }
   if (warp < 2 && from < to) {
     const uint32_t s = sequence_of(p, warp == 0 ? from : to - 1);
     if (lane == 0) span[warp] = s;
-  }
-  float lp[16], ref[16];
-  uint32_t mine = 0, bits = 0;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const uint64_t t = tile + warp * (kTile / 8) + 32 * j + lane;
-    const bool inside = t >= from && t < to;
-    lp[j] = inside ? ld_stream(o.logprob + t) : 0.f;
-    ref[j] = inside && o.reference ? ld_stream(o.reference + t) : 0.f;
-    const uint32_t b = __ballot_sync(0xffffffffu, inside && p.counts(t));
-    if (lane == j) mine = b;
-    bits |= (b >> lane & 1) << j;
   }
   if (lane < 16) w.bits[tile / 32 + warp * 16 + lane] = mine;
   const uint32_t n = __reduce_add_sync(0xffffffffu, __popc(mine));
@@ -610,27 +657,25 @@ __device__ __forceinline__ double sum_of(const Workspace& w, uint32_t s, uint64_
   return warp_sum(v) + w.tail[first];
 }
 
-// A warp per pair; the last CTA writes the loss.
+// A warp per sequence; the last CTA writes the loss.
 template <class Id>
 __global__ void __launch_bounds__(kThreads) pairs_kernel(Packed<Id> p, Workspace w, Pairs o, float inv_count) {
   __shared__ float slots[kThreads / 8];
-  __shared__ double wide[kThreads / 8];
+  __shared__ double wide[kThreads / 8], sums[kThreads / 32];
+  __shared__ uint64_t counts[kThreads / 32];
   pdl_enter();
-  const uint32_t pair = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, s = blockIdx.x * (kThreads / 32) + warp;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  if (2 * pair < p.sequences) {
-    double d[2];
-    uint64_t n[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const uint64_t from = p.offset(2 * pair + k), to = p.offset(2 * pair + k + 1);
-      d[k] = from < to ? sum_of(w, 2 * pair + k, from, to) : 0;
-      n[k] = o.average && from < to ? counted(w, from, to) : 0;
-    }
-    if (lane == 0) {
-      const Pair2 r = pair_terms(o, pair, d[0], d[1], n[0], n[1], inv_count, w.share + 2 * pair, w.share + 2 * pair + 1);
-      sum[0] = r.loss * inv_count, sum[1] = r.right * inv_count, sum[2] = r.gap * inv_count;
-    }
+  if (s < p.sequences) {
+    const uint64_t from = p.offset(s), to = p.offset(s + 1);
+    const double d = from < to ? sum_of(w, s, from, to) : 0;
+    const uint64_t n = o.average && from < to ? counted(w, from, to) : 0;
+    if (lane == 0) sums[warp] = d, counts[warp] = n;
+  }
+  __syncthreads();
+  if (lane == 0 && (warp & 1) == 0 && s < p.sequences) {
+    const Pair2 r = pair_terms(o, s / 2, sums[warp], sums[warp + 1], counts[warp], counts[warp + 1], inv_count, w.share + s, w.share + s + 1);
+    sum[0] = r.loss * inv_count, sum[1] = r.right * inv_count, sum[2] = r.gap * inv_count;
   }
   sums4<kThreads>(sum, slots);
   double total[4];
@@ -668,9 +713,10 @@ __global__ void __launch_bounds__(kFewThreads) pairs_few_kernel(Packed<Id> p, Pa
   float lp[kFewEach], ref[kFewEach];
 #pragma unroll
   for (int j = 0; j < kFewEach; ++j) {
-    const uint32_t t = j * kFewThreads + threadIdx.x;
-    lp[j] = t < p.tokens ? o.logprob[t] : 0.f;
-    ref[j] = t < p.tokens && o.reference ? o.reference[t] : 0.f;
+    if (j * kFewThreads >= p.tokens) break;
+    const uint32_t t = min(j * kFewThreads + threadIdx.x, (uint32_t)p.tokens - 1);
+    lp[j] = ld_stream(o.logprob + t);
+    ref[j] = o.reference ? ld_stream(o.reference + t) : 0.f;
   }
   few_tokens(p, f);
 #pragma unroll
@@ -769,8 +815,11 @@ int run_policy(const Packed<Id>& p, const Policy& o, void* workspace, uint64_t w
     if (rc) return rc;
     const bool vectors = aligned16(o.logprob) && aligned16(o.old) && aligned16(o.reference) && aligned16(o.entropy) && aligned16(o.g_logprob) &&
                          aligned16(o.g_entropy) && (!o.per_token || aligned16(o.advantage));
-    auto kernel = o.by_sequence || !o.per_token ? policy_kernel<Id, true> : policy_kernel<Id, false>;
-    return launch("fpolicy_loss", kernel, dim3((unsigned)((p.tokens + kPass - 1) / kPass)), kThreads, 0, st, p, w, o, vectors);
+    // (half as many tokens to a CTA where there would not be one for each SM)
+    const bool look = o.by_sequence || !o.per_token, short_ = p.tokens <= 2ull * kPart * sm_count();
+    auto kernel = short_ ? (look ? policy_kernel<Id, true, 1> : policy_kernel<Id, false, 1>) : look ? policy_kernel<Id, true, 2> : policy_kernel<Id, false, 2>;
+    const uint64_t each = short_ ? kPart : 2 * kPart;
+    return launch("fpolicy_loss", kernel, dim3((unsigned)((p.tokens + each - 1) / each)), kThreads, 0, st, p, w, o, vectors);
   });
 }
 
@@ -790,7 +839,7 @@ int run_pairs(const Packed<Id>& p, const Pairs& o, void* workspace, uint64_t wor
     const uint32_t tiles = (uint32_t)tiles_of(p.tokens);
     int rc = launch("fpreference_loss: sums", sums_kernel<Id>, dim3(tiles), kThreads, 0, st, p, w, o);
     if (rc) return rc;
-    rc = launch("fpreference_loss", pairs_kernel<Id>, dim3((p.sequences / 2 + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, st, p, w, o, inv_count);
+    rc = launch("fpreference_loss", pairs_kernel<Id>, dim3((p.sequences + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, st, p, w, o, inv_count);
     if (rc || !o.g_logprob || !p.tokens) return rc;
     return launch("fpreference_loss: gradient", pairs_grad_kernel<Id>, dim3((unsigned)((p.tokens + kPass - 1) / kPass)), kThreads, 0, st, p, w,
                   o.g_logprob, aligned16(o.g_logprob));
@@ -848,6 +897,8 @@ int polar_b200_fpolicy_loss(const polar_b200_policy_batch* b, const polar_b200_p
   k.loss = loss, k.g_logprob = gLogProb, k.g_entropy = gEntropy;
   k.high = 1.f + o->clip_high, k.low = 1.f - o->clip_low;
   k.log_high = std::log1p((double)o->clip_high), k.log_low = o->clip_low == 1.f ? -std::numeric_limits<double>::infinity() : std::log1p(-(double)o->clip_low);
+  // d and the border are each rounded by 2^-24 of themselves
+  k.near_high = std::isinf(k.log_high) ? 0.f : (float)(k.log_high * 2.4e-7), k.near_low = std::isinf(k.log_low) ? 0.f : (float)(-k.log_low * 2.4e-7);
   k.kl = b->refLogProb ? o->kl_weight : 0.f, k.bonus = b->entropy ? o->entropy_weight : 0.f, k.count = o->count;
   k.by_sequence = o->by_sequence, k.per_token = b->advantage_per_token;
   return with_ids(b->id_type, [&](auto id) {
