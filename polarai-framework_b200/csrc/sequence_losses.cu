@@ -7,6 +7,7 @@
 //   few tokens (kFew): everything by one CTA in one launch;
 //   else a pass over the ids (policy) or over all (pairs), one over the sequences, one over the tokens.
 // Every sum is taken in a fixed order, over a CTA's tokens in fp32 and beyond that, as of the sums over a sequence, in 64 bits.
+#include <algorithm>
 #include <cmath>
 #include <limits>
 #include <type_traits>
@@ -157,6 +158,11 @@ __device__ __forceinline__ void sums4(T (&v)[4], T* slots) {
     for (int i = 0; i < 4; ++i) v[i] = warp_sum(lane < kWarps ? slots[lane * 4 + i] : T(0));
 }
 
+// Up to this many CTAs the last one of a pass adds up what all have left.  It costs each of them a fence and an atomic at its end, some 1.5 us in which nothing else takes
+// its place: with several CTAs one after another on an SM a kernel for the sums is cheaper (8.4 M tokens, 4096 CTAs: 60 -> 50 us).
+constexpr uint32_t kFewCtas = 1024;
+constexpr int kFinishThreads = 1024;
+
 // Leaves a CTA's sums and tells whether it was the last one to; then the sums of all CTAs are in `total` of its first thread, added in an
 // order that does not hang on which CTA was last.
 template <int THREADS>
@@ -242,7 +248,9 @@ __device__ __forceinline__ uint64_t counted(const Workspace& w, uint64_t from, u
 
 // What a token's term is multiplied by: the tokens that count altogether by one CTA, or of each sequence by a warp.
 constexpr int kTotalThreads = 1024;
-__global__ void __launch_bounds__(kTotalThreads) total_kernel(Workspace w, uint32_t tiles, float count) {
+// (Up to kFewTiles tiles every CTA of the next kernel adds the counts up by itself while its loads are on their way: a launch less.)
+constexpr uint32_t kFewTiles = 4096;
+__global__ void __launch_bounds__(kTotalThreads) total_kernel(Workspace w, uint32_t tiles) {
   __shared__ unsigned long long sums[kTotalThreads / 32];
   pdl_enter();
   unsigned long long n = 0;
@@ -255,7 +263,7 @@ __global__ void __launch_bounds__(kTotalThreads) total_kernel(Workspace w, uint3
   if (threadIdx.x == 0) {
     n = 0;
     for (unsigned long long s : sums) n += s;
-    w.shared->share = count > 0.f ? 1.f / count : n ? 1.f / (float)n : 0.f;
+    w.shared->share = n ? 1.f / (float)n : 0.f;
   }
 }
 template <class Id>
@@ -283,51 +291,76 @@ struct Policy {
   float *loss, *g_logprob, *g_entropy;
   float high, low;                                         // what the ratio is clipped to
   double log_high, log_low;
-  float near_high, near_low;                               // how far from these borders fp32 decides
+  float fp32_high, fp32_low, near;                         // the same in fp32, and how far from them it decides
   float kl, bonus, count;
   int by_sequence, per_token;
 };
 
-// exp(q) - 1 - q and, in `grown`, exp(q) - 1.  Near zero by the series from its second term on (the ninth is below 2^-24 of the first
-// up to 1/2): as a difference all digits of it would go.
-__device__ __forceinline__ float excess(float q, float* grown) {
-  if (fabsf(q) < 0.5f) {
-    float s = 1.f / 40320;
-    s = fmaf(s, q, 1.f / 5040), s = fmaf(s, q, 1.f / 720), s = fmaf(s, q, 1.f / 120), s = fmaf(s, q, 1.f / 24);
-    s = fmaf(s, q, 1.f / 6), s = fmaf(s, q, 0.5f);
-    const float k = s * q * q;
-    *grown = q + k;
-    return k;
-  }
-  *grown = expm1f(q);
-  return *grown - q;
-}
-
-struct Term {
-  float surrogate, kl, clipped, slope;
+// The terms of N tokens, whatever they hold; of those that do not count nothing is used.
+template <int N>
+struct Terms {
+  float surrogate[N], kl[N], slope[N];
+  float beyond[N];                                         // above zero: the ratio is past the border that its advantage drives it to
 };
-// A token that counts.  On which side of the clipping border it lies is decided by the difference of the logarithms in 64 bits, where it is
-// exact: in fp32 rounding would decide for tokens on the border.  Away from the border both agree, and fp32 is asked, which is
-// three conversions and a sum in 64 bits less.
-__device__ __forceinline__ Term term(const Policy& o, float logprob, float old, float reference, float advantage) {
-  const float d = logprob - old, high = (float)o.log_high, low = (float)o.log_low;
-  bool over = d > high, under = d < low;
-  if (fabsf(d - high) <= o.near_high || fabsf(d - low) <= o.near_low) {
-    const double exact = (double)logprob - (double)old;
-    over = exact > o.log_high, under = exact < o.log_low;
+// On which side of the clipping border a token lies is decided by the difference of the logarithms in 64 bits, where it is exact: in fp32 rounding would decide
+// for tokens on the border.  Away from it both agree, and fp32 is asked.
+// exp(q) - 1 - q is taken near zero by the series from its second term on (the ninth is below 2^-24 of the first up to 1/2): as a difference all
+// its digits would go.  Both take the slow way for all N where one needs it; two tokens at a time share an instruction of the series.
+// (The exponential's argument has d's rounding, so that the approximate one, good to 2 ulp and the argument's rounding, gives nothing away.)
+template <int N>
+__device__ __forceinline__ Terms<N> terms(const Policy& o, const float* logprob, const float* old, const float* reference, const float* advantage) {
+  Terms<N> t;
+  float d[N], nearest = 1.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    d[k] = logprob[k] - old[k];
+    t.beyond[k] = advantage[k] < 0.f ? o.fp32_low - d[k] : d[k] - o.fp32_high;
+    nearest = fminf(nearest, fabsf(t.beyond[k]));
   }
-  const bool cut = (advantage > 0.f && over) || (advantage < 0.f && under);
-  const float free = expf(d) * advantage;
-  Term t;
-  t.surrogate = cut ? (over ? o.high : o.low) * advantage : free;
-  t.clipped = cut ? 1.f : 0.f;
-  t.slope = cut ? 0.f : -free;
-  t.kl = 0.f;
-  if (o.reference) {
-    float grown;
-    t.kl = excess(reference - logprob, &grown);
-    t.slope -= o.kl * grown;
+  if (nearest <= o.near) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const double exact = (double)logprob[k] - (double)old[k];
+      if (d[k] == d[k]) t.beyond[k] = (advantage[k] < 0.f ? exact < o.log_low : exact > o.log_high) ? 1.f : -1.f;
+    }
   }
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const bool cut = t.beyond[k] > 0.f;
+    float ratio;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(ratio) : "f"(d[k] * 1.4426950408889634f));
+    t.surrogate[k] = (cut ? (advantage[k] < 0.f ? o.low : o.high) : ratio) * advantage[k];
+    t.slope[k] = cut ? 0.f : -t.surrogate[k];
+    t.kl[k] = 0.f;
+  }
+  if (!o.reference) return t;
+  float q[N], grown[N], farthest = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    q[k] = reference[k] - logprob[k];
+    farthest = fmaxf(farthest, fabsf(q[k]));               // (a NaN stays one by the series too)
+  }
+  auto both = [](float v) { return pair(v, v); };
+#pragma unroll
+  for (int k = 0; k < N; k += 2) {
+    const Pair x = pair(q[k], q[N > 1 ? k + 1 : k]);
+    Pair y = fma2(both(1.f / 40320), x, both(1.f / 5040));
+    y = fma2(y, x, both(1.f / 720)), y = fma2(y, x, both(1.f / 120)), y = fma2(y, x, both(1.f / 24)), y = fma2(y, x, both(1.f / 6));
+    y = mul2(mul2(fma2(y, x, both(0.5f)), x), x);
+    const float2 kl = halves(y), more = halves(add2(x, y));
+    t.kl[k] = kl.x, grown[k] = more.x;
+    if (N > 1) t.kl[k + 1] = kl.y, grown[k + 1] = more.y;
+  }
+  if (farthest >= 0.5f) {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (fabsf(q[k]) >= 0.5f) {
+        grown[k] = expm1f(q[k]);
+        t.kl[k] = grown[k] - q[k];
+      }
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) t.slope[k] = fmaf(-o.kl, grown[k], t.slope[k]);
   return t;
 }
 __device__ __forceinline__ void write_loss(const Policy& o, const double* total) {
@@ -357,17 +390,17 @@ __device__ __forceinline__ void store4(float* p, float4 v, uint64_t t, uint64_t 
     if (t + k >= begin && t + k < end) p[t + k] = (&v.x)[k];
 }
 
-// LOOK: a token's sequence is needed.  PARTS: of kPart tokens that a CTA has, with all their loads on their way.
+// few_tiles: the tiles whose counts each CTA adds up by itself.  LOOK: a token's sequence is needed.  PARTS: of kPart tokens that a CTA has, with all their loads on their way.
 constexpr uint32_t kPart = kThreads * 4;
 template <class Id, bool LOOK, int PARTS>
-__global__ void __launch_bounds__(kThreads) policy_kernel(Packed<Id> p, Workspace w, Policy o, bool vectors) {
+__global__ void __launch_bounds__(kThreads) policy_kernel(Packed<Id> p, Workspace w, Policy o, bool vectors, uint32_t few_tiles) {
   __shared__ float slots[kThreads / 8];
+  __shared__ uint32_t tokens[kThreads / 32];
   __shared__ double wide[kThreads / 8];
   pdl_enter();
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint64_t begin = p.offset(0), end = p.offset(p.sequences);
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  const float even = o.by_sequence ? (o.count > 0.f ? 1.f / o.count : 1.f / (float)w.shared->live) : w.shared->share;
   float4 lp[PARTS], old[PARTS], ref[PARTS], ent[PARTS], adv[PARTS];
   uint32_t bits[PARTS];
   const bool whole = vectors && (uint64_t)(blockIdx.x + 1) * PARTS * kPart <= p.tokens;
@@ -379,29 +412,69 @@ __global__ void __launch_bounds__(kThreads) policy_kernel(Packed<Id> p, Workspac
     adv[h] = load4(o.per_token ? o.advantage : nullptr, t, p.tokens, whole);
     bits[h] = w.bits[t / 32] >> (t & 31) & 15;             // (the last tile's words are all there)
   }
+  float even;
+  if (o.count > 0.f) {
+    even = 1.f / o.count;
+  } else if (o.by_sequence) {
+    even = 1.f / (float)w.shared->live;
+  } else if (few_tiles) {
+    uint32_t n = 0;
+    for (uint32_t i = threadIdx.x; i < few_tiles; i += kThreads) n += w.counts[i];
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) tokens[warp] = n;
+    __syncthreads();
+    n = 0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 32; ++i) n += tokens[i];
+    even = n ? 1.f / (float)n : 0.f;
+  } else {
+    even = w.shared->share;
+  }
 #pragma unroll
   for (int h = 0; h < PARTS; ++h) {
     const uint64_t base = ((uint64_t)blockIdx.x * PARTS + h) * kPart + warp * 128, t = base + 4 * lane;
     uint32_t of[4] = {0, 0, 0, 0};
     if (LOOK && base < end) sequences_of(p, base, of);
     float4 g, ge;
+    if (LOOK && !o.per_token)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) (&adv[h].x)[k] = bits[h] >> k & 1 ? o.advantage[of[k]] : 0.f;
+    const Terms<4> e = terms<4>(o, &lp[h].x, &old[h].x, &ref[h].x, &adv[h].x);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const bool counts = bits[h] >> k & 1;
-      const float a = o.per_token ? (&adv[h].x)[k] : counts ? o.advantage[of[k]] : 0.f;
-      const float weight = counts ? (o.by_sequence ? even * w.share[of[k]] : even) : 0.f;
-      const Term e = term(o, (&lp[h].x)[k], (&old[h].x)[k], (&ref[h].x)[k], a);
-      if (counts) sum[0] += e.surrogate * weight, sum[1] += e.kl * weight, sum[2] += (&ent[h].x)[k] * weight, sum[3] += e.clipped * weight;
-      (&g.x)[k] = counts ? e.slope * weight : 0.f;
-      (&ge.x)[k] = -o.bonus * weight;
+      const float weight = LOOK && o.by_sequence && counts ? even * w.share[of[k]] : even;
+      if (counts) {
+        sum[0] += e.surrogate[k] * weight, sum[1] += e.kl[k] * weight, sum[2] += (&ent[h].x)[k] * weight;
+        // (of two zeros neither is above the other)
+        if (e.beyond[k] > 0.f && (&adv[h].x)[k] != 0.f) sum[3] += weight;
+      }
+      (&g.x)[k] = counts ? e.slope[k] * weight : 0.f;
+      (&ge.x)[k] = counts ? -o.bonus * weight : 0.f;
     }
     if (o.g_logprob) store4(o.g_logprob, g, t, begin, end, vectors);
     if (o.g_entropy) store4(o.g_entropy, ge, t, begin, end, vectors);
   }
   sums4<kThreads>(sum, slots);
+  if (gridDim.x > kFewCtas) {
+    if (threadIdx.x == 0) w.partial[blockIdx.x] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+    return;
+  }
   double total[4];
   if (last_sums<kThreads>(make_float4(sum[0], sum[1], sum[2], sum[3]), w.partial, gridDim.x, &w.shared->ticket, total, wide) && threadIdx.x == 0)
     write_loss(o, total);
+}
+__global__ void __launch_bounds__(kFinishThreads) policy_finish_kernel(Workspace w, Policy o, uint32_t ctas) {
+  __shared__ double slots[kFinishThreads / 8];
+  pdl_enter();
+  double total[4] = {0, 0, 0, 0};
+#pragma unroll 4
+  for (uint32_t c = threadIdx.x; c < ctas; c += kFinishThreads) {
+    const float4 p = w.partial[c];
+    total[0] += p.x, total[1] += p.y, total[2] += p.z, total[3] += p.w;
+  }
+  sums4<kFinishThreads>(total, slots);
+  if (threadIdx.x == 0) write_loss(o, total);
 }
 
 // ---- one CTA for few tokens: which of them count, and how many before each word of 32
@@ -503,11 +576,12 @@ __global__ void __launch_bounds__(kFewThreads) policy_few_kernel(Packed<Id> p, P
     if (counts) {
       const uint32_t s = look ? f.sequence(t, p.sequences) : 0;
       weight = o.by_sequence ? even * share[s] : even;
-      const Term e = term(o, j ? o.logprob[t] : first_lp, j ? o.old[t] : first_old, j ? (o.reference ? o.reference[t] : 0.f) : first_ref,
-                          o.advantage[o.per_token ? t : s]);
-      total[0] += e.surrogate * weight, total[1] += e.kl * weight, total[3] += e.clipped * weight;
+      const float lp = j ? o.logprob[t] : first_lp, old = j ? o.old[t] : first_old, ref = j ? (o.reference ? o.reference[t] : 0.f) : first_ref;
+      const Terms<1> e = terms<1>(o, &lp, &old, &ref, o.advantage + (o.per_token ? t : s));
+      total[0] += e.surrogate[0] * weight, total[1] += e.kl[0] * weight;
+      if (e.beyond[0] > 0.f && o.advantage[o.per_token ? t : s] != 0.f) total[3] += weight;
       if (o.entropy) total[2] += (j ? o.entropy[t] : first_entropy) * weight;
-      g = e.slope * weight;
+      g = e.slope[0] * weight;
     }
     if (o.g_logprob) o.g_logprob[t] = g;
     if (o.g_entropy) o.g_entropy[t] = -o.bonus * weight;
@@ -809,8 +883,8 @@ int run_policy(const Packed<Id>& p, const Policy& o, void* workspace, uint64_t w
     if (o.by_sequence) {
       const uint64_t ctas = ((uint64_t)p.sequences + kThreads / 32 - 1) / (kThreads / 32), most = 8ull * sm_count();
       rc = launch("fpolicy_loss: shares", shares_kernel<Id>, dim3((unsigned)(ctas < most ? ctas : most)), kThreads, 0, st, p, w);
-    } else {
-      rc = launch("fpolicy_loss: total", total_kernel, dim3(1), kTotalThreads, 0, st, w, tiles, o.count);
+    } else if (o.count == 0.f && tiles > kFewTiles) {
+      rc = launch("fpolicy_loss: total", total_kernel, dim3(1), kTotalThreads, 0, st, w, tiles);
     }
     if (rc) return rc;
     const bool vectors = aligned16(o.logprob) && aligned16(o.old) && aligned16(o.reference) && aligned16(o.entropy) && aligned16(o.g_logprob) &&
@@ -819,7 +893,10 @@ int run_policy(const Packed<Id>& p, const Policy& o, void* workspace, uint64_t w
     const bool look = o.by_sequence || !o.per_token, short_ = p.tokens <= 2ull * kPart * sm_count();
     auto kernel = short_ ? (look ? policy_kernel<Id, true, 1> : policy_kernel<Id, false, 1>) : look ? policy_kernel<Id, true, 2> : policy_kernel<Id, false, 2>;
     const uint64_t each = short_ ? kPart : 2 * kPart;
-    return launch("fpolicy_loss", kernel, dim3((unsigned)((p.tokens + each - 1) / each)), kThreads, 0, st, p, w, o, vectors);
+    const uint32_t ctas = (uint32_t)((p.tokens + each - 1) / each);
+    rc = launch("fpolicy_loss", kernel, dim3(ctas), kThreads, 0, st, p, w, o, vectors, tiles <= kFewTiles ? tiles : 0u);
+    if (rc || ctas <= kFewCtas) return rc;
+    return launch("fpolicy_loss: sums", policy_finish_kernel, dim3(1), kFinishThreads, 0, st, w, o, ctas);
   });
 }
 
@@ -898,7 +975,8 @@ int polar_b200_fpolicy_loss(const polar_b200_policy_batch* b, const polar_b200_p
   k.high = 1.f + o->clip_high, k.low = 1.f - o->clip_low;
   k.log_high = std::log1p((double)o->clip_high), k.log_low = o->clip_low == 1.f ? -std::numeric_limits<double>::infinity() : std::log1p(-(double)o->clip_low);
   // d and the border are each rounded by 2^-24 of themselves
-  k.near_high = std::isinf(k.log_high) ? 0.f : (float)(k.log_high * 2.4e-7), k.near_low = std::isinf(k.log_low) ? 0.f : (float)(-k.log_low * 2.4e-7);
+  k.fp32_high = (float)k.log_high, k.fp32_low = (float)k.log_low;
+  k.near = (float)(2.4e-7 * std::max(std::isinf(k.log_high) ? 0.0 : k.log_high, std::isinf(k.log_low) ? 0.0 : -k.log_low));
   k.kl = b->refLogProb ? o->kl_weight : 0.f, k.bonus = b->entropy ? o->entropy_weight : 0.f, k.count = o->count;
   k.by_sequence = o->by_sequence, k.per_token = b->advantage_per_token;
   return with_ids(b->id_type, [&](auto id) {
