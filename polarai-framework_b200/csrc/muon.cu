@@ -177,9 +177,10 @@ template <int BN>
 struct Cfg {
   static constexpr uint32_t kAPlane = BM * BK * 2, kBPlane = BN * BK * 2;
   static constexpr uint32_t kStageBytes = 2 * (kAPlane + kBPlane);
-  static constexpr int kStages = (int)((200u * 1024u) / kStageBytes);
+  static constexpr int kStages = (int)((194u * 1024u) / kStageBytes);
   static constexpr uint32_t kTileBytes = kStages * kStageBytes;
-  static constexpr uint32_t kSmemBytes = kTileBytes + 1024 + 256;
+  // (behind the slabs and the barriers: 32 x 33 floats for each warp of the epilogue)
+  static constexpr uint32_t kSmemBytes = kTileBytes + 1024 + 256 + kEpilogueWarps * 32 * 33 * 4;
 };
 
 enum Kind : int { kSymmetric, kRound, kUpdate };
@@ -265,50 +266,33 @@ __device__ __forceinline__ Target target_of(const Product& p, const Shape& q, co
   return q.kind == kUpdate ? p.targets[q.first_target + at.z] : Target{};
 }
 
-// Writes 16 columns of the result from c0 on of row r0 + lane, whose sums are in `v`.
-__device__ __forceinline__ void finish(const Shape& q, const Place& at, const Target& target, float lr, uint32_t r0, uint32_t c0, int lane, uint32_t* v) {
-  const uint32_t row = r0 + lane, block = c0 & ~31u;
-  if (c0 >= q.n || r0 >= q.m) return;
-  if (q.kind == kSymmetric && block < r0) return;          // below the diagonal: written by the block above it
-  if (q.kind == kUpdate) {
-    const float keep = 1.f - lr * target.decay, rate = q.by * lr * target.scale;
-    float* const w = target.weights + (uint64_t)row * q.n + c0;
-    if (row >= q.m) return;
-    if ((q.n & 3) == 0 && (reinterpret_cast<uintptr_t>(target.weights) & 15) == 0 && c0 + 16 <= q.n) {
+__device__ __forceinline__ bool aligned_weights(const Shape& q, const Target& t) { return (q.n & 3) == 0 && (reinterpret_cast<uintptr_t>(t.weights) & 15) == 0; }
+// What 16 columns of a row need besides their sums: both planes of what is added, or the weights where they lie on 16 bytes.  Loaded ahead of use, since no load
+// moves before a store by itself.
+struct Beside {
+  uint4 v[4];
+};
+__device__ __forceinline__ Beside beside16(const Shape& q, const Place& at, const Target& target, uint32_t row, uint32_t c0) {
+  Beside b = {};
+  if (row >= q.m || c0 >= q.n) return b;
+  if (q.add && (c0 | 31u) >= (row & ~31u)) {
+    const uint4* const add = reinterpret_cast<const uint4*>(q.add + 2 * at.z * q.plane + (uint64_t)row * q.pitch + c0);
+    b.v[0] = add[0], b.v[1] = add[1], b.v[2] = add[q.plane / 8], b.v[3] = add[q.plane / 8 + 1];
+  } else if (q.kind == kUpdate && aligned_weights(q, target) && c0 + 16 <= q.n) {
+    const uint4* const w = reinterpret_cast<const uint4*>(target.weights + (uint64_t)row * q.n + c0);
 #pragma unroll
-      for (int j = 0; j < 16; j += 4) {
-        float4 x = *reinterpret_cast<const float4*>(w + j);
-        x.x = x.x * keep - rate * __uint_as_float(v[j]), x.y = x.y * keep - rate * __uint_as_float(v[j + 1]);
-        x.z = x.z * keep - rate * __uint_as_float(v[j + 2]), x.w = x.w * keep - rate * __uint_as_float(v[j + 3]);
-        *reinterpret_cast<float4*>(w + j) = x;
-      }
-    } else {
-      float x[16];                                         // (all loads before the first store, which might change what they read)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) x[j] = c0 + j < q.n ? w[j] : 0.f;
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (c0 + j < q.n) w[j] = x[j] * keep - rate * __uint_as_float(v[j]);
-    }
-    return;
+    for (int j = 0; j < 4; ++j) b.v[j] = w[j];
   }
-  __half* const matrix = q.out + 2 * at.z * q.plane;
-  uint32_t hi[8], lo[8];                                   // two columns in each
+  return b;
+}
+// The result's 16 columns from c0 on of a row, from their sums: by * sum + add_by * add + diagonal.
+__device__ __forceinline__ void complete(const Shape& q, uint32_t row, uint32_t c0, const Beside& beside, uint32_t* v) {
   if (q.add) {
-    const __half* add = q.add + 2 * at.z * q.plane + (uint64_t)row * q.pitch + c0;
-    if (row < q.m) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint4 h = *reinterpret_cast<const uint4*>(add + 8 * j), l = *reinterpret_cast<const uint4*>(add + q.plane + 8 * j);
-        hi[4 * j] = h.x, hi[4 * j + 1] = h.y, hi[4 * j + 2] = h.z, hi[4 * j + 3] = h.w;
-        lo[4 * j] = l.x, lo[4 * j + 1] = l.y, lo[4 * j + 2] = l.z, lo[4 * j + 3] = l.w;
-      }
-    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float2 h = __half22float2(*reinterpret_cast<__half2*>(&hi[j])), l = __half22float2(*reinterpret_cast<__half2*>(&lo[j]));
-      float a = fmaf(q.by, __uint_as_float(v[2 * j]), q.add_by * (h.x + l.x));
-      float b = fmaf(q.by, __uint_as_float(v[2 * j + 1]), q.add_by * (h.y + l.y));
+      const float2 x = __half22float2(reinterpret_cast<const __half2*>(beside.v)[j]), y = __half22float2(reinterpret_cast<const __half2*>(beside.v + 2)[j]);
+      float a = fmaf(q.by, __uint_as_float(v[2 * j]), q.add_by * (x.x + y.x));
+      float b = fmaf(q.by, __uint_as_float(v[2 * j + 1]), q.add_by * (x.y + y.y));
       if (c0 + 2 * j == row) a += q.diagonal;
       if (c0 + 2 * j + 1 == row) b += q.diagonal;
       v[2 * j] = __float_as_uint(a), v[2 * j + 1] = __float_as_uint(b);
@@ -317,6 +301,9 @@ __device__ __forceinline__ void finish(const Shape& q, const Place& at, const Ta
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(q.by * __uint_as_float(v[j]));
   }
+}
+// 16 neighbours as pairs, two of them to each word of `hi` and `lo`.
+__device__ __forceinline__ void split16(const uint32_t* v, uint32_t (&hi)[8], uint32_t (&lo)[8]) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float a = __uint_as_float(v[2 * j]), b = __uint_as_float(v[2 * j + 1]);
@@ -325,11 +312,109 @@ __device__ __forceinline__ void finish(const Shape& q, const Place& at, const Ta
     const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
     hi[j] = *reinterpret_cast<const uint32_t*>(&h), lo[j] = *reinterpret_cast<const uint32_t*>(&l);
   }
-  if (row < q.m) {                                         // (columns behind the last one lie in the row's padding)
-    __half* const out = matrix + (uint64_t)row * q.pitch + c0;
-    st_v8(out, hi);
-    st_v8(out + q.plane, lo);
+}
+__device__ __forceinline__ void store16(const Shape& q, __half* matrix, uint64_t row, uint32_t col, const uint32_t (&hi)[8], const uint32_t (&lo)[8]) {
+  __half* const out = matrix + row * q.pitch + col;        // (columns behind the last one lie in the row's padding)
+  st_v8(out, hi);
+  st_v8(out + q.plane, lo);
+}
+// w <- w * keep - rate * X for 16 columns of a row.
+__device__ __forceinline__ void update16(const Shape& q, const Target& target, float keep, float rate, uint32_t row, uint32_t c0, const Beside& beside, const uint32_t* v) {
+  float* const w = target.weights + (uint64_t)row * q.n + c0;
+  if (row >= q.m) return;
+  if (aligned_weights(q, target) && c0 + 16 <= q.n) {
+    const float* const old = reinterpret_cast<const float*>(beside.v);
+#pragma unroll
+    for (int j = 0; j < 16; j += 4)
+      *reinterpret_cast<float4*>(w + j) = make_float4(old[j] * keep - rate * __uint_as_float(v[j]), old[j + 1] * keep - rate * __uint_as_float(v[j + 1]),
+                                                      old[j + 2] * keep - rate * __uint_as_float(v[j + 2]), old[j + 3] * keep - rate * __uint_as_float(v[j + 3]));
+  } else {
+    float x[16];                                           // (all loads before the first store, which might change what they read)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = c0 + j < q.n ? w[j] : 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (c0 + j < q.n) w[j] = x[j] * keep - rate * __uint_as_float(v[j]);
   }
+}
+
+// Writes 32 rows from r0 on (one to each lane) and COLS columns from c0 on, whose sums are in `v`; `beside` belongs to the first 16 of them.  What has to be turned over
+// goes through `turn`, 32 rows of 33 words of this warp's own: the mirror image of a symmetric matrix's block, so that it is written in rows too, and unaligned weights.
+template <int COLS>
+__device__ __forceinline__ void finish(const Shape& q, const Place& at, const Target& target, float lr, uint32_t r0, uint32_t c0, int lane, uint32_t (&v)[COLS], Beside beside,
+                                       uint32_t* turn) {
+  const uint32_t row = r0 + lane;
+  const float keep = 1.f - lr * target.decay, rate = q.by * lr * target.scale;
+  __half* const matrix = q.out + 2 * at.z * q.plane;
+#pragma unroll
+  for (int part = 0; part < COLS / 32; ++part) {           // blocks of 32 columns
+    const uint32_t block = c0 + 32 * part;
+    uint32_t* const x = v + 32 * part;
+    if (block >= q.n || r0 >= q.m) return;
+    const bool mirror = q.kind == kSymmetric && block > r0;
+    const bool turned = mirror || (q.kind == kUpdate && !(aligned_weights(q, target) && block + 32 <= q.n));
+    if (turned) __syncwarp();
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const uint32_t col = block + 16 * half;
+      const Beside now = beside;
+      if (32 * part + 16 * half + 16 < COLS) beside = beside16(q, at, target, row, col + 16);
+      if (q.kind == kSymmetric && block < r0) continue;    // below the diagonal: written by the block above it
+      if (q.kind == kUpdate) {
+        if (!turned) update16(q, target, keep, rate, row, col, now, x + 16 * half);
+        else
+#pragma unroll
+          for (int j = 0; j < 16; ++j) turn[lane * 33 + 16 * half + j] = x[16 * half + j];
+        continue;
+      }
+      uint32_t hi[8], lo[8];
+      complete(q, row, col, now, x + 16 * half);
+      split16(x + 16 * half, hi, lo);
+      if (row < q.m) store16(q, matrix, row, col, hi, lo);
+      if (mirror)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {                      // a pair to a word
+          turn[lane * 33 + 16 * half + 2 * j] = __byte_perm(hi[j], lo[j], 0x5410);
+          turn[lane * 33 + 16 * half + 2 * j + 1] = __byte_perm(hi[j], lo[j], 0x7632);
+        }
+    }
+    if (!turned) continue;
+    __syncwarp();
+    if (block + lane >= q.n) continue;                     // (a lane is a column now)
+    if (mirror) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t a = turn[(16 * half + 2 * j) * 33 + lane], b = turn[(16 * half + 2 * j + 1) * 33 + lane];
+          hi[j] = __byte_perm(a, b, 0x5410), lo[j] = __byte_perm(a, b, 0x7632);
+        }
+        store16(q, matrix, block + lane, r0 + 16 * half, hi, lo);
+      }
+    } else {
+      float* const w = target.weights + (uint64_t)r0 * q.n + block + lane;
+      float old[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) old[i] = r0 + i < q.m ? w[(uint64_t)i * q.n] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (r0 + i < q.m) w[(uint64_t)i * q.n] = old[i] * keep - rate * __uint_as_float(turn[i * 33 + lane]);
+    }
+  }
+}
+// The same for 16 columns, of which clusters' CTAs have few: without the detour.
+__device__ __forceinline__ void finish16(const Shape& q, const Place& at, const Target& target, float lr, uint32_t r0, uint32_t c0, int lane, uint32_t (&v)[16]) {
+  const uint32_t row = r0 + lane, block = c0 & ~31u;
+  if (c0 >= q.n || r0 >= q.m) return;
+  if (q.kind == kSymmetric && block < r0) return;
+  const Beside beside = beside16(q, at, target, row, c0);
+  if (q.kind == kUpdate) return update16(q, target, 1.f - lr * target.decay, q.by * lr * target.scale, row, c0, beside, v);
+  __half* const matrix = q.out + 2 * at.z * q.plane;
+  uint32_t hi[8], lo[8];
+  complete(q, row, c0, beside, v);
+  split16(v, hi, lo);
+  if (row < q.m) store16(q, matrix, row, c0, hi, lo);
   if (q.kind == kSymmetric && block > r0) {                // its mirror image: a column of the block is a row there, 32 lanes side by side
     unsigned short* const mirror = reinterpret_cast<unsigned short*>(matrix) + (uint64_t)c0 * q.pitch + row;
 #pragma unroll
@@ -401,36 +486,35 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
     for (uint32_t t = first; ok && t < p.tiles; t += step) {
       const Place at = place_of<BN>(p, t);
       const Shape& q = p.s[at.shape];
-      uint32_t sum[BN / 64][32];                           // this thread's row of its half of the tile, as bits of floats
+      const uint32_t r0 = (uint32_t)at.m0 + quarter * 32, c0 = (uint32_t)at.n0 + half * (BN / 2);
+      uint32_t sum[BN / 2];                                // this thread's row of its half of the tile, as bits of floats
       int end;
       const int begin = slabs_of(q, &end), runs = (end - begin + kRun - 1) / kRun;
+      const Target target = target_of(p, q, at);
+      Beside beside = {};
       if (SPLIT && runs == 0) {
 #pragma unroll
-        for (int j = 0; j < BN / 64; ++j)
-#pragma unroll
-          for (int e = 0; e < 32; ++e) sum[j][e] = 0;
+        for (int e = 0; e < BN / 2; ++e) sum[e] = 0;
       }
       for (int i = 0; i < runs; ++i, ++run) {
         const uint32_t as = run & 1u;
+        if (!SPLIT && i + 1 == runs) beside = beside16(q, at, target, r0 + lane, c0);
         ok = mbar_wait(acc_full(as), (run >> 1) & 1u, abort_flag, p.status, 704, p.wait_ns);
         if (!ok) break;
         tc_fence_after();
         const uint32_t acc = tmem_base + as * BN + half * (BN / 2) + ((uint32_t)(quarter * 32) << 16);
         if (i == 0) {
 #pragma unroll
-          for (int j = 0; j < BN / 64; ++j) tmem_ld_32x32(acc + 32 * j, sum[j]);
+          for (int j = 0; j < BN / 2; j += 32) tmem_ld_32x32(acc + j, sum + j);
           tmem_ld_wait();
         } else {
 #pragma unroll
-          for (int j = 0; j < BN / 32; ++j) {
+          for (int j = 0; j < BN / 2; j += 16) {
             uint32_t v[16];
-            tmem_ld_32x16(acc + 16 * j, v);
+            tmem_ld_32x16(acc + j, v);
             tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              uint32_t& x = sum[j / 2][j % 2 * 16 + e];
-              x = __float_as_uint(__uint_as_float(x) + __uint_as_float(v[e]));
-            }
+            for (int e = 0; e < 16; ++e) sum[j + e] = __float_as_uint(__uint_as_float(sum[j + e]) + __uint_as_float(v[e]));
           }
         }
         tc_fence_before();
@@ -438,19 +522,15 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
         if (lane == 0) mbar_arrive(acc_empty(as));
       }
       if (!ok) break;
-      const Target target = target_of(p, q, at);
       if constexpr (SPLIT) {
         // (the slabs have been read: the last product has been waited for)
         float* const shared = reinterpret_cast<float*>(smem_gen);
 #pragma unroll
-        for (int j = 0; j < BN / 64; ++j)
-#pragma unroll
-          for (int e = 0; e < 32; ++e) shared[(half * (BN / 2) + 32 * j + e) * BM + quarter * 32 + lane] = __uint_as_float(sum[j][e]);
+        for (int j = 0; j < BN / 2; ++j) shared[(half * (BN / 2) + j) * BM + quarter * 32 + lane] = __uint_as_float(sum[j]);
       } else {
-#pragma unroll
-        for (int part = 0; part < BN / 32; ++part)
-          finish(q, at, target, lr, (uint32_t)at.m0 + quarter * 32, (uint32_t)at.n0 + half * (BN / 2) + 16 * part, lane,
-                 sum[part / 2] + part % 2 * 16);
+        uint32_t* const turn = reinterpret_cast<uint32_t*>(smem_gen + C::kTileBytes + 256) + (warp - 4) * (32 * 33);
+        finish(q, at, target, lr, r0, c0, lane, sum, beside, turn);
+        __syncwarp();
       }
     }
   } else {
@@ -545,7 +625,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
 #pragma unroll
           for (int j = 0; j < 16; ++j)
             v[j] = __float_as_uint(__uint_as_float(v[j]) + ld_cluster(shared + (c + j) * BM + quarter * 32 + lane, r));
-        finish(q, at, target, lr, (uint32_t)at.m0 + quarter * 32, (uint32_t)at.n0 + c, lane, v);
+        finish16(q, at, target, lr, (uint32_t)at.m0 + quarter * 32, (uint32_t)at.n0 + c, lane, v);
       }
     }
     __syncthreads();
