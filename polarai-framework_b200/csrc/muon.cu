@@ -170,23 +170,25 @@ __global__ void __launch_bounds__(kThreads) begin_kernel(const __grid_constant__
 constexpr int BM = 128, BK = 32;
 constexpr int kRun = 4;                                    // slabs that are summed in tensor memory
 constexpr int kEpilogueWarps = 8, kProductThreads = 32 * (4 + kEpilogueWarps);
-// Registers of a thread: 168 at launch (three warpgroups of 128 threads, 64512 in all), then what the sums need for the epilogue's two and
+// Registers of a thread where tiles are 256 wide: 168 at launch (three warpgroups of 128 threads, 64512 in all), then what the sums need for the epilogue's two and
 // what is left for the other: 2 * 128 * 232 + 128 * 40 = 64512.
 constexpr int kFewRegisters = 40, kManyRegisters = 232;
+constexpr uint32_t kSlotBytes = 32 * 32 * 2 * 2;           // a block of 32 x 32 as pairs
 template <int BN>
 struct Cfg {
-  static constexpr uint32_t kAPlane = BM * BK * 2, kBPlane = BN * BK * 2;
-  static constexpr uint32_t kStageBytes = 2 * (kAPlane + kBPlane);
-  static constexpr int kStages = (int)((194u * 1024u) / kStageBytes);
-  static constexpr uint32_t kTileBytes = kStages * kStageBytes;
-  // (behind the slabs and the barriers: 32 x 33 floats for each warp of the epilogue)
-  static constexpr uint32_t kSmemBytes = kTileBytes + 1024 + 256 + kEpilogueWarps * 32 * 33 * 4;
+  static constexpr uint32_t kAPlane = BM * BK * 2, kBPlane = BN * BK * 2, kStageBytes = 2 * (kAPlane + kBPlane);   // both planes of both operands
+  static constexpr int kStages = BN == 256 ? 4 : 5;
+  static constexpr int kSlots = BN == 256 ? 1 : 2;         // blocks on their way to memory, for each warp of the epilogue
+  static constexpr uint32_t kWarpBytes = kSlots * kSlotBytes;
+  static constexpr uint32_t kTileBytes = kStages * kStageBytes, kTurnBytes = kEpilogueWarps * kWarpBytes;
+  static constexpr uint32_t kBytes = kTileBytes + kTurnBytes + 1024 + 256;
+  static_assert(kBytes <= 227 * 1024, "shared memory");
 };
 
 enum Kind : int { kSymmetric, kRound, kUpdate };
 
 struct Shape {                                             // the matrices of one shape, in one product
-  CUtensorMap a, b;
+  CUtensorMap a, b, c;                                     // operands and result
   int kind;
   float by, add_by, diagonal;                              // result = by * sum + add_by * add + diagonal (on the diagonal)
   uint32_t m, n, k;
@@ -213,7 +215,7 @@ struct Place {
   uint32_t shape, z;
   int m0, n0;
 };
-// The launch's tile t.  A symmetric product has the tiles that reach above the diagonal, row by row; else 16 tile rows walk the columns
+// The launch's tile t, of 128 x BN.  A symmetric product has the tiles that reach above the diagonal, row by row; else 16 tile rows walk the columns
 // together and share their operands in L2.
 template <int BN>
 __device__ __forceinline__ Place place_of(const Product& p, uint32_t t) {
@@ -228,8 +230,7 @@ __device__ __forceinline__ Place place_of(const Product& p, uint32_t t) {
     uint32_t i = 0, skip = 0;
     while (t >= s.tiles_n - skip) {
       t -= s.tiles_n - skip;
-      ++i;
-      skip = i * BM / BN;
+      skip = ++i * BM / BN;
     }
     at.m0 = (int)(i * BM);
     at.n0 = (int)((skip + t) * BN);
@@ -247,7 +248,17 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       "r"(x), "r"(y), "r"(z), "r"(w)
       : "memory");
 }
-__device__ __forceinline__ void tc_mma_f16(uint32_t d_tmem, Operand a, uint32_t a_units, Operand b, uint32_t b_units, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void store_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(src), "r"(x), "r"(y), "r"(z) : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+template <int GROUPS>
+__device__ __forceinline__ void stores_read() {            // all but the last GROUPS stores have read their shared memory
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(GROUPS) : "memory");
+}
+__device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, Operand a, uint32_t a_units, Operand b, uint32_t b_units, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
       "mov.b64 da, {%1, %2};\n\t"
@@ -257,32 +268,23 @@ __device__ __forceinline__ void tc_mma_f16(uint32_t d_tmem, Operand a, uint32_t 
       "r"(a.lo + a_units), "r"(a.hi), "r"(b.lo + b_units), "r"(b.hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// fp32 sums of fp16 operands (format 0 of both).
+// fp32 sums of fp16 operands (format 0 of both), 128 x n.
 __device__ __forceinline__ uint32_t f16_idesc(int n, int a_mn, int b_mn) {
   return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
 }
-__device__ __forceinline__ void st_v8(void* dst, const uint32_t* r) { st_global_v8(static_cast<float*>(dst), r); }
 __device__ __forceinline__ Target target_of(const Product& p, const Shape& q, const Place& at) {
   return q.kind == kUpdate ? p.targets[q.first_target + at.z] : Target{};
 }
 
-__device__ __forceinline__ bool aligned_weights(const Shape& q, const Target& t) { return (q.n & 3) == 0 && (reinterpret_cast<uintptr_t>(t.weights) & 15) == 0; }
-// What 16 columns of a row need besides their sums: both planes of what is added, or the weights where they lie on 16 bytes.  Loaded ahead of use, since no load
-// moves before a store by itself.
+// Both planes of 16 columns of what is added to a product.  Loaded ahead of use, since no load moves before a store by itself.
 struct Beside {
   uint4 v[4];
 };
-__device__ __forceinline__ Beside beside16(const Shape& q, const Place& at, const Target& target, uint32_t row, uint32_t c0) {
+__device__ __forceinline__ Beside beside16(const Shape& q, const Place& at, uint32_t row, uint32_t c0) {
   Beside b = {};
-  if (row >= q.m || c0 >= q.n) return b;
-  if (q.add && (c0 | 31u) >= (row & ~31u)) {
-    const uint4* const add = reinterpret_cast<const uint4*>(q.add + 2 * at.z * q.plane + (uint64_t)row * q.pitch + c0);
-    b.v[0] = add[0], b.v[1] = add[1], b.v[2] = add[q.plane / 8], b.v[3] = add[q.plane / 8 + 1];
-  } else if (q.kind == kUpdate && aligned_weights(q, target) && c0 + 16 <= q.n) {
-    const uint4* const w = reinterpret_cast<const uint4*>(target.weights + (uint64_t)row * q.n + c0);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) b.v[j] = w[j];
-  }
+  if (!q.add || row >= q.m || c0 >= q.n || (c0 | 31u) < (row & ~31u)) return b;
+  const uint4* const add = reinterpret_cast<const uint4*>(q.add + 2 * at.z * q.plane + (uint64_t)row * q.pitch + c0);
+  b.v[0] = add[0], b.v[1] = add[1], b.v[2] = add[q.plane / 8], b.v[3] = add[q.plane / 8 + 1];
   return b;
 }
 // The result's 16 columns from c0 on of a row, from their sums: by * sum + add_by * add + diagonal.
@@ -303,7 +305,7 @@ __device__ __forceinline__ void complete(const Shape& q, uint32_t row, uint32_t 
   }
 }
 // 16 neighbours as pairs, two of them to each word of `hi` and `lo`.
-__device__ __forceinline__ void split16(const uint32_t* v, uint32_t (&hi)[8], uint32_t (&lo)[8]) {
+__device__ __forceinline__ void split16(const uint32_t* v, uint32_t* hi, uint32_t* lo) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float a = __uint_as_float(v[2 * j]), b = __uint_as_float(v[2 * j + 1]);
@@ -313,108 +315,114 @@ __device__ __forceinline__ void split16(const uint32_t* v, uint32_t (&hi)[8], ui
     hi[j] = *reinterpret_cast<const uint32_t*>(&h), lo[j] = *reinterpret_cast<const uint32_t*>(&l);
   }
 }
-__device__ __forceinline__ void store16(const Shape& q, __half* matrix, uint64_t row, uint32_t col, const uint32_t (&hi)[8], const uint32_t (&lo)[8]) {
-  __half* const out = matrix + row * q.pitch + col;        // (columns behind the last one lie in the row's padding)
-  st_v8(out, hi);
-  st_v8(out + q.plane, lo);
-}
-// w <- w * keep - rate * X for 16 columns of a row.
-__device__ __forceinline__ void update16(const Shape& q, const Target& target, float keep, float rate, uint32_t row, uint32_t c0, const Beside& beside, const uint32_t* v) {
-  float* const w = target.weights + (uint64_t)row * q.n + c0;
-  if (row >= q.m) return;
-  if (aligned_weights(q, target) && c0 + 16 <= q.n) {
-    const float* const old = reinterpret_cast<const float*>(beside.v);
-#pragma unroll
-    for (int j = 0; j < 16; j += 4)
-      *reinterpret_cast<float4*>(w + j) = make_float4(old[j] * keep - rate * __uint_as_float(v[j]), old[j + 1] * keep - rate * __uint_as_float(v[j + 1]),
-                                                      old[j + 2] * keep - rate * __uint_as_float(v[j + 2]), old[j + 3] * keep - rate * __uint_as_float(v[j + 3]));
-  } else {
-    float x[16];                                           // (all loads before the first store, which might change what they read)
-#pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] = c0 + j < q.n ? w[j] : 0.f;
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (c0 + j < q.n) w[j] = x[j] * keep - rate * __uint_as_float(v[j]);
-  }
-}
 
-// Writes 32 rows from r0 on (one to each lane) and COLS columns from c0 on, whose sums are in `v`; `beside` belongs to the first 16 of them.  What has to be turned over
-// goes through `turn`, 32 rows of 33 words of this warp's own: the mirror image of a symmetric matrix's block, so that it is written in rows too, and unaligned weights.
-template <int COLS>
+// Writes 32 rows from r0 on (one to each lane) and COLS columns from c0 on, whose sums are in `v`; `beside` belongs to the first 16 of them.  Blocks of 32 x 32 go
+// through SLOTS places in shared memory of this warp's own by turns (64-byte rows in the 64-byte swizzle, hi behind lo) and leave them by TMA, for a symmetric
+// product the mirror image too: with a lane's own stores, 32 rows of 32 bytes to an instruction, the epilogue took 12 us a tile.  Weights are turned over
+// there, so that the warp reads and writes 32 neighbours.  `stores`: how many have left so far.
+template <int COLS, int SLOTS>
 __device__ __forceinline__ void finish(const Shape& q, const Place& at, const Target& target, float lr, uint32_t r0, uint32_t c0, int lane, uint32_t (&v)[COLS], Beside beside,
-                                       uint32_t* turn) {
+                                       uint8_t* place, uint32_t& stores) {
   const uint32_t row = r0 + lane;
-  const float keep = 1.f - lr * target.decay, rate = q.by * lr * target.scale;
-  __half* const matrix = q.out + 2 * at.z * q.plane;
+  auto send = [&](int x, int y, auto write) {
+    uint8_t* const slot = place + (SLOTS == 1 ? 0 : (stores & 1) * kSlotBytes);
+    if (lane == 0) stores_read<SLOTS - 1>();
+    __syncwarp();
+    write(slot);
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) store_3d(&q.c, smem_u32(slot), x, y, (int)(2 * at.z));
+    ++stores;
+  };
 #pragma unroll
   for (int part = 0; part < COLS / 32; ++part) {           // blocks of 32 columns
     const uint32_t block = c0 + 32 * part;
     uint32_t* const x = v + 32 * part;
     if (block >= q.n || r0 >= q.m) return;
-    const bool mirror = q.kind == kSymmetric && block > r0;
-    const bool turned = mirror || (q.kind == kUpdate && !(aligned_weights(q, target) && block + 32 <= q.n));
-    if (turned) __syncwarp();
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const uint32_t col = block + 16 * half;
-      const Beside now = beside;
-      if (32 * part + 16 * half + 16 < COLS) beside = beside16(q, at, target, row, col + 16);
-      if (q.kind == kSymmetric && block < r0) continue;    // below the diagonal: written by the block above it
-      if (q.kind == kUpdate) {
-        if (!turned) update16(q, target, keep, rate, row, col, now, x + 16 * half);
-        else
-#pragma unroll
-          for (int j = 0; j < 16; ++j) turn[lane * 33 + 16 * half + j] = x[16 * half + j];
-        continue;
-      }
-      uint32_t hi[8], lo[8];
-      complete(q, row, col, now, x + 16 * half);
-      split16(x + 16 * half, hi, lo);
-      if (row < q.m) store16(q, matrix, row, col, hi, lo);
-      if (mirror)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {                      // a pair to a word
-          turn[lane * 33 + 16 * half + 2 * j] = __byte_perm(hi[j], lo[j], 0x5410);
-          turn[lane * 33 + 16 * half + 2 * j + 1] = __byte_perm(hi[j], lo[j], 0x7632);
-        }
-    }
-    if (!turned) continue;
-    __syncwarp();
-    if (block + lane >= q.n) continue;                     // (a lane is a column now)
-    if (mirror) {
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t hi[8], lo[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t a = turn[(16 * half + 2 * j) * 33 + lane], b = turn[(16 * half + 2 * j + 1) * 33 + lane];
-          hi[j] = __byte_perm(a, b, 0x5410), lo[j] = __byte_perm(a, b, 0x7632);
-        }
-        store16(q, matrix, block + lane, r0 + 16 * half, hi, lo);
-      }
-    } else {
+    if (q.kind == kUpdate) {
+      const float keep = 1.f - lr * target.decay, rate = q.by * lr * target.scale;
+      uint32_t* const turn = reinterpret_cast<uint32_t*>(place);
       float* const w = target.weights + (uint64_t)r0 * q.n + block + lane;
+      const bool live = block + lane < q.n;                // (a lane is a column here)
       float old[32];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) old[i] = r0 + i < q.m ? w[(uint64_t)i * q.n] : 0.f;
+      for (int i = 0; i < 32; ++i) old[i] = live && r0 + i < q.m ? w[(uint64_t)i * q.n] : 0.f;
+      if (lane == 0) stores_read<0>();
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) turn[lane * 32 + (j ^ lane)] = x[j];
+      __syncwarp();
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        if (r0 + i < q.m) w[(uint64_t)i * q.n] = old[i] * keep - rate * __uint_as_float(turn[i * 33 + lane]);
+        if (live && r0 + i < q.m) w[(uint64_t)i * q.n] = old[i] * keep - rate * __uint_as_float(turn[i * 32 + (lane ^ i)]);
+      __syncwarp();
+      continue;
     }
+    const bool below = q.kind == kSymmetric && block < r0; // written by the block above the diagonal
+    uint32_t hi[16], lo[16];                               // two columns to a word
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const Beside now = beside;
+      if (32 * part + 16 * half + 16 < COLS) beside = beside16(q, at, row, block + 16 * half + 16);
+      if (below) continue;
+      complete(q, row, block + 16 * half, now, x + 16 * half);
+      split16(x + 16 * half, hi + 8 * half, lo + 8 * half);
+    }
+    if (below) continue;
+    send((int)block, (int)r0, [&](uint8_t* slot) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint8_t* const at16 = slot + lane * 64 + (j ^ (lane >> 1 & 3)) * 16;
+        *reinterpret_cast<uint4*>(at16) = make_uint4(hi[4 * j], hi[4 * j + 1], hi[4 * j + 2], hi[4 * j + 3]);
+        *reinterpret_cast<uint4*>(at16 + kSlotBytes / 2) = make_uint4(lo[4 * j], lo[4 * j + 1], lo[4 * j + 2], lo[4 * j + 3]);
+      }
+    });
+    if (q.kind == kSymmetric && block > r0)                // its mirror image: a column of the block is a row there
+      send((int)r0, (int)block, [&](uint8_t* slot) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          uint8_t* const at2 = slot + c * 64 + ((lane >> 3) ^ (c >> 1 & 3)) * 16 + (lane & 7) * 2;
+          *reinterpret_cast<uint16_t*>(at2) = (uint16_t)(hi[c / 2] >> (c & 1) * 16);
+          *reinterpret_cast<uint16_t*>(at2 + kSlotBytes / 2) = (uint16_t)(lo[c / 2] >> (c & 1) * 16);
+        }
+      });
   }
 }
-// The same for 16 columns, of which clusters' CTAs have few: without the detour.
+// 16 columns of a row, of which the CTAs of a cluster that shares a tile have few: straight to memory.
 __device__ __forceinline__ void finish16(const Shape& q, const Place& at, const Target& target, float lr, uint32_t r0, uint32_t c0, int lane, uint32_t (&v)[16]) {
   const uint32_t row = r0 + lane, block = c0 & ~31u;
   if (c0 >= q.n || r0 >= q.m) return;
   if (q.kind == kSymmetric && block < r0) return;
-  const Beside beside = beside16(q, at, target, row, c0);
-  if (q.kind == kUpdate) return update16(q, target, 1.f - lr * target.decay, q.by * lr * target.scale, row, c0, beside, v);
+  if (q.kind == kUpdate) {
+    const float keep = 1.f - lr * target.decay, rate = q.by * lr * target.scale;
+    float* const w = target.weights + (uint64_t)row * q.n + c0;
+    if (row >= q.m) return;
+    float x[16];                                           // (all loads before the first store, which might change what they read)
+    if ((q.n & 3) == 0 && (reinterpret_cast<uintptr_t>(target.weights) & 15) == 0 && c0 + 16 <= q.n) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(x + 4 * j) = reinterpret_cast<const float4*>(w)[j];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = x[j] * keep - rate * __uint_as_float(v[j]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) reinterpret_cast<float4*>(w)[j] = *reinterpret_cast<const float4*>(x + 4 * j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = c0 + j < q.n ? w[j] : 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (c0 + j < q.n) w[j] = x[j] * keep - rate * __uint_as_float(v[j]);
+    }
+    return;
+  }
   __half* const matrix = q.out + 2 * at.z * q.plane;
   uint32_t hi[8], lo[8];
-  complete(q, row, c0, beside, v);
+  complete(q, row, c0, beside16(q, at, row, c0), v);
   split16(v, hi, lo);
-  if (row < q.m) store16(q, matrix, row, c0, hi, lo);
+  if (row < q.m) {                                         // (columns behind the last one lie in the row's padding)
+    float* const out = reinterpret_cast<float*>(matrix + (uint64_t)row * q.pitch + c0);
+    st_global_v8(out, hi);
+    st_global_v8(out + q.plane / 2, lo);
+  }
   if (q.kind == kSymmetric && block > r0) {                // its mirror image: a column of the block is a row there, 32 lanes side by side
     unsigned short* const mirror = reinterpret_cast<unsigned short*>(matrix) + (uint64_t)c0 * q.pitch + row;
 #pragma unroll
@@ -427,8 +435,9 @@ __device__ __forceinline__ void finish16(const Shape& q, const Place& at, const 
   }
 }
 
-// One CTA per SM walks 128 x BN tiles; or, SPLIT, where there are too few tiles to go round, a cluster of up to eight CTAs has one tile, each CTA
-// a share of its slabs, and they add their sums through shared memory, each a part of the tile.
+// One CTA per SM walks tiles of 128 x BN; or, SPLIT, where there are too few tiles to go round, a cluster of up to eight CTAs has one, each CTA a share of its
+// slabs, and they add their sums through shared memory, each a part of the tile.  (Pairs of CTAs on tiles of 256 x 256, which fetch a third less, were slower:
+// 4096 x 16384 10.2 ms for 8.5.  A slab of 128 x 256 x 32 takes 0.58 us, which is what the library's largest products of this type take.)
 //   warp 0     TMA: both planes of a slab of 32 k of each operand, one instruction each.  An operand that is contiguous along k is K-major
 //              (rows of 64 bytes in the 64-byte swizzle), else MN-major (chunks of 64 columns, 128-byte swizzle, a row per k).
 //   warp 1     tcgen05.mma: per 16 k  hi hi, lo hi, hi lo, into two accumulators in tensor memory by turns, each for kRun slabs.
@@ -445,12 +454,12 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
-  const uint32_t bar_base = smem_base + C::kTileBytes;
+  const uint32_t bar_base = smem_base + C::kTileBytes + C::kTurnBytes;
   auto full = [&](int s) { return bar_base + 8u * s; };
   auto empty = [&](int s) { return bar_base + 8u * (S + s); };
   auto acc_full = [&](int a) { return bar_base + 8u * (2 * S + a); };
   auto acc_empty = [&](int a) { return bar_base + 8u * (2 * S + 2 + a); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + C::kTileBytes + 8 * (2 * S + 4));
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + C::kTileBytes + C::kTurnBytes + 8 * (2 * S + 4));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = uniform_warp();
   const int lane = threadIdx.x & 31;
@@ -469,10 +478,15 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   pdl_enter();
-  const uint32_t splits = SPLIT ? p.splits : 1, rank = SPLIT ? cluster_rank() : 0;
+  const uint32_t rank = SPLIT ? cluster_rank() : 0, splits = SPLIT ? p.splits : 1;
   const uint32_t first = SPLIT ? blockIdx.x / splits : blockIdx.x, step = SPLIT ? p.tiles : gridDim.x;
-  auto slabs_of = [&](const Shape& q, int* end) {            // this CTA's
-    const int slabs = (int)((q.k + BK - 1) / BK), each = (slabs + (int)splits - 1) / (int)splits;
+  auto slabs_of = [&](const Shape& q, int* end) {          // the CTA's
+    const int slabs = (int)((q.k + BK - 1) / BK);
+    if (!SPLIT) {
+      *end = slabs;
+      return 0;
+    }
+    const int each = (slabs + (int)splits - 1) / (int)splits;
     *end = min(slabs, (int)(rank + 1) * each);
     return min(slabs, (int)rank * each);
   };
@@ -481,16 +495,16 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
   if (warp >= 4) {
     if constexpr (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
     const int quarter = warp & 3, half = (warp - 4) >> 2;
-    uint32_t run = 0;
+    uint8_t* const place = smem_gen + C::kTileBytes + (warp - 4) * C::kWarpBytes;
+    uint32_t run = 0, stores = 0;
     bool ok = true;
     for (uint32_t t = first; ok && t < p.tiles; t += step) {
       const Place at = place_of<BN>(p, t);
       const Shape& q = p.s[at.shape];
       const uint32_t r0 = (uint32_t)at.m0 + quarter * 32, c0 = (uint32_t)at.n0 + half * (BN / 2);
-      uint32_t sum[BN / 2];                                // this thread's row of its half of the tile, as bits of floats
+      uint32_t sum[BN / 2];                              // this thread's row of its half of the tile, as bits of floats
       int end;
       const int begin = slabs_of(q, &end), runs = (end - begin + kRun - 1) / kRun;
-      const Target target = target_of(p, q, at);
       Beside beside = {};
       if (SPLIT && runs == 0) {
 #pragma unroll
@@ -498,7 +512,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
       }
       for (int i = 0; i < runs; ++i, ++run) {
         const uint32_t as = run & 1u;
-        if (!SPLIT && i + 1 == runs) beside = beside16(q, at, target, r0 + lane, c0);
+        if (!SPLIT && i + 1 == runs) beside = beside16(q, at, r0 + lane, c0);
         ok = mbar_wait(acc_full(as), (run >> 1) & 1u, abort_flag, p.status, 704, p.wait_ns);
         if (!ok) break;
         tc_fence_after();
@@ -528,81 +542,81 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
 #pragma unroll
         for (int j = 0; j < BN / 2; ++j) shared[(half * (BN / 2) + j) * BM + quarter * 32 + lane] = __uint_as_float(sum[j]);
       } else {
-        uint32_t* const turn = reinterpret_cast<uint32_t*>(smem_gen + C::kTileBytes + 256) + (warp - 4) * (32 * 33);
-        finish(q, at, target, lr, r0, c0, lane, sum, beside, turn);
+        finish<BN / 2, C::kSlots>(q, at, target_of(p, q, at), lr, r0, c0, lane, sum, beside, place, stores);
         __syncwarp();
       }
     }
+    if (!SPLIT && lane == 0) stores_done();
   } else {
     if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
-  if (warp == 0) {
-    const bool leader = elect_one();
-    int s = 0;
-    uint32_t ph = 1;
-    bool ok = true;
-    for (uint32_t t = first; ok && t < p.tiles; t += step) {
-      const Place at = place_of<BN>(p, t);
-      const Shape& q = p.s[at.shape];
-      const int plane = (int)(2 * at.z);
-      int end;
-      for (int kb = slabs_of(q, &end); kb < end; ++kb) {
-        if (!mbar_wait(empty(s), ph, abort_flag, p.status, 701, p.wait_ns)) { ok = false; break; }
-        if (leader) {
-          const uint32_t stage = smem_base + s * C::kStageBytes;
-          mbar_expect_tx(full(s), C::kStageBytes);
-          if (q.a_mn) tma_load_4d(stage, &q.a, full(s), 0, kb * BK, at.m0 / 64, plane);
-          else tma_load_3d(stage, &q.a, full(s), kb * BK, at.m0, plane);
-          if (q.b_mn) tma_load_4d(stage + 2 * C::kAPlane, &q.b, full(s), 0, kb * BK, at.n0 / 64, plane);
-          else tma_load_3d(stage + 2 * C::kAPlane, &q.b, full(s), kb * BK, at.n0, plane);
-        }
-        if (++s == S) s = 0, ph ^= 1;
-      }
-    }
-  } else if (warp == 1) {
-    const bool leader = elect_one();
-    int s = 0;
-    uint32_t ph = 0, run = 0;
-    bool ok = true;
-    for (uint32_t t = first; ok && t < p.tiles; t += step) {
-      const Place at = place_of<BN>(p, t);
-      const Shape& q = p.s[at.shape];
-      // where the left half of a symmetric product's tile lies below the diagonal, the right half alone: 128 rows or two chunks further
-      const uint32_t left_out = BN == 256 && q.kind == kSymmetric && at.m0 == at.n0 + 128 ? 128 : 0;
-      const uint32_t idesc = f16_idesc(BN - left_out, q.a_mn, q.b_mn);
-      // K-major: 64-byte swizzle (layout 4), groups of 8 rows 512 bytes apart, 16 k 32 bytes on.  MN-major: 128-byte swizzle (layout 2), chunks
-      // of 64 columns BK rows apart, groups of 8 k 1024 bytes, 16 k 2048 bytes on.
-      const Operand a_op = q.a_mn ? make_desc(0, BK * 128, 1024, 2) : make_desc(0, 16, 512, 4);
-      const Operand b_op = q.b_mn ? make_desc(0, BK * 128, 1024, 2) : make_desc(0, 16, 512, 4);
-      const uint32_t a_step = (q.a_mn ? 2048u : 32u) >> 4, b_step = (q.b_mn ? 2048u : 32u) >> 4;
-      int slabs;
-      for (int kb = slabs_of(q, &slabs); kb < slabs; ++run) {
-        const uint32_t as = run & 1u, acc = tmem_base + as * BN + left_out;
-        ok = mbar_wait(acc_empty(as), ((run >> 1) & 1u) ^ 1u, abort_flag, p.status, 702, p.wait_ns);
-        if (!ok) break;
-        tc_fence_after();
-        const int end = min(kb + kRun, slabs);             // of the run
-        for (uint32_t more = 0; kb < end; ++kb, more = 1) {
-          ok = mbar_wait(full(s), ph, abort_flag, p.status, 703, p.wait_ns);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t a_hi = ((smem_base & 0x3FFFFu) + s * C::kStageBytes) >> 4, a_lo = a_hi + (C::kAPlane >> 4);
-          const uint32_t b_hi = a_lo + (C::kAPlane >> 4) + left_out * (BK * 2) / 16, b_lo = b_hi + (C::kBPlane >> 4);
+    if (warp == 0) {
+      const bool leader = elect_one();
+      int s = 0;
+      uint32_t ph = 1;
+      bool ok = true;
+      for (uint32_t t = first; ok && t < p.tiles; t += step) {
+        const Place at = place_of<BN>(p, t);
+        const Shape& q = p.s[at.shape];
+        const int plane = (int)(2 * at.z);
+        int end;
+        for (int kb = slabs_of(q, &end); kb < end; ++kb) {
+          if (!mbar_wait(empty(s), ph, abort_flag, p.status, 701, p.wait_ns)) { ok = false; break; }
           if (leader) {
-#pragma unroll
-            for (int kk = 0; kk < BK / 16; ++kk) {
-              tc_mma_f16(acc, a_op, a_hi + kk * a_step, b_op, b_hi + kk * b_step, idesc, kk ? 1u : more);
-              tc_mma_f16(acc, a_op, a_lo + kk * a_step, b_op, b_hi + kk * b_step, idesc, 1u);
-              tc_mma_f16(acc, a_op, a_hi + kk * a_step, b_op, b_lo + kk * b_step, idesc, 1u);
-            }
-            tc_commit(empty(s));
+            const uint32_t stage = smem_base + s * C::kStageBytes;
+            mbar_expect_tx(full(s), C::kStageBytes);
+            if (q.a_mn) tma_load_4d(stage, &q.a, full(s), 0, kb * BK, at.m0 / 64, plane);
+            else tma_load_3d(stage, &q.a, full(s), kb * BK, at.m0, plane);
+            if (q.b_mn) tma_load_4d(stage + 2 * C::kAPlane, &q.b, full(s), 0, kb * BK, at.n0 / 64, plane);
+            else tma_load_3d(stage + 2 * C::kAPlane, &q.b, full(s), kb * BK, at.n0, plane);
           }
           if (++s == S) s = 0, ph ^= 1;
         }
-        if (!ok) break;
-        if (leader) tc_commit(acc_full(as));
+      }
+    } else if (warp == 1) {
+      const bool leader = elect_one();
+      int s = 0;
+      uint32_t ph = 0, run = 0;
+      bool ok = true;
+      for (uint32_t t = first; ok && t < p.tiles; t += step) {
+        const Place at = place_of<BN>(p, t);
+        const Shape& q = p.s[at.shape];
+        // where the left half of a symmetric product's tile lies below the diagonal, the right half alone: 128 rows or two chunks further
+        const uint32_t left_out = BN == 256 && q.kind == kSymmetric && at.m0 == at.n0 + 128 ? 128 : 0;
+        const uint32_t idesc = f16_idesc(BN - left_out, q.a_mn, q.b_mn);
+        // K-major: 64-byte swizzle (layout 4), groups of 8 rows 512 bytes apart, 16 k 32 bytes on.  MN-major: 128-byte swizzle (layout 2), chunks
+        // of 64 columns BK rows apart, groups of 8 k 1024 bytes, 16 k 2048 bytes on.
+        const Operand a_op = q.a_mn ? make_desc(0, BK * 128, 1024, 2) : make_desc(0, 16, 512, 4);
+        const Operand b_op = q.b_mn ? make_desc(0, BK * 128, 1024, 2) : make_desc(0, 16, 512, 4);
+        const uint32_t a_step = (q.a_mn ? 2048u : 32u) >> 4, b_step = (q.b_mn ? 2048u : 32u) >> 4;
+        int slabs;
+        for (int kb = slabs_of(q, &slabs); kb < slabs; ++run) {
+          const uint32_t as = run & 1u, acc = tmem_base + as * BN + left_out;
+          ok = mbar_wait(acc_empty(as), ((run >> 1) & 1u) ^ 1u, abort_flag, p.status, 702, p.wait_ns);
+          if (!ok) break;
+          tc_fence_after();
+          const int end = min(kb + kRun, slabs);           // of the run
+          for (uint32_t more = 0; kb < end; ++kb, more = 1) {
+            ok = mbar_wait(full(s), ph, abort_flag, p.status, 703, p.wait_ns);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t a_hi = ((smem_base & 0x3FFFFu) + s * C::kStageBytes) >> 4, a_lo = a_hi + (C::kAPlane >> 4);
+            const uint32_t b_hi = a_lo + (C::kAPlane >> 4) + left_out * (BK * 2) / 16, b_lo = b_hi + (C::kBPlane >> 4);
+            if (leader) {
+#pragma unroll
+              for (int kk = 0; kk < BK / 16; ++kk) {
+                mma_f16(acc, a_op, a_hi + kk * a_step, b_op, b_hi + kk * b_step, idesc, kk ? 1u : more);
+                mma_f16(acc, a_op, a_lo + kk * a_step, b_op, b_hi + kk * b_step, idesc, 1u);
+                mma_f16(acc, a_op, a_hi + kk * a_step, b_op, b_lo + kk * b_step, idesc, 1u);
+              }
+              tc_commit(empty(s));
+            }
+            if (++s == S) s = 0, ph ^= 1;
+          }
+          if (!ok) break;
+          if (leader) tc_commit(acc_full(as));
+        }
       }
     }
-  }
   }
 
   tc_fence_before();
@@ -615,7 +629,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
       const Shape& q = p.s[at.shape];
       const Target target = target_of(p, q, at);
       const float* const shared = reinterpret_cast<const float*>(smem_gen);
-      // pieces of 32 rows and 16 columns: those of a block of 32 x 32 need not be written by one warp, as each writes its own columns
+      // pieces of 32 rows and 16 columns
       for (uint32_t piece = rank * kEpilogueWarps + warp - 4; piece < 4 * BN / 16; piece += splits * kEpilogueWarps) {
         const uint32_t quarter = piece & 3, c = piece / 4 * 16;
         uint32_t v[16];
@@ -629,14 +643,17 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
       }
     }
     __syncthreads();
-    cluster_arrive();                                      // (no CTA leaves while another one reads its shared memory)
-    cluster_wait();
   }
   if (*abort_flag) {
-    // let copies and products in flight finish before the tensor memory goes away
+    // let copies and products in flight finish before the memory that they use goes away
     const long long t0 = clock64();
     while (clock64() - t0 < 2000000ll) { }
     __syncthreads();
+  }
+  if constexpr (SPLIT) {
+    __syncthreads();
+    cluster_arrive();                                      // (no CTA leaves while another one reads its shared memory)
+    cluster_wait();
   }
   if (warp == 1) {
     tc_fence_after();
@@ -785,9 +802,9 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
   };
   auto three = [&](uint32_t acc, Operand a, uint32_t a_hi, uint32_t a_lo, Operand b, uint32_t b_hi, uint32_t b_lo, uint32_t idesc, uint32_t more) {
     if (!leader) return;
-    tc_mma_f16(acc, a, a_hi, b, b_hi, idesc, more);
-    tc_mma_f16(acc, a, a_lo, b, b_hi, idesc, 1u);
-    tc_mma_f16(acc, a, a_hi, b, b_lo, idesc, 1u);
+    mma_f16(acc, a, a_hi, b, b_hi, idesc, more);
+    mma_f16(acc, a, a_lo, b, b_hi, idesc, 1u);
+    mma_f16(acc, a, a_hi, b, b_lo, idesc, 1u);
   };
   auto k_offset = [&](uint32_t k16) { return (k16 / 4 * chunk + k16 % 4 * 32) >> 4; };
   // 16 columns of this thread's row as pairs
@@ -924,7 +941,8 @@ EncodeTiled encode_tiled() {
   return fn;
 }
 
-// `planes` matrices of fp16 [rows][cols], rows `pitch` (a multiple of 64) apart.  MN-major boxes are chunks of 64 columns: the last one may
+// `planes` matrices of fp16 [rows][cols], rows `pitch` (a multiple of 64) apart, as an operand, in boxes of `tile` rows or columns and BK k, or as
+// a result, in blocks of 32 x 32.  MN-major boxes are chunks of 64 columns: the last one may
 // reach into a row's padding, whose values end in rows or columns of a product that nobody reads.
 int make_map(CUtensorMap* map, const __half* base, uint64_t rows, uint64_t cols, uint64_t pitch, uint64_t planes, bool mn, uint32_t tile) {
   EncodeTiled encode = encode_tiled();
@@ -938,7 +956,7 @@ int make_map(CUtensorMap* map, const __half* base, uint64_t rows, uint64_t cols,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   } else {
     const cuuint64_t dims[3] = {cols, rows, planes}, strides[2] = {pitch * 2, rows * pitch * 2};
-    const cuuint32_t box[3] = {BK, tile, 2};
+    const cuuint32_t box[3] = {BK, tile, 2};               // (a result's blocks are 32 columns wide as well)
     r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(base), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   }
@@ -1086,14 +1104,14 @@ struct Extent {
   uint64_t m, n, k, count;
   bool symmetric;
 };
-// The way whose busiest SM is done first.  A slab takes 0.42 us with tiles of 256 columns and 0.25 with tiles of 128, what stands around a tile 5 and 4 us (and with
-// a cluster, which adds its sums, 1.5 more).  Clusters of four or eight leave some SMs out.
+// The way whose busiest SM is done first.  A slab takes 0.58 us with tiles of 256 columns and 0.3 with tiles of 128, what stands around a tile 5 and 4 us (and with
+// a cluster that shares one, and adds its sums, 1.5 more).  Clusters of four or eight leave some SMs out.
 Way way_of(const std::vector<Extent>& e) {
   Way best = {256, 1};
   double least = 0;
   for (const Way w : {Way{256, 1}, Way{128, 1}, Way{128, 2}, Way{128, 4}, Way{128, 8}}) {
     const uint64_t sms = w.splits == 1 ? (uint64_t)sm_count() : w.splits == 2 ? 146 : w.splits == 4 ? 136 : 128;
-    const double slab = w.bn == 256 ? 0.42 : 0.25, around = w.bn == 256 ? 5.0 : w.splits == 1 ? 4.0 : 5.5;
+    const double slab = w.bn == 256 ? 0.58 : 0.3, around = w.bn == 256 ? 5.0 : w.splits == 1 ? 4.0 : 5.5;
     double us = 0;
     uint64_t before = 0, next = 0;                         // tiles passed, and the next one of the first SM
     for (const Extent& x : e) {
@@ -1122,10 +1140,8 @@ int launch_product(const std::vector<Kin>& kin, const std::vector<std::pair<size
       const bool wide = q.rows <= q.cols, square = op.what != Operation::kMove;
       Shape& s = p.s[p.shapes];
       int rc = POLAR_B200_OK;
-      auto x = [&](CUtensorMap* map, bool mn, uint32_t tile) { return make_map(map, q.x[from], q.rows, q.cols, q.pitch, 2 * q.count, mn, tile); };
-      auto symmetric = [&](CUtensorMap* map, int t, uint32_t tile) {
-        return make_map(map, q.s[t], q.side, q.side, q.side_pitch, 2 * q.count, false, tile);
-      };
+      auto x = [&](CUtensorMap* map, int which, bool mn, uint32_t tile) { return make_map(map, q.x[which], q.rows, q.cols, q.pitch, 2 * q.count, mn, tile); };
+      auto symmetric = [&](CUtensorMap* map, int t, uint32_t tile) { return make_map(map, q.s[t], q.side, q.side, q.side_pitch, 2 * q.count, false, tile); };
       s.kind = square ? kSymmetric : op.last ? kUpdate : kRound;
       s.by = op.by, s.add_by = op.add_by, s.diagonal = op.diagonal;
       s.add = op.add >= 0 ? q.s[op.add] : nullptr;
@@ -1133,8 +1149,8 @@ int launch_product(const std::vector<Kin>& kin, const std::vector<std::pair<size
       if (op.what == Operation::kGram) {                   // X X^T, or X^T X
         s.m = s.n = (uint32_t)q.side, s.k = (uint32_t)std::max(q.rows, q.cols);
         s.a_mn = s.b_mn = !wide;
-        rc = x(&s.a, !wide, BM);
-        if (!rc) rc = x(&s.b, !wide, BN);
+        rc = x(&s.a, from, !wide, BM);
+        if (!rc) rc = x(&s.b, from, !wide, BN);
       } else if (op.what == Operation::kProduct) {
         s.m = s.n = s.k = (uint32_t)q.side;
         rc = symmetric(&s.a, op.left, BM);
@@ -1142,9 +1158,10 @@ int launch_product(const std::vector<Kin>& kin, const std::vector<std::pair<size
       } else {                                             // P X, or X P
         s.m = (uint32_t)q.rows, s.n = (uint32_t)q.cols, s.k = (uint32_t)q.side;
         s.b_mn = wide;
-        rc = wide ? symmetric(&s.a, op.left, BM) : x(&s.a, false, BM);
-        if (!rc) rc = wide ? x(&s.b, true, BN) : symmetric(&s.b, op.left, BN);
+        rc = wide ? symmetric(&s.a, op.left, BM) : x(&s.a, from, false, BM);
+        if (!rc) rc = wide ? x(&s.b, from, true, BN) : symmetric(&s.b, op.left, BN);
       }
+      if (!rc && !SPLIT && !op.last) rc = square ? symmetric(&s.c, op.out, 32) : x(&s.c, from ^ 1, false, 32);
       if (rc) return rc;
       s.out = square ? q.s[op.out] : q.x[from ^ 1];
       s.pitch = (uint32_t)(square ? q.side_pitch : q.pitch);
@@ -1159,7 +1176,7 @@ int launch_product(const std::vector<Kin>& kin, const std::vector<std::pair<size
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3(SPLIT ? p.tiles * splits : std::min(p.tiles, (uint32_t)sm_count()));
     c.blockDim = dim3(kProductThreads);
-    c.dynamicSmemBytes = Cfg<BN>::kSmemBytes;
+    c.dynamicSmemBytes = Cfg<BN>::kBytes;
     c.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1169,7 +1186,7 @@ int launch_product(const std::vector<Kin>& kin, const std::vector<std::pair<size
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     c.attrs = at;
     c.numAttrs = SPLIT ? 2 : 1;
-    cudaError_t e = cudaFuncSetAttribute(product_kernel<BN, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<BN>::kSmemBytes);
+    cudaError_t e = cudaFuncSetAttribute(product_kernel<BN, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<BN>::kBytes);
     void* args[1] = {&p};
     if (e == cudaSuccess) e = cudaLaunchKernelExC(&c, reinterpret_cast<const void*>(product_kernel<BN, SPLIT>), args);
     if (e != cudaSuccess) {
@@ -1278,7 +1295,7 @@ int run_group(const std::vector<One>& all, size_t from, size_t to, const polar_b
       extents.push_back(Extent{square ? q.side : q.rows, square ? q.side : q.cols, sum(a), q.count, square});
     }
     const Way way = way_of(extents);
-    rc = way.splits > 1 ? launch_product<128, true>(kin, now, from_x, o, targets, status, st, way.splits)
+    rc = way.splits > 1  ? launch_product<128, true>(kin, now, from_x, o, targets, status, st, way.splits)
          : way.bn == 128 ? launch_product<128, false>(kin, now, from_x, o, targets, status, st, 1)
                          : launch_product<256, false>(kin, now, from_x, o, targets, status, st, 1);
     if (rc) return rc;
