@@ -276,14 +276,15 @@ __device__ __forceinline__ Target target_of(const Product& p, const Shape& q, co
   return q.kind == kUpdate ? p.targets[q.first_target + at.z] : Target{};
 }
 
-// Both planes of 16 columns of what is added to a product.  Loaded ahead of use, since no load moves before a store by itself.
+// Both planes of 16 columns of what is added to a product.  Loaded ahead of use, since no load moves before a store by itself, and (as all loads here) not behind
+// a branch of a lane's own, where each would be waited for: a row past the last one reads the last.
 struct Beside {
   uint4 v[4];
 };
 __device__ __forceinline__ Beside beside16(const Shape& q, const Place& at, uint32_t row, uint32_t c0) {
   Beside b = {};
-  if (!q.add || row >= q.m || c0 >= q.n || (c0 | 31u) < (row & ~31u)) return b;
-  const uint4* const add = reinterpret_cast<const uint4*>(q.add + 2 * at.z * q.plane + (uint64_t)row * q.pitch + c0);
+  if (!q.add || (row & ~31u) >= q.m || c0 >= q.n || (c0 | 31u) < (row & ~31u)) return b;   // (the same for all lanes)
+  const uint4* const add = reinterpret_cast<const uint4*>(q.add + 2 * at.z * q.plane + (uint64_t)min(row, q.m - 1) * q.pitch + c0);
   b.v[0] = add[0], b.v[1] = add[1], b.v[2] = add[q.plane / 8], b.v[3] = add[q.plane / 8 + 1];
   return b;
 }
@@ -342,11 +343,11 @@ __device__ __forceinline__ void finish(const Shape& q, const Place& at, const Ta
     if (q.kind == kUpdate) {
       const float keep = 1.f - lr * target.decay, rate = q.by * lr * target.scale;
       uint32_t* const turn = reinterpret_cast<uint32_t*>(place);
-      float* const w = target.weights + (uint64_t)r0 * q.n + block + lane;
       const bool live = block + lane < q.n;                // (a lane is a column here)
+      float* const w = target.weights + (uint64_t)r0 * q.n + min(block + lane, q.n - 1);
       float old[32];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) old[i] = live && r0 + i < q.m ? w[(uint64_t)i * q.n] : 0.f;
+      for (int i = 0; i < 32; ++i) old[i] = w[(uint64_t)min((uint32_t)i, q.m - 1 - r0) * q.n];
       if (lane == 0) stores_read<0>();
       __syncwarp();
 #pragma unroll
@@ -395,19 +396,20 @@ __device__ __forceinline__ void finish16(const Shape& q, const Place& at, const 
   if (q.kind == kSymmetric && block < r0) return;
   if (q.kind == kUpdate) {
     const float keep = 1.f - lr * target.decay, rate = q.by * lr * target.scale;
-    float* const w = target.weights + (uint64_t)row * q.n + c0;
-    if (row >= q.m) return;
+    float* const w = target.weights + (uint64_t)min(row, q.m - 1) * q.n + c0;
     float x[16];                                           // (all loads before the first store, which might change what they read)
     if ((q.n & 3) == 0 && (reinterpret_cast<uintptr_t>(target.weights) & 15) == 0 && c0 + 16 <= q.n) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(x + 4 * j) = reinterpret_cast<const float4*>(w)[j];
 #pragma unroll
       for (int j = 0; j < 16; ++j) x[j] = x[j] * keep - rate * __uint_as_float(v[j]);
+      if (row >= q.m) return;
 #pragma unroll
       for (int j = 0; j < 4; ++j) reinterpret_cast<float4*>(w)[j] = *reinterpret_cast<const float4*>(x + 4 * j);
     } else {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) x[j] = c0 + j < q.n ? w[j] : 0.f;
+      for (int j = 0; j < 16; ++j) x[j] = w[min((uint32_t)j, q.n - 1 - c0)];
+      if (row >= q.m) return;
 #pragma unroll
       for (int j = 0; j < 16; ++j)
         if (c0 + j < q.n) w[j] = x[j] * keep - rate * __uint_as_float(v[j]);
@@ -734,14 +736,14 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t e = (from + i) * kSmallThreads + threadIdx.x;
-      g[i] = e < count ? m.gradient[e] : 0.f, v[i] = e < count ? m.momentum[e] : 0.f;
+      g[i] = m.gradient[min(e, count - 1)], v[i] = m.momentum[min(e, count - 1)];
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t e = (from + i) * kSmallThreads + threadIdx.x;
       v[i] = fmaf(t.momentum, v[i], g[i]);
       if (e < count) m.momentum[e] = v[i];
-      u[from + i] = t.nesterov ? fmaf(t.momentum, v[i], g[i]) : v[i];
+      u[from + i] = e >= count ? 0.f : t.nesterov ? fmaf(t.momentum, v[i], g[i]) : v[i];
       sum += (double)u[from + i] * (double)u[from + i];
     }
   }
@@ -883,30 +885,32 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
       __syncwarp();
       tmem_ld_32x16(lane_at + col, v);
       tmem_ld_wait();
-      if (row >= side) continue;
       float x[16];
 #pragma unroll
       for (int j = 0; j < 16; ++j) x[j] = __uint_as_float(v[j]) * (last ? rate : 1.f / kP);
       if (!last) {
         // (behind the last column X is zeros, and so are these)
-        keep(0, x_plane, col, x);
+        if (row < side) keep(0, x_plane, col, x);
       } else {
-        float* const w = m.weights + (tall ? col * m.cols + row : row * m.cols + col);
+        const uint32_t r = min(row, side - 1);             // (no load behind a branch of a lane's own)
+        float* const w = m.weights + (tall ? col * m.cols + r : r * m.cols + col);
         const uint32_t next = tall ? m.cols : 1;
         if (!tall && (m.cols & 3) == 0 && (reinterpret_cast<uintptr_t>(m.weights) & 15) == 0 && col + 16 <= length) {
 #pragma unroll
           for (int j = 0; j < 16; j += 4) {
-            float4 o = *reinterpret_cast<const float4*>(w + j);
-            o.x = o.x * kept - x[j], o.y = o.y * kept - x[j + 1], o.z = o.z * kept - x[j + 2], o.w = o.w * kept - x[j + 3];
-            *reinterpret_cast<float4*>(w + j) = o;
+            const float4 o = *reinterpret_cast<const float4*>(w + j);
+            x[j] = o.x * kept - x[j], x[j + 1] = o.y * kept - x[j + 1], x[j + 2] = o.z * kept - x[j + 2], x[j + 3] = o.w * kept - x[j + 3];
           }
+          if (row < side)
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(w + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
         } else {
           float o[16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) o[j] = col + j < length ? w[j * next] : 0.f;
+          for (int j = 0; j < 16; ++j) o[j] = w[min((uint32_t)j, length - 1 - col) * next];
 #pragma unroll
           for (int j = 0; j < 16; ++j)
-            if (col + j < length) w[j * next] = o[j] * kept - x[j];
+            if (row < side && col + j < length) w[j * next] = o[j] * kept - x[j];
         }
       }
     }
@@ -1104,14 +1108,14 @@ struct Extent {
   uint64_t m, n, k, count;
   bool symmetric;
 };
-// The way whose busiest SM is done first.  A slab takes 0.58 us with tiles of 256 columns and 0.3 with tiles of 128, what stands around a tile 5 and 4 us (and with
-// a cluster that shares one, and adds its sums, 1.5 more).  Clusters of four or eight leave some SMs out.
+// The way whose busiest SM is done first.  A slab takes 0.45 us with tiles of 256 columns and 0.28 with tiles of 128 (few at a time; all SMs at once are held up by
+// the power they take), what stands around a tile 5.2 and 4 us, and with a cluster that shares one, and adds its sums, 6.5.  Clusters of four or eight leave some SMs out.
 Way way_of(const std::vector<Extent>& e) {
   Way best = {256, 1};
   double least = 0;
   for (const Way w : {Way{256, 1}, Way{128, 1}, Way{128, 2}, Way{128, 4}, Way{128, 8}}) {
     const uint64_t sms = w.splits == 1 ? (uint64_t)sm_count() : w.splits == 2 ? 146 : w.splits == 4 ? 136 : 128;
-    const double slab = w.bn == 256 ? 0.58 : 0.3, around = w.bn == 256 ? 5.0 : w.splits == 1 ? 4.0 : 5.5;
+    const double slab = w.bn == 256 ? 0.45 : 0.28, around = w.bn == 256 ? 5.2 : w.splits == 1 ? 4.0 : 6.5;
     double us = 0;
     uint64_t before = 0, next = 0;                         // tiles passed, and the next one of the first SM
     for (const Extent& x : e) {
