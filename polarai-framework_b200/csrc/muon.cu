@@ -174,11 +174,11 @@ constexpr int kEpilogueWarps = 8, kProductThreads = 32 * (4 + kEpilogueWarps);
 // what is left for the other: 2 * 128 * 232 + 128 * 40 = 64512.
 constexpr int kFewRegisters = 40, kManyRegisters = 232;
 constexpr uint32_t kSlotBytes = 32 * 32 * 2 * 2;           // a block of 32 x 32 as pairs
-template <int BN>
+template <int BN, bool SPLIT>
 struct Cfg {
   static constexpr uint32_t kAPlane = BM * BK * 2, kBPlane = BN * BK * 2, kStageBytes = 2 * (kAPlane + kBPlane);   // both planes of both operands
-  static constexpr int kStages = BN == 256 ? 4 : 5;
-  static constexpr int kSlots = BN == 256 ? 1 : 2;         // blocks on their way to memory, for each warp of the epilogue
+  static constexpr int kStages = BN == 256 ? 3 : 5;
+  static constexpr int kSlots = SPLIT ? 0 : 2;             // blocks on their way to memory, for each warp of the epilogue
   static constexpr uint32_t kWarpBytes = kSlots * kSlotBytes;
   static constexpr uint32_t kTileBytes = kStages * kStageBytes, kTurnBytes = kEpilogueWarps * kWarpBytes;
   static constexpr uint32_t kBytes = kTileBytes + kTurnBytes + 1024 + 256;
@@ -317,24 +317,32 @@ __device__ __forceinline__ void split16(const uint32_t* v, uint32_t* hi, uint32_
   }
 }
 
+// A block of 32 x 32 pairs in shared memory as TMA takes it: 64-byte rows in the 64-byte swizzle, hi, and lo behind it.  Where 8 columns of a row lie:
+__device__ __forceinline__ uint32_t in_slot(uint32_t row, uint32_t eighth) { return row * 64 + (eighth ^ (row >> 1 & 3)) * 16; }
+// The block turned over, 8 x 8 at a time.
+__device__ __forceinline__ void turn_over(uint32_t from, uint32_t to, int lane) {
+#pragma unroll
+  for (uint32_t plane = 0; plane < kSlotBytes; plane += kSlotBytes / 2)
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {                     // eight rows; each eight lanes look at eight columns of them
+      uint32_t r[4];
+      asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                   : "r"(from + plane + in_slot(8 * i + (lane & 7), lane >> 3))
+                   : "memory");
+      asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(to + plane + in_slot(lane, i)), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+                   : "memory");
+    }
+}
+
 // Writes 32 rows from r0 on (one to each lane) and COLS columns from c0 on, whose sums are in `v`; `beside` belongs to the first 16 of them.  Blocks of 32 x 32 go
-// through SLOTS places in shared memory of this warp's own by turns (64-byte rows in the 64-byte swizzle, hi behind lo) and leave them by TMA, for a symmetric
-// product the mirror image too: with a lane's own stores, 32 rows of 32 bytes to an instruction, the epilogue took 12 us a tile.  Weights are turned over
-// there, so that the warp reads and writes 32 neighbours.  `stores`: how many have left so far.
-template <int COLS, int SLOTS>
+// through two slots in shared memory of this warp's own by turns and leave them by TMA, for a symmetric product the mirror image too: with a lane's own stores,
+// 32 rows of 32 bytes to an instruction, the epilogue took 12 us a tile.  Weights are turned over there, so that the warp reads and writes 32
+// neighbours.  `stores`: how many have left so far.
+template <int COLS>
 __device__ __forceinline__ void finish(const Shape& q, const Place& at, const Target& target, float lr, uint32_t r0, uint32_t c0, int lane, uint32_t (&v)[COLS], Beside beside,
-                                       uint8_t* place, uint32_t& stores) {
+                                       uint8_t* slots, uint32_t& stores) {
   const uint32_t row = r0 + lane;
-  auto send = [&](int x, int y, auto write) {
-    uint8_t* const slot = place + (SLOTS == 1 ? 0 : (stores & 1) * kSlotBytes);
-    if (lane == 0) stores_read<SLOTS - 1>();
-    __syncwarp();
-    write(slot);
-    fence_async_smem();
-    __syncwarp();
-    if (lane == 0) store_3d(&q.c, smem_u32(slot), x, y, (int)(2 * at.z));
-    ++stores;
-  };
 #pragma unroll
   for (int part = 0; part < COLS / 32; ++part) {           // blocks of 32 columns
     const uint32_t block = c0 + 32 * part;
@@ -342,7 +350,7 @@ __device__ __forceinline__ void finish(const Shape& q, const Place& at, const Ta
     if (block >= q.n || r0 >= q.m) return;
     if (q.kind == kUpdate) {
       const float keep = 1.f - lr * target.decay, rate = q.by * lr * target.scale;
-      uint32_t* const turn = reinterpret_cast<uint32_t*>(place);
+      uint32_t* const turn = reinterpret_cast<uint32_t*>(slots);
       const bool live = block + lane < q.n;                // (a lane is a column here)
       float* const w = target.weights + (uint64_t)r0 * q.n + min(block + lane, q.n - 1);
       float old[32];
@@ -360,33 +368,39 @@ __device__ __forceinline__ void finish(const Shape& q, const Place& at, const Ta
       continue;
     }
     const bool below = q.kind == kSymmetric && block < r0; // written by the block above the diagonal
-    uint32_t hi[16], lo[16];                               // two columns to a word
+    uint8_t* const slot = slots + (stores & 1) * kSlotBytes;
+    if (lane == 0) stores_read<1>();
+    __syncwarp();
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const Beside now = beside;
       if (32 * part + 16 * half + 16 < COLS) beside = beside16(q, at, row, block + 16 * half + 16);
       if (below) continue;
+      uint32_t hi[8], lo[8];                               // two columns to a word
       complete(q, row, block + 16 * half, now, x + 16 * half);
-      split16(x + 16 * half, hi + 8 * half, lo + 8 * half);
-    }
-    if (below) continue;
-    send((int)block, (int)r0, [&](uint8_t* slot) {
+      split16(x + 16 * half, hi, lo);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint8_t* const at16 = slot + lane * 64 + (j ^ (lane >> 1 & 3)) * 16;
+      for (int j = 0; j < 2; ++j) {
+        uint8_t* const at16 = slot + in_slot(lane, 2 * half + j);
         *reinterpret_cast<uint4*>(at16) = make_uint4(hi[4 * j], hi[4 * j + 1], hi[4 * j + 2], hi[4 * j + 3]);
         *reinterpret_cast<uint4*>(at16 + kSlotBytes / 2) = make_uint4(lo[4 * j], lo[4 * j + 1], lo[4 * j + 2], lo[4 * j + 3]);
       }
-    });
-    if (q.kind == kSymmetric && block > r0)                // its mirror image: a column of the block is a row there
-      send((int)r0, (int)block, [&](uint8_t* slot) {
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          uint8_t* const at2 = slot + c * 64 + ((lane >> 3) ^ (c >> 1 & 3)) * 16 + (lane & 7) * 2;
-          *reinterpret_cast<uint16_t*>(at2) = (uint16_t)(hi[c / 2] >> (c & 1) * 16);
-          *reinterpret_cast<uint16_t*>(at2 + kSlotBytes / 2) = (uint16_t)(lo[c / 2] >> (c & 1) * 16);
-        }
-      });
+    }
+    if (below) continue;
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) store_3d(&q.c, smem_u32(slot), (int)block, (int)r0, (int)(2 * at.z));
+    ++stores;
+    if (q.kind == kSymmetric && block > r0) {
+      uint8_t* const other = slots + (stores & 1) * kSlotBytes;
+      if (lane == 0) stores_read<1>();
+      __syncwarp();
+      turn_over(smem_u32(slot), smem_u32(other), lane);
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) store_3d(&q.c, smem_u32(other), (int)r0, (int)block, (int)(2 * at.z));
+      ++stores;
+    }
   }
 }
 // 16 columns of a row, of which the CTAs of a cluster that shares a tile have few: straight to memory.
@@ -451,7 +465,7 @@ __device__ __forceinline__ void finish16(const Shape& q, const Place& at, const 
 // Every wait is bounded; when one gives up, all roles leave, and the status word holds its code (7xx).
 template <int BN, bool SPLIT>
 __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __grid_constant__ Product p) {
-  using C = Cfg<BN>;
+  using C = Cfg<BN, SPLIT>;
   constexpr int S = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -470,6 +484,11 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
     for (int a = 0; a < 2; ++a) mbar_init(acc_full(a), 1), mbar_init(acc_empty(a), kEpilogueWarps);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0 && elect_one()) {                          // (the maps are parameters: they may be fetched before the kernel before has finished)
+    const Shape& q = p.s[place_of<BN>(p, SPLIT ? blockIdx.x / p.splits : blockIdx.x).shape];
+    prefetch_map(&q.a);
+    prefetch_map(&q.b);
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), 2 * BN);
@@ -508,6 +527,12 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
       int end;
       const int begin = slabs_of(q, &end), runs = (end - begin + kRun - 1) / kRun;
       Beside beside = {};
+      if (!SPLIT && q.kind == kUpdate) {                   // the weights come to L2 meanwhile
+        const Target target = target_of(p, q, at);
+        const uint32_t row = min(r0 + lane, q.m - 1);
+        for (uint32_t c = c0; c < min(c0 + BN / 2, q.n); c += 32)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(target.weights + (uint64_t)row * q.n + c));
+      }
       if (SPLIT && runs == 0) {
 #pragma unroll
         for (int e = 0; e < BN / 2; ++e) sum[e] = 0;
@@ -544,7 +569,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
 #pragma unroll
         for (int j = 0; j < BN / 2; ++j) shared[(half * (BN / 2) + j) * BM + quarter * 32 + lane] = __uint_as_float(sum[j]);
       } else {
-        finish<BN / 2, C::kSlots>(q, at, target_of(p, q, at), lr, r0, c0, lane, sum, beside, place, stores);
+        finish<BN / 2>(q, at, target_of(p, q, at), lr, r0, c0, lane, sum, beside, place, stores);
         __syncwarp();
       }
     }
@@ -635,12 +660,18 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
       for (uint32_t piece = rank * kEpilogueWarps + warp - 4; piece < 4 * BN / 16; piece += splits * kEpilogueWarps) {
         const uint32_t quarter = piece & 3, c = piece / 4 * 16;
         uint32_t v[16];
+        float x[4][16];                                    // four CTAs' sums on their way
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] = 0;
-        for (uint32_t r = 0; r < splits; ++r)
+        for (uint32_t r = 0; r < splits; r += 4) {         // (two, four or eight of them)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[i][j] = ld_cluster(shared + (c + j) * BM + quarter * 32 + lane, min(r + i, splits - 1));
 #pragma unroll
           for (int j = 0; j < 16; ++j)
-            v[j] = __float_as_uint(__uint_as_float(v[j]) + ld_cluster(shared + (c + j) * BM + quarter * 32 + lane, r));
+            v[j] = __float_as_uint(__uint_as_float(v[j]) + x[0][j] + x[1][j] + (splits > 2 ? x[2][j] + x[3][j] : 0.f));
+        }
         finish16(q, at, target, lr, (uint32_t)at.m0 + quarter * 32, (uint32_t)at.n0 + c, lane, v);
       }
     }
@@ -654,7 +685,8 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
   }
   if constexpr (SPLIT) {
     __syncthreads();
-    cluster_arrive();                                      // (no CTA leaves while another one reads its shared memory)
+    // no CTA leaves while another one reads its shared memory; nothing that was written has to be seen by then (with a release, which waits for the stores, 1 us more)
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     cluster_wait();
   }
   if (warp == 1) {
@@ -1180,7 +1212,7 @@ int launch_product(const std::vector<Kin>& kin, const std::vector<std::pair<size
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3(SPLIT ? p.tiles * splits : std::min(p.tiles, (uint32_t)sm_count()));
     c.blockDim = dim3(kProductThreads);
-    c.dynamicSmemBytes = Cfg<BN>::kBytes;
+    c.dynamicSmemBytes = Cfg<BN, SPLIT>::kBytes;
     c.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1190,7 +1222,7 @@ int launch_product(const std::vector<Kin>& kin, const std::vector<std::pair<size
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     c.attrs = at;
     c.numAttrs = SPLIT ? 2 : 1;
-    cudaError_t e = cudaFuncSetAttribute(product_kernel<BN, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<BN>::kBytes);
+    cudaError_t e = cudaFuncSetAttribute(product_kernel<BN, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<BN, SPLIT>::kBytes);
     void* args[1] = {&p};
     if (e == cudaSuccess) e = cudaLaunchKernelExC(&c, reinterpret_cast<const void*>(product_kernel<BN, SPLIT>), args);
     if (e != cudaSuccess) {
