@@ -163,6 +163,11 @@ __device__ __forceinline__ void sums4(T (&v)[4], T* slots) {
 constexpr uint32_t kFewCtas = 1024;
 constexpr int kFinishThreads = 1024;
 
+__device__ __forceinline__ float4 ld_l2(const float4* p) {
+  float4 v;
+  asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+  return v;
+}
 // Leaves a CTA's sums and tells whether it was the last one to; then the sums of all CTAs are in `total` of its first thread, added in an
 // order that does not hang on which CTA was last.
 template <int THREADS>
@@ -180,7 +185,7 @@ __device__ bool last_sums(float4 mine, float4* partial, uint32_t ctas, uint32_t*
   for (int i = 0; i < 4; ++i) total[i] = 0;
 #pragma unroll 8
   for (uint32_t c = threadIdx.x; c < ctas; c += THREADS) {
-    const float4 p = __ldcg(partial + c);
+    const float4 p = ld_l2(partial + c);
     total[0] += p.x, total[1] += p.y, total[2] += p.z, total[3] += p.w;
   }
   sums4<THREADS>(total, slots);
