@@ -17,9 +17,9 @@
 namespace polar_b200 {
 namespace {
 
-constexpr uint32_t kTile = 4096;                           // tokens of a CTA in the passes that count and sum
+constexpr uint32_t kTile = 2048;                           // tokens of a CTA in the passes that count and sum
 constexpr uint32_t kWords = kTile / 32;
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kEach = kTile / kThreads;   // (with 16 tokens to a thread the loads in flight took the registers of all but two CTAs)
 constexpr uint32_t kPass = 2048;                           // tokens of a CTA in the pass that writes gradients
 constexpr uint32_t kFew = 8192, kFewSequences = 2048;      // what one CTA does alone
 constexpr int kFewThreads = 1024, kFewEach = kFew / kFewThreads;
@@ -66,13 +66,25 @@ __device__ __forceinline__ uint32_t sequence_of(const Packed<Id>& p, uint64_t t)
   return lo;
 }
 
-// The sequences of the warp's 128 tokens from `base` on, four neighbours to each lane.
+// A sequence, and where it ends, that the warp has found before.
+struct Found {
+  uint32_t s;
+  uint64_t end = 0;
+};
+// The sequences of the warp's 128 tokens from `base` on, four neighbours to each lane.  `before`: of tokens before them; long sequences are looked for once.
 template <class Id>
-__device__ __forceinline__ void sequences_of(const Packed<Id>& p, uint64_t base, uint32_t (&of)[4]) {
+__device__ __forceinline__ void sequences_of(const Packed<Id>& p, uint64_t base, uint32_t (&of)[4], Found& before) {
+  if (base + 128 <= before.end) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) of[k] = before.s;
+    return;
+  }
   const uint32_t lane = threadIdx.x & 31, first = sequence_of(p, base);
   const uint64_t none = ~0ull, next = first + 1 + lane < p.sequences ? p.offset(first + 1 + lane) : none;
   const uint32_t begins = __popc(__ballot_sync(0xffffffffu, next < base + 128));
   const uint64_t mine = base + 4 * lane;
+  before.s = first;
+  before.end = __shfl_sync(0xffffffffu, next, 0);
 #pragma unroll
   for (int k = 0; k < 4; ++k) of[k] = first;
   if (begins < 32) {                                       // the 32 next beginnings reach over the 128 tokens
@@ -200,18 +212,18 @@ __global__ void __launch_bounds__(kThreads) mark_kernel(Packed<Id> p, Workspace 
   if (blockIdx.x == 0 && threadIdx.x == 0) w.shared->ticket = w.shared->live = 0;
   const uint64_t begin = p.offset(0), end = p.offset(p.sequences);
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint64_t base = (uint64_t)blockIdx.x * kTile + warp * (kTile / 8);
+  const uint64_t base = (uint64_t)blockIdx.x * kTile + warp * (32 * kEach);
   uint32_t mine = 0;
-  Id ids[16];                                              // (all loads on their way before the first vote, and none behind a branch)
+  Id ids[kEach];                                           // (all loads on their way before the first vote, and none behind a branch)
 #pragma unroll
-  for (int j = 0; j < 16; ++j) ids[j] = ld_id(p.ids + min(base + 32 * j + lane, p.tokens - 1));
+  for (int j = 0; j < kEach; ++j) ids[j] = ld_id(p.ids + min(base + 32 * j + lane, p.tokens - 1));
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
+  for (int j = 0; j < kEach; ++j) {
     const uint64_t t = base + 32 * j + lane;
     const uint32_t b = __ballot_sync(0xffffffffu, !(ids[j] < Id(0)) && t >= begin && t < end);
     if (lane == j) mine = b;
   }
-  if (lane < 16) w.bits[base / 32 + lane] = mine;
+  if (lane < kEach) w.bits[base / 32 + lane] = mine;
   const uint32_t n = __reduce_add_sync(0xffffffffu, __popc(mine));
   if (lane == 0) sums[warp] = n;
   __syncthreads();
@@ -417,6 +429,7 @@ __global__ void __launch_bounds__(kThreads) policy_kernel(Packed<Id> p, Workspac
     adv[h] = load4(o.per_token ? o.advantage : nullptr, t, p.tokens, whole);
     bits[h] = w.bits[t / 32] >> (t & 31) & 15;             // (the last tile's words are all there)
   }
+  Found found;
   float even;
   if (o.count > 0.f) {
     even = 1.f / o.count;
@@ -439,7 +452,7 @@ __global__ void __launch_bounds__(kThreads) policy_kernel(Packed<Id> p, Workspac
   for (int h = 0; h < PARTS; ++h) {
     const uint64_t base = ((uint64_t)blockIdx.x * PARTS + h) * kPart + warp * 128, t = base + 4 * lane;
     uint32_t of[4] = {0, 0, 0, 0};
-    if (LOOK && base < end) sequences_of(p, base, of);
+    if (LOOK && base < end) sequences_of(p, base, of, found);
     float4 g, ge;
     if (LOOK && !o.per_token)
 #pragma unroll
@@ -646,43 +659,44 @@ __global__ void __launch_bounds__(kThreads) sums_kernel(Packed<Id> p, Workspace 
   const uint64_t begin = p.offset(0), end = p.offset(p.sequences);
   const uint64_t tile = (uint64_t)blockIdx.x * kTile, tile_end = min(tile + kTile, p.tokens);
   const uint64_t from = max(tile, begin), to = min(tile_end, end);
-  float lp[16], ref[16];
-  Id ids[16];                                              // (all loads on their way before the first vote, and none behind a branch)
+  float lp[kEach], ref[kEach];
+  Id ids[kEach];                                              // (all loads on their way before the first vote, and none behind a branch)
   uint32_t mine = 0, bits = 0;
   if (p.tokens) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const uint64_t t = min(tile + warp * (kTile / 8) + 32 * j + lane, p.tokens - 1);
+    for (int j = 0; j < kEach; ++j) {
+      const uint64_t t = min(tile + warp * (32 * kEach) + 32 * j + lane, p.tokens - 1);
       ids[j] = ld_id(p.ids + t);
       lp[j] = ld_stream(o.logprob + t);
       ref[j] = 0.f;
     }
+    // (the tile's first and last sequence are looked for while these are on their way)
     if (o.reference)
 #pragma unroll
-      for (int j = 0; j < 16; ++j) ref[j] = ld_stream(o.reference + min(tile + warp * (kTile / 8) + 32 * j + lane, p.tokens - 1));
+      for (int j = 0; j < kEach; ++j) ref[j] = ld_stream(o.reference + min(tile + warp * (32 * kEach) + 32 * j + lane, p.tokens - 1));
+    if (warp < 2 && from < to) {
+      const uint32_t s = sequence_of(p, warp == 0 ? from : to - 1);
+      if (lane == 0) span[warp] = s;
+    }
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const uint64_t t = tile + warp * (kTile / 8) + 32 * j + lane;
+    for (int j = 0; j < kEach; ++j) {
+      const uint64_t t = tile + warp * (32 * kEach) + 32 * j + lane;
       const uint32_t b = __ballot_sync(0xffffffffu, !(ids[j] < Id(0)) && t >= from && t < to);
       if (lane == j) mine = b;
       bits |= (b >> lane & 1) << j;
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) lp[j] = ref[j] = 0.f;
+    for (int j = 0; j < kEach; ++j) lp[j] = ref[j] = 0.f;
   }
-  if (warp < 2 && from < to) {
-    const uint32_t s = sequence_of(p, warp == 0 ? from : to - 1);
-    if (lane == 0) span[warp] = s;
-  }
-  if (lane < 16) w.bits[tile / 32 + warp * 16 + lane] = mine;
+  if (lane < kEach) w.bits[tile / 32 + warp * kEach + lane] = mine;
   const uint32_t n = __reduce_add_sync(0xffffffffu, __popc(mine));
   if (lane == 0) sums[warp] = n;
   double sum = 0;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
+  for (int j = 0; j < kEach; ++j) {
     const double d = bits >> j & 1 ? (double)lp[j] - (double)ref[j] : 0.0;
-    values[warp * (kTile / 8) + 32 * j + lane] = d;
+    values[warp * (32 * kEach) + 32 * j + lane] = d;
     sum += d;
   }
   sum = warp_sum(sum);
@@ -767,13 +781,14 @@ __global__ void __launch_bounds__(kThreads) pairs_grad_kernel(Packed<Id> p, Work
   pdl_enter();
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint64_t begin = p.offset(0), end = p.offset(p.sequences);
+  Found found;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const uint64_t base = (uint64_t)blockIdx.x * kPass + h * (kPass / 2) + warp * 128, t = base + 4 * lane;
     if (base >= end) return;
     uint32_t of[4];
     const uint32_t bits = t < p.tokens ? w.bits[t / 32] >> (t & 31) & 15 : 0;
-    sequences_of(p, base, of);
+    sequences_of(p, base, of, found);
     float4 g;
 #pragma unroll
     for (int k = 0; k < 4; ++k) (&g.x)[k] = bits >> k & 1 ? w.share[of[k]] : 0.f;
