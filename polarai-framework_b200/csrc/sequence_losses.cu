@@ -215,13 +215,26 @@ __global__ void __launch_bounds__(kThreads) mark_kernel(Packed<Id> p, Workspace 
   const uint64_t base = (uint64_t)blockIdx.x * kTile + warp * (32 * kEach);
   uint32_t mine = 0;
   Id ids[kEach];                                           // (all loads on their way before the first vote, and none behind a branch)
+  if (base + 32 * kEach <= p.tokens) {                     // (the same for the whole warp)
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) ids[j] = ld_id(p.ids + min(base + 32 * j + lane, p.tokens - 1));
+    for (int j = 0; j < kEach; ++j) ids[j] = ld_id(p.ids + base + lane + 32 * j);
+  } else {
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) {
-    const uint64_t t = base + 32 * j + lane;
-    const uint32_t b = __ballot_sync(0xffffffffu, !(ids[j] < Id(0)) && t >= begin && t < end);
-    if (lane == j) mine = b;
+    for (int j = 0; j < kEach; ++j) ids[j] = ld_id(p.ids + min(base + 32 * j + lane, p.tokens - 1));
+  }
+  if (base >= begin && base + 32 * kEach <= end) {
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const uint32_t b = __ballot_sync(0xffffffffu, !(ids[j] < Id(0)));
+      if (lane == j) mine = b;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const uint64_t t = base + 32 * j + lane;
+      const uint32_t b = __ballot_sync(0xffffffffu, !(ids[j] < Id(0)) && t >= begin && t < end);
+      if (lane == j) mine = b;
+    }
   }
   if (lane < kEach) w.bits[base / 32 + lane] = mine;
   const uint32_t n = __reduce_add_sync(0xffffffffu, __popc(mine));
@@ -660,34 +673,41 @@ __global__ void __launch_bounds__(kThreads) sums_kernel(Packed<Id> p, Workspace 
   const uint64_t tile = (uint64_t)blockIdx.x * kTile, tile_end = min(tile + kTile, p.tokens);
   const uint64_t from = max(tile, begin), to = min(tile_end, end);
   float lp[kEach], ref[kEach];
-  Id ids[kEach];                                              // (all loads on their way before the first vote, and none behind a branch)
+  Id ids[kEach];                                           // (all loads on their way before the first vote, and none behind a branch)
   uint32_t mine = 0, bits = 0;
-  if (p.tokens) {
+  // places within the tile: the thread's first one, and what lies in a sequence
+  const uint32_t at = warp * (32 * kEach) + lane, low = from < to ? (uint32_t)(from - tile) : 0, high = from < to ? (uint32_t)(to - tile) : 0;
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      const uint64_t t = min(tile + warp * (32 * kEach) + 32 * j + lane, p.tokens - 1);
-      ids[j] = ld_id(p.ids + t);
-      lp[j] = ld_stream(o.logprob + t);
-      ref[j] = 0.f;
-    }
-    // (the tile's first and last sequence are looked for while these are on their way)
+  for (int j = 0; j < kEach; ++j) lp[j] = ref[j] = 0.f;
+  if (tile + kTile <= p.tokens) {
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) ids[j] = ld_id(p.ids + tile + at + 32 * j), lp[j] = ld_stream(o.logprob + tile + at + 32 * j);
     if (o.reference)
 #pragma unroll
-      for (int j = 0; j < kEach; ++j) ref[j] = ld_stream(o.reference + min(tile + warp * (32 * kEach) + 32 * j + lane, p.tokens - 1));
-    if (warp < 2 && from < to) {
-      const uint32_t s = sequence_of(p, warp == 0 ? from : to - 1);
-      if (lane == 0) span[warp] = s;
-    }
+      for (int j = 0; j < kEach; ++j) ref[j] = ld_stream(o.reference + tile + at + 32 * j);
+  } else if (p.tokens) {
+    const uint32_t last = (uint32_t)(p.tokens - 1 - tile);
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-      const uint64_t t = tile + warp * (32 * kEach) + 32 * j + lane;
-      const uint32_t b = __ballot_sync(0xffffffffu, !(ids[j] < Id(0)) && t >= from && t < to);
-      if (lane == j) mine = b;
-      bits |= (b >> lane & 1) << j;
+      const uint64_t t = tile + min(at + 32 * j, last);
+      ids[j] = ld_id(p.ids + t), lp[j] = ld_stream(o.logprob + t);
+      if (o.reference) ref[j] = ld_stream(o.reference + t);
     }
-  } else {
+  }
+  // (the tile's first and last sequence are looked for while these are on their way)
+  if (warp < 2 && from < to) {
+    const uint32_t s = sequence_of(p, warp == 0 ? from : to - 1);
+    if (lane == 0) span[warp] = s;
+  }
+  if (from < to) {
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) lp[j] = ref[j] = 0.f;
+    for (int j = 0; j < kEach; ++j) {
+      const uint32_t i = at + 32 * j;
+      const bool counts = !(ids[j] < Id(0)) && i >= low && i < high;
+      const uint32_t b = __ballot_sync(0xffffffffu, counts);
+      if (lane == j) mine = b;
+      bits |= (uint32_t)counts << j;
+    }
   }
   if (lane < kEach) w.bits[tile / 32 + warp * kEach + lane] = mine;
   const uint32_t n = __reduce_add_sync(0xffffffffu, __popc(mine));
@@ -787,11 +807,15 @@ __global__ void __launch_bounds__(kThreads) pairs_grad_kernel(Packed<Id> p, Work
     const uint64_t base = (uint64_t)blockIdx.x * kPass + h * (kPass / 2) + warp * 128, t = base + 4 * lane;
     if (base >= end) return;
     uint32_t of[4];
-    const uint32_t bits = t < p.tokens ? w.bits[t / 32] >> (t & 31) & 15 : 0;
+    const uint32_t bits = w.bits[t / 32] >> (t & 31) & 15; // (the last tile's words are all there)
     sequences_of(p, base, of, found);
-    float4 g;
+    float4 g, share;
+    share.x = w.share[of[0]];
+    // (mostly the whole warp's tokens are of one sequence)
+    if (base + 128 <= found.end) share.y = share.z = share.w = share.x;
+    else share.y = w.share[of[1]], share.z = w.share[of[2]], share.w = w.share[of[3]];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) (&g.x)[k] = bits >> k & 1 ? w.share[of[k]] : 0.f;
+    for (int k = 0; k < 4; ++k) (&g.x)[k] = bits >> k & 1 ? (&share.x)[k] : 0.f;
     store4(g_logprob, g, t, begin, end, vectors);
   }
 }
