@@ -695,13 +695,11 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
   }
 }
 
-// ---- matrices with a short side: a whole step by one CTA, or by a cluster of up to eight
+// ---- small matrices: a whole step by one CTA for each
 
-// X lies in shared memory as pairs all the while, the shorter side's rows behind one another: 16, 32, 64 or 128 of them, in chunks of 64 columns and the
-// 128-byte swizzle, which is a K-major operand for X X^T and an MN-major one for P X.  Tall matrices are turned over on the way in and out.  A CTA has room for
-// 32768 elements; a longer matrix has its columns in several CTAs' shared memory, which add their shares of G: each sums up some columns of it and
-// hands them to all, and the rest of the round each does for itself.  The products are 0.2 to 0.8 us each; what stands between them - the sums out of tensor
-// memory, the pairs into shared memory, a barrier - is as much, and the exchange 3 us a round.
+// Its X lies in shared memory as pairs all the while, the shorter side's rows behind one another: 64 or 128 rows, in chunks of 64 columns and the 128-byte
+// swizzle, which is a K-major operand for X X^T and an MN-major one for P X.  Tall matrices are turned over on the way in and out.  The products are 0.2
+// to 0.8 us each; what stands between them - the sums out of tensor memory, the pairs into shared memory, a barrier - is as much.
 struct Small {
   float* weights;
   const float* gradient;
@@ -713,7 +711,7 @@ template <int N>
 struct SmallTable {
   float lr, momentum, a, b, c;
   int nesterov;
-  uint32_t steps, ctas;                                    // ctas: of a matrix
+  uint32_t steps;
   const float* schedule;
   int* status;
   unsigned long long wait_ns;
@@ -723,45 +721,29 @@ constexpr int kFewSmall = 64, kManySmall = 800;
 static_assert(sizeof(SmallTable<kManySmall>) <= 32764, "kernel parameters");
 constexpr int kSmallThreads = 512, kSmallEach = 64;        // elements of a thread at most
 constexpr uint32_t kSmallX = 128 * 1024, kSmallP = 64 * 1024;
-// (an operand of 128 rows may reach as far past the end of what lies there: those rows of the result are not read)
+// (an operand of 128 rows may reach 64 rows past the end of what lies there: those rows of the result are not read)
 constexpr uint32_t kSmallBytes = kSmallX + kSmallP + 16 * 1024 + 1024 + 256;
-constexpr uint64_t kMostCtas = 8;
-__host__ __device__ constexpr uint32_t height_of(uint64_t side) { return side <= 16 ? 16 : side <= 32 ? 32 : side <= 64 ? 64 : 128; }
-// How many CTAs hold the matrix; 0: it is too large for them.
-constexpr uint64_t ctas_of(uint64_t rows, uint64_t cols) {
+__host__ __device__ constexpr bool is_small(uint64_t rows, uint64_t cols) {
   const uint64_t side = rows < cols ? rows : cols, other = rows < cols ? cols : rows;
-  if (side > 128) return 0;
-  const uint64_t room = kSmallThreads * kSmallEach / height_of(side);
-  uint64_t ctas = 1;
-  while (ctas <= kMostCtas && ctas * room < other) ctas *= 2;
-  return ctas <= kMostCtas ? ctas : 0;
+  return (side <= 128 && other <= 256) || (side <= 64 && other <= 512);
 }
 
-__device__ __forceinline__ void st_cluster(uint32_t address, uint32_t rank, uint4 v) {
-  uint32_t remote;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(address), "r"(rank));
-  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
-
-template <int N, bool SEVERAL>
+template <int N>
 __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_constant__ SmallTable<N> t) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ double slots[kSmallThreads / 32], total;
+  __shared__ double slots[kSmallThreads / 32];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const smem = smem_raw + (smem_base - smem_u32(smem_raw));
   const uint32_t bar = smem_base + kSmallBytes - 1024 - 256;
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + kSmallBytes - 1024 - 256 + 8);
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
-  const uint32_t ctas = SEVERAL ? t.ctas : 1, rank = SEVERAL ? cluster_rank() : 0;
-  const Small& m = t.m[blockIdx.x / ctas];
+  const Small& m = t.m[blockIdx.x];
   const bool tall = m.rows > m.cols;
-  const uint32_t side = tall ? m.cols : m.rows, longer = tall ? m.rows : m.cols;
-  // this CTA's columns of X
-  const uint32_t each = SEVERAL ? ((longer + ctas - 1) / ctas + 63) / 64 * 64 : longer, first = min(longer, rank * each), length = min(each, longer - first);
-  const uint32_t height = height_of(side);                 // rows that are held
+  const uint32_t side = tall ? m.cols : m.rows, length = tall ? m.rows : m.cols;
+  const uint32_t height = side <= 64 ? 64 : 128;           // rows that are held
   const uint32_t chunk = height * 128;                     // bytes of a chunk of 64 columns
-  const uint32_t x_plane = (each + 63) / 64 * chunk, p_plane = (side + 63) / 64 * chunk;
+  const uint32_t x_plane = (length + 63) / 64 * chunk, p_plane = (side + 63) / 64 * chunk;
   if (threadIdx.x == 0) {
     mbar_init(bar, 1);
     *abort_flag = 0;
@@ -776,36 +758,25 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
   pdl_enter();
 
   // the momentum, u and its size
-  const uint32_t count = side * length, inner = tall ? side : length;   // elements as they lie in memory, and in a row of them
-  const float* const gradient = m.gradient + (uint64_t)first * (tall ? side : 1);
-  float* const momentum = m.momentum + (uint64_t)first * (tall ? side : 1);
-  const uint32_t pitch = tall ? side : longer;
-  const uint32_t down = inner ? kSmallThreads / inner : 0, right = inner ? kSmallThreads - down * inner : 0;   // kSmallThreads elements on
+  const uint32_t count = m.rows * m.cols;
   float u[kSmallEach];
   double sum = 0;
-  {
-    uint32_t row = inner ? threadIdx.x / inner : 0, col = inner ? threadIdx.x - row * inner : 0;
 #pragma unroll
-    for (int from = 0; from < kSmallEach; from += 8) {      // eight elements' loads on their way
-      if (from * kSmallThreads >= count) break;
-      float g[8], v[8];
-      uint32_t at[8];
+  for (int from = 0; from < kSmallEach; from += 8) {        // eight elements' loads on their way
+    if (from * kSmallThreads >= count) break;
+    float g[8], v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t e = (from + i) * kSmallThreads + threadIdx.x;
-        at[i] = e < count ? row * pitch + col : 0;
-        g[i] = gradient[at[i]], v[i] = momentum[at[i]];
-        row += down, col += right;
-        if (col >= inner) col -= inner, ++row;
-      }
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t e = (from + i) * kSmallThreads + threadIdx.x;
+      g[i] = m.gradient[min(e, count - 1)], v[i] = m.momentum[min(e, count - 1)];
+    }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t e = (from + i) * kSmallThreads + threadIdx.x;
-        v[i] = fmaf(t.momentum, v[i], g[i]);
-        if (e < count) momentum[at[i]] = v[i];
-        u[from + i] = e >= count ? 0.f : t.nesterov ? fmaf(t.momentum, v[i], g[i]) : v[i];
-        sum += (double)u[from + i] * (double)u[from + i];
-      }
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t e = (from + i) * kSmallThreads + threadIdx.x;
+      v[i] = fmaf(t.momentum, v[i], g[i]);
+      if (e < count) m.momentum[e] = v[i];
+      u[from + i] = e >= count ? 0.f : t.nesterov ? fmaf(t.momentum, v[i], g[i]) : v[i];
+      sum += (double)u[from + i] * (double)u[from + i];
     }
   }
 #pragma unroll
@@ -818,28 +789,22 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
   sum = 0;
 #pragma unroll
   for (int i = 0; i < kSmallThreads / 32; ++i) sum += slots[i];
-  if constexpr (SEVERAL) {
-    if (threadIdx.x == 0) total = sum;
-    cluster_arrive();
-    cluster_wait();
-    sum = 0;
-    for (uint32_t r = 0; r < ctas; ++r) sum += ld_cluster(&total, r);
-  }
   const double by = sum == 0 ? 0 : (double)kX / sqrt(sum);
   // where 16 bytes of a row lie
   auto place = [&](uint32_t row, uint32_t col) { return col / 64 * chunk + row * 128 + (((col & 63) / 8 ^ (row & 7)) << 4); };
   {
-    uint32_t row = inner ? threadIdx.x / inner : 0, col = inner ? threadIdx.x - row * inner : 0;
+    uint32_t row = threadIdx.x / m.cols, col = threadIdx.x - row * m.cols;
+    const uint32_t down = kSmallThreads / m.cols, right = kSmallThreads - down * m.cols;
 #pragma unroll
     for (int i = 0; i < kSmallEach; ++i) {
       if (i * kSmallThreads >= count) break;
-      if (i * kSmallThreads + threadIdx.x < count) {
+      if (row < m.rows) {
         const uint32_t r = tall ? col : row, c = tall ? row : col;
         __half* const x = reinterpret_cast<__half*>(smem + place(r, c)) + (c & 7);
         split((float)((double)u[i] * by), x, x + x_plane / 2);
       }
       row += down, col += right;
-      if (col >= inner) col -= inner, ++row;
+      if (col >= m.cols) col -= m.cols, ++row;
     }
   }
 
@@ -889,158 +854,95 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
     }
   };
 
-  bool ok = true;                                          // (of a cluster, all CTAs meet in every round whatever happens)
-  for (uint32_t step = 0; step < t.steps && (ok || SEVERAL); ++step) {
+  for (uint32_t step = 0; step < t.steps; ++step) {
     // G = X X^T; every 128 k in an accumulator of its own, as in the product kernel
-    ok = ok && multiplied([&] {
-      for (uint32_t k = 0; k < length16 / 16; ++k) {
-        const uint32_t at = x_at + k_offset(k);
-        three(tmem + k / 8 * side16, k_major, at, at + (x_plane >> 4), k_major, at, at + (x_plane >> 4), f16_idesc((int)side16, 0, 0), k % 8 ? 1u : 0u);
-      }
-    });
+    if (!multiplied([&] {
+          for (uint32_t k = 0; k < length16 / 16; ++k) {
+            const uint32_t at = x_at + k_offset(k);
+            three(tmem + k / 8 * 128, k_major, at, at + (x_plane >> 4), k_major, at, at + (x_plane >> 4), f16_idesc((int)side16, 0, 0), k % 8 ? 1u : 0u);
+          }
+        }))
+      break;
     float g[32];
     if (mine && (uint32_t)group * 32 < side16) {
 #pragma unroll
       for (int j = 0; j < 32; ++j) g[j] = 0.f;
       for (uint32_t run = 0; run < (length16 + 127) / 128; ++run) {
         uint32_t v[32];
-        tmem_ld_32x32(lane_at + run * side16 + group * 32, v);
+        tmem_ld_32x32(lane_at + run * 128 + group * 32, v);
         tmem_ld_wait();
 #pragma unroll
         for (int j = 0; j < 32; ++j) g[j] += __uint_as_float(v[j]);
       }
 #pragma unroll
       for (int j = 0; j < 32; ++j) g[j] = group * 32 + j < side ? g[j] * (kG / (kX * kX)) : 0.f;
-      if (!SEVERAL && row < side) keep(kSmallX, p_plane, group * 32, g), keep(kSmallX, p_plane, group * 32 + 16, g + 16);
-    }
-    if constexpr (SEVERAL) {
-      // this CTA's share, [column][row], where P was
-      float* const share = reinterpret_cast<float*>(smem + kSmallX);
-      if (mine && (uint32_t)group * 32 < side16)
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (group * 32 + j < side16) share[(group * 32 + j) * 128 + row] = g[j];
-      __syncthreads();
-      cluster_arrive();
-      cluster_wait();
-      // eight columns of a row to a thread, of those that are this CTA's to sum up: every eighth, fourth or second eight
-      uint4 hi[2], lo[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t unit = i * kSmallThreads + threadIdx.x, eight = rank + unit / 128 * ctas, r = unit % 128;
-        if (eight * 8 >= side16) continue;                 // (the same for the whole warp)
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (uint32_t from = 0; from < ctas; from += 2) {
-          float x[2][8];
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[k][j] = ld_cluster(share + (eight * 8 + j) * 128 + r, from + k);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] += x[0][j] + x[1][j];
-        }
-        union { __half h[8]; uint4 bits; } h, l;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) split(v[j], &h.h[j], &l.h[j]);
-        hi[i] = h.bits, lo[i] = l.bits;
-      }
-      cluster_arrive();                                    // (all have read the shares, which lie where the sums go)
-      cluster_wait();
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t unit = i * kSmallThreads + threadIdx.x, eight = rank + unit / 128 * ctas, r = unit % 128;
-        if (eight * 8 >= side16 || r >= side) continue;
-        const uint32_t at = smem_base + kSmallX + place(r, eight * 8);
-        for (uint32_t to = 0; to < ctas; ++to) st_cluster(at, to, hi[i]), st_cluster(at + p_plane, to, lo[i]);
-      }
-      asm volatile("fence.proxy.async;" ::: "memory");
-      __syncwarp();
-      cluster_arrive();
-      cluster_wait();
+      if (row < side) keep(kSmallX, p_plane, group * 32, g), keep(kSmallX, p_plane, group * 32 + 16, g + 16);
     }
     // P = a + b G + c G G, in the place of G
-    ok = ok && multiplied([&] {
-      for (uint32_t k = 0; k < side16 / 16; ++k) {
-        const uint32_t at = p_at + k_offset(k);
-        three(tmem, k_major, at, at + (p_plane >> 4), k_major, at, at + (p_plane >> 4), f16_idesc((int)side16, 0, 0), k ? 1u : 0u);
-      }
-    });
-    if (ok && mine && (uint32_t)group * 32 < side16) {
+    if (!multiplied([&] {
+          for (uint32_t k = 0; k < side16 / 16; ++k) {
+            const uint32_t at = p_at + k_offset(k);
+            three(tmem, k_major, at, at + (p_plane >> 4), k_major, at, at + (p_plane >> 4), f16_idesc((int)side16, 0, 0), k ? 1u : 0u);
+          }
+        }))
+      break;
+    if (mine && (uint32_t)group * 32 < side16) {
       uint32_t v[32];
       tmem_ld_32x32(lane_at + group * 32, v);
       tmem_ld_wait();
-      if (SEVERAL) {                                       // G as the cluster has summed it
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          // (rows past the last one, and columns of another warp's where there are 16 in all: nothing is made of them)
-          const uint8_t* const x = smem + kSmallX + place(min(row, side - 1), min(group * 32u + 8 * j, side16 - 8));
-          const uint4 h = *reinterpret_cast<const uint4*>(x), l = *reinterpret_cast<const uint4*>(x + p_plane);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 a = __half22float2(reinterpret_cast<const __half2*>(&h)[k]), b = __half22float2(reinterpret_cast<const __half2*>(&l)[k]);
-            g[8 * j + 2 * k] = a.x + b.x, g[8 * j + 2 * k + 1] = a.y + b.y;
-          }
-        }
-        __syncwarp();
-      }
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
         const uint32_t col = group * 32 + j;
         g[j] = fmaf(t.c * (kP / (kG * kG)), __uint_as_float(v[j]), t.b * (kP / kG) * g[j]) + (col == row ? t.a * kP : 0.f);
         if (col >= side) g[j] = 0.f;
       }
-      if (row < side) {
-        keep(kSmallX, p_plane, group * 32, g);
-        if ((uint32_t)group * 32 + 16 < side16) keep(kSmallX, p_plane, group * 32 + 16, g + 16);
-      }
+      if (row < side) keep(kSmallX, p_plane, group * 32, g), keep(kSmallX, p_plane, group * 32 + 16, g + 16);
     }
-    // P X, as many columns at a time as tensor memory has
+    // P X
+    if (!multiplied([&] {
+          for (uint32_t from = 0; from < length16; from += 256) {
+            const uint32_t n = min(length16 - from, 256u), b_at = x_at + (from / 64 * chunk >> 4);
+            for (uint32_t k = 0; k < side16 / 16; ++k) {
+              const uint32_t a_at = p_at + k_offset(k), b = b_at + (k * 2048 >> 4);
+              three(tmem + from, k_major, a_at, a_at + (p_plane >> 4), mn_major, b, b + (x_plane >> 4), f16_idesc((int)n, 0, 1), k ? 1u : 0u);
+            }
+          }
+        }))
+      break;
+    if (!mine) continue;
     const bool last = step + 1 == t.steps;
     const float lr = t.schedule ? t.schedule[1] : t.lr, kept = 1.f - lr * m.decay, rate = lr * m.scale / (kP * kX);
-    for (uint32_t part = 0; part < length16 && ok; part += 512) {
-      const uint32_t end = min(length16, part + 512);
-      ok = multiplied([&] {
-        for (uint32_t from = part; from < end; from += 256) {
-          const uint32_t n = min(end - from, 256u), b_at = x_at + (from / 64 * chunk >> 4);
-          for (uint32_t k = 0; k < side16 / 16; ++k) {
-            const uint32_t a_at = p_at + k_offset(k), b = b_at + (k * 2048 >> 4);
-            three(tmem + from - part, k_major, a_at, a_at + (p_plane >> 4), mn_major, b, b + (x_plane >> 4), f16_idesc((int)n, 0, 1), k ? 1u : 0u);
-          }
-        }
-      });
-      if (!ok || !mine) continue;
-      for (uint32_t col = part + group * 16; col < end; col += 64) {
-        uint32_t v[16];
-        __syncwarp();
-        tmem_ld_32x16(lane_at + col - part, v);
-        tmem_ld_wait();
-        float x[16];
+    for (uint32_t col = group * 16; col < length16; col += 64) {
+      uint32_t v[16];
+      __syncwarp();
+      tmem_ld_32x16(lane_at + col, v);
+      tmem_ld_wait();
+      float x[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = __uint_as_float(v[j]) * (last ? rate : 1.f / kP);
-        if (!last) {
-          // (behind the last column X is zeros, and so are these)
-          if (row < side) keep(0, x_plane, col, x);
+      for (int j = 0; j < 16; ++j) x[j] = __uint_as_float(v[j]) * (last ? rate : 1.f / kP);
+      if (!last) {
+        // (behind the last column X is zeros, and so are these)
+        if (row < side) keep(0, x_plane, col, x);
+      } else {
+        const uint32_t r = min(row, side - 1);             // (no load behind a branch of a lane's own)
+        float* const w = m.weights + (tall ? col * m.cols + r : r * m.cols + col);
+        const uint32_t next = tall ? m.cols : 1;
+        if (!tall && (m.cols & 3) == 0 && (reinterpret_cast<uintptr_t>(m.weights) & 15) == 0 && col + 16 <= length) {
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) {
+            const float4 o = *reinterpret_cast<const float4*>(w + j);
+            x[j] = o.x * kept - x[j], x[j + 1] = o.y * kept - x[j + 1], x[j + 2] = o.z * kept - x[j + 2], x[j + 3] = o.w * kept - x[j + 3];
+          }
+          if (row < side)
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(w + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
         } else {
-          const uint32_t r = min(row, side - 1);           // (no load behind a branch of a lane's own)
-          const uint32_t next = tall ? m.cols : 1;
-          float* const w = m.weights + (uint64_t)(first + col) * next + (uint64_t)r * (tall ? 1 : m.cols);
-          if (!tall && (m.cols & 3) == 0 && (reinterpret_cast<uintptr_t>(m.weights) & 15) == 0 && col + 16 <= length) {
+          float o[16];
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-              const float4 o = *reinterpret_cast<const float4*>(w + j);
-              x[j] = o.x * kept - x[j], x[j + 1] = o.y * kept - x[j + 1], x[j + 2] = o.z * kept - x[j + 2], x[j + 3] = o.w * kept - x[j + 3];
-            }
-            if (row < side)
+          for (int j = 0; j < 16; ++j) o[j] = w[min((uint32_t)j, length - 1 - col) * next];
 #pragma unroll
-              for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(w + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
-          } else {
-            float o[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] = w[min((uint32_t)j, length - 1 - col) * next];
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (row < side && col + j < length) w[j * next] = o[j] * kept - x[j];
-          }
+          for (int j = 0; j < 16; ++j)
+            if (row < side && col + j < length) w[j * next] = o[j] * kept - x[j];
         }
       }
     }
@@ -1052,10 +954,6 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
     const long long t0 = clock64();
     while (clock64() - t0 < 2000000ll) { }
     __syncthreads();
-  }
-  if constexpr (SEVERAL) {                                 // (no CTA leaves while another one reads its shared memory)
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-    cluster_wait();
   }
   if (warp == 0) {
     tc_fence_after();
@@ -1336,51 +1234,39 @@ int launch_product(const std::vector<Kin>& kin, const std::vector<std::pair<size
   return POLAR_B200_OK;
 }
 
-// Where a matrix is done: 0 by products with the other ones, else how many CTAs do it alone.  One that several CTAs hold goes along with the
-// products where there are any, for which it costs nothing (784 x 4096 and 4096 x 10: 266 us), and alone takes a third of their time.
-uint64_t alone(const One& o, bool products) {
-  const uint64_t ctas = ctas_of(o.rows, o.cols);
-  return ctas > 1 && products ? 0 : ctas;
-}
-// The matrices of the call: first those of the products, longest sums first, in groups that end at `ends`, then those that CTAs do alone, the most CTAs first.  True: there
-// are products.
-bool matrices_of(const polar_b200_muon_tensor* tensors, uint64_t count, std::vector<One>* all, std::vector<size_t>* ends) {
-  bool products = false;
+// The matrices of the call, longest sums first, and the groups they are done in; behind the last group's end the small ones.
+void matrices_of(const polar_b200_muon_tensor* tensors, uint64_t count, std::vector<One>* all, std::vector<size_t>* ends, bool large_only) {
   all->reserve(count);
   for (uint64_t i = 0; i < count; ++i) {
     const polar_b200_muon_tensor& t = tensors[i];
-    if (!t.rows || !t.cols || !t.matrices) continue;
-    products = products || ctas_of(t.rows, t.cols) == 0;
-    for (uint64_t z = 0; z < t.matrices; ++z) {
+    if (large_only && is_small(t.rows, t.cols)) continue;
+    for (uint64_t z = 0; z < t.matrices && t.rows && t.cols; ++z) {
       const uint64_t at = z * t.rows * t.cols;
       all->push_back(One{t.weights + at, t.gradient + at, t.momentum + at, t.rows, t.cols, t.weight_decay, t.scale});
     }
   }
-  std::stable_sort(all->begin(), all->end(), [&](const One& a, const One& b) {
-    const uint64_t sa = alone(a, products), sb = alone(b, products);
+  std::stable_sort(all->begin(), all->end(), [](const One& a, const One& b) {
+    const bool sa = is_small(a.rows, a.cols), sb = is_small(b.rows, b.cols);
     const uint64_t la = std::max(a.rows, a.cols), lb = std::max(b.rows, b.cols);
-    if (!sa != !sb) return !sa;
-    return sa != sb ? sa > sb : la != lb ? la > lb : a.rows != b.rows ? a.rows > b.rows : a.cols > b.cols;
+    return sa != sb ? sb : la != lb ? la > lb : a.rows != b.rows ? a.rows > b.rows : a.cols > b.cols;
   });
   uint64_t bytes = 0;
   size_t large = all->size();
-  while (large && alone((*all)[large - 1], products)) --large;
+  while (large && is_small((*all)[large - 1].rows, (*all)[large - 1].cols)) --large;
   for (size_t i = 0; i < large; ++i) {
     const uint64_t more = bytes_of((*all)[i].rows, (*all)[i].cols);
     if (bytes && bytes + more > kGroupBytes) ends->push_back(i), bytes = 0;
     bytes += more;
   }
   if (large) ends->push_back(large);
-  return products;
 }
 
-// Matrices that `ctas` CTAs each do alone.
-template <int N, bool SEVERAL>
-int launch_small(const std::vector<One>& all, size_t from, size_t to, uint32_t ctas, const polar_b200_muon_options& o, int* status, cudaStream_t st) {
+template <int N>
+int launch_small(const std::vector<One>& all, size_t from, size_t to, const polar_b200_muon_options& o, int* status, cudaStream_t st) {
   static thread_local SmallTable<N> t;
   t.lr = o.lr, t.momentum = o.momentum, t.a = o.a, t.b = o.b, t.c = o.c, t.nesterov = o.nesterov, t.steps = o.steps, t.schedule = o.schedule;
-  t.status = status, t.wait_ns = wait_limit_ns(2000000000ull), t.ctas = ctas;
-  cudaError_t e = cudaFuncSetAttribute(small_kernel<N, SEVERAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmallBytes);
+  t.status = status, t.wait_ns = wait_limit_ns(2000000000ull);
+  cudaError_t e = cudaFuncSetAttribute(small_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmallBytes);
   if (e != cudaSuccess) return fail(POLAR_B200_ERR_CUDA, "fmuon: small matrices", e);
   while (from < to) {
     const size_t n = std::min<size_t>(to - from, N);
@@ -1389,20 +1275,17 @@ int launch_small(const std::vector<One>& all, size_t from, size_t to, uint32_t c
       t.m[i] = Small{q.weights, q.gradient, q.momentum, (uint32_t)q.rows, (uint32_t)q.cols, q.decay, q.scale};
     }
     cudaLaunchConfig_t c = {};
-    c.gridDim = dim3((unsigned)n * ctas);
+    c.gridDim = dim3((unsigned)n);
     c.blockDim = dim3(kSmallThreads);
     c.dynamicSmemBytes = kSmallBytes;
     c.stream = st;
-    cudaLaunchAttribute at[2];
+    cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
-    at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = ctas;
-    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     c.attrs = at;
-    c.numAttrs = SEVERAL ? 2 : 1;
+    c.numAttrs = 1;
     void* args[1] = {&t};
-    e = cudaLaunchKernelExC(&c, reinterpret_cast<const void*>(small_kernel<N, SEVERAL>), args);
+    e = cudaLaunchKernelExC(&c, reinterpret_cast<const void*>(small_kernel<N>), args);
     if (e != cudaSuccess) {
       cudaGetLastError();
       return fail(POLAR_B200_ERR_CUDA, "fmuon: small matrices", e);
@@ -1543,7 +1426,7 @@ uint64_t polar_b200_fmuon_workspace_bytes(const polar_b200_muon_tensor* tensors,
   try {
     std::vector<One> all;
     std::vector<size_t> ends;
-    matrices_of(tensors, count, &all, &ends);
+    matrices_of(tensors, count, &all, &ends, true);
     return workspace_of(all, ends);
   } catch (const std::exception&) {
     return 0;
@@ -1570,7 +1453,7 @@ int polar_b200_fmuon(const polar_b200_muon_tensor* tensors, uint64_t count, cons
     if (!muon_independent(tensors, count, o->schedule)) return fail(POLAR_B200_ERR_INVALID, "fmuon: what is written overlaps something else");
     std::vector<One> all;
     std::vector<size_t> ends;
-    const bool products = matrices_of(tensors, count, &all, &ends);
+    matrices_of(tensors, count, &all, &ends, false);
     const uint64_t need = workspace_of(all, ends);
     if (workspace && (workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
       return fail(POLAR_B200_ERR_WORKSPACE, "workspace too small or not 256-byte aligned");
@@ -1588,15 +1471,10 @@ int polar_b200_fmuon(const polar_b200_muon_tensor* tensors, uint64_t count, cons
       if (rc) break;
       from = to;
     }
-    while (rc == POLAR_B200_OK && from < all.size()) {
-      const uint32_t ctas = (uint32_t)alone(all[from], products);
-      size_t to = from;
-      while (to < all.size() && alone(all[to], products) == ctas) ++to;
+    if (rc == POLAR_B200_OK && from < all.size()) {
       int* status = device_status_word(&rc);
-      if (rc) break;
-      auto go = [&](auto some, auto more) { return (to - from <= kFewSmall ? some : more)(all, from, to, ctas, *o, status, st); };
-      rc = ctas > 1 ? go(launch_small<kFewSmall, true>, launch_small<kManySmall, true>) : go(launch_small<kFewSmall, false>, launch_small<kManySmall, false>);
-      from = to;
+      if (!rc) rc = all.size() - from <= kFewSmall ? launch_small<kFewSmall>(all, from, all.size(), *o, status, st)
+                                                   : launch_small<kManySmall>(all, from, all.size(), *o, status, st);
     }
     if (own) {
       cudaError_t e = scratch_free(own, st);

@@ -82,7 +82,7 @@ def step(d, ts, lr=0.5, **k):
 SHAPES = [(1, 1), (1, 2), (2, 1), (1, 1000), (1000, 1), (3, 5), (5, 3), (16, 16), (31, 33), (33, 31), (63, 65), (64, 64), (64, 128), (128, 64), (127, 129), (128, 128),
           (129, 127), (128, 1000), (1000, 128), (130, 70), (70, 130), (255, 257), (256, 256), (257, 255), (300, 1000), (1000, 300), (384, 640), (640, 384), (513, 511), (10, 4096),
           (4096, 10), (777, 1511), (1511, 777), (1024, 1024), (65, 5000), (5000, 65), (1280, 128), (2048, 512),
-          # what one CTA holds ends at 128 x 256, 64 x 512, 32 x 1024 and 16 x 2048, and what eight hold at eight times as much
+          # what one CTA holds ends at 128 x 256 and 64 x 512; far longer than wide beyond that
           (128, 300), (128, 512), (512, 128), (127, 513), (128, 2048), (2048, 128), (128, 2049), (100, 1000), (1000, 100), (64, 4096), (4096, 64), (64, 4097), (65, 2048),
           (33, 3000), (3000, 33), (32, 1025), (32, 8192), (8200, 32), (16, 2049), (16, 16384), (16384, 16), (17, 2000), (16, 20000), (5, 9000), (9000, 5), (1, 16384), (2, 2050),
           (48, 700), (700, 48), (96, 1030), (81, 1999),
@@ -155,15 +155,14 @@ def test_more_shapes_than_a_launch_holds_and_more_matrices_than_a_table(d):
         check(nw, nm, *t)
 
 
-def test_matrices_of_several_ctas_beside_one_another(d):
-    # clusters of eight, four and two, and single CTAs; then the same with one among them that makes all but the small ones go the way of the products
+def test_narrow_and_small_matrices_beside_one_another(d):
     ts = [make(s, i) for i, s in enumerate([(128, 2000), (900, 100), (64, 700), (30, 8000), (60, 60), (16, 4000), (2, 5000), (128, 2000), (4, 120, 300)])]
     for (nw, nm), t in zip(step(d, ts), ts):
         check(nw, nm, *t)
     ts.append(make((300, 400), 20))
     for (nw, nm), t in zip(step(d, ts), ts):
         check(nw, nm, *t)
-    ts = [make((100, 600 + i), i) for i in range(70)]        # more than a small table holds
+    ts = [make((100, 100 + i), i) for i in range(70)]        # more than the smaller table of small ones holds
     for (nw, nm), t in list(zip(step(d, ts), ts))[::9]:
         check(nw, nm, *t)
 
