@@ -1019,9 +1019,9 @@ uint64_t chunk_of(uint64_t count) {
 }
 // Two rounds at a time where the shorter side is so much shorter (see `operations_of`): then there are three symmetric matrices, else two.
 bool in_pairs(uint64_t rows, uint64_t cols) { return std::max(rows, cols) >= 2 * std::min(rows, cols); }
-uint64_t bytes_of(uint64_t rows, uint64_t cols) {          // of one matrix: X twice and the symmetric ones, two planes each
+uint64_t bytes_of(uint64_t rows, uint64_t cols) {          // of one matrix: X twice and the symmetric ones, two planes each, and what is small, rounded up
   const uint64_t side = std::min(rows, cols);
-  return 2 * 2 * (2 * rows * up64(cols) + (in_pairs(rows, cols) ? 3 : 2) * side * up64(side)) + 5 * 256;
+  return 2 * 2 * (2 * rows * up64(cols) + (in_pairs(rows, cols) ? 3 : 2) * side * up64(side)) + kMostChunks * sizeof(double) + sizeof(Target) + 7 * 256;
 }
 // What one group of matrices may take; a step of more is done in several.
 constexpr uint64_t kGroupBytes = 3ull << 30;

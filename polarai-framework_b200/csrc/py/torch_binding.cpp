@@ -469,14 +469,15 @@ bool operations(PyObject* list, std::vector<polar_b200_op>* ops) {
   }
   return true;
 }
-// workspace_bytes(operations): what the most demanding one asks for; fmuon builtins in a row, which share their launches, ask together.
+// workspace_bytes(operations): what the most demanding one asks for; fmuon builtins in a row, which share their launches, ask together, but for
+// no more than 3 GiB, beyond which they are done in groups.
 BUILTIN(workspace_bytes) {
   std::vector<polar_b200_op> ops;
   if (n != 1 || !operations(args[0], &ops)) return nullptr;
   uint64_t need = 0, row = 0;
   for (const polar_b200_op& o : ops) {
     const uint64_t one = polar_b200_launch_workspace_bytes(o.name, o.args, o.argc);
-    row = std::strcmp(o.name, "fmuon") ? 0 : row + one;
+    row = std::strcmp(o.name, "fmuon") ? 0 : std::min<uint64_t>(row + one, 3ull << 30);
     need = std::max<uint64_t>({need, one, row});
   }
   return PyLong_FromUnsignedLongLong(need);

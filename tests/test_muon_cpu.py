@@ -76,6 +76,37 @@ def test_workspace(c):
     assert call(c, big, workspace=P << 8, workspace_bytes=n - 1) == 5 and call(c, big, workspace=(P << 8) + 16, workspace_bytes=n) == 5
 
 
+def test_workspace_of_steps_in_a_row(c):
+    """Steps in a row share a workspace: what all of them take together, but no more than a group of them."""
+    native = ge.load_package().capi.binding()
+    keep = []
+
+    def op(rows, cols):
+        given = [(rows, cols), (2,), 0.95, 1.0, 5.0, 0.0, 1.0, (rows, cols), (rows, cols)]
+        arr = (Arg * len(given))()
+        for a, x in zip(arr, given):
+            if isinstance(x, tuple):
+                shape = (ctypes.c_uint64 * len(x))(*x)
+                keep.append(shape)
+                a.is_tensor, a.tensor.dims, a.tensor.shape, a.tensor.data = 1, len(x), shape, P
+            else:
+                a.scalar = x
+        keep.append(arr)
+        return b"fmuon", ctypes.addressof(arr), len(given)
+
+    need = lambda *t: c.polar_b200_fmuon_workspace_bytes(tensors(*t), len(t))  # noqa: E731
+    for count, rows, cols in ((1, 300, 200), (3, 300, 200), (2, 1024, 4096), (40, 4096, 16384), (40, 8192, 8192), (3, 16384, 32768), (500, 129, 257)):
+        got = native.workspace_bytes([op(rows, cols) for _ in range(count)])
+        together = need(*[{"rows": rows, "cols": cols}] * count)
+        assert together <= got <= max(3 << 30, need({"rows": rows, "cols": cols}))
+    # what stands between them has a workspace of its own
+    fill = (Arg * 2)()
+    shape = (ctypes.c_uint64 * 1)(4)
+    fill[0].scalar, fill[1].is_tensor, fill[1].tensor.dims, fill[1].tensor.shape, fill[1].tensor.data = 1.0, 1, 1, shape, P
+    apart = native.workspace_bytes([op(300, 200), (b"ffill", ctypes.addressof(fill), 2), op(300, 200)])
+    assert apart == need({"rows": 300, "cols": 200})
+
+
 def test_by_name_patterns(c):
     keep = []
 
