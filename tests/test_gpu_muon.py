@@ -4,6 +4,7 @@ Tolerance of the update, in the Frobenius norm and relative: a product holds 22 
 sums are cut towards zero up to 24 times between two rounded additions, each time by less than 2^-23: 3.4e-6 of the terms' magnitude, whose
 cuts all have one direction.  15 products make 5.1e-5, and a round changes a relative error by |s p'(s) / p(s)|, which is 1 for small singular
 values s and below 2 where they have settled: 1e-4."""
+import ctypes
 import math
 
 import numpy as np
@@ -310,3 +311,50 @@ def test_by_name_and_in_a_program_with_its_neighbours(d):
     before = d.lib.launch_count()
     ex1.run()
     assert shared < 2 * (d.lib.launch_count() - before) + 20   # three in a row share their launches
+
+
+@pytest.mark.parametrize("short", [False, True])
+def test_steps_of_a_program_run_again_and_again_with_any_workspace(d, short):
+    """Four steps one after another of a program of short launches, which becomes a graph on the way; with the library's own scratch where the program's is too small."""
+    from polarai_framework_b200.capi import binding
+    from polarai_framework_b200.program import DeviceExecutor, Program
+    p = Program("updates")
+    shapes = {"U": (90, 600), "V": (300, 200), "W": (300, 200), "S": (40, 50)}
+    for n, s in shapes.items():
+        for k in ("", "d", "m"):
+            p.tensor(k + n, *s)
+    p.tensor("schedule", 2)
+    p.inputs = [k + n for n in shapes for k in ("", "d", "m")] + ["schedule"]
+    p.outputs = list(shapes)
+    rows = [["U", "V"], ["W"], ["S"]]
+    p.tensor("T", 90, 90)
+    for row in rows:
+        for n in row:
+            p.op("fmuon", "d" + n, "schedule", 0.9, 1.0, 5.0, 0.01, 0.7, n, "m" + n)
+        p.op("fmatmul_f_t", "dU", "dU", "T")
+    ex = DeviceExecutor(p)
+    rng = np.random.default_rng(13)
+    data = {n: rng.standard_normal(s).astype(np.float32) for n, s in p.tensors.items() if n not in ("schedule", "T")}
+    ex.set_inputs(**data, schedule=np.array([1, 0.5], np.float32))
+    eager = {n: tuple(torch.from_numpy(data[k + n]).cuda() for k in ("", "d", "m")) for n in shapes}
+    native = binding()
+    handle = None
+    if short:                                              # enough for the first matrix alone
+        need = native.workspace_bytes([(k, ctypes.addressof(a), n) for k, a, n in ex._compiled[:1]])
+        assert need < ex._ws_bytes
+        status, handle = native.create_program([(k, ctypes.addressof(a), n) for k, a, n in ex._compiled], ex._ws_ptr, need)
+        assert status == 0
+    torch.cuda.synchronize()
+    for _ in range(4):
+        if short:
+            assert d.lib.cdll.polar_b200_program_run(handle, torch.cuda.current_stream().cuda_stream) == 0
+        else:
+            ex.run()
+        for row in rows:
+            d.fmuon(*([eager[n][i] for n in row] for i in range(3)), lr=0.5, momentum=0.9, weight_decay=0.01, scale=0.7)
+    torch.cuda.synchronize()
+    assert d.device_status() == 0
+    for n, (w, _, m) in eager.items():
+        assert torch.equal(ex.t[n], w) and torch.equal(ex.t["m" + n], m)
+    if short:
+        d.lib.cdll.polar_b200_program_destroy(handle)
