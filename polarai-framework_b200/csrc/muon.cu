@@ -180,7 +180,9 @@ struct Cfg {
   static constexpr int kStages = BN == 256 ? 3 : 5;
   static constexpr int kSlots = SPLIT ? 0 : 2;             // blocks on their way to memory, for each warp of the epilogue
   static constexpr uint32_t kWarpBytes = kSlots * kSlotBytes;
-  static constexpr uint32_t kTileBytes = kStages * kStageBytes, kTurnBytes = kEpilogueWarps * kWarpBytes;
+  static constexpr uint32_t kTileBytes = kStages * kStageBytes;
+  // behind the slabs: those blocks; or what the other CTAs of a cluster, up to seven, send
+  static constexpr uint32_t kTurnBytes = SPLIT ? BM * BN * 4 / 8 * 7 : kEpilogueWarps * kWarpBytes;
   static constexpr uint32_t kBytes = kTileBytes + kTurnBytes + 1024 + 256;
   static_assert(kBytes <= 227 * 1024, "shared memory");
 };
@@ -271,6 +273,13 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, Operand a, uint32_t a_u
 // fp32 sums of fp16 operands (format 0 of both), 128 x n.
 __device__ __forceinline__ uint32_t f16_idesc(int n, int a_mn, int b_mn) {
   return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+}
+// Shared memory of this CTA to that of another one of its cluster, whose mbarrier (at the same place as `bar` here) counts the bytes.
+__device__ __forceinline__ void send(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar, uint32_t rank) {
+  uint32_t there, count;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(dst), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(count) : "r"(bar), "r"(rank));
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(there), "r"(src), "r"(bytes), "r"(count) : "memory");
 }
 __device__ __forceinline__ Target target_of(const Product& p, const Shape& q, const Place& at) {
   return q.kind == kUpdate ? p.targets[q.first_target + at.z] : Target{};
@@ -404,7 +413,8 @@ __device__ __forceinline__ void finish(const Shape& q, const Place& at, const Ta
   }
 }
 // 16 columns of a row, of which the CTAs of a cluster that shares a tile have few: straight to memory.
-__device__ __forceinline__ void finish16(const Shape& q, const Place& at, const Target& target, float lr, uint32_t r0, uint32_t c0, int lane, uint32_t (&v)[16]) {
+__device__ __forceinline__ void finish16(const Shape& q, const Place& at, const Target& target, float lr, uint32_t r0, uint32_t c0, int lane, uint32_t (&v)[16],
+                                         const Beside& beside) {
   const uint32_t row = r0 + lane, block = c0 & ~31u;
   if (c0 >= q.n || r0 >= q.m) return;
   if (q.kind == kSymmetric && block < r0) return;
@@ -432,7 +442,7 @@ __device__ __forceinline__ void finish16(const Shape& q, const Place& at, const 
   }
   __half* const matrix = q.out + 2 * at.z * q.plane;
   uint32_t hi[8], lo[8];
-  complete(q, row, c0, beside16(q, at, row, c0), v);
+  complete(q, row, c0, beside, v);
   split16(v, hi, lo);
   if (row < q.m) {                                         // (columns behind the last one lie in the row's padding)
     float* const out = reinterpret_cast<float*>(matrix + (uint64_t)row * q.pitch + c0);
@@ -475,13 +485,18 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
   auto empty = [&](int s) { return bar_base + 8u * (S + s); };
   auto acc_full = [&](int a) { return bar_base + 8u * (2 * S + a); };
   auto acc_empty = [&](int a) { return bar_base + 8u * (2 * S + 2 + a); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + C::kTileBytes + C::kTurnBytes + 8 * (2 * S + 4));
+  const uint32_t received = bar_base + 8u * (2 * S + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + C::kTileBytes + C::kTurnBytes + 8 * (2 * S + 5));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = uniform_warp();
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
     for (int a = 0; a < 2; ++a) mbar_init(acc_full(a), 1), mbar_init(acc_empty(a), kEpilogueWarps);
+    if (SPLIT) {
+      mbar_init(received, 1);
+      mbar_expect_tx(received, BM * BN * 4 / p.splits * (p.splits - 1));
+    }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -498,7 +513,9 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  if (SPLIT) cluster_arrive();                             // (nothing is sent before the receiver's barrier is there)
   pdl_enter();
+  if (SPLIT) cluster_wait();
   const uint32_t rank = SPLIT ? cluster_rank() : 0, splits = SPLIT ? p.splits : 1;
   const uint32_t first = SPLIT ? blockIdx.x / splits : blockIdx.x, step = SPLIT ? p.tiles : gridDim.x;
   auto slabs_of = [&](const Shape& q, int* end) {          // the CTA's
@@ -562,12 +579,43 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
         __syncwarp();
         if (lane == 0) mbar_arrive(acc_empty(as));
       }
-      if (!ok) break;
+      if (!SPLIT && !ok) break;                            // (SPLIT: all eight warps meet below, whatever has given up; there is one tile)
       if constexpr (SPLIT) {
-        // (the slabs have been read: the last product has been waited for)
-        float* const shared = reinterpret_cast<float*>(smem_gen);
+        // Each CTA completes its share of the columns: the sums of the others' go to them, theirs come here.
+        // (The slabs have been read: the last product has been waited for.)
+        const uint32_t cols = BN / splits, share = cols * BM * 4;
+        uint4* const mine = reinterpret_cast<uint4*>(smem_gen);   // four neighbours of a row to a place, rows side by side
 #pragma unroll
-        for (int j = 0; j < BN / 2; ++j) shared[(half * (BN / 2) + j) * BM + quarter * 32 + lane] = __uint_as_float(sum[j]);
+        for (int j = 0; j < BN / 8; ++j)
+          mine[(half * (BN / 8) + j) * BM + quarter * 32 + lane] = make_uint4(sum[4 * j], sum[4 * j + 1], sum[4 * j + 2], sum[4 * j + 3]);
+        fence_async_smem();
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogueWarps) : "memory");
+        if (ok && warp == 4 && lane < (int)splits && lane != (int)rank)
+          send(smem_base + C::kTileBytes + (rank - (rank > (uint32_t)lane)) * share, smem_base + lane * share, share, received, lane);
+        const Target target = target_of(p, q, at);
+        const float4* const sent = reinterpret_cast<const float4*>(smem_gen + C::kTileBytes);
+        // pieces of 32 rows and 16 columns
+        for (uint32_t piece = warp - 4; ok && piece < cols / 4; piece += kEpilogueWarps) {
+          const uint32_t rows = piece & 3, c = piece / 4 * 16, from = c / 4 * BM + rows * 32 + lane;
+          const Beside now = beside16(q, at, (uint32_t)at.m0 + rows * 32 + lane, (uint32_t)at.n0 + rank * cols + c);
+          ok = mbar_wait(received, 0, abort_flag, p.status, 705, p.wait_ns);
+          if (!ok) break;
+          float v[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = 0.f;
+          for (uint32_t r = 0; r < splits; ++r) {
+            const float4* const x = r == rank ? reinterpret_cast<const float4*>(mine) + rank * (share / 16) : sent + (r - (r > rank)) * (share / 16);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float4 y = x[from + j * BM];
+              v[4 * j] += y.x, v[4 * j + 1] += y.y, v[4 * j + 2] += y.z, v[4 * j + 3] += y.w;
+            }
+          }
+          uint32_t bits[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) bits[j] = __float_as_uint(v[j]);
+          finish16(q, at, target, lr, (uint32_t)at.m0 + rows * 32, (uint32_t)at.n0 + rank * cols + c, lane, bits, now);
+        }
       } else {
         finish<BN / 2>(q, at, target_of(p, q, at), lr, r0, c0, lane, sum, beside, place, stores);
         __syncwarp();
@@ -648,35 +696,6 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
 
   tc_fence_before();
   __syncthreads();
-  if constexpr (SPLIT) {
-    cluster_arrive();
-    cluster_wait();
-    if (warp >= 4) {
-      const Place at = place_of<BN>(p, first);
-      const Shape& q = p.s[at.shape];
-      const Target target = target_of(p, q, at);
-      const float* const shared = reinterpret_cast<const float*>(smem_gen);
-      // pieces of 32 rows and 16 columns
-      for (uint32_t piece = rank * kEpilogueWarps + warp - 4; piece < 4 * BN / 16; piece += splits * kEpilogueWarps) {
-        const uint32_t quarter = piece & 3, c = piece / 4 * 16;
-        uint32_t v[16];
-        float x[4][16];                                    // four CTAs' sums on their way
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = 0;
-        for (uint32_t r = 0; r < splits; r += 4) {         // (two, four or eight of them)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) x[i][j] = ld_cluster(shared + (c + j) * BM + quarter * 32 + lane, min(r + i, splits - 1));
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            v[j] = __float_as_uint(__uint_as_float(v[j]) + x[0][j] + x[1][j] + (splits > 2 ? x[2][j] + x[3][j] : 0.f));
-        }
-        finish16(q, at, target, lr, (uint32_t)at.m0 + quarter * 32, (uint32_t)at.n0 + c, lane, v);
-      }
-    }
-    __syncthreads();
-  }
   if (*abort_flag) {
     // let copies and products in flight finish before the memory that they use goes away
     const long long t0 = clock64();
@@ -684,8 +703,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
     __syncthreads();
   }
   if constexpr (SPLIT) {
-    __syncthreads();
-    // no CTA leaves while another one reads its shared memory; nothing that was written has to be seen by then (with a release, which waits for the stores, 1 us more)
+    // no CTA leaves before all have what it has sent; nothing that was written has to be seen by then (with a release, which waits for the stores, 1 us more)
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     cluster_wait();
   }
