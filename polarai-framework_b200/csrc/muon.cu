@@ -102,21 +102,36 @@ __global__ void __launch_bounds__(kThreads) momentum_kernel(const __grid_constan
     const float u = t.nesterov ? fmaf(t.momentum, v, g) : v;
     sum += (double)u * (double)u;
   };
+  // (four loads on their way before the first store, past which none moves by itself, and none behind a branch: what lies behind the end reads the end)
+  uint64_t i = from + threadIdx.x;
   if (vectors) {
-#pragma unroll 4
-    for (uint64_t i = from + 4 * threadIdx.x; i < to; i += 4 * kThreads) {
-      if (i + 4 <= to) {
-        const float4 g = *reinterpret_cast<const float4*>(m.gradient + i);
-        float4 v = *reinterpret_cast<const float4*>(m.momentum + i);
-        one(g.x, v.x), one(g.y, v.y), one(g.z, v.z), one(g.w, v.w);
-        *reinterpret_cast<float4*>(m.momentum + i) = v;
-      } else {
-        for (uint64_t e = i; e < to; ++e) one(m.gradient[e], m.momentum[e]);
+    const uint64_t end = from + (to - from) / 4 * 4;
+    for (uint64_t first = from + 4 * threadIdx.x; first < end; first += 16 * kThreads) {
+      float4 g[4], v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint64_t at = min(first + 4 * kThreads * k, end - 4);
+        g[k] = *reinterpret_cast<const float4*>(m.gradient + at), v[k] = *reinterpret_cast<const float4*>(m.momentum + at);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (first + 4 * kThreads * k >= end) break;
+        one(g[k].x, v[k].x), one(g[k].y, v[k].y), one(g[k].z, v[k].z), one(g[k].w, v[k].w);
+        *reinterpret_cast<float4*>(m.momentum + first + 4 * kThreads * k) = v[k];
       }
     }
-  } else {
-#pragma unroll 4
-    for (uint64_t i = from + threadIdx.x; i < to; i += kThreads) one(m.gradient[i], m.momentum[i]);
+    i = end + threadIdx.x;
+  }
+  for (; i < to; i += 4 * kThreads) {
+    float g[4], v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) g[k] = m.gradient[min(i + kThreads * k, to - 1)], v[k] = m.momentum[min(i + kThreads * k, to - 1)];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (i + kThreads * k >= to) break;
+      one(g[k], v[k]);
+      m.momentum[i + kThreads * k] = v[k];
+    }
   }
   sum = block_sum(sum, slots);
   if (threadIdx.x == 0) t.partial[t.chunks_before + blockIdx.x] = sum;
@@ -143,25 +158,45 @@ __global__ void __launch_bounds__(kThreads) begin_kernel(const __grid_constant__
   const uint64_t from = (uint64_t)chunk * m.chunk, to = min(from + m.chunk, m.count);
   const bool vectors = ((reinterpret_cast<uintptr_t>(m.gradient) | reinterpret_cast<uintptr_t>(m.momentum)) & 15) == 0 && (m.cols & 3) == 0;
   auto value = [&](float g, float v) { return (float)((double)(t.nesterov ? fmaf(t.momentum, v, g) : v) * by); };
-  if (vectors) {
-#pragma unroll 2
-    for (uint64_t i = from + 4 * threadIdx.x; i < to; i += 4 * kThreads) {
-      const float4 g = *reinterpret_cast<const float4*>(m.gradient + i), v = *reinterpret_cast<const float4*>(m.momentum + i);
-      const uint64_t row = i / m.cols;
-      __half* x = m.x + row * m.pitch + (i - row * m.cols);
-      union { __half h[4]; uint2 bits; } hi, lo;
+  // places in 32 bits from the chunk's first row on; loads before stores as above
+  const uint64_t row0 = from / m.cols;
+  const uint32_t in_row = (uint32_t)(from - row0 * m.cols), n = (uint32_t)(to - from);
+  const float *const gradient = m.gradient + from, *const momentum = m.momentum + from;
+  auto place = [&](uint32_t i) {
+    const uint32_t row = (in_row + i) / m.cols;
+    return m.x + (row0 + row) * m.pitch + (in_row + i - row * m.cols);
+  };
+  if (vectors) {                                           // (the chunk is vectors: whole rows are)
+    for (uint32_t first = 4 * threadIdx.x; first < n; first += 8 * kThreads) {
+      float4 g[2], v[2];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) split(value((&g.x)[k], (&v.x)[k]), &hi.h[k], &lo.h[k]);
-      *reinterpret_cast<uint2*>(x) = hi.bits;
-      *reinterpret_cast<uint2*>(x + m.plane) = lo.bits;
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t at = min(first + 4 * kThreads * k, n - 4);
+        g[k] = *reinterpret_cast<const float4*>(gradient + at), v[k] = *reinterpret_cast<const float4*>(momentum + at);
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (first + 4 * kThreads * k >= n) break;
+        union { __half h[4]; uint2 bits; } hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) split(value((&g[k].x)[e], (&v[k].x)[e]), &hi.h[e], &lo.h[e]);
+        __half* const x = place(first + 4 * kThreads * k);
+        *reinterpret_cast<uint2*>(x) = hi.bits;
+        *reinterpret_cast<uint2*>(x + m.plane) = lo.bits;
+      }
     }
     return;
   }
-#pragma unroll 4
-  for (uint64_t i = from + threadIdx.x; i < to; i += kThreads) {
-    const uint64_t row = i / m.cols;
-    __half* x = m.x + row * m.pitch + (i - row * m.cols);
-    split(value(m.gradient[i], m.momentum[i]), x, x + m.plane);
+  for (uint32_t first = threadIdx.x; first < n; first += 4 * kThreads) {
+    float g[4], v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) g[k] = gradient[min(first + kThreads * k, n - 1)], v[k] = momentum[min(first + kThreads * k, n - 1)];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (first + kThreads * k >= n) break;
+      __half* const x = place(first + kThreads * k);
+      split(value(g[k], v[k]), x, x + m.plane);
+    }
   }
 }
 
