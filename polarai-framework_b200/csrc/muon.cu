@@ -30,6 +30,7 @@ namespace {
 using namespace tc;
 
 constexpr float kX = 32768.f, kG = 32768.f, kP = 16384.f;  // what X, G and P are held times
+constexpr float kQ = 4096.f;                               // and the product of two P: kBoundP^2 * 2^12 is below 65504
 constexpr float kBound = 1.4f, kBoundP = 3.98f;            // largest singular value of X, of P: 1.4^2 * 2^15 and 3.98 * 2^14 are below 65504
 
 // ---- the passes before the products
@@ -1019,6 +1020,186 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
   }
 }
 
+// ---- narrow matrices: what lies between two products with X, by one CTA for each
+
+// The symmetric matrices of a matrix with a short side of up to 128 fit a CTA's shared memory: P, T, G', P' and Q of two rounds (or P of one), 1 to 1.5 us each, in
+// one launch for five of some 7.  Matrices as in the kernel above, 128 rows.
+struct Chain {
+  const __half* g;                                         // matrix z: planes 2 z (hi) and 2 z + 1 (lo)
+  __half* out;
+  uint64_t plane;
+  uint32_t side, pitch, first;                             // first: its first CTA
+};
+constexpr int kChains = 64;
+struct ChainTable {
+  float a, b, c;
+  int two;
+  uint32_t shapes;
+  int* status;
+  unsigned long long wait_ns;
+  Chain s[kChains];
+};
+constexpr uint32_t kSquare = 64 * 1024;                    // 128 x 128 pairs
+constexpr uint32_t kChainBytes = 3 * kSquare + 1024 + 256;
+
+__global__ void __launch_bounds__(kSmallThreads, 1) chain_kernel(const __grid_constant__ ChainTable t) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* const smem = smem_raw + (smem_base - smem_u32(smem_raw));
+  const uint32_t bar = smem_base + 3 * kSquare;
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + 3 * kSquare + 8);
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = uniform_warp(), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(bar, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) {
+    tmem_alloc(smem_u32(tmem_slot), 128);
+    tmem_relinquish();
+  }
+  uint32_t shape = 0;
+  while (shape + 1 < t.shapes && t.s[shape + 1].first <= blockIdx.x) ++shape;
+  const Chain& q = t.s[shape];
+  const uint64_t first = 2 * (uint64_t)(blockIdx.x - q.first) * q.plane;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  pdl_enter();
+
+  const uint32_t side = q.side, side16 = (side + 15) / 16 * 16, row = (warp & 3) * 32 + lane, col = (warp >> 2) * 32;
+  const bool mine = (warp & 3) * 32 < side && col < side16;   // a block of 32 x 32 (the whole warp)
+  constexpr uint32_t kChunk64 = 128 * 128, kPlane = kSquare / 2;
+  const Operand k_major = make_desc(0, 16, 1024, 2);
+  const bool leader = elect_one();
+  uint32_t phase = 0;
+  // The product of the matrices in squares l and r.
+  auto product = [&](uint32_t l, uint32_t r) {
+    fence_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag) return false;
+    if (warp == 0) {
+      tc_fence_after();
+      const uint32_t base = (smem_base & 0x3FFFFu) >> 4, lo = kPlane >> 4, idesc = f16_idesc((int)side16, 0, 0);
+      if (leader) {
+        for (uint32_t k = 0; k < side16 / 16; ++k) {
+          const uint32_t at = (k / 4 * kChunk64 + k % 4 * 32) >> 4, a = base + (l * kSquare >> 4) + at, b = base + (r * kSquare >> 4) + at;
+          mma_f16(tmem, k_major, a, k_major, b, idesc, k ? 1u : 0u);
+          mma_f16(tmem, k_major, a + lo, k_major, b, idesc, 1u);
+          mma_f16(tmem, k_major, a, k_major, b + lo, idesc, 1u);
+        }
+        tc_commit(bar);
+      }
+      __syncwarp();
+    }
+    mbar_wait(bar, phase, abort_flag, t.status, 721, t.wait_ns);
+    phase ^= 1;
+    tc_fence_after();
+    return true;
+  };
+  auto sums = [&](float* v) {
+    uint32_t bits[32];
+    tmem_ld_32x32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + col, bits);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(bits[j]);
+  };
+  // 32 columns of this thread's row into a square; behind the last column zeros, which are part of sums
+  auto keep = [&](uint32_t square, float* v) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = col + j < side ? v[j] : 0.f;
+    if (row >= side) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      union { __half h[8]; uint4 bits; } hi, lo;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) split(v[8 * i + j], &hi.h[j], &lo.h[j]);
+      uint8_t* const x = smem + square * kSquare + col / 64 * kChunk64 + row * 128 + (((col & 63) / 8 + i) ^ (row & 7)) * 16;
+      *reinterpret_cast<uint4*>(x) = hi.bits;
+      *reinterpret_cast<uint4*>(x + kPlane) = lo.bits;
+    }
+  };
+  auto polynomial = [&](const float* g, float* v) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = fmaf(t.c * (kP / (kG * kG)), v[j], t.b * (kP / kG) * g[j]) + (col + j == row ? t.a * kP : 0.f);
+  };
+  auto times = [&](float by, float* v) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] *= by;
+  };
+
+  float g[32], v[32];
+  if (mine) {
+    const __half* const in = q.g + first + (uint64_t)min(row, side - 1) * q.pitch + col;
+    uint4 hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) hi[i] = reinterpret_cast<const uint4*>(in)[i], lo[i] = reinterpret_cast<const uint4*>(in + q.plane)[i];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float2 x = __half22float2(reinterpret_cast<const __half2*>(hi)[j]), y = __half22float2(reinterpret_cast<const __half2*>(lo)[j]);
+      g[2 * j] = x.x + y.x, g[2 * j + 1] = x.y + y.y;
+    }
+    keep(0, g);
+  }
+  bool ok = product(0, 0);
+  if (mine && ok) {
+    sums(v);
+    polynomial(g, v);
+    if (t.two) keep(1, v);
+  }
+  if (t.two) {
+    ok = ok && product(1, 0);                              // T
+    if (mine && ok) {
+      sums(v);
+      times(1.f / kP, v);
+      keep(2, v);
+    }
+    ok = ok && product(1, 2);                              // G'
+    if (mine && ok) {
+      sums(g);
+      times(1.f / kP, g);
+      keep(0, g);
+    }
+    ok = ok && product(0, 0);                              // P'
+    if (mine && ok) {
+      sums(v);
+      polynomial(g, v);
+      keep(2, v);
+    }
+    ok = ok && product(2, 1);                              // Q
+    if (mine && ok) {
+      sums(v);
+      times(kQ / (kP * kP), v);
+    }
+  }
+  if (mine && ok && row < side) {                          // (columns behind the last one lie in the row's padding)
+    __half* const out = q.out + first + (uint64_t)row * q.pitch + col;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      union { __half h[8]; uint4 bits; } hi, lo;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) split(v[8 * i + j], &hi.h[j], &lo.h[j]);
+      reinterpret_cast<uint4*>(out)[i] = hi.bits;
+      reinterpret_cast<uint4*>(out + q.plane)[i] = lo.bits;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000ll) { }
+    __syncthreads();
+  }
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 128);
+  }
+}
+
 // ---- host side
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -1150,9 +1331,10 @@ int launch_tables(const std::vector<One>& all, size_t from, size_t to, const std
   return POLAR_B200_OK;
 }
 
-// One product of the matrices of a shape: of X (from x[from]) with itself, of symmetric matrices s[left] s[right] that commute, or of s[left] and X.
+// One product of the matrices of a shape: of X (from x[from]) with itself, of symmetric matrices s[left] s[right] that commute, or of s[left] and X; or all
+// products of symmetric matrices of a round, or of two, from s[left] to s[out].
 struct Operation {
-  enum { kGram, kProduct, kMove } what;
+  enum { kGram, kProduct, kMove, kChain, kChain2 } what;
   int left, right, out, add;                               // add: -1 for none
   float by, add_by, diagonal;
   bool last;
@@ -1161,16 +1343,16 @@ struct Operation {
 //   G, P, T = P G, G' = P T, P', Q = P' P, X <- Q X
 // are five products of the shorter side alone in place of two products with X (work of 3 short^2 long for one of 3 short^3): 1024 x 4096 takes three quarters
 // of the operations.  Not more rounds at a time: what rounding leaves in G for small singular values grows by a^2 in each further one.
-std::vector<Operation> operations_of(const Kin& k, const polar_b200_muon_options& o) {
+std::vector<Operation> operations_of(const Kin& k, const polar_b200_muon_options& o, bool chain) {
   std::vector<Operation> ops;
-  constexpr float kQ = 4096.f;                             // kBoundP^2 * 2^12 is below 65504
   auto product = [&](int l, int r, int out, float by) { ops.push_back(Operation{Operation::kProduct, l, r, out, -1, by, 0.f, 0.f, false}); };
   auto polynomial = [&](int g, int out) { ops.push_back(Operation{Operation::kProduct, g, g, out, g, o.c * (kP / (kG * kG)), o.b * (kP / kG), o.a * kP, false}); };
   for (uint32_t i = 0; i < o.steps;) {
     ops.push_back(Operation{Operation::kGram, 0, 0, 0, -1, kG / (kX * kX), 0.f, 0.f, false});
-    polynomial(0, 1);
     const bool two = i + 1 < o.steps && in_pairs(k.rows, k.cols);
-    if (two) {
+    if (chain) ops.push_back(Operation{two ? Operation::kChain2 : Operation::kChain, 0, 0, 1, -1, 0.f, 0.f, 0.f, false});
+    else polynomial(0, 1);
+    if (two && !chain) {
       product(1, 0, 2, 1.f / kP);                          // T as G: its eigenvalues are products of two singular values of X, before and after
       product(1, 2, 0, 1.f / kP);
       polynomial(0, 2);
@@ -1178,7 +1360,7 @@ std::vector<Operation> operations_of(const Kin& k, const polar_b200_muon_options
     }
     i += two ? 2 : 1;
     const float held = two ? kQ : kP;
-    ops.push_back(Operation{Operation::kMove, two ? 0 : 1, 0, 0, -1, i < o.steps ? 1.f / held : 1.f / (held * kX), 0.f, 0.f, i == o.steps});
+    ops.push_back(Operation{Operation::kMove, two && !chain ? 0 : 1, 0, 0, -1, i < o.steps ? 1.f / held : 1.f / (held * kX), 0.f, 0.f, i == o.steps});
   }
   return ops;
 }
@@ -1292,6 +1474,26 @@ int launch_product(const std::vector<Kin>& kin, const std::vector<std::pair<size
   return POLAR_B200_OK;
 }
 
+// The products of symmetric matrices between two with X, of all shapes.
+int launch_chain(const std::vector<Kin>& kin, const Operation& op, const polar_b200_muon_options& o, int* status, cudaStream_t st) {
+  static thread_local ChainTable t;
+  t.a = o.a, t.b = o.b, t.c = o.c, t.two = op.what == Operation::kChain2;
+  t.status = status, t.wait_ns = wait_limit_ns(2000000000ull);
+  cudaError_t e = cudaFuncSetAttribute(chain_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kChainBytes);
+  if (e != cudaSuccess) return fail(POLAR_B200_ERR_CUDA, "fmuon: narrow matrices", e);
+  for (size_t k = 0; k < kin.size();) {
+    uint32_t ctas = 0;
+    for (t.shapes = 0; k < kin.size() && t.shapes < kChains; ++k) {
+      const Kin& q = kin[k];
+      t.s[t.shapes++] = Chain{q.s[op.left], q.s[op.out], q.side * q.side_pitch, (uint32_t)q.side, (uint32_t)q.side_pitch, ctas};
+      ctas += (uint32_t)q.count;
+    }
+    const int rc = launch("fmuon: narrow matrices", chain_kernel, dim3(ctas), kSmallThreads, kChainBytes, st, t);
+    if (rc) return rc;
+  }
+  return POLAR_B200_OK;
+}
+
 // The matrices of the call, longest sums first, and the groups they are done in; behind the last group's end the small ones.
 void matrices_of(const polar_b200_muon_tensor* tensors, uint64_t count, std::vector<One>* all, std::vector<size_t>* ends, bool large_only) {
   all->reserve(count);
@@ -1370,11 +1572,19 @@ int run_group(const std::vector<One>& all, size_t from, size_t to, const polar_b
   std::vector<std::vector<Operation>> ops;
   std::vector<int> from_x(kin.size(), 0);
   size_t most = 0;
+  // (Beside larger matrices the products of narrow ones cost no launch of their own.)
+  bool chain = true;
+  for (const Kin& k : kin) chain = chain && k.side <= 128;
   for (const Kin& k : kin) {
-    ops.push_back(operations_of(k, o));
+    ops.push_back(operations_of(k, o, chain));
     most = std::max(most, ops.back().size());
   }
   for (size_t i = 0; i < most; ++i) {
+    if (ops[0][i].what == Operation::kChain || ops[0][i].what == Operation::kChain2) {   // (and so it is for all shapes: narrow ones go in pairs)
+      rc = launch_chain(kin, ops[0][i], o, status, st);
+      if (rc) return rc;
+      continue;
+    }
     std::vector<std::pair<size_t, Operation>> now;
     for (size_t k = 0; k < kin.size(); ++k)
       if (i < ops[k].size()) now.emplace_back(k, ops[k][i]);
