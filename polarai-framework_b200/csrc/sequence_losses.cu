@@ -7,7 +7,7 @@
 //   few tokens (kFew): everything by one CTA in one launch;
 //   else a pass over the ids (policy) or over all (pairs), one over the sequences, one over the tokens.
 // 600 tokens take 3.8 us (a launch), 131072 of 256 sequences 10.8, 8.4 M with 64-bit ids 52.5 (their 235 MB at a copy's rate 35.7): 12 for the ids, 36 for the
-// tokens at 55 % of the issue slots.  Pairs: 1500 tokens 5.4 us, 400001 12.5, 4.2 M of 128 sequences 23.5 (7.7): 9 to 10 each for sums and gradient.
+// tokens at 55 % of the issue slots.  Pairs: 1500 tokens 5.4 us, 400001 10.9, 4.2 M of 128 sequences 22.1 (7.7): 9 to 10 each for sums and gradient.
 // Every sum is taken in a fixed order, over a CTA's tokens in fp32 and beyond that, as of the sums over a sequence, in 64 bits.
 #include <algorithm>
 #include <cmath>
@@ -182,6 +182,17 @@ __device__ __forceinline__ float4 ld_l2(const float4* p) {
   asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
   return v;
 }
+template <int THREADS>
+__device__ void all_sums(const float4* partial, uint32_t ctas, double (&total)[4], double* slots) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) total[i] = 0;
+#pragma unroll 8
+  for (uint32_t c = threadIdx.x; c < ctas; c += THREADS) {
+    const float4 p = ld_l2(partial + c);
+    total[0] += p.x, total[1] += p.y, total[2] += p.z, total[3] += p.w;
+  }
+  sums4<THREADS>(total, slots);
+}
 // Leaves a CTA's sums and tells whether it was the last one to; then the sums of all CTAs are in `total` of its first thread, added in an
 // order that does not hang on which CTA was last.
 template <int THREADS>
@@ -195,14 +206,7 @@ __device__ bool last_sums(float4 mine, float4* partial, uint32_t ctas, uint32_t*
   __syncthreads();
   if (!last) return false;
   __threadfence();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) total[i] = 0;
-#pragma unroll 8
-  for (uint32_t c = threadIdx.x; c < ctas; c += THREADS) {
-    const float4 p = ld_l2(partial + c);
-    total[0] += p.x, total[1] += p.y, total[2] += p.z, total[3] += p.w;
-  }
-  sums4<THREADS>(total, slots);
+  all_sums<THREADS>(partial, ctas, total, slots);
   return true;
 }
 
@@ -772,9 +776,12 @@ __device__ __forceinline__ double sum_of(const Workspace& w, uint32_t s, uint64_
   return warp_sum(v) + w.tail[first];
 }
 
-// A warp per sequence; the last CTA writes the loss.
+// A warp per sequence.  The loss is written by the last CTA or, where the gradient's kernel comes next, by one more CTA of that, while nothing waits for it.
+__device__ __forceinline__ void write_loss(const Pairs& o, const double* total) {
+  o.loss[0] = (float)total[0], o.loss[1] = (float)total[1], o.loss[2] = (float)total[2];
+}
 template <class Id>
-__global__ void __launch_bounds__(kThreads) pairs_kernel(Packed<Id> p, Workspace w, Pairs o, float inv_count) {
+__global__ void __launch_bounds__(kThreads) pairs_kernel(Packed<Id> p, Workspace w, Pairs o, float inv_count, bool gradient_next) {
   __shared__ float slots[kThreads / 8];
   __shared__ double wide[kThreads / 8], sums[kThreads / 32];
   __shared__ uint64_t counts[kThreads / 32];
@@ -793,20 +800,30 @@ __global__ void __launch_bounds__(kThreads) pairs_kernel(Packed<Id> p, Workspace
     sum[0] = r.loss * inv_count, sum[1] = r.right * inv_count, sum[2] = r.gap * inv_count;
   }
   sums4<kThreads>(sum, slots);
+  if (gradient_next) {
+    if (threadIdx.x == 0) w.partial[blockIdx.x] = make_float4(sum[0], sum[1], sum[2], 0.f);
+    return;
+  }
   double total[4];
-  if (last_sums<kThreads>(make_float4(sum[0], sum[1], sum[2], 0.f), w.partial, gridDim.x, &w.shared->ticket, total, wide) && threadIdx.x == 0)
-    o.loss[0] = (float)total[0], o.loss[1] = (float)total[1], o.loss[2] = (float)total[2];
+  if (last_sums<kThreads>(make_float4(sum[0], sum[1], sum[2], 0.f), w.partial, gridDim.x, &w.shared->ticket, total, wide) && threadIdx.x == 0) write_loss(o, total);
 }
 
 template <class Id>
-__global__ void __launch_bounds__(kThreads) pairs_grad_kernel(Packed<Id> p, Workspace w, float* g_logprob, bool vectors) {
+__global__ void __launch_bounds__(kThreads) pairs_grad_kernel(Packed<Id> p, Workspace w, Pairs o, uint32_t partials, bool vectors) {
+  __shared__ double wide[kThreads / 8];
   pdl_enter();
+  if (blockIdx.x == 0) {
+    double total[4];
+    all_sums<kThreads>(w.partial, partials, total, wide);
+    if (threadIdx.x == 0) write_loss(o, total);
+    return;
+  }
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint64_t begin = p.offset(0), end = p.offset(p.sequences);
   Found found;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const uint64_t base = (uint64_t)blockIdx.x * kPass + h * (kPass / 2) + warp * 128, t = base + 4 * lane;
+    const uint64_t base = (uint64_t)(blockIdx.x - 1) * kPass + h * (kPass / 2) + warp * 128, t = base + 4 * lane;
     if (base >= end) return;
     uint32_t of[4];
     const uint32_t bits = w.bits[t / 32] >> (t & 31) & 15; // (the last tile's words are all there)
@@ -818,7 +835,7 @@ __global__ void __launch_bounds__(kThreads) pairs_grad_kernel(Packed<Id> p, Work
     else share.y = w.share[of[1]], share.z = w.share[of[2]], share.w = w.share[of[3]];
 #pragma unroll
     for (int k = 0; k < 4; ++k) (&g.x)[k] = bits >> k & 1 ? (&share.x)[k] : 0.f;
-    store4(g_logprob, g, t, begin, end, vectors);
+    store4(o.g_logprob, g, t, begin, end, vectors);
   }
 }
 
@@ -962,10 +979,12 @@ int run_pairs(const Packed<Id>& p, const Pairs& o, void* workspace, uint64_t wor
     const uint32_t tiles = (uint32_t)tiles_of(p.tokens);
     int rc = launch("fpreference_loss: sums", sums_kernel<Id>, dim3(tiles), kThreads, 0, st, p, w, o);
     if (rc) return rc;
-    rc = launch("fpreference_loss", pairs_kernel<Id>, dim3((p.sequences + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, st, p, w, o, inv_count);
-    if (rc || !o.g_logprob || !p.tokens) return rc;
-    return launch("fpreference_loss: gradient", pairs_grad_kernel<Id>, dim3((unsigned)((p.tokens + kPass - 1) / kPass)), kThreads, 0, st, p, w,
-                  o.g_logprob, aligned16(o.g_logprob));
+    const uint32_t ctas = (p.sequences + kThreads / 32 - 1) / (kThreads / 32);
+    const bool gradient = o.g_logprob && p.tokens;
+    rc = launch("fpreference_loss", pairs_kernel<Id>, dim3(ctas), kThreads, 0, st, p, w, o, inv_count, gradient);
+    if (rc || !gradient) return rc;
+    return launch("fpreference_loss: gradient", pairs_grad_kernel<Id>, dim3((unsigned)((p.tokens + kPass - 1) / kPass) + 1), kThreads, 0, st, p, w, o, ctas,
+                  aligned16(o.g_logprob));
   });
 }
 
