@@ -182,6 +182,12 @@ __device__ __forceinline__ float4 ld_l2(const float4* p) {
   asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
   return v;
 }
+// What this thread has written is seen by who takes a later ticket, and by those it meets at a barrier then.
+__device__ __forceinline__ uint32_t take_ticket(uint32_t* ticket) {
+  uint32_t before;
+  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(ticket) : "memory");
+  return before;
+}
 template <int THREADS>
 __device__ void all_sums(const float4* partial, uint32_t ctas, double (&total)[4], double* slots) {
 #pragma unroll
@@ -200,12 +206,10 @@ __device__ bool last_sums(float4 mine, float4* partial, uint32_t ctas, uint32_t*
   __shared__ bool last;
   if (threadIdx.x == 0) {
     partial[blockIdx.x] = mine;
-    __threadfence();
-    last = atomicAdd(ticket, 1u) == ctas - 1;
+    last = take_ticket(ticket) == ctas - 1;
   }
   __syncthreads();
   if (!last) return false;
-  __threadfence();
   all_sums<THREADS>(partial, ctas, total, slots);
   return true;
 }
