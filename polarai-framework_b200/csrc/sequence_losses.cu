@@ -6,7 +6,7 @@
 // that the second one reads an eighth of a byte in their place.
 //   few tokens (kFew): everything by one CTA in one launch;
 //   else a pass over the ids (policy) or over all (pairs), one over the sequences, one over the tokens.
-// 600 tokens take 3.8 us (a launch), 131072 of 256 sequences 10.8, 8.4 M with 64-bit ids 52.5 (their 235 MB at a copy's rate 35.7): 12 for the ids, 36 for the
+// 600 tokens take 3.8 us (a launch), 131072 of 256 sequences 10.4, 8.4 M with 64-bit ids 52.5 (their 235 MB at a copy's rate 35.7): 12 for the ids, 36 for the
 // tokens at 55 % of the issue slots.  Pairs: 1500 tokens 5.4 us, 400001 10.9, 4.2 M of 128 sequences 22.1 (7.7): 9 to 10 each for sums and gradient.
 // Every sum is taken in a fixed order, over a CTA's tokens in fp32 and beyond that, as of the sums over a sequence, in 64 bits.
 #include <algorithm>
