@@ -168,6 +168,14 @@ def test_narrow_and_small_matrices_beside_one_another(d):
         check(nw, nm, *t)
 
 
+@pytest.mark.parametrize("steps", [5, 2])
+def test_more_narrow_shapes_than_a_launch_holds(d, steps):
+    # short sides from 1 to 128, each matrix longer than one CTA holds, and stacks of them
+    ts = [make((1 + i * 127 // 69, 520 + 3 * i), i) for i in range(70)] + [make((600 + i, 9 + i), i) for i in range(3)] + [make((5, 33, 1111), 3), make((4, 128, 513), 4)]
+    for (nw, nm), t in zip(step(d, ts, steps=steps), ts):
+        check(nw, nm, *t, steps=steps)
+
+
 @pytest.mark.parametrize("offset", [1, 2, 3])
 @pytest.mark.parametrize("shape", [(60, 64), (130, 257), (512, 300), (300, 512), (60, 2000), (2000, 60)])
 def test_tensors_off_16_bytes(d, shape, offset):

@@ -324,6 +324,14 @@ def test_pairs_options(d, tokens, pairs):
     preference(d, b, beta=0.0)
 
 
+@pytest.mark.parametrize("tokens,pairs", [(2000, 9), (30000, 11), (30000, 9000), (9000, 3000)])
+def test_pairs_loss_is_the_same_without_the_gradient(d, tokens, pairs):
+    b = batch(36, tokens, 2 * pairs)
+    for k in ({}, {"average": True, "smoothing": 0.2}):
+        whole = preference(d, b, **k)
+        assert (whole == preference(d, b, gradient=False, **k)).all() and (whole == preference(d, b, rewards=False, **k)).all()
+
+
 @pytest.mark.parametrize("tokens", [1000, 30000])
 def test_pairs_masked_places_and_empty_sequences(d, tokens):
     b = batch(33, tokens, 12)
