@@ -6,8 +6,8 @@
 // that the second one reads an eighth of a byte in their place.
 //   few tokens (kFew): everything by one CTA in one launch;
 //   else a pass over the ids (policy) or over all (pairs), one over the sequences, one over the tokens.
-// 600 tokens take 3.8 us (a launch), 131072 of 256 sequences 10.4, 8.4 M with 64-bit ids 52.5 (their 235 MB at a copy's rate 35.7): 12 for the ids, 36 for the
-// tokens at 55 % of the issue slots.  Pairs: 1500 tokens 5.4 us, 400001 10.9, 4.2 M of 128 sequences 22.1 (7.7): 9 to 10 each for sums and gradient.
+// 600 tokens take 3.0 us (a launch), 131072 of 256 sequences 10.4, 8.4 M with 64-bit ids 52.5 (their 235 MB at a copy's rate 35.7): 12 for the ids, 36 for the
+// tokens at 55 % of the issue slots.  Pairs: 1500 tokens 3.9 us, 400001 10.9, 4.2 M of 128 sequences 22.1 (7.7): 9 to 10 each for sums and gradient.
 // Every sum is taken in a fixed order, over a CTA's tokens in fp32 and beyond that, as of the sums over a sequence, in 64 bits.
 #include <algorithm>
 #include <cmath>
@@ -538,26 +538,38 @@ struct FewTokens {
   }
   __device__ __forceinline__ bool counts(uint32_t t) const { return bits[t / 32] >> (t & 31) & 1; }
 };
-// Thread i's tokens are i, i + kFewThreads, ...
-template <class Id>
-__device__ __forceinline__ void few_tokens(const Packed<Id>& p, FewTokens& f) {
-  const uint32_t lane = threadIdx.x & 31;
+// Which tokens count, and the offsets, to be read behind a barrier.  Thread i's tokens are i, i + kFewThreads, ..., EACH at most; the result: which of its own count.
+// (One, two, four or eight: instructions that come from memory are much of such a launch.  600 tokens 3.0 us where eight take 3.4, 1500 in pairs 3.9 for 4.2.)
+template <int EACH, class Id>
+__device__ __forceinline__ uint32_t few_tokens(const Packed<Id>& p, FewTokens& f) {
   const uint32_t begin = (uint32_t)p.offset(0), end = (uint32_t)p.offset(p.sequences);
   for (uint32_t s = threadIdx.x; s <= p.sequences; s += kFewThreads) f.offsets[s] = (uint32_t)p.offset(s);
-  Id ids[kFewEach];
+  Id ids[EACH];
 #pragma unroll
-  for (int j = 0; j < kFewEach; ++j) {
+  for (int j = 0; j < EACH; ++j) {
     if (j * kFewThreads >= p.tokens) break;
     ids[j] = ld_id(p.ids + min((uint64_t)(j * kFewThreads + threadIdx.x), p.tokens - 1));
   }
+  uint32_t mine = 0;
 #pragma unroll
-  for (int j = 0; j < kFewEach; ++j) {
+  for (int j = 0; j < EACH; ++j) {
     const uint32_t t = j * kFewThreads + threadIdx.x;
-    const uint32_t b = j * kFewThreads < p.tokens ? __ballot_sync(0xffffffffu, t >= begin && t < end && !(ids[j] < Id(0))) : 0;
-    if (lane == 0) f.bits[t / 32] = b;
+    uint32_t b = 0;
+    if (j * kFewThreads < p.tokens) {
+      const bool counts = t >= begin && t < end && !(ids[j] < Id(0));
+      b = __ballot_sync(0xffffffffu, counts);
+      mine |= (uint32_t)counts << j;
+    }
+    if ((threadIdx.x & 31) == 0) f.bits[t / 32] = b;
   }
-  __syncthreads();
-  if (threadIdx.x < kFew / 32) {                           // the words' counts, summed up over the warps of the first 256 threads
+  return mine;
+}
+// How many count before each word, between two barriers.
+template <int EACH>
+__device__ __forceinline__ void few_counts(FewTokens& f) {
+  constexpr uint32_t kHeld = EACH * kFewThreads / 32;
+  const uint32_t lane = threadIdx.x & 31;
+  if (threadIdx.x < kHeld) {                               // the words' counts, summed up over the warps of those threads
     const uint32_t n = __popc(f.bits[threadIdx.x]);
     uint32_t upto = n;
 #pragma unroll
@@ -569,65 +581,88 @@ __device__ __forceinline__ void few_tokens(const Packed<Id>& p, FewTokens& f) {
     if (lane == 31) f.warps[threadIdx.x >> 5] = upto;
   }
   __syncthreads();
-  if (threadIdx.x < kFew / 32) {
+  if (threadIdx.x < kHeld) {
     uint32_t more = 0;
     for (uint32_t i = 0; i < threadIdx.x >> 5; ++i) more += f.warps[i];
     f.before[threadIdx.x] += more;
-    if (threadIdx.x == kFew / 32 - 1) f.before[kFew / 32] = f.before[threadIdx.x] + __popc(f.bits[threadIdx.x]);
+    if (threadIdx.x == kHeld - 1) f.before[kHeld] = f.before[threadIdx.x] + __popc(f.bits[threadIdx.x]);
   }
   __syncthreads();
 }
 
-template <class Id>
+template <class Id, int EACH>
 __global__ void __launch_bounds__(kFewThreads) policy_few_kernel(Packed<Id> p, Policy o) {
   __shared__ FewTokens f;
-  __shared__ float share[kFewSequences];
+  __shared__ float share[kFewSequences], advantage[kFewSequences];
   __shared__ double slots[kFewThreads / 8];
   __shared__ uint32_t live;
   if (threadIdx.x == 0) live = 0;
   pdl_enter();
-  // the first tokens' values are on their way while the ids are counted
+  // the first tokens' values and the sequences' are on their way while the ids are counted
   const uint32_t early = min(threadIdx.x, (uint32_t)p.tokens - 1);
   const float first_lp = ld_stream(o.logprob + early), first_old = ld_stream(o.old + early);
   const float first_ref = o.reference ? ld_stream(o.reference + early) : 0.f, first_entropy = o.entropy ? ld_stream(o.entropy + early) : 0.f;
-  few_tokens(p, f);
+  const uint32_t advantages = o.per_token ? (uint32_t)p.tokens : p.sequences;
+  static_assert(kFewSequences == 2 * kFewThreads, "two sequences to a thread");
+  const float first_adv = ld_stream(o.advantage + min(threadIdx.x, advantages - 1));
+  const float next_adv = ld_stream(o.advantage + min(threadIdx.x + kFewThreads, advantages - 1));
+  const uint32_t mine = few_tokens<EACH>(p, f);
+  advantage[threadIdx.x] = first_adv, advantage[threadIdx.x + kFewThreads] = next_adv;
+  __syncthreads();
   const bool look = o.by_sequence || !o.per_token;
   float even;
   if (o.by_sequence) {
-    uint32_t mine = 0;
+    few_counts<EACH>(f);
+    uint32_t full = 0;
     for (uint32_t s = threadIdx.x; s < p.sequences; s += kFewThreads) {
       const uint32_t from = f.offsets[s], to = f.offsets[s + 1], n = from < to ? f.until(to) - f.until(from) : 0;
       share[s] = n ? 1.f / (float)n : 0.f;
-      mine += n != 0;
+      full += n != 0;
     }
-    if (mine) atomicAdd(&live, mine);
+    if (full) atomicAdd(&live, full);
     __syncthreads();
     even = o.count > 0.f ? 1.f / o.count : 1.f / (float)live;
   } else {
-    const uint32_t n = f.before[kFew / 32];
+    uint32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < EACH * kFewThreads / 32; i += 32) n += __popc(f.bits[i + (threadIdx.x & 31)]);
+    n = __reduce_add_sync(0xffffffffu, n);
     even = o.count > 0.f ? 1.f / o.count : n ? 1.f / (float)n : 0.f;
   }
   const uint32_t begin = f.offsets[0], end = f.offsets[p.sequences];
-  double total[4] = {0, 0, 0, 0};
-  for (int j = 0; j < kFewEach && j * kFewThreads < (int)p.tokens; ++j) {
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < EACH && j * kFewThreads < (int)p.tokens; ++j) {
     const uint32_t t = j * kFewThreads + threadIdx.x;
     if (t < begin || t >= end) continue;
-    const bool counts = f.counts(t);
+    const bool counts = mine >> j & 1;
     float g = 0.f, weight = 0.f;
     if (counts) {
       const uint32_t s = look ? f.sequence(t, p.sequences) : 0;
       weight = o.by_sequence ? even * share[s] : even;
       const float lp = j ? o.logprob[t] : first_lp, old = j ? o.old[t] : first_old, ref = j ? (o.reference ? o.reference[t] : 0.f) : first_ref;
-      const Terms<1> e = terms<1>(o, &lp, &old, &ref, o.advantage + (o.per_token ? t : s));
-      total[0] += e.surrogate[0] * weight, total[1] += e.kl[0] * weight;
-      if (e.beyond[0] > 0.f && o.advantage[o.per_token ? t : s] != 0.f) total[3] += weight;
-      if (o.entropy) total[2] += (j ? o.entropy[t] : first_entropy) * weight;
+      const float a = !o.per_token ? advantage[s] : j ? o.advantage[t] : first_adv;
+      const Terms<1> e = terms<1>(o, &lp, &old, &ref, &a);
+      sum[0] += e.surrogate[0] * weight, sum[1] += e.kl[0] * weight;
+      if (e.beyond[0] > 0.f && a != 0.f) sum[3] += weight;
+      if (o.entropy) sum[2] += (j ? o.entropy[t] : first_entropy) * weight;
       g = e.slope[0] * weight;
     }
     if (o.g_logprob) o.g_logprob[t] = g;
     if (o.g_entropy) o.g_entropy[t] = -o.bonus * weight;
   }
-  sums4<kFewThreads>(total, slots);
+  // (shuffles are what this costs: warps without tokens take none, and the others 32 bits)
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (warp * 32 < p.tokens) sum[i] = warp_sum(sum[i]);
+    if (lane == 0) slots[warp * 4 + i] = sum[i];
+  }
+  __syncthreads();
+  if (warp != 0) return;
+  static_assert(kFewThreads == 32 * 32, "a lane for each warp's sums");
+  double total[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) total[i] = warp_sum(slots[lane * 4 + i]);
   if (threadIdx.x == 0) write_loss(o, total);
 }
 
@@ -843,7 +878,7 @@ __global__ void __launch_bounds__(kThreads) pairs_grad_kernel(Packed<Id> p, Work
   }
 }
 
-template <class Id>
+template <class Id, int EACH>
 __global__ void __launch_bounds__(kFewThreads) pairs_few_kernel(Packed<Id> p, Pairs o, float inv_count) {
   extern __shared__ double values[];
   __shared__ FewTokens f;
@@ -851,40 +886,46 @@ __global__ void __launch_bounds__(kFewThreads) pairs_few_kernel(Packed<Id> p, Pa
   __shared__ double slots[kFewThreads / 8];
   pdl_enter();
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float lp[kFewEach], ref[kFewEach];
+  float lp[EACH], ref[EACH];
 #pragma unroll
-  for (int j = 0; j < kFewEach; ++j) {
+  for (int j = 0; j < EACH; ++j) {
     if (j * kFewThreads >= p.tokens) break;
     const uint32_t t = min(j * kFewThreads + threadIdx.x, (uint32_t)p.tokens - 1);
     lp[j] = ld_stream(o.logprob + t);
     ref[j] = o.reference ? ld_stream(o.reference + t) : 0.f;
   }
-  few_tokens(p, f);
+  const uint32_t mine = few_tokens<EACH>(p, f);
 #pragma unroll
-  for (int j = 0; j < kFewEach; ++j) {
+  for (int j = 0; j < EACH; ++j) {
     const uint32_t t = j * kFewThreads + threadIdx.x;
-    if (t < p.tokens) values[t] = f.counts(t) ? (double)lp[j] - (double)ref[j] : 0.0;
+    if (t < p.tokens) values[t] = mine >> j & 1 ? (double)lp[j] - (double)ref[j] : 0.0;
   }
   __syncthreads();
+  if (o.average) few_counts<EACH>(f);
   double total[4] = {0, 0, 0, 0};
-  for (uint32_t pair = warp; 2 * pair < p.sequences; pair += kFewThreads / 32) {
-    double d[2];
-    uint32_t n[2];
+  for (uint32_t pair = warp; 2 * pair < p.sequences; pair += kFewThreads / 32) {   // (half a warp for each of its sequences)
+    const uint32_t s = 2 * pair + lane / 16, from = f.offsets[s], to = f.offsets[s + 1];
+    double v = 0;
+#pragma unroll 4
+    for (uint32_t t = from + lane % 16; t < to; t += 16) v += values[t];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const uint32_t from = f.offsets[2 * pair + k], to = f.offsets[2 * pair + k + 1];
-      double v = 0;
-      for (uint32_t t = from + lane; t < to; t += 32) v += values[t];
-      d[k] = warp_sum(v);
-      n[k] = from < to ? f.until(to) - f.until(from) : 0;
-    }
+    for (int off = 8; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    const uint32_t n = o.average && from < to ? f.until(to) - f.until(from) : 0;
+    const double rejected = __shfl_sync(0xffffffffu, v, 16);
+    const uint32_t n_rejected = __shfl_sync(0xffffffffu, n, 16);
     if (lane == 0) {
-      const Pair2 r = pair_terms(o, pair, d[0], d[1], n[0], n[1], inv_count, share + 2 * pair, share + 2 * pair + 1);
+      const Pair2 r = pair_terms(o, pair, v, rejected, n, n_rejected, inv_count, share + 2 * pair, share + 2 * pair + 1);
       total[0] += (double)(r.loss * inv_count), total[1] += (double)(r.right * inv_count), total[2] += (double)(r.gap * inv_count);
     }
   }
-  sums4<kFewThreads>(total, slots);                        // (with a barrier, behind which the shares are read)
-  if (threadIdx.x == 0) o.loss[0] = (float)total[0], o.loss[1] = (float)total[1], o.loss[2] = (float)total[2];
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    if (lane == 0) slots[warp * 4 + i] = total[i];
+  __syncthreads();                                         // (behind which the shares are read, too)
+  if (warp == 0)
+#pragma unroll
+    for (int i = 0; i < 3; ++i) total[i] = warp_sum(slots[lane * 4 + i]);
+  if (threadIdx.x == 0) write_loss(o, total);
   if (!o.g_logprob) return;
   const uint32_t begin = f.offsets[0], end = f.offsets[p.sequences];
   for (uint32_t t = begin + threadIdx.x; t < end; t += kFewThreads)
@@ -939,7 +980,11 @@ int with_workspace(void* workspace, uint64_t workspace_bytes, uint64_t need, cud
 
 template <class Id>
 int run_policy(const Packed<Id>& p, const Policy& o, void* workspace, uint64_t workspace_bytes, cudaStream_t st) {
-  if (few(p.tokens, p.sequences)) return launch("fpolicy_loss", policy_few_kernel<Id>, dim3(1), kFewThreads, 0, st, p, o);
+  if (few(p.tokens, p.sequences)) {
+    const uint64_t each = (p.tokens + kFewThreads - 1) / kFewThreads;
+    auto kernel = each <= 1 ? policy_few_kernel<Id, 1> : each <= 2 ? policy_few_kernel<Id, 2> : each <= 4 ? policy_few_kernel<Id, 4> : policy_few_kernel<Id, kFewEach>;
+    return launch("fpolicy_loss", kernel, dim3(1), kFewThreads, 0, st, p, o);
+  }
   uint64_t need;
   lay_out(nullptr, p.tokens, p.sequences, false, &need);
   return with_workspace(workspace, workspace_bytes, need, st, [&](void* base) {
@@ -972,9 +1017,11 @@ int run_pairs(const Packed<Id>& p, const Pairs& o, void* workspace, uint64_t wor
   const float inv_count = o.count > 0.f ? 1.f / o.count : 2.f / (float)p.sequences;
   if (few(p.tokens, p.sequences)) {
     constexpr size_t kBytes = kFew * sizeof(double);
-    const cudaError_t e = cudaFuncSetAttribute(pairs_few_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBytes);
+    const uint64_t each = (p.tokens + kFewThreads - 1) / kFewThreads;
+    auto kernel = each <= 1 ? pairs_few_kernel<Id, 1> : each <= 2 ? pairs_few_kernel<Id, 2> : each <= 4 ? pairs_few_kernel<Id, 4> : pairs_few_kernel<Id, kFewEach>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBytes);
     if (e != cudaSuccess) return fail(POLAR_B200_ERR_CUDA, "fpreference_loss", e);
-    return launch("fpreference_loss", pairs_few_kernel<Id>, dim3(1), kFewThreads, p.tokens * sizeof(double), st, p, o, inv_count);
+    return launch("fpreference_loss", kernel, dim3(1), kFewThreads, p.tokens * sizeof(double), st, p, o, inv_count);
   }
   uint64_t need;
   lay_out(nullptr, p.tokens, p.sequences, true, &need);

@@ -401,3 +401,17 @@ def test_gradients_against_differences(d):
             c["logprob"][i] += s
             shifted.append(pair_loss(c))
         assert abs((shifted[0] - shifted[1]) / 2e-4 - g[i].item()) < 1e-6
+
+
+@pytest.mark.parametrize("tokens", [1023, 1024, 1025, 2047, 2048, 2049, 4095, 4096, 4097, 6000])
+def test_few_tokens_where_the_threads_shares_change(d, tokens):
+    for sequences in (2, 64, 2048):
+        b = batch(tokens + sequences, tokens, sequences)
+        for by_sequence in (False, True):
+            for per_token in (False, True):
+                check(policy(d, b, per_token=per_token, by_sequence=by_sequence))
+        for average in (False, True):
+            preference(d, b, average=average)
+    b = batch(tokens, tokens - 50, 12, before=20, behind=30)
+    check(policy(d, b, by_sequence=True))
+    preference(d, b, average=True)
