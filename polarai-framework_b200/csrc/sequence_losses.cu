@@ -6,8 +6,8 @@
 // that the second one reads an eighth of a byte in their place.
 //   few tokens (kFew): everything by one CTA in one launch;
 //   else a pass over the ids (policy) or over all (pairs), one over the sequences, one over the tokens.
-// 600 tokens take 3.0 us (a launch), 131072 of 256 sequences 10.4, 8.4 M with 64-bit ids 52.5 (their 235 MB at a copy's rate 35.7): 12 for the ids, 36 for the
-// tokens at 55 % of the issue slots.  Pairs: 1500 tokens 3.9 us, 400001 10.9, 4.2 M of 128 sequences 22.1 (7.7): 9 to 10 each for sums and gradient.
+// 600 tokens take 3.0 us (a launch), 131072 of 256 sequences 10.3, 8.4 M with 64-bit ids 52.5 (their 235 MB at a copy's rate 35.7): 12 for the ids, 36 for the
+// tokens at 55 % of the issue slots.  Pairs: 1500 tokens 3.9 us, 400001 10.7, 4.2 M of 128 sequences 21.7 (7.7): 9 to 10 each for sums and gradient.
 // Every sum is taken in a fixed order, over a CTA's tokens in fp32 and beyond that, as of the sums over a sequence, in 64 bits.
 #include <algorithm>
 #include <cmath>
@@ -74,14 +74,16 @@ struct Found {
   uint64_t end = 0;
 };
 // The sequences of the warp's 128 tokens from `base` on, four neighbours to each lane.  `before`: of tokens before them; long sequences are looked for once.
+// `owner`: the first one where it is known (see note_owner), else kNone.
+constexpr uint32_t kNone = 0xffffffffu, kBlock = 128;
 template <class Id>
-__device__ __forceinline__ void sequences_of(const Packed<Id>& p, uint64_t base, uint32_t (&of)[4], Found& before) {
+__device__ __forceinline__ void sequences_of(const Packed<Id>& p, uint64_t base, uint32_t owner, uint32_t (&of)[4], Found& before) {
   if (base + 128 <= before.end) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) of[k] = before.s;
     return;
   }
-  const uint32_t lane = threadIdx.x & 31, first = sequence_of(p, base);
+  const uint32_t lane = threadIdx.x & 31, first = owner == kNone ? sequence_of(p, base) : owner;
   const uint64_t none = ~0ull, next = first + 1 + lane < p.sequences ? p.offset(first + 1 + lane) : none;
   const uint32_t begins = __popc(__ballot_sync(0xffffffffu, next < base + 128));
   const uint64_t mine = base + 4 * lane;
@@ -119,6 +121,7 @@ struct Workspace {
   Shared* shared;
   uint32_t* counts;                                        // of each tile
   uint32_t* bits;                                          // which tokens count
+  uint32_t* owner;                                         // of each kBlock tokens: the sequence of the first one
   float* share;                                            // of each sequence: 1 / its tokens that count (0: there is none); or its gradient
   float4* partial;                                         // of each CTA of the pass over the tokens
   double *whole, *head, *tail;                             // sums: of sequences inside a tile; of a tile's part of one that began before, or goes on
@@ -137,6 +140,7 @@ Workspace lay_out(void* base, uint64_t tokens, uint64_t sequences, bool pairs, u
   w.shared = reinterpret_cast<Shared*>(take(sizeof(Shared)));
   w.counts = reinterpret_cast<uint32_t*>(take(tiles * 4));
   w.bits = reinterpret_cast<uint32_t*>(take(tiles * kWords * 4));
+  w.owner = reinterpret_cast<uint32_t*>(take(tiles * (kTile / kBlock) * 4));
   w.share = reinterpret_cast<float*>(take(sequences * 4));
   if (pairs) {
     w.partial = reinterpret_cast<float4*>(take((sequences + kThreads / 32 - 1) / (kThreads / 32) * sizeof(float4)));
@@ -148,6 +152,18 @@ Workspace lay_out(void* base, uint64_t tokens, uint64_t sequences, bool pairs, u
   }
   *bytes = at;
   return w;
+}
+
+// A warp that looks at sequence s = [from, to) leaves it at the blocks that begin in it, which then need no search (two round trips to memory: 131072 tokens
+// of 256 sequences 10.5 -> 10.3 us, 400001 in pairs 10.9 -> 10.7).
+__device__ __forceinline__ void note_owner(const Workspace& w, uint32_t s, uint64_t from, uint64_t to) {
+  for (uint64_t b = (from + kBlock - 1) / kBlock + (threadIdx.x & 31); b * kBlock < to; b += 32) w.owner[b] = s;
+}
+// The block's, as it is used: whatever the memory holds, one of the sequences.
+template <class Id>
+__device__ __forceinline__ uint32_t owner_of(const Packed<Id>& p, const Workspace& w, uint64_t base, uint64_t begin) {
+  const uint32_t s = w.owner[base / kBlock];
+  return base < begin ? 0 : min(s, p.sequences - 1);
 }
 
 using polar_b200::warp_sum;
@@ -316,6 +332,7 @@ __global__ void __launch_bounds__(kThreads) shares_kernel(Packed<Id> p, Workspac
   for (uint32_t s = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); s < p.sequences; s += gridDim.x * (kThreads / 32)) {
     const uint64_t from = p.offset(s), to = p.offset(s + 1);
     const uint64_t n = from < to ? counted(w, from, to) : 0;
+    note_owner(w, s, from, to);
     if ((threadIdx.x & 31) == 0) w.share[s] = n ? 1.f / (float)n : 0.f;
     mine += n != 0;
   }
@@ -442,7 +459,7 @@ __global__ void __launch_bounds__(kThreads) policy_kernel(Packed<Id> p, Workspac
   const uint64_t begin = p.offset(0), end = p.offset(p.sequences);
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
   float4 lp[PARTS], old[PARTS], ref[PARTS], ent[PARTS], adv[PARTS];
-  uint32_t bits[PARTS];
+  uint32_t bits[PARTS], owner[PARTS];
   const bool whole = vectors && (uint64_t)(blockIdx.x + 1) * PARTS * kPart <= p.tokens;
 #pragma unroll
   for (int h = 0; h < PARTS; ++h) {
@@ -451,6 +468,7 @@ __global__ void __launch_bounds__(kThreads) policy_kernel(Packed<Id> p, Workspac
     ref[h] = load4(o.reference, t, p.tokens, whole), ent[h] = load4(o.entropy, t, p.tokens, whole);
     adv[h] = load4(o.per_token ? o.advantage : nullptr, t, p.tokens, whole);
     bits[h] = w.bits[t / 32] >> (t & 31) & 15;             // (the last tile's words are all there)
+    owner[h] = LOOK && o.by_sequence ? owner_of(p, w, t - 4 * lane, begin) : kNone;
   }
   Found found;
   float even;
@@ -475,7 +493,7 @@ __global__ void __launch_bounds__(kThreads) policy_kernel(Packed<Id> p, Workspac
   for (int h = 0; h < PARTS; ++h) {
     const uint64_t base = ((uint64_t)blockIdx.x * PARTS + h) * kPart + warp * 128, t = base + 4 * lane;
     uint32_t of[4] = {0, 0, 0, 0};
-    if (LOOK && base < end) sequences_of(p, base, of, found);
+    if (LOOK && base < end) sequences_of(p, base, owner[h], of, found);
     float4 g, ge;
     if (LOOK && !o.per_token)
 #pragma unroll
@@ -829,6 +847,7 @@ __global__ void __launch_bounds__(kThreads) pairs_kernel(Packed<Id> p, Workspace
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
   if (s < p.sequences) {
     const uint64_t from = p.offset(s), to = p.offset(s + 1);
+    note_owner(w, s, from, to);
     const double d = from < to ? sum_of(w, s, from, to) : 0;
     const uint64_t n = o.average && from < to ? counted(w, from, to) : 0;
     if (lane == 0) sums[warp] = d, counts[warp] = n;
@@ -866,7 +885,7 @@ __global__ void __launch_bounds__(kThreads) pairs_grad_kernel(Packed<Id> p, Work
     if (base >= end) return;
     uint32_t of[4];
     const uint32_t bits = w.bits[t / 32] >> (t & 31) & 15; // (the last tile's words are all there)
-    sequences_of(p, base, of, found);
+    sequences_of(p, base, owner_of(p, w, base, begin), of, found);
     float4 g, share;
     share.x = w.share[of[0]];
     // (mostly the whole warp's tokens are of one sequence)
