@@ -23,8 +23,11 @@ constexpr uint32_t kTile = 2048;                           // tokens of a CTA in
 constexpr uint32_t kWords = kTile / 32;
 constexpr int kThreads = 256, kEach = kTile / kThreads;   // (with 16 tokens to a thread the loads in flight took the registers of all but two CTAs)
 constexpr uint32_t kPass = 2048;                           // tokens of a CTA in the pass that writes gradients
-constexpr uint32_t kFew = 8192, kFewSequences = 2048;      // what one CTA does alone
+// What one CTA does alone: the policy loss of up to 4096 tokens (20 sequences: 7.7 us for 8.7 of three kernels; 6000 tokens 10.2 for 8.7), pairs up to 6144 (6.6 for
+// 7.5; 8000 tokens 7.9 for 7.7), of up to 2048 sequences.
+constexpr uint32_t kFewPolicy = 4096, kFew = 6144, kFewSequences = 2048;
 constexpr int kFewThreads = 1024, kFewEach = kFew / kFewThreads;
+constexpr uint32_t kShort = 24;                            // tokens of a sequence that a lane sums by itself
 
 // ---- sequences
 
@@ -557,7 +560,7 @@ struct FewTokens {
   __device__ __forceinline__ bool counts(uint32_t t) const { return bits[t / 32] >> (t & 31) & 1; }
 };
 // Which tokens count, and the offsets, to be read behind a barrier.  Thread i's tokens are i, i + kFewThreads, ..., EACH at most; the result: which of its own count.
-// (One, two, four or eight: instructions that come from memory are much of such a launch.  600 tokens 3.0 us where eight take 3.4, 1500 in pairs 3.9 for 4.2.)
+// (One, two, four or six: instructions that come from memory are much of such a launch.  600 tokens 3.0 us where eight took 3.4, 1500 in pairs 3.8 for 4.2.)
 template <int EACH, class Id>
 __device__ __forceinline__ uint32_t few_tokens(const Packed<Id>& p, FewTokens& f) {
   const uint32_t begin = (uint32_t)p.offset(0), end = (uint32_t)p.offset(p.sequences);
@@ -805,11 +808,18 @@ __global__ void __launch_bounds__(kThreads) sums_kernel(Packed<Id> p, Workspace 
     }
     return;
   }
-  // each lane looks at one sequence, the warp sums those that are not empty
+  // each lane looks at one sequence and, where there are many, sums a short one by itself; the warp sums the others in turn
+  const uint32_t alone = last - first >= 64 ? kShort : 0;
   for (uint32_t chunk = first; chunk <= last; chunk += kThreads) {
     const uint32_t s = chunk + lane * (kThreads / 32) + warp;
     const uint64_t a = s <= last ? p.offset(s) : 0, b = s <= last ? p.offset(s + 1) : 0;
-    for (uint32_t todo = __ballot_sync(0xffffffffu, max(a, from) < min(b, to)); todo; todo &= todo - 1) {
+    const uint32_t lo = (uint32_t)(max(a, from) - tile), hi = max(a, from) < min(b, to) ? (uint32_t)(min(b, to) - tile) : lo;
+    if (hi > lo && hi - lo <= alone) {
+      double v = 0;
+      for (uint32_t i = lo; i < hi; ++i) v += values[i];
+      keep(s, a, b, v);
+    }
+    for (uint32_t todo = __ballot_sync(0xffffffffu, hi - lo > alone); todo; todo &= todo - 1) {
       const int who = __ffs(todo) - 1;
       const uint64_t sa = __shfl_sync(0xffffffffu, a, who), sb = __shfl_sync(0xffffffffu, b, who);
       double v = 0;
@@ -900,6 +910,7 @@ __global__ void __launch_bounds__(kThreads) pairs_grad_kernel(Packed<Id> p, Work
 template <class Id, int EACH>
 __global__ void __launch_bounds__(kFewThreads) pairs_few_kernel(Packed<Id> p, Pairs o, float inv_count) {
   extern __shared__ double values[];
+  double* const sums = values + p.tokens;                  // of each sequence
   __shared__ FewTokens f;
   __shared__ float share[kFewSequences];
   __shared__ double slots[kFewThreads / 8];
@@ -922,20 +933,45 @@ __global__ void __launch_bounds__(kFewThreads) pairs_few_kernel(Packed<Id> p, Pa
   __syncthreads();
   if (o.average) few_counts<EACH>(f);
   double total[4] = {0, 0, 0, 0};
-  for (uint32_t pair = warp; 2 * pair < p.sequences; pair += kFewThreads / 32) {   // (half a warp for each of its sequences)
-    const uint32_t s = 2 * pair + lane / 16, from = f.offsets[s], to = f.offsets[s + 1];
-    double v = 0;
+  auto terms_of = [&](uint32_t pair, double chosen, double rejected) {
+    auto counted = [&](uint32_t s) { return o.average && f.offsets[s] < f.offsets[s + 1] ? f.until(f.offsets[s + 1]) - f.until(f.offsets[s]) : 0; };
+    const Pair2 r = pair_terms(o, pair, chosen, rejected, counted(2 * pair), counted(2 * pair + 1), inv_count, share + 2 * pair, share + 2 * pair + 1);
+    total[0] += (double)(r.loss * inv_count), total[1] += (double)(r.right * inv_count), total[2] += (double)(r.gap * inv_count);
+  };
+  const uint32_t pairs = p.sequences / 2;
+  if (pairs <= kFewThreads / 32) {                         // a warp for each pair, half of it for each of its sequences
+    if (warp < pairs) {
+      const uint32_t s = 2 * warp + lane / 16, to = f.offsets[s + 1];
+      double v = 0;
 #pragma unroll 4
-    for (uint32_t t = from + lane % 16; t < to; t += 16) v += values[t];
+      for (uint32_t t = f.offsets[s] + lane % 16; t < to; t += 16) v += values[t];
 #pragma unroll
-    for (int off = 8; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-    const uint32_t n = o.average && from < to ? f.until(to) - f.until(from) : 0;
-    const double rejected = __shfl_sync(0xffffffffu, v, 16);
-    const uint32_t n_rejected = __shfl_sync(0xffffffffu, n, 16);
-    if (lane == 0) {
-      const Pair2 r = pair_terms(o, pair, v, rejected, n, n_rejected, inv_count, share + 2 * pair, share + 2 * pair + 1);
-      total[0] += (double)(r.loss * inv_count), total[1] += (double)(r.right * inv_count), total[2] += (double)(r.gap * inv_count);
+      for (int off = 8; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+      const double rejected = __shfl_sync(0xffffffffu, v, 16);
+      if (lane == 0) terms_of(warp, v, rejected);
     }
+  } else {                                                 // a lane for each short sequence, the warp for the others in turn; then a thread for each pair
+    for (uint32_t first = warp; first < p.sequences; first += kFewThreads) {
+      const uint32_t s = first + lane * (kFewThreads / 32), from = s < p.sequences ? f.offsets[s] : 0, to = s < p.sequences ? max(f.offsets[s + 1], from) : 0;
+      double mine_sum = 0;
+      if (to - from <= kShort)
+        for (uint32_t t = from; t < to; ++t) mine_sum += values[t];
+      for (uint32_t todo = __ballot_sync(0xffffffffu, to - from > kShort); todo; todo &= todo - 1) {
+        const int who = __ffs(todo) - 1;
+        const uint32_t a = __shfl_sync(0xffffffffu, from, who), b = __shfl_sync(0xffffffffu, to, who);
+        double v = 0;
+#pragma unroll 4
+        for (uint32_t t = a + lane; t < b; t += 32) v += values[t];
+        v = warp_sum(v);
+        if (lane == who) mine_sum = v;
+      }
+      if (s < p.sequences) sums[s] = mine_sum;
+    }
+    __syncthreads();
+    if (threadIdx.x < pairs) terms_of(threadIdx.x, sums[2 * threadIdx.x], sums[2 * threadIdx.x + 1]);
+    static_assert(kFewSequences == 2 * kFewThreads, "a pair to a thread");
+#pragma unroll
+    for (int i = 0; i < 3; ++i) total[i] = warp_sum(total[i]);
   }
 #pragma unroll
   for (int i = 0; i < 3; ++i)
@@ -961,7 +997,7 @@ int with_ids(int id_type, F f) {
     default: return f(int64_t());
   }
 }
-bool few(uint64_t tokens, uint64_t sequences) { return tokens <= kFew && sequences <= kFewSequences; }
+bool few(uint64_t tokens, uint64_t sequences, uint64_t most) { return tokens <= most && sequences <= kFewSequences; }
 int check_sequences(const void* ids, const void* offsets, int id_type, uint64_t tokens, uint64_t sequences) {
   if (id_type < POLAR_B200_IDS_F32 || id_type > POLAR_B200_IDS_I64) return fail(POLAR_B200_ERR_INVALID, "unknown type of ids");
   if (tokens > 1ull << 36 || sequences > 0x7fffffffull) return fail(POLAR_B200_ERR_INVALID, "too many tokens or sequences");
@@ -999,9 +1035,9 @@ int with_workspace(void* workspace, uint64_t workspace_bytes, uint64_t need, cud
 
 template <class Id>
 int run_policy(const Packed<Id>& p, const Policy& o, void* workspace, uint64_t workspace_bytes, cudaStream_t st) {
-  if (few(p.tokens, p.sequences)) {
+  if (few(p.tokens, p.sequences, kFewPolicy)) {
     const uint64_t each = (p.tokens + kFewThreads - 1) / kFewThreads;
-    auto kernel = each <= 1 ? policy_few_kernel<Id, 1> : each <= 2 ? policy_few_kernel<Id, 2> : each <= 4 ? policy_few_kernel<Id, 4> : policy_few_kernel<Id, kFewEach>;
+    auto kernel = each <= 1 ? policy_few_kernel<Id, 1> : each <= 2 ? policy_few_kernel<Id, 2> : policy_few_kernel<Id, kFewPolicy / kFewThreads>;
     return launch("fpolicy_loss", kernel, dim3(1), kFewThreads, 0, st, p, o);
   }
   uint64_t need;
@@ -1034,13 +1070,13 @@ int run_policy(const Packed<Id>& p, const Policy& o, void* workspace, uint64_t w
 template <class Id>
 int run_pairs(const Packed<Id>& p, const Pairs& o, void* workspace, uint64_t workspace_bytes, cudaStream_t st) {
   const float inv_count = o.count > 0.f ? 1.f / o.count : 2.f / (float)p.sequences;
-  if (few(p.tokens, p.sequences)) {
-    constexpr size_t kBytes = kFew * sizeof(double);
+  if (few(p.tokens, p.sequences, kFew)) {
+    constexpr size_t kBytes = (kFew + kFewSequences) * sizeof(double);
     const uint64_t each = (p.tokens + kFewThreads - 1) / kFewThreads;
     auto kernel = each <= 1 ? pairs_few_kernel<Id, 1> : each <= 2 ? pairs_few_kernel<Id, 2> : each <= 4 ? pairs_few_kernel<Id, 4> : pairs_few_kernel<Id, kFewEach>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBytes);
     if (e != cudaSuccess) return fail(POLAR_B200_ERR_CUDA, "fpreference_loss", e);
-    return launch("fpreference_loss", kernel, dim3(1), kFewThreads, p.tokens * sizeof(double), st, p, o, inv_count);
+    return launch("fpreference_loss", kernel, dim3(1), kFewThreads, (p.tokens + p.sequences) * sizeof(double), st, p, o, inv_count);
   }
   uint64_t need;
   lay_out(nullptr, p.tokens, p.sequences, true, &need);
@@ -1066,13 +1102,13 @@ using namespace polar_b200;
 extern "C" {
 
 uint64_t polar_b200_fpolicy_loss_workspace_bytes(uint64_t tokens, uint64_t sequences) {
-  if (tokens > 1ull << 36 || sequences > 0x7fffffffull || few(tokens, sequences)) return 0;
+  if (tokens > 1ull << 36 || sequences > 0x7fffffffull || few(tokens, sequences, kFewPolicy)) return 0;
   uint64_t bytes;
   lay_out(nullptr, tokens, sequences, false, &bytes);
   return bytes;
 }
 uint64_t polar_b200_fpreference_loss_workspace_bytes(uint64_t tokens, uint64_t pairs) {
-  if (tokens > 1ull << 36 || pairs > 0x3fffffffull || few(tokens, 2 * pairs)) return 0;
+  if (tokens > 1ull << 36 || pairs > 0x3fffffffull || few(tokens, 2 * pairs, kFew)) return 0;
   uint64_t bytes;
   lay_out(nullptr, tokens, 2 * pairs, true, &bytes);
   return bytes;

@@ -81,7 +81,7 @@ def check(got, gradient=True, entropy=True):
         assert (g == 7).all()
 
 
-# one CTA: up to 8192 tokens of 2048 sequences; beyond, tiles of 4096 and 2048 tokens
+# one CTA: up to 4096 tokens (pairs: 6144) of 2048 sequences; beyond, tiles of 2048 tokens
 SIZES = [(1, 1), (2, 1), (3, 7), (31, 2), (33, 5), (1000, 1), (1025, 40), (4095, 2000), (8191, 2048), (8192, 1), (8193, 3), (8192, 2049), (5000, 6000),
          (12289, 1), (20000, 19), (65537, 4000), (100001, 99999), (300007, 2)]
 
@@ -403,7 +403,7 @@ def test_gradients_against_differences(d):
         assert abs((shifted[0] - shifted[1]) / 2e-4 - g[i].item()) < 1e-6
 
 
-@pytest.mark.parametrize("tokens", [1023, 1024, 1025, 2047, 2048, 2049, 4095, 4096, 4097, 6000])
+@pytest.mark.parametrize("tokens", [1023, 1024, 1025, 2047, 2048, 2049, 4095, 4096, 4097, 6143, 6144, 6145])
 def test_few_tokens_where_the_threads_shares_change(d, tokens):
     for sequences in (2, 64, 2048):
         b = batch(tokens + sequences, tokens, sequences)

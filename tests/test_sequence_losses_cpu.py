@@ -57,7 +57,7 @@ def test_policy_statuses(c):
     assert policy(c, g=at(4), advantage_per_token=1, sequences=100) != 0   # (a per-token array: no overlap, but there is no GPU)
     # a workspace that is too small or misplaced
     need = c.polar_b200_fpolicy_loss_workspace_bytes(100000, 4)
-    assert need > 100000 // 8 and c.polar_b200_fpolicy_loss_workspace_bytes(8192, 2048) == 0 and c.polar_b200_fpolicy_loss_workspace_bytes(1 << 40, 4) == 0
+    assert need > 100000 // 8 and c.polar_b200_fpolicy_loss_workspace_bytes(4096, 2048) == 0 and c.polar_b200_fpolicy_loss_workspace_bytes(1 << 40, 4) == 0
     assert policy(c, tokens=100000, ws=at(20), ws_bytes=need - 1) == 5 and policy(c, tokens=100000, ws=at(20) + 4, ws_bytes=need) == 5
 
 
@@ -81,7 +81,7 @@ def test_preference_statuses(c):
         assert preference(c, g=g) == 1 and b"overlaps" in c.polar_b200_last_error()
     assert preference(c, rewards=at(0)) == 1 and preference(c, rewards=at(3) + 32) == 1 and preference(c, loss=at(5) + 12) == 1
     need = c.polar_b200_fpreference_loss_workspace_bytes(100000, 4)
-    assert need > 100000 // 8 and c.polar_b200_fpreference_loss_workspace_bytes(8192, 1024) == 0
+    assert need > 100000 // 8 and c.polar_b200_fpreference_loss_workspace_bytes(6144, 1024) == 0
     assert preference(c, tokens=100000, ws=at(20), ws_bytes=need - 1) == 5
 
 
