@@ -325,21 +325,67 @@ __global__ void __launch_bounds__(kTotalThreads) total_kernel(Workspace w, uint3
     w.shared->share = n ? 1.f / (float)n : 0.f;
   }
 }
+// Where sequences are short a lane looks at each, and its warp at the others in turn; else a warp at each.
+constexpr uint64_t kLane = 64;                             // tokens of a sequence that a lane looks at by itself
 template <class Id>
+bool short_ones(const Packed<Id>& p) {
+  return p.sequences >= 1024 && p.tokens <= kLane * p.sequences;
+}
+// How many tokens of [from, to) count, by a lane: at most kLane of them, in three words.
+__device__ __forceinline__ uint32_t counted_alone(const Workspace& w, uint64_t from, uint64_t to) {
+  const uint64_t first = from / 32, last = (to - 1) / 32;
+  uint32_t bits[3], n = 0;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) bits[k] = w.bits[min(first + k, last)];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    if (first + k > last) break;
+    if (k == 0) bits[k] &= ~0u << (from & 31);
+    if (first + k == last) bits[k] &= ~0u >> (31 - ((to - 1) & 31));
+    n += __popc(bits[k]);
+  }
+  return n;
+}
+// note_owner by a lane, of a sequence of fewer tokens than a block has.
+__device__ __forceinline__ void note_owner_alone(const Workspace& w, uint32_t s, uint64_t from, uint64_t to) {
+  const uint64_t b = (from + kBlock - 1) / kBlock;
+  if (b * kBlock < to) w.owner[b] = s;
+}
+static_assert(kLane < kBlock && kLane <= 64, "three words, one block");
+
+template <class Id, bool SHORT>
 __global__ void __launch_bounds__(kThreads) shares_kernel(Packed<Id> p, Workspace w) {
   __shared__ uint32_t live;
   if (threadIdx.x == 0) live = 0;
   __syncthreads();
   pdl_enter();
+  const uint32_t lane = threadIdx.x & 31;
   uint32_t mine = 0;
-  for (uint32_t s = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); s < p.sequences; s += gridDim.x * (kThreads / 32)) {
-    const uint64_t from = p.offset(s), to = p.offset(s + 1);
-    const uint64_t n = from < to ? counted(w, from, to) : 0;
-    note_owner(w, s, from, to);
-    if ((threadIdx.x & 31) == 0) w.share[s] = n ? 1.f / (float)n : 0.f;
-    mine += n != 0;
+  for (uint32_t i = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); SHORT ? i <= (p.sequences - 1) / 32 : i < p.sequences; i += gridDim.x * (kThreads / 32)) {
+    if (SHORT) {
+      const uint32_t s = i * 32 + lane;
+      const bool there = s < p.sequences;
+      const uint64_t from = there ? p.offset(s) : 0, to = there ? p.offset(s + 1) : 0;
+      const bool some = from < to, alone = some && to - from <= kLane;
+      uint64_t n = 0;
+      if (alone) n = counted_alone(w, from, to), note_owner_alone(w, s, from, to);
+      for (uint32_t todo = __ballot_sync(0xffffffffu, some && !alone); todo; todo &= todo - 1) {
+        const int who = __ffs(todo) - 1;
+        const uint64_t a = __shfl_sync(0xffffffffu, from, who), b = __shfl_sync(0xffffffffu, to, who), all = counted(w, a, b);
+        note_owner(w, i * 32 + who, a, b);
+        if (lane == who) n = all;
+      }
+      if (there) w.share[s] = n ? 1.f / (float)n : 0.f;
+      mine += __popc(__ballot_sync(0xffffffffu, n != 0));
+    } else {
+      const uint64_t from = p.offset(i), to = p.offset(i + 1);
+      const uint64_t n = from < to ? counted(w, from, to) : 0;
+      note_owner(w, i, from, to);
+      if (lane == 0) w.share[i] = n ? 1.f / (float)n : 0.f;
+      mine += n != 0;
+    }
   }
-  if ((threadIdx.x & 31) == 0 && mine) atomicAdd(&live, mine);
+  if (lane == 0 && mine) atomicAdd(&live, mine);
   __syncthreads();
   if (threadIdx.x == 0 && live) atomicAdd(&w.shared->live, live);
 }
@@ -843,29 +889,59 @@ __device__ __forceinline__ double sum_of(const Workspace& w, uint32_t s, uint64_
   return warp_sum(v) + w.tail[first];
 }
 
-// A warp per sequence.  The loss is written by the last CTA or, where the gradient's kernel comes next, by one more CTA of that, while nothing waits for it.
+// A warp per sequence, or a lane for each short one.  The loss is written by the last CTA or, where the gradient's kernel comes next, by one more CTA of that, while nothing waits for it.
 __device__ __forceinline__ void write_loss(const Pairs& o, const double* total) {
   o.loss[0] = (float)total[0], o.loss[1] = (float)total[1], o.loss[2] = (float)total[2];
 }
-template <class Id>
+template <class Id, bool SHORT>
 __global__ void __launch_bounds__(kThreads) pairs_kernel(Packed<Id> p, Workspace w, Pairs o, float inv_count, bool gradient_next) {
   __shared__ float slots[kThreads / 8];
   __shared__ double wide[kThreads / 8], sums[kThreads / 32];
   __shared__ uint64_t counts[kThreads / 32];
   pdl_enter();
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, s = blockIdx.x * (kThreads / 32) + warp;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  if (s < p.sequences) {
-    const uint64_t from = p.offset(s), to = p.offset(s + 1);
-    note_owner(w, s, from, to);
-    const double d = from < to ? sum_of(w, s, from, to) : 0;
-    const uint64_t n = o.average && from < to ? counted(w, from, to) : 0;
-    if (lane == 0) sums[warp] = d, counts[warp] = n;
-  }
-  __syncthreads();
-  if (lane == 0 && (warp & 1) == 0 && s < p.sequences) {
-    const Pair2 r = pair_terms(o, s / 2, sums[warp], sums[warp + 1], counts[warp], counts[warp + 1], inv_count, w.share + s, w.share + s + 1);
-    sum[0] = r.loss * inv_count, sum[1] = r.right * inv_count, sum[2] = r.gap * inv_count;
+  if (SHORT) {
+    const uint32_t s = blockIdx.x * kThreads + threadIdx.x;
+    const bool there = s < p.sequences;
+    const uint64_t from = there ? p.offset(s) : 0, to = there ? p.offset(s + 1) : 0;
+    const bool some = from < to, alone = some && to - from <= kLane;
+    double d = 0;
+    uint64_t n = 0;
+    if (alone) {
+      const uint64_t first = from / kTile, last = (to - 1) / kTile;
+      d = first == last ? w.whole[s] : w.head[last] + w.tail[first];
+      if (o.average) n = counted_alone(w, from, to);
+      note_owner_alone(w, s, from, to);
+    }
+    for (uint32_t todo = __ballot_sync(0xffffffffu, some && !alone); todo; todo &= todo - 1) {
+      const int who = __ffs(todo) - 1;
+      const uint32_t its = s - lane + who;
+      const uint64_t a = __shfl_sync(0xffffffffu, from, who), b = __shfl_sync(0xffffffffu, to, who), all = o.average ? counted(w, a, b) : 0;
+      const double v = sum_of(w, its, a, b);
+      note_owner(w, its, a, b);
+      if (lane == who) d = v, n = all;
+    }
+    const double rejected = __shfl_down_sync(0xffffffffu, d, 1);
+    const uint64_t n_rejected = __shfl_down_sync(0xffffffffu, n, 1);
+    if (there && (lane & 1) == 0) {
+      const Pair2 r = pair_terms(o, s / 2, d, rejected, n, n_rejected, inv_count, w.share + s, w.share + s + 1);
+      sum[0] = r.loss * inv_count, sum[1] = r.right * inv_count, sum[2] = r.gap * inv_count;
+    }
+  } else {
+    const uint32_t s = blockIdx.x * (kThreads / 32) + warp;
+    if (s < p.sequences) {
+      const uint64_t from = p.offset(s), to = p.offset(s + 1);
+      note_owner(w, s, from, to);
+      const double d = from < to ? sum_of(w, s, from, to) : 0;
+      const uint64_t n = o.average && from < to ? counted(w, from, to) : 0;
+      if (lane == 0) sums[warp] = d, counts[warp] = n;
+    }
+    __syncthreads();
+    if (lane == 0 && (warp & 1) == 0 && s < p.sequences) {
+      const Pair2 r = pair_terms(o, s / 2, sums[warp], sums[warp + 1], counts[warp], counts[warp + 1], inv_count, w.share + s, w.share + s + 1);
+      sum[0] = r.loss * inv_count, sum[1] = r.right * inv_count, sum[2] = r.gap * inv_count;
+    }
   }
   sums4<kThreads>(sum, slots);
   if (gradient_next) {
@@ -1048,8 +1124,8 @@ int run_policy(const Packed<Id>& p, const Policy& o, void* workspace, uint64_t w
     int rc = launch("fpolicy_loss: ids", mark_kernel<Id>, dim3(tiles), kThreads, 0, st, p, w);
     if (rc) return rc;
     if (o.by_sequence) {
-      const uint64_t ctas = ((uint64_t)p.sequences + kThreads / 32 - 1) / (kThreads / 32), most = 8ull * sm_count();
-      rc = launch("fpolicy_loss: shares", shares_kernel<Id>, dim3((unsigned)(ctas < most ? ctas : most)), kThreads, 0, st, p, w);
+      const uint64_t each = short_ones(p) ? kThreads : kThreads / 32, ctas = (p.sequences + each - 1) / each, most = 8ull * sm_count();
+      rc = launch("fpolicy_loss: shares", short_ones(p) ? shares_kernel<Id, true> : shares_kernel<Id, false>, dim3((unsigned)(ctas < most ? ctas : most)), kThreads, 0, st, p, w);
     } else if (o.count == 0.f && tiles > kFewTiles) {
       rc = launch("fpolicy_loss: total", total_kernel, dim3(1), kTotalThreads, 0, st, w, tiles);
     }
@@ -1085,9 +1161,9 @@ int run_pairs(const Packed<Id>& p, const Pairs& o, void* workspace, uint64_t wor
     const uint32_t tiles = (uint32_t)tiles_of(p.tokens);
     int rc = launch("fpreference_loss: sums", sums_kernel<Id>, dim3(tiles), kThreads, 0, st, p, w, o);
     if (rc) return rc;
-    const uint32_t ctas = (p.sequences + kThreads / 32 - 1) / (kThreads / 32);
+    const uint32_t each = short_ones(p) ? kThreads : kThreads / 32, ctas = (uint32_t)(((uint64_t)p.sequences + each - 1) / each);
     const bool gradient = o.g_logprob && p.tokens;
-    rc = launch("fpreference_loss", pairs_kernel<Id>, dim3(ctas), kThreads, 0, st, p, w, o, inv_count, gradient);
+    rc = launch("fpreference_loss", short_ones(p) ? pairs_kernel<Id, true> : pairs_kernel<Id, false>, dim3(ctas), kThreads, 0, st, p, w, o, inv_count, gradient);
     if (rc || !gradient) return rc;
     return launch("fpreference_loss: gradient", pairs_grad_kernel<Id>, dim3((unsigned)((p.tokens + kPass - 1) / kPass) + 1), kThreads, 0, st, p, w, o, ctas,
                   aligned16(o.g_logprob));
