@@ -102,9 +102,12 @@ __device__ __forceinline__ void sequences_of(const Packed<Id>& p, uint64_t base,
     }
     return;
   }
+  uint32_t lo = first;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {                            // sequences of a few tokens, or many empty ones: each lane for itself
-    uint32_t lo = first, end = p.sequences;
+  for (int k = 0; k < 4; ++k) {                            // sequences of a few tokens, or many empty ones: each lane for itself, in growing steps from where it is
+    uint32_t step = 1;
+    while (step < p.sequences - lo && p.offset(lo + step) <= mine + k) lo += step, step *= 2;
+    uint32_t end = min(step, p.sequences - lo) + lo;
     while (end - lo > 1) {
       const uint32_t middle = lo + (end - lo) / 2;
       if (p.offset(middle) <= mine + k) lo = middle;
