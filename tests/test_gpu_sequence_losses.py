@@ -415,3 +415,21 @@ def test_few_tokens_where_the_threads_shares_change(d, tokens):
     b = batch(tokens, tokens - 50, 12, before=20, behind=30)
     check(policy(d, b, by_sequence=True))
     preference(d, b, average=True)
+
+
+@pytest.mark.parametrize("seed", [1, 2, 3])
+def test_long_sequences_among_many_short_ones(d, seed):
+    # a lane looks at sequences of up to 64 tokens, its warp at the others; tiles end at 2048
+    rng = np.random.default_rng(seed)
+    lengths = rng.integers(0, 7, 4000)
+    lengths[rng.choice(4000, 12, replace=False)] = [63, 64, 65, 127, 128, 129, 2047, 2048, 2049, 5000, 9000, 1000]
+    o = np.concatenate([[0], np.cumsum(lengths)]) + 5 * seed
+    tokens = int(o[-1]) + 100
+    b = batch(seed, tokens, 4000)
+    b["ids"], b["offsets"] = np.where(rng.random(tokens) < 0.6, 3, -1), o
+    for by_sequence in (False, True):
+        for per_token in (False, True):
+            check(policy(d, b, per_token=per_token, by_sequence=by_sequence))
+    for average in (False, True):
+        preference(d, b, average=average)
+        preference(d, b, average=average, gradient=False)
