@@ -22,15 +22,15 @@
 #include <utility>
 #include <vector>
 
+#include "muon_plan.hpp"
 #include "rows.cuh"
 #include "tc_ptx.cuh"
 
 namespace polar_b200 {
 namespace {
 using namespace tc;
+using namespace muon;
 
-constexpr float kX = 32768.f, kG = 32768.f, kP = 16384.f;  // what X, G and P are held times
-constexpr float kQ = 4096.f;                               // and the product of two P: kBoundP^2 * 2^12 is below 65504
 constexpr float kBound = 1.4f, kBoundP = 3.98f;            // largest singular value of X, of P: 1.4^2 * 2^15 and 3.98 * 2^14 are below 65504
 
 // ---- the passes before the products
@@ -1040,6 +1040,7 @@ struct ChainTable {
   Chain s[kChains];
 };
 constexpr uint32_t kSquare = 64 * 1024;                    // 128 x 128 pairs
+static_assert(kSquare == kNarrow * kNarrow * 4, "a square for each of them");
 constexpr uint32_t kChainBytes = 3 * kSquare + 1024 + 256;
 
 __global__ void __launch_bounds__(kSmallThreads, 1) chain_kernel(const __grid_constant__ ChainTable t) {
@@ -1256,8 +1257,6 @@ uint64_t chunk_of(uint64_t count) {
   const uint64_t each = (count + kMostChunks - 1) / kMostChunks;
   return each <= kChunk ? kChunk : (each + kChunk - 1) / kChunk * kChunk;
 }
-// Two rounds at a time where the shorter side is so much shorter (see `operations_of`): then there are three symmetric matrices, else two.
-bool in_pairs(uint64_t rows, uint64_t cols) { return std::max(rows, cols) >= 2 * std::min(rows, cols); }
 uint64_t bytes_of(uint64_t rows, uint64_t cols) {          // of one matrix: X twice and the symmetric ones, two planes each, and what is small, rounded up
   const uint64_t side = std::min(rows, cols);
   return 2 * 2 * (2 * rows * up64(cols) + (in_pairs(rows, cols) ? 3 : 2) * side * up64(side)) + kMostChunks * sizeof(double) + sizeof(Target) + 7 * 256;
@@ -1329,40 +1328,6 @@ int launch_tables(const std::vector<One>& all, size_t from, size_t to, const std
     chunks_before += chunks;
   }
   return POLAR_B200_OK;
-}
-
-// One product of the matrices of a shape: of X (from x[from]) with itself, of symmetric matrices s[left] s[right] that commute, or of s[left] and X; or all
-// products of symmetric matrices of a round, or of two, from s[left] to s[out].
-struct Operation {
-  enum { kGram, kProduct, kMove, kChain, kChain2 } what;
-  int left, right, out, add;                               // add: -1 for none
-  float by, add_by, diagonal;
-  bool last;
-};
-// A round by itself: G, P = a + b G + c G G, X <- P X.  Two rounds P' P X with the second one's G' = (P X)(P X)^T = P G P:
-//   G, P, T = P G, G' = P T, P', Q = P' P, X <- Q X
-// are five products of the shorter side alone in place of two products with X (work of 3 short^2 long for one of 3 short^3): 1024 x 4096 takes three quarters
-// of the operations.  Not more rounds at a time: what rounding leaves in G for small singular values grows by a^2 in each further one.
-std::vector<Operation> operations_of(const Kin& k, const polar_b200_muon_options& o, bool chain) {
-  std::vector<Operation> ops;
-  auto product = [&](int l, int r, int out, float by) { ops.push_back(Operation{Operation::kProduct, l, r, out, -1, by, 0.f, 0.f, false}); };
-  auto polynomial = [&](int g, int out) { ops.push_back(Operation{Operation::kProduct, g, g, out, g, o.c * (kP / (kG * kG)), o.b * (kP / kG), o.a * kP, false}); };
-  for (uint32_t i = 0; i < o.steps;) {
-    ops.push_back(Operation{Operation::kGram, 0, 0, 0, -1, kG / (kX * kX), 0.f, 0.f, false});
-    const bool two = i + 1 < o.steps && in_pairs(k.rows, k.cols);
-    if (chain) ops.push_back(Operation{two ? Operation::kChain2 : Operation::kChain, 0, 0, 1, -1, 0.f, 0.f, 0.f, false});
-    else polynomial(0, 1);
-    if (two && !chain) {
-      product(1, 0, 2, 1.f / kP);                          // T as G: its eigenvalues are products of two singular values of X, before and after
-      product(1, 2, 0, 1.f / kP);
-      polynomial(0, 2);
-      product(2, 1, 0, kQ / (kP * kP));
-    }
-    i += two ? 2 : 1;
-    const float held = two ? kQ : kP;
-    ops.push_back(Operation{Operation::kMove, two && !chain ? 0 : 1, 0, 0, -1, i < o.steps ? 1.f / held : 1.f / (held * kX), 0.f, 0.f, i == o.steps});
-  }
-  return ops;
 }
 
 // How a launch's products are computed: in tiles of 128 x bn, of which a cluster of `splits` CTAs has one (1: a CTA at a time).
@@ -1474,7 +1439,7 @@ int launch_product(const std::vector<Kin>& kin, const std::vector<std::pair<size
   return POLAR_B200_OK;
 }
 
-// The products of symmetric matrices between two with X, of all shapes.
+// The products of symmetric matrices between two with X, of all shapes (which are all narrow).
 int launch_chain(const std::vector<Kin>& kin, const Operation& op, const polar_b200_muon_options& o, int* status, cudaStream_t st) {
   static thread_local ChainTable t;
   t.a = o.a, t.b = o.b, t.c = o.c, t.two = op.what == Operation::kChain2;
@@ -1569,25 +1534,16 @@ int run_group(const std::vector<One>& all, size_t from, size_t to, const polar_b
                                    : launch_tables<kManyMatrices>(all, from, to, kin, o, partial, targets, st, begin);
     if (rc) return rc;
   }
-  std::vector<std::vector<Operation>> ops;
   std::vector<int> from_x(kin.size(), 0);
-  size_t most = 0;
-  // (Beside larger matrices the products of narrow ones cost no launch of their own.)
-  bool chain = true;
-  for (const Kin& k : kin) chain = chain && k.side <= 128;
-  for (const Kin& k : kin) {
-    ops.push_back(operations_of(k, o, chain));
-    most = std::max(most, ops.back().size());
-  }
-  for (size_t i = 0; i < most; ++i) {
-    if (ops[0][i].what == Operation::kChain || ops[0][i].what == Operation::kChain2) {   // (and so it is for all shapes: narrow ones go in pairs)
-      rc = launch_chain(kin, ops[0][i], o, status, st);
+  std::vector<Sides> shapes;
+  for (const Kin& k : kin) shapes.push_back(Sides{k.rows, k.cols});
+  for (Launch& next : launches_of(shapes, o.steps, o.a, o.b, o.c)) {
+    if (next.chain) {
+      rc = launch_chain(kin, next.ops[0].second, o, status, st);
       if (rc) return rc;
       continue;
     }
-    std::vector<std::pair<size_t, Operation>> now;
-    for (size_t k = 0; k < kin.size(); ++k)
-      if (i < ops[k].size()) now.emplace_back(k, ops[k][i]);
+    auto& now = next.ops;
     auto sum = [&](const std::pair<size_t, Operation>& a) {
       return a.second.what == Operation::kGram ? std::max(kin[a.first].rows, kin[a.first].cols) : kin[a.first].side;
     };
