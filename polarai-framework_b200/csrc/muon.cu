@@ -57,6 +57,7 @@ struct Table {
   int nesterov;
   double* partial;                                         // of each chunk: the sum of its squares
   Target* targets;
+  int* failed;                                             // not zero: a wait of this step has given up (the last products leave the weights alone then)
   Matrix m[N];
 };
 constexpr int kFewMatrices = 16, kManyMatrices = 400;
@@ -96,6 +97,7 @@ __global__ void __launch_bounds__(kThreads) momentum_kernel(const __grid_constan
   const Matrix& m = t.m[at];
   const uint32_t chunk = blockIdx.x - m.first;
   if (chunk == 0 && threadIdx.x == 0) t.targets[t.matrices_before + at] = Target{m.weights, m.decay, m.scale};
+  if (t.chunks_before == 0 && blockIdx.x == 0 && threadIdx.x == 0) *t.failed = 0;
   const uint64_t from = (uint64_t)chunk * m.chunk, to = min(from + m.chunk, m.count);
   const bool vectors = ((reinterpret_cast<uintptr_t>(m.gradient) | reinterpret_cast<uintptr_t>(m.momentum)) & 15) == 0;
   double sum = 0;
@@ -247,7 +249,7 @@ struct Product {
   float lr;
   const float* schedule;
   const Target* targets;
-  int* status;
+  int *status, *failed;
   unsigned long long wait_ns;
   Shape s[kShapes];
 };
@@ -387,7 +389,7 @@ __device__ __forceinline__ void turn_over(uint32_t from, uint32_t to, int lane) 
 // 32 rows of 32 bytes to an instruction, two matrices each of 301 x 514, 999 x 301 and 1511 x 777 took 393 us for 348.  Weights are turned over there, so that the warp reads and writes 32
 // neighbours.  `stores`: how many have left so far.
 template <int COLS>
-__device__ __forceinline__ void finish(const Shape& q, const Place& at, const Target& target, float lr, uint32_t r0, uint32_t c0, int lane, uint32_t (&v)[COLS], Beside beside,
+__device__ __forceinline__ void finish(const Shape& q, const Place& at, const Target& target, const int* failed, float lr, uint32_t r0, uint32_t c0, int lane, uint32_t (&v)[COLS], Beside beside,
                                        uint8_t* slots, uint32_t& stores) {
   const uint32_t row = r0 + lane;
 #pragma unroll
@@ -403,6 +405,7 @@ __device__ __forceinline__ void finish(const Shape& q, const Place& at, const Ta
       float old[32];
 #pragma unroll
       for (int i = 0; i < 32; ++i) old[i] = w[(uint64_t)min((uint32_t)i, q.m - 1 - r0) * q.n];
+      const bool sound = *failed == 0;
       if (lane == 0) stores_read<0>();
       __syncwarp();
 #pragma unroll
@@ -410,7 +413,7 @@ __device__ __forceinline__ void finish(const Shape& q, const Place& at, const Ta
       __syncwarp();
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        if (live && r0 + i < q.m) w[(uint64_t)i * q.n] = old[i] * keep - rate * __uint_as_float(turn[i * 32 + (lane ^ i)]);
+        if (live && sound && r0 + i < q.m) w[(uint64_t)i * q.n] = old[i] * keep - rate * __uint_as_float(turn[i * 32 + (lane ^ i)]);
       __syncwarp();
       continue;
     }
@@ -451,7 +454,7 @@ __device__ __forceinline__ void finish(const Shape& q, const Place& at, const Ta
   }
 }
 // 16 columns of a row, of which the CTAs of a cluster that shares a tile have few: straight to memory.
-__device__ __forceinline__ void finish16(const Shape& q, const Place& at, const Target& target, float lr, uint32_t r0, uint32_t c0, int lane, uint32_t (&v)[16],
+__device__ __forceinline__ void finish16(const Shape& q, const Place& at, const Target& target, const int* failed, float lr, uint32_t r0, uint32_t c0, int lane, uint32_t (&v)[16],
                                          const Beside& beside) {
   const uint32_t row = r0 + lane, block = c0 & ~31u;
   if (c0 >= q.n || r0 >= q.m) return;
@@ -459,19 +462,20 @@ __device__ __forceinline__ void finish16(const Shape& q, const Place& at, const 
   if (q.kind == kUpdate) {
     const float keep = 1.f - lr * target.decay, rate = q.by * lr * target.scale;
     float* const w = target.weights + (uint64_t)min(row, q.m - 1) * q.n + c0;
+    const bool sound = *failed == 0;
     float x[16];                                           // (all loads before the first store, which might change what they read)
     if ((q.n & 3) == 0 && (reinterpret_cast<uintptr_t>(target.weights) & 15) == 0 && c0 + 16 <= q.n) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(x + 4 * j) = reinterpret_cast<const float4*>(w)[j];
 #pragma unroll
       for (int j = 0; j < 16; ++j) x[j] = x[j] * keep - rate * __uint_as_float(v[j]);
-      if (row >= q.m) return;
+      if (row >= q.m || !sound) return;
 #pragma unroll
       for (int j = 0; j < 4; ++j) reinterpret_cast<float4*>(w)[j] = *reinterpret_cast<const float4*>(x + 4 * j);
     } else {
 #pragma unroll
       for (int j = 0; j < 16; ++j) x[j] = w[min((uint32_t)j, q.n - 1 - c0)];
-      if (row >= q.m) return;
+      if (row >= q.m || !sound) return;
 #pragma unroll
       for (int j = 0; j < 16; ++j)
         if (c0 + j < q.n) w[j] = x[j] * keep - rate * __uint_as_float(v[j]);
@@ -512,7 +516,8 @@ __device__ __forceinline__ void finish16(const Shape& q, const Place& at, const 
 // The tensor core cuts every sum off at fp32's last bit, towards zero: over the 3 k / 16 additions of a long k that makes the sums too small by
 // more than all else does to them (784 x 4096: the update 6.4e-5 from the exact one).  The registers' sums are rounded to nearest, and with runs
 // of 128 k there are 24 additions to a cut sum (784 x 4096: 7.7e-6); reading the accumulators costs the tensor core nothing.
-// Every wait is bounded; when one gives up, all roles leave, and the status word holds its code (7xx).
+// Every wait is bounded; when one gives up, all roles leave, the status word holds its code (7xx), and the step's last products, whose operands
+// then mean nothing, leave the weights alone.
 template <int BN, bool SPLIT>
 __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __grid_constant__ Product p) {
   using C = Cfg<BN, SPLIT>;
@@ -654,10 +659,10 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
           uint32_t bits[16];
 #pragma unroll
           for (int j = 0; j < 16; ++j) bits[j] = __float_as_uint(v[j]);
-          finish16(q, at, target, lr, (uint32_t)at.m0 + rows * 32, (uint32_t)at.n0 + rank * cols + c, lane, bits, now);
+          finish16(q, at, target, p.failed, lr, (uint32_t)at.m0 + rows * 32, (uint32_t)at.n0 + rank * cols + c, lane, bits, now);
         }
       } else {
-        finish<BN / 2>(q, at, target_of(p, q, at), lr, r0, c0, lane, sum, beside, place, stores);
+        finish<BN / 2>(q, at, target_of(p, q, at), p.failed, lr, r0, c0, lane, sum, beside, place, stores);
         __syncwarp();
       }
     }
@@ -737,6 +742,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
   tc_fence_before();
   __syncthreads();
   if (*abort_flag) {
+    if (threadIdx.x == 0) *p.failed = 1;
     // let copies and products in flight finish before the memory that they use goes away
     const long long t0 = clock64();
     while (clock64() - t0 < 2000000ll) { }
@@ -968,8 +974,12 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
           }
         }))
       break;
-    if (!mine) continue;
     const bool last = step + 1 == t.steps;
+    if (last) {                                            // (a wait that has given up shows behind the next barrier)
+      __syncthreads();
+      if (*abort_flag) break;
+    }
+    if (!mine) continue;
     const float lr = t.schedule ? t.schedule[1] : t.lr, kept = 1.f - lr * m.decay, rate = lr * m.scale / (kP * kX);
     for (uint32_t col = group * 16; col < length16; col += 64) {
       uint32_t v[16];
@@ -1035,7 +1045,7 @@ struct ChainTable {
   float a, b, c;
   int two;
   uint32_t shapes;
-  int* status;
+  int *status, *failed;
   unsigned long long wait_ns;
   Chain s[kChains];
 };
@@ -1191,6 +1201,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) chain_kernel(const __grid_co
   tc_fence_before();
   __syncthreads();
   if (*abort_flag) {
+    if (threadIdx.x == 0) *t.failed = 1;
     const long long t0 = clock64();
     while (clock64() - t0 < 2000000ll) { }
     __syncthreads();
@@ -1259,13 +1270,20 @@ uint64_t chunk_of(uint64_t count) {
 }
 uint64_t bytes_of(uint64_t rows, uint64_t cols) {          // of one matrix: X twice and the symmetric ones, two planes each, and what is small, rounded up
   const uint64_t side = std::min(rows, cols);
-  return 2 * 2 * (2 * rows * up64(cols) + (in_pairs(rows, cols) ? 3 : 2) * side * up64(side)) + kMostChunks * sizeof(double) + sizeof(Target) + 7 * 256;
+  return 2 * 2 * (2 * rows * up64(cols) + (in_pairs(rows, cols) ? 3 : 2) * side * up64(side)) + kMostChunks * sizeof(double) + sizeof(Target) + 8 * 256;
 }
 // What one group of matrices may take; a step of more is done in several.
 constexpr uint64_t kGroupBytes = 3ull << 30;
 
 // Lays out a group that is sorted by shape, in what lies behind `base`; its bytes.
-uint64_t lay_out(char* base, const std::vector<One>& all, size_t from, size_t to, std::vector<Kin>* kin, double** partial, Target** targets) {
+struct Group {
+  std::vector<Kin> kin;
+  int* failed;                                             // first of all (tests set it between two launches)
+  double* partial;
+  Target* targets;
+};
+uint64_t lay_out(char* base, const std::vector<One>& all, size_t from, size_t to, Group* group) {
+  std::vector<Kin>* const kin = &group->kin;
   uint64_t at = 0, chunks = 0;
   auto take = [&](uint64_t n) {
     char* p = base + at;
@@ -1281,8 +1299,9 @@ uint64_t lay_out(char* base, const std::vector<One>& all, size_t from, size_t to
     }
     ++kin->back().count;
   }
-  *partial = reinterpret_cast<double*>(take(chunks * sizeof(double)));
-  *targets = reinterpret_cast<Target*>(take((to - from) * sizeof(Target)));
+  group->failed = reinterpret_cast<int*>(take(sizeof(int)));
+  group->partial = reinterpret_cast<double*>(take(chunks * sizeof(double)));
+  group->targets = reinterpret_cast<Target*>(take((to - from) * sizeof(Target)));
   for (Kin& k : *kin) {
     for (int b = 0; b < 2; ++b) k.x[b] = reinterpret_cast<__half*>(take(k.count * 4 * k.rows * k.pitch));
     for (int b = 0; b < (in_pairs(k.rows, k.cols) ? 3 : 2); ++b) k.s[b] = reinterpret_cast<__half*>(take(k.count * 4 * k.side * k.side_pitch));
@@ -1294,25 +1313,23 @@ uint64_t workspace_of(const std::vector<One>& all, const std::vector<size_t>& en
   uint64_t most = 0;
   size_t from = 0;
   for (size_t to : ends) {
-    std::vector<Kin> kin;
-    double* partial;
-    Target* targets;
-    most = std::max(most, lay_out(nullptr, all, from, to, &kin, &partial, &targets));
+    Group group;
+    most = std::max(most, lay_out(nullptr, all, from, to, &group));
     from = to;
   }
   return most;
 }
 
 template <int N>
-int launch_tables(const std::vector<One>& all, size_t from, size_t to, const std::vector<Kin>& kin, const polar_b200_muon_options& o, double* partial,
-                  Target* targets, cudaStream_t st, bool begin) {
+int launch_tables(const std::vector<One>& all, size_t from, size_t to, const Group& group, const polar_b200_muon_options& o, cudaStream_t st, bool begin) {
+  const std::vector<Kin>& kin = group.kin;
   static thread_local Table<N> t;
   size_t k = 0, i = from;
   uint32_t chunks_before = 0;
   while (i < to) {
     t.count = 0;
     t.chunks_before = chunks_before, t.matrices_before = (uint32_t)(i - from);
-    t.momentum = o.momentum, t.nesterov = o.nesterov, t.partial = partial, t.targets = targets;
+    t.momentum = o.momentum, t.nesterov = o.nesterov, t.partial = group.partial, t.targets = group.targets, t.failed = group.failed;
     uint32_t chunks = 0;
     for (; i < to && t.count < N; ++i) {
       while (k + 1 < kin.size() && i - from >= kin[k + 1].first) ++k;
@@ -1367,11 +1384,12 @@ Way way_of(const std::vector<Extent>& e) {
 
 // The next operation of every shape, longest sums first.
 template <int BN, bool SPLIT>
-int launch_product(const std::vector<Kin>& kin, const std::vector<std::pair<size_t, Operation>>& ops, const std::vector<int>& from_x, const polar_b200_muon_options& o,
-                   const Target* targets, int* status, cudaStream_t st, uint32_t splits) {
+int launch_product(const Group& group, const std::vector<std::pair<size_t, Operation>>& ops, const std::vector<int>& from_x, const polar_b200_muon_options& o,
+                   int* status, cudaStream_t st, uint32_t splits) {
+  const std::vector<Kin>& kin = group.kin;
   static thread_local Product p;
   p.splits = splits;
-  p.lr = o.lr, p.schedule = o.schedule, p.targets = targets, p.status = status, p.wait_ns = wait_limit_ns(2000000000ull);
+  p.lr = o.lr, p.schedule = o.schedule, p.targets = group.targets, p.status = status, p.failed = group.failed, p.wait_ns = wait_limit_ns(2000000000ull);
   for (size_t k = 0; k < ops.size();) {
     p.shapes = p.tiles = 0;
     for (; k < ops.size() && p.shapes < kShapes; ++k) {
@@ -1440,10 +1458,11 @@ int launch_product(const std::vector<Kin>& kin, const std::vector<std::pair<size
 }
 
 // The products of symmetric matrices between two with X, of all shapes (which are all narrow).
-int launch_chain(const std::vector<Kin>& kin, const Operation& op, const polar_b200_muon_options& o, int* status, cudaStream_t st) {
+int launch_chain(const Group& group, const Operation& op, const polar_b200_muon_options& o, int* status, cudaStream_t st) {
+  const std::vector<Kin>& kin = group.kin;
   static thread_local ChainTable t;
   t.a = o.a, t.b = o.b, t.c = o.c, t.two = op.what == Operation::kChain2;
-  t.status = status, t.wait_ns = wait_limit_ns(2000000000ull);
+  t.status = status, t.failed = group.failed, t.wait_ns = wait_limit_ns(2000000000ull);
   cudaError_t e = cudaFuncSetAttribute(chain_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kChainBytes);
   if (e != cudaSuccess) return fail(POLAR_B200_ERR_CUDA, "fmuon: narrow matrices", e);
   for (size_t k = 0; k < kin.size();) {
@@ -1522,16 +1541,15 @@ int launch_small(const std::vector<One>& all, size_t from, size_t to, const pola
 }
 
 int run_group(const std::vector<One>& all, size_t from, size_t to, const polar_b200_muon_options& o, char* base, cudaStream_t st) {
-  std::vector<Kin> kin;
-  double* partial;
-  Target* targets;
-  lay_out(base, all, from, to, &kin, &partial, &targets);
+  Group group;
+  lay_out(base, all, from, to, &group);
+  const std::vector<Kin>& kin = group.kin;
   int rc;
   int* status = device_status_word(&rc);
   if (rc) return rc;
   for (int begin = 0; begin < 2; ++begin) {
-    rc = to - from <= kFewMatrices ? launch_tables<kFewMatrices>(all, from, to, kin, o, partial, targets, st, begin)
-                                   : launch_tables<kManyMatrices>(all, from, to, kin, o, partial, targets, st, begin);
+    rc = to - from <= kFewMatrices ? launch_tables<kFewMatrices>(all, from, to, group, o, st, begin)
+                                   : launch_tables<kManyMatrices>(all, from, to, group, o, st, begin);
     if (rc) return rc;
   }
   std::vector<int> from_x(kin.size(), 0);
@@ -1539,7 +1557,7 @@ int run_group(const std::vector<One>& all, size_t from, size_t to, const polar_b
   for (const Kin& k : kin) shapes.push_back(Sides{k.rows, k.cols});
   for (Launch& next : launches_of(shapes, o.steps, o.a, o.b, o.c)) {
     if (next.chain) {
-      rc = launch_chain(kin, next.ops[0].second, o, status, st);
+      rc = launch_chain(group, next.ops[0].second, o, status, st);
       if (rc) return rc;
       continue;
     }
@@ -1555,9 +1573,9 @@ int run_group(const std::vector<One>& all, size_t from, size_t to, const polar_b
       extents.push_back(Extent{square ? q.side : q.rows, square ? q.side : q.cols, sum(a), q.count, square});
     }
     const Way way = way_of(extents);
-    rc = way.splits > 1  ? launch_product<128, true>(kin, now, from_x, o, targets, status, st, way.splits)
-         : way.bn == 128 ? launch_product<128, false>(kin, now, from_x, o, targets, status, st, 1)
-                         : launch_product<256, false>(kin, now, from_x, o, targets, status, st, 1);
+    rc = way.splits > 1  ? launch_product<128, true>(group, now, from_x, o, status, st, way.splits)
+         : way.bn == 128 ? launch_product<128, false>(group, now, from_x, o, status, st, 1)
+                         : launch_product<256, false>(group, now, from_x, o, status, st, 1);
     if (rc) return rc;
     for (const auto& a : now) from_x[a.first] ^= a.second.what == Operation::kMove;
   }
