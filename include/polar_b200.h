@@ -507,6 +507,8 @@ uint64_t polar_b200_fpolicy_loss_workspace_bytes(uint64_t tokens, uint64_t seque
  *   loss[0] = mean((1 - smoothing) * -log(sigmoid(z)) + smoothing * -log(sigmoid(-z))),
  *   loss[1] = the share of pairs with a gap above zero,  loss[2] = mean(gap),  rewards[2 * pairs] (NULL: not wanted),
  *   gLogProb (NULL: not wanted) the derivative of loss[0] at each token.
+ * A side of weight zero (smoothing 0 or 1) is left out, also where a gap is infinite: with smoothing 0 a counted log probability of minus infinity makes
+ * the loss infinite where it is the chosen one's, and its pair's loss 0 where it is the rejected one's.  The gradient is finite either way.
  * Sums over sequences are held in 64 bits.  `count` above zero takes the place of the number of pairs.  What is written may overlap
  * nothing that the call names, but gLogProb may be logProb or refLogProb.
  * As a builtin: T logProb, T refLogProb, T ids, T offsets[2 * pairs + 1], f32 beta, f32 smoothing, f32 margin, f32 count, f32 average (0 or 1),

@@ -175,7 +175,8 @@ def preference_loss64(logprob, reference, ids, offsets, beta, smoothing, margin,
     gap = rewards[0::2] - rewards[1::2]
     z = gap - margin
     units = f(count) if count > 0 else max(len(gap), 1)
-    loss = (1 - e) * np.logaddexp(0, -z) + e * np.logaddexp(0, z)
+    # (a side of weight zero is none, also where z is infinite)
+    loss = sum(by * np.logaddexp(0, side) for by, side in ((1 - e, -z), (e, z)) if by != 0)
     with np.errstate(over="ignore"):
         slope = (e / (1 + np.exp(-z)) - (1 - e) / (1 + np.exp(z))) * beta / units
     g = np.where(counts, (np.stack([slope, -slope], 1).ravel() / per)[of], 0.0)

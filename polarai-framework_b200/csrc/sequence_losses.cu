@@ -746,13 +746,15 @@ struct Pairs {
 };
 
 // A pair's loss by z, its rewards' difference without the margin, and the loss's derivative.  log(1 + e^-|z|) and e^-|z| / (1 + e^-|z|):
-// nothing overflows.
+// nothing overflows.  Each side of the loss is a sum of what is not below zero, and a side of weight zero is none: z may be infinite (a token
+// whose logit was masked), and where smoothing leaves the small side alone nothing cancels.
 __device__ __forceinline__ float pair_loss(float z, float smoothing, float* slope) {
   const float e = expf(-fabsf(z)), more = log1pf(e);
   const float against = e / (1.f + e), with = 1.f / (1.f + e);   // sigmoid(-|z|), sigmoid(|z|)
   *slope = z >= 0.f ? smoothing * with - (1.f - smoothing) * against : smoothing * against - (1.f - smoothing) * with;
-  // smoothing * z is what the wrong side's logarithm has more
-  return more + fmaxf(-z, 0.f) + smoothing * z;
+  const float right = smoothing == 1.f ? 0.f : (1.f - smoothing) * (more + fmaxf(-z, 0.f));
+  const float wrong = smoothing == 0.f ? 0.f : smoothing * (more + fmaxf(z, 0.f));
+  return right + wrong;
 }
 struct Pair2 {
   float loss, right, gap;
