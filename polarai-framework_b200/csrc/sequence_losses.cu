@@ -409,7 +409,7 @@ struct Policy {
 template <int N>
 struct Terms {
   float surrogate[N], kl[N], slope[N];
-  float beyond[N];                                         // above zero: the ratio is past the border that its advantage drives it to
+  bool clipped[N];
 };
 // On which side of the clipping border a token lies is decided by the difference of the logarithms in 64 bits, where it is exact: in fp32 rounding would decide
 // for tokens on the border.  Away from it both agree, and fp32 is asked.
@@ -419,27 +419,28 @@ struct Terms {
 template <int N>
 __device__ __forceinline__ Terms<N> terms(const Policy& o, const float* logprob, const float* old, const float* reference, const float* advantage) {
   Terms<N> t;
-  float d[N], nearest = 1.f;
+  float d[N], beyond[N], nearest = 1.f;                    // beyond: above zero where the ratio is past the border that its advantage drives it to
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     d[k] = logprob[k] - old[k];
-    t.beyond[k] = advantage[k] < 0.f ? o.fp32_low - d[k] : d[k] - o.fp32_high;
-    nearest = fminf(nearest, fabsf(t.beyond[k]));
+    beyond[k] = advantage[k] < 0.f ? o.fp32_low - d[k] : d[k] - o.fp32_high;
+    nearest = fminf(nearest, fabsf(beyond[k]));
   }
   if (nearest <= o.near) {
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const double exact = (double)logprob[k] - (double)old[k];
-      if (d[k] == d[k]) t.beyond[k] = (advantage[k] < 0.f ? exact < o.log_low : exact > o.log_high) ? 1.f : -1.f;
+      if (d[k] == d[k]) beyond[k] = (advantage[k] < 0.f ? exact < o.log_low : exact > o.log_high) ? 1.f : -1.f;
     }
   }
 #pragma unroll
   for (int k = 0; k < N; ++k) {
-    const bool cut = t.beyond[k] > 0.f;
+    const bool cut = beyond[k] > 0.f;
+    t.clipped[k] = cut && fabsf(advantage[k]) > 0.f;       // (of two zeros neither is above the other; nor is a NaN, which then shows in the gradient)
     float ratio;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(ratio) : "f"(d[k] * 1.4426950408889634f));
     t.surrogate[k] = (cut ? (advantage[k] < 0.f ? o.low : o.high) : ratio) * advantage[k];
-    t.slope[k] = cut ? 0.f : -t.surrogate[k];
+    t.slope[k] = t.clipped[k] ? 0.f : -t.surrogate[k];
     t.kl[k] = 0.f;
   }
   if (!o.reference) return t;
@@ -557,8 +558,7 @@ __global__ void __launch_bounds__(kThreads) policy_kernel(Packed<Id> p, Workspac
       const float weight = LOOK && o.by_sequence && counts ? even * w.share[of[k]] : even;
       if (counts) {
         sum[0] += e.surrogate[k] * weight, sum[1] += e.kl[k] * weight, sum[2] += (&ent[h].x)[k] * weight;
-        // (of two zeros neither is above the other)
-        if (e.beyond[k] > 0.f && (&adv[h].x)[k] != 0.f) sum[3] += weight;
+        if (e.clipped[k]) sum[3] += weight;
       }
       (&g.x)[k] = counts ? e.slope[k] * weight : 0.f;
       (&ge.x)[k] = counts ? -o.bonus * weight : 0.f;
@@ -713,7 +713,7 @@ __global__ void __launch_bounds__(kFewThreads) policy_few_kernel(Packed<Id> p, P
       const float a = !o.per_token ? advantage[s] : j ? o.advantage[t] : first_adv;
       const Terms<1> e = terms<1>(o, &lp, &old, &ref, &a);
       sum[0] += e.surrogate[0] * weight, sum[1] += e.kl[0] * weight;
-      if (e.beyond[0] > 0.f && a != 0.f) sum[3] += weight;
+      if (e.clipped[0]) sum[3] += weight;
       if (o.entropy) sum[2] += (j ? o.entropy[t] : first_entropy) * weight;
       g = e.slope[0] * weight;
     }
