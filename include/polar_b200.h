@@ -473,6 +473,7 @@ int polar_b200_fadamw(const polar_b200_adamw_tensor* tensors, uint64_t count, co
  *   loss[0] = sum(w * (-surrogate + kl_weight * kl - entropy_weight * entropy)),
  *   loss[1..4] = sum(w * surrogate), sum(w * kl), sum(w * entropy), sum(w) over the tokens whose ratio is clipped (r * a above the other),
  *   gLogProb = w * (-(r * a where it is not clipped) + kl_weight * (1 - exp(q))),  gEntropy = -entropy_weight * w.
+ * A term of weight zero is left out of loss[0] and the gradients, whatever it comes to (its mean is in loss[2] or loss[3] all the same).
  * The advantage is one for each token or for each sequence.  refLogProb or entropy may be NULL (without that term), gLogProb and
  * gEntropy too (not wanted).  `count` above zero takes the place of the number of tokens (by_sequence: sequences) that count, where the
  * batch is a part of a larger one.  On which side of the border a token lies is decided by d in 64 bits.  Nothing counts: all zeros.

@@ -144,14 +144,16 @@ def policy_loss64(logprob, old, reference, entropy, advantage, ids, offsets, cli
         beta = beta if reference is not None else 0.0
         h = pick(entropy) if entropy is not None else np.zeros(len(lp))
         alpha = alpha if entropy is not None else 0.0
-        g = np.where(counts, (slope - beta * np.expm1(q)) * w, 0.0)
+        # (a term of weight zero is none, whatever its arrays hold)
+        grown = np.expm1(q) if beta != 0 else np.zeros(len(q))
+        g = np.where(counts, (slope - beta * grown) * w, 0.0)
         parts = [np.where(counts, t * w, 0.0) for t in (surrogate, kl, h, cut * 1.0)]
         sums = [t.sum() for t in parts]
         # (an exponential has its argument's rounding times the argument)
         sizes = [np.abs(t * by).sum() for t, by in zip(parts, (1 + np.abs(d) * ~cut, 1 + np.abs(q), 1.0, 1.0))]
-        loss = np.array([beta * sums[1] - sums[0] - alpha * sums[2], *sums])
+        loss = np.array([sum(by * t for by, t in ((-1.0, sums[0]), (beta, sums[1]), (-alpha, sums[2])) if by != 0), *sums])
         size = np.array([beta * sizes[1] + sizes[0] + alpha * sizes[2], *sizes])
-        token = w * (np.abs(slope) * (1 + np.abs(d)) + np.abs(beta * np.expm1(q)) + np.abs(beta * q * np.exp(q)))
+        token = w * (np.abs(slope) * (1 + np.abs(d)) + np.abs(beta * grown) + (np.abs(beta * q * np.exp(q)) if beta != 0 else 0.0))
     spread = lambda v: np.concatenate([np.full(span.start, np.nan), v, np.full(n - span.stop, np.nan)])  # noqa: E731
     return loss, spread(g), spread(-alpha * w), (size, spread(np.where(counts, token, 0.0)))
 

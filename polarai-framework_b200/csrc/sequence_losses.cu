@@ -469,12 +469,16 @@ __device__ __forceinline__ Terms<N> terms(const Policy& o, const float* logprob,
         t.kl[k] = grown[k] - q[k];
       }
   }
+  if (o.kl != 0.f) {                                       // (a term of weight zero is none: exp(q) may have left fp32)
 #pragma unroll
-  for (int k = 0; k < N; ++k) t.slope[k] = fmaf(-o.kl, grown[k], t.slope[k]);
+    for (int k = 0; k < N; ++k) t.slope[k] = fmaf(-o.kl, grown[k], t.slope[k]);
+  }
   return t;
 }
 __device__ __forceinline__ void write_loss(const Policy& o, const double* total) {
-  const double loss = (double)o.kl * total[1] - total[0] - (double)o.bonus * total[2];
+  double loss = -total[0];
+  if (o.kl != 0.f) loss += (double)o.kl * total[1];
+  if (o.bonus != 0.f) loss -= (double)o.bonus * total[2];
   o.loss[0] = (float)loss;
 #pragma unroll
   for (int i = 0; i < 4; ++i) o.loss[i + 1] = (float)total[i];
