@@ -479,8 +479,9 @@ int polar_b200_fadamw(const polar_b200_adamw_tensor* tensors, uint64_t count, co
  * batch is a part of a larger one.  On which side of the border a token lies is decided by d in 64 bits.  Nothing counts: all zeros.
  * A gradient may be one of the arrays of a value per token that are read; else what is written may overlap nothing that the call names.
  * As a builtin: T logProb, T oldLogProb, T refLogProb, T entropy, T advantage[tokens or sequences], T ids, T offsets, f32 clip_low,
- * f32 clip_high, f32 kl_weight, f32 entropy_weight, f32 count, f32 by_sequence (0 or 1), T loss[5], T gLogProb, T gEntropy (three results); ids
- * and offsets in fp32; an advantage of as many values as there are tokens is one for each token.  Scratch as for fmatmul. */
+ * f32 clip_high, f32 kl_weight, f32 entropy_weight, f32 count, f32 by_sequence (0 or 1), [f32 advantage_per_token (0 or 1),] T loss[5], T gLogProb,
+ * T gEntropy (three results); ids and offsets in fp32.  Without advantage_per_token the advantage's size tells whose it is, and a batch of as many
+ * sequences as tokens, where it cannot, is refused.  Scratch as for fmatmul. */
 typedef struct polar_b200_policy_batch {
   const float* logProb;
   const float* oldLogProb;

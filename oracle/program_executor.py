@@ -80,7 +80,7 @@ class OracleExecutor:
                 continue
             if kernel in ("fpolicy_loss", "fpreference_loss"):
                 a = [t[x].ravel() if isinstance(x, str) else x for x in args]
-                r = (rows_oracle.fpolicy_loss(*a[:13], a[14], a[15]) if kernel == "fpolicy_loss" else rows_oracle.fpreference_loss(*a[:9], a[11]))
+                r = (rows_oracle.fpolicy_loss(*a[:13], *a[-2:], per_token=bool(a[13]) if len(a) == 17 else None) if kernel == "fpolicy_loss" else rows_oracle.fpreference_loss(*a[:9], a[11]))
                 for name, value in zip(args[-3:], r):
                     t[name] = np.asarray(value, np.float32).reshape(self.program.tensors[name])
                 continue

@@ -187,11 +187,17 @@ def preference_loss64(logprob, reference, ids, offsets, beta, smoothing, margin,
 
 
 def fpolicy_loss(logprob, old, reference, entropy, advantage, ids, offsets, clip_low, clip_high, kl_weight, entropy_weight, count, by_sequence,
-                 g_logprob, g_entropy):
-    """(loss[5], g_logprob, g_entropy) as the builtin of a program gives them."""
+                 g_logprob, g_entropy, per_token=None):
+    """(loss[5], g_logprob, g_entropy) as the builtin of a program gives them.  per_token: whether the advantage is one for each token; None: its size tells."""
     tokens = len(ids)
+    if per_token is None:
+        if tokens == len(offsets) - 1 and tokens > 1:
+            raise ValueError("fpolicy_loss: as many sequences as tokens: whose are the advantages?")
+        per_token = np.size(advantage) == tokens
+    if np.size(advantage) != (tokens if per_token else len(offsets) - 1):
+        raise ValueError("fpolicy_loss: shapes do not agree")
     loss, g, ge, _ = policy_loss64(logprob, old, reference, entropy, advantage, ids, offsets, clip_low, clip_high, kl_weight, entropy_weight, bool(by_sequence),
-                                   np.size(advantage) == tokens, count)
+                                   per_token, count)
     return _f32(loss), _f32(_over(g_logprob, g)), _f32(_over(g_entropy, ge))
 
 

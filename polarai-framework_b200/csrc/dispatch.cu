@@ -390,7 +390,7 @@ uint64_t polar_b200_launch_workspace_bytes(const char* name, const polar_b200_ar
     rows_of(a[0].tensor, &rows, &cols);
     return polar_b200_flayernorm_grad_workspace_bytes(rows, cols);
   }
-  if (name && a && !std::strcmp(name, "fpolicy_loss") && argc == 16 && a[5].is_tensor && a[6].is_tensor && a[5].tensor.dims == 1 &&
+  if (name && a && !std::strcmp(name, "fpolicy_loss") && (argc == 16 || argc == 17) && a[5].is_tensor && a[6].is_tensor && a[5].tensor.dims == 1 &&
       a[6].tensor.dims == 1 && a[5].tensor.shape && a[6].tensor.shape && a[6].tensor.shape[0])
     return polar_b200_fpolicy_loss_workspace_bytes(a[5].tensor.shape[0], a[6].tensor.shape[0] - 1);
   if (name && a && !std::strcmp(name, "fpreference_loss") && argc == 12 && a[2].is_tensor && a[3].is_tensor && a[2].tensor.dims == 1 &&
@@ -925,18 +925,24 @@ int polar_b200_launch_by_name(const char* name, const polar_b200_arg* a, uint64_
   auto flag = [&](uint64_t i) { return a[i].scalar == 0.f || a[i].scalar == 1.f; };
   if (!std::strcmp(name, "fpolicy_loss")) {
     // (T logProb, T oldLogProb, T refLogProb, T entropy, T advantage, T ids, T offsets, f32 clip_low, f32 clip_high, f32 kl_weight,
-    //  f32 entropy_weight, f32 count, f32 by_sequence, T loss[5], T gLogProb, T gEntropy): three results
-    if (!pattern("TTTTTTTffffffTTT") || a[5].tensor.dims != 1 || a[6].tensor.dims != 1 || a[6].tensor.shape[0] < 1 || !flag(12))
+    //  f32 entropy_weight, f32 count, f32 by_sequence, [f32 advantage_per_token,] T loss[5], T gLogProb, T gEntropy): three results
+    const bool told = pattern("TTTTTTTfffffffTTT");
+    if ((!told && !pattern("TTTTTTTffffffTTT")) || a[5].tensor.dims != 1 || a[6].tensor.dims != 1 || a[6].tensor.shape[0] < 1 || !flag(12) || (told && !flag(13)))
       return fail(bad_args, "fpolicy_loss expects (T logProb, T oldLogProb, T refLogProb, T entropy, T advantage, T ids[tokens], T offsets[sequences + 1], f32 clip_low, "
-                            "f32 clip_high, f32 kl_weight, f32 entropy_weight, f32 count, f32 by_sequence, T loss[5], T gLogProb, T gEntropy)");
+                            "f32 clip_high, f32 kl_weight, f32 entropy_weight, f32 count, f32 by_sequence, [f32 advantage_per_token,] T loss[5], T gLogProb, T gEntropy)");
     const uint64_t tokens = a[5].tensor.shape[0], sequences = a[6].tensor.shape[0] - 1, advantages = numel(a[4].tensor);
-    for (int i : {0, 1, 2, 3, 14, 15})
-      if (numel(a[i].tensor) != tokens) return fail(bad_args, "fpolicy_loss: shapes do not agree");
-    if ((advantages != tokens && advantages != sequences) || numel(a[13].tensor) != 5) return fail(bad_args, "fpolicy_loss: shapes do not agree");
+    const polar_b200_arg* const r = a + argc - 3;
+    for (const polar_b200_arg* x : {a, a + 1, a + 2, a + 3, r + 1, r + 2})
+      if (numel(x->tensor) != tokens) return fail(bad_args, "fpolicy_loss: shapes do not agree");
+    // (one token of one sequence has the same advantage either way)
+    if (!told && tokens == sequences && tokens > 1)
+      return fail(bad_args, "fpolicy_loss: where there are as many sequences as tokens, f32 advantage_per_token behind by_sequence says whose the advantages are");
+    const bool per_token = told ? a[13].scalar != 0.f : advantages == tokens;
+    if (advantages != (per_token ? tokens : sequences) || numel(r[0].tensor) != 5) return fail(bad_args, "fpolicy_loss: shapes do not agree");
     const polar_b200_policy_batch b = {a[0].tensor.data, a[1].tensor.data, a[2].tensor.data, a[3].tensor.data, a[4].tensor.data, a[5].tensor.data,
-                                       a[6].tensor.data, POLAR_B200_IDS_F32, advantages == tokens, tokens, sequences};
+                                       a[6].tensor.data, POLAR_B200_IDS_F32, per_token, tokens, sequences};
     const polar_b200_policy_options o = {a[7].scalar, a[8].scalar, a[9].scalar, a[10].scalar, a[11].scalar, a[12].scalar != 0.f};
-    return polar_b200_fpolicy_loss(&b, &o, a[13].tensor.data, a[14].tensor.data, a[15].tensor.data, workspace, workspace_bytes, stream);
+    return polar_b200_fpolicy_loss(&b, &o, r[0].tensor.data, r[1].tensor.data, r[2].tensor.data, workspace, workspace_bytes, stream);
   }
   if (!std::strcmp(name, "fpreference_loss")) {
     // (T logProb, T refLogProb, T ids, T offsets, f32 beta, f32 smoothing, f32 margin, f32 count, f32 average, T loss[3], T rewards, T gLogProb): three results

@@ -448,7 +448,7 @@ auto B200Device::launch(BackendAllocator& allocator, LaunchCommand& cmd, Event* 
     if (be->getDevice() != this && be->native())
       note("cudaStreamWaitEvent", cudaStreamWaitEvent(s, be->native(), 0));
   }
-  constexpr uint64_t kMaxArgs = 16;
+  constexpr uint64_t kMaxArgs = 17;
   polar_b200_arg args[kMaxArgs];
   const char* name = cmd.nativeKernelName ? cmd.nativeKernelName : "";
   if (cmd.argsCount > kMaxArgs || (cmd.argsCount && !cmd.args)) {

@@ -250,7 +250,7 @@ def norm_policy_program(batch, sequences, n_in=784, n_hidden=4096, n_actions=10,
     # rows outside the sequences have no gradient: the loss leaves what stands there
     p.constants = {"ones_h": 1.0, "g": 0.0, "g_entropy": 0.0}
     p.op("fpolicy_loss", "logp", "old_logp", "ref_logp", "entropy", "advantage", "actions", "offsets", clip_low, clip_high, kl_weight, entropy_weight, count,
-         float(by_sequence), "loss", "g", "g_entropy")
+         float(by_sequence), 0.0, "loss", "g", "g_entropy")
     p.op("flogprob_grad", "Z2", "actions", "lse", "entropy", "g", "g_entropy", "dZ2")
     _norm_network_backward(p)
     p.op("fadd", "schedule", 1.0, "tick", 1.0, "schedule")
