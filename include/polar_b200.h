@@ -538,8 +538,8 @@ uint64_t polar_b200_fpreference_loss_workspace_bytes(uint64_t tokens, uint64_t p
  * (A matrix that one CTA's shared memory holds, 128 x 256 or 64 x 512 at most, needs none.)
  * When a wait on the device gives up (polar_b200_device_status is 7xx then), the weights of the matrices done together with that one stay as they were, but
  * for parts that the very last product may have done without it; their momenta have had their step.
- * As a builtin: T gradient[..., rows, cols], T schedule[2], f32 momentum, f32 nesterov (0 or 1), f32 steps, f32 weight_decay, f32 scale, T weights,
- * T momentum (two results), with the polynomial above.  In a program, fmuon builtins in a row share their launches. */
+ * As a builtin: T gradient[..., rows, cols], T schedule[2], f32 momentum, f32 nesterov (0 or 1), f32 steps, f32 weight_decay, f32 scale, T weights[..., rows, cols],
+ * T momentum[..., rows, cols] (two results), with the polynomial above.  In a program, fmuon builtins in a row share their launches. */
 typedef struct polar_b200_muon_tensor {
   float* weights;
   const float* gradient;

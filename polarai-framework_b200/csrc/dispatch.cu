@@ -961,7 +961,7 @@ int polar_b200_launch_by_name(const char* name, const polar_b200_arg* a, uint64_
     polar_b200_muon_tensor t;
     polar_b200_muon_options o;
     if (!muon_arguments(name, a, argc, &t, &o))
-      return fail(bad_args, "fmuon expects (T gradient, T schedule[2], f32 momentum, f32 nesterov, f32 steps, f32 weight_decay, f32 scale, T weights[..., rows, cols], T momentum)");
+      return fail(bad_args, "fmuon expects (T gradient[..., rows, cols], T schedule[2], f32 momentum, f32 nesterov, f32 steps, f32 weight_decay, f32 scale, T weights[..., rows, cols], T momentum[..., rows, cols])");
     return polar_b200_fmuon(&t, 1, &o, workspace, workspace_bytes, stream);
   }
   if (!std::strcmp(name, "fsum")) {

@@ -1650,6 +1650,10 @@ bool muon_arguments(const char* name, const polar_b200_arg* a, uint64_t argc, po
       !(steps >= 1.f && steps <= 32.f) || steps != (float)(uint32_t)steps)
     return false;
   const uint64_t rows = w.shape[w.dims - 2], cols = w.shape[w.dims - 1];
+  for (int i : {0, 8}) {                                   // (as many elements of another shape would be other matrices)
+    const polar_b200_tensor& x = a[i].tensor;
+    if (x.dims < 2 || x.shape[x.dims - 2] != rows || x.shape[x.dims - 1] != cols) return false;
+  }
   *t = polar_b200_muon_tensor{w.data, a[0].tensor.data, a[8].tensor.data, rows && cols ? n[7] / (rows * cols) : 0, rows, cols, a[5].scalar, a[6].scalar};
   *o = polar_b200_muon_options{0.f, a[2].scalar, a[3].scalar != 0.f, (uint32_t)steps, 3.4445f, -4.7750f, 2.0315f, a[1].tensor.data};
   return true;

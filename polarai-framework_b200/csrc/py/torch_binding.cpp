@@ -392,7 +392,9 @@ BUILTIN(fmuon) {
     polar_b200_muon_tensor& t = tensors[(size_t)i];
     const at::Tensor *wt = c.element(w[i], 4), *gt = c.element(g[i], 4), *mt = c.element(m[i], 4);
     if (!c.ok()) break;
-    c.require(wt->dim() >= 2 && numel(gt) == numel(wt) && numel(mt) == numel(wt));
+    c.require(wt->dim() >= 2);
+    for (const at::Tensor* x : {gt, mt})                   // matrices of the same shape, however many dimensions count them
+      c.require(c.ok() && x->dim() >= 2 && x->size(-1) == wt->size(-1) && x->size(-2) == wt->size(-2) && numel(x) == numel(wt));
     if (!c.ok()) break;
     t.weights = data(wt), t.gradient = data(gt), t.momentum = data(mt);
     t.rows = (uint64_t)wt->size(-2), t.cols = (uint64_t)wt->size(-1);

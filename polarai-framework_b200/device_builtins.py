@@ -341,7 +341,7 @@ class DeviceBuiltins:
     def fmuon(self, weights, gradients, momenta, *, lr=0.0, momentum=0.95, nesterov=True, steps=5, weight_decay=0.0, scale=None,
               coefficients=(3.4445, -4.7750, 2.0315), schedule=None):
         """One step of orthogonalised momentum over lists of matrices - tensors [rows, cols], or [..., rows, cols] of several, each by
-        itself - in place.  weight_decay and scale, by which the update is multiplied: one for all, or a list; no scale: sqrt(rows / cols) where
+        itself - in place; gradients and momenta have their shape.  weight_decay and scale, by which the update is multiplied: one for all, or a list; no scale: sqrt(rows / cols) where
         that is above 1.  lr comes from the call or, for steps that are captured, from `schedule`, fadamw's device tensor of the step's number and lr."""
         if not self._native.fmuon(weights, gradients, momenta, lr, momentum, bool(nesterov), steps, weight_decay, scale, *coefficients, schedule):
             decays = [weight_decay] * len(weights) if isinstance(weight_decay, numbers.Real) else weight_decay
@@ -356,6 +356,8 @@ class DeviceBuiltins:
                 _exactly("fmuon", w.numel(), g, m)
                 if len(w.shape) < 2:
                     raise ValueError("fmuon: weights are matrices (vectors are for fadamw)")
+                if any(tuple(x.shape[-2:]) != tuple(w.shape[-2:]) for x in (g, m)):
+                    raise ValueError("fmuon: a gradient and a momentum have the shape of their weights")
                 t.weights, t.gradient, t.momentum = (x.data_ptr() for x in (w, g, m))
                 t.rows, t.cols = w.shape[-2:]
                 t.matrices = w.numel() // (t.rows * t.cols) if t.rows and t.cols else 0
