@@ -247,8 +247,10 @@ def norm_policy_program(batch, sequences, n_in=784, n_hidden=4096, n_actions=10,
     moments = {w: adamw_moments(p, w) for w in ("gamma", "beta")}
     p.inputs = ["X", "actions", "offsets", "old_logp", "ref_logp", "advantage", "schedule", "tick", *weights, *momenta,
                 *[m for ms in moments.values() for m in ms]]
-    # rows outside the sequences have no gradient: the loss leaves what stands there
-    p.constants = {"ones_h": 1.0, "g": 0.0, "g_entropy": 0.0}
+    p.constants = {"ones_h": 1.0}
+    # rows outside the sequences have no gradient: the loss leaves what stands there, which is the step's before otherwise
+    for g in ("g", "g_entropy"):
+        p.op("ffill", 0.0, g)
     p.op("fpolicy_loss", "logp", "old_logp", "ref_logp", "entropy", "advantage", "actions", "offsets", clip_low, clip_high, kl_weight, entropy_weight, count,
          float(by_sequence), 0.0, "loss", "g", "g_entropy")
     p.op("flogprob_grad", "Z2", "actions", "lse", "entropy", "g", "g_entropy", "dZ2")
