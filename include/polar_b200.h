@@ -536,8 +536,8 @@ uint64_t polar_b200_fpreference_loss_workspace_bytes(uint64_t tokens, uint64_t p
  * used, and lr) lr is read on the device.  The shorter side is at most 32768, the longer one 2^20.
  * Scratch as for fmatmul, 256-byte aligned: 16 bytes per element of a square matrix, down to 8 of a narrow one, for 3 GiB or one matrix at a time.
  * (A matrix that one CTA's shared memory holds, 128 x 256 or 64 x 512 at most, needs none.)
- * When a wait on the device gives up (polar_b200_device_status is 7xx then), the weights of the matrices done together with that one stay as they were, but
- * for parts that the very last product may have done without it; their momenta have had their step.
+ * When a wait on the device gives up (polar_b200_device_status is 7xx then), weights whose last product has not begun by then stay as they were, while
+ * all momenta have had their step; where it gives up in a last product itself, parts of those weights have theirs and parts have not.
  * As a builtin: T gradient[..., rows, cols], T schedule[2], f32 momentum, f32 nesterov (0 or 1), f32 steps, f32 weight_decay, f32 scale, T weights[..., rows, cols],
  * T momentum[..., rows, cols] (two results), with the polynomial above.  In a program, fmuon builtins in a row share their launches. */
 typedef struct polar_b200_muon_tensor {

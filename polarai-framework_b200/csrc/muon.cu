@@ -505,7 +505,7 @@ __device__ __forceinline__ void finish16(const Shape& q, const Place& at, const 
 
 // One CTA per SM walks tiles of 128 x BN; or, SPLIT, where there are too few tiles to go round, a cluster of up to eight CTAs has one, each CTA a share of its
 // slabs, and they send one another their sums, each for a part of the tile (784 x 4096 and 4096 x 10: 590 us without clusters, 266 with sums pulled by loads,
-// 256 with sums sent by bulk copies).  Large products are bound by the power limit: 4096 x 16384, five rounds, 8.7 ms, 1160 TFLOP/s of fp16 products, the tensor
+// 256 with sums sent by bulk copies).  Large products are bound by the power limit: 4096 x 16384, five rounds, 8.7 to 8.9 ms, 1120 to 1150 TFLOP/s of fp16 products, the tensor
 // pipe at 72 to 81 % of its cycles; those of a few hundred columns by what stands around them, 7.5 us of 9.5.  (Pairs of CTAs on tiles of 256 x 256, which fetch a third less, were slower:
 // 4096 x 16384 10.2 ms for 8.5.  A slab of 128 x 256 x 32 takes 0.58 us, which is what the library's largest products of this type take.)
 //   warp 0     TMA: both planes of a slab of 32 k of each operand, one instruction each.  An operand that is contiguous along k is K-major
@@ -1275,13 +1275,13 @@ uint64_t bytes_of(uint64_t rows, uint64_t cols) {          // of one matrix: X t
 // What one group of matrices may take; a step of more is done in several.
 constexpr uint64_t kGroupBytes = 3ull << 30;
 
-// Lays out a group that is sorted by shape, in what lies behind `base`; its bytes.
-struct Group {
+struct Group {                                             // what lies in the workspace
   std::vector<Kin> kin;
-  int* failed;                                             // first of all (tests set it between two launches)
+  int* failed;                                             // whether a wait has given up; it comes first
   double* partial;
   Target* targets;
 };
+// Lays out a group that is sorted by shape, in what lies behind `base`; its bytes.
 uint64_t lay_out(char* base, const std::vector<One>& all, size_t from, size_t to, Group* group) {
   std::vector<Kin>* const kin = &group->kin;
   uint64_t at = 0, chunks = 0;

@@ -6,8 +6,8 @@
 // that the second one reads an eighth of a byte in their place.
 //   few tokens (kFew): everything by one CTA in one launch;
 //   else a pass over the ids (policy) or over all (pairs), one over the sequences, one over the tokens.
-// 600 tokens take 3.0 us (a launch), 131072 of 256 sequences 10.3, 8.4 M with 64-bit ids 52.5 (their 235 MB at a copy's rate 35.7): 12 for the ids, 36 for the
-// tokens at 55 % of the issue slots.  Pairs: 1500 tokens 3.9 us, 400001 10.7, 4.2 M of 128 sequences 21.7 (7.7): 9 to 10 each for sums and gradient.
+// 600 tokens take 3.0 us (a launch), 131072 of 256 sequences 10.7, 8.4 M with 64-bit ids 48.9 (their 235 MB at a copy's rate 35.7): 12 for the ids, 33 for the
+// tokens, with half of the warps that an SM could hold (64 registers, most of them loads on their way) and neither memory nor the issue slots full.  Pairs: 1500 tokens 3.9 us, 400001 10.7, 4.2 M of 128 sequences 21.7 (7.7): 9 to 10 each for sums and gradient.
 // Every sum is taken in a fixed order, over a CTA's tokens in fp32 and beyond that, as of the sums over a sequence, in 64 bits.
 #include <algorithm>
 #include <cmath>
@@ -310,7 +310,9 @@ __device__ __forceinline__ uint64_t counted(const Workspace& w, uint64_t from, u
 
 // What a token's term is multiplied by: the tokens that count altogether by one CTA, or of each sequence by a warp.
 constexpr int kTotalThreads = 1024;
-// (Up to kFewTiles tiles every CTA of the next kernel adds the counts up by itself while its loads are on their way: a launch less.)
+// (Up to kFewTiles tiles every CTA of the next kernel adds the counts up by itself while its loads are on their way: a launch less.  77777 tokens 6.2 us for 8.2 with
+// this kernel, 1 M 10.2 for 11.0, 2 M 14.4 both; beyond, what the CTAs read through L2 costs more than the launch: 4 M 21.3 for 19.6, 8.4 M without a reference and with
+// ids of 32 bits, where the bound is, 40.0 for 36.9.)
 constexpr uint32_t kFewTiles = 4096;
 __global__ void __launch_bounds__(kTotalThreads) total_kernel(Workspace w, uint32_t tiles) {
   __shared__ unsigned long long sums[kTotalThreads / 32];

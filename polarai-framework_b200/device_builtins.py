@@ -379,7 +379,8 @@ class DeviceBuiltins:
         entropy, share of clipped tokens - and its gradients at the log probabilities and the entropies.  Sequence s has the tokens
         [offsets[s], offsets[s + 1]), a token with an id below zero does not count; `reference`: log probabilities for the KL term.
         The mean goes over the tokens or, by_sequence, over the sequences' means; `count` above zero is divided by in place of their number.
-        The advantage is one for each sequence or, advantage_per_token, for each token."""
+        The advantage is one for each sequence or, advantage_per_token, for each token.  Gradients before the first sequence and behind the last one
+        are left as they are."""
         if not self._native.fpolicy_loss(logprob, old_logprob, reference, entropy, advantage, ids, offsets, advantage_per_token, clip_low, clip_high,
                                          kl_weight, entropy_weight, count, by_sequence, loss, g_logprob, g_entropy):
             arrays = _present(logprob, old_logprob, reference, entropy, g_logprob, g_entropy)
@@ -400,7 +401,8 @@ class DeviceBuiltins:
                          average=False, count=0.0):
         """The loss of pairs of packed sequences, 2i the chosen and 2i + 1 the rejected one, into loss[3] - the loss, the share of pairs in the
         right order, their mean difference - with the sequences' rewards, beta times the sum (average: the mean) of logprob - reference over
-        the tokens that count, and the loss's gradient at the log probabilities.  `count` above zero is divided by in place of the pairs' number."""
+        the tokens that count, and the loss's gradient at the log probabilities, which stays as it is before the first sequence and behind the last one.
+        `count` above zero is divided by in place of the pairs' number."""
         if not self._native.fpreference_loss(logprob, reference, ids, offsets, beta, smoothing, margin, count, average, loss, rewards, g_logprob):
             arrays = _present(logprob, reference, g_logprob)
             tokens, sequences, kind = _packed("fpreference_loss", ids, offsets, loss, *_present(rewards), *arrays)
