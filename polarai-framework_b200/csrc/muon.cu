@@ -211,7 +211,8 @@ constexpr int kRun = 4;                                    // slabs that are sum
 constexpr int kEpilogueWarps = 8, kProductThreads = 32 * (4 + kEpilogueWarps);
 // Registers of a thread where tiles are 256 wide: 168 at launch (three warpgroups of 128 threads, 64512 in all), then what the sums need for the epilogue's two and
 // what is left for the other: 2 * 128 * 232 + 128 * 40 = 64512.
-constexpr int kFewRegisters = 40, kManyRegisters = 232;
+constexpr int kFewRegisters = 40, kManyRegisters = 232, kSplitRegisters = 128 * kFewRegisters + 256 * kManyRegisters;
+static_assert(kProductThreads == 384, "one warpgroup with few registers, two with many");
 constexpr uint32_t kSlotBytes = 32 * 32 * 2 * 2;           // a block of 32 x 32 as pairs
 template <int BN, bool SPLIT>
 struct Cfg {
@@ -1387,6 +1388,14 @@ template <int BN, bool SPLIT>
 int launch_product(const Group& group, const std::vector<std::pair<size_t, Operation>>& ops, const std::vector<int>& from_x, const polar_b200_muon_options& o,
                    int* status, cudaStream_t st, uint32_t splits) {
   const std::vector<Kin>& kin = group.kin;
+  if constexpr (BN == 256) {
+    // the split waits for registers that the launch has to hold: built with fewer of them it would wait for good
+    static const bool enough = [] {
+      cudaFuncAttributes a;
+      return cudaFuncGetAttributes(&a, product_kernel<BN, SPLIT>) == cudaSuccess && a.numRegs * kProductThreads >= kSplitRegisters;
+    }();
+    if (!enough) return fail(POLAR_B200_ERR_CUDA, "fmuon: the product kernel was built with too few registers");
+  }
   static thread_local Product p;
   p.splits = splits;
   p.lr = o.lr, p.schedule = o.schedule, p.targets = group.targets, p.status = status, p.failed = group.failed, p.wait_ns = wait_limit_ns(2000000000ull);
