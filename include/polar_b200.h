@@ -480,8 +480,8 @@ int polar_b200_fadamw(const polar_b200_adamw_tensor* tensors, uint64_t count, co
  * A gradient may be one of the arrays of a value per token that are read; else what is written may overlap nothing that the call names.
  * As a builtin: T logProb, T oldLogProb, T refLogProb, T entropy, T advantage[tokens or sequences], T ids, T offsets, f32 clip_low,
  * f32 clip_high, f32 kl_weight, f32 entropy_weight, f32 count, f32 by_sequence (0 or 1), [f32 advantage_per_token (0 or 1),] T loss[5], T gLogProb,
- * T gEntropy (three results); ids and offsets in fp32.  Without advantage_per_token the advantage's size tells whose it is, and a batch of as many
- * sequences as tokens, where it cannot, is refused.  Scratch as for fmatmul. */
+ * T gEntropy (three results); ids and offsets in fp32; without a reference or an entropy: any array, and a weight of zero.  Without advantage_per_token the
+ * advantage's size tells whose it is, and a batch of as many sequences as tokens, where it cannot, is refused.  Scratch as for fmatmul. */
 typedef struct polar_b200_policy_batch {
   const float* logProb;
   const float* oldLogProb;
@@ -514,7 +514,7 @@ uint64_t polar_b200_fpolicy_loss_workspace_bytes(uint64_t tokens, uint64_t seque
  * Sums over sequences are held in 64 bits.  `count` above zero takes the place of the number of pairs.  What is written may overlap
  * nothing that the call names, but gLogProb may be logProb or refLogProb.
  * As a builtin: T logProb, T refLogProb, T ids, T offsets[2 * pairs + 1], f32 beta, f32 smoothing, f32 margin, f32 count, f32 average (0 or 1),
- * T loss[3], T rewards[2 * pairs], T gLogProb (three results); ids and offsets in fp32.  Scratch as for fmatmul. */
+ * T loss[3], T rewards[2 * pairs], T gLogProb (three results); ids and offsets in fp32; without a reference: an array of zeros.  Scratch as for fmatmul. */
 typedef struct polar_b200_preference_options {
   float beta, smoothing, margin, count;
   int average;
